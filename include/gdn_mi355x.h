@@ -26,7 +26,7 @@
 extern "C" {
 #endif
 
-#define GDN_ABI_VERSION 5
+#define GDN_ABI_VERSION 6
 
 #define GDN_OK 0
 #define GDN_ERR_INVALID_ARG (-1) /* shape / stride / pointer rejected */
@@ -37,7 +37,8 @@ extern "C" {
  * (one per GPU, held until the process ends). */
 #define GDN_NOALLOC_SCRATCH_BYTES (128LL << 20)
 
-/* ABI version of the loaded library (GDN_ABI_VERSION; 5 added gdn_decode_step). */
+/* ABI version of the loaded library (GDN_ABI_VERSION; 5 added gdn_decode_step, 6 the
+ * 8-bit projections and the tree verify). */
 int gdn_abi_version(void);
 
 /*
@@ -422,6 +423,104 @@ int gdn_rmsnorm_gated(const uint16_t* x, int64_t sx_tok, const uint16_t* z, int6
 int gdn_rmsnorm_gated_ranges(const uint16_t* x, int64_t sx_tok, const uint16_t* z, int64_t sz_tok,
                              const uint16_t* w, uint16_t* y, int64_t n_tok, const int64_t* ranges, int n_ranges,
                              int64_t n_sel_tok, int H, int D, float eps, void* stream);
+
+/*
+ * Rows or blocks to e4m3 (OCP, 1-4-3 bits, no infinities) with one fp32 scale for
+ * each group: y = e4m3(x * fp32(1 / scale)), to nearest, ties to even, with scale =
+ * max(amax * fp32(1 / 448), 2^-126) over the group.  A NaN does not count in amax and
+ * stays NaN; an infinity makes the scale infinite, itself NaN and the rest of its
+ * group 0 (a product with them is NaN).  No counterpart in the reference, whose
+ * projections are bf16 (nanovllm/layers/linear.py:56-75, :133-158).
+ *   x      [M, K] bf16 or fp32 (x_is_fp32), row stride sx, 16-byte aligned rows; K a
+ *          multiple of 128
+ *   y      [M, K] e4m3 bytes, row stride sy (a multiple of 8)
+ *   rows_per_scale 1: scale of row m, columns 128 g .. at scale[m ss_row + g ss_grp]
+ *          (activations); 128: one scale for each 128 x 128 block (weights), of rows
+ *          128 n .. at scale[n ss_row + g ss_grp], the last block of rows cut off at M
+ */
+int gdn_quantize_fp8(const void* x, int x_is_fp32, int64_t sx, uint8_t* y, int64_t sy, float* scale, int64_t ss_row,
+                     int64_t ss_grp, int64_t M, int K, int rows_per_scale, void* stream);
+
+/*
+ * C = A B^T with 8-bit operands and block scales:
+ *   C[m][n] = bf16(sum over kb of sa[m][kb] sb[n / 128][kb] (sum over k of block kb of A[m][k] B[n][k]))
+ * in fp32.  For the projections of gdn_gemm_bf16_cols at half the weight bytes.
+ *   A  [M, K] e4m3, row stride lda; sa fp32, scale of row m and columns 128 kb .. at
+ *      sa[m sa_row + kb sa_grp] (read fastest with sa_row = 1)
+ *   B  [N, K] e4m3 (the weight), row stride ldb; sb [ceil(N / 128), K / 128] fp32, row
+ *      stride sb_row
+ *   C  bf16, n_parts column parts as gdn_gemm_bf16_cols
+ * K a multiple of 128; lda and ldb multiples of 16, A and B 16-byte aligned.  The order
+ * in which the blocks' sums are added may depend on M, N and K.
+ */
+int gdn_gemm_fp8(const uint8_t* A, int64_t lda, const float* sa, int64_t sa_row, int64_t sa_grp, const uint8_t* B,
+                 int64_t ldb, const float* sb, int64_t sb_row, int M, int N, int K, int n_parts, uint16_t* const* C,
+                 const int64_t* ldc, const int* col_end, void* stream);
+
+/*
+ * The gated RMSNorm of gdn_rmsnorm_gated written in e4m3: per token, groups of 128 of
+ * the H * D columns (H * D a multiple of 128; a head of 128 or two of 64), as
+ * gdn_quantize_fp8 of fp32(x rsqrt(mean(x^2) + eps) w silu(z)), which is not rounded
+ * before.  y [n_tok, H, D] e4m3 contiguous; scale of token t, group g at
+ * scale[t ss_tok + g ss_grp].
+ */
+int gdn_rmsnorm_gated_fp8(const uint16_t* x, int64_t sx_tok, const uint16_t* z, int64_t sz_tok, const uint16_t* w,
+                          uint8_t* y, float* scale, int64_t ss_tok, int64_t ss_grp, int64_t n_tok, int H, int D,
+                          float eps, void* stream);
+
+/*
+ * Speculative verify over a tree of drafted tokens (no counterpart in the reference:
+ * spec decode is disabled for qwen3_5, nanovllm/config.py:84).  Three entry points:
+ * the conv and the gated delta rule of T nodes (1 to 64) per sequence against the
+ * pools, and the accepted paths' way into the pools.
+ *   parents  int32, of sequence b at parents + b p_b (0: one tree for all): the node
+ *            before node t: -1 the sequence's own state (a tree may have several such
+ *            nodes), else a node s < t.  Any other value (-2 for padding) or an unused
+ *            parent makes node t unused: its outputs are 0 and it has no effect.
+ *   ids      int64 [B] slots; a sequence whose slot is outside [0, n_slots) has outputs 0
+ *            and nothing of it is written.  Duplicate ids (the dummy slot) are tolerated.
+ *   accepted int64 [B] or NULL: the node of the step before, last_*, up to which its
+ *            tokens were accepted.  Its path from the root goes into the pool rows first
+ *            (in place), and the new tree starts from there; a value that is no used
+ *            node (-1) leaves the row as it is.  The last_* buffers may not be this
+ *            call's outputs.  commit does the same without a new tree.
+ *
+ * gdn_conv_tree: y[b][t] = silu(w[3] x[t] + w[2] x[p] + w[1] x[pp] + w[0] x[ppp]), p, pp,
+ * ppp the ancestors, past the root the pool's taps from the newest: gdn_conv_decode's
+ * arithmetic along each path.  x [B, T, C] bf16 strides x_b, x_t (multiples of 8), pool as
+ * gdn_conv_decode, w [C, 4], y [B, T, C] contiguous; last_x like x with last_T nodes.
+ */
+int gdn_conv_tree(const uint16_t* x, int64_t x_b, int64_t x_t, uint16_t* pool, int64_t sp_slot, int64_t sp_ch,
+                  int64_t n_slots, const int64_t* ids, const uint16_t* w, const int32_t* parents, int64_t p_b,
+                  const uint16_t* last_x, int64_t lx_b, int64_t lx_t, const int32_t* last_parents, int64_t lp_b,
+                  const int64_t* accepted, int last_T, uint16_t* y, int B, int T, int C, void* stream);
+
+/*
+ * gdn_rule_tree: the update of gdn_recurrent along every path of the tree (q, k
+ * L2-normalised, scale on q).  With W_t the product of e^g over the path to t and
+ * w(t, s) that over its nodes after s:
+ *   u_t = beta_t (v_t - W_t S^T k_t - sum over ancestors s of w(t, s) (k_s . k_t) u_s)
+ *   o_t = scale (W_t S^T q_t + sum over ancestors and t of w(t, s) (k_s . q_t) u_s)
+ * The state after a node is W S + sum of w k u^T over its path; it is formed for the
+ * accepted node only, from k, g and u (which the caller keeps until then).
+ *   q, k [B, T, Hk, D], v [B, T, Hv, D] bf16, strides per sequence and token (multiples of
+ *   8, head stride D); g [B, T, Hv] fp32 and beta [B, T, Hv] bf16 contiguous; s_pool, s_slot
+ *   as gdn_recurrent; o [B, T, Hv, D] bf16 and u [B, T, Hv, D] fp32 contiguous; last_k,
+ *   last_g, last_u: k, g and u of the step before (last_T nodes).  D 64 or 128.
+ */
+int gdn_rule_tree(const uint16_t* q, int64_t q_b, int64_t q_t, const uint16_t* k, int64_t k_b, int64_t k_t,
+                  const uint16_t* v, int64_t v_b, int64_t v_t, const float* g, const uint16_t* beta, float* s_pool,
+                  int64_t s_slot, int64_t n_slots, const int64_t* ids, const int32_t* parents, int64_t p_b,
+                  const uint16_t* last_k, int64_t lk_b, int64_t lk_t, const float* last_g, const float* last_u,
+                  const int32_t* last_parents, int64_t lp_b, const int64_t* accepted, int last_T, uint16_t* o,
+                  float* u, int B, int T, int Hk, int Hv, int D, float scale, void* stream);
+
+/* gdn_commit_tree: the accepted paths into the state and conv pools (x, k, g, u and
+ * parents of the verified step). */
+int gdn_commit_tree(float* s_pool, int64_t s_slot, uint16_t* conv_pool, int64_t sp_slot, int64_t sp_ch,
+                    int64_t n_slots, const int64_t* ids, const int32_t* parents, int64_t p_b, const int64_t* accepted,
+                    const uint16_t* x, int64_t x_b, int64_t x_t, const uint16_t* k, int64_t k_b, int64_t k_t,
+                    const float* g, const float* u, int B, int T, int Hk, int Hv, int D, int C, void* stream);
 
 #ifdef __cplusplus
 }

@@ -18,13 +18,20 @@ from .ops import (  # noqa: F401
     chunk_gated_delta_rule,
     chunk_gated_delta_rule_varlen,
     commit_states,
+    commit_tree,
     conv_decode_step,
+    conv_tree_step,
     fused_g_beta,
     linear,
+    linear_fp8,
+    quantize_fp8,
+    quantize_weight_fp8,
     recurrent_gated_delta_rule,
     recurrent_gdn_inplace,
     recurrent_gdn_multitoken,
+    recurrent_gdn_tree,
     rms_norm_gated,
+    rms_norm_gated_fp8,
 )
-from .gdn_layer import GatedDeltaNetCore, GatedDeltaNetLayer, Switches  # noqa: F401
+from .gdn_layer import GatedDeltaNetCore, GatedDeltaNetLayer, Switches, TreeStep  # noqa: F401
 from .state_pool import LinearStatePool, allocate_state_pools, reset_linear_states, varlen_meta  # noqa: F401

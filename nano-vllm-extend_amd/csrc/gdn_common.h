@@ -128,23 +128,43 @@ __device__ __forceinline__ f32x4_t mfma16x16x4f32(float a, float b, const f32x4_
   return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0);
 }
 
-// One element of the gated RMSNorm after the row's r = rsqrt(mean(x^2) + eps)
-// (nanovllm/models/qwen3_5.py:121-131, eager rounding order):
-//   n = bf16(x r), wn = bf16(w n), y = wn * silu(z)   (the caller rounds y)
 // silu(z) = z / (1 + e^-z): e^-z within a few ulp (exp_acc) and the divide as
 // a hardware reciprocal refined by one Newton step (within an ulp of the
 // divide); the exponent is capped at 88 so the step never sees an infinite
-// operand.  Every gated-norm output goes through this function, so the
-// standalone and the fused norms agree bit for bit.
-__device__ __forceinline__ float norm_gate(float x, float r, float w, float z) {
-  const float n = bf2f(f2bf(x * r));
-  const float wn = bf2f(f2bf(w * n));
+// operand.
+__device__ __forceinline__ float silu_ulp(float z) {
   // (0 - z rather than -z: a subtraction's result needs no canonicalising
   // before the min; exp of +0 and -0 are the same)
   const float d = 1.0f + exp_acc(fminf(0.0f - z, 88.0f));
   float rc = __builtin_amdgcn_rcpf(d);
   rc = fmaf(rc, fmaf(-d, rc, 1.0f), rc);
-  return wn * (z * rc);
+  return z * rc;
+}
+
+// One element of the gated RMSNorm after the row's r = rsqrt(mean(x^2) + eps)
+// (nanovllm/models/qwen3_5.py:121-131, eager rounding order):
+//   n = bf16(x r), wn = bf16(w n), y = wn * silu(z)   (the caller rounds y)
+// Every gated-norm output in bf16 goes through this function, so the
+// standalone and the fused norms agree bit for bit.
+__device__ __forceinline__ float norm_gate(float x, float r, float w, float z) {
+  const float n = bf2f(f2bf(x * r));
+  const float wn = bf2f(f2bf(w * n));
+  return wn * silu_ulp(z);
+}
+
+// ---- e4m3 values with one fp32 scale for each group of 128 ----
+// scale = amax * fp32(1 / 448), at least 2^-126 so that its reciprocal is finite
+// (a group of zeros; magnitudes below 2^-117 go to zero); a value is
+// e4m3(x * fp32(1 / scale)), to nearest, ties to even.  The product is at most 448
+// times 1 + 2^-22, which rounds to 448, the largest e4m3 value.  A NaN does not
+// count in amax and stays NaN; an infinity makes the scale infinite, itself NaN
+// and the rest of its group 0.
+constexpr float kFp8Max = 448.0f;
+constexpr int kFp8Group = 128;
+__device__ __forceinline__ float fp8_scale(float amax) { return fmaxf(amax * (1.0f / kFp8Max), 0x1p-126f); }
+__device__ __forceinline__ uint32_t f2fp8x4(float a, float b, float c, float d) {
+  const int lo = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
+  return static_cast<uint32_t>(__builtin_amdgcn_cvt_pk_fp8_f32(c, d, lo, true));
 }
 
 // ---- wave-level reductions (wave64) ----

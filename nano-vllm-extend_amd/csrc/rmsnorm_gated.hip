@@ -84,6 +84,59 @@ __global__ __launch_bounds__(256) void rmsnorm_gated_kernel(const uint16_t* __re
   if (active) *reinterpret_cast<uint4*>(y + row * D + lane * 8) = out;  // y rows [tok, h] dense
 }
 
+// The same norm written in e4m3 with one fp32 scale for each 128 columns of a token
+// (a head of 128, or two of 64): what the 8-bit out projection reads.  y = x r w
+// silu(z) in fp32, rounded once, to e4m3 (the bf16 output's three roundings are the
+// reference's; no reference has this output).  16 lanes per 128 columns.
+template <int D>
+__global__ __launch_bounds__(256) void rmsnorm_gated_fp8_kernel(const uint16_t* __restrict__ x, int64_t sx_tok,
+                                                                const uint16_t* __restrict__ z, int64_t sz_tok,
+                                                                const uint16_t* __restrict__ w,
+                                                                uint8_t* __restrict__ y, float* __restrict__ scale,
+                                                                int64_t ss_tok, int64_t ss_grp, int64_t n_tok, int G,
+                                                                float eps) {
+  constexpr int kLanes = D / 8;  // lanes per head
+  const int lane = threadIdx.x % 16;
+  const uint32_t b = blockIdx.x;
+  const int g = static_cast<int>(b % static_cast<uint32_t>(G));
+  const int64_t tok = static_cast<int64_t>(b / static_cast<uint32_t>(G)) * 16 + threadIdx.x / 16;
+  const bool active = tok < n_tok;
+  const int64_t col = static_cast<int64_t>(g) * gdn::kFp8Group + lane * 8;
+  uint4 xv = make_uint4(0, 0, 0, 0), zv = make_uint4(0, 0, 0, 0);
+  if (active) {
+    xv = *reinterpret_cast<const uint4*>(x + tok * sx_tok + col);
+    zv = *reinterpret_cast<const uint4*>(z + tok * sz_tok + col);
+  }
+  const uint4 wv = *reinterpret_cast<const uint4*>(w + lane % kLanes * 8);
+  const uint16_t* xs = reinterpret_cast<const uint16_t*>(&xv);
+  const uint16_t* zs = reinterpret_cast<const uint16_t*>(&zv);
+  const uint16_t* ws = reinterpret_cast<const uint16_t*>(&wv);
+  float v[8], ss = 0.0f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    v[i] = gdn::bf2f(xs[i]);
+    ss += v[i] * v[i];
+  }
+#pragma unroll
+  for (int m = kLanes / 2; m >= 1; m >>= 1) ss += __shfl_xor(ss, m, 64);
+  const float r = rsqrtf(ss / static_cast<float>(D) + eps);
+  float top = 0.0f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    v[i] = v[i] * r * gdn::bf2f(ws[i]) * gdn::silu_ulp(gdn::bf2f(zs[i]));
+    top = fmaxf(top, fabsf(v[i]));
+  }
+#pragma unroll
+  for (int m = 8; m >= 1; m >>= 1) top = fmaxf(top, __shfl_xor(top, m, 64));
+  const float s = gdn::fp8_scale(top);
+  const float inv = 1.0f / s;
+  if (!active) return;
+  *reinterpret_cast<uint2*>(y + tok * G * gdn::kFp8Group + col) =
+      make_uint2(gdn::f2fp8x4(v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv),
+                 gdn::f2fp8x4(v[4] * inv, v[5] * inv, v[6] * inv, v[7] * inv));
+  if (lane == 0) scale[tok * ss_tok + g * ss_grp] = s;
+}
+
 }  // namespace
 
 extern "C" int gdn_rmsnorm_gated(const uint16_t* x, int64_t sx_tok, const uint16_t* z,
@@ -134,5 +187,31 @@ extern "C" int gdn_rmsnorm_gated_ranges(const uint16_t* x, int64_t sx_tok, const
     rmsnorm_gated_kernel<64><<<dim3(static_cast<unsigned>(nb * H)), dim3(256), 0, s>>>(
         x, sx_tok, z, sz_tok, w, y, n_sel_tok, H, eps, ranges, n_ranges, n_tok);
   }
+  return gdn_launch_status();
+}
+
+extern "C" int gdn_rmsnorm_gated_fp8(const uint16_t* x, int64_t sx_tok, const uint16_t* z, int64_t sz_tok,
+                                     const uint16_t* w, uint8_t* y, float* scale, int64_t ss_tok, int64_t ss_grp,
+                                     int64_t n_tok, int H, int D, float eps, void* stream) {
+  if (n_tok < 0 || H <= 0) return GDN_ERR_INVALID_ARG;
+  if (D != 64 && D != 128) return GDN_ERR_UNSUPPORTED;
+  if (H * D % gdn::kFp8Group) return GDN_ERR_INVALID_ARG;  // whole groups
+  if (n_tok == 0) return GDN_OK;
+  if (!x || !z || !w || !y || !scale) return GDN_ERR_INVALID_ARG;
+  if ((sx_tok % 8) || (sz_tok % 8) || (reinterpret_cast<uintptr_t>(x) % 16) ||
+      (reinterpret_cast<uintptr_t>(z) % 16) || (reinterpret_cast<uintptr_t>(w) % 16) ||
+      (reinterpret_cast<uintptr_t>(y) % 16) || (reinterpret_cast<uintptr_t>(scale) % 4))
+    return GDN_ERR_INVALID_ARG;
+  const int G = H * D / gdn::kFp8Group;
+  const int64_t nb = (n_tok + 15) / 16 * G;
+  if (nb >= (1LL << 31)) return GDN_ERR_UNSUPPORTED;
+  const dim3 grid(static_cast<unsigned>(nb)), block(256);
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  if (D == 128)
+    rmsnorm_gated_fp8_kernel<128><<<grid, block, 0, s>>>(x, sx_tok, z, sz_tok, w, y, scale, ss_tok, ss_grp, n_tok, G,
+                                                         eps);
+  else
+    rmsnorm_gated_fp8_kernel<64><<<grid, block, 0, s>>>(x, sx_tok, z, sz_tok, w, y, scale, ss_tok, ss_grp, n_tok, G,
+                                                        eps);
   return gdn_launch_status();
 }

@@ -125,6 +125,30 @@ def late_split(lens_q: list[int], Hv: int):
 _NOT_TIMED = contextlib.nullcontext()
 
 
+@dataclass
+class TreeStep:
+    """What a verify step over trees of drafted tokens leaves for the commit of its
+    accepted paths: the raw rows, the keys after the conv, the gates, the
+    corrections and the trees (GatedDeltaNetCore.verify_tree).  accept() names the
+    last accepted node of each sequence; the step is then the next verify's
+    `pending`, or goes to commit_tree."""
+    x: torch.Tensor          # [B, T, C]
+    k: torch.Tensor          # [B, T, Hk, D]
+    g: torch.Tensor          # [B, T, Hv]
+    u: torch.Tensor          # [B, T, Hv, D]
+    parents: torch.Tensor    # [B, T] or [T]
+    accepted: torch.Tensor | None = None
+
+    def accept(self, accepted: torch.Tensor) -> "TreeStep":
+        """accepted [B] int64 on the device: a node of each tree, whose path from
+        the root is kept, or -1 where nothing is."""
+        if accepted.shape != (self.x.shape[0],) or accepted.device != self.x.device:
+            raise ValueError(f"accepted must be [{self.x.shape[0]}] on {self.x.device}, got {list(accepted.shape)} "
+                             f"on {accepted.device}")
+        self.accepted = accepted
+        return self
+
+
 @contextlib.contextmanager
 def _timing(timer, name: str):
     timer.start(name)
@@ -195,6 +219,10 @@ class GatedDeltaNetCore:
         with self._timed("rmsnorm_gated"):
             return ops.rms_norm_gated(core, z, self.norm_w, self.eps, out)
 
+    def _norm_fp8(self, core, z):
+        with self._timed("rmsnorm_gated"):
+            return ops.rms_norm_gated_fp8(core, z, self.norm_w, self.eps)
+
     # --------------------------------------------------------------- decode --
     def decode(self, mixed, z, b, a, ids, conv_cache, s_cache, gb=None, out=None):
         """One token per row (the T == 1 branch of _gdn_padded, qwen3_5.py:1008-1030).
@@ -242,14 +270,59 @@ class GatedDeltaNetCore:
             s_cache[ids] = new_s
         return self._norm(core.view(B, Hv, D), z.view(B, Hv, D), out).view(B, Hv, D)
 
+    # -------------------------------------------------- verify over trees --
+    def verify_tree(self, mixed, z, b, a, ids, conv_cache, s_cache, parents, pending: TreeStep | None = None,
+                    fp8: bool = False):
+        """One verify step over a tree of T drafted tokens for each sequence (not in
+        the reference, which has no spec decode for this model,
+        nanovllm/config.py:84): conv, gates, delta rule and gated norm of every
+        node after its ancestors.  mixed [B, T, C], z [B, T, Hv*D], b/a [B, T, Hv];
+        parents [B, T] or [T] (ops.conv_tree_step); the pools' rows ids [B] are
+        read, and stay, except that pending (the step before, with its accepted
+        nodes) goes into them first.  Returns (core [B, T, Hv, D] bf16, or with fp8
+        its (e4m3, scales) as the 8-bit out projection reads it; TreeStep)."""
+        self._to(mixed.device)
+        if not self.sw.gbeta or not self.sw.conv_kernel or self.K != 4:
+            raise NotImplementedError("verify_tree runs the gate and conv kernels (conv width 4) only")
+        if pending is not None and pending.accepted is None:
+            raise ValueError("pending has no accepted nodes: accept() follows each verify")
+        B, T, _ = mixed.shape
+        Hk, Hv, D, kd = self.Hk, self.Hv, self.D, self.key_dim
+        last_conv = last_rule = None
+        if pending is not None:
+            last_conv = (pending.x, pending.parents, pending.accepted)
+            last_rule = (pending.k, pending.g, pending.u, pending.parents, pending.accepted)
+        with self._timed("conv_tree"):
+            y = ops.conv_tree_step(mixed, conv_cache, ids, self.conv_w, parents, pending=last_conv)
+        g, beta = self._g_beta(b.contiguous(), a.contiguous(), None)
+        k = y[..., kd:2 * kd].unflatten(-1, (Hk, D))
+        with self._timed("recurrent_tree"):
+            o, u = ops.recurrent_gdn_tree(y[..., :kd].unflatten(-1, (Hk, D)), k, y[..., 2 * kd:].unflatten(-1, (Hv, D)),
+                                          g, beta, s_cache, ids, parents, pending=last_rule)
+        step = TreeStep(mixed, k, g, u, parents)
+        if z.stride(0) % 8 or z.stride(1) % 8 or z.data_ptr() % 16:
+            z = z.contiguous()      # (the norm reads 16-byte pieces)
+        z = z.reshape(B, T, Hv, D)
+        return (self._norm_fp8(o, z) if fp8 else self._norm(o, z)), step
+
+    def commit_tree(self, step: TreeStep, ids, conv_cache, s_cache) -> None:
+        """The accepted paths of a verify step into both pools, for another user of
+        the slots than the next verify."""
+        if step.accepted is None:
+            raise ValueError("the step has no accepted nodes: accept() first")
+        with self._timed("commit_tree"):
+            ops.commit_tree(s_cache, conv_cache, ids, step.parents, step.accepted, step.x, step.k, step.g, step.u)
+
     # ------------------------------------------------------- varlen prefill --
-    def prefill_varlen(self, mixed, z, b, a, lens_q, ids, conv_cache, s_cache, fresh=None, gb=None, out=None):
+    def prefill_varlen(self, mixed, z, b, a, lens_q, ids, conv_cache, s_cache, fresh=None, gb=None, out=None,
+                       fp8=False):
         """Varlen prefill group (_gdn_prefill_varlen, qwen3_5.py:922-965) with the
         conv and recurrent states read / written in the pools at `ids`.
         mixed [N, C], z [N, Hv*D], b/a [N, Hv].  fresh: optional bool [n],
         sequences that start from zero states (their slots need no zeroing
         beforehand, model_runner.py:305-322).  Returns core [N, Hv, D] bf16 (in
-        `out` where given, except with the split state pass)."""
+        `out` where given, except with the split state pass); with fp8 (and no
+        `out`) its (e4m3, scales), except with the split state pass."""
         self._to(mixed.device)
         N = mixed.shape[0]
         Hk, Hv, D = self.Hk, self.Hv, self.D
@@ -265,6 +338,8 @@ class GatedDeltaNetCore:
                 o = ops.conv_chunk_prefill_varlen(mixed, conv_cache, self.conv_w, b, a, self.A_log, self.dt_bias,
                                                   cu64_gpu, s_cache, ids, Hk, Hv, D, fresh=fresh,
                                                   cu_seqlens_cpu=cu64_cpu)
+            if fp8 and out is None:
+                return self._norm_fp8(o, z.view(N, Hv, D))
             return self._norm(o, z.view(N, Hv, D), out).view(N, Hv, D)
         if fresh is not None:
             zero = ids[fresh.to(device=ids.device, dtype=torch.bool)]
@@ -282,6 +357,8 @@ class GatedDeltaNetCore:
             o, _ = ops.chunk_gated_delta_rule_varlen(q.view(N, Hk, D), k.view(N, Hk, D), v.view(N, Hv, D),
                                                      g, beta, cu64_gpu, s_cache, state_ids=ids,
                                                      final_state=s_cache, cu_seqlens_cpu=cu64_cpu)
+        if fp8 and out is None:
+            return self._norm_fp8(o, z.view(N, Hv, D))
         return self._norm(o, z.view(N, Hv, D), out).view(N, Hv, D)
 
     def _prefill_split(self, mixed, z, b, a, lens_q, ids, conv_cache, s_cache, fresh, cu64_cpu, cu64_gpu, split):
@@ -387,13 +464,15 @@ class GatedDeltaNetCore:
 
     # ------------------------------------------------------------- dispatch --
     def forward(self, mixed, z, b, a, cu_seqlens_q, max_seqlen_q, ids, conv_cache, s_cache,
-                lens_q: list[int] | None = None, gb=None):
+                lens_q: list[int] | None = None, gb=None, fp8: bool = False):
         """Dispatch of Qwen3_5GatedDeltaNet.forward (qwen3_5.py:864-920) over a
         varlen step: all-decode -> decode; a contiguous decode prefix goes to
         the decode path and the rest to the varlen (or padded) prefill.
         mixed [N, C], z [N, Hv*D], b/a [N, Hv]; gb: optional (g [N, Hv] fp32,
         beta [N, Hv] bf16) already computed from b, a (used by the paths that
-        would run the gate kernel).  Returns [N, Hv*D] bf16."""
+        would run the gate kernel).  Returns [N, Hv*D] bf16; with fp8, a step of
+        prompts alone returns (e4m3 [N, Hv, D], scales) instead where its norm is a
+        launch of its own (ops.rms_norm_gated_fp8)."""
         rows = (lambda i, j: None) if gb is None else (lambda i, j: (gb[0][i:j], gb[1][i:j]))
         N = mixed.shape[0]
         T = int(max_seqlen_q)
@@ -420,7 +499,10 @@ class GatedDeltaNetCore:
             rest = None if out is None else out[off:]
             if self.sw.varlen:
                 core = self.prefill_varlen(mixed[off:], z[off:], b[off:], a[off:], lens_q[off:], ids[off:],
-                                           conv_cache, s_cache, gb=rows(off, N), out=rest).view(-1, self.value_dim)
+                                           conv_cache, s_cache, gb=rows(off, N), out=rest, fp8=fp8)
+                if isinstance(core, tuple):
+                    return core
+                core = core.view(-1, self.value_dim)
             else:
                 lens_p = lens_dev()[off:]
                 Tp = T if off == 0 else max(lens_q[off:])
@@ -468,24 +550,70 @@ class GatedDeltaNetLayer:
     path would run the gate kernel instead, the GEMM's epilogue computes g and
     beta from the b and a columns and that path uses them).
     out_proj [hidden, Hv*D] (:838-839) runs on the gated norm's output.  Both
-    GEMMs are ops.linear (bf16 matrix cores, fp32 accumulation)."""
+    GEMMs are ops.linear (bf16 matrix cores, fp32 accumulation).
+
+    weights="fp8" holds in_proj_qkv, in_proj_z and out_proj in e4m3 with one fp32
+    scale for each 128 x 128 block (half the weight bytes) and multiplies with
+    ops.linear_fp8, whose activations are brought to e4m3 per row and 128 columns;
+    hidden and Hv*D are then multiples of 128.  Those three come in bf16 (they are
+    converted here, once) or as a checkpoint's (e4m3, scales) pairs.  in_proj_b and
+    in_proj_a, the gates' inputs, stay bf16: they are 2 Hv rows, and an error in
+    them is an error in every decay."""
 
     def __init__(self, w_qkv, w_z, w_b, w_a, w_out, num_k_heads: int, num_v_heads: int, head_dim: int,
-                 conv_weight, A_log, dt_bias, norm_weight, eps: float = 1e-6, switches: Switches | None = None):
+                 conv_weight, A_log, dt_bias, norm_weight, eps: float = 1e-6, switches: Switches | None = None,
+                 weights: str = "bf16"):
         self.core = GatedDeltaNetCore(num_k_heads, num_v_heads, head_dim, conv_weight, A_log, dt_bias, norm_weight,
                                       eps=eps, switches=switches)
         c = self.core
+        if weights not in ("bf16", "fp8"):
+            raise ValueError(f"weights must be 'bf16' or 'fp8', got {weights!r}")
+        self.fp8 = weights == "fp8"
+        self.timer = None
+        if self.fp8:
+            self._take_fp8(w_qkv, w_z, w_b, w_a, w_out)
+            return
         assert w_qkv.shape[0] == c.conv_dim and w_z.shape[0] == c.value_dim
         assert w_b.shape[0] == num_v_heads and w_a.shape[0] == num_v_heads
         self.hidden = w_qkv.shape[1]
         self.w_in = torch.cat([w_qkv, w_z, w_b, w_a], dim=0).contiguous()
         self.w_out = w_out.contiguous()
         assert self.w_out.shape == (self.hidden, c.value_dim)
-        self.timer = None
+
+    def _take_fp8(self, w_qkv, w_z, w_b, w_a, w_out):
+        c = self.core
+
+        def pair(w, rows, name):
+            w8, scale = w if isinstance(w, (tuple, list)) else ops.quantize_weight_fp8(w)
+            if w8.dtype != ops.FP8 or w8.shape[0] != rows or w8.shape[1] % ops.FP8_GROUP:
+                raise ValueError(f"{name} must be e4m3 [{rows}, K] with K a multiple of {ops.FP8_GROUP}, got "
+                                 f"{w8.dtype} {list(w8.shape)}")
+            want = (-(-rows // ops.FP8_GROUP), w8.shape[1] // ops.FP8_GROUP)
+            if scale.dtype != torch.float32 or tuple(scale.shape) != want:
+                raise ValueError(f"{name}'s scales must be float32 {list(want)}, got {scale.dtype} {list(scale.shape)}")
+            return w8, scale
+
+        if isinstance(w_qkv, (tuple, list)) != isinstance(w_z, (tuple, list)):
+            raise ValueError("w_qkv and w_z come both in bf16 or both as (e4m3, scales)")
+        if isinstance(w_qkv, (tuple, list)) and c.conv_dim % ops.FP8_GROUP == 0:
+            parts = pair(w_qkv, c.conv_dim, "w_qkv"), pair(w_z, c.value_dim, "w_z")
+            self.w_in, self.w_in_scale = (torch.cat(t, 0).contiguous() for t in zip(*parts))
+        elif isinstance(w_qkv, (tuple, list)):
+            raise ValueError(f"the {c.conv_dim} rows of w_qkv end inside of a block of {ops.FP8_GROUP}: its blocks "
+                             "and w_z's cannot share one product")
+        else:
+            if w_qkv.shape[0] != c.conv_dim or w_z.shape[0] != c.value_dim:
+                raise ValueError(f"w_qkv and w_z must have {c.conv_dim} and {c.value_dim} rows")
+            self.w_in, self.w_in_scale = ops.quantize_weight_fp8(torch.cat([w_qkv, w_z], 0))
+        self.hidden = self.w_in.shape[1]
+        self.w_out, self.w_out_scale = pair(w_out, self.hidden, "w_out")
+        if self.w_out.shape[1] != c.value_dim or w_b.shape != (c.Hv, self.hidden) or w_a.shape != w_b.shape:
+            raise ValueError(f"w_out must be [{self.hidden}, {c.value_dim}], w_b and w_a [{c.Hv}, {self.hidden}]")
+        self.w_ba = torch.cat([w_b, w_a], 0).contiguous()
 
     @property
     def n_in(self) -> int:
-        return self.w_in.shape[0]
+        return self.w_in.shape[0] + (self.w_ba.shape[0] if self.fp8 else 0)
 
     def _timed(self, name):
         return _NOT_TIMED if self.timer is None else _timing(self.timer, name)
@@ -509,6 +637,17 @@ class GatedDeltaNetLayer:
         c = self.core
         C, V, Hv = c.conv_dim, c.value_dim, c.Hv
         widths = [C, V, Hv, Hv]
+        if self.fp8:
+            with self._timed("in_proj"):
+                mixed, z = ops.linear_fp8_cols(hidden, self.w_in, self.w_in_scale, [C, V])
+                how = {"gate_col": 0, "A_log": c.A_log, "dt_bias": c.dt_bias} if gates else None
+                if Hv % 16 == 0:
+                    y = ops.linear_cols(hidden, self.w_ba, [Hv, Hv], gates=how)
+                    (b, a), gb = (y[0], y[1:]) if gates else (y, None)
+                    return mixed, z, b, a, gb
+                y = ops.linear(hidden, self.w_ba, gates=how)
+                y, gb = (y[0], y[1:]) if gates else (y, None)
+                return mixed, z, y[..., :Hv], y[..., Hv:], gb
         with self._timed("in_proj"):
             if all(w % 16 == 0 for w in widths[:-1]):
                 if gates:
@@ -533,6 +672,31 @@ class GatedDeltaNetLayer:
         mixed, z, b, a, gb = self.project_in(hidden, gates=self.gates_in_gemm())
         self.core.timer = self.timer
         core = self.core.forward(mixed, z, b.contiguous(), a.contiguous(), cu_seqlens_q, max_seqlen_q, ids,
-                                 conv_cache, s_cache, lens_q=lens_q, gb=gb)
+                                 conv_cache, s_cache, lens_q=lens_q, gb=gb, fp8=self.fp8)
+        return self._project_out(core, hidden.shape)
+
+    def _project_out(self, core, shape):
         with self._timed("out_proj"):
-            return ops.linear(core, self.w_out)
+            if not self.fp8:
+                return ops.linear(core, self.w_out)
+            core, scale = core if isinstance(core, tuple) else (core, None)
+            return ops.linear_fp8(core.reshape(*shape[:-1], self.core.value_dim), self.w_out, self.w_out_scale,
+                                  x_scale=scale)
+
+    def verify_tree(self, hidden, ids, conv_cache, s_cache, parents, pending: TreeStep | None = None):
+        """The mixer of one verify step over trees of T drafted tokens: hidden [B, T,
+        hidden] bf16 -> ([B, T, hidden] bf16, TreeStep).  ids, parents and pending as
+        GatedDeltaNetCore.verify_tree; in_proj, core and out_proj as forward."""
+        B, T, _ = hidden.shape
+        mixed, z, b, a, _ = self.project_in(hidden.reshape(B * T, -1))
+        self.core.timer = self.timer
+        core, step = self.core.verify_tree(mixed.reshape(B, T, -1), z.reshape(B, T, -1), b.reshape(B, T, -1),
+                                           a.reshape(B, T, -1), ids, conv_cache, s_cache, parents, pending=pending,
+                                           fp8=self.fp8)
+        if not isinstance(core, tuple):
+            core = core.reshape(B, T, self.core.value_dim)
+        return self._project_out(core, hidden.shape), step
+
+    def commit_tree(self, step: TreeStep, ids, conv_cache, s_cache) -> None:
+        self.core.timer = self.timer
+        self.core.commit_tree(step, ids, conv_cache, s_cache)

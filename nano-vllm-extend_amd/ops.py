@@ -48,6 +48,15 @@ def _stream(dev: torch.device) -> int:
     return _lib.stream_handle(dev)
 
 
+def _call_on(dev: torch.device, name: str, *args) -> None:
+    """_lib.call with `dev` as the current device: a launch goes to the stream's own."""
+    if dev.type == "cuda" and dev.index is not None and dev.index != torch.cuda.current_device():
+        with torch.cuda.device(dev):
+            _lib.call(name, *args)
+    else:
+        _lib.call(name, *args)
+
+
 # ------------------------------------------------------- fp16 operand range --
 # The chunk kernels run their state-path products on fp16 matrix cores: the
 # raw k and v rows (after the conv), Q', the block inverses, A, the state S
@@ -826,6 +835,189 @@ def state_tile_copy(src_pool: torch.Tensor, dst_pool: torch.Tensor, ids: torch.T
               ids64.numel(), src_pool.shape[1], src_pool.shape[-1], _stream(dev))
 
 
+# --------------------------------------------- verify over a tree of drafts --
+MAX_TREE_NODES = 64
+
+
+def _tree_parents(parents: torch.Tensor, B: int, T: int):
+    """(int32 parents, row stride) of a [B, T] or [T] (one tree for all) tensor."""
+    if parents.dtype not in (torch.int32, torch.int64) or tuple(parents.shape) not in ((B, T), (T,)):
+        raise ValueError(f"parents must be int32 or int64 [{B}, {T}] or [{T}], got {parents.dtype} "
+                         f"{tuple(parents.shape)}")
+    if not 1 <= T <= MAX_TREE_NODES:
+        raise ValueError(f"a tree has 1 to {MAX_TREE_NODES} nodes, got {T}")
+    if parents.dtype == torch.int64:
+        # (out of int32's range: not a node either way)
+        parents = parents.clamp(-2, MAX_TREE_NODES).to(torch.int32)
+    parents = parents.contiguous()
+    return parents, T if parents.dim() == 2 else 0
+
+
+def _tree_ids(ids: torch.Tensor, B: int, name: str = "ids") -> torch.Tensor:
+    if ids.shape != (B,) or ids.dtype not in (torch.int32, torch.int64):
+        raise ValueError(f"{name} must be int64 (or int32) [{B}], got {ids.dtype} {tuple(ids.shape)}")
+    return ids.to(torch.int64).contiguous()
+
+
+def _tree_rows(t: torch.Tensor, name: str, shape: tuple) -> torch.Tensor:
+    """bf16 [B, T, ...] with dense rows that the kernels read in 16-byte pieces (else copied once)."""
+    _bf16(t, name)
+    if tuple(t.shape) != shape:
+        raise ValueError(f"{name} must be {list(shape)}, got {list(t.shape)}")
+    width, dense, st = 1, True, t.stride()
+    for n, s in zip(reversed(shape[2:]), reversed(st[2:])):
+        dense &= n == 1 or s == width
+        width *= n
+    if not dense or t.data_ptr() % 16 or st[0] % 8 or st[1] % 8 or st[1] < width:
+        t = t.contiguous() if not t.is_contiguous() else t.clone()
+    return t
+
+
+def _tree_f32(t: torch.Tensor, name: str, shape: tuple) -> torch.Tensor:
+    if t.dtype != torch.float32 or tuple(t.shape) != shape:
+        raise ValueError(f"{name} must be float32 {list(shape)}, got {t.dtype} {list(t.shape)}")
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+def _conv_pool_ok(pool: torch.Tensor, C: int) -> None:
+    _bf16(pool, "conv_pool")
+    if pool.dim() != 3 or tuple(pool.shape[1:]) != (C, 3) or pool.stride(2) != 1:
+        raise ValueError(f"conv_pool must be a [slots, {C}, 3] view with contiguous taps, got {list(pool.shape)}")
+
+
+def _s_pool_ok(pool: torch.Tensor, Hv: int, D: int) -> None:
+    if not _state_view_ok(pool, Hv, D):
+        raise ValueError(f"s_pool must be an fp32 [slots, {Hv}, {D}, {D}] view with dense slots")
+
+
+def conv_tree_step(x: torch.Tensor, conv_pool: torch.Tensor, ids: torch.Tensor, weight: torch.Tensor,
+                   parents: torch.Tensor, pending: tuple | None = None) -> torch.Tensor:
+    """Causal conv + SiLU of a tree of T drafted tokens per sequence: the taps of a
+    node are its ancestors' rows and, past the root, the sequence's taps in the
+    pool, which stays as it is.  x [B, T, C] bf16; conv_pool [slots, C, 3]; ids
+    [B]; weight [C, 4] (or [C, 1, 4]); parents [B, T] (or [T], one tree for all):
+    the node before each node, -1 for the sequence's own state; a node whose
+    parent is neither -1 nor an earlier used node (-2 for padding) is unused and
+    its output 0.  A sequence whose id is no slot has zero outputs.
+
+    pending = (x, parents, accepted) of the step before: the rows on the path to
+    node accepted[b] of each sequence (-1: none) go into the pool first.  Along a
+    path the results are conv_decode_step's, bit for bit.  Returns y [B, T, C].
+    (No reference counterpart: spec decode is disabled for qwen3_5,
+    nanovllm/config.py:84.)"""
+    last_x, last_parents, accepted = pending if pending is not None else (None, None, None)
+    dev = _check_cuda(x, conv_pool, ids, weight, parents, last_x, last_parents, accepted)
+    if x.dim() != 3:
+        raise ValueError(f"x must be [B, T, C], got {list(x.shape)}")
+    B, T, C = x.shape
+    x = _tree_rows(x, "x", (B, T, C))
+    _conv_pool_ok(conv_pool, C)
+    _bf16(weight, "weight")
+    if weight.numel() != 4 * C or weight.shape[-1] != 4 or C % 8:
+        raise ValueError(f"weight must be [{C}, 4] (conv width 4) and C a multiple of 8")
+    w = weight.reshape(C, 4).contiguous()
+    ids64 = _tree_ids(ids, B)
+    par, p_b = _tree_parents(parents, B, T)
+    last = (None, 0, 0, None, 0, None, 0)
+    if pending is not None:
+        last_T = last_x.shape[1]
+        last_x = _tree_rows(last_x, "pending x", (B, last_T, C))
+        last_parents, lp_b = _tree_parents(last_parents, B, last_T)
+        accepted = _tree_ids(accepted, B, "accepted")
+        last = (_lib.ptr(last_x), last_x.stride(0), last_x.stride(1), _lib.ptr(last_parents), lp_b,
+                _lib.ptr(accepted), last_T)
+    y = torch.empty(B, T, C, dtype=torch.bfloat16, device=x.device)
+    _call_on(dev, "gdn_conv_tree", _lib.ptr(x), x.stride(0), x.stride(1), _lib.ptr(conv_pool), conv_pool.stride(0),
+             conv_pool.stride(1), conv_pool.shape[0], _lib.ptr(ids64), _lib.ptr(w), _lib.ptr(par), p_b, *last,
+             _lib.ptr(y), B, T, C, _stream(dev))
+    return y
+
+
+def recurrent_gdn_tree(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch.Tensor, beta: torch.Tensor,
+                       s_pool: torch.Tensor, ids: torch.Tensor, parents: torch.Tensor,
+                       pending: tuple | None = None):
+    """The gated delta rule over a tree of T drafted tokens per sequence: node t
+    continues from its parent's state, a root from the sequence's state in the
+    pool, which stays as it is.  q, k [B, T, Hk, D] and v [B, T, Hv, D] bf16 (after
+    the conv; q and k are L2-normalised here), g [B, T, Hv] fp32, beta [B, T, Hv]
+    bf16, s_pool [slots, Hv, D, D] fp32, ids [B], parents as conv_tree_step.
+
+    Returns (o [B, T, Hv, D] bf16, u [B, T, Hv, D] fp32): the outputs, and the
+    corrections from which, with k and g, the state after any node follows (no
+    state of a node is stored).  pending = (k, g, u, parents, accepted) of the
+    step before: the states after the accepted nodes go into the pool first, in
+    the same pass over them, and the trees start from there (accepted[b] -1, or no
+    used node: the row's state stays).
+    (No reference counterpart: spec decode is disabled for qwen3_5,
+    nanovllm/config.py:84; one token: qwen3_5.py:575-594.)"""
+    last_k, last_g, last_u, last_parents, accepted = pending if pending is not None else (None,) * 5
+    dev = _check_cuda(q, k, v, g, beta, s_pool, ids, parents, last_k, last_g, last_u, last_parents, accepted)
+    if k.dim() != 4 or v.dim() != 4:
+        raise ValueError(f"q, k, v must be [B, T, heads, D], got {list(k.shape)} and {list(v.shape)}")
+    B, T, Hk, D = k.shape
+    Hv = v.shape[2]
+    if Hk == 0 or Hv % Hk:
+        raise ValueError(f"{Hv} value heads are no multiple of {Hk} key heads")
+    q, k = _tree_rows(q, "q", (B, T, Hk, D)), _tree_rows(k, "k", (B, T, Hk, D))
+    v = _tree_rows(v, "v", (B, T, Hv, D))
+    g = _tree_f32(g, "g", (B, T, Hv))
+    _bf16(beta, "beta")
+    if beta.shape != (B, T, Hv):
+        raise ValueError(f"beta must be {[B, T, Hv]}, got {list(beta.shape)}")
+    beta = beta.contiguous()
+    _s_pool_ok(s_pool, Hv, D)
+    ids64 = _tree_ids(ids, B)
+    par, p_b = _tree_parents(parents, B, T)
+    last = (None, 0, 0, None, None, None, 0, None, 0)
+    if pending is not None:
+        last_T = last_k.shape[1]
+        last_k = _tree_rows(last_k, "pending k", (B, last_T, Hk, D))
+        last_g = _tree_f32(last_g, "pending g", (B, last_T, Hv))
+        last_u = _tree_f32(last_u, "pending u", (B, last_T, Hv, D))
+        last_parents, lp_b = _tree_parents(last_parents, B, last_T)
+        accepted = _tree_ids(accepted, B, "accepted")
+        last = (_lib.ptr(last_k), last_k.stride(0), last_k.stride(1), _lib.ptr(last_g), _lib.ptr(last_u),
+                _lib.ptr(last_parents), lp_b, _lib.ptr(accepted), last_T)
+    o = torch.empty(B, T, Hv, D, dtype=torch.bfloat16, device=v.device)
+    u = torch.empty(B, T, Hv, D, dtype=torch.float32, device=v.device)
+    _call_on(dev, "gdn_rule_tree", _lib.ptr(q), q.stride(0), q.stride(1), _lib.ptr(k), k.stride(0), k.stride(1),
+             _lib.ptr(v), v.stride(0), v.stride(1), _lib.ptr(g), _lib.ptr(beta), _lib.ptr(s_pool), s_pool.stride(0),
+             s_pool.shape[0], _lib.ptr(ids64), _lib.ptr(par), p_b, *last, _lib.ptr(o), _lib.ptr(u), B, T, Hk, Hv, D,
+             float(D ** -0.5), _stream(dev))
+    return o, u
+
+
+def commit_tree(s_pool: torch.Tensor, conv_pool: torch.Tensor, ids: torch.Tensor, parents: torch.Tensor,
+                accepted: torch.Tensor, x: torch.Tensor, k: torch.Tensor, g: torch.Tensor, u: torch.Tensor) -> None:
+    """The accepted path of a verified tree into both pools, for another user of the
+    slots than the next verify (whose `pending` does the same): row ids[b] of
+    s_pool becomes the state after node accepted[b], that of conv_pool the last
+    three raw rows on its path; -1 (or no used node) leaves both as they are.
+    x [B, T, C] the raw rows, k [B, T, Hk, D], g [B, T, Hv], u [B, T, Hv, D] and
+    parents those of the verified step."""
+    dev = _check_cuda(s_pool, conv_pool, ids, parents, accepted, x, k, g, u)
+    if k.dim() != 4 or u.dim() != 4 or x.dim() != 3:
+        raise ValueError(f"x, k, u must be [B, T, C], [B, T, Hk, D], [B, T, Hv, D], got {list(x.shape)}, "
+                         f"{list(k.shape)}, {list(u.shape)}")
+    B, T, Hk, D = k.shape
+    Hv, C = u.shape[2], x.shape[2]
+    if Hk == 0 or Hv % Hk:
+        raise ValueError(f"{Hv} value heads are no multiple of {Hk} key heads")
+    x, k = _tree_rows(x, "x", (B, T, C)), _tree_rows(k, "k", (B, T, Hk, D))
+    g, u = _tree_f32(g, "g", (B, T, Hv)), _tree_f32(u, "u", (B, T, Hv, D))
+    _s_pool_ok(s_pool, Hv, D)
+    _conv_pool_ok(conv_pool, C)
+    if conv_pool.shape[0] != s_pool.shape[0]:
+        raise ValueError(f"the pools have {s_pool.shape[0]} and {conv_pool.shape[0]} slots")
+    ids64, acc = _tree_ids(ids, B), _tree_ids(accepted, B, "accepted")
+    par, p_b = _tree_parents(parents, B, T)
+    _call_on(dev, "gdn_commit_tree", _lib.ptr(s_pool), s_pool.stride(0), _lib.ptr(conv_pool), conv_pool.stride(0),
+             conv_pool.stride(1), s_pool.shape[0], _lib.ptr(ids64), _lib.ptr(par), p_b, _lib.ptr(acc), _lib.ptr(x),
+             x.stride(0), x.stride(1), _lib.ptr(k), k.stride(0), k.stride(1), _lib.ptr(g), _lib.ptr(u), B, T, Hk, Hv,
+             D, C, _stream(dev))
+
+
 # ------------------------------------------------------------- projections --
 def linear(x: torch.Tensor, weight: torch.Tensor, out: torch.Tensor | None = None,
            gates: dict | None = None) -> torch.Tensor:
@@ -927,6 +1119,145 @@ def linear_cols(x: torch.Tensor, weight: torch.Tensor, widths: list[int],
     return parts if gates is None else (parts, g, beta)
 
 
+# ------------------------------------------------------- 8-bit projections --
+FP8 = torch.float8_e4m3fn
+FP8_GROUP = 128   # values with one scale
+
+
+def _rows_of(x: torch.Tensor, align: int) -> torch.Tensor:
+    """x [..., K] as [M, K] rows that the kernels read in 16-byte pieces."""
+    x2 = x.reshape(-1, x.shape[-1])
+    if x2.stride(1) != 1 or x2.stride(0) % align or x2.stride(0) < x2.shape[1] or x2.data_ptr() % 16:
+        x2 = x2.contiguous() if not x2.is_contiguous() else x2.clone()
+    return x2
+
+
+def _fp8_scales(M: int, G: int, dev) -> torch.Tensor:
+    """[M, G] fp32 with the rows of one group side by side (as the GEMM reads them)."""
+    return torch.empty(G, M, dtype=torch.float32, device=dev).t()
+
+
+def quantize_fp8(x: torch.Tensor):
+    """x [..., K] bf16 or fp32 (K a multiple of 128) -> (e4m3 [..., K], scales [M, K /
+    128] fp32): each row's groups of 128 columns have the scale max(amax * fp32(1 /
+    448), 2^-126), and a value is x times the scale's fp32 reciprocal, rounded to
+    nearest.  NaN stays NaN without counting in amax; an infinity makes its group's
+    scale infinite.  (The scales' memory holds the rows of a group side by side.)"""
+    dev = _check_cuda(x)
+    if x.dtype not in (torch.bfloat16, torch.float32):
+        raise TypeError(f"x must be bfloat16 or float32, got {x.dtype}")
+    K = x.shape[-1]
+    if x.dim() < 1 or K == 0 or K % FP8_GROUP:
+        raise ValueError(f"the last dim must be a positive multiple of {FP8_GROUP}, got {K}")
+    f32 = x.dtype == torch.float32
+    x2 = _rows_of(x, 4 if f32 else 8)
+    M = x2.shape[0]
+    y = torch.empty(x.shape, dtype=FP8, device=x.device)
+    scale = _fp8_scales(M, K // FP8_GROUP, x.device)
+    _call_on(dev, "gdn_quantize_fp8", _lib.ptr(x2), int(f32), x2.stride(0), _lib.ptr(y), K, _lib.ptr(scale),
+             1, M, M, K, 1, _stream(dev))
+    return y, scale
+
+
+def quantize_weight_fp8(weight: torch.Tensor):
+    """weight [N, K] bf16 or fp32 (nn.Linear layout, K a multiple of 128) -> (e4m3 [N,
+    K], scales [ceil(N / 128), K / 128] fp32), a scale for each 128 x 128 block; once,
+    when the weights are loaded.  The rounding is quantize_fp8's."""
+    dev = _check_cuda(weight)
+    if weight.dtype not in (torch.bfloat16, torch.float32):
+        raise TypeError(f"weight must be bfloat16 or float32, got {weight.dtype}")
+    if weight.dim() != 2 or weight.shape[1] == 0 or weight.shape[1] % FP8_GROUP:
+        raise ValueError(f"weight must be [N, K] with K a positive multiple of {FP8_GROUP}, got {list(weight.shape)}")
+    f32 = weight.dtype == torch.float32
+    w = _rows_of(weight, 4 if f32 else 8)
+    N, K = w.shape
+    y = torch.empty(N, K, dtype=FP8, device=w.device)
+    scale = torch.empty(-(-N // FP8_GROUP), K // FP8_GROUP, dtype=torch.float32, device=w.device)
+    _call_on(dev, "gdn_quantize_fp8", _lib.ptr(w), int(f32), w.stride(0), _lib.ptr(y), K, _lib.ptr(scale),
+             K // FP8_GROUP, 1, N, K, FP8_GROUP, _stream(dev))
+    return y, scale
+
+
+def _linear_fp8(x, weight, weight_scale, x_scale, outs, widths):
+    """The product into outs, whose columns are widths wide."""
+    dev = _check_cuda(x, weight, weight_scale, x_scale, *outs)
+    K, N = x.shape[-1], weight.shape[0]
+    G = K // FP8_GROUP
+    w = weight
+    if w.stride(1) != 1 or w.stride(0) % 16 or w.stride(0) < K or w.data_ptr() % 16:
+        w = w.contiguous() if not w.is_contiguous() else w.clone()
+    ws = weight_scale if weight_scale.stride(1) == 1 or G == 1 else weight_scale.contiguous()
+    if x_scale is None:
+        x, x_scale = quantize_fp8(x)
+    x2 = _rows_of(x, 16)
+    M = x2.shape[0]
+    n, ends, e = len(widths), [], 0
+    for wd in widths:
+        e += wd
+        ends.append(e)
+    c_arr = (ctypes.c_void_p * n)(*[p.data_ptr() for p in outs])
+    ld_arr = (ctypes.c_int64 * n)(*[p.stride(0) if M > 1 else max(p.stride(0), p.shape[1]) for p in outs])
+    end_arr = (ctypes.c_int * n)(*ends)
+    _call_on(dev, "gdn_gemm_fp8", _lib.ptr(x2), x2.stride(0), _lib.ptr(x_scale), x_scale.stride(0),
+             x_scale.stride(1), _lib.ptr(w), w.stride(0), _lib.ptr(ws), ws.stride(0) if ws.shape[0] > 1 else G, M, N, K,
+             n, c_arr, ld_arr, end_arr, _stream(dev))
+
+
+def _check_fp8(x, weight, weight_scale, x_scale):
+    if weight.dtype != FP8 or weight.dim() != 2:
+        raise TypeError(f"weight must be float8_e4m3fn [N, K], got {weight.dtype} {list(weight.shape)}")
+    N, K = weight.shape
+    if K == 0 or K % FP8_GROUP or x.shape[-1] != K:
+        raise ValueError(f"x [..., {x.shape[-1]}] and weight [{N}, {K}]: equal last dims, a positive multiple of "
+                         f"{FP8_GROUP}")
+    G = K // FP8_GROUP
+    if weight_scale.dtype != torch.float32 or tuple(weight_scale.shape) != (-(-N // FP8_GROUP), G):
+        raise ValueError(f"weight_scale must be float32 {[-(-N // FP8_GROUP), G]}, got {weight_scale.dtype} "
+                         f"{list(weight_scale.shape)}")
+    M = x.numel() // K
+    if x.dtype == FP8:
+        if x_scale is None or x_scale.dtype != torch.float32 or tuple(x_scale.shape) != (M, G):
+            raise ValueError(f"a float8_e4m3fn x needs x_scale float32 {[M, G]}")
+    elif x.dtype != torch.bfloat16 or x_scale is not None:
+        raise TypeError(f"x must be bfloat16, or float8_e4m3fn with x_scale, got {x.dtype}"
+                        + ("" if x_scale is None else " with x_scale"))
+
+
+def linear_fp8(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor,
+               x_scale: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """linear(x, weight) with the weight in e4m3 [N, K] and weight_scale [ceil(N / 128),
+    K / 128] fp32, one for each 128 x 128 block (quantize_weight_fp8's, or a
+    checkpoint's).  x [..., K] bf16, quantized in the call (quantize_fp8), or e4m3 with
+    its x_scale [M, K / 128] (any strides).  K a multiple of 128.  fp32 accumulation;
+    returns [..., N] bf16 (or writes `out`, a [M, N] view with contiguous rows)."""
+    _check_fp8(x, weight, weight_scale, x_scale)
+    N = weight.shape[0]
+    M = x.numel() // x.shape[-1]
+    if out is None:
+        y = torch.empty(M, N, dtype=torch.bfloat16, device=x.device)
+    else:
+        _bf16(out, "out")
+        if out.shape != (M, N) or (N > 1 and out.stride(1) != 1) or (M > 1 and out.stride(0) < N):
+            raise ValueError(f"out must be a {[M, N]} view with contiguous rows that do not overlap")
+        y = out
+    _linear_fp8(x, weight, weight_scale, x_scale, [y], [N])
+    return y.view(*x.shape[:-1], N) if out is None else y
+
+
+def linear_fp8_cols(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor, widths: list[int],
+                    x_scale: torch.Tensor | None = None) -> list[torch.Tensor]:
+    """linear_fp8 with the output's columns split into len(widths) (1-4) contiguous
+    tensors [..., widths[s]], every boundary a multiple of 16 (as linear_cols)."""
+    _check_fp8(x, weight, weight_scale, x_scale)
+    if not 1 <= len(widths) <= 4 or sum(widths) != weight.shape[0] or min(widths) <= 0 \
+            or any(w % 16 for w in widths[:-1]):
+        raise ValueError(f"widths {widths}: 1 to 4 parts of {weight.shape[0]} columns, boundaries at multiples of 16")
+    M = x.numel() // x.shape[-1]
+    parts = [torch.empty(M, w, dtype=torch.bfloat16, device=x.device) for w in widths]
+    _linear_fp8(x, weight, weight_scale, x_scale, parts, widths)
+    return [p.view(*x.shape[:-1], p.shape[1]) for p in parts]
+
+
 # -------------------------------------------------------------- gated norm --
 def rms_norm_gated(hidden_states: torch.Tensor, gate: torch.Tensor, weight: torch.Tensor,
                    eps: float, out: torch.Tensor | None = None) -> torch.Tensor:
@@ -976,6 +1307,32 @@ def rms_norm_gated_ranges(hidden_states: torch.Tensor, gate: torch.Tensor, weigh
     _lib.call("gdn_rmsnorm_gated_ranges", _lib.ptr(hidden_states), hidden_states.stride(0), _lib.ptr(gate),
               gate.stride(0), _lib.ptr(w), _lib.ptr(out), N, _lib.ptr(ranges), ranges.numel() // 3, n_sel_tok, H,
               D, float(eps), _stream(dev))
+
+
+def rms_norm_gated_fp8(hidden_states: torch.Tensor, gate: torch.Tensor, weight: torch.Tensor, eps: float):
+    """rms_norm_gated written in e4m3 for an 8-bit out projection: y = x * rsqrt(mean(x^2)
+    + eps) * w * silu(z) in fp32 over the last dim, then quantize_fp8's groups of 128
+    over a token's H * D columns (a multiple of 128), rounded once.  hidden_states / gate
+    [..., H, D] bf16.  Returns (e4m3 [..., H, D], scales [tokens, H * D / 128] fp32)."""
+    dev = _check_cuda(hidden_states, gate, weight)
+    _bf16(hidden_states, "hidden_states")
+    _bf16(gate, "gate")
+    if hidden_states.dim() < 2 or gate.shape != hidden_states.shape:
+        raise ValueError(f"hidden_states and gate must be [..., H, D] alike, got {list(hidden_states.shape)} and "
+                         f"{list(gate.shape)}")
+    H, D = hidden_states.shape[-2:]
+    w = weight.to(torch.bfloat16).contiguous()
+    if w.numel() != D or H == 0 or H * D % FP8_GROUP:
+        raise ValueError(f"weight must have {D} values and H * D = {H * D} be a multiple of {FP8_GROUP}")
+    x3, z3 = (t.reshape(-1, H, D) for t in (hidden_states, gate))
+    x3, z3 = (t if t.stride(2) == 1 and t.stride(1) == D and t.stride(0) % 8 == 0 and t.data_ptr() % 16 == 0
+              else t.contiguous() if not t.is_contiguous() else t.clone() for t in (x3, z3))
+    n_tok = x3.shape[0]
+    y = torch.empty(hidden_states.shape, dtype=FP8, device=hidden_states.device)
+    scale = _fp8_scales(n_tok, H * D // FP8_GROUP, hidden_states.device)
+    _call_on(dev, "gdn_rmsnorm_gated_fp8", _lib.ptr(x3), x3.stride(0), _lib.ptr(z3), z3.stride(0), _lib.ptr(w),
+             _lib.ptr(y), _lib.ptr(scale), 1, n_tok, n_tok, H, D, float(eps), _stream(dev))
+    return y, scale
 
 
 class Qwen3_5RMSNormGated(torch.nn.Module):

@@ -30,7 +30,6 @@ import torch
 own = False
 
 HK = 16          # key heads
-HIDDEN = 2048
 LAYERS = 2       # layers in a pool; the calls use the last one
 EPS = 1e-6
 BF16, F32, F64 = torch.bfloat16, torch.float32, torch.float64

@@ -1,0 +1,233 @@
+"""The 8-bit projections: quantize_fp8 and quantize_weight_fp8 bit for bit against the
+same fp32 steps in torch on the CPU; linear_fp8 against a 64-bit product of the values
+that its operands stand for; the gated norm in e4m3 against 64 bits; the mixer with
+8-bit weights against its own parts."""
+import pytest
+import torch
+
+import tree_ref as ref
+from helpers import BF16
+
+pytestmark = pytest.mark.gpu
+FP8 = torch.float8_e4m3fn
+
+
+def _rows(gen, M, K):
+    """Rows of very different sizes with a few loud columns."""
+    x = torch.randn(M, K, generator=gen) * torch.exp(4 * torch.rand(M, 1, generator=gen) - 2)
+    x[:, torch.rand(K, generator=gen) < 0.02] *= 30
+    return x
+
+
+def _bits(t):
+    return t.cpu().contiguous().view(torch.uint8)
+
+
+@pytest.mark.parametrize("M,K", [(1, 128), (1, 2048), (37, 4096), (257, 640), (1000, 1152)])
+@pytest.mark.parametrize("dtype", [BF16, torch.float32])
+def test_quantize_rows(pkg, dev, M, K, dtype):
+    x = _rows(torch.Generator().manual_seed(M + K), M, K).to(dtype)
+    x[0, :128] = 0                      # a group of zeros
+    if M > 3:
+        x[1, 0:128] = 1e-38             # below the smallest scale's range
+        x[2, 128 % K] = 3e38 if dtype == torch.float32 else 3.3e38
+    q, s = pkg.quantize_fp8(x.to(dev))
+    torch.cuda.synchronize()
+    rq, rs = ref.to_e4m3(x.float(), 1)
+    assert q.dtype == FP8 and q.shape == x.shape and tuple(s.shape) == (M, K // 128)
+    assert torch.equal(s.cpu(), rs)
+    assert torch.equal(_bits(q), _bits(rq))
+
+
+def test_quantize_rows_views_and_batches(pkg, dev):
+    gen = torch.Generator().manual_seed(3)
+    x = _rows(gen, 60, 1024).to(BF16)
+    rq, rs = ref.to_e4m3(x[:, 128:640].float(), 1)
+    xd = x.to(dev)
+    for view in (xd[:, 128:640], xd.view(5, 12, 1024)[..., 128:640], xd.t().contiguous().t()[:, 128:640]):
+        q, s = pkg.quantize_fp8(view)
+        torch.cuda.synchronize()
+        assert q.shape == view.shape
+        assert torch.equal(s.cpu(), rs) and torch.equal(_bits(q.view(60, 512)), _bits(rq))
+    odd = torch.empty(60 * 512 + 1, dtype=BF16, device=dev)[1:].view(60, 512)   # not 16-byte aligned
+    odd.copy_(xd[:, 128:640])
+    q, s = pkg.quantize_fp8(odd)
+    assert torch.equal(s.cpu(), rs) and torch.equal(_bits(q), _bits(rq))
+    q, s = pkg.quantize_fp8(xd[:0])
+    assert q.shape == (0, 1024) and tuple(s.shape) == (0, 8)
+
+
+def test_quantize_non_finite(pkg, dev):
+    """NaN stays NaN and does not count; an infinity makes the scale infinite, itself NaN, the rest 0."""
+    x = torch.randn(4, 256, generator=torch.Generator().manual_seed(4)).to(BF16)
+    clean_q, clean_s = pkg.quantize_fp8(x.to(dev))
+    x[1, 5], x[2, 200] = float("nan"), float("-inf")
+    q, s = pkg.quantize_fp8(x.to(dev))
+    qf = q.float().cpu()
+    keep = torch.ones(4, 256, dtype=torch.bool)
+    keep[1, 5] = False
+    keep[2, 128:] = False
+    assert torch.equal(_bits(q)[keep], _bits(clean_q)[keep])
+    assert torch.isnan(qf[1, 5]) and torch.isnan(qf[2, 200])
+    rest = torch.cat([qf[2, 128:200], qf[2, 201:]])
+    assert bool((rest == 0).all()) and torch.isinf(s[2, 1]).item() and torch.equal(s[1].cpu(), clean_s[1].cpu())
+
+
+@pytest.mark.parametrize("N,K", [(1, 128), (128, 256), (200, 1152), (2048, 2048)])
+@pytest.mark.parametrize("dtype", [BF16, torch.float32])
+def test_quantize_weight_blocks(pkg, dev, N, K, dtype):
+    w = _rows(torch.Generator().manual_seed(N + K), N, K).to(dtype)
+    q, s = pkg.quantize_weight_fp8(w.to(dev))
+    torch.cuda.synchronize()
+    rq, rs = ref.to_e4m3(w.float(), 128)
+    assert torch.equal(s.cpu(), rs) and torch.equal(_bits(q), _bits(rq))
+
+
+def _check(y, want, slack, tag):
+    d = (y.to(want.device).double() - want).abs()
+    bound = ref.HALF_BF16 * (want.abs() + slack) + slack
+    worst = float((d / bound.clamp(min=1e-300)).max()) if d.numel() else 0.0
+    assert bool((d <= bound).all()), f"{tag}: max |diff| / bound {worst:.2f}"
+
+
+# one row to thousands, K of one block, odd counts of blocks and many, N below, at and past the blocks' edges
+SHAPES = [(1, 1, 128), (1, 2048, 2048), (1, 12288, 2048), (3, 200, 128), (16, 256, 384), (17, 2048, 4096),
+          (33, 72, 640), (37, 8192, 2048), (64, 1000, 1152), (65, 130, 2048), (100, 520, 4992), (129, 2048, 2048),
+          (200, 12288, 2048), (256, 2048, 4096), (257, 384, 256), (300, 8192, 2048), (511, 513, 896),
+          (700, 4096, 2048), (1024, 12288, 2048), (1025, 2048, 1920), (2049, 2048, 2048), (4100, 333, 640)]
+
+
+@pytest.mark.parametrize("M,N,K", SHAPES)
+def test_linear_fp8(pkg, dev, M, N, K):
+    gen = torch.Generator().manual_seed(M * 7 + N + K)
+    x = _rows(gen, M, K).to(BF16)
+    w8, ws = ref.to_e4m3(_rows(gen, N, K) * K ** -0.5, 128)
+    x8, xs = ref.to_e4m3(x.float(), 1)
+    w8d, wsd = w8.to(dev), ws.to(dev)
+    y = pkg.linear_fp8(x.to(dev), w8d, wsd)
+    ready = pkg.linear_fp8(x8.to(dev), w8d, wsd, x_scale=xs.to(dev))
+    out = torch.full((M, N + 9), 7.0, dtype=BF16, device=dev)
+    pkg.linear_fp8(x8.to(dev), w8d, wsd, x_scale=xs.t().contiguous().t().to(dev), out=out[:, :N])
+    torch.cuda.synchronize()
+    assert y.shape == (M, N) and y.dtype == BF16
+    _check(y, *ref.linear(*(t.to(dev) for t in (x8, xs, w8, ws))), "from bf16")
+    assert torch.equal(ready, y)
+    # some rows and columns, the last ones among them, by the tight bound
+    rows = torch.cat([torch.randint(0, M, (8,), generator=gen), torch.arange(max(0, M - 8), M)])
+    cols = torch.cat([torch.randint(0, N, (100,), generator=gen), torch.arange(max(0, N - 40), N)])
+    _check(y[rows][:, cols], *ref.linear_tight(x8, xs, w8, ws, rows, cols), "tight")
+    assert torch.equal(out[:, :N], ready) and bool((out[:, N:] == 7).all())
+
+
+@pytest.mark.parametrize("M", [5, 300, 2000])
+def test_linear_fp8_cols(pkg, dev, M):
+    gen = torch.Generator().manual_seed(M)
+    K, widths = 512, [256, 144, 48, 100]
+    N = sum(widths)
+    x = _rows(gen, M, K).to(BF16).to(dev)
+    w8, ws = (t.to(dev) for t in ref.to_e4m3(_rows(gen, N, K), 128))
+    y = pkg.linear_fp8(x, w8, ws)
+    parts = pkg.ops.linear_fp8_cols(x.view(M, 1, K), w8, ws, widths)
+    torch.cuda.synchronize()
+    assert [tuple(p.shape) for p in parts] == [(M, 1, w) for w in widths]
+    assert torch.equal(torch.cat(parts, -1).view(M, N), y)
+
+
+def test_linear_fp8_views_empty_and_non_finite(pkg, dev):
+    gen = torch.Generator().manual_seed(8)
+    M, N, K = 70, 300, 512
+    big = _rows(gen, M, 2 * K).to(BF16).to(dev)
+    w8, ws = ref.to_e4m3(_rows(gen, N, 2 * K), 128)
+    w8, ws = w8.to(dev), ws.to(dev)
+    x, w, s = big[:, K:], w8[:, K:], ws[:, K // 128:]                    # strided operands and scales
+    y = pkg.linear_fp8(x, w, s)
+    assert torch.equal(y, pkg.linear_fp8(x.contiguous(), w.contiguous(), s.contiguous()))
+    x8, xs = pkg.quantize_fp8(big)
+    assert torch.equal(y, pkg.linear_fp8(x8[:, K:], w, s, x_scale=xs[:, K // 128:]))
+    assert pkg.linear_fp8(x[:0], w, s).shape == (0, N)
+    assert pkg.linear_fp8(x, w[:0], s[:0]).shape == (M, 0)
+    # a row with a NaN or an infinity is NaN, the others are what they were
+    bad = big.clone()
+    bad[3, K + 7], bad[9, K + 300] = float("nan"), float("inf")
+    z = pkg.linear_fp8(bad[:, K:], w, s)
+    rows = [r for r in range(M) if r not in (3, 9)]
+    assert torch.isnan(z[[3, 9]]).all().item() and torch.equal(z[rows], y[rows])
+
+
+def test_linear_fp8_same_bits_again(pkg, dev):
+    gen = torch.Generator().manual_seed(9)
+    w8, ws = (t.to(dev) for t in ref.to_e4m3(_rows(gen, 2048, 4096), 128))
+    for M in (1, 37, 600):
+        x = _rows(gen, M, 4096).to(BF16).to(dev)
+        y = pkg.linear_fp8(x, w8, ws)
+        for _ in range(3):
+            assert torch.equal(pkg.linear_fp8(x, w8, ws), y)
+
+
+@pytest.mark.parametrize("M,H,D", [(1, 1, 128), (1, 32, 128), (5, 2, 64), (33, 6, 64), (201, 32, 128), (1000, 16, 128)])
+def test_norm_fp8(pkg, dev, M, H, D):
+    """Scales within 64 half steps of fp32 of the 64-bit ones (the mean square over D
+    values, its root, exp and four products: under 48), values within half an e4m3 step (2^-4 of the value, 2^-10 of the
+    scale where steps are smallest) and the scaled value's own fp32 error."""
+    gen = torch.Generator().manual_seed(M + H)
+    x = (torch.randn(M, H, D, generator=gen) * torch.exp(-4 * torch.rand(M, H, 1, generator=gen))).to(BF16)
+    z = torch.randn(M, H, D, generator=gen).to(BF16) * 3
+    w = (1 + 0.1 * torch.randn(D, generator=gen)).to(BF16)
+    x[0] = 0                                                   # rows of zeros: smallest scale, zero values
+    y8, s = pkg.rms_norm_gated_fp8(x.to(dev), z.to(dev), w.to(dev), 1e-6)
+    strided = pkg.rms_norm_gated_fp8(torch.cat([x, x], 1).to(dev)[:, H:], torch.cat([z, z], 1).to(dev)[:, :H],
+                                     w.to(dev), 1e-6)
+    torch.cuda.synchronize()
+    xd, zd = x.double(), z.double()
+    want = xd / (xd.square().mean(-1, keepdim=True) + 1e-6).sqrt() * w.double() * zd * torch.sigmoid(zd)
+    flat = want.view(M, -1, 128)
+    scale = (flat.abs().amax(-1) / 448).clamp(min=2.0 ** -126)
+    assert y8.dtype == FP8 and y8.shape == x.shape and s.shape == scale.shape
+    assert bool(((s.cpu().double() - scale).abs() <= 64 * ref.U32 * scale).all())
+    got = y8.float().cpu().double().view(M, -1, 128) * s.cpu().double()[..., None]
+    bound = (2.0 ** -4 + 1e-5) * flat.abs() + (2.0 ** -10 + 1e-5) * scale[..., None]
+    assert bool(((got - flat).abs() <= bound).all())
+    assert torch.equal(_bits(strided[0]), _bits(y8)) and torch.equal(strided[1], s)
+
+
+def _layer(pkg, gen, dev, Hk, Hv, D, hidden, **kw):
+    C, V = 2 * Hk * D + Hv * D, Hv * D
+    n = lambda *s, std=1.0: (torch.randn(*s, generator=gen) * std).to(BF16).to(dev)  # noqa: E731
+    ws = [n(r, hidden, std=hidden ** -0.5) for r in (C, V, Hv, Hv)] + [n(hidden, V, std=V ** -0.5)]
+    rest = (Hk, Hv, D, n(C, 4, std=0.5), n(Hv), n(Hv), n(D, std=0.1) + 1)
+    return pkg.GatedDeltaNetLayer(*ws, *rest, weights="fp8", **kw), ws, rest
+
+
+@pytest.mark.parametrize("Hk,Hv,D,hidden", [(2, 4, 128, 256), (16, 16, 128, 2048), (2, 2, 64, 384)])
+def test_mixer_with_8_bit_weights(pkg, dev, Hk, Hv, D, hidden):
+    """The mixer's steps (prompts, one-token rows, both at once) are its parts called one by
+    one: linear_fp8 on the quantized weights, the core, linear_fp8 on the core's output."""
+    gen = torch.Generator().manual_seed(Hv + D)
+    layer, (w_qkv, w_z, w_b, w_a, w_out), rest = _layer(pkg, gen, dev, Hk, Hv, D, hidden)
+    C, V = layer.core.conv_dim, Hv * D
+    w_in8, w_in_s = pkg.quantize_weight_fp8(torch.cat([w_qkv, w_z]))
+    w_out8, w_out_s = pkg.quantize_weight_fp8(w_out)
+    if C % 128 == 0:      # a checkpoint's pairs give the same layer
+        pairs = [(w_in8[:C], w_in_s[:C // 128]), (w_in8[C:], w_in_s[C // 128:]), w_b, w_a, (w_out8, w_out_s)]
+        again = pkg.GatedDeltaNetLayer(*pairs, *rest, weights="fp8")
+        assert torch.equal(_bits(again.w_in), _bits(layer.w_in)) and torch.equal(again.w_in_scale, layer.w_in_scale)
+    core = pkg.GatedDeltaNetCore(*rest)
+    slots = 12
+    pools = [(torch.randn(slots, Hv, D, D, generator=gen) * 0.1).to(dev),
+             torch.randn(slots, C, 3, generator=gen).to(BF16).to(dev)]
+    for lens in ([1] * 5, [70, 3, 130], [1, 1, 1, 90, 20]):
+        N = sum(lens)
+        hidden_rows = torch.randn(N, hidden, generator=gen).to(BF16).to(dev)
+        ids = torch.randperm(slots, generator=gen)[:len(lens)].to(dev)
+        cu = torch.tensor([0] + lens).cumsum(0).to(torch.int32).to(dev)
+        mine, theirs = [t.clone() for t in pools], [t.clone() for t in pools]
+        y = layer.forward(hidden_rows, cu, max(lens), ids, mine[1], mine[0], lens_q=lens)
+        mixed, z = pkg.ops.linear_fp8_cols(hidden_rows, w_in8, w_in_s, [C, V])
+        ba = pkg.linear(hidden_rows, torch.cat([w_b, w_a]))
+        o = core.forward(mixed, z, ba[:, :Hv].contiguous(), ba[:, Hv:].contiguous(), cu, max(lens), ids, theirs[1],
+                         theirs[0], lens_q=lens, fp8=True)
+        o, s = o if isinstance(o, tuple) else (o, None)
+        want = pkg.linear_fp8(o.reshape(N, V), w_out8, w_out_s, x_scale=s)
+        torch.cuda.synchronize()
+        assert (s is not None) == (1 not in lens)
+        assert torch.equal(y, want) and torch.equal(mine[0], theirs[0]) and torch.equal(mine[1], theirs[1])

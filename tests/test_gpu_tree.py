@@ -1,0 +1,374 @@
+"""Verify steps over trees of drafted tokens: the conv and the gated delta rule of every
+node, and the accepted paths' way into the pools, against 64-bit forms that keep a state
+per node; chains against the token-by-token calls; steps in a row, in a captured graph
+and through the mixer."""
+import pytest
+import torch
+
+import tree_ref as ref
+from helpers import BF16
+
+pytestmark = pytest.mark.gpu
+
+
+def _inputs(gen, B, T, Hk, Hv, D, slow=False):
+    C = 2 * Hk * D + Hv * D
+    n = lambda *s: torch.randn(*s, generator=gen).to(BF16)  # noqa: E731
+    g = -torch.nn.functional.softplus(torch.randn(B, T, Hv, generator=gen)) * (0.02 if slow else 2.0)
+    return dict(y=n(B, T, C), x=n(B, T, C), g=g, beta=torch.sigmoid(torch.randn(B, T, Hv, generator=gen)).to(BF16),
+                u=torch.randn(B, T, Hv, D, generator=gen) * 0.5)
+
+
+def _qkv(y, Hk, Hv, D):
+    kd = Hk * D
+    return (y[..., :kd].unflatten(-1, (Hk, D)), y[..., kd:2 * kd].unflatten(-1, (Hk, D)),
+            y[..., 2 * kd:].unflatten(-1, (Hv, D)))
+
+
+def _close(got, want, bound, tag):
+    d = (got.detach().cpu().double() - want).abs()
+    worst = float((d / bound.clamp(min=1e-300)).max()) if d.numel() else 0.0
+    assert bool((d <= bound).all()), f"{tag}: max |diff| / bound {worst:.2f}"
+
+
+# one node, chains, bushy trees, the most nodes; one and several value heads per key head; both head dims
+RULE = [(1, 1, 1, 1, 128, 1), (2, 2, 2, 4, 128, 1), (3, 8, 2, 2, 128, 3), (2, 16, 1, 4, 128, 4), (3, 17, 2, 2, 64, 2),
+        (1, 33, 1, 2, 128, 1), (2, 48, 2, 2, 128, 8), (1, 64, 1, 1, 128, 1), (2, 64, 2, 2, 64, 5), (5, 7, 1, 3, 64, 2)]
+
+
+@pytest.mark.parametrize("B,T,Hk,Hv,D,back", RULE)
+@pytest.mark.parametrize("pending", [False, True])
+@pytest.mark.parametrize("slow", [False, True])
+def test_rule_against_a_state_per_node(pkg, dev, B, T, Hk, Hv, D, back, pending, slow):
+    gen = torch.Generator().manual_seed(1000 * B + T + Hv + 7 * pending)
+    i, last = _inputs(gen, B, T, Hk, Hv, D, slow), _inputs(gen, B, T + 3 if T + 3 <= 64 else T, Hk, Hv, D, slow)
+    parents, _ = ref.tree(gen, B, T, back, ragged=B > 1)
+    last_parents, accepted = ref.tree(gen, B, last["y"].shape[1], back, ragged=True)
+    slots = B + 2
+    pool = torch.randn(slots, 2, Hv, D, D, generator=gen) * 0.3          # two layers: strided slots
+    ids = torch.randperm(slots, generator=gen)[:B]
+    pool_d = pool.to(dev)
+    q, k, v = _qkv(i["y"].to(dev), Hk, Hv, D)
+    last_k = _qkv(last["y"], Hk, Hv, D)[1]
+    pend = tuple(t.to(dev) for t in (last_k, last["g"], last["u"], last_parents, accepted)) if pending else None
+    o, u = pkg.recurrent_gdn_tree(q, k, v, i["g"].to(dev), i["beta"].to(dev), pool_d[:, 1], ids.to(dev),
+                                  parents.to(dev), pending=pend)
+    torch.cuda.synchronize()
+    after = pool_d.cpu()
+    q, k, v = _qkv(i["y"], Hk, Hv, D)
+    for b in range(B):
+        S, extra = pool[ids[b], 1].double(), torch.zeros(Hv, D, D, dtype=torch.float64)
+        if pending and accepted[b] >= 0:
+            S, extra = ref.advanced(S, last_k[b], last["g"][b], last["u"][b], last_parents[b], int(accepted[b]))
+            _close(after[ids[b], 1], S, extra, f"row {b}: state")
+            S = after[ids[b], 1].double()      # the tree starts from the state as it was stored
+        else:
+            assert torch.equal(after[ids[b], 1], pool[ids[b], 1])
+        ro, ru, _, eo, eu = ref.rule(q[b], k[b], v[b], i["g"][b], i["beta"][b], S, parents[b])
+        _close(u[b], ru, eu, f"row {b}: u")
+        _close(o[b], ro, eo + ref.HALF_BF16 * (ro.abs() + eo) + 1e-30, f"row {b}: o")
+    others = [s for s in range(slots) if s not in ids.tolist()]
+    assert torch.equal(after[others], pool[others]) and torch.equal(after[:, 0], pool[:, 0])
+
+
+def test_rule_states_follow_from_u(pkg, dev):
+    """commit_tree's state after any node is the 64-bit state of that node."""
+    gen = torch.Generator().manual_seed(5)
+    B, T, Hk, Hv, D = 4, 13, 2, 4, 128
+    i = _inputs(gen, B, T, Hk, Hv, D)
+    parents, _ = ref.tree(gen, 1, T, 3)
+    parents = parents.expand(B, T).contiguous()
+    pool = torch.randn(B, Hv, D, D, generator=gen) * 0.3
+    ids = torch.arange(B)
+    q, k, v = _qkv(i["y"].to(dev), Hk, Hv, D)
+    gd = i["g"].to(dev)
+    o, u = pkg.recurrent_gdn_tree(q, k, v, gd, i["beta"].to(dev), pool.to(dev), ids.to(dev), parents[0].to(dev))
+    conv_pool = torch.zeros(B, i["x"].shape[2], 3, dtype=BF16, device=dev)
+    nodes = torch.tensor([0, 5, T - 1, 7])
+    got = pool.to(dev)
+    pkg.commit_tree(got, conv_pool, ids.to(dev), parents.to(dev), nodes.to(dev), i["x"].to(dev), k, gd, u)
+    torch.cuda.synchronize()
+    qc, kc, vc = _qkv(i["y"], Hk, Hv, D)
+    for b in range(B):
+        _, ru, states, _, eu = ref.rule(qc[b], kc[b], vc[b], i["g"][b], i["beta"][b], pool[b], parents[b])
+        P, A, depth = states[int(nodes[b])]
+        bound = (2 * D + 3 * T + 64) * (depth + 2) * ref.U32 * A
+        _close(got[b], P, bound, f"row {b}")
+
+
+@pytest.mark.parametrize("B,T,C,back", [(1, 1, 64, 1), (3, 5, 384, 2), (2, 16, 1032, 4), (1, 64, 8192, 1), (7, 33, 200, 6)])
+@pytest.mark.parametrize("pending", [False, True])
+def test_conv_against_64_bits(pkg, dev, B, T, C, back, pending):
+    gen = torch.Generator().manual_seed(B + T + C)
+    n = lambda *s: torch.randn(*s, generator=gen).to(BF16)  # noqa: E731
+    slots = B + 3
+    x, last_x, pool, w = n(B, T, C), n(B, min(64, T + 2), C), n(slots, 2, C, 3), n(C, 4)
+    parents, _ = ref.tree(gen, B, T, back, ragged=B > 1)
+    last_parents, accepted = ref.tree(gen, B, last_x.shape[1], back, ragged=True)
+    ids = torch.randperm(slots, generator=gen)[:B]
+    pool_d = pool.to(dev)
+    pend = tuple(t.to(dev) for t in (last_x, last_parents, accepted)) if pending else None
+    y = pkg.conv_tree_step(x.to(dev), pool_d[:, 1], ids.to(dev), w.to(dev), parents.to(dev), pending=pend)
+    torch.cuda.synchronize()
+    after = pool_d.cpu()
+    want_pool = pool.clone()
+    for b in range(B):
+        if pending and accepted[b] >= 0:
+            want_pool[ids[b], 1] = ref.taps_after(pool[ids[b], 1], last_x[b], last_parents[b], int(accepted[b]))
+        ry, e = ref.conv(x[b], want_pool[ids[b], 1], w, parents[b])
+        _close(y[b], ry, e, f"row {b}")
+    assert torch.equal(after.view(torch.int16), want_pool.view(torch.int16))
+
+
+@pytest.mark.parametrize("T,Hk,Hv,D", [(6, 2, 4, 128), (9, 2, 2, 64)])
+def test_a_chain_is_the_decode_steps(pkg, dev, T, Hk, Hv, D):
+    """A chain's conv rows are conv_decode_step's one after the other, bit for bit, and its
+    outputs and final state those of recurrent_gdn_multitoken up to fp32's rounding."""
+    gen = torch.Generator().manual_seed(T)
+    B = 3
+    C = 2 * Hk * D + Hv * D
+    i = _inputs(gen, B, T, Hk, Hv, D)
+    w = torch.randn(C, 4, generator=gen).to(BF16).to(dev)
+    conv_pool = torch.randn(B, C, 3, generator=gen).to(BF16).to(dev)
+    pool = (torch.randn(B, Hv, D, D, generator=gen) * 0.3).to(dev)
+    pool_before = pool.clone()
+    ids = torch.tensor([2, 0, 1], device=dev)
+    chain = torch.arange(-1, T - 1, device=dev)
+    x, g, beta = i["x"].to(dev), i["g"].to(dev), i["beta"].to(dev)
+    y = pkg.conv_tree_step(x, conv_pool, ids, w, chain)
+    step_pool = conv_pool.clone()
+    steps = torch.stack([pkg.conv_decode_step(x[:, t].contiguous(), step_pool, ids, w) for t in range(T)], 1)
+    q, k, v = _qkv(y, Hk, Hv, D)
+    o, u = pkg.recurrent_gdn_tree(q, k, v, g, beta, pool, ids, chain)
+    chain_pool = pool.clone()
+    want = pkg.recurrent_gdn_multitoken(q, k, v, g, beta, chain_pool, ids)
+    all_of_it = torch.full((B,), T - 1, device=dev)
+    pkg.commit_tree(pool, conv_pool, ids, chain, all_of_it, x, k, g, u)
+    torch.cuda.synchronize()
+    assert torch.equal(y.view(torch.int16), steps.view(torch.int16))
+    assert torch.equal(conv_pool.float(), step_pool.float())
+    # two fp32 evaluations, each within the 64-bit form's bounds
+    before = pool_before.cpu()
+    for n in range(B):
+        ro, _, states, eo, _ = ref.rule(*(t[n].cpu() for t in (q, k, v, g, beta)), before[ids[n]], chain.cpu())
+        bound = eo + ref.HALF_BF16 * (ro.abs() + eo)
+        _close(o[n], ro, bound, "tree o")
+        _close(want[n], ro, bound, "multitoken o")
+        P, A, depth = states[T - 1]
+        bound = (2 * D + 3 * T + 64) * (depth + 2) * ref.U32 * A
+        _close(pool[ids[n]], P, bound, "tree state")
+        _close(chain_pool[ids[n]], P, bound, "multitoken state")
+
+
+def test_unused_nodes_ids_out_of_range_and_nothing_accepted(pkg, dev):
+    """Links that lead nowhere, slots that are none and accepted nodes that are none: zeros
+    out, pools as they were, the other rows as without them."""
+    gen = torch.Generator().manual_seed(11)
+    B, T, Hk, Hv, D, slots = 6, 9, 1, 2, 128, 7
+    C = 2 * Hk * D + Hv * D
+    i, last = _inputs(gen, B, T, Hk, Hv, D), _inputs(gen, B, T, Hk, Hv, D)
+    parents, _ = ref.tree(gen, B, T, 3)
+    parents[1] = torch.tensor([-1, 0, 7, 2, -2, 4, 1, -5, 200])     # 2 waits on 7, 3 on 2; 4 unused, 5 on 4; -5, 200
+    parents[2] = -2                                                # no node at all
+    parents[3, 0] = 0                                              # its own parent: the whole tree hangs on it
+    ids = torch.tensor([3, 5, 0, 1, -1, slots])
+    accepted = torch.tensor([-1, 3, 4, T, 2, 2])                   # 3 of row 1 is unused; row 2's tree below is whole
+    last_parents = parents.clone()
+    last_parents[2] = torch.arange(-1, T - 1)
+    pool = torch.randn(slots, Hv, D, D, generator=gen)
+    conv_pool = torch.randn(slots, C, 3, generator=gen).to(BF16)
+    w = torch.randn(C, 4, generator=gen).to(BF16)
+    pd, cd = pool.to(dev), conv_pool.to(dev)
+    dv = lambda *ts: tuple(t.to(dev) for t in ts)  # noqa: E731
+    last_k = _qkv(last["y"], Hk, Hv, D)[1]
+    y = pkg.conv_tree_step(*dv(i["x"]), cd, *dv(ids, w, parents), pending=dv(last["x"], last_parents, accepted))
+    o, u = pkg.recurrent_gdn_tree(*_qkv(*dv(i["y"]), Hk, Hv, D), *dv(i["g"], i["beta"]), pd, *dv(ids, parents),
+                                  pending=dv(last_k, last["g"], last["u"], last_parents, accepted))
+    torch.cuda.synchronize()
+    y, o, u, pc, cc = y.cpu(), o.cpu(), u.cpu(), pd.cpu(), cd.cpu()
+    assert ref.used(parents[1].tolist()) == [True, True, False, False, False, False, True, False, False]
+    for b in range(B):
+        ok = torch.tensor(ref.used(parents[b].tolist())) & (0 <= int(ids[b]) < slots)
+        for t in (y[b], o[b], u[b]):
+            assert bool((t[~ok] == 0).all()) and (not ok.any() or bool((t[ok] != 0).any()))
+    keep = [s for s in range(slots) if s != 0]                     # row 2 alone committed (slot 0)
+    assert torch.equal(pc[keep], pool[keep]) and torch.equal(cc[keep], conv_pool[keep])
+    S, e = ref.advanced(pool[0], last_k[2], last["g"][2], last["u"][2], last_parents[2], 4)
+    _close(pc[0], S, e, "row 2")
+    assert torch.equal(cc[0], ref.taps_after(conv_pool[0], last["x"][2], last_parents[2], 4))
+    # the same through commit_tree
+    p2, c2 = pool.to(dev), conv_pool.to(dev)
+    pkg.commit_tree(p2, c2, *dv(ids, last_parents, accepted, last["x"], last_k, last["g"], last["u"]))
+    torch.cuda.synchronize()
+    assert torch.equal(c2.cpu(), cc) and torch.equal(p2.cpu()[keep], pool[keep])
+    _close(p2.cpu()[0], S, e, "row 2 by commit_tree")
+
+
+def test_extreme_decays(pkg, dev):
+    """g of -inf (all forgotten), of -1e4 and of 0: no NaN, the 64-bit values."""
+    gen = torch.Generator().manual_seed(13)
+    B, T, Hk, Hv, D = 2, 12, 1, 2, 128
+    i = _inputs(gen, B, T, Hk, Hv, D)
+    g = i["g"]
+    g[0, 3], g[0, 7], g[1, 5], g[1, 1] = float("-inf"), -1e4, 0.0, -200.0
+    parents = torch.arange(-1, T - 1, dtype=torch.int32)
+    pool = torch.randn(B, Hv, D, D, generator=gen)
+    q, k, v = _qkv(i["y"], Hk, Hv, D)
+    o, u = pkg.recurrent_gdn_tree(*_qkv(i["y"].to(dev), Hk, Hv, D), g.to(dev), i["beta"].to(dev), pool.to(dev),
+                                  torch.arange(B, device=dev), parents.to(dev))
+    torch.cuda.synchronize()
+    for b in range(B):
+        ro, ru, _, eo, eu = ref.rule(q[b], k[b], v[b], g[b], i["beta"][b], pool[b], parents)
+        _close(u[b], ru, eu, "u")
+        _close(o[b], ro, eo + ref.HALF_BF16 * (ro.abs() + eo), "o")
+
+
+def _mixer(pkg, gen, dev, weights, Hk, Hv, D, hidden):
+    C, V = 2 * Hk * D + Hv * D, Hv * D
+    n = lambda *s, std=1.0: (torch.randn(*s, generator=gen) * std).to(BF16).to(dev)  # noqa: E731
+    ws = [n(r, hidden, std=hidden ** -0.5) for r in (C, V, Hv, Hv)] + [n(hidden, V, std=V ** -0.5)]
+    return pkg.GatedDeltaNetLayer(*ws, Hk, Hv, D, n(C, 4, std=0.5), n(Hv), n(Hv), n(D, std=0.1) + 1, weights=weights)
+
+
+@pytest.mark.parametrize("weights", ["bf16", "fp8"])
+@pytest.mark.parametrize("Hk,Hv,D,hidden", [(2, 16, 128, 256), (8, 16, 64, 256)])  # (bf16 rows of 16-byte pieces)
+def test_mixer_steps_in_a_row(pkg, dev, weights, Hk, Hv, D, hidden):
+    """Three verify steps through the mixer, each committing the one before, then a commit
+    and a plain decode step: every node's output, the pools and the decode row are those of
+    a second layer's plain decode steps along each path (bf16 rounding of two ways)."""
+    gen = torch.Generator().manual_seed(17)
+    layer = _mixer(pkg, gen, dev, weights, Hk, Hv, D, hidden)
+    B, T, slots = 3, 6, 5
+    C = layer.core.conv_dim
+    pool = (torch.randn(slots, Hv, D, D, generator=gen) * 0.1).to(dev)
+    cpool = torch.randn(slots, C, 3, generator=gen).to(BF16).to(dev)
+    plain_pool, plain_cpool = pool.clone(), cpool.clone()
+    ids = torch.tensor([4, 1, 2], device=dev)
+
+    def decode(row, b, s, c):
+        """One token of sequence b on scratch pools."""
+        return layer.forward(row[None], torch.tensor([0, 1], dtype=torch.int32, device=dev), 1, ids[b:b + 1], c, s)[0]
+
+    step, worst = None, 0.0
+    for _ in range(3):
+        hidden_rows = torch.randn(B, T, hidden, generator=gen).to(BF16).to(dev)
+        parents, accepted = ref.tree(gen, B, T, 2)
+        y, step = layer.verify_tree(hidden_rows, ids, cpool, pool, parents.to(dev), pending=step)
+        step.accept(accepted.to(dev))
+        for b in range(B):
+            for t in range(T):
+                s, c = plain_pool.clone(), plain_cpool.clone()
+                for n in ref.path(parents[b].tolist(), t):
+                    out = decode(hidden_rows[b, n], b, s, c)
+                worst = max(worst, float((y[b, t].float() - out.float()).norm() / out.float().norm()))
+        for b in range(B):
+            for n in ref.path(parents[b].tolist(), int(accepted[b])):
+                decode(hidden_rows[b, n], b, plain_pool, plain_cpool)
+    layer.commit_tree(step, ids, cpool, pool)
+    torch.cuda.synchronize()
+    # Two evaluations in bf16 (or e4m3) of the same numbers: the projections of a row differ
+    # by a rounding now and then, each of relative 2^-8 (2^-4) on some of the values; the mixer's
+    # output is a sum over hundreds of them.
+    assert worst < (2e-2 if weights == "bf16" else 6e-2), worst
+    rel = float((pool - plain_pool).norm() / plain_pool.norm())
+    assert rel < (1e-2 if weights == "bf16" else 3e-2), rel
+    assert float((cpool.float() - plain_cpool.float()).norm() / plain_cpool.float().norm()) < 1e-2
+    untouched = [0, 3]
+    assert torch.equal(pool[untouched], plain_pool[untouched]) and torch.equal(cpool[untouched], plain_cpool[untouched])
+
+
+def test_pending_is_commit_then_verify(pkg, dev):
+    """A verify with the last step pending is commit_tree followed by one without."""
+    gen = torch.Generator().manual_seed(19)
+    B, T, Hk, Hv, D = 5, 16, 2, 4, 128
+    C = 2 * Hk * D + Hv * D
+    core = pkg.GatedDeltaNetCore(Hk, Hv, D, torch.randn(C, 4, generator=gen).to(BF16).to(dev),
+                                 *(torch.randn(Hv, generator=gen).to(BF16).to(dev) for _ in range(2)),
+                                 torch.ones(D, dtype=BF16, device=dev))
+    n = lambda *s: torch.randn(*s, generator=gen).to(BF16).to(dev)  # noqa: E731
+    s1 = (torch.randn(B + 1, Hv, D, D, generator=gen) * 0.1).to(dev)
+    c1 = n(B + 1, C, 3)
+    s2, c2 = s1.clone(), c1.clone()
+    ids = torch.randperm(B + 1, generator=gen)[:B].to(dev)
+    rows = [(n(B, T, C), n(B, T, Hv * D), n(B, T, Hv), n(B, T, Hv)) for _ in range(2)]
+    trees = [ref.tree(gen, B, T, 3, ragged=True) for _ in range(2)]
+    _, step = core.verify_tree(*rows[0], ids, c1, s1, trees[0][0].to(dev))
+    step.accept(trees[0][1].to(dev))
+    got, after = core.verify_tree(*rows[1], ids, c1, s1, trees[1][0].to(dev), pending=step)
+    core.commit_tree(step, ids, c2, s2)
+    want, other = core.verify_tree(*rows[1], ids, c2, s2, trees[1][0].to(dev))
+    torch.cuda.synchronize()
+    assert torch.equal(s1, s2) and torch.equal(c1, c2)
+    assert torch.equal(got, want) and torch.equal(after.u, other.u) and torch.equal(after.k, other.k)
+
+
+def test_graph_replays_equal_eager_steps(pkg, dev):
+    """Two alternating verify steps captured in one graph, each committing the other's accepted
+    paths, replayed with new rows, trees and accepted nodes; other work between the replays."""
+    gen = torch.Generator().manual_seed(23)
+    B, T, Hk, Hv, D, hidden = 4, 8, 2, 4, 128, 256
+    layer = _mixer(pkg, gen, dev, "fp8", Hk, Hv, D, hidden)
+    C = layer.core.conv_dim
+    pool = (torch.randn(B + 1, Hv, D, D, generator=gen) * 0.1).to(dev)
+    cpool = torch.randn(B + 1, C, 3, generator=gen).to(BF16).to(dev)
+    ids = torch.tensor([2, 0, 4, 1], device=dev)
+    hid = [torch.zeros(B, T, hidden, dtype=BF16, device=dev) for _ in range(2)]
+    par = [torch.zeros(B, T, dtype=torch.int32, device=dev) for _ in range(2)]
+    acc = [torch.full((B,), -1, device=dev) for _ in range(2)]
+
+    def both(step):
+        outs = []
+        for n in range(2):
+            y, step = layer.verify_tree(hid[n], ids, cpool, pool, par[n], pending=step)
+            step.accept(acc[n])
+            outs.append(y)
+        return outs, step
+
+    def load():
+        for n in range(2):
+            p, a = ref.tree(gen, B, T, 3, ragged=True)
+            hid[n].copy_(torch.randn(B, T, hidden, generator=gen).to(BF16))
+            par[n].copy_(p)
+            acc[n].copy_(a)
+
+    load()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        both(None)
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs, step = both(None)
+        layer.commit_tree(step, ids, cpool, pool)
+    for _ in range(3):
+        load()
+        start = pool.clone(), cpool.clone()
+        graph.replay()
+        torch.cuda.synchronize()
+        replayed = [t.clone() for t in (*outs, pool, cpool)]
+        pool.copy_(start[0])
+        cpool.copy_(start[1])
+        eager, step = both(None)
+        layer.commit_tree(step, ids, cpool, pool)
+        torch.cuda.synchronize()
+        for r, e in zip(replayed, (*eager, pool, cpool)):
+            assert torch.equal(r, e)
+
+
+def test_other_stream(pkg, dev):
+    gen = torch.Generator().manual_seed(29)
+    B, T, Hk, Hv, D = 3, 10, 1, 2, 128
+    i = _inputs(gen, B, T, Hk, Hv, D)
+    parents, _ = ref.tree(gen, B, T, 3)
+    pool = torch.randn(B, Hv, D, D, generator=gen).to(dev)
+    args = (*_qkv(i["y"].to(dev), Hk, Hv, D), i["g"].to(dev), i["beta"].to(dev), pool, torch.arange(B, device=dev),
+            parents.to(dev))
+    want = pkg.recurrent_gdn_tree(*args)
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        got = pkg.recurrent_gdn_tree(*args)
+    side.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))

@@ -1,0 +1,184 @@
+"""What the tree verify's and the 8-bit projections' entry points refuse, before any
+launch: the wrappers with the device check and the launch stubbed (CPU tensors), the C
+entry points with NULL or, where no GPU is visible, dummy aligned addresses."""
+import ctypes
+
+import pytest
+import torch
+
+BF16, FP8 = torch.bfloat16, torch.float8_e4m3fn
+
+
+class Launched(Exception):
+    pass
+
+
+@pytest.fixture
+def ops(pkg, monkeypatch):
+    def fake_call(*a, **k):
+        raise Launched()
+
+    monkeypatch.setattr(pkg.ops, "_check_cuda", lambda *ts: torch.device("cpu"))
+    monkeypatch.setattr(pkg.ops, "_stream", lambda dev: 0)
+    monkeypatch.setattr(pkg.ops._lib, "call", fake_call)
+    return pkg.ops
+
+
+def _refused(fn, good, **bad):
+    """fn with good arguments reaches the launch; with each bad one it does not."""
+    with pytest.raises(Launched):
+        fn(**good)
+    for name, values in bad.items():
+        for value in values:
+            with pytest.raises((ValueError, TypeError)):
+                fn(**{**good, name: value})
+
+
+def test_conv_tree_step_refuses(ops):
+    B, T, C = 3, 5, 64
+    x, pool, w = torch.zeros(B, T, C, dtype=BF16), torch.zeros(6, C, 3, dtype=BF16), torch.zeros(C, 1, 4, dtype=BF16)
+    ids, par = torch.arange(B), torch.zeros(B, T, dtype=torch.int32)
+    acc = torch.zeros(B, dtype=torch.int64)
+    _refused(ops.conv_tree_step, dict(x=x, conv_pool=pool, ids=ids, weight=w, parents=par, pending=(x, par, acc)),
+             x=[x.float(), x[0], torch.zeros(B, 65, C, dtype=BF16), x[..., :60]],
+             conv_pool=[pool.float(), pool[:, :60], pool[..., :2], pool.permute(0, 2, 1)],
+             ids=[ids[:2], ids.float(), ids[None]], weight=[w.float(), w[:60], torch.zeros(C, 3, dtype=BF16)],
+             parents=[par.float(), par[:2], par[:, :4], torch.zeros(T + 1, dtype=torch.int32)],
+             pending=[(x[:2], par, acc), (x, par[:, :4], acc), (x, par, acc[:2]), (x.float(), par, acc),
+                      (x, par, acc.float())])
+    for good in (torch.zeros(T, dtype=torch.int64), par.long(), par.expand(B, T)):
+        with pytest.raises(Launched):
+            ops.conv_tree_step(x, pool, ids, w, good)
+
+
+def test_recurrent_gdn_tree_refuses(ops):
+    B, T, Hk, Hv, D = 2, 4, 2, 4, 64
+    q, v = torch.zeros(B, T, Hk, D, dtype=BF16), torch.zeros(B, T, Hv, D, dtype=BF16)
+    g, beta, pool = torch.zeros(B, T, Hv), torch.zeros(B, T, Hv, dtype=BF16), torch.zeros(5, Hv, D, D)
+    ids, par, u = torch.arange(B), torch.zeros(B, T, dtype=torch.int32), torch.zeros(B, T, Hv, D)
+    _refused(ops.recurrent_gdn_tree, dict(q=q, k=q, v=v, g=g, beta=beta, s_pool=pool, ids=ids, parents=par,
+                                          pending=(q, g, u, par, ids)),
+             q=[q.float(), q[:, :3], q[..., :32]], k=[q[:1], q[:, :, :1], q[0]],
+             v=[v.float(), v[:, :, :3], v[..., :32]], g=[g.double(), g[..., :2], g[:1]],
+             beta=[beta.float(), beta[..., :2]], s_pool=[pool.double(), pool[:, :2], pool.transpose(2, 3)],
+             ids=[ids[:1], ids.float()], parents=[par[:1], par.bool()],
+             pending=[(q[:, :, :1], g, u, par, ids), (q, g[:, :3], u, par, ids), (q, g, u.double(), par, ids),
+                      (q, g, u, par[:, :2], ids), (q, g, u, par, ids[:1])])
+
+
+def test_commit_tree_refuses(ops):
+    B, T, Hk, Hv, D, C = 2, 4, 2, 4, 64, 512
+    k, u = torch.zeros(B, T, Hk, D, dtype=BF16), torch.zeros(B, T, Hv, D)
+    x, g, pool = torch.zeros(B, T, C, dtype=BF16), torch.zeros(B, T, Hv), torch.zeros(5, Hv, D, D)
+    cpool, ids, par = torch.zeros(5, C, 3, dtype=BF16), torch.arange(B), torch.zeros(B, T, dtype=torch.int32)
+    _refused(ops.commit_tree, dict(s_pool=pool, conv_pool=cpool, ids=ids, parents=par, accepted=ids, x=x, k=k, g=g,
+                                   u=u),
+             s_pool=[pool[:4], pool[:, :2]], conv_pool=[cpool[:, :8], cpool.float()], ids=[ids[:1]],
+             parents=[par[:, :2]], accepted=[ids[:1], ids.float()], x=[x[:, :3], x[0]], k=[k[:1], k.float()],
+             g=[g[:1]], u=[u[..., :32], u[0]])
+
+
+def test_8_bit_calls_refuse(ops):
+    M, N, K = 5, 200, 256
+    x, w8, ws = torch.zeros(M, K, dtype=BF16), torch.zeros(N, K, dtype=FP8), torch.ones(2, 2)
+    x8, xs = torch.zeros(M, K, dtype=FP8), torch.ones(M, 2)
+    out = torch.zeros(M, N, dtype=BF16)
+    _refused(ops.quantize_fp8, dict(x=x), x=[x.half(), x[:, :100], x[:, :0], x8])
+    _refused(ops.quantize_weight_fp8, dict(weight=out.new_zeros(N, K)),
+             weight=[x[0], x.half(), x[:, :130], w8])
+    _refused(ops.linear_fp8, dict(x=x8, weight=w8, weight_scale=ws, x_scale=xs, out=out),
+             x=[x, x8[:, :128], x.float()], weight=[w8.float(), w8[:, :128], w8[0]],
+             weight_scale=[ws[:1], ws[:, :1], ws.to(BF16)], x_scale=[None, xs[:4], xs[:, :1], xs.double()],
+             out=[out.float(), out[:4], out.t(), out.expand(M, N)[:, :100], out[:1].expand(M, N)])
+    _refused(ops.linear_fp8_cols, dict(x=x, weight=w8, weight_scale=ws, widths=[96, 104]),
+             widths=[[100, 100], [], [96, 96], [16] * 5 + [120], [-16, 216]])
+    n = torch.zeros(M, 4, 64, dtype=BF16)
+    _refused(ops.rms_norm_gated_fp8, dict(hidden_states=n, gate=n, weight=torch.ones(64), eps=1e-6),
+             hidden_states=[n.float(), n[:, :3], n[0, 0]], gate=[n.float(), n[:, :2]], weight=[torch.ones(32)])
+    odd = n[:, :3]
+    with pytest.raises(ValueError):      # 192 columns: no whole groups
+        ops.rms_norm_gated_fp8(odd, odd, torch.ones(64), 1e-6)
+
+
+def test_no_cpu_path(pkg):
+    with pytest.raises(ValueError):
+        pkg.quantize_fp8(torch.zeros(1, 128, dtype=BF16))
+    with pytest.raises(ValueError):
+        pkg.linear_fp8(torch.zeros(1, 128, dtype=BF16), torch.zeros(1, 128, dtype=FP8), torch.ones(1, 1))
+
+
+def test_steps_without_accepted_nodes_are_refused(pkg):
+    Hk = Hv = 2
+    D, C = 64, 384
+    core = pkg.GatedDeltaNetCore(Hk, Hv, D, torch.zeros(C, 4, dtype=BF16), torch.zeros(Hv), torch.zeros(Hv),
+                                 torch.ones(D), switches=pkg.Switches())
+    z = torch.zeros(1, 3, C, dtype=BF16)
+    step = pkg.TreeStep(z, z, z, z, torch.zeros(3, dtype=torch.int32))
+    with pytest.raises(ValueError):
+        core.commit_tree(step, None, None, None)
+    with pytest.raises(ValueError):
+        core.verify_tree(z, z, z, z, None, None, None, None, pending=step)
+    with pytest.raises(ValueError):
+        step.accept(torch.zeros(2, dtype=torch.int64))
+    off = pkg.GatedDeltaNetCore(Hk, Hv, D, torch.zeros(C, 4, dtype=BF16), torch.zeros(Hv), torch.zeros(Hv),
+                                torch.ones(D), switches=pkg.Switches(conv_kernel=False))
+    with pytest.raises(NotImplementedError):
+        off.verify_tree(z, z, z, z, None, None, None, None)
+    with pytest.raises(ValueError):
+        pkg.GatedDeltaNetLayer(*[torch.zeros(1, 1)] * 5, Hk, Hv, D, torch.zeros(C, 4), torch.zeros(Hv),
+                               torch.zeros(Hv), torch.ones(D), weights="int8")
+
+
+def test_c_entry_points_reject_before_launch(pkg):
+    lib, _lib = pkg._lib.load(), pkg._lib
+    inv, uns, ok = _lib.GDN_ERR_INVALID_ARG, _lib.GDN_ERR_UNSUPPORTED, _lib.GDN_OK
+    if torch.cuda.device_count() > 0:
+        pytest.skip("dummy device addresses are passed only where no GPU is visible")
+    P, odd = ctypes.c_void_p(1 << 20), ctypes.c_void_p((1 << 20) + 8)
+    # quantizer
+    q = lambda x=P, sx=256, y=P, sy=256, s=P, M=4, K=256, rows=1: lib.gdn_quantize_fp8(  # noqa: E731
+        x, 0, sx, y, sy, s, 2, 1, M, K, rows, None)
+    assert q(M=0) == ok and q(K=0) == ok
+    for bad in (dict(x=None), dict(x=odd), dict(sx=252), dict(sx=128), dict(y=None), dict(sy=250), dict(s=None),
+                dict(K=200), dict(rows=64), dict(M=-1)):
+        assert q(**bad) == inv, bad
+    # product
+    C1, ld1, end1 = (ctypes.c_void_p * 1)(1 << 20), (ctypes.c_int64 * 1)(96), (ctypes.c_int * 1)(96)
+    f = lambda A=P, lda=256, sa=P, ar=1, B=P, ldb=256, sb=P, br=2, M=4, N=96, K=256, n=1, C=C1, ld=ld1, e=end1: (  # noqa: E731,E501
+        lib.gdn_gemm_fp8(A, lda, sa, ar, 4, B, ldb, sb, br, M, N, K, n, C, ld, e, None))
+    assert f(M=0) == ok and f(N=0) == ok
+    for bad in (dict(A=None), dict(A=odd), dict(lda=248), dict(lda=128), dict(sa=None), dict(B=None), dict(B=odd),
+                dict(ldb=250), dict(sb=None), dict(br=1), dict(K=0), dict(K=192), dict(n=0), dict(n=5), dict(C=None),
+                dict(ld=(ctypes.c_int64 * 1)(90)), dict(e=(ctypes.c_int * 1)(90)), dict(M=1 << 24), dict(ar=-1),
+                dict(ar=1 << 28)):
+        assert f(**bad) == inv, bad
+    # norm
+    n = lambda x=P, sx=256, w=P, y=P, s=P, N=4, H=2, D=128: lib.gdn_rmsnorm_gated_fp8(  # noqa: E731
+        x, sx, P, 256, w, y, s, 1, 4, N, H, D, 1e-6, None)
+    assert n(N=0) == ok and n(D=96) == uns
+    for bad in (dict(x=None), dict(sx=252), dict(w=odd), dict(y=None), dict(s=None), dict(H=0), dict(H=3, D=64),
+                dict(N=-1)):
+        assert n(**bad) == inv, bad
+    # trees
+    C = 512
+    cv = lambda x=P, xb=8 * C, xt=C, pool=P, slot=3 * C, ch=3, y=P, B=2, T=8, Cc=C, lx=P, lt=C, acc=P, lT=8: (  # noqa: E731,E501
+        lib.gdn_conv_tree(x, xb, xt, pool, slot, ch, 4, P, P, P, 8, lx, 8 * C, lt, P, 8, acc, lT, y, B, T, Cc, None))
+    assert cv(B=0) == ok and cv(T=0) == ok and cv(T=65) == uns and cv(lT=65) == uns and cv(Cc=516) == uns
+    for bad in (dict(x=None), dict(x=odd), dict(xt=C - 8), dict(xb=4), dict(pool=None), dict(slot=3 * C - 3),
+                dict(ch=2), dict(y=None), dict(lx=None), dict(lt=C - 8), dict(lT=0), dict(B=-1)):
+        assert cv(**bad) == inv, bad
+    slot = 4 * 64 * 64
+    r = lambda q=P, qt=128, vt=256, g=P, s=P, st=slot, o=P, u=P, B=2, T=8, Hk=2, Hv=4, D=64, lu=P, lT=8: (  # noqa: E731,E501
+        lib.gdn_rule_tree(q, 8 * 128, qt, P, 8 * 128, 128, P, 8 * 256, vt, g, P, s, st, 4, P, P, 8, P, 8 * 128, 128,
+                          P, lu, P, 8, P, lT, o, u, B, T, Hk, Hv, D, 1.0, None))
+    assert r(B=0) == ok and r(T=65) == uns and r(D=96) == uns and r(lT=65) == uns
+    for bad in (dict(q=None), dict(qt=120), dict(vt=248), dict(g=None), dict(s=odd), dict(st=slot - 4), dict(o=None),
+                dict(u=odd), dict(Hk=3), dict(Hk=0), dict(lu=None), dict(lT=0), dict(T=-1)):
+        assert r(**bad) == inv, bad
+    c = lambda s=P, st=slot, cp=P, cs=3 * C, x=P, k=P, u=P, acc=P, B=2, T=8, Hk=2, Hv=4, D=64, Cc=C: (  # noqa: E731
+        lib.gdn_commit_tree(s, st, cp, cs, 3, 4, P, P, 8, acc, x, 8 * C, C, k, 8 * 128, 128, P, u, B, T, Hk, Hv, D,
+                            Cc, None))
+    assert c(B=0) == ok and c(T=65) == uns and c(D=32) == uns and c(Cc=500) == uns
+    for bad in (dict(s=None), dict(st=slot - 4), dict(cp=None), dict(cs=3 * C - 3), dict(x=None), dict(k=odd),
+                dict(u=None), dict(acc=None), dict(Hk=3)):
+        assert c(**bad) == inv, bad
