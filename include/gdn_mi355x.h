@@ -446,16 +446,26 @@ int gdn_quantize_fp8(const void* x, int x_is_fp32, int64_t sx, uint8_t* y, int64
  *   C[m][n] = bf16(sum over kb of sa[m][kb] sb[n / 128][kb] (sum over k of block kb of A[m][k] B[n][k]))
  * in fp32.  For the projections of gdn_gemm_bf16_cols at half the weight bytes.
  *   A  [M, K] e4m3, row stride lda; sa fp32, scale of row m and columns 128 kb .. at
- *      sa[m sa_row + kb sa_grp] (read fastest with sa_row = 1)
+ *      sa[m sa_row + kb sa_grp] (read fastest with sa_row = 1).  Or with a_is_bf16: bf16
+ *      rows, brought to e4m3 in the call as gdn_quantize_fp8 does (sa unused), through
+ *      workspace: gdn_gemm_fp8_workspace_size bytes (0: none is needed), 16-byte aligned,
+ *      dead after the call
  *   B  [N, K] e4m3 (the weight), row stride ldb; sb [ceil(N / 128), K / 128] fp32, row
  *      stride sb_row
  *   C  bf16, n_parts column parts as gdn_gemm_bf16_cols
- * K a multiple of 128; lda and ldb multiples of 16, A and B 16-byte aligned.  The order
- * in which the blocks' sums are added may depend on M, N and K.
+ * K a multiple of 128; lda a multiple of 16 (bf16: 8), ldb of 16, A and B 16-byte aligned.
+ * The order in which the blocks' sums are added may depend on M, N and K (not on which of
+ * the two A is: a call from bf16 rows has the bits of gdn_quantize_fp8 and one from its
+ * rows).  Inside of a
+ * block the matrix cores drop what lies below 2^-13 of the block's largest products.
  */
-int gdn_gemm_fp8(const uint8_t* A, int64_t lda, const float* sa, int64_t sa_row, int64_t sa_grp, const uint8_t* B,
-                 int64_t ldb, const float* sb, int64_t sb_row, int M, int N, int K, int n_parts, uint16_t* const* C,
-                 const int64_t* ldc, const int* col_end, void* stream);
+int gdn_gemm_fp8(const void* A, int a_is_bf16, int64_t lda, const float* sa, int64_t sa_row, int64_t sa_grp,
+                 const uint8_t* B, int64_t ldb, const float* sb, int64_t sb_row, int M, int N, int K, int n_parts,
+                 uint16_t* const* C, const int64_t* ldc, const int* col_end, void* workspace,
+                 int64_t workspace_bytes, void* stream);
+
+/* Workspace bytes of gdn_gemm_fp8; -1 on bad args. */
+int64_t gdn_gemm_fp8_workspace_size(int M, int N, int K, int a_is_bf16);
 
 /*
  * The gated RMSNorm of gdn_rmsnorm_gated written in e4m3: per token, groups of 128 of

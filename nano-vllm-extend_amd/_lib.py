@@ -68,7 +68,9 @@ SIGNATURES: dict[str, list] = {
     "gdn_state_tile_copy": [_p, _p, _i64, _p, _i32, _i32, _i32, _p],
     "gdn_rmsnorm_gated_ranges": [_p, _i64, _p, _i64, _p, _p, _i64, _p, _i32, _i64, _i32, _i32, _f32, _p],
     "gdn_quantize_fp8": [_p, _i32, _i64, _p, _i64, _p, _i64, _i64, _i64, _i32, _i32, _p],
-    "gdn_gemm_fp8": [_p, _i64, _p, _i64, _i64, _p, _i64, _p, _i64, _i32, _i32, _i32, _i32, _p, _p, _p, _p],
+    "gdn_gemm_fp8": [_p, _i32, _i64, _p, _i64, _i64, _p, _i64, _p, _i64, _i32, _i32, _i32, _i32, _p, _p, _p, _p, _i64,
+                     _p],
+    "gdn_gemm_fp8_workspace_size": [_i32, _i32, _i32, _i32],
     "gdn_rmsnorm_gated_fp8": [_p, _i64, _p, _i64, _p, _p, _p, _i64, _i64, _i64, _i32, _i32, _f32, _p],
     "gdn_conv_tree": [_p, _i64, _i64, _p, _i64, _i64, _i64, _p, _p, _p, _i64, _p, _i64, _i64, _p, _i64, _p, _i32, _p,
                       _i32, _i32, _i32, _p],
@@ -80,7 +82,8 @@ SIGNATURES: dict[str, list] = {
 
 # entry points whose return type is not int (status)
 RESTYPES = {"gdn_chunk_prefill_workspace_size": ctypes.c_int64,
-            "gdn_conv_chunk_prefill_workspace_size": ctypes.c_int64}
+            "gdn_conv_chunk_prefill_workspace_size": ctypes.c_int64,
+            "gdn_gemm_fp8_workspace_size": ctypes.c_int64}
 
 _LIB: ctypes.CDLL | None = None
 

@@ -42,71 +42,6 @@ struct Fp8Scales {
   int64_t b_row;
 };
 
-// 64 x 64 tiles, 4 waves of 32 x 32, one LDS stage: the plain kernel.
-__global__ __launch_bounds__(kFp8Threads) void gemm_fp8_kernel(const uint8_t* __restrict__ A, int64_t lda,
-                                                               const uint8_t* __restrict__ B, int64_t ldb,
-                                                               Fp8Scales sc, GemmOut out, int M, int N, int K) {
-  __shared__ __align__(16) uint8_t st[128 * 128];
-  const int mb_n = (M + 63) / 64;
-  const int64_t L = gdn::xcd_remap(blockIdx.x, static_cast<int64_t>(mb_n) * ((N + 63) / 64));
-  if (L < 0) return;
-  const int m0 = 64 * static_cast<int>(L % mb_n), n0 = 64 * static_cast<int>(L / mb_n);
-  const int lane = threadIdx.x & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int wm = wave >> 1, wn = wave & 1;
-  const int lr = lane & 15, lg = lane >> 4;
-  const __amdgpu_buffer_rsrc_t ra = rsrc_of(A), rb = rsrc_of(B);
-  // the wave's 1 KiB blocks: A rows 8 wave .. and 32 + 8 wave .., the same of B
-  int va[2], vb[2];
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int r = 32 * i + 8 * wave + (lane >> 3);
-    va[i] = static_cast<int>(min(m0 + r, M - 1) * lda + 16 * ((lane & 7) ^ ((r >> 1) & 7)));
-    vb[i] = static_cast<int>(min(n0 + r, N - 1) * ldb + 16 * ((lane & 7) ^ (((r >> 1) & 1) | (((r >> 3) & 3) << 1))));
-  }
-  gdn::f32x4_t acc[2][2];
-#pragma unroll
-  for (int i = 0; i < 2; ++i)
-#pragma unroll
-    for (int t = 0; t < 2; ++t) acc[i][t] = gdn::f32x4_t{0.f, 0.f, 0.f, 0.f};
-  const float* sa[2];
-#pragma unroll
-  for (int i = 0; i < 2; ++i) sa[i] = sc.a + min(m0 + 32 * wm + 16 * i + lr, M - 1) * sc.a_row;
-  const float* sb = sc.b + n0 / 128 * sc.b_row;
-  for (int kb = 0; kb < K / 128; ++kb) {
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      dma16(ra, st + (32 * i + 8 * wave) * 128, va[i], 128 * kb);
-      dma16(rb, st + (64 + 32 * i + 8 * wave) * 128, vb[i], 128 * kb);
-    }
-    __syncthreads();
-    Frag8 fa[2], fb[2];
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int r = 32 * wm + 16 * i + lr;
-      fa[i].lo = *reinterpret_cast<const i32x4_t*>(st + sw_off(r, lg));
-      fa[i].hi = *reinterpret_cast<const i32x4_t*>(st + sw_off(r, 4 + lg));
-      const int c = 32 * wn + 8 * (lr >> 2) + 4 * i + (lr & 3);
-      fb[i].lo = *reinterpret_cast<const i32x4_t*>(st + 64 * 128 + swb_off(c, lg));
-      fb[i].hi = *reinterpret_cast<const i32x4_t*>(st + 64 * 128 + swb_off(c, 4 + lg));
-    }
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const float s = sa[i][kb * sc.a_grp] * sb[kb];
-#pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        const gdn::f32x4_t p = mfma_fp8(fb[t], fa[i]);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) acc[i][t][e] = fmaf(p[e], s, acc[i][t][e]);
-      }
-    }
-    __syncthreads();
-  }
-#pragma unroll
-  for (int i = 0; i < 2; ++i)
-    gemm_store16(acc[i][0], acc[i][1], out, M, N, m0 + 32 * wm + 16 * i, n0 + 32 * wn, lane, GemmGates{}, nullptr);
-}
-
 // ---- 256 x 256 tiles, 8 waves in two alternating groups ----
 // gemm_tn_pp_kernel of the bf16 GEMM with K-steps of 128: the same bytes per step, the
 // same sections and waits, one product where it has two.  What is added per section:
@@ -423,46 +358,473 @@ __global__ __launch_bounds__(kPPThreads, 2) void gemm_fp8_pp_kernel(const uint8_
   __builtin_amdgcn_s_waitcnt(0);
 }
 
-int fp8_launch(const uint8_t* A, int64_t lda, const uint8_t* B, int64_t ldb, const Fp8Scales& sc, const GemmOut& out,
-               int M, int N, int K, hipStream_t st) {
-  const int64_t t256 = static_cast<int64_t>((M + 255) / 256) * ((N + 255) / 256);
-  const int64_t t128 = static_cast<int64_t>((M + 127) / 128) * ((N + 127) / 128);
-  const int64_t tiles = static_cast<int64_t>((M + 63) / 64) * ((N + 63) / 64);
+// the larger of each pair of 16-bit halves
+typedef uint16_t u16x2_t __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {
+  const u16x2_t x = __builtin_bit_cast(u16x2_t, a), y = __builtin_bit_cast(u16x2_t, b);
+  return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(x, y));
+}
+
+// ---- few rows: a load ring per wave ----
+// As the bf16 GEMM's ring kernel: BM rows x BN columns of C per workgroup, the K-steps
+// of 128 dealt to its NW waves in turn, each wave with NS stages of its own in LDS and
+// no barrier in the loop; the partial sums are added through LDS in wave order.  What
+// bounds it: the loads' latency times the bytes in flight.
+//
+// kQuant: A is bf16 and is brought to e4m3 here (gdn::fp8_scale, the bits of
+// gdn_quantize_fp8), a lane's 32 values of a row in its registers and the largest
+// magnitude over the four lanes that share the row: no launch of its own and nothing
+// written.  Every workgroup repeats it for its rows, so it is for few of them.
+template <int BM, int BN, int NW, int NS, bool kQuant>
+__global__ __launch_bounds__(64 * NW) void gemm_fp8_ring_kernel(const void* __restrict__ A, int64_t lda,
+                                                                const uint8_t* __restrict__ B, int64_t ldb,
+                                                                Fp8Scales sc, GemmOut out, int M, int N, int K) {
+  constexpr int MT = BM / 16, NT = BN / 32;
+  constexpr int kARow = kQuant ? 256 : 128;               // bytes of a row of A in LDS
+  constexpr int kABytes = BM * kARow, kBBytes = BN * 128;
+  constexpr int kStage = kABytes + kBBytes + 256 * (kQuant ? 1 : 2);
+  constexpr int kAPer = kABytes / 1024, kBPer = kBBytes / 1024;
+  constexpr int kPer = kAPer + kBPer + (kQuant ? 1 : 2);  // loads of a stage
+  constexpr int kVm = (NS - 1) * kPer;
+  static_assert(kVm < 64 && NS >= 2 && NS <= 3, "vmcnt field");
+  constexpr int kWait = (kVm & 15) | (7 << 4) | (15 << 8) | ((kVm >> 4) << 14);
+  __shared__ __align__(16) uint8_t st0[NW * kStage];
+  __shared__ __align__(16) uint8_t st1[NW * kStage];
+  __shared__ __align__(16) uint8_t st2[NS > 2 ? NW * kStage : 16];
+  static_assert(MT * NT * 2048 <= kStage, "the partial sums fit a stage");
+  const int mb_n = (M + BM - 1) / BM, nb_n = (N + BN - 1) / BN;
+  // the row blocks of a column block on one XCD, so that its L2 reads the weights once
+  const int64_t L = gdn::xcd_remap(blockIdx.x, static_cast<int64_t>(mb_n) * nb_n);
+  if (L < 0) return;
+  const int m0 = BM * static_cast<int>(L % mb_n), n0 = BN * static_cast<int>(L / mb_n);
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lr = lane & 15, lg = lane >> 4;
+  const __amdgpu_buffer_rsrc_t ra = rsrc_of(A), rb = rsrc_of(B), rsa = rsrc_of(sc.a), rsb = rsrc_of(sc.b);
+  int goff[kAPer + kBPer];
+#pragma unroll
+  for (int i = 0; i < kAPer; ++i) {
+    if constexpr (kQuant) {
+      // 4 rows of 256 bytes; granule c of row r at slot c ^ (r % 16)
+      const int r = 4 * i + (lane >> 4);
+      goff[i] = static_cast<int>(min(m0 + r, M - 1) * lda * 2 + 16 * ((lane & 15) ^ (r & 15)));
+    } else {
+      const int r = 8 * i + (lane >> 3);
+      goff[i] = static_cast<int>(min(m0 + r, M - 1) * lda + 16 * ((lane & 7) ^ ((r >> 1) & 7)));
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < kBPer; ++i) {
+    const int r = 8 * i + (lane >> 3);
+    goff[kAPer + i] = static_cast<int>(min(n0 + r, N - 1) * ldb +
+                                       16 * ((lane & 7) ^ (((r >> 1) & 1) | (((r >> 3) & 3) << 1))));
+  }
+  const int va = kQuant ? 0 : static_cast<int>(min(m0 + lane % BM, M - 1) * sc.a_row * 4);
+  const int vb = static_cast<int>(n0 / 128 * sc.b_row * 4);
+  const int nk = K / 128;
+  auto issue = [&](uint8_t* st, int step) {
+    const int s = min(step, nk - 1);
+    uint8_t* w = st + wave * kStage;
+#pragma unroll
+    for (int i = 0; i < kAPer; ++i) dma16(ra, w + i * 1024, goff[i], kARow * s);
+#pragma unroll
+    for (int i = 0; i < kBPer; ++i) dma16(rb, w + kABytes + i * 1024, goff[kAPer + i], 128 * s);
+    dma4(rsb, w + kABytes + kBBytes, vb, 4 * s);
+    if constexpr (!kQuant) dma4(rsa, w + kABytes + kBBytes + 256, va, static_cast<int>(sc.a_grp) * 4 * s);
+  };
+  gdn::f32x4_t acc[MT][NT][2];
+#pragma unroll
+  for (int i = 0; i < MT; ++i)
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+      for (int t = 0; t < 2; ++t) acc[i][j][t] = gdn::f32x4_t{0.f, 0.f, 0.f, 0.f};
+  auto one = [&](uint8_t* st, int step) {
+    const uint8_t* a = st + wave * kStage;
+    const uint8_t* b = a + kABytes;
+    const float* p = reinterpret_cast<const float*>(b + kBBytes);
+    Frag8 fa[MT], fb[NT][2];
+    float f[MT];
+    uint4 raw[kQuant ? MT : 1][4];
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+      const int r = 16 * i + lr;
+      if constexpr (kQuant) {
+#pragma unroll
+        for (int c = 0; c < 4; ++c)  // granules 2 lg, 2 lg + 1, 8 + 2 lg, 9 + 2 lg
+          raw[i][c] = *reinterpret_cast<const uint4*>(a + r * 256 + 16 * ((8 * (c >> 1) + 2 * lg + (c & 1)) ^ (r & 15)));
+      } else {
+        fa[i].lo = *reinterpret_cast<const i32x4_t*>(a + sw_off(r, lg));
+        fa[i].hi = *reinterpret_cast<const i32x4_t*>(a + sw_off(r, 4 + lg));
+        f[i] = p[64 + r];
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        const int r = 8 * (lr >> 2) + 4 * t + (lr & 3);
+        fb[j][t].lo = *reinterpret_cast<const i32x4_t*>(b + 4096 * j + swb_off(r, lg));
+        fb[j][t].hi = *reinterpret_cast<const i32x4_t*>(b + 4096 * j + swb_off(r, 4 + lg));
+      }
+    const float sb = p[0];
+    // the reads have returned before the stage is loaded again
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_waitcnt(kWaitLds);
+    __builtin_amdgcn_sched_barrier(0);
+    issue(st, step + NS * NW);
+    if constexpr (kQuant) {
+#pragma unroll
+      for (int i = 0; i < MT; ++i) {
+        // the largest magnitude, two values at a time in 16-bit integers (bf16 magnitudes
+        // are ordered as such), then as a float; one at a time where there is a NaN,
+        // which sorts above infinity there and must not count
+        float v[32];
+        uint32_t top = 0;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          const uint32_t w[4] = {raw[i][c].x, raw[i][c].y, raw[i][c].z, raw[i][c].w};
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            v[8 * c + 2 * e] = __uint_as_float(w[e] << 16);
+            v[8 * c + 2 * e + 1] = __uint_as_float(w[e] & 0xffff0000u);
+            top = max2(top, w[e] & 0x7fff7fffu);
+          }
+        }
+        float m = __uint_as_float(max(top & 0xffffu, top >> 16) << 16);
+        if (__builtin_expect(m != m, 0)) {
+          m = 0.0f;
+#pragma unroll
+          for (int e = 0; e < 32; ++e) m = fmaxf(m, fabsf(v[e]));
+        }
+        m = fmaxf(m, __shfl_xor(m, 16, 64));
+        m = fmaxf(m, __shfl_xor(m, 32, 64));
+        f[i] = gdn::fp8_scale(m);
+        const float inv = 1.0f / f[i];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          fa[i].lo[e] = gdn::f2fp8x4(v[4 * e] * inv, v[4 * e + 1] * inv, v[4 * e + 2] * inv, v[4 * e + 3] * inv);
+          fa[i].hi[e] = gdn::f2fp8x4(v[16 + 4 * e] * inv, v[17 + 4 * e] * inv, v[18 + 4 * e] * inv,
+                                     v[19 + 4 * e] * inv);
+        }
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+      const float s = f[i] * sb;
+#pragma unroll
+      for (int j = 0; j < NT; ++j)
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          const gdn::f32x4_t r = mfma_fp8(fb[j][t], fa[i]);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[i][j][t][e] = fmaf(r[e], s, acc[i][j][t][e]);
+        }
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_waitcnt(kWait);
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  issue(st0, wave);
+  issue(st1, wave + NW);
+  if constexpr (NS == 3) issue(st2, wave + 2 * NW);
+  __builtin_amdgcn_s_waitcnt(kWait);
+  int s = wave;
+  for (; s + (NS - 1) * NW < nk; s += NS * NW) {
+    one(st0, s);
+    one(st1, s + NW);
+    if constexpr (NS == 3) one(st2, s + 2 * NW);
+  }
+  if (s < nk) one(st0, s);
+  if (NS == 3 && s + NW < nk) one(st1, s + NW);
+  // the repeated loads past the last step land before the stages are reused
+  __builtin_amdgcn_s_waitcnt(0);
+  __syncthreads();
+  gdn::f32x4_t* red = reinterpret_cast<gdn::f32x4_t*>(st0);  // [wave][row tile][column tile][lane]
+#pragma unroll
+  for (int i = 0; i < MT; ++i)
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+      for (int t = 0; t < 2; ++t) red[(((wave * MT + i) * NT + j) * 2 + t) * 64 + lane] = acc[i][j][t];
+  __syncthreads();
+  for (int ij = wave; ij < MT * NT; ij += NW) {
+    gdn::f32x4_t c0 = red[(ij * 2) * 64 + lane], c1 = red[(ij * 2 + 1) * 64 + lane];
+#pragma unroll
+    for (int w = 1; w < NW; ++w) {
+      c0 += red[((w * MT * NT + ij) * 2) * 64 + lane];
+      c1 += red[((w * MT * NT + ij) * 2 + 1) * 64 + lane];
+    }
+    gemm_store16(c0, c1, out, M, N, m0 + 16 * (ij / NT), n0 + 32 * (ij % NT), lane, GemmGates{}, nullptr);
+  }
+}
+
+// ---- 64-row tiles with a deeper load pipeline ----
+// As the bf16 GEMM's deep kernel: 64 x BN tiles, NS stages as objects of their own, the
+// loads of step s + NS - 1 at the start of step s, the barrier before it waiting for
+// step s alone.  The scales of a step come with its operands (wave 0 the rows', the
+// others B's: a load each).
+template <int BN, int NS>
+__global__ __launch_bounds__(kFp8Threads, 2) void gemm_fp8_deep_kernel(const uint8_t* __restrict__ A, int64_t lda,
+                                                                       const uint8_t* __restrict__ B, int64_t ldb,
+                                                                       Fp8Scales sc, GemmOut out, int M, int N,
+                                                                       int K) {
+  static_assert(NS == 3 || NS == 4, "three or four stages");
+  constexpr int BM = 64, NJ = BN / 64;  // column pairs of 32 per wave
+  constexpr int kStage = (BM + BN) * 128 + 1024;
+  constexpr int kAPer = BM / 32, kBPer = BN / 32, kPer = kAPer + kBPer + 1;
+  constexpr int kVm = (NS - 2) * kPer;
+  static_assert(kVm < 64, "vmcnt field");
+  constexpr int kWait = (kVm & 15) | (7 << 4) | ((kVm >> 4) << 14);
+  __shared__ __align__(16) uint8_t st0[kStage];
+  __shared__ __align__(16) uint8_t st1[kStage];
+  __shared__ __align__(16) uint8_t st2[kStage];
+  __shared__ __align__(16) uint8_t st3[NS == 4 ? kStage : 16];
+
+  const int mb_n = (M + BM - 1) / BM, nb_n = (N + BN - 1) / BN;
+  const int64_t L = gdn::xcd_remap(blockIdx.x, static_cast<int64_t>(mb_n) * nb_n);
+  if (L < 0) return;
+  const int64_t per_group = static_cast<int64_t>(kGroupM8) * nb_n;
+  const int64_t grp = L / per_group, in_grp = L % per_group;
+  const int gm = static_cast<int>(min<int64_t>(kGroupM8, mb_n - grp * kGroupM8));
+  const int m0 = BM * static_cast<int>(grp * kGroupM8 + in_grp % gm), n0 = BN * static_cast<int>(in_grp / gm);
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wm = wave >> 1, wn = wave & 1;
+  const int lr = lane & 15, lg = lane >> 4;
+  const __amdgpu_buffer_rsrc_t ra = rsrc_of(A), rb = rsrc_of(B), rs = rsrc_of(wave == 0 ? sc.a : sc.b);
+  int goff[kAPer + kBPer];
+#pragma unroll
+  for (int i = 0; i < kAPer + kBPer; ++i) {
+    const int r = 8 * wave + 32 * (i < kAPer ? i : i - kAPer) + (lane >> 3);
+    goff[i] = i < kAPer ? static_cast<int>(min(m0 + r, M - 1) * lda + 16 * ((lane & 7) ^ ((r >> 1) & 7)))
+                        : static_cast<int>(min(n0 + r, N - 1) * ldb +
+                                           16 * ((lane & 7) ^ (((r >> 1) & 1) | (((r >> 3) & 3) << 1))));
+  }
+  const int vs = wave == 0 ? static_cast<int>(min(m0 + lane, M - 1) * sc.a_row * 4)
+                           : static_cast<int>(n0 / 128 * sc.b_row * 4);
+  const int s_step = wave == 0 ? static_cast<int>(sc.a_grp) * 4 : 4;
+  const int nk = K / 128;
+  auto issue = [&](uint8_t* st, int step) {
+    const int s = min(step, nk - 1);
+#pragma unroll
+    for (int i = 0; i < kAPer + kBPer; ++i)
+      dma16(i < kAPer ? ra : rb, st + (i < kAPer ? 0 : BM * 128) + (wave + 4 * (i < kAPer ? i : i - kAPer)) * 1024,
+            goff[i], 128 * s);
+    dma4(rs, st + (BM + BN) * 128 + 256 * wave, vs, s_step * s);
+  };
+  gdn::f32x4_t acc[2][NJ][2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int j = 0; j < NJ; ++j)
+#pragma unroll
+      for (int t = 0; t < 2; ++t) acc[i][j][t] = gdn::f32x4_t{0.f, 0.f, 0.f, 0.f};
+  // step s from `cur`, the loads of step s + NS - 1 into `nxt` (the stage of step
+  // s - 1, which every wave has finished reading at the barrier)
+  auto one = [&](const uint8_t* cur, uint8_t* nxt, int step) {
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_waitcnt(kWait);
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_sched_barrier(0);
+    issue(nxt, step + NS - 1);
+    __builtin_amdgcn_sched_barrier(0);
+    const uint8_t* b = cur + BM * 128;
+    const float* p = reinterpret_cast<const float*>(cur + (BM + BN) * 128);
+    Frag8 fa[2], fb[NJ][2];
+    float f[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int r = 32 * wm + 16 * i + lr;
+      fa[i].lo = *reinterpret_cast<const i32x4_t*>(cur + sw_off(r, lg));
+      fa[i].hi = *reinterpret_cast<const i32x4_t*>(cur + sw_off(r, 4 + lg));
+      f[i] = p[r];
+    }
+#pragma unroll
+    for (int j = 0; j < NJ; ++j)
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        const int r = 32 * (NJ * wn + j) + 8 * (lr >> 2) + 4 * t + (lr & 3);
+        fb[j][t].lo = *reinterpret_cast<const i32x4_t*>(b + swb_off(r, lg));
+        fb[j][t].hi = *reinterpret_cast<const i32x4_t*>(b + swb_off(r, 4 + lg));
+      }
+    const float sb = p[64];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const float s = f[i] * sb;
+#pragma unroll
+      for (int j = 0; j < NJ; ++j)
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          const gdn::f32x4_t r = mfma_fp8(fb[j][t], fa[i]);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[i][j][t][e] = fmaf(r[e], s, acc[i][j][t][e]);
+        }
+    }
+  };
+  issue(st0, 0);
+  issue(st1, 1);
+  if constexpr (NS == 4) issue(st2, 2);
+  // (no exit inside a trip: the compiler's load counting would merge its states at the
+  // loop head and wait there for loads that are meant to stay in flight)
+  int s = 0;
+  if constexpr (NS == 4) {
+    for (; s + 3 < nk; s += 4) {
+      one(st0, st3, s);
+      one(st1, st0, s + 1);
+      one(st2, st1, s + 2);
+      one(st3, st2, s + 3);
+    }
+    if (s < nk) one(st0, st3, s);
+    if (s + 1 < nk) one(st1, st0, s + 1);
+    if (s + 2 < nk) one(st2, st1, s + 2);
+  } else {
+    for (; s + 2 < nk; s += 3) {
+      one(st0, st2, s);
+      one(st1, st0, s + 1);
+      one(st2, st1, s + 2);
+    }
+    if (s < nk) one(st0, st2, s);
+    if (s + 1 < nk) one(st1, st0, s + 1);
+  }
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int j = 0; j < NJ; ++j)
+      gemm_store16(acc[i][j][0], acc[i][j][1], out, M, N, m0 + 32 * wm + 16 * i, n0 + 32 * (NJ * wn + j), lane,
+                   GemmGates{}, nullptr);
+  __builtin_amdgcn_s_waitcnt(0);  // the repeated loads past the last step
+}
+
+// The kernels (fp8_plan says which is taken); the last two take bf16 rows.  Those and the
+// two that take the same calls' e4m3 rows deal K to as many waves, so that a call from
+// bf16 rows has the bits of gdn_quantize_fp8 and a call from e4m3 ones.  (Four waves of
+// three stages for kRing16x32: 1 x 2048 3.6 us against 3.8, 64 x 2048 x 4096 4.8 / 5.1.)
+enum Fp8Kernel { kPP, kDeep64, kDeep128, kRing16x32, kRing16x64, kRing32x32, kRing64x32, kRingQ16x32, kRingQ16x64 };
+
+// Times: one launch replayed from a graph, operands in the caches, K = 2048 unless
+// said.
+Fp8Kernel fp8_plan(int M, int N, int K, bool quant) {
+  auto blocks = [&](int bm, int bn) { return static_cast<int64_t>((M + bm - 1) / bm) * ((N + bn - 1) / bn); };
+  // Ring tiles with at most one workgroup per CU, the fewest rows first: 1 x 2048 3.8 us
+  // (64 x 64 tiles 6.5, 128 x 128 blocks 11.6), 64 x 2048 4.0 (6.9), 128 x 2048 4.7
+  // (7.0), 256 x 2048 6.4 (7.1), 64 x 8192 6.2 (7.1); 37 x 2048 x 4096 4.6 (10.8).  With
+  // more workgroups the 64 x 64 tiles move fewer bytes: 64 x 12288 7.2 against 10.8-12.
+  // One row block of wide outputs takes 64 columns: 1 x 12288 4.8 (32 columns 5.2, 64 x
+  // 64 tiles 6.9), 1 x 16384 5.2 (5.6, 7.3); past one workgroup per CU 1 x 32768 14.3,
+  // 64 x 64 tiles 12.4.
+  if (quant && K <= 4096) {
+    // A bf16 A's own launch takes 2.0 to 2.4 us; in the ring it takes 0.5 per K-step of a
+    // wave (2048 columns: two of them for each of 8 waves): 1 x 2048 5.0 against 3.8 +
+    // 2.0, 64 x 2048 5.4 against 4.0 + 2.4, 37 x 2048 x 4096 6.8 against 4.6 + 2.3, 1 x
+    // 12288 6.3 against 4.8 + 2.1.  Longer rows take more, and so do row blocks past one
+    // workgroup per CU (64 x 8192 17.5 against 6.2 + 2.4).
+    if (blocks(16, 32) <= kCUs8) return kRingQ16x32;
+    if (M <= 16 && blocks(16, 64) <= kCUs8) return kRingQ16x64;
+  }
+  if (blocks(16, 32) <= kCUs8) return kRing16x32;
+  if (M <= 16 && blocks(16, 64) <= kCUs8) return kRing16x64;
+  if (blocks(32, 32) <= kCUs8) return kRing32x32;
+  if (blocks(64, 32) <= kCUs8) return kRing64x32;
+  // Up to two 64 x 64 tiles per CU: 200 x 8192 8.5 us (64 x 128 tiles 10.4, 128 x 128
+  // blocks 13.1), 1024 x 2048 9.0 (10.3, 13.2), 128 x 12288 8.6 (10.3, 13.3); with three
+  // 256 x 12288 14.5 (12.4, 14.3).
+  if (blocks(64, 64) <= 2 * kCUs8) return kDeep64;
+  // Up to nearly four 64 x 128 tiles per CU: 400 x 12288 22.2 (pp 25.9), 700 x 8192 22.4
+  // (25.8), 900 x 8192 26.7 (28.7), 1500 x 2048 13.1 (13.9); then the large tiles: 1024 x
+  // 8192 28.2 against 28.2, 700 x 12288 34.1 against 32.7, 1024 x 12288 40.0 against 34.4.
+  if (blocks(64, 128) <= 15 * kCUs8 / 4) return kDeep128;
+  return kPP;
+}
+
+bool fp8_quantizes(Fp8Kernel k) { return k >= kRingQ16x32; }
+
+int fp8_launch(Fp8Kernel kernel, const void* A, int64_t lda, const uint8_t* B, int64_t ldb, const Fp8Scales& sc,
+               const GemmOut& out, int M, int N, int K, hipStream_t st) {
+  auto blocks = [&](int bm, int bn) { return static_cast<int64_t>((M + bm - 1) / bm) * ((N + bn - 1) / bn); };
   auto grid = [](int64_t wgs) {
     return dim3(static_cast<unsigned>(gdn::kNumXcd * ((wgs + gdn::kNumXcd - 1) / gdn::kNumXcd)));
   };
-  if (tiles > kCUs8) {
-    const int64_t rem = t256 % kCUs8;
-    const int64_t whole = rem <= kCUs8 / 2 ? t256 - rem : t256;
-    const int64_t wgs = std::min<int64_t>(kCUs8, whole ? std::max(whole, 4 * (t256 - whole)) : t128);
-    gemm_fp8_pp_kernel<<<grid(wgs), dim3(kPPThreads), 0, st>>>(A, lda, B, ldb, sc, out, M, N, K,
-                                                               static_cast<int>(whole));
-    return gdn_launch_status();
+  const uint8_t* A8 = static_cast<const uint8_t*>(A);
+  switch (kernel) {
+    case kPP: {
+      // whole 256 x 256 tiles for full rounds of the CUs, the rest (up to half a round)
+      // as quarters; less than half a round: all of it in 128 x 128 blocks
+      const int64_t t256 = blocks(256, 256), rem = t256 % kCUs8;
+      const int64_t whole = rem <= kCUs8 / 2 ? t256 - rem : t256;
+      const int64_t wgs = std::min<int64_t>(kCUs8, whole ? std::max(whole, 4 * (t256 - whole)) : blocks(128, 128));
+      gemm_fp8_pp_kernel<<<grid(wgs), dim3(kPPThreads), 0, st>>>(A8, lda, B, ldb, sc, out, M, N, K,
+                                                                 static_cast<int>(whole));
+      break;
+    }
+    case kDeep64:
+      gemm_fp8_deep_kernel<64, 4><<<grid(blocks(64, 64)), dim3(kFp8Threads), 0, st>>>(A8, lda, B, ldb, sc, out, M, N,
+                                                                                     K);
+      break;
+    case kDeep128:
+      gemm_fp8_deep_kernel<128, 3><<<grid(blocks(64, 128)), dim3(kFp8Threads), 0, st>>>(A8, lda, B, ldb, sc, out, M,
+                                                                                       N, K);
+      break;
+#define GDN_RING(name, BM, BN, NW, NS, Q)                                                                          \
+  case name:                                                                                                       \
+    gemm_fp8_ring_kernel<BM, BN, NW, NS, Q><<<grid(blocks(BM, BN)), dim3(64 * NW), 0, st>>>(A, lda, B, ldb, sc, out, \
+                                                                                           M, N, K);               \
+    break
+      GDN_RING(kRing16x32, 16, 32, 8, 2, false);
+      GDN_RING(kRing16x64, 16, 64, 4, 3, false);
+      GDN_RING(kRing32x32, 32, 32, 4, 3, false);
+      GDN_RING(kRing64x32, 64, 32, 4, 3, false);
+      GDN_RING(kRingQ16x32, 16, 32, 8, 2, true);
+      GDN_RING(kRingQ16x64, 16, 64, 4, 2, true);
+#undef GDN_RING
   }
-  gemm_fp8_kernel<<<grid(tiles), dim3(kFp8Threads), 0, st>>>(A, lda, B, ldb, sc, out, M, N, K);
   return gdn_launch_status();
 }
 
 }  // namespace
 
-extern "C" int gdn_gemm_fp8(const uint8_t* A, int64_t lda, const float* sa, int64_t sa_row, int64_t sa_grp,
+// x's rows in e4m3 and their scales, of a call from bf16 rows that no kernel above quantizes itself.
+extern "C" int64_t gdn_gemm_fp8_workspace_size(int M, int N, int K, int a_is_bf16) {
+  if (M < 0 || N < 0 || K < 0 || K % gdn::kFp8Group) return -1;
+  if (!a_is_bf16 || M == 0 || N == 0 || K == 0 || fp8_quantizes(fp8_plan(M, N, K, true))) return 0;
+  return static_cast<int64_t>(M) * K + static_cast<int64_t>(M) * (K / gdn::kFp8Group) * 4;
+}
+
+extern "C" int gdn_gemm_fp8(const void* A, int a_is_bf16, int64_t lda, const float* sa, int64_t sa_row, int64_t sa_grp,
                             const uint8_t* B, int64_t ldb, const float* sb, int64_t sb_row, int M, int N, int K,
-                            int n_parts, uint16_t* const* C, const int64_t* ldc, const int* col_end, void* stream) {
+                            int n_parts, uint16_t* const* C, const int64_t* ldc, const int* col_end, void* workspace,
+                            int64_t workspace_bytes, void* stream) {
   if (M < 0 || N < 0 || K < 0 || n_parts < 1 || n_parts > kMaxParts || !C || !ldc || !col_end)
     return GDN_ERR_INVALID_ARG;
   if (M == 0 || N == 0) return GDN_OK;
-  if (!A || !B || !sa || !sb) return GDN_ERR_INVALID_ARG;
+  if (!A || !B || !sb || (!a_is_bf16 && !sa)) return GDN_ERR_INVALID_ARG;
   // K in whole groups; 16-byte row pieces of A and B; 32-bit buffer offsets
   const int64_t kLimit = 1LL << 31;
   const int64_t groups = K / gdn::kFp8Group;
-  if (K == 0 || K % gdn::kFp8Group || lda % 16 || ldb % 16 || lda < K || ldb < K ||
-      reinterpret_cast<uintptr_t>(A) % 16 || reinterpret_cast<uintptr_t>(B) % 16 || M * lda >= kLimit ||
-      N * ldb >= kLimit || sa_row < 0 || sa_grp < 0 || sb_row < groups ||
-      4 * ((M - 1) * sa_row + (groups - 1) * sa_grp) >= kLimit ||
+  if (K == 0 || K % gdn::kFp8Group || lda % (a_is_bf16 ? 8 : 16) || ldb % 16 || lda < K || ldb < K ||
+      reinterpret_cast<uintptr_t>(A) % 16 || reinterpret_cast<uintptr_t>(B) % 16 ||
+      M * lda * (a_is_bf16 ? 2 : 1) >= kLimit || N * ldb >= kLimit || sb_row < groups ||
       4 * ((N + 127) / 128 * sb_row) >= kLimit)
+    return GDN_ERR_INVALID_ARG;
+  if (!a_is_bf16 && (sa_row < 0 || sa_grp < 0 || 4 * ((M - 1) * sa_row + (groups - 1) * sa_grp) >= kLimit))
     return GDN_ERR_INVALID_ARG;
   GemmOut out{};
   if (!parts_of(out, n_parts, C, ldc, col_end, N)) return GDN_ERR_INVALID_ARG;
-  return fp8_launch(A, lda, B, ldb, Fp8Scales{sa, sa_row, sa_grp, sb, sb_row}, out, M, N, K,
+  const Fp8Kernel kernel = fp8_plan(M, N, K, a_is_bf16 != 0);
+  if (a_is_bf16 && !fp8_quantizes(kernel)) {
+    if (workspace_bytes < gdn_gemm_fp8_workspace_size(M, N, K, 1) || !workspace ||
+        reinterpret_cast<uintptr_t>(workspace) % 16)
+      return GDN_ERR_INVALID_ARG;
+    uint8_t* x8 = static_cast<uint8_t*>(workspace);
+    float* scale = reinterpret_cast<float*>(x8 + static_cast<int64_t>(M) * K);
+    const int st = gdn_quantize_fp8(A, 0, lda, x8, K, scale, 1, M, M, K, 1, stream);
+    if (st != GDN_OK) return st;
+    A = x8;
+    lda = K;
+    sa = scale;
+    sa_row = 1;
+    sa_grp = M;
+  }
+  return fp8_launch(kernel, A, lda, B, ldb, Fp8Scales{sa, sa_row, sa_grp, sb, sb_row}, out, M, N, K,
                     static_cast<hipStream_t>(stream));
 }

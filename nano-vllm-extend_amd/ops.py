@@ -1187,10 +1187,11 @@ def _linear_fp8(x, weight, weight_scale, x_scale, outs, widths):
     if w.stride(1) != 1 or w.stride(0) % 16 or w.stride(0) < K or w.data_ptr() % 16:
         w = w.contiguous() if not w.is_contiguous() else w.clone()
     ws = weight_scale if weight_scale.stride(1) == 1 or G == 1 else weight_scale.contiguous()
-    if x_scale is None:
-        x, x_scale = quantize_fp8(x)
-    x2 = _rows_of(x, 16)
+    bf16 = x_scale is None
+    x2 = _rows_of(x, 8 if bf16 else 16)
     M = x2.shape[0]
+    ws_bytes = _lib.load().gdn_gemm_fp8_workspace_size(M, N, K, 1) if bf16 else 0
+    work = torch.empty(ws_bytes, dtype=torch.uint8, device=x.device) if ws_bytes > 0 else None
     n, ends, e = len(widths), [], 0
     for wd in widths:
         e += wd
@@ -1198,9 +1199,10 @@ def _linear_fp8(x, weight, weight_scale, x_scale, outs, widths):
     c_arr = (ctypes.c_void_p * n)(*[p.data_ptr() for p in outs])
     ld_arr = (ctypes.c_int64 * n)(*[p.stride(0) if M > 1 else max(p.stride(0), p.shape[1]) for p in outs])
     end_arr = (ctypes.c_int * n)(*ends)
-    _call_on(dev, "gdn_gemm_fp8", _lib.ptr(x2), x2.stride(0), _lib.ptr(x_scale), x_scale.stride(0),
-             x_scale.stride(1), _lib.ptr(w), w.stride(0), _lib.ptr(ws), ws.stride(0) if ws.shape[0] > 1 else G, M, N, K,
-             n, c_arr, ld_arr, end_arr, _stream(dev))
+    _call_on(dev, "gdn_gemm_fp8", _lib.ptr(x2), int(bf16), x2.stride(0), _lib.ptr(x_scale),
+             0 if bf16 else x_scale.stride(0), 0 if bf16 else x_scale.stride(1), _lib.ptr(w), w.stride(0),
+             _lib.ptr(ws), ws.stride(0) if ws.shape[0] > 1 else G, M, N, K, n, c_arr, ld_arr, end_arr, _lib.ptr(work),
+             ws_bytes, _stream(dev))
 
 
 def _check_fp8(x, weight, weight_scale, x_scale):

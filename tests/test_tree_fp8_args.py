@@ -144,14 +144,22 @@ def test_c_entry_points_reject_before_launch(pkg):
         assert q(**bad) == inv, bad
     # product
     C1, ld1, end1 = (ctypes.c_void_p * 1)(1 << 20), (ctypes.c_int64 * 1)(96), (ctypes.c_int * 1)(96)
-    f = lambda A=P, lda=256, sa=P, ar=1, B=P, ldb=256, sb=P, br=2, M=4, N=96, K=256, n=1, C=C1, ld=ld1, e=end1: (  # noqa: E731,E501
-        lib.gdn_gemm_fp8(A, lda, sa, ar, 4, B, ldb, sb, br, M, N, K, n, C, ld, e, None))
+    f = lambda A=P, lda=256, sa=P, ar=1, B=P, ldb=256, sb=P, br=2, M=4, N=96, K=256, n=1, C=C1, ld=ld1, e=end1, q=0, ws=None, wb=0: (  # noqa: E731,E501
+        lib.gdn_gemm_fp8(A, q, lda, sa, ar, 4, B, ldb, sb, br, M, N, K, n, C, ld, e, ws, wb, None))
     assert f(M=0) == ok and f(N=0) == ok
     for bad in (dict(A=None), dict(A=odd), dict(lda=248), dict(lda=128), dict(sa=None), dict(B=None), dict(B=odd),
                 dict(ldb=250), dict(sb=None), dict(br=1), dict(K=0), dict(K=192), dict(n=0), dict(n=5), dict(C=None),
                 dict(ld=(ctypes.c_int64 * 1)(90)), dict(e=(ctypes.c_int * 1)(90)), dict(M=1 << 24), dict(ar=-1),
                 dict(ar=1 << 28)):
         assert f(**bad) == inv, bad
+    # from bf16 rows: the workspace that the size says, of rows that no kernel quantizes itself
+    size = lib.gdn_gemm_fp8_workspace_size
+    assert size(5000, 96, 256, 0) == 0 and size(0, 96, 256, 1) == 0 and size(-1, 96, 256, 1) == -1
+    assert size(4, 96, 200, 1) == -1
+    need = size(5000, 96, 256, 1)
+    assert need == 5000 * (256 + 8)
+    for bad in (dict(ws=None, wb=need), dict(ws=odd, wb=need), dict(ws=P, wb=need - 1), dict(lda=252)):
+        assert f(**{**dict(q=1, M=5000, ws=P, wb=need), **bad}) == inv, bad
     # norm
     n = lambda x=P, sx=256, w=P, y=P, s=P, N=4, H=2, D=128: lib.gdn_rmsnorm_gated_fp8(  # noqa: E731
         x, sx, P, 256, w, y, s, 1, 4, N, H, D, 1e-6, None)
