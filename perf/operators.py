@@ -198,8 +198,14 @@ def run(state):
     return (_own if own else _plain)[state["op"]](state)
 
 
+_package = None
+
+
 def _ops():
-    return importlib.import_module("nano-vllm-extend_amd").ops
+    global _package
+    if _package is None:    # (a program imports it once)
+        _package = importlib.import_module("nano-vllm-extend_amd")
+    return _package.ops
 
 
 def _own_linear(s):
