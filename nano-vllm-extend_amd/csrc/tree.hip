@@ -15,17 +15,19 @@
 // form (gdn_recurrent) writes one D x D state per token, and a commit forms one state
 // from the path's k, g and u.  The weights are products of factors in [0, 1], never
 // differences of sums: no cancellation, and a decay of 0 stays 0.
+#include <algorithm>
+
 #include "gdn_common.h"
 
 namespace {
 
 constexpr int kMaxNodes = 64;
 
-// A tree's links, by the 64 lanes of one wave: link[t] the parent (-1: the state),
-// or kUnused.  (Each walk goes to smaller nodes, so it ends.)
+// A tree's links, by the 64 lanes of one wave, lane t with node t's parent: link[t] the
+// parent (-1: the state), or kUnused.  (Each walk goes to smaller nodes, so it ends.)
 constexpr int kUnused = -2;
-__device__ __forceinline__ void tree_links(const int32_t* __restrict__ parents, int T, int lane, int* raw, int* link) {
-  if (lane < T) raw[lane] = parents[lane];
+__device__ __forceinline__ void tree_links(int parent, int T, int lane, int* raw, int* link) {
+  if (lane < T) raw[lane] = parent;
   __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront", "local");
   __builtin_amdgcn_wave_barrier();
   __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront", "local");
@@ -94,9 +96,10 @@ __global__ __launch_bounds__(256) void conv_tree_kernel(const uint16_t* __restri
   const int b = blockIdx.y;
   const int c = blockIdx.x * 256 + threadIdx.x;
   if (threadIdx.x < 64) {
-    tree_links(parents + b * p_b, T, threadIdx.x, raw[0], link[0]);
+    tree_links(parents[b * p_b + min<int>(threadIdx.x, T - 1)], T, threadIdx.x, raw[0], link[0]);
   } else if (threadIdx.x < 128 && pd.accepted) {
-    tree_links(pd.parents + b * pd.p_b, pd.T, threadIdx.x - 64, raw[1], link[1]);
+    const int lane = threadIdx.x - 64;
+    tree_links(pd.parents[b * pd.p_b + min(lane, pd.T - 1)], pd.T, lane, raw[1], link[1]);
   }
   __syncthreads();
   if (c >= C) return;
@@ -134,189 +137,547 @@ __global__ __launch_bounds__(256) void conv_tree_kernel(const uint16_t* __restri
 }
 
 // ---- rule ----
-// The path to an accepted node, newest first: its nodes and the weight w(a, s) of each
-// one's correction; returns the weight of the state, W_a.  One thread.
-__device__ __forceinline__ float path_of(int a, const int* link, const float* __restrict__ g, int64_t g_t, int* node,
-                                         float* weight, int& n) {
-  float w = 1.0f;
-  n = 0;
-  for (int s = a; s >= 0; s = link[s]) {
-    node[n] = s;
-    weight[n++] = w;
-    w *= expf(g[s * g_t]);
-  }
-  return w;
+// One workgroup of D / 32 waves per (sequence, value head): wave w holds columns 32 w ..
+// of the state, lane (lr, lg) = (lane % 16, lane / 16) columns 2 lr and 2 lr + 1 of rows
+// 32 kk + 8 lg + e, in registers from the one read of it to the one write.  That is the
+// second operand's layout of a 16 x 16 x 32 product over the rows, for the even columns
+// and for the odd ones, with the nodes' raw bf16 rows as the first: S^T k and S^T q are
+// products of 16 nodes, 32 rows and 16 columns.  S goes in as three bf16 terms that add
+// up to it exactly (8 bits of the significand each), k and q are not normalised before
+// (their norms scale the results), so the products are those of fp32 operands.
+//
+// What bounds it: the state's way in (and out, where a path is pending).  The tree's
+// weights, the nodes' norms and dot products (on the matrix cores as well) and the
+// pending path's rows are worked on while the state is on its way.
+typedef float f32x2_t __attribute__((ext_vector_type(2)));
+constexpr float kEps = 1e-6f;
+
+__device__ __forceinline__ void wave_lds_order() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront", "local");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront", "local");
 }
 
-// 1 / |row| of a bf16 row of D values for each lane of a wave (lane holds D / 64 values)
+// The state tile of a workgroup: S[kk][e] = columns 2 lr, 2 lr + 1 of row 32 kk + 8 lg + e.
 template <int D>
-__device__ __forceinline__ void unit_row(const uint16_t* __restrict__ p, int lane, float* out) {
-  constexpr int E = D / 64;
-  float v[E], ss = 0.0f;
-#pragma unroll
-  for (int e = 0; e < E; ++e) {
-    v[e] = gdn::bf2f(p[lane * E + e]);
-    ss += v[e] * v[e];
-  }
-  const float r = rsqrtf(gdn::wave_sum(ss) + 1e-6f);
-#pragma unroll
-  for (int e = 0; e < E; ++e) out[lane * E + e] = v[e] * r;
-}
+struct Tile {
+  f32x2_t s[D / 32][8];
 
-// The column of S that a thread holds, after the pending path of row b (value head h).
-template <int D>
-__device__ __forceinline__ bool advance_column(float (&S)[D], const RulePending& pd, int b, int h, int kh, int Hv,
-                                               const int* link, int* node, float* weight, float* total, int* count,
-                                               float* key) {
-  const int a = accepted_node(pd.accepted[b], pd.T, link);
-  if (a < 0) return false;  // (the whole workgroup)
-  if (threadIdx.x == 0) {
-    int n;
-    *total = path_of(a, link, pd.g + (static_cast<int64_t>(b) * pd.T) * Hv + h, Hv, node, weight, n);
-    *count = n;
+  __device__ __forceinline__ void load(const float* p) {  // p: the lane's first row and column
+#pragma unroll
+    for (int kk = 0; kk < D / 32; ++kk)
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        s[kk][e] = __builtin_nontemporal_load(reinterpret_cast<const f32x2_t*>(p + (32 * kk + e) * D));
   }
-  __syncthreads();
-  const float w = *total;
+  __device__ __forceinline__ void store(float* p) const {
 #pragma unroll
-  for (int i = 0; i < D; ++i) S[i] *= w;
-  for (int p = 0; p < *count; ++p) {
-    const int s = node[p];
-    __syncthreads();
-    if (threadIdx.x < 64) unit_row<D>(pd.k + b * pd.k_b + s * pd.k_t + kh * D, threadIdx.x, key);
-    __syncthreads();
-    const float c = weight[p] * pd.u[((static_cast<int64_t>(b) * pd.T + s) * Hv + h) * D + threadIdx.x];
+    for (int kk = 0; kk < D / 32; ++kk)
 #pragma unroll
-    for (int i = 0; i < D; ++i) S[i] = fmaf(c, key[i], S[i]);
+      for (int e = 0; e < 8; ++e)
+        __builtin_nontemporal_store(s[kk][e], reinterpret_cast<f32x2_t*>(p + (32 * kk + e) * D));
   }
-  return true;
-}
-
-// One workgroup of D threads per (sequence, value head); a thread holds a column of S.
-template <int D>
-__global__ __launch_bounds__(D) void rule_tree_kernel(const uint16_t* __restrict__ q, int64_t q_b, int64_t q_t,
-                                                      const uint16_t* __restrict__ k, int64_t k_b, int64_t k_t,
-                                                      const uint16_t* __restrict__ v, int64_t v_b, int64_t v_t,
-                                                      const float* __restrict__ g, const uint16_t* __restrict__ beta,
-                                                      float* __restrict__ pool, int64_t s_slot, int64_t n_slots,
-                                                      const int64_t* __restrict__ ids,
-                                                      const int32_t* __restrict__ parents, int64_t p_b,
-                                                      RulePending pd, uint16_t* __restrict__ o, float* __restrict__ u,
-                                                      int T, int Hk, int Hv, float scale) {
-  __shared__ int raw[2][kMaxNodes], link[2][kMaxNodes], node[kMaxNodes];
-  __shared__ float weight[kMaxNodes], dec[kMaxNodes], bt[kMaxNodes];
-  __shared__ float key[D], qry[D], su[kMaxNodes][D], sk[kMaxNodes][D];
-  __shared__ float total, kk[kMaxNodes], qk[kMaxNodes];
-  __shared__ int count;
-  const int b = blockIdx.x / Hv, h = blockIdx.x % Hv, kh = h / (Hv / Hk);
-  const int j = threadIdx.x, wave = threadIdx.x / 64, lane = threadIdx.x % 64;
-  const int64_t slot = ids[b];
-  const bool row_ok = slot >= 0 && slot < n_slots;
-  if (j < 64) {
-    tree_links(parents + b * p_b, T, lane, raw[0], link[0]);
-    if (pd.accepted) tree_links(pd.parents + b * pd.p_b, pd.T, lane, raw[1], link[1]);
-    if (lane < T) {
-      const int64_t at = (static_cast<int64_t>(b) * T + lane) * Hv + h;
-      dec[lane] = expf(g[at]);
-      bt[lane] = gdn::bf2f(beta[at]);
-    }
-  }
-  for (int t = wave; t < T; t += D / 64) unit_row<D>(k + b * k_b + t * k_t + kh * D, lane, sk[t]);
-  __syncthreads();
-  float* S0 = pool + slot * s_slot + static_cast<int64_t>(h) * D * D + j;
-  float S[D];
+  // S <- total S + sum over the path of (w k)[row] u[column], both from LDS rows
+  template <int TM>
+  __device__ __forceinline__ void advance(float total, int count, const float (&wk)[TM][D], const float (&u)[TM][D],
+                                          int wave, int lr, int lg) {
 #pragma unroll
-  for (int i = 0; i < D; ++i) S[i] = row_ok ? S0[i * D] : 0.0f;
-  if (pd.accepted && row_ok &&
-      advance_column<D>(S, pd, b, h, kh, Hv, link[1], node, weight, &total, &count, key)) {
+    for (int kk = 0; kk < D / 32; ++kk)
 #pragma unroll
-    for (int i = 0; i < D; ++i) S0[i * D] = S[i];
-  }
-  for (int t = 0; t < T; ++t) {
-    const int64_t at = ((static_cast<int64_t>(b) * T + t) * Hv + h) * D + j;
-    if (!row_ok || link[0][t] == kUnused) {  // (the whole workgroup)
-      o[at] = 0;
-      u[at] = 0.0f;
-      continue;
-    }
-    __syncthreads();
-    if (wave == 0) unit_row<D>(q + b * q_b + t * q_t + kh * D, lane, qry);
-    __syncthreads();
-    // the products with the path's keys: a wave per node
-    if (j < 64) {
-      for (int s = t; s >= 0; s = link[0][s]) {
-        float a = 0.0f, c = 0.0f;
+      for (int e = 0; e < 8; ++e) s[kk][e] *= total;
+    for (int p = 0; p < count; ++p) {
+      const f32x2_t c = *reinterpret_cast<const f32x2_t*>(&u[p][32 * wave + 2 * lr]);
 #pragma unroll
-        for (int e = 0; e < D / 64; ++e) {
-          a += sk[s][lane + 64 * e] * sk[t][lane + 64 * e];
-          c += sk[s][lane + 64 * e] * qry[lane + 64 * e];
-        }
-        a = gdn::wave_sum(a);
-        c = gdn::wave_sum(c);
-        if (lane == 0) {
-          kk[s] = a;
-          qk[s] = c;
+      for (int kk = 0; kk < D / 32; ++kk) {
+        const float4 a = *reinterpret_cast<const float4*>(&wk[p][32 * kk + 8 * lg]);
+        const float4 b = *reinterpret_cast<const float4*>(&wk[p][32 * kk + 8 * lg + 4]);
+        const float r[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          s[kk][e].x = fmaf(r[e], c.x, s[kk][e].x);
+          s[kk][e].y = fmaf(r[e], c.y, s[kk][e].y);
         }
       }
     }
-    __syncthreads();
-    float ks = 0.0f, qs = 0.0f;
-#pragma unroll
-    for (int i = 0; i < D; ++i) {
-      ks = fmaf(sk[t][i], S[i], ks);
-      qs = fmaf(qry[i], S[i], qs);
+  }
+};
+
+// A pending path in LDS: its nodes from the accepted one up to the root, the weight of
+// each one's correction and that of the state.
+struct Path {
+  int raw[kMaxNodes], link[kMaxNodes];
+  int node[kMaxNodes];
+  float weight[kMaxNodes];
+  float dec[kMaxNodes];
+  float total;
+  int count;  // 0: nothing was accepted
+};
+
+// By one wave: the links and decays of the pending tree, then the walk.  What it reads
+// comes as PathIn, so that it can be asked for ahead of the state.
+struct PathIn {
+  int64_t want;
+  float g;
+  int parent;
+
+  __device__ __forceinline__ void load(const RulePending& pd, int b, int h, int Hv, int lane) {
+    const int t = min(lane, pd.T - 1);
+    want = pd.accepted[b];
+    g = pd.g[(static_cast<int64_t>(b) * pd.T + t) * Hv + h];
+    parent = pd.parents[b * pd.p_b + t];
+  }
+};
+__device__ __forceinline__ void find_path(const PathIn& in, int T, int lane, Path& path) {
+  path.dec[lane] = expf(in.g);
+  tree_links(in.parent, T, lane, path.raw, path.link);
+  wave_lds_order();
+  if (lane == 0) {
+    float w = 1.0f;
+    int n = 0;
+    for (int s = accepted_node(in.want, T, path.link); s >= 0; s = path.link[s]) {
+      path.node[n] = s;
+      path.weight[n++] = w;
+      w *= path.dec[s];
     }
-    float w = dec[t], au = 0.0f, ao = 0.0f;
-    for (int s = link[0][t]; s >= 0; s = link[0][s]) {
-      au = fmaf(w * kk[s], su[s][j], au);
-      ao = fmaf(w * qk[s], su[s][j], ao);
-      w *= dec[s];
-    }
-    const float ut = bt[t] * (gdn::bf2f(v[b * v_b + t * v_t + h * D + j]) - fmaf(w, ks, au));
-    su[t][j] = ut;
-    u[at] = ut;
-    o[at] = gdn::f2bf(scale * (fmaf(w, qs, ao) + qk[t] * ut));
+    path.total = w;
+    path.count = n;
   }
 }
 
-// Grid: B * Hv workgroups for the states, then B * ceil(C / D) for the taps.
-template <int D>
-__global__ __launch_bounds__(D) void commit_tree_kernel(float* __restrict__ pool, int64_t s_slot,
-                                                        uint16_t* __restrict__ cpool, int64_t sp_slot, int64_t sp_ch,
-                                                        int64_t n_slots, const int64_t* __restrict__ ids,
-                                                        RulePending pd, ConvPending cd, int B, int Hk, int Hv, int C) {
-  __shared__ int raw[kMaxNodes], link[kMaxNodes], node[kMaxNodes];
-  __shared__ float weight[kMaxNodes], key[D], total;
-  __shared__ int count;
-  const int parts = (C + D - 1) / D;
-  const bool conv = blockIdx.x >= static_cast<unsigned>(B * Hv);
-  const int at = conv ? blockIdx.x - B * Hv : blockIdx.x;
-  const int b = conv ? at / parts : at / Hv;
+// The path's rows into LDS, a wave per node: its normalised key times its weight, and its
+// correction.
+template <int D, int TM>
+__device__ __forceinline__ void stage_path(const RulePending& pd, const Path& path, int b, int h, int kh, int Hv,
+                                           int wave, int waves, int lane, float (&wk)[TM][D], float (&u)[TM][D]) {
+  constexpr int E = D / 64;
+  for (int p = wave; p < path.count; p += waves) {
+    const int s = path.node[p];
+    const uint16_t* kr = pd.k + b * pd.k_b + s * pd.k_t + kh * D + lane * E;
+    const float* ur = pd.u + ((static_cast<int64_t>(b) * pd.T + s) * Hv + h) * D + lane * E;
+    float v[E], ss = 0.0f;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      u[p][lane * E + e] = ur[e];
+      v[e] = gdn::bf2f(kr[e]);
+      ss += v[e] * v[e];
+    }
+    const float r = path.weight[p] * rsqrtf(gdn::wave_sum(ss) + kEps);
+#pragma unroll
+    for (int e = 0; e < E; ++e) wk[p][lane * E + e] = v[e] * r;
+  }
+}
+
+// Three bf16 terms of two fp32 values that add up to them exactly: the leading 8 bits of
+// the significand, the next 8, the last 8 (cut, not rounded), in the low and the high half.
+__device__ __forceinline__ void split3(float a, float b, uint32_t& hi, uint32_t& mid, uint32_t& lo) {
+  const uint32_t ua = __float_as_uint(a), ub = __float_as_uint(b);
+  hi = __builtin_amdgcn_perm(ub, ua, 0x07060302u);
+  const float ra = a - __uint_as_float(ua & 0xffff0000u), rb = b - __uint_as_float(ub & 0xffff0000u);
+  const uint32_t va = __float_as_uint(ra), vb = __float_as_uint(rb);
+  mid = __builtin_amdgcn_perm(vb, va, 0x07060302u);
+  const float sa = ra - __uint_as_float(va & 0xffff0000u), sb = rb - __uint_as_float(vb & 0xffff0000u);
+  lo = __builtin_amdgcn_perm(__float_as_uint(sb), __float_as_uint(sa), 0x07060302u);
+}
+
+__device__ __forceinline__ gdn::s16x8_t row_frag(const uint16_t* p) { return *reinterpret_cast<const gdn::s16x8_t*>(p); }
+
+__device__ __forceinline__ bool finite(float x) { return fabsf(x) <= 3.4028234664e38f; }
+
+// a[i] += f * sum over s of c[i][s] us[s], 16 x 16 coefficients from LDS rows
+template <int TM, int N>
+__device__ __forceinline__ void add_block(float (&a)[N], float f, const float (&c)[TM][TM], int t0, int s0,
+                                          const float (&us)[16]) {
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+#pragma unroll
+    for (int p = 0; p < 4; ++p) {
+      const float4 r = *reinterpret_cast<const float4*>(&c[t0 + i][s0 + 4 * p]);
+      a[i] = fmaf(f * r.x, us[4 * p], a[i]);
+      a[i] = fmaf(f * r.y, us[4 * p + 1], a[i]);
+      a[i] = fmaf(f * r.z, us[4 * p + 2], a[i]);
+      a[i] = fmaf(f * r.w, us[4 * p + 3], a[i]);
+    }
+}
+
+// NT: 16-node tiles of the tree (and of the pending one).
+template <int D, int NT>
+__global__ __launch_bounds__(2 * D, NT == 1 ? 3 : 1) void rule_tree_kernel(
+    const uint16_t* __restrict__ q, int64_t q_b, int64_t q_t, const uint16_t* __restrict__ k, int64_t k_b, int64_t k_t,
+    const uint16_t* __restrict__ v, int64_t v_b, int64_t v_t, const float* __restrict__ g,
+    const uint16_t* __restrict__ beta, float* __restrict__ pool, int64_t s_slot, int64_t n_slots,
+    const int64_t* __restrict__ ids, const int32_t* __restrict__ parents, int64_t p_b, RulePending pd,
+    uint16_t* __restrict__ o, float* __restrict__ u, int B, int T, int Hk, int Hv, float scale) {
+  constexpr int NW = D / 32, KK = D / 32, TM = 16 * NT;
+  __shared__ __align__(16) float wt[TM][TM];   // weights w(t, s)
+  __shared__ __align__(16) float cu[TM][TM];   // coefficients of u_s in u_t
+  __shared__ __align__(16) float co[TM][TM];   // and in o_t
+  __shared__ __align__(16) float xk[TM][D];    // the pending path's keys; S^T k; u
+  __shared__ __align__(16) float xq[TM][D];    // the pending path's corrections; S^T q
+  __shared__ int raw[kMaxNodes], link[kMaxNodes];
+  __shared__ float dec[TM], total[TM], bt[TM], rk[TM], rq[TM];
+  __shared__ int any_cu[NT][NT];               // whether a tile of coefficients holds an ancestor
+  __shared__ Path path;
+
+  const int64_t wi = gdn::xcd_remap(blockIdx.x, static_cast<int64_t>(B) * Hv);
+  if (wi < 0) return;
+  const int b = static_cast<int>(wi / Hv), h = static_cast<int>(wi % Hv), kh = h / (Hv / Hk);
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int lr = lane & 15, lg = lane >> 4;
+  const int64_t out_t = static_cast<int64_t>(Hv) * D;
+  const int64_t out0 = static_cast<int64_t>(b) * T * out_t + h * D;  // row t at out0 + t out_t
   const int64_t slot = ids[b];
-  if (slot < 0 || slot >= n_slots) return;
-  if (threadIdx.x < 64) tree_links(pd.parents + b * pd.p_b, pd.T, threadIdx.x, raw, link);
-  __syncthreads();
-  if (conv) {
-    const int c = at % parts * D + threadIdx.x;
-    const int a = accepted_node(cd.accepted[b], cd.T, link);
-    if (c >= C || a < 0) return;
-    uint16_t* p = cpool + slot * sp_slot + c * sp_ch;
-    uint16_t tap[3];
-#pragma unroll
-    for (int j = 0; j < 3; ++j) tap[j] = p[j];
-    advance_taps(tap, cd, b, c, a, link);
-#pragma unroll
-    for (int j = 0; j < 3; ++j) p[j] = tap[j];
+  if (slot < 0 || slot >= n_slots) {  // (the whole workgroup)
+    for (int t = tid / D; t < T; t += 2) {
+      o[out0 + t * out_t + tid % D] = 0;
+      u[out0 + t * out_t + tid % D] = 0.0f;
+    }
     return;
   }
-  const int h = at % Hv;
-  float* S0 = pool + slot * s_slot + static_cast<int64_t>(h) * D * D + threadIdx.x;
-  float S[D];
+  // Loads return in order: what the tree and the coefficients need goes out ahead of the
+  // state, which is then on its way while they are worked on.
+  const uint16_t* kb = k + b * k_b + kh * D + 8 * lg;
+  const uint16_t* qb = q + b * q_b + kh * D + 8 * lg;
+  auto k_frag = [&](int I, int kk) { return row_frag(kb + min(16 * I + lr, T - 1) * k_t + 32 * kk); };
+  auto q_frag = [&](int I, int kk) { return row_frag(qb + min(16 * I + lr, T - 1) * q_t + 32 * kk); };
+  constexpr bool kHold = NT <= 2;  // the nodes' rows in registers from here on
+  gdn::s16x8_t fk[kHold ? NT : 1][KK], fq[kHold ? NT : 1][KK];
+  if constexpr (kHold) {
 #pragma unroll
-  for (int i = 0; i < D; ++i) S[i] = S0[i * D];
-  if (advance_column<D>(S, pd, b, h, h / (Hv / Hk), Hv, link, node, weight, &total, &count, key)) {
+    for (int I = 0; I < NT; ++I)
 #pragma unroll
-    for (int i = 0; i < D; ++i) S0[i * D] = S[i];
+      for (int kk = 0; kk < KK; ++kk) {
+        fk[I][kk] = k_frag(I, kk);
+        fq[I][kk] = q_frag(I, kk);
+      }
   }
+  int my_parent = 0;
+  float my_g = 0.0f, my_beta = 0.0f;
+  PathIn pin = {-1, 0.0f, 0};
+  if (wave == 0) {
+    const int64_t at = (static_cast<int64_t>(b) * T + min(lane, T - 1)) * Hv + h;
+    my_g = g[at];
+    my_beta = gdn::bf2f(beta[at]);
+    my_parent = parents[b * p_b + min(lane, T - 1)];
+  } else if (wave == 1 && pd.accepted) {
+    pin.load(pd, b, h, Hv, lane);
+  }
+  gdn::keep_loads_here();
+  float* S0 = pool + slot * s_slot + static_cast<int64_t>(h) * D * D + 8 * lg * D + 32 * wave + 2 * lr;
+  Tile<D> S;
+  S.load(S0);
+  const uint16_t* vb = v + b * v_b + static_cast<int64_t>(h) * D + tid;  // (threads below D)
+  uint16_t vv[16];
+  auto load_v = [&](int I) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) vv[i] = vb[min(16 * I + i, T - 1) * v_t];
+  };
+  if (tid < D) load_v(0);
+  gdn::keep_loads_here();
+
+  // --- the tree and the nodes' norms; the pending path ---
+  if (wave == 0) {
+    if (lane < TM) {
+      dec[lane] = expf(my_g);
+      bt[lane] = my_beta;
+    }
+    for (int i = lane; i < TM * TM / 4; i += 64) reinterpret_cast<float4*>(wt)[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+    tree_links(my_parent, T, lane, raw, link);
+    wave_lds_order();
+    if (lane < T && link[lane] != kUnused) {
+      float w = 1.0f;
+      for (int s = lane; s >= 0; s = link[s]) {
+        wt[lane][s] = w;
+        w *= dec[s];
+      }
+      total[lane] = w;
+    }
+  } else if (wave == 1 && pd.accepted) {
+    find_path(pin, pd.T, lane, path);
+  }
+#pragma unroll
+  for (int I = 0; I < NT; ++I) {
+    // row 16 I + lr: the lane's 8 values of every 32, then the four lanes of the row
+    if (16 * I >= T || I % NW != wave) continue;
+    float sk = 0.0f, sq = 0.0f;
+#pragma unroll
+    for (int kk = 0; kk < KK; ++kk) {
+      const gdn::s16x8_t x = kHold ? fk[kHold ? I : 0][kk] : k_frag(I, kk);
+      const gdn::s16x8_t y = kHold ? fq[kHold ? I : 0][kk] : q_frag(I, kk);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float a = gdn::bf2f(static_cast<uint16_t>(x[e])), c = gdn::bf2f(static_cast<uint16_t>(y[e]));
+        sk = fmaf(a, a, sk);
+        sq = fmaf(c, c, sq);
+      }
+    }
+    sk += __shfl_xor(sk, 16, 64);
+    sq += __shfl_xor(sq, 16, 64);
+    sk += __shfl_xor(sk, 32, 64);
+    sq += __shfl_xor(sq, 32, 64);
+    if (lg == 0) {
+      rk[16 * I + lr] = rsqrtf(sk + kEps);
+      rq[16 * I + lr] = rsqrtf(sq + kEps);
+    }
+  }
+  gdn::lds_barrier();
+  const bool pending = pd.accepted && path.count > 0;  // (the whole workgroup)
+  if (pending) stage_path<D, TM>(pd, path, b, h, kh, Hv, wave, NW, lane, xk, xq);
+
+  // --- the nodes' products with each other: coefficients of u_s in u_t and in o_t ---
+  // Tile (I, J), J <= I, of K K^T and of Q K^T: lane (lr, lg), register r: t = 16 I + 4 lg
+  // + r, s = 16 J + lr.  A weight of 0 is not multiplied: nothing of an unused node, of
+  // another branch or past T gets in.
+#pragma unroll
+  for (int it = 0; it < NT * (NT + 1); ++it) {
+    const int type = it & 1;
+    int I = 0, J = it >> 1;
+    while (J > I) J -= ++I;
+    if (16 * I >= T || it % NW != wave) continue;
+    gdn::f32x4_t c = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int kk = 0; kk < KK; ++kk) {
+      if constexpr (kHold)
+        c = gdn::mfma16x16x32(type ? fq[I][kk] : fk[I][kk], fk[J][kk], c);
+      else
+        c = gdn::mfma16x16x32(type ? q_frag(I, kk) : k_frag(I, kk), k_frag(J, kk), c);
+    }
+    const int s = 16 * J + lr;
+    const float rs = rk[s];
+    bool some = false;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int t = 16 * I + 4 * lg + r;
+      const float w = wt[t][s];
+      if (type) {
+        co[t][s] = w != 0.0f ? (scale * rq[t]) * (rs * w) * c[r] : 0.0f;
+      } else {
+        const bool on = w != 0.0f && s < t;
+        cu[t][s] = on ? (bt[t] * rk[t]) * (rs * w) * c[r] : 0.0f;
+        some |= on;
+      }
+    }
+    if (!type) {
+      some = __any(some);
+      if (lane == 0) any_cu[I][J] = some;
+    }
+  }
+
+  // --- the state after the pending path; its products with the nodes' rows ---
+  if (pending) {
+    gdn::lds_barrier();
+    S.advance(path.total, path.count, xk, xq, wave, lr, lg);
+    S.store(S0);
+  }
+  gdn::f32x4_t ak[NT][2], aq[NT][2];  // [node tile][even, odd columns]
+#pragma unroll
+  for (int I = 0; I < NT; ++I)
+#pragma unroll
+    for (int c = 0; c < 2; ++c) ak[I][c] = aq[I][c] = gdn::f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int kk = 0; kk < KK; ++kk) {
+    typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+    u32x4 f[2][3];
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        uint32_t hi, mid, lo;
+        split3(S.s[kk][2 * e][c], S.s[kk][2 * e + 1][c], hi, mid, lo);
+        f[c][0][e] = hi;
+        f[c][1][e] = mid;
+        f[c][2][e] = lo;
+      }
+#pragma unroll
+    for (int I = 0; I < NT; ++I) {
+      if (16 * I >= T) break;
+      const gdn::s16x8_t x = kHold ? fk[kHold ? I : 0][kk] : k_frag(I, kk);
+      const gdn::s16x8_t y = kHold ? fq[kHold ? I : 0][kk] : q_frag(I, kk);
+#pragma unroll
+      for (int n = 2; n >= 0; --n)  // (the smallest terms first)
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          ak[I][c] = gdn::mfma16x16x32(x, __builtin_bit_cast(gdn::s16x8_t, f[c][n]), ak[I][c]);
+          aq[I][c] = gdn::mfma16x16x32(y, __builtin_bit_cast(gdn::s16x8_t, f[c][n]), aq[I][c]);
+        }
+    }
+  }
+  if (pending) gdn::lds_barrier();  // the path's rows have been read
+#pragma unroll
+  for (int I = 0; I < NT; ++I) {
+    if (16 * I >= T) break;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int t = 16 * I + 4 * lg + r;
+      *reinterpret_cast<f32x2_t*>(&xk[t][32 * wave + 2 * lr]) = f32x2_t{ak[I][0][r], ak[I][1][r]};
+      *reinterpret_cast<f32x2_t*>(&xq[t][32 * wave + 2 * lr]) = f32x2_t{aq[I][0][r], aq[I][1][r]};
+    }
+  }
+  gdn::lds_barrier();
+
+  // --- u, a column per thread: 16 nodes at a time, the earlier tiles' share and then one
+  // node after the other, in registers.  Coefficients of nodes that are no ancestors are 0:
+  // where a result is not finite, it is formed again from the ancestors alone (a branch's
+  // infinity or NaN stays in it). ---
+  if (tid < D) {
+#pragma unroll 1
+    for (int I = 0; 16 * I < T; ++I) {
+      float a[16], us[16];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const int t = 16 * I + i;
+        a[i] = t < T && link[min(t, T - 1)] != kUnused
+                   ? bt[t] * (gdn::bf2f(vv[i]) - (total[t] * rk[t]) * xk[t][tid])
+                   : 0.0f;
+      }
+      if (16 * I + 16 < T) load_v(I + 1);
+#pragma unroll 1
+      for (int J = 0; J < I; ++J) {
+        if (!any_cu[I][J]) continue;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) us[i] = xk[16 * J + i][tid];
+        add_block(a, -1.0f, cu, 16 * I, 16 * J, us);
+      }
+#pragma unroll
+      for (int p = 0; p < 4; ++p) {
+        // columns 4 p .. of the tile's coefficients
+        float4 c[16];
+#pragma unroll
+        for (int i = 4 * p + 1; i < 16; ++i)
+          c[i] = *reinterpret_cast<const float4*>(&cu[16 * I + i][16 * I + 4 * p]);
+#pragma unroll
+        for (int i = 4 * p + 1; i < 16; ++i) a[i] = fmaf(-c[i].x, a[4 * p], a[i]);
+#pragma unroll
+        for (int i = 4 * p + 2; i < 16; ++i) a[i] = fmaf(-c[i].y, a[4 * p + 1], a[i]);
+#pragma unroll
+        for (int i = 4 * p + 3; i < 16; ++i) a[i] = fmaf(-c[i].z, a[4 * p + 2], a[i]);
+#pragma unroll
+        for (int i = 4 * p + 4; i < 16; ++i) a[i] = fmaf(-c[i].w, a[4 * p + 3], a[i]);
+      }
+      bool fine = true;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) fine &= finite(a[i]);
+      if (__any(!fine)) {
+#pragma unroll 1
+        for (int t = 16 * I; t < min(T, 16 * I + 16); ++t) {
+          float x = 0.0f;
+          if (link[t] != kUnused) {
+            x = bt[t] * (gdn::bf2f(vb[t * v_t]) - (total[t] * rk[t]) * xk[t][tid]);
+            for (int s = link[t]; s >= 0; s = link[s]) x = fmaf(-cu[t][s], xk[s][tid], x);
+          }
+          xk[t][tid] = x;
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) xk[16 * I + i][tid] = a[i];
+      }
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        if (16 * I + i < T) u[out0 + (16 * I + i) * out_t + tid] = xk[16 * I + i][tid];
+    }
+  }
+  gdn::lds_barrier();
+
+  // --- o: two threads per column, 8 of every 16 nodes each ---
+  {
+    const int col = tid % D, half = tid / D;
+#pragma unroll 1
+    for (int I = 0; 16 * I < T; ++I) {
+      const int t0 = 16 * I + 8 * half;
+      if (t0 >= T) break;
+      float a[8], us[16];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int t = t0 + i;
+        a[i] = t < T && link[min(t, T - 1)] != kUnused ? (scale * rq[t]) * total[t] * xq[t][col] : 0.0f;
+      }
+#pragma unroll 1
+      for (int J = 0; J <= I; ++J) {
+        if (J < I && !any_cu[I][J]) continue;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) us[i] = xk[16 * J + i][col];
+        add_block(a, 1.0f, co, t0, 16 * J, us);
+      }
+      bool fine = true;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) fine &= finite(a[i]);
+      if (__any(!fine)) {
+#pragma unroll 1
+        for (int t = t0; t < min(T, t0 + 8); ++t) {
+          float x = 0.0f;
+          if (link[t] != kUnused) {
+            x = (scale * rq[t]) * total[t] * xq[t][col];
+            for (int s = t; s >= 0; s = link[s]) x = fmaf(co[t][s], xk[s][col], x);
+          }
+          o[out0 + t * out_t + col] = gdn::f2bf(x);
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (t0 + i < T) o[out0 + (t0 + i) * out_t + col] = gdn::f2bf(a[i]);
+      }
+    }
+  }
+}
+
+// ---- commit ----
+// The first `states` workgroups: the state tiles, one each.  Then the taps, 8 channels per
+// thread.
+template <int D, int NT>
+__global__ __launch_bounds__(2 * D) void commit_tree_kernel(float* __restrict__ pool, int64_t s_slot,
+                                                            uint16_t* __restrict__ cpool, int64_t sp_slot,
+                                                            int64_t sp_ch, int64_t n_slots,
+                                                            const int64_t* __restrict__ ids, RulePending pd,
+                                                            ConvPending cd, int B, int Hk, int Hv, int C,
+                                                            int states) {
+  constexpr int NW = D / 32, TM = 16 * NT;
+  __shared__ __align__(16) float wk[TM][D];
+  __shared__ __align__(16) float us[TM][D];
+  __shared__ Path path;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  if (static_cast<int>(blockIdx.x) >= states) {
+    const int parts = (C + 16 * D - 1) / (16 * D);
+    const int at = blockIdx.x - states, b = at / parts;
+    const int64_t slot = ids[b];
+    if (slot < 0 || slot >= n_slots) return;
+    if (wave == 0) tree_links(cd.parents[b * cd.p_b + min(lane, cd.T - 1)], cd.T, lane, path.raw, path.link);
+    __syncthreads();
+    const int a = accepted_node(cd.accepted[b], cd.T, path.link);
+    const int c0 = (at % parts * 2 * D + tid) * 8;
+    if (c0 >= C || a < 0) return;
+#pragma unroll 1
+    for (int c = c0; c < c0 + 8; ++c) {
+      uint16_t* p = cpool + slot * sp_slot + c * sp_ch;
+      uint16_t tap[3];
+#pragma unroll
+      for (int j = 0; j < 3; ++j) tap[j] = p[j];
+      advance_taps(tap, cd, b, c, a, path.link);
+#pragma unroll
+      for (int j = 0; j < 3; ++j) p[j] = tap[j];
+    }
+    return;
+  }
+  const int64_t wi = gdn::xcd_remap(blockIdx.x, static_cast<int64_t>(B) * Hv);
+  if (wi < 0) return;
+  const int b = static_cast<int>(wi / Hv), h = static_cast<int>(wi % Hv);
+  const int lr = lane & 15, lg = lane >> 4;
+  const int64_t slot = ids[b];
+  if (slot < 0 || slot >= n_slots) return;
+  float* S0 = pool + slot * s_slot + static_cast<int64_t>(h) * D * D + 8 * lg * D + 32 * wave + 2 * lr;
+  PathIn pin = {-1, 0.0f, 0};
+  if (wave == 0) pin.load(pd, b, h, Hv, lane);
+  gdn::keep_loads_here();
+  Tile<D> S;
+  S.load(S0);
+  gdn::keep_loads_here();
+  if (wave == 0) find_path(pin, pd.T, lane, path);
+  gdn::lds_barrier();
+  if (path.count == 0) return;  // (the whole workgroup)
+  stage_path<D, TM>(pd, path, b, h, h / (Hv / Hk), Hv, wave, NW, lane, wk, us);
+  gdn::lds_barrier();
+  S.advance(path.total, path.count, wk, us, wave, lr, lg);
+  S.store(S0);
 }
 
 bool rows_ok(const void* p, int64_t s_b, int64_t s_t, int width, int T) {
@@ -366,14 +727,18 @@ extern "C" int gdn_rule_tree(const uint16_t* q, int64_t q_b, int64_t q_t, const 
     return GDN_ERR_INVALID_ARG;
   if (static_cast<int64_t>(B) * Hv >= (1LL << 24)) return GDN_ERR_UNSUPPORTED;
   const RulePending pd{last_k, lk_b, lk_t, last_g, last_u, last_parents, lp_b, accepted, last_T};
-  const dim3 grid(static_cast<unsigned>(B * Hv));
+  const dim3 grid(static_cast<unsigned>(gdn::kNumXcd * ((B * Hv + gdn::kNumXcd - 1) / gdn::kNumXcd)));
   hipStream_t st = static_cast<hipStream_t>(stream);
+  const int nodes = accepted ? std::max(T, last_T) : T;
+#define GDN_RULE(DD, NT)                                                                                            \
+  rule_tree_kernel<DD, NT><<<grid, dim3(2 * DD), 0, st>>>(q, q_b, q_t, k, k_b, k_t, v, v_b, v_t, g, beta, s_pool,    \
+                                                          s_slot, n_slots, ids, parents, p_b, pd, o, u, B, T, Hk, Hv, \
+                                                          scale)
   if (D == 128)
-    rule_tree_kernel<128><<<grid, dim3(128), 0, st>>>(q, q_b, q_t, k, k_b, k_t, v, v_b, v_t, g, beta, s_pool, s_slot,
-                                                      n_slots, ids, parents, p_b, pd, o, u, T, Hk, Hv, scale);
+    nodes <= 16 ? GDN_RULE(128, 1) : nodes <= 32 ? GDN_RULE(128, 2) : GDN_RULE(128, 4);
   else
-    rule_tree_kernel<64><<<grid, dim3(64), 0, st>>>(q, q_b, q_t, k, k_b, k_t, v, v_b, v_t, g, beta, s_pool, s_slot,
-                                                    n_slots, ids, parents, p_b, pd, o, u, T, Hk, Hv, scale);
+    nodes <= 16 ? GDN_RULE(64, 1) : nodes <= 32 ? GDN_RULE(64, 2) : GDN_RULE(64, 4);
+#undef GDN_RULE
   return gdn_launch_status();
 }
 
@@ -393,13 +758,17 @@ extern "C" int gdn_commit_tree(float* s_pool, int64_t s_slot, uint16_t* conv_poo
   if (static_cast<int64_t>(B) * (Hv + (C + D - 1) / D) >= (1LL << 24)) return GDN_ERR_UNSUPPORTED;
   const RulePending pd{k, k_b, k_t, g, u, parents, p_b, accepted, T};
   const ConvPending cd{x, x_b, x_t, parents, p_b, accepted, T};
-  const dim3 grid(static_cast<unsigned>(B * (Hv + (C + D - 1) / D)));
+  // (the conv workgroups after the states')
+  const int states = gdn::kNumXcd * ((B * Hv + gdn::kNumXcd - 1) / gdn::kNumXcd);
+  const dim3 grid(static_cast<unsigned>(states + B * ((C + 8 * 2 * D - 1) / (8 * 2 * D))));
   hipStream_t st = static_cast<hipStream_t>(stream);
+#define GDN_COMMIT(DD, NT)                                                                                          \
+  commit_tree_kernel<DD, NT><<<grid, dim3(2 * DD), 0, st>>>(s_pool, s_slot, conv_pool, sp_slot, sp_ch, n_slots, ids, \
+                                                            pd, cd, B, Hk, Hv, C, states)
   if (D == 128)
-    commit_tree_kernel<128><<<grid, dim3(128), 0, st>>>(s_pool, s_slot, conv_pool, sp_slot, sp_ch, n_slots, ids, pd,
-                                                        cd, B, Hk, Hv, C);
+    T <= 16 ? GDN_COMMIT(128, 1) : GDN_COMMIT(128, 4);
   else
-    commit_tree_kernel<64><<<grid, dim3(64), 0, st>>>(s_pool, s_slot, conv_pool, sp_slot, sp_ch, n_slots, ids, pd, cd,
-                                                      B, Hk, Hv, C);
+    T <= 16 ? GDN_COMMIT(64, 1) : GDN_COMMIT(64, 4);
+#undef GDN_COMMIT
   return gdn_launch_status();
 }
