@@ -146,6 +146,11 @@ def ptr(t) -> int | None:
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 
+def stream_of(index: int) -> int:
+    """hipStream_t of torch's current stream on device `index`."""
+    return torch.cuda.current_stream(index).cuda_stream if _raw_stream is None else _raw_stream(index)
+
+
 def stream_handle(device) -> int:
     """hipStream_t of torch's current stream on `device`."""
     if _raw_stream is None or device.index is None:

@@ -71,68 +71,196 @@ struct ConvPending {
 // The row before row r of a tree: r >= 0 a node, -1, -2, -3 the taps from the newest.
 __device__ __forceinline__ int row_before(int r, const int* link) { return r >= 0 ? link[r] : r - 1; }
 
-// The taps of channel c after the accepted node: rows a, its parent and its grandparent.
-__device__ __forceinline__ void advance_taps(uint16_t (&tap)[3], const ConvPending& pd, int b, int c, int a,
-                                             const int* link) {
-  uint16_t now[3];
-  int r = a;
-#pragma unroll
-  for (int j = 2; j >= 0; --j) {
-    now[j] = r >= 0 ? pd.x[b * pd.x_b + r * pd.x_t + c] : r == -1 ? tap[2] : r == -2 ? tap[1] : tap[0];
-    r = row_before(r, link);
-  }
-#pragma unroll
-  for (int j = 0; j < 3; ++j) tap[j] = now[j];
+// Eight channels' values (of a row, or of one tap).
+struct Row8 {
+  uint16_t v[8];
+};
+static_assert(sizeof(Row8) == 16, "one 16-byte piece");
+__device__ __forceinline__ Row8 row8(const uint16_t* p) {
+  return __builtin_bit_cast(Row8, *reinterpret_cast<const uint4*>(p));
 }
 
-// grid (ceil(C / 256), B): a channel per thread
-__global__ __launch_bounds__(256) void conv_tree_kernel(const uint16_t* __restrict__ x, int64_t x_b, int64_t x_t,
-                                                        uint16_t* __restrict__ pool, int64_t sp_slot, int64_t sp_ch,
-                                                        int64_t n_slots, const int64_t* __restrict__ ids,
-                                                        const uint16_t* __restrict__ w,
-                                                        const int32_t* __restrict__ parents, int64_t p_b,
-                                                        ConvPending pd, uint16_t* __restrict__ y, int T, int C) {
+// The three taps of channels c .. c + 7 of a slot, oldest first.  dense: the channels'
+// taps lie one behind the other in 16-byte pieces.
+struct Taps {
+  Row8 tap[3];
+
+  __device__ __forceinline__ void load(const uint16_t* p, int64_t sp_ch, bool dense) {
+    if (dense) {
+      Row8 raw[3];
+#pragma unroll
+      for (int i = 0; i < 3; ++i) raw[i] = row8(p + 8 * i);
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+#pragma unroll
+        for (int j = 0; j < 3; ++j) tap[j].v[i] = raw[(3 * i + j) / 8].v[(3 * i + j) % 8];
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+#pragma unroll
+        for (int j = 0; j < 3; ++j) tap[j].v[i] = p[i * sp_ch + j];
+    }
+  }
+  __device__ __forceinline__ void store(uint16_t* p, int64_t sp_ch, bool dense) const {
+    if (dense) {
+      Row8 raw[3];
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+#pragma unroll
+        for (int j = 0; j < 3; ++j) raw[(3 * i + j) / 8].v[(3 * i + j) % 8] = tap[j].v[i];
+#pragma unroll
+      for (int i = 0; i < 3; ++i) *reinterpret_cast<uint4*>(p + 8 * i) = __builtin_bit_cast(uint4, raw[i]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+#pragma unroll
+        for (int j = 0; j < 3; ++j) p[i * sp_ch + j] = tap[j].v[i];
+    }
+  }
+  __device__ __forceinline__ const Row8& before(int r) const {  // r in -1, -2, -3
+    return r == -1 ? tap[2] : r == -2 ? tap[1] : tap[0];
+  }
+  // The taps after the accepted node: its row, its parent's and its grandparent's.
+  __device__ __forceinline__ void advance(const ConvPending& pd, int b, int c, int a, const int* link) {
+    const uint16_t* x = pd.x + b * pd.x_b + c;
+    const int r1 = row_before(a, link), r0 = row_before(r1, link);
+    const Row8 n2 = row8(x + a * pd.x_t);
+    const Row8 n1 = r1 >= 0 ? row8(x + r1 * pd.x_t) : before(r1);
+    const Row8 n0 = r0 >= 0 ? row8(x + r0 * pd.x_t) : before(r0);
+    tap[0] = n0;
+    tap[1] = n1;
+    tap[2] = n2;
+  }
+};
+
+__device__ __forceinline__ bool dense_taps(const uint16_t* pool, int64_t sp_slot, int64_t sp_ch) {
+  return sp_ch == 3 && sp_slot % 8 == 0 && reinterpret_cast<uintptr_t>(pool) % 16 == 0;
+}
+
+// A workgroup is one wave: 128 channels of one sequence, two per thread, all nodes.  A
+// thread's rows go through its own column of LDS, where their children find them: every
+// row is read once, no wave waits for another, and a thread rolls its own channels' taps.
+// Rows come 8 at a time, the next ones on their way while these are worked on.  Bound by
+// the rows' way in and out (2 + 2 bytes per value) and the SiLU's two transcendentals per
+// value, with few sequences by the latency of links, rows and taps.  (256 threads of 8
+// channels that share the nodes of a sequence: 64 trees of 16 nodes, 8192 channels 17.7
+// us, one tree of 8 nodes 5.5.)
+__global__ __launch_bounds__(64) void conv_tree_kernel(const uint16_t* __restrict__ x, int64_t x_b, int64_t x_t,
+                                                       uint16_t* __restrict__ pool, int64_t sp_slot, int64_t sp_ch,
+                                                       int64_t n_slots, const int64_t* __restrict__ ids,
+                                                       const uint16_t* __restrict__ w,
+                                                       const int32_t* __restrict__ parents, int64_t p_b,
+                                                       ConvPending pd, uint16_t* __restrict__ y, int T, int C) {
+  // [3 + T][64], two channels per thread: the taps, oldest first, then the nodes' rows, so
+  // that row r is at r + 3 (row_before)
+  extern __shared__ uint32_t rows[];
   __shared__ int raw[2][kMaxNodes], link[2][kMaxNodes];
-  const int b = blockIdx.y;
-  const int c = blockIdx.x * 256 + threadIdx.x;
-  if (threadIdx.x < 64) {
-    tree_links(parents[b * p_b + min<int>(threadIdx.x, T - 1)], T, threadIdx.x, raw[0], link[0]);
-  } else if (threadIdx.x < 128 && pd.accepted) {
-    const int lane = threadIdx.x - 64;
-    tree_links(pd.parents[b * pd.p_b + min(lane, pd.T - 1)], pd.T, lane, raw[1], link[1]);
-  }
-  __syncthreads();
-  if (c >= C) return;
+  const int b = blockIdx.y, lane = threadIdx.x;
+  const int c = 2 * (blockIdx.x * 64 + lane);
+  const bool in = c < C;
+  uint32_t* yb = reinterpret_cast<uint32_t*>(y + static_cast<int64_t>(b) * T * C + c);
   const int64_t slot = ids[b];
-  const bool row_ok = slot >= 0 && slot < n_slots;
-  uint16_t tap[3] = {0, 0, 0};
-  if (row_ok) {
-    uint16_t* p = pool + slot * sp_slot + c * sp_ch;
+  if (slot < 0 || slot >= n_slots) {  // (the whole workgroup)
+    for (int t = 0; t < T && in; ++t) yb[t * (C / 2)] = 0;
+    return;
+  }
+  // what the links need first, then weights and rows, then the taps and the pending rows
+  const int parent = parents[b * p_b + min(lane, T - 1)];
+  int last_parent = 0;
+  int64_t want = -1;
+  if (pd.accepted) {
+    last_parent = pd.parents[b * pd.p_b + min(lane, pd.T - 1)];
+    want = pd.accepted[b];
+  }
+  const uint16_t* xb = x + b * x_b + (in ? c : 0);
+  uint16_t* tp = pool + slot * sp_slot + (in ? c : 0) * sp_ch;
+  const uint4 wv = *reinterpret_cast<const uint4*>(w + (in ? c : 0) * 4);
+  auto pair = [](const uint16_t* p) { return *reinterpret_cast<const uint32_t*>(p); };
+  uint32_t next[8];
 #pragma unroll
-    for (int j = 0; j < 3; ++j) tap[j] = p[j];
-    const int a = pd.accepted ? accepted_node(pd.accepted[b], pd.T, link[1]) : -1;
-    if (a >= 0) {
-      advance_taps(tap, pd, b, c, a, link[1]);
+  for (int i = 0; i < 8; ++i) next[i] = pair(xb + min(i, T - 1) * x_t);
+  uint32_t tap[3];  // of both channels, oldest first
+  const bool dense = sp_ch == 3 && sp_slot % 2 == 0 && reinterpret_cast<uintptr_t>(pool) % 4 == 0;
+  if (dense) {
+    const uint32_t u0 = pair(tp), u1 = pair(tp + 2), u2 = pair(tp + 4);
+    tap[0] = (u0 & 0xffffu) | (u1 & 0xffff0000u);
+    tap[1] = (u0 >> 16) | (u2 << 16);
+    tap[2] = (u1 & 0xffffu) | (u2 & 0xffff0000u);
+  } else {
 #pragma unroll
-      for (int j = 0; j < 3; ++j) p[j] = tap[j];
+    for (int j = 0; j < 3; ++j) tap[j] = tp[j] | static_cast<uint32_t>(tp[sp_ch + j]) << 16;
+  }
+  gdn::keep_loads_here();
+  tree_links(parent, T, lane, raw[0], link[0]);
+  if (pd.accepted) tree_links(last_parent, pd.T, lane, raw[1], link[1]);
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront", "local");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront", "local");
+  auto before = [](int r, const int* l) { return __builtin_amdgcn_readfirstlane(row_before(r, l)); };
+  auto old = [&](int r) { return r == -1 ? tap[2] : r == -2 ? tap[1] : tap[0]; };
+  const int a = pd.accepted ? __builtin_amdgcn_readfirstlane(accepted_node(want, pd.T, link[1])) : -1;
+  if (a >= 0) {
+    // the taps after the accepted node: its row, its parent's and its grandparent's
+    const uint16_t* lx = pd.x + b * pd.x_b + (in ? c : 0);
+    const int r1 = before(a, link[1]), r0 = before(r1, link[1]);
+    const uint32_t n2 = pair(lx + a * pd.x_t);
+    const uint32_t n1 = r1 >= 0 ? pair(lx + r1 * pd.x_t) : old(r1);
+    const uint32_t n0 = r0 >= 0 ? pair(lx + r0 * pd.x_t) : old(r0);
+    tap[0] = n0;
+    tap[1] = n1;
+    tap[2] = n2;
+    if (in && dense) {
+      uint32_t* q = reinterpret_cast<uint32_t*>(tp);
+      q[0] = (n0 & 0xffffu) | (n1 << 16);
+      q[1] = (n2 & 0xffffu) | (n0 & 0xffff0000u);
+      q[2] = (n1 >> 16) | (n2 & 0xffff0000u);
+    } else if (in) {
+#pragma unroll
+      for (int j = 0; j < 3; ++j) {
+        tp[j] = static_cast<uint16_t>(tap[j]);
+        tp[sp_ch + j] = static_cast<uint16_t>(tap[j] >> 16);
+      }
     }
   }
-  float wk[4];
+  float w0[4], w1[4];
+  const uint32_t ww[4] = {wv.x, wv.y, wv.z, wv.w};
 #pragma unroll
-  for (int j = 0; j < 4; ++j) wk[j] = gdn::bf2f(w[c * 4 + j]);
-  for (int t = 0; t < T; ++t) {
-    uint16_t out = 0;
-    if (row_ok && link[0][t] != kUnused) {
-      float s[3];
-      int r = t;
+  for (int j = 0; j < 4; ++j) {
+    w0[j] = __uint_as_float(j % 2 ? ww[j / 2] & 0xffff0000u : ww[j / 2] << 16);
+    w1[j] = __uint_as_float(j % 2 ? ww[2 + j / 2] & 0xffff0000u : ww[2 + j / 2] << 16);
+  }
 #pragma unroll
-      for (int j = 2; j >= 0; --j) {
-        r = row_before(r, link[0]);
-        s[j] = gdn::bf2f(r >= 0 ? x[b * x_b + r * x_t + c] : r == -1 ? tap[2] : r == -2 ? tap[1] : tap[0]);
-      }
-      out = gdn::f2bf(gdn::conv_decode_silu(gdn::bf2f(x[b * x_b + t * x_t + c]), s[0], s[1], s[2], wk));
+  for (int j = 0; j < 3; ++j) rows[j * 64 + lane] = tap[j];
+  // lane t: the places of node t's three predecessors, a byte each; negative: unused
+  int places = -1;
+  if (lane < T && link[0][lane] != kUnused) {
+    const int r2 = link[0][lane], r1 = row_before(r2, link[0]), r0 = row_before(r1, link[0]);
+    places = (r2 + 3) | (r1 + 3) << 8 | (r0 + 3) << 16;
+  }
+  auto lo = [](uint32_t u) { return __uint_as_float(u << 16); };
+  auto hi = [](uint32_t u) { return __uint_as_float(u & 0xffff0000u); };
+  for (int t0 = 0; t0 < T; t0 += 8) {
+    uint32_t now[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) now[i] = next[i];
+    if (t0 + 8 < T) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) next[i] = pair(xb + min(t0 + 8 + i, T - 1) * x_t);
     }
-    y[(static_cast<int64_t>(b) * T + t) * C + c] = out;
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (t0 + i < T) rows[(3 + t0 + i) * 64 + lane] = now[i];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int t = t0 + i;
+      if (t >= T) break;
+      const int place = __builtin_amdgcn_readlane(places, t), at = max(place, 0);
+      const uint32_t x3 = now[i], x2 = rows[(at & 255) * 64 + lane], x1 = rows[(at >> 8 & 255) * 64 + lane],
+                     x0 = rows[(at >> 16 & 255) * 64 + lane];
+      const uint32_t out = gdn::f2bf2(gdn::conv_decode_silu(lo(x3), lo(x0), lo(x1), lo(x2), w0),
+                                      gdn::conv_decode_silu(hi(x3), hi(x0), hi(x1), hi(x2), w1));
+      if (in) yb[t * (C / 2)] = place < 0 ? 0 : out;
+    }
   }
 }
 
@@ -301,7 +429,7 @@ __device__ __forceinline__ void add_block(float (&a)[N], float f, const float (&
 
 // NT: 16-node tiles of the tree (and of the pending one).
 template <int D, int NT>
-__global__ __launch_bounds__(2 * D, NT == 1 ? 3 : 1) void rule_tree_kernel(
+__global__ __launch_bounds__(2 * D, NT == 1 ? 4 : 2) void rule_tree_kernel(
     const uint16_t* __restrict__ q, int64_t q_b, int64_t q_t, const uint16_t* __restrict__ k, int64_t k_b, int64_t k_t,
     const uint16_t* __restrict__ v, int64_t v_b, int64_t v_t, const float* __restrict__ g,
     const uint16_t* __restrict__ beta, float* __restrict__ pool, int64_t s_slot, int64_t n_slots,
@@ -340,7 +468,7 @@ __global__ __launch_bounds__(2 * D, NT == 1 ? 3 : 1) void rule_tree_kernel(
   const uint16_t* qb = q + b * q_b + kh * D + 8 * lg;
   auto k_frag = [&](int I, int kk) { return row_frag(kb + min(16 * I + lr, T - 1) * k_t + 32 * kk); };
   auto q_frag = [&](int I, int kk) { return row_frag(qb + min(16 * I + lr, T - 1) * q_t + 32 * kk); };
-  constexpr bool kHold = NT <= 2;  // the nodes' rows in registers from here on
+  constexpr bool kHold = NT == 1;  // the nodes' rows, for their norms and products with each other
   gdn::s16x8_t fk[kHold ? NT : 1][KK], fq[kHold ? NT : 1][KK];
   if constexpr (kHold) {
 #pragma unroll
@@ -372,7 +500,6 @@ __global__ __launch_bounds__(2 * D, NT == 1 ? 3 : 1) void rule_tree_kernel(
 #pragma unroll
     for (int i = 0; i < 16; ++i) vv[i] = vb[min(16 * I + i, T - 1) * v_t];
   };
-  if (tid < D) load_v(0);
   gdn::keep_loads_here();
 
   // --- the tree and the nodes' norms; the pending path ---
@@ -491,8 +618,8 @@ __global__ __launch_bounds__(2 * D, NT == 1 ? 3 : 1) void rule_tree_kernel(
 #pragma unroll
     for (int I = 0; I < NT; ++I) {
       if (16 * I >= T) break;
-      const gdn::s16x8_t x = kHold ? fk[kHold ? I : 0][kk] : k_frag(I, kk);
-      const gdn::s16x8_t y = kHold ? fq[kHold ? I : 0][kk] : q_frag(I, kk);
+      // (again from the caches: in registers they would cost a workgroup per CU)
+      const gdn::s16x8_t x = k_frag(I, kk), y = q_frag(I, kk);
 #pragma unroll
       for (int n = 2; n >= 0; --n)  // (the smallest terms first)
 #pragma unroll
@@ -502,6 +629,7 @@ __global__ __launch_bounds__(2 * D, NT == 1 ? 3 : 1) void rule_tree_kernel(
         }
     }
   }
+  if (tid < D) load_v(0);
   if (pending) gdn::lds_barrier();  // the path's rows have been read
 #pragma unroll
   for (int I = 0; I < NT; ++I) {
@@ -646,16 +774,12 @@ __global__ __launch_bounds__(2 * D) void commit_tree_kernel(float* __restrict__ 
     const int a = accepted_node(cd.accepted[b], cd.T, path.link);
     const int c0 = (at % parts * 2 * D + tid) * 8;
     if (c0 >= C || a < 0) return;
-#pragma unroll 1
-    for (int c = c0; c < c0 + 8; ++c) {
-      uint16_t* p = cpool + slot * sp_slot + c * sp_ch;
-      uint16_t tap[3];
-#pragma unroll
-      for (int j = 0; j < 3; ++j) tap[j] = p[j];
-      advance_taps(tap, cd, b, c, a, path.link);
-#pragma unroll
-      for (int j = 0; j < 3; ++j) p[j] = tap[j];
-    }
+    uint16_t* p = cpool + slot * sp_slot + c0 * sp_ch;
+    const bool dense = dense_taps(cpool, sp_slot, sp_ch);
+    Taps taps;
+    taps.load(p, sp_ch, dense);
+    taps.advance(cd, b, c0, a, path.link);
+    taps.store(p, sp_ch, dense);
     return;
   }
   const int64_t wi = gdn::xcd_remap(blockIdx.x, static_cast<int64_t>(B) * Hv);
@@ -702,7 +826,7 @@ extern "C" int gdn_conv_tree(const uint16_t* x, int64_t x_b, int64_t x_t, uint16
   if (accepted && (!rows_ok(last_x, lx_b, lx_t, C, last_T) || !last_parents || lp_b < 0)) return GDN_ERR_INVALID_ARG;
   if (B > 65535) return GDN_ERR_UNSUPPORTED;
   const ConvPending pd{last_x, lx_b, lx_t, last_parents, lp_b, accepted, last_T};
-  conv_tree_kernel<<<dim3((C + 255) / 256, B), dim3(256), 0, static_cast<hipStream_t>(stream)>>>(
+  conv_tree_kernel<<<dim3((C + 127) / 128, B), dim3(64), (T + 3) * 256, static_cast<hipStream_t>(stream)>>>(
       x, x_b, x_t, pool, sp_slot, sp_ch, n_slots, ids, w, parents, p_b, pd, y, T, C);
   return gdn_launch_status();
 }
@@ -735,9 +859,9 @@ extern "C" int gdn_rule_tree(const uint16_t* q, int64_t q_b, int64_t q_t, const 
                                                           s_slot, n_slots, ids, parents, p_b, pd, o, u, B, T, Hk, Hv, \
                                                           scale)
   if (D == 128)
-    nodes <= 16 ? GDN_RULE(128, 1) : nodes <= 32 ? GDN_RULE(128, 2) : GDN_RULE(128, 4);
+    nodes <= 16 ? GDN_RULE(128, 1) : nodes <= 32 ? GDN_RULE(128, 2) : nodes <= 48 ? GDN_RULE(128, 3) : GDN_RULE(128, 4);
   else
-    nodes <= 16 ? GDN_RULE(64, 1) : nodes <= 32 ? GDN_RULE(64, 2) : GDN_RULE(64, 4);
+    nodes <= 16 ? GDN_RULE(64, 1) : nodes <= 32 ? GDN_RULE(64, 2) : nodes <= 48 ? GDN_RULE(64, 3) : GDN_RULE(64, 4);
 #undef GDN_RULE
   return gdn_launch_status();
 }

@@ -48,13 +48,26 @@ def _stream(dev: torch.device) -> int:
     return _lib.stream_handle(dev)
 
 
-def _call_on(dev: torch.device, name: str, *args) -> None:
-    """_lib.call with `dev` as the current device: a launch goes to the stream's own."""
-    if dev.type == "cuda" and dev.index is not None and dev.index != torch.cuda.current_device():
-        with torch.cuda.device(dev):
-            _lib.call(name, *args)
+def _device_of(first: torch.Tensor, *others: torch.Tensor | None) -> int:
+    """The index of the device that all of them are on (as _check_cuda; a few lookups
+    cheaper)."""
+    idx = first.get_device()
+    for t in others:
+        if t is not None and t.get_device() != idx:
+            _check_cuda(first, *others)
+    if idx < 0 or not first.is_cuda:
+        _check_cuda(first, *others)
+    return idx
+
+
+def _call_on(idx: int, name: str, *args) -> None:
+    """_lib.call on device idx's current stream, which is appended to args: a launch
+    goes to its stream's device, so that one is made current where it is not."""
+    if idx == torch.cuda.current_device():
+        _lib.call(name, *args, _lib.stream_of(idx))
     else:
-        _lib.call(name, *args)
+        with torch.cuda.device(idx):
+            _lib.call(name, *args, _lib.stream_of(idx))
 
 
 # ------------------------------------------------------- fp16 operand range --
@@ -841,49 +854,56 @@ MAX_TREE_NODES = 64
 
 def _tree_parents(parents: torch.Tensor, B: int, T: int):
     """(int32 parents, row stride) of a [B, T] or [T] (one tree for all) tensor."""
-    if parents.dtype not in (torch.int32, torch.int64) or tuple(parents.shape) not in ((B, T), (T,)):
-        raise ValueError(f"parents must be int32 or int64 [{B}, {T}] or [{T}], got {parents.dtype} "
-                         f"{tuple(parents.shape)}")
     if not 1 <= T <= MAX_TREE_NODES:
         raise ValueError(f"a tree has 1 to {MAX_TREE_NODES} nodes, got {T}")
+    stride = T if parents.dim() == 2 else 0
+    if parents.shape != ((B, T) if stride else (T,)) or parents.dtype not in (torch.int32, torch.int64):
+        raise ValueError(f"parents must be int32 or int64 [{B}, {T}] or [{T}], got {parents.dtype} "
+                         f"{list(parents.shape)}")
     if parents.dtype == torch.int64:
         # (out of int32's range: not a node either way)
         parents = parents.clamp(-2, MAX_TREE_NODES).to(torch.int32)
-    parents = parents.contiguous()
-    return parents, T if parents.dim() == 2 else 0
+    return parents if parents.is_contiguous() else parents.contiguous(), stride
 
 
 def _tree_ids(ids: torch.Tensor, B: int, name: str = "ids") -> torch.Tensor:
+    if ids.dtype == torch.int64 and ids.shape == (B,) and ids.is_contiguous():
+        return ids
     if ids.shape != (B,) or ids.dtype not in (torch.int32, torch.int64):
-        raise ValueError(f"{name} must be int64 (or int32) [{B}], got {ids.dtype} {tuple(ids.shape)}")
+        raise ValueError(f"{name} must be int64 (or int32) [{B}], got {ids.dtype} {list(ids.shape)}")
     return ids.to(torch.int64).contiguous()
 
 
-def _tree_rows(t: torch.Tensor, name: str, shape: tuple) -> torch.Tensor:
-    """bf16 [B, T, ...] with dense rows that the kernels read in 16-byte pieces (else copied once)."""
-    _bf16(t, name)
-    if tuple(t.shape) != shape:
+def _tree_rows(t: torch.Tensor, name: str, shape: tuple):
+    """bf16 [B, T, heads, D] or [B, T, C] with dense rows that the kernels read in
+    16-byte pieces (else copied once), and its strides per sequence and node."""
+    if t.shape != shape or t.dtype != torch.bfloat16:
+        if t.dtype != torch.bfloat16:
+            raise TypeError(f"{name} must be bfloat16, got {t.dtype}")
         raise ValueError(f"{name} must be {list(shape)}, got {list(t.shape)}")
-    width, dense, st = 1, True, t.stride()
-    for n, s in zip(reversed(shape[2:]), reversed(st[2:])):
-        dense &= n == 1 or s == width
-        width *= n
-    if not dense or t.data_ptr() % 16 or st[0] % 8 or st[1] % 8 or st[1] < width:
-        t = t.contiguous() if not t.is_contiguous() else t.clone()
-    return t
+    width = shape[2] if len(shape) == 3 else shape[2] * shape[3]
+    st = t.stride()
+    dense = st[-1] == 1 and (len(shape) == 3 or st[2] == shape[3] or shape[2] == 1)
+    if not dense or st[1] < width or st[0] % 8 or st[1] % 8 or t.data_ptr() % 16:
+        t = t.contiguous() if not t.is_contiguous() else t.clone(memory_format=torch.contiguous_format)
+        return t, shape[1] * width, width
+    return t, st[0], st[1]
 
 
 def _tree_f32(t: torch.Tensor, name: str, shape: tuple) -> torch.Tensor:
-    if t.dtype != torch.float32 or tuple(t.shape) != shape:
+    if t.dtype != torch.float32 or t.shape != shape:
         raise ValueError(f"{name} must be float32 {list(shape)}, got {t.dtype} {list(t.shape)}")
-    t = t.contiguous()
-    return t if t.data_ptr() % 16 == 0 else t.clone()
+    if not t.is_contiguous():
+        return t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format)
 
 
-def _conv_pool_ok(pool: torch.Tensor, C: int) -> None:
+def _conv_pool_ok(pool: torch.Tensor, C: int) -> tuple:
     _bf16(pool, "conv_pool")
-    if pool.dim() != 3 or tuple(pool.shape[1:]) != (C, 3) or pool.stride(2) != 1:
+    st = pool.stride()
+    if pool.dim() != 3 or pool.shape[1] != C or pool.shape[2] != 3 or st[2] != 1:
         raise ValueError(f"conv_pool must be a [slots, {C}, 3] view with contiguous taps, got {list(pool.shape)}")
+    return st
 
 
 def _s_pool_ok(pool: torch.Tensor, Hv: int, D: int) -> None:
@@ -907,30 +927,28 @@ def conv_tree_step(x: torch.Tensor, conv_pool: torch.Tensor, ids: torch.Tensor, 
     (No reference counterpart: spec decode is disabled for qwen3_5,
     nanovllm/config.py:84.)"""
     last_x, last_parents, accepted = pending if pending is not None else (None, None, None)
-    dev = _check_cuda(x, conv_pool, ids, weight, parents, last_x, last_parents, accepted)
+    idx = _device_of(x, conv_pool, ids, weight, parents, last_x, last_parents, accepted)
     if x.dim() != 3:
         raise ValueError(f"x must be [B, T, C], got {list(x.shape)}")
-    B, T, C = x.shape
-    x = _tree_rows(x, "x", (B, T, C))
-    _conv_pool_ok(conv_pool, C)
+    shape = B, T, C = x.shape
+    x, x_b, x_t = _tree_rows(x, "x", shape)
+    pool_st = _conv_pool_ok(conv_pool, C)
     _bf16(weight, "weight")
     if weight.numel() != 4 * C or weight.shape[-1] != 4 or C % 8:
         raise ValueError(f"weight must be [{C}, 4] (conv width 4) and C a multiple of 8")
-    w = weight.reshape(C, 4).contiguous()
-    ids64 = _tree_ids(ids, B)
+    w = weight if weight.is_contiguous() else weight.contiguous()
+    ids = _tree_ids(ids, B)
     par, p_b = _tree_parents(parents, B, T)
     last = (None, 0, 0, None, 0, None, 0)
     if pending is not None:
         last_T = last_x.shape[1]
-        last_x = _tree_rows(last_x, "pending x", (B, last_T, C))
+        last_x, lx_b, lx_t = _tree_rows(last_x, "pending x", (B, last_T, C))
         last_parents, lp_b = _tree_parents(last_parents, B, last_T)
         accepted = _tree_ids(accepted, B, "accepted")
-        last = (_lib.ptr(last_x), last_x.stride(0), last_x.stride(1), _lib.ptr(last_parents), lp_b,
-                _lib.ptr(accepted), last_T)
-    y = torch.empty(B, T, C, dtype=torch.bfloat16, device=x.device)
-    _call_on(dev, "gdn_conv_tree", _lib.ptr(x), x.stride(0), x.stride(1), _lib.ptr(conv_pool), conv_pool.stride(0),
-             conv_pool.stride(1), conv_pool.shape[0], _lib.ptr(ids64), _lib.ptr(w), _lib.ptr(par), p_b, *last,
-             _lib.ptr(y), B, T, C, _stream(dev))
+        last = (last_x.data_ptr(), lx_b, lx_t, last_parents.data_ptr(), lp_b, accepted.data_ptr(), last_T)
+    y = torch.empty(shape, dtype=torch.bfloat16, device=x.device)
+    _call_on(idx, "gdn_conv_tree", x.data_ptr(), x_b, x_t, conv_pool.data_ptr(), pool_st[0], pool_st[1],
+             conv_pool.shape[0], ids.data_ptr(), w.data_ptr(), par.data_ptr(), p_b, *last, y.data_ptr(), B, T, C)
     return y
 
 
@@ -952,39 +970,41 @@ def recurrent_gdn_tree(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: tor
     (No reference counterpart: spec decode is disabled for qwen3_5,
     nanovllm/config.py:84; one token: qwen3_5.py:575-594.)"""
     last_k, last_g, last_u, last_parents, accepted = pending if pending is not None else (None,) * 5
-    dev = _check_cuda(q, k, v, g, beta, s_pool, ids, parents, last_k, last_g, last_u, last_parents, accepted)
+    idx = _device_of(k, q, v, g, beta, s_pool, ids, parents, last_k, last_g, last_u, last_parents, accepted)
     if k.dim() != 4 or v.dim() != 4:
         raise ValueError(f"q, k, v must be [B, T, heads, D], got {list(k.shape)} and {list(v.shape)}")
-    B, T, Hk, D = k.shape
+    k_shape = B, T, Hk, D = k.shape
     Hv = v.shape[2]
     if Hk == 0 or Hv % Hk:
         raise ValueError(f"{Hv} value heads are no multiple of {Hk} key heads")
-    q, k = _tree_rows(q, "q", (B, T, Hk, D)), _tree_rows(k, "k", (B, T, Hk, D))
-    v = _tree_rows(v, "v", (B, T, Hv, D))
-    g = _tree_f32(g, "g", (B, T, Hv))
+    v_shape, g_shape = (B, T, Hv, D), (B, T, Hv)
+    q, q_b, q_t = _tree_rows(q, "q", k_shape)
+    k, k_b, k_t = _tree_rows(k, "k", k_shape)
+    v, v_b, v_t = _tree_rows(v, "v", v_shape)
+    g = _tree_f32(g, "g", g_shape)
     _bf16(beta, "beta")
-    if beta.shape != (B, T, Hv):
-        raise ValueError(f"beta must be {[B, T, Hv]}, got {list(beta.shape)}")
-    beta = beta.contiguous()
+    if beta.shape != g_shape:
+        raise ValueError(f"beta must be {list(g_shape)}, got {list(beta.shape)}")
+    if not beta.is_contiguous():
+        beta = beta.contiguous()
     _s_pool_ok(s_pool, Hv, D)
-    ids64 = _tree_ids(ids, B)
+    ids = _tree_ids(ids, B)
     par, p_b = _tree_parents(parents, B, T)
     last = (None, 0, 0, None, None, None, 0, None, 0)
     if pending is not None:
         last_T = last_k.shape[1]
-        last_k = _tree_rows(last_k, "pending k", (B, last_T, Hk, D))
+        last_k, lk_b, lk_t = _tree_rows(last_k, "pending k", (B, last_T, Hk, D))
         last_g = _tree_f32(last_g, "pending g", (B, last_T, Hv))
         last_u = _tree_f32(last_u, "pending u", (B, last_T, Hv, D))
         last_parents, lp_b = _tree_parents(last_parents, B, last_T)
         accepted = _tree_ids(accepted, B, "accepted")
-        last = (_lib.ptr(last_k), last_k.stride(0), last_k.stride(1), _lib.ptr(last_g), _lib.ptr(last_u),
-                _lib.ptr(last_parents), lp_b, _lib.ptr(accepted), last_T)
-    o = torch.empty(B, T, Hv, D, dtype=torch.bfloat16, device=v.device)
-    u = torch.empty(B, T, Hv, D, dtype=torch.float32, device=v.device)
-    _call_on(dev, "gdn_rule_tree", _lib.ptr(q), q.stride(0), q.stride(1), _lib.ptr(k), k.stride(0), k.stride(1),
-             _lib.ptr(v), v.stride(0), v.stride(1), _lib.ptr(g), _lib.ptr(beta), _lib.ptr(s_pool), s_pool.stride(0),
-             s_pool.shape[0], _lib.ptr(ids64), _lib.ptr(par), p_b, *last, _lib.ptr(o), _lib.ptr(u), B, T, Hk, Hv, D,
-             float(D ** -0.5), _stream(dev))
+        last = (last_k.data_ptr(), lk_b, lk_t, last_g.data_ptr(), last_u.data_ptr(), last_parents.data_ptr(), lp_b,
+                accepted.data_ptr(), last_T)
+    o = torch.empty(v_shape, dtype=torch.bfloat16, device=v.device)
+    u = torch.empty(v_shape, dtype=torch.float32, device=v.device)
+    _call_on(idx, "gdn_rule_tree", q.data_ptr(), q_b, q_t, k.data_ptr(), k_b, k_t, v.data_ptr(), v_b, v_t,
+             g.data_ptr(), beta.data_ptr(), s_pool.data_ptr(), s_pool.stride(0), s_pool.shape[0], ids.data_ptr(),
+             par.data_ptr(), p_b, *last, o.data_ptr(), u.data_ptr(), B, T, Hk, Hv, D, D ** -0.5)
     return o, u
 
 
@@ -996,26 +1016,27 @@ def commit_tree(s_pool: torch.Tensor, conv_pool: torch.Tensor, ids: torch.Tensor
     three raw rows on its path; -1 (or no used node) leaves both as they are.
     x [B, T, C] the raw rows, k [B, T, Hk, D], g [B, T, Hv], u [B, T, Hv, D] and
     parents those of the verified step."""
-    dev = _check_cuda(s_pool, conv_pool, ids, parents, accepted, x, k, g, u)
+    idx = _device_of(s_pool, conv_pool, ids, parents, accepted, x, k, g, u)
     if k.dim() != 4 or u.dim() != 4 or x.dim() != 3:
         raise ValueError(f"x, k, u must be [B, T, C], [B, T, Hk, D], [B, T, Hv, D], got {list(x.shape)}, "
                          f"{list(k.shape)}, {list(u.shape)}")
-    B, T, Hk, D = k.shape
+    k_shape = B, T, Hk, D = k.shape
     Hv, C = u.shape[2], x.shape[2]
     if Hk == 0 or Hv % Hk:
         raise ValueError(f"{Hv} value heads are no multiple of {Hk} key heads")
-    x, k = _tree_rows(x, "x", (B, T, C)), _tree_rows(k, "k", (B, T, Hk, D))
+    x, x_b, x_t = _tree_rows(x, "x", (B, T, C))
+    k, k_b, k_t = _tree_rows(k, "k", k_shape)
     g, u = _tree_f32(g, "g", (B, T, Hv)), _tree_f32(u, "u", (B, T, Hv, D))
     _s_pool_ok(s_pool, Hv, D)
-    _conv_pool_ok(conv_pool, C)
-    if conv_pool.shape[0] != s_pool.shape[0]:
-        raise ValueError(f"the pools have {s_pool.shape[0]} and {conv_pool.shape[0]} slots")
-    ids64, acc = _tree_ids(ids, B), _tree_ids(accepted, B, "accepted")
+    pool_st = _conv_pool_ok(conv_pool, C)
+    slots = s_pool.shape[0]
+    if conv_pool.shape[0] != slots:
+        raise ValueError(f"the pools have {slots} and {conv_pool.shape[0]} slots")
+    ids, accepted = _tree_ids(ids, B), _tree_ids(accepted, B, "accepted")
     par, p_b = _tree_parents(parents, B, T)
-    _call_on(dev, "gdn_commit_tree", _lib.ptr(s_pool), s_pool.stride(0), _lib.ptr(conv_pool), conv_pool.stride(0),
-             conv_pool.stride(1), s_pool.shape[0], _lib.ptr(ids64), _lib.ptr(par), p_b, _lib.ptr(acc), _lib.ptr(x),
-             x.stride(0), x.stride(1), _lib.ptr(k), k.stride(0), k.stride(1), _lib.ptr(g), _lib.ptr(u), B, T, Hk, Hv,
-             D, C, _stream(dev))
+    _call_on(idx, "gdn_commit_tree", s_pool.data_ptr(), s_pool.stride(0), conv_pool.data_ptr(), pool_st[0], pool_st[1],
+             slots, ids.data_ptr(), par.data_ptr(), p_b, accepted.data_ptr(), x.data_ptr(), x_b, x_t, k.data_ptr(), k_b,
+             k_t, g.data_ptr(), u.data_ptr(), B, T, Hk, Hv, D, C)
 
 
 # ------------------------------------------------------------- projections --
@@ -1124,12 +1145,19 @@ FP8 = torch.float8_e4m3fn
 FP8_GROUP = 128   # values with one scale
 
 
-def _rows_of(x: torch.Tensor, align: int) -> torch.Tensor:
-    """x [..., K] as [M, K] rows that the kernels read in 16-byte pieces."""
-    x2 = x.reshape(-1, x.shape[-1])
-    if x2.stride(1) != 1 or x2.stride(0) % align or x2.stride(0) < x2.shape[1] or x2.data_ptr() % 16:
-        x2 = x2.contiguous() if not x2.is_contiguous() else x2.clone()
-    return x2
+def _rows_of(x: torch.Tensor, align: int):
+    """x [..., K] as [M, K] rows that the kernels read in 16-byte pieces, and their stride."""
+    K = x.shape[-1]
+    if x.is_contiguous():
+        if x.data_ptr() % 16:
+            x = x.clone(memory_format=torch.contiguous_format)
+        return x, x.numel() // K, K
+    x2 = x.reshape(-1, K)
+    st = x2.stride()
+    if st[1] != 1 or st[0] % align or st[0] < K or x2.data_ptr() % 16:
+        x2 = x2.contiguous() if not x2.is_contiguous() else x2.clone(memory_format=torch.contiguous_format)
+        return x2, x2.shape[0], K
+    return x2, x2.shape[0], st[0]
 
 
 def _fp8_scales(M: int, G: int, dev) -> torch.Tensor:
@@ -1143,19 +1171,18 @@ def quantize_fp8(x: torch.Tensor):
     448), 2^-126), and a value is x times the scale's fp32 reciprocal, rounded to
     nearest.  NaN stays NaN without counting in amax; an infinity makes its group's
     scale infinite.  (The scales' memory holds the rows of a group side by side.)"""
-    dev = _check_cuda(x)
+    idx = _device_of(x)
     if x.dtype not in (torch.bfloat16, torch.float32):
         raise TypeError(f"x must be bfloat16 or float32, got {x.dtype}")
     K = x.shape[-1]
-    if x.dim() < 1 or K == 0 or K % FP8_GROUP:
+    if K == 0 or K % FP8_GROUP:
         raise ValueError(f"the last dim must be a positive multiple of {FP8_GROUP}, got {K}")
     f32 = x.dtype == torch.float32
-    x2 = _rows_of(x, 4 if f32 else 8)
-    M = x2.shape[0]
+    rows, M, stride = _rows_of(x, 4 if f32 else 8)
     y = torch.empty(x.shape, dtype=FP8, device=x.device)
     scale = _fp8_scales(M, K // FP8_GROUP, x.device)
-    _call_on(dev, "gdn_quantize_fp8", _lib.ptr(x2), int(f32), x2.stride(0), _lib.ptr(y), K, _lib.ptr(scale),
-             1, M, M, K, 1, _stream(dev))
+    _call_on(idx, "gdn_quantize_fp8", rows.data_ptr(), int(f32), stride, y.data_ptr(), K, scale.data_ptr(), 1, M, M, K,
+             1)
     return y, scale
 
 
@@ -1163,49 +1190,23 @@ def quantize_weight_fp8(weight: torch.Tensor):
     """weight [N, K] bf16 or fp32 (nn.Linear layout, K a multiple of 128) -> (e4m3 [N,
     K], scales [ceil(N / 128), K / 128] fp32), a scale for each 128 x 128 block; once,
     when the weights are loaded.  The rounding is quantize_fp8's."""
-    dev = _check_cuda(weight)
+    idx = _device_of(weight)
     if weight.dtype not in (torch.bfloat16, torch.float32):
         raise TypeError(f"weight must be bfloat16 or float32, got {weight.dtype}")
     if weight.dim() != 2 or weight.shape[1] == 0 or weight.shape[1] % FP8_GROUP:
         raise ValueError(f"weight must be [N, K] with K a positive multiple of {FP8_GROUP}, got {list(weight.shape)}")
     f32 = weight.dtype == torch.float32
-    w = _rows_of(weight, 4 if f32 else 8)
-    N, K = w.shape
-    y = torch.empty(N, K, dtype=FP8, device=w.device)
-    scale = torch.empty(-(-N // FP8_GROUP), K // FP8_GROUP, dtype=torch.float32, device=w.device)
-    _call_on(dev, "gdn_quantize_fp8", _lib.ptr(w), int(f32), w.stride(0), _lib.ptr(y), K, _lib.ptr(scale),
-             K // FP8_GROUP, 1, N, K, FP8_GROUP, _stream(dev))
+    N, K = weight.shape
+    rows, _, stride = _rows_of(weight, 4 if f32 else 8)
+    y = torch.empty(N, K, dtype=FP8, device=weight.device)
+    scale = torch.empty(-(-N // FP8_GROUP), K // FP8_GROUP, dtype=torch.float32, device=weight.device)
+    _call_on(idx, "gdn_quantize_fp8", rows.data_ptr(), int(f32), stride, y.data_ptr(), K, scale.data_ptr(),
+             K // FP8_GROUP, 1, N, K, FP8_GROUP)
     return y, scale
 
 
-def _linear_fp8(x, weight, weight_scale, x_scale, outs, widths):
-    """The product into outs, whose columns are widths wide."""
-    dev = _check_cuda(x, weight, weight_scale, x_scale, *outs)
-    K, N = x.shape[-1], weight.shape[0]
-    G = K // FP8_GROUP
-    w = weight
-    if w.stride(1) != 1 or w.stride(0) % 16 or w.stride(0) < K or w.data_ptr() % 16:
-        w = w.contiguous() if not w.is_contiguous() else w.clone()
-    ws = weight_scale if weight_scale.stride(1) == 1 or G == 1 else weight_scale.contiguous()
-    bf16 = x_scale is None
-    x2 = _rows_of(x, 8 if bf16 else 16)
-    M = x2.shape[0]
-    ws_bytes = _lib.load().gdn_gemm_fp8_workspace_size(M, N, K, 1) if bf16 else 0
-    work = torch.empty(ws_bytes, dtype=torch.uint8, device=x.device) if ws_bytes > 0 else None
-    n, ends, e = len(widths), [], 0
-    for wd in widths:
-        e += wd
-        ends.append(e)
-    c_arr = (ctypes.c_void_p * n)(*[p.data_ptr() for p in outs])
-    ld_arr = (ctypes.c_int64 * n)(*[p.stride(0) if M > 1 else max(p.stride(0), p.shape[1]) for p in outs])
-    end_arr = (ctypes.c_int * n)(*ends)
-    _call_on(dev, "gdn_gemm_fp8", _lib.ptr(x2), int(bf16), x2.stride(0), _lib.ptr(x_scale),
-             0 if bf16 else x_scale.stride(0), 0 if bf16 else x_scale.stride(1), _lib.ptr(w), w.stride(0),
-             _lib.ptr(ws), ws.stride(0) if ws.shape[0] > 1 else G, M, N, K, n, c_arr, ld_arr, end_arr, _lib.ptr(work),
-             ws_bytes, _stream(dev))
-
-
 def _check_fp8(x, weight, weight_scale, x_scale):
+    """The shapes of a product: (M, N, K)."""
     if weight.dtype != FP8 or weight.dim() != 2:
         raise TypeError(f"weight must be float8_e4m3fn [N, K], got {weight.dtype} {list(weight.shape)}")
     N, K = weight.shape
@@ -1213,28 +1214,60 @@ def _check_fp8(x, weight, weight_scale, x_scale):
         raise ValueError(f"x [..., {x.shape[-1]}] and weight [{N}, {K}]: equal last dims, a positive multiple of "
                          f"{FP8_GROUP}")
     G = K // FP8_GROUP
-    if weight_scale.dtype != torch.float32 or tuple(weight_scale.shape) != (-(-N // FP8_GROUP), G):
+    if weight_scale.dtype != torch.float32 or weight_scale.shape != (-(-N // FP8_GROUP), G):
         raise ValueError(f"weight_scale must be float32 {[-(-N // FP8_GROUP), G]}, got {weight_scale.dtype} "
                          f"{list(weight_scale.shape)}")
     M = x.numel() // K
     if x.dtype == FP8:
-        if x_scale is None or x_scale.dtype != torch.float32 or tuple(x_scale.shape) != (M, G):
+        if x_scale is None or x_scale.dtype != torch.float32 or x_scale.shape != (M, G):
             raise ValueError(f"a float8_e4m3fn x needs x_scale float32 {[M, G]}")
     elif x.dtype != torch.bfloat16 or x_scale is not None:
         raise TypeError(f"x must be bfloat16, or float8_e4m3fn with x_scale, got {x.dtype}"
                         + ("" if x_scale is None else " with x_scale"))
+    return M, N, K
+
+
+def _linear_fp8(x, weight, weight_scale, x_scale, M, N, K, outs, widths):
+    """The product into outs, [M, widths[s]] each."""
+    idx = _device_of(x, weight, weight_scale, x_scale, *outs)
+    w, w_st = weight, weight.stride()
+    if w_st[1] != 1 or w_st[0] % 16 or w_st[0] < K or w.data_ptr() % 16:
+        w = w.contiguous() if not w.is_contiguous() else w.clone(memory_format=torch.contiguous_format)
+        w_st = (K, 1)
+    G = K // FP8_GROUP
+    ws = weight_scale if weight_scale.stride(1) == 1 or G == 1 else weight_scale.contiguous()
+    bf16 = x_scale is None
+    x2, _, x_row = _rows_of(x, 8 if bf16 else 16)
+    work, ws_bytes, xs = None, 0, (None, 0, 0)
+    if bf16:
+        ws_bytes = _lib.load().gdn_gemm_fp8_workspace_size(M, N, K, 1)
+        if ws_bytes > 0:
+            work = torch.empty(ws_bytes, dtype=torch.uint8, device=x.device)
+    else:
+        xs = (x_scale.data_ptr(), *x_scale.stride())
+    n = len(widths)
+    if n == 1:
+        y = outs[0]
+        ld = y.stride(0)
+        tables = (ctypes.byref(ctypes.c_void_p(y.data_ptr())), ctypes.byref(ctypes.c_int64(ld if ld >= N else N)),
+                  ctypes.byref(ctypes.c_int(N)))
+    else:
+        ends = [sum(widths[:i + 1]) for i in range(n)]
+        tables = ((ctypes.c_void_p * n)(*[p.data_ptr() for p in outs]), (ctypes.c_int64 * n)(*widths),
+                  (ctypes.c_int * n)(*ends))
+    _call_on(idx, "gdn_gemm_fp8", x2.data_ptr(), int(bf16), x_row, *xs, w.data_ptr(), w_st[0], ws.data_ptr(),
+             ws.stride(0) if N > FP8_GROUP else G, M, N, K, n, *tables, _lib.ptr(work), ws_bytes)
 
 
 def linear_fp8(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor,
                x_scale: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
     """linear(x, weight) with the weight in e4m3 [N, K] and weight_scale [ceil(N / 128),
     K / 128] fp32, one for each 128 x 128 block (quantize_weight_fp8's, or a
-    checkpoint's).  x [..., K] bf16, quantized in the call (quantize_fp8), or e4m3 with
-    its x_scale [M, K / 128] (any strides).  K a multiple of 128.  fp32 accumulation;
-    returns [..., N] bf16 (or writes `out`, a [M, N] view with contiguous rows)."""
-    _check_fp8(x, weight, weight_scale, x_scale)
-    N = weight.shape[0]
-    M = x.numel() // x.shape[-1]
+    checkpoint's).  x [..., K] bf16, quantized in the call (the bits of quantize_fp8 and
+    a call with its result), or e4m3 with its x_scale [M, K / 128] (any strides).  K a
+    multiple of 128.  fp32 accumulation; returns [..., N] bf16 (or writes `out`, a [M, N]
+    view with contiguous rows)."""
+    M, N, K = _check_fp8(x, weight, weight_scale, x_scale)
     if out is None:
         y = torch.empty(M, N, dtype=torch.bfloat16, device=x.device)
     else:
@@ -1242,22 +1275,20 @@ def linear_fp8(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor
         if out.shape != (M, N) or (N > 1 and out.stride(1) != 1) or (M > 1 and out.stride(0) < N):
             raise ValueError(f"out must be a {[M, N]} view with contiguous rows that do not overlap")
         y = out
-    _linear_fp8(x, weight, weight_scale, x_scale, [y], [N])
-    return y.view(*x.shape[:-1], N) if out is None else y
+    _linear_fp8(x, weight, weight_scale, x_scale, M, N, K, (y,), (N,))
+    return y if out is not None or x.dim() == 2 else y.view(*x.shape[:-1], N)
 
 
 def linear_fp8_cols(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor, widths: list[int],
                     x_scale: torch.Tensor | None = None) -> list[torch.Tensor]:
     """linear_fp8 with the output's columns split into len(widths) (1-4) contiguous
     tensors [..., widths[s]], every boundary a multiple of 16 (as linear_cols)."""
-    _check_fp8(x, weight, weight_scale, x_scale)
-    if not 1 <= len(widths) <= 4 or sum(widths) != weight.shape[0] or min(widths) <= 0 \
-            or any(w % 16 for w in widths[:-1]):
-        raise ValueError(f"widths {widths}: 1 to 4 parts of {weight.shape[0]} columns, boundaries at multiples of 16")
-    M = x.numel() // x.shape[-1]
+    M, N, K = _check_fp8(x, weight, weight_scale, x_scale)
+    if not 1 <= len(widths) <= 4 or sum(widths) != N or min(widths) <= 0 or any(w % 16 for w in widths[:-1]):
+        raise ValueError(f"widths {widths}: 1 to 4 parts of {N} columns, boundaries at multiples of 16")
     parts = [torch.empty(M, w, dtype=torch.bfloat16, device=x.device) for w in widths]
-    _linear_fp8(x, weight, weight_scale, x_scale, parts, widths)
-    return [p.view(*x.shape[:-1], p.shape[1]) for p in parts]
+    _linear_fp8(x, weight, weight_scale, x_scale, M, N, K, parts, widths)
+    return parts if x.dim() == 2 else [p.view(*x.shape[:-1], p.shape[1]) for p in parts]
 
 
 # -------------------------------------------------------------- gated norm --
@@ -1316,24 +1347,34 @@ def rms_norm_gated_fp8(hidden_states: torch.Tensor, gate: torch.Tensor, weight: 
     + eps) * w * silu(z) in fp32 over the last dim, then quantize_fp8's groups of 128
     over a token's H * D columns (a multiple of 128), rounded once.  hidden_states / gate
     [..., H, D] bf16.  Returns (e4m3 [..., H, D], scales [tokens, H * D / 128] fp32)."""
-    dev = _check_cuda(hidden_states, gate, weight)
+    idx = _device_of(hidden_states, gate, weight)
     _bf16(hidden_states, "hidden_states")
     _bf16(gate, "gate")
     if hidden_states.dim() < 2 or gate.shape != hidden_states.shape:
         raise ValueError(f"hidden_states and gate must be [..., H, D] alike, got {list(hidden_states.shape)} and "
                          f"{list(gate.shape)}")
     H, D = hidden_states.shape[-2:]
-    w = weight.to(torch.bfloat16).contiguous()
-    if w.numel() != D or H == 0 or H * D % FP8_GROUP:
+    if weight.dtype != torch.bfloat16 or not weight.is_contiguous():
+        weight = weight.to(torch.bfloat16).contiguous()
+    if weight.numel() != D or H == 0 or H * D % FP8_GROUP:
         raise ValueError(f"weight must have {D} values and H * D = {H * D} be a multiple of {FP8_GROUP}")
-    x3, z3 = (t.reshape(-1, H, D) for t in (hidden_states, gate))
-    x3, z3 = (t if t.stride(2) == 1 and t.stride(1) == D and t.stride(0) % 8 == 0 and t.data_ptr() % 16 == 0
-              else t.contiguous() if not t.is_contiguous() else t.clone() for t in (x3, z3))
-    n_tok = x3.shape[0]
+
+    def tokens(t):  # dense heads of a token, in 16-byte pieces
+        if t.is_contiguous():
+            return (t if t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format)), H * D
+        t = t.reshape(-1, H, D)
+        st = t.stride()
+        if st[2] != 1 or st[1] != D or st[0] % 8 or t.data_ptr() % 16:
+            return t.contiguous() if not t.is_contiguous() else t.clone(memory_format=torch.contiguous_format), H * D
+        return t, st[0]
+
+    x, x_tok = tokens(hidden_states)
+    z, z_tok = tokens(gate)
+    n_tok = hidden_states.numel() // (H * D)
     y = torch.empty(hidden_states.shape, dtype=FP8, device=hidden_states.device)
     scale = _fp8_scales(n_tok, H * D // FP8_GROUP, hidden_states.device)
-    _call_on(dev, "gdn_rmsnorm_gated_fp8", _lib.ptr(x3), x3.stride(0), _lib.ptr(z3), z3.stride(0), _lib.ptr(w),
-             _lib.ptr(y), _lib.ptr(scale), 1, n_tok, n_tok, H, D, float(eps), _stream(dev))
+    _call_on(idx, "gdn_rmsnorm_gated_fp8", x.data_ptr(), x_tok, z.data_ptr(), z_tok, weight.data_ptr(), y.data_ptr(),
+             scale.data_ptr(), 1, n_tok, n_tok, H, D, float(eps))
     return y, scale
 
 

@@ -18,9 +18,8 @@ def ops(pkg, monkeypatch):
     def fake_call(*a, **k):
         raise Launched()
 
-    monkeypatch.setattr(pkg.ops, "_check_cuda", lambda *ts: torch.device("cpu"))
-    monkeypatch.setattr(pkg.ops, "_stream", lambda dev: 0)
-    monkeypatch.setattr(pkg.ops._lib, "call", fake_call)
+    monkeypatch.setattr(pkg.ops, "_device_of", lambda *ts: 0)
+    monkeypatch.setattr(pkg.ops, "_call_on", fake_call)
     return pkg.ops
 
 
