@@ -377,21 +377,32 @@ __device__ __forceinline__ void find_path(const PathIn& in, int T, int lane, Pat
 template <int D, int TM>
 __device__ __forceinline__ void stage_path(const RulePending& pd, const Path& path, int b, int h, int kh, int Hv,
                                            int wave, int waves, int lane, float (&wk)[TM][D], float (&u)[TM][D]) {
+  typedef uint16_t halves __attribute__((ext_vector_type(D / 64)));
+  typedef float floats __attribute__((ext_vector_type(D / 64)));
   constexpr int E = D / 64;
-  for (int p = wave; p < path.count; p += waves) {
-    const int s = path.node[p];
-    const uint16_t* kr = pd.k + b * pd.k_b + s * pd.k_t + kh * D + lane * E;
-    const float* ur = pd.u + ((static_cast<int64_t>(b) * pd.T + s) * Hv + h) * D + lane * E;
-    float v[E], ss = 0.0f;
+  for (int p0 = wave; p0 < path.count; p0 += 4 * waves) {
+    halves kr[4];
+    floats ur[4];
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-      u[p][lane * E + e] = ur[e];
-      v[e] = gdn::bf2f(kr[e]);
-      ss += v[e] * v[e];
+    for (int i = 0; i < 4; ++i) {
+      const int s = path.node[min(p0 + i * waves, path.count - 1)];
+      kr[i] = *reinterpret_cast<const halves*>(pd.k + b * pd.k_b + s * pd.k_t + kh * D + lane * E);
+      ur[i] = *reinterpret_cast<const floats*>(pd.u + ((static_cast<int64_t>(b) * pd.T + s) * Hv + h) * D + lane * E);
     }
-    const float r = path.weight[p] * rsqrtf(gdn::wave_sum(ss) + kEps);
 #pragma unroll
-    for (int e = 0; e < E; ++e) wk[p][lane * E + e] = v[e] * r;
+    for (int i = 0; i < 4; ++i) {
+      const int p = p0 + i * waves;
+      if (p >= path.count) break;
+      floats v;
+      float ss = 0.0f;
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        v[e] = gdn::bf2f(kr[i][e]);
+        ss = fmaf(v[e], v[e], ss);
+      }
+      *reinterpret_cast<floats*>(&u[p][lane * E]) = ur[i];
+      *reinterpret_cast<floats*>(&wk[p][lane * E]) = v * (path.weight[p] * rsqrtf(gdn::wave_sum(ss) + kEps));
+    }
   }
 }
 
@@ -429,7 +440,7 @@ __device__ __forceinline__ void add_block(float (&a)[N], float f, const float (&
 
 // NT: 16-node tiles of the tree (and of the pending one).
 template <int D, int NT>
-__global__ __launch_bounds__(2 * D, NT == 1 ? 4 : 2) void rule_tree_kernel(
+__global__ __launch_bounds__(2 * D, NT == 1 ? 4 : NT == 2 ? 3 : NT == 3 ? 2 : 1) void rule_tree_kernel(
     const uint16_t* __restrict__ q, int64_t q_b, int64_t q_t, const uint16_t* __restrict__ k, int64_t k_b, int64_t k_t,
     const uint16_t* __restrict__ v, int64_t v_b, int64_t v_t, const float* __restrict__ g,
     const uint16_t* __restrict__ beta, float* __restrict__ pool, int64_t s_slot, int64_t n_slots,
@@ -466,18 +477,27 @@ __global__ __launch_bounds__(2 * D, NT == 1 ? 4 : 2) void rule_tree_kernel(
   // state, which is then on its way while they are worked on.
   const uint16_t* kb = k + b * k_b + kh * D + 8 * lg;
   const uint16_t* qb = q + b * q_b + kh * D + 8 * lg;
-  auto k_frag = [&](int I, int kk) { return row_frag(kb + min(16 * I + lr, T - 1) * k_t + 32 * kk); };
-  auto q_frag = [&](int I, int kk) { return row_frag(qb + min(16 * I + lr, T - 1) * q_t + 32 * kk); };
-  constexpr bool kHold = NT == 1;  // the nodes' rows, for their norms and products with each other
-  gdn::s16x8_t fk[kHold ? NT : 1][KK], fq[kHold ? NT : 1][KK];
-  if constexpr (kHold) {
+  auto row_of = [&](int I) { return min(16 * I + lr, T - 1); };
+  // the wave's units (I, k or q): the 16 nodes' rows of tile I, for their norms and, against
+  // the keys of tiles J <= I, their products.  From the last wave on: the first two have the
+  // trees to follow.
+  constexpr int kUnits = 2 * NT, UW = (kUnits + NW - 1) / NW;
+  auto unit = [&](int j) { return (NW - 1 - wave) + j * NW; };
+  gdn::s16x8_t fr[UW][KK], fc[NT][KK];
 #pragma unroll
-    for (int I = 0; I < NT; ++I)
+  for (int j = 0; j < UW; ++j) {
+    if (unit(j) >= kUnits) break;
+    const uint16_t* p = unit(j) & 1 ? qb + row_of(unit(j) >> 1) * q_t : kb + row_of(unit(j) >> 1) * k_t;
 #pragma unroll
-      for (int kk = 0; kk < KK; ++kk) {
-        fk[I][kk] = k_frag(I, kk);
-        fq[I][kk] = q_frag(I, kk);
-      }
+    for (int kk = 0; kk < KK; ++kk) fr[j][kk] = row_frag(p + 32 * kk);
+  }
+#pragma unroll
+  for (int J = 0; J < NT; ++J) {
+    // (up to the tile of the wave's last unit)
+    if (unit(0) >= kUnits || 2 * J > unit(unit(UW - 1) < kUnits ? UW - 1 : 0) || 16 * J >= T) break;
+    const uint16_t* p = kb + row_of(J) * k_t;
+#pragma unroll
+    for (int kk = 0; kk < KK; ++kk) fc[J][kk] = row_frag(p + 32 * kk);
   }
   int my_parent = 0;
   float my_g = 0.0f, my_beta = 0.0f;
@@ -523,29 +543,20 @@ __global__ __launch_bounds__(2 * D, NT == 1 ? 4 : 2) void rule_tree_kernel(
     find_path(pin, pd.T, lane, path);
   }
 #pragma unroll
-  for (int I = 0; I < NT; ++I) {
+  for (int j = 0; j < UW; ++j) {
     // row 16 I + lr: the lane's 8 values of every 32, then the four lanes of the row
-    if (16 * I >= T || I % NW != wave) continue;
-    float sk = 0.0f, sq = 0.0f;
+    if (unit(j) >= kUnits) break;
+    float ss = 0.0f;
 #pragma unroll
-    for (int kk = 0; kk < KK; ++kk) {
-      const gdn::s16x8_t x = kHold ? fk[kHold ? I : 0][kk] : k_frag(I, kk);
-      const gdn::s16x8_t y = kHold ? fq[kHold ? I : 0][kk] : q_frag(I, kk);
+    for (int kk = 0; kk < KK; ++kk)
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const float a = gdn::bf2f(static_cast<uint16_t>(x[e])), c = gdn::bf2f(static_cast<uint16_t>(y[e]));
-        sk = fmaf(a, a, sk);
-        sq = fmaf(c, c, sq);
+        const float x = gdn::bf2f(static_cast<uint16_t>(fr[j][kk][e]));
+        ss = fmaf(x, x, ss);
       }
-    }
-    sk += __shfl_xor(sk, 16, 64);
-    sq += __shfl_xor(sq, 16, 64);
-    sk += __shfl_xor(sk, 32, 64);
-    sq += __shfl_xor(sq, 32, 64);
-    if (lg == 0) {
-      rk[16 * I + lr] = rsqrtf(sk + kEps);
-      rq[16 * I + lr] = rsqrtf(sq + kEps);
-    }
+    ss += __shfl_xor(ss, 16, 64);
+    ss += __shfl_xor(ss, 32, 64);
+    if (lg == 0) (unit(j) & 1 ? rq : rk)[16 * (unit(j) >> 1) + lr] = rsqrtf(ss + kEps);
   }
   gdn::lds_barrier();
   const bool pending = pd.accepted && path.count > 0;  // (the whole workgroup)
@@ -556,37 +567,34 @@ __global__ __launch_bounds__(2 * D, NT == 1 ? 4 : 2) void rule_tree_kernel(
   // + r, s = 16 J + lr.  A weight of 0 is not multiplied: nothing of an unused node, of
   // another branch or past T gets in.
 #pragma unroll
-  for (int it = 0; it < NT * (NT + 1); ++it) {
-    const int type = it & 1;
-    int I = 0, J = it >> 1;
-    while (J > I) J -= ++I;
-    if (16 * I >= T || it % NW != wave) continue;
-    gdn::f32x4_t c = {0.f, 0.f, 0.f, 0.f};
+  for (int j = 0; j < UW; ++j) {
+    const int I = unit(j) >> 1, type = unit(j) & 1;
+    if (unit(j) >= kUnits || 16 * I >= T) break;
 #pragma unroll
-    for (int kk = 0; kk < KK; ++kk) {
-      if constexpr (kHold)
-        c = gdn::mfma16x16x32(type ? fq[I][kk] : fk[I][kk], fk[J][kk], c);
-      else
-        c = gdn::mfma16x16x32(type ? q_frag(I, kk) : k_frag(I, kk), k_frag(J, kk), c);
-    }
-    const int s = 16 * J + lr;
-    const float rs = rk[s];
-    bool some = false;
+    for (int J = 0; J < NT; ++J) {
+      if (J > I) break;
+      gdn::f32x4_t c = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int t = 16 * I + 4 * lg + r;
-      const float w = wt[t][s];
-      if (type) {
-        co[t][s] = w != 0.0f ? (scale * rq[t]) * (rs * w) * c[r] : 0.0f;
-      } else {
-        const bool on = w != 0.0f && s < t;
-        cu[t][s] = on ? (bt[t] * rk[t]) * (rs * w) * c[r] : 0.0f;
-        some |= on;
+      for (int kk = 0; kk < KK; ++kk) c = gdn::mfma16x16x32(fr[j][kk], fc[J][kk], c);
+      const int s = 16 * J + lr;
+      const float rs = rk[s];
+      bool some = false;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int t = 16 * I + 4 * lg + r;
+        const float w = wt[t][s];
+        if (type) {
+          co[t][s] = w != 0.0f ? (scale * rq[t]) * (rs * w) * c[r] : 0.0f;
+        } else {
+          const bool on = w != 0.0f && s < t;
+          cu[t][s] = on ? (bt[t] * rk[t]) * (rs * w) * c[r] : 0.0f;
+          some |= on;
+        }
       }
-    }
-    if (!type) {
-      some = __any(some);
-      if (lane == 0) any_cu[I][J] = some;
+      if (!type) {
+        some = __any(some);
+        if (lane == 0) any_cu[I][J] = some;
+      }
     }
   }
 
@@ -601,6 +609,10 @@ __global__ __launch_bounds__(2 * D, NT == 1 ? 4 : 2) void rule_tree_kernel(
   for (int I = 0; I < NT; ++I)
 #pragma unroll
     for (int c = 0; c < 2; ++c) ak[I][c] = aq[I][c] = gdn::f32x4_t{0.f, 0.f, 0.f, 0.f};
+  // (the nodes' rows come again, from the caches, one product ahead: held in registers from
+  // the start they would cost a workgroup per CU)
+  const int tiles = (T + 15) / 16;
+  gdn::s16x8_t nk = row_frag(kb + row_of(0) * k_t), nq = row_frag(qb + row_of(0) * q_t);
 #pragma unroll
   for (int kk = 0; kk < KK; ++kk) {
     typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
@@ -617,9 +629,13 @@ __global__ __launch_bounds__(2 * D, NT == 1 ? 4 : 2) void rule_tree_kernel(
       }
 #pragma unroll
     for (int I = 0; I < NT; ++I) {
-      if (16 * I >= T) break;
-      // (again from the caches: in registers they would cost a workgroup per CU)
-      const gdn::s16x8_t x = k_frag(I, kk), y = q_frag(I, kk);
+      if (I >= tiles) break;
+      const gdn::s16x8_t x = nk, y = nq;
+      const int In = I + 1 < tiles && I + 1 < NT ? I + 1 : 0, kn = In ? kk : kk + 1;
+      if (kn < KK) {
+        nk = row_frag(kb + row_of(In) * k_t + 32 * kn);
+        nq = row_frag(qb + row_of(In) * q_t + 32 * kn);
+      }
 #pragma unroll
       for (int n = 2; n >= 0; --n)  // (the smallest terms first)
 #pragma unroll
