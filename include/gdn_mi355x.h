@@ -497,7 +497,8 @@ int gdn_rmsnorm_gated_fp8(const uint16_t* x, int64_t sx_tok, const uint16_t* z, 
  *
  * gdn_conv_tree: y[b][t] = silu(w[3] x[t] + w[2] x[p] + w[1] x[pp] + w[0] x[ppp]), p, pp,
  * ppp the ancestors, past the root the pool's taps from the newest: gdn_conv_decode's
- * arithmetic along each path.  x [B, T, C] bf16 strides x_b, x_t (multiples of 8), pool as
+ * arithmetic along each path.  x [B, T, C] bf16 strides x_b, x_t (multiples of 8, x_t
+ * below 2^24), pool as
  * gdn_conv_decode, w [C, 4], y [B, T, C] contiguous; last_x like x with last_T nodes.
  */
 int gdn_conv_tree(const uint16_t* x, int64_t x_b, int64_t x_t, uint16_t* pool, int64_t sp_slot, int64_t sp_ch,
@@ -514,7 +515,7 @@ int gdn_conv_tree(const uint16_t* x, int64_t x_b, int64_t x_t, uint16_t* pool, i
  * The state after a node is W S + sum of w k u^T over its path; it is formed for the
  * accepted node only, from k, g and u (which the caller keeps until then).
  *   q, k [B, T, Hk, D], v [B, T, Hv, D] bf16, strides per sequence and token (multiples of
- *   8, head stride D); g [B, T, Hv] fp32 and beta [B, T, Hv] bf16 contiguous; s_pool, s_slot
+ *   8, the token's below 2^24; head stride D); g [B, T, Hv] fp32 and beta [B, T, Hv] bf16 contiguous; s_pool, s_slot
  *   as gdn_recurrent; o [B, T, Hv, D] bf16 and u [B, T, Hv, D] fp32 contiguous; last_k,
  *   last_g, last_u: k, g and u of the step before (last_T nodes).  D 64 or 128.
  */

@@ -15,8 +15,6 @@
 // form (gdn_recurrent) writes one D x D state per token, and a commit forms one state
 // from the path's k, g and u.  The weights are products of factors in [0, 1], never
 // differences of sums: no cancellation, and a decay of 0 stays 0.
-#include <algorithm>
-
 #include "gdn_common.h"
 
 namespace {
@@ -274,11 +272,31 @@ __global__ __launch_bounds__(64) void conv_tree_kernel(const uint16_t* __restric
 // up to it exactly (8 bits of the significand each), k and q are not normalised before
 // (their norms scale the results), so the products are those of fp32 operands.
 //
+// The corrections u of 16 nodes are the product of the inverse of their 16 x 16 triangle
+// (found by substitution while the state is on its way) with what the state, v and the
+// nodes of earlier tiles give, and o adds the products of the second coefficients with u:
+// fp32 products of 16 x 16 x 4, in which a lane's results are its part of the next
+// operand (register r of lane group lg: node 4 lg + r), so that nothing goes through LDS.
+//
 // What bounds it: the state's way in (and out, where a path is pending).  The tree's
 // weights, the nodes' norms and dot products (on the matrix cores as well) and the
 // pending path's rows are worked on while the state is on its way.
 typedef float f32x2_t __attribute__((ext_vector_type(2)));
 constexpr float kEps = 1e-6f;
+constexpr int kPathRows = 16;  // of a pending path in LDS at a time
+
+// Rows and tiles move through buffer loads and stores: the base, which the workgroup
+// shares, in the descriptor, the lane's offset in one register, the rest in the
+// instruction, so that no address pairs sit in the registers beside the state.  The range
+// is left open: the offsets stay inside of the arrays.
+typedef __amdgpu_buffer_rsrc_t buf_t;
+constexpr int kNT = 2;  // cache policy: non-temporal
+__device__ __forceinline__ buf_t buf_of(const void* base) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), static_cast<short>(0), 0x7fffffff, 0x00020000);
+}
+__device__ __forceinline__ gdn::s16x8_t buf_row(buf_t r, int voff) {
+  return __builtin_bit_cast(gdn::s16x8_t, __builtin_amdgcn_raw_buffer_load_b128(r, voff, 0, 0));
+}
 
 __device__ __forceinline__ void wave_lds_order() {
   __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront", "local");
@@ -291,28 +309,37 @@ template <int D>
 struct Tile {
   f32x2_t s[D / 32][8];
 
-  __device__ __forceinline__ void load(const float* p) {  // p: the lane's first row and column
+  // r: the tile; voff: byte offset of the lane's first row and column
+  __device__ __forceinline__ void load(buf_t r, int voff) {
 #pragma unroll
     for (int kk = 0; kk < D / 32; ++kk)
 #pragma unroll
       for (int e = 0; e < 8; ++e)
-        s[kk][e] = __builtin_nontemporal_load(reinterpret_cast<const f32x2_t*>(p + (32 * kk + e) * D));
+        s[kk][e] = __builtin_bit_cast(
+            f32x2_t, __builtin_amdgcn_raw_buffer_load_b64(r, voff + e * D * 4, 32 * kk * D * 4, kNT));
   }
-  __device__ __forceinline__ void store(float* p) const {
+  __device__ __forceinline__ void store(buf_t r, int voff) const {
+    typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+    // (a region of its own: nothing overwrites a register whose store is being issued)
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int kk = 0; kk < D / 32; ++kk)
 #pragma unroll
       for (int e = 0; e < 8; ++e)
-        __builtin_nontemporal_store(s[kk][e], reinterpret_cast<f32x2_t*>(p + (32 * kk + e) * D));
+        __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u32x2, s[kk][e]), r, voff + e * D * 4,
+                                              32 * kk * D * 4, kNT);
+    asm volatile("s_nop 1");
+    __builtin_amdgcn_sched_barrier(0);
   }
-  // S <- total S + sum over the path of (w k)[row] u[column], both from LDS rows
-  template <int TM>
-  __device__ __forceinline__ void advance(float total, int count, const float (&wk)[TM][D], const float (&u)[TM][D],
-                                          int wave, int lr, int lg) {
+  __device__ __forceinline__ void scale(float total) {
 #pragma unroll
     for (int kk = 0; kk < D / 32; ++kk)
 #pragma unroll
       for (int e = 0; e < 8; ++e) s[kk][e] *= total;
+  }
+  // S += sum over count nodes of (w k)[row] u[column], both from LDS rows
+  __device__ __forceinline__ void advance(int count, const float (&wk)[kPathRows][D], const float (&u)[kPathRows][D],
+                                          int wave, int lr, int lg) {
     for (int p = 0; p < count; ++p) {
       const f32x2_t c = *reinterpret_cast<const f32x2_t*>(&u[p][32 * wave + 2 * lr]);
 #pragma unroll
@@ -333,16 +360,15 @@ struct Tile {
 // A pending path in LDS: its nodes from the accepted one up to the root, the weight of
 // each one's correction and that of the state.
 struct Path {
-  int raw[kMaxNodes], link[kMaxNodes];
   int node[kMaxNodes];
   float weight[kMaxNodes];
-  float dec[kMaxNodes];
   float total;
   int count;  // 0: nothing was accepted
 };
 
-// By one wave: the links and decays of the pending tree, then the walk.  What it reads
-// comes as PathIn, so that it can be asked for ahead of the state.
+// By one wave, lane t with node t's parent and decay: the walk from the accepted node up,
+// lane by lane in scalar registers.  What it reads comes as PathIn, so that it can be asked
+// for ahead of the state.
 struct PathIn {
   int64_t want;
   float g;
@@ -355,44 +381,59 @@ struct PathIn {
     parent = pd.parents[b * pd.p_b + t];
   }
 };
+__device__ __forceinline__ float lane_f(float v, int lane) {
+  return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), lane));
+}
 __device__ __forceinline__ void find_path(const PathIn& in, int T, int lane, Path& path) {
-  path.dec[lane] = expf(in.g);
-  tree_links(in.parent, T, lane, path.raw, path.link);
-  wave_lds_order();
-  if (lane == 0) {
-    float w = 1.0f;
-    int n = 0;
-    for (int s = accepted_node(in.want, T, path.link); s >= 0; s = path.link[s]) {
-      path.node[n] = s;
-      path.weight[n++] = w;
-      w *= path.dec[s];
+  const float dec = expf(in.g);
+  int s = in.want >= 0 && in.want < T ? __builtin_amdgcn_readfirstlane(static_cast<int>(in.want)) : -1;
+  int n = 0, node = 0;
+  float w = 1.0f, weight = 0.0f;
+  bool fine = s >= 0;
+  while (s >= 0) {
+    if (lane == n) {
+      node = s;
+      weight = w;
     }
+    ++n;
+    w *= lane_f(dec, s);
+    const int p = __builtin_amdgcn_readlane(in.parent, s);
+    fine = p >= -1 && p < s;  // (so that the walk ends; else node s is unused, and what follows it)
+    s = fine ? p : -1;
+  }
+  if (lane < n) {
+    path.node[lane] = node;
+    path.weight[lane] = weight;
+  }
+  if (lane == 0) {
     path.total = w;
-    path.count = n;
+    path.count = fine ? n : 0;
   }
 }
 
-// The path's rows into LDS, a wave per node: its normalised key times its weight, and its
-// correction.
-template <int D, int TM>
-__device__ __forceinline__ void stage_path(const RulePending& pd, const Path& path, int b, int h, int kh, int Hv,
-                                           int wave, int waves, int lane, float (&wk)[TM][D], float (&u)[TM][D]) {
+// Up to 16 rows of the path from the p0-th on into LDS, a wave per node: its normalised key
+// times its weight, and its correction.
+template <int D>
+__device__ __forceinline__ void stage_path(const RulePending& pd, const Path& path, int first, int b, int h, int kh,
+                                           int Hv, int wave, int waves, int lane, float (&wk)[kPathRows][D],
+                                           float (&u)[kPathRows][D]) {
   typedef uint16_t halves __attribute__((ext_vector_type(D / 64)));
   typedef float floats __attribute__((ext_vector_type(D / 64)));
   constexpr int E = D / 64;
-  for (int p0 = wave; p0 < path.count; p0 += 4 * waves) {
+  const int rows = min(path.count - first, kPathRows);
+  for (int p0 = wave; p0 < rows; p0 += 4 * waves) {
     halves kr[4];
     floats ur[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const int s = path.node[min(p0 + i * waves, path.count - 1)];
+      const int s = path.node[first + min(p0 + i * waves, rows - 1)];
       kr[i] = *reinterpret_cast<const halves*>(pd.k + b * pd.k_b + s * pd.k_t + kh * D + lane * E);
       ur[i] = *reinterpret_cast<const floats*>(pd.u + ((static_cast<int64_t>(b) * pd.T + s) * Hv + h) * D + lane * E);
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int p = p0 + i * waves;
-      if (p >= path.count) break;
+      if (p >= rows) break;
       floats v;
       float ss = 0.0f;
 #pragma unroll
@@ -401,7 +442,7 @@ __device__ __forceinline__ void stage_path(const RulePending& pd, const Path& pa
         ss = fmaf(v[e], v[e], ss);
       }
       *reinterpret_cast<floats*>(&u[p][lane * E]) = ur[i];
-      *reinterpret_cast<floats*>(&wk[p][lane * E]) = v * (path.weight[p] * rsqrtf(gdn::wave_sum(ss) + kEps));
+      *reinterpret_cast<floats*>(&wk[p][lane * E]) = v * (path.weight[first + p] * rsqrtf(gdn::wave_sum(ss) + kEps));
     }
   }
 }
@@ -418,43 +459,37 @@ __device__ __forceinline__ void split3(float a, float b, uint32_t& hi, uint32_t&
   lo = __builtin_amdgcn_perm(__float_as_uint(sb), __float_as_uint(sa), 0x07060302u);
 }
 
-__device__ __forceinline__ gdn::s16x8_t row_frag(const uint16_t* p) { return *reinterpret_cast<const gdn::s16x8_t*>(p); }
-
 __device__ __forceinline__ bool finite(float x) { return fabsf(x) <= 3.4028234664e38f; }
 
-// a[i] += f * sum over s of c[i][s] us[s], 16 x 16 coefficients from LDS rows
-template <int TM, int N>
-__device__ __forceinline__ void add_block(float (&a)[N], float f, const float (&c)[TM][TM], int t0, int s0,
-                                          const float (&us)[16]) {
+// c += a b, 16 x 16 x 16 in fp32: a the lane's row lr, columns 4 lg .. + 3; b and c in the
+// results' layout (register r of lane (lr, lg): row 4 lg + r, column lr).
+__device__ __forceinline__ gdn::f32x4_t mul16(const gdn::f32x4_t& a, const gdn::f32x4_t& b, gdn::f32x4_t c) {
 #pragma unroll
-  for (int i = 0; i < N; ++i)
-#pragma unroll
-    for (int p = 0; p < 4; ++p) {
-      const float4 r = *reinterpret_cast<const float4*>(&c[t0 + i][s0 + 4 * p]);
-      a[i] = fmaf(f * r.x, us[4 * p], a[i]);
-      a[i] = fmaf(f * r.y, us[4 * p + 1], a[i]);
-      a[i] = fmaf(f * r.z, us[4 * p + 2], a[i]);
-      a[i] = fmaf(f * r.w, us[4 * p + 3], a[i]);
-    }
+  for (int r = 0; r < 4; ++r) c = gdn::mfma16x16x4f32(a[r], b[r], c);
+  return c;
 }
 
-// NT: 16-node tiles of the tree (and of the pending one).
+__device__ __forceinline__ const gdn::f32x4_t& four(const float* p) { return *reinterpret_cast<const gdn::f32x4_t*>(p); }
+
+// NT: 16-node tiles of the tree.
 template <int D, int NT>
-__global__ __launch_bounds__(2 * D, NT == 1 ? 4 : NT == 2 ? 3 : NT == 3 ? 2 : 1) void rule_tree_kernel(
+__global__ __launch_bounds__(2 * D, NT <= 2 ? 3 : NT == 3 || D == 128 ? 2 : 1) void rule_tree_kernel(
     const uint16_t* __restrict__ q, int64_t q_b, int64_t q_t, const uint16_t* __restrict__ k, int64_t k_b, int64_t k_t,
     const uint16_t* __restrict__ v, int64_t v_b, int64_t v_t, const float* __restrict__ g,
     const uint16_t* __restrict__ beta, float* __restrict__ pool, int64_t s_slot, int64_t n_slots,
     const int64_t* __restrict__ ids, const int32_t* __restrict__ parents, int64_t p_b, RulePending pd,
     uint16_t* __restrict__ o, float* __restrict__ u, int B, int T, int Hk, int Hv, float scale) {
   constexpr int NW = D / 32, KK = D / 32, TM = 16 * NT;
-  __shared__ __align__(16) float wt[TM][TM];   // weights w(t, s)
-  __shared__ __align__(16) float cu[TM][TM];   // coefficients of u_s in u_t
-  __shared__ __align__(16) float co[TM][TM];   // and in o_t
-  __shared__ __align__(16) float xk[TM][D];    // the pending path's keys; S^T k; u
-  __shared__ __align__(16) float xq[TM][D];    // the pending path's corrections; S^T q
-  __shared__ int raw[kMaxNodes], link[kMaxNodes];
-  __shared__ float dec[TM], total[TM], bt[TM], rk[TM], rq[TM];
-  __shared__ int any_cu[NT][NT];               // whether a tile of coefficients holds an ancestor
+  __shared__ __align__(16) float wt[TM][TM];    // weights w(t, s)
+  __shared__ __align__(16) float cu[TM][TM];    // minus the coefficients of u_s in u_t
+  __shared__ __align__(16) float co[TM][TM];    // the coefficients of u_s in o_t
+  __shared__ __align__(16) float inv[TM][16];   // the inverses of the 16-node triangles
+  __shared__ __align__(16) float xk[kPathRows][D];  // the pending path's keys
+  __shared__ __align__(16) float xq[kPathRows][D];  // and corrections (and see the end)
+  __shared__ __align__(16) int link[TM];
+  __shared__ __align__(16) float bt[TM], total[TM], rk[TM], rq[TM];
+  __shared__ __align__(16) float fv[TM], fk[TM], fq[TM];  // factors of v, S^T k, S^T q: 0 for an unused node
+  __shared__ int any_cu[NT][NT];                // whether a tile of coefficients holds an ancestor
   __shared__ Path path;
 
   const int64_t wi = gdn::xcd_remap(blockIdx.x, static_cast<int64_t>(B) * Hv);
@@ -463,6 +498,7 @@ __global__ __launch_bounds__(2 * D, NT == 1 ? 4 : NT == 2 ? 3 : NT == 3 ? 2 : 1)
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int lr = lane & 15, lg = lane >> 4;
+  const int col = 32 * wave + 2 * lr;                            // the lane's columns col, col + 1
   const int64_t out_t = static_cast<int64_t>(Hv) * D;
   const int64_t out0 = static_cast<int64_t>(b) * T * out_t + h * D;  // row t at out0 + t out_t
   const int64_t slot = ids[b];
@@ -475,30 +511,12 @@ __global__ __launch_bounds__(2 * D, NT == 1 ? 4 : NT == 2 ? 3 : NT == 3 ? 2 : 1)
   }
   // Loads return in order: what the tree and the coefficients need goes out ahead of the
   // state, which is then on its way while they are worked on.
-  const uint16_t* kb = k + b * k_b + kh * D + 8 * lg;
-  const uint16_t* qb = q + b * q_b + kh * D + 8 * lg;
-  auto row_of = [&](int I) { return min(16 * I + lr, T - 1); };
-  // the wave's units (I, k or q): the 16 nodes' rows of tile I, for their norms and, against
-  // the keys of tiles J <= I, their products.  From the last wave on: the first two have the
-  // trees to follow.
-  constexpr int kUnits = 2 * NT, UW = (kUnits + NW - 1) / NW;
-  auto unit = [&](int j) { return (NW - 1 - wave) + j * NW; };
-  gdn::s16x8_t fr[UW][KK], fc[NT][KK];
-#pragma unroll
-  for (int j = 0; j < UW; ++j) {
-    if (unit(j) >= kUnits) break;
-    const uint16_t* p = unit(j) & 1 ? qb + row_of(unit(j) >> 1) * q_t : kb + row_of(unit(j) >> 1) * k_t;
-#pragma unroll
-    for (int kk = 0; kk < KK; ++kk) fr[j][kk] = row_frag(p + 32 * kk);
-  }
-#pragma unroll
-  for (int J = 0; J < NT; ++J) {
-    // (up to the tile of the wave's last unit)
-    if (unit(0) >= kUnits || 2 * J > unit(unit(UW - 1) < kUnits ? UW - 1 : 0) || 16 * J >= T) break;
-    const uint16_t* p = kb + row_of(J) * k_t;
-#pragma unroll
-    for (int kk = 0; kk < KK; ++kk) fc[J][kk] = row_frag(p + 32 * kk);
-  }
+  const buf_t bk = buf_of(k + b * k_b + kh * D), bq = buf_of(q + b * q_b + kh * D);
+  const buf_t bv = buf_of(v + b * v_b + static_cast<int64_t>(h) * D);
+  const int k_row = static_cast<int>(k_t) * 2, q_row = static_cast<int>(q_t) * 2, v_row = static_cast<int>(v_t) * 2;
+  // the lane's 8 values of every 32 of node 16 I + lr
+  auto k_frag = [&](int I, int kk) { return buf_row(bk, min(16 * I + lr, T - 1) * k_row + 16 * lg + 64 * kk); };
+  auto q_frag = [&](int I, int kk) { return buf_row(bq, min(16 * I + lr, T - 1) * q_row + 16 * lg + 64 * kk); };
   int my_parent = 0;
   float my_g = 0.0f, my_beta = 0.0f;
   PathIn pin = {-1, 0.0f, 0};
@@ -510,33 +528,60 @@ __global__ __launch_bounds__(2 * D, NT == 1 ? 4 : NT == 2 ? 3 : NT == 3 ? 2 : 1)
   } else if (wave == 1 && pd.accepted) {
     pin.load(pd, b, h, Hv, lane);
   }
-  gdn::keep_loads_here();
-  float* S0 = pool + slot * s_slot + static_cast<int64_t>(h) * D * D + 8 * lg * D + 32 * wave + 2 * lr;
-  Tile<D> S;
-  S.load(S0);
-  const uint16_t* vb = v + b * v_b + static_cast<int64_t>(h) * D + tid;  // (threads below D)
-  uint16_t vv[16];
-  auto load_v = [&](int I) {
+  // the wave's units (I, k or q): the 16 nodes' rows of tile I, for their norms and, against
+  // the keys of tiles J <= I, their products.  From the last wave on: the first two have the
+  // trees to follow.
+  constexpr int kUnits = 2 * NT, UW = (kUnits + NW - 1) / NW;
+  auto unit = [&](int j) { return (NW - 1 - wave) + j * NW; };
+  gdn::s16x8_t fr[UW][KK], fc[NT][KK];
 #pragma unroll
-    for (int i = 0; i < 16; ++i) vv[i] = vb[min(16 * I + i, T - 1) * v_t];
-  };
+  for (int j = 0; j < UW; ++j) {
+    if (unit(j) >= kUnits) break;
+#pragma unroll
+    for (int kk = 0; kk < KK; ++kk) fr[j][kk] = unit(j) & 1 ? q_frag(unit(j) >> 1, kk) : k_frag(unit(j) >> 1, kk);
+  }
+#pragma unroll
+  for (int J = 0; J < NT; ++J) {
+    // (up to the tile of the wave's last unit)
+    if (unit(0) >= kUnits || 2 * J > unit(unit(UW - 1) < kUnits ? UW - 1 : 0) || 16 * J >= T) break;
+#pragma unroll
+    for (int kk = 0; kk < KK; ++kk) fc[J][kk] = k_frag(J, kk);
+  }
+  uint32_t vv[NT][4];  // rows 16 I + 4 lg + r, both columns
+#pragma unroll
+  for (int I = 0; I < NT; ++I)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) 
+      vv[I][r] = __builtin_amdgcn_raw_buffer_load_b32(bv, min(16 * I + 4 * lg + r, T - 1) * v_row + 2 * col, 0, 0);
+  gdn::keep_loads_here();
+  const buf_t bs = buf_of(pool + slot * s_slot + static_cast<int64_t>(h) * D * D);
+  const int s_off = (8 * lg * D + col) * 4;
+  Tile<D> S;
+  S.load(bs, s_off);
   gdn::keep_loads_here();
 
-  // --- the tree and the nodes' norms; the pending path ---
+  // --- the tree: lane t of wave 0 from node t up to the root; the pending path ---
   if (wave == 0) {
-    if (lane < TM) {
-      dec[lane] = expf(my_g);
-      bt[lane] = my_beta;
-    }
     for (int i = lane; i < TM * TM / 4; i += 64) reinterpret_cast<float4*>(wt)[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-    tree_links(my_parent, T, lane, raw, link);
-    wave_lds_order();
-    if (lane < T && link[lane] != kUnused) {
-      float w = 1.0f;
-      for (int s = lane; s >= 0; s = link[s]) {
+    const float dec = expf(my_g);
+    bool fine = lane < T && my_parent >= -1 && my_parent < lane;
+    int s = fine ? my_parent : -1;
+    float w = dec;
+    if (fine) wt[lane][lane] = 1.0f;
+    while (__any(s >= 0)) {
+      const int at = max(s, 0);
+      const float d = __shfl(dec, at, 64);
+      const int p = __shfl(my_parent, at, 64);
+      if (s >= 0) {
         wt[lane][s] = w;
-        w *= dec[s];
+        w *= d;
+        fine = p >= -1 && p < s;  // (each step goes to an earlier node: the walk ends)
+        s = fine ? p : -1;
       }
+    }
+    if (lane < TM) {
+      link[lane] = fine ? my_parent : kUnused;
+      bt[lane] = my_beta;
       total[lane] = w;
     }
   } else if (wave == 1 && pd.accepted) {
@@ -560,7 +605,13 @@ __global__ __launch_bounds__(2 * D, NT == 1 ? 4 : NT == 2 ? 3 : NT == 3 ? 2 : 1)
   }
   gdn::lds_barrier();
   const bool pending = pd.accepted && path.count > 0;  // (the whole workgroup)
-  if (pending) stage_path<D, TM>(pd, path, b, h, kh, Hv, wave, NW, lane, xk, xq);
+  if (pending) stage_path<D>(pd, path, 0, b, h, kh, Hv, wave, NW, lane, xk, xq);
+  if (tid < TM) {
+    const bool on = link[tid] != kUnused;
+    fv[tid] = on ? bt[tid] : 0.0f;
+    fk[tid] = on ? -(bt[tid] * total[tid]) * rk[tid] : 0.0f;
+    fq[tid] = on ? (scale * total[tid]) * rq[tid] : 0.0f;
+  }
 
   // --- the nodes' products with each other: coefficients of u_s in u_t and in o_t ---
   // Tile (I, J), J <= I, of K K^T and of Q K^T: lane (lr, lg), register r: t = 16 I + 4 lg
@@ -583,12 +634,12 @@ __global__ __launch_bounds__(2 * D, NT == 1 ? 4 : NT == 2 ? 3 : NT == 3 ? 2 : 1)
       for (int r = 0; r < 4; ++r) {
         const int t = 16 * I + 4 * lg + r;
         const float w = wt[t][s];
+        const bool on = w != 0.0f && link[t] != kUnused;
         if (type) {
-          co[t][s] = w != 0.0f ? (scale * rq[t]) * (rs * w) * c[r] : 0.0f;
+          co[t][s] = on ? (scale * rq[t]) * (rs * w) * c[r] : 0.0f;
         } else {
-          const bool on = w != 0.0f && s < t;
-          cu[t][s] = on ? (bt[t] * rk[t]) * (rs * w) * c[r] : 0.0f;
-          some |= on;
+          cu[t][s] = on && s < t ? -(bt[t] * rk[t]) * (rs * w) * c[r] : 0.0f;
+          some |= on && s < t;
         }
       }
       if (!type) {
@@ -596,13 +647,51 @@ __global__ __launch_bounds__(2 * D, NT == 1 ? 4 : NT == 2 ? 3 : NT == 3 ? 2 : 1)
         if (lane == 0) any_cu[I][J] = some;
       }
     }
+    if (!type) {
+      // the inverse of the triangle by substitution: lane (lr, lg) rows 4 lg .. + 3 of its
+      // column lr; four rows at a time are finished and handed to the later ones (in few
+      // registers: the state is on its way into most of them)
+      wave_lds_order();
+      gdn::f32x4_t x;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) x[r] = 4 * lg + r == lr ? 1.0f : 0.0f;
+#pragma unroll
+      for (int p = 0; p < 4; ++p) {
+        gdn::f32x4_t c[4], y = x;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) c[r] = four(&cu[16 * I + 4 * lg + r][16 * I + 4 * p]);
+        y[1] = fmaf(c[1][0], y[0], y[1]);
+        y[2] = fmaf(c[2][1], y[1], fmaf(c[2][0], y[0], y[2]));
+        y[3] = fmaf(c[3][2], y[2], fmaf(c[3][1], y[1], fmaf(c[3][0], y[0], y[3])));
+        float z[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) z[e] = __shfl(y[e], 16 * p + lr, 64);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          float n = x[r];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) n = fmaf(c[r][e], z[e], n);
+          x[r] = lg == p ? y[r] : n;
+        }
+      }
+#pragma unroll
+      for (int r = 0; r < 4; ++r) inv[16 * I + 4 * lg + r][lr] = x[r];
+    }
   }
 
   // --- the state after the pending path; its products with the nodes' rows ---
+  gdn::lds_barrier();
   if (pending) {
-    gdn::lds_barrier();
-    S.advance(path.total, path.count, xk, xq, wave, lr, lg);
-    S.store(S0);
+    S.scale(path.total);
+    S.advance(min(path.count, kPathRows), xk, xq, wave, lr, lg);
+    for (int p = kPathRows; p < path.count; p += kPathRows) {
+      gdn::lds_barrier();
+      stage_path<D>(pd, path, p, b, h, kh, Hv, wave, NW, lane, xk, xq);
+      gdn::lds_barrier();
+      S.advance(min(path.count - p, kPathRows), xk, xq, wave, lr, lg);
+    }
+    S.store(bs, s_off);
+    gdn::lds_barrier();  // the path's rows have been read
   }
   gdn::f32x4_t ak[NT][2], aq[NT][2];  // [node tile][even, odd columns]
 #pragma unroll
@@ -612,7 +701,7 @@ __global__ __launch_bounds__(2 * D, NT == 1 ? 4 : NT == 2 ? 3 : NT == 3 ? 2 : 1)
   // (the nodes' rows come again, from the caches, one product ahead: held in registers from
   // the start they would cost a workgroup per CU)
   const int tiles = (T + 15) / 16;
-  gdn::s16x8_t nk = row_frag(kb + row_of(0) * k_t), nq = row_frag(qb + row_of(0) * q_t);
+  gdn::s16x8_t nk = k_frag(0, 0), nq = q_frag(0, 0);
 #pragma unroll
   for (int kk = 0; kk < KK; ++kk) {
     typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
@@ -633,8 +722,8 @@ __global__ __launch_bounds__(2 * D, NT == 1 ? 4 : NT == 2 ? 3 : NT == 3 ? 2 : 1)
       const gdn::s16x8_t x = nk, y = nq;
       const int In = I + 1 < tiles && I + 1 < NT ? I + 1 : 0, kn = In ? kk : kk + 1;
       if (kn < KK) {
-        nk = row_frag(kb + row_of(In) * k_t + 32 * kn);
-        nq = row_frag(qb + row_of(In) * q_t + 32 * kn);
+        nk = k_frag(In, kn);
+        nq = q_frag(In, kn);
       }
 #pragma unroll
       for (int n = 2; n >= 0; --n)  // (the smallest terms first)
@@ -645,138 +734,103 @@ __global__ __launch_bounds__(2 * D, NT == 1 ? 4 : NT == 2 ? 3 : NT == 3 ? 2 : 1)
         }
     }
   }
-  if (tid < D) load_v(0);
-  if (pending) gdn::lds_barrier();  // the path's rows have been read
+
+  // --- u and o, 16 nodes at a time ---
+  gdn::f32x4_t uu[NT][2];
+  bool fine = true;
 #pragma unroll
   for (int I = 0; I < NT; ++I) {
-    if (16 * I >= T) break;
+    if (I >= tiles) break;
+    const gdn::f32x4_t xv = four(&fv[16 * I + 4 * lg]), xk4 = four(&fk[16 * I + 4 * lg]), xq4 = four(&fq[16 * I + 4 * lg]);
+    gdn::f32x4_t rhs[2], out[2];
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        const float x = __uint_as_float(c ? vv[I][r] & 0xffff0000u : vv[I][r] << 16);
+        // (a factor of 0 keeps what its row holds out)
+        rhs[c][r] = (xv[r] != 0.0f ? xv[r] * x : 0.0f) + (xk4[r] != 0.0f ? xk4[r] * ak[I][c][r] : 0.0f);
+        out[c][r] = xq4[r] != 0.0f ? xq4[r] * aq[I][c][r] : 0.0f;
+      }
+#pragma unroll
+    for (int J = 0; J < I; ++J) {
+      if (!any_cu[I][J]) continue;
+      const gdn::f32x4_t a = four(&cu[16 * I + lr][16 * J + 4 * lg]), e = four(&co[16 * I + lr][16 * J + 4 * lg]);
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        rhs[c] = mul16(a, uu[J][c], rhs[c]);
+        out[c] = mul16(e, uu[J][c], out[c]);
+      }
+    }
+    const gdn::f32x4_t a = four(&inv[16 * I + lr][4 * lg]), e = four(&co[16 * I + lr][16 * I + 4 * lg]);
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      uu[I][c] = mul16(a, rhs[c], gdn::f32x4_t{0.f, 0.f, 0.f, 0.f});
+      out[c] = mul16(e, uu[I][c], out[c]);
+    }
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       const int t = 16 * I + 4 * lg + r;
-      *reinterpret_cast<f32x2_t*>(&xk[t][32 * wave + 2 * lr]) = f32x2_t{ak[I][0][r], ak[I][1][r]};
-      *reinterpret_cast<f32x2_t*>(&xq[t][32 * wave + 2 * lr]) = f32x2_t{aq[I][0][r], aq[I][1][r]};
+      fine &= finite(uu[I][0][r]) && finite(uu[I][1][r]);
+      if (t < T) {
+        *reinterpret_cast<f32x2_t*>(u + out0 + t * out_t + col) = f32x2_t{uu[I][0][r], uu[I][1][r]};
+        *reinterpret_cast<uint32_t*>(o + out0 + t * out_t + col) = gdn::f2bf2(out[0][r], out[1][r]);
+      }
     }
   }
-  gdn::lds_barrier();
+  if (!__any(!fine)) return;
 
-  // --- u, a column per thread: 16 nodes at a time, the earlier tiles' share and then one
-  // node after the other, in registers.  Coefficients of nodes that are no ancestors are 0:
-  // where a result is not finite, it is formed again from the ancestors alone (a branch's
-  // infinity or NaN stays in it). ---
-  if (tid < D) {
+  // --- where a correction is not finite (an infinity or a NaN in a row or in the state): the
+  // products above let it into every node of its column, coefficient 0 or not.  So the
+  // wave's columns again, a column per lane, each node from its ancestors alone. ---
+  const int mine = 32 * wave + (lane & 31);
 #pragma unroll 1
-    for (int I = 0; 16 * I < T; ++I) {
-      float a[16], us[16];
+  for (int I = 0; I < tiles; ++I) {
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const int t = 16 * I + i;
-        a[i] = t < T && link[min(t, T - 1)] != kUnused
-                   ? bt[t] * (gdn::bf2f(vv[i]) - (total[t] * rk[t]) * xk[t][tid])
-                   : 0.0f;
-      }
-      if (16 * I + 16 < T) load_v(I + 1);
-#pragma unroll 1
-      for (int J = 0; J < I; ++J) {
-        if (!any_cu[I][J]) continue;
+    for (int J = 0; J < NT; ++J)
+      if (J == I)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) us[i] = xk[16 * J + i][tid];
-        add_block(a, -1.0f, cu, 16 * I, 16 * J, us);
-      }
-#pragma unroll
-      for (int p = 0; p < 4; ++p) {
-        // columns 4 p .. of the tile's coefficients
-        float4 c[16];
-#pragma unroll
-        for (int i = 4 * p + 1; i < 16; ++i)
-          c[i] = *reinterpret_cast<const float4*>(&cu[16 * I + i][16 * I + 4 * p]);
-#pragma unroll
-        for (int i = 4 * p + 1; i < 16; ++i) a[i] = fmaf(-c[i].x, a[4 * p], a[i]);
-#pragma unroll
-        for (int i = 4 * p + 2; i < 16; ++i) a[i] = fmaf(-c[i].y, a[4 * p + 1], a[i]);
-#pragma unroll
-        for (int i = 4 * p + 3; i < 16; ++i) a[i] = fmaf(-c[i].z, a[4 * p + 2], a[i]);
-#pragma unroll
-        for (int i = 4 * p + 4; i < 16; ++i) a[i] = fmaf(-c[i].w, a[4 * p + 3], a[i]);
-      }
-      bool fine = true;
-#pragma unroll
-      for (int i = 0; i < 16; ++i) fine &= finite(a[i]);
-      if (__any(!fine)) {
-#pragma unroll 1
-        for (int t = 16 * I; t < min(T, 16 * I + 16); ++t) {
-          float x = 0.0f;
-          if (link[t] != kUnused) {
-            x = bt[t] * (gdn::bf2f(vb[t * v_t]) - (total[t] * rk[t]) * xk[t][tid]);
-            for (int s = link[t]; s >= 0; s = link[s]) x = fmaf(-cu[t][s], xk[s][tid], x);
-          }
-          xk[t][tid] = x;
+        for (int r = 0; r < 4; ++r) {
+          *reinterpret_cast<f32x2_t*>(&xk[4 * lg + r][col]) = f32x2_t{ak[J][0][r], ak[J][1][r]};
+          *reinterpret_cast<f32x2_t*>(&xq[4 * lg + r][col]) = f32x2_t{aq[J][0][r], aq[J][1][r]};
         }
-      } else {
-#pragma unroll
-        for (int i = 0; i < 16; ++i) xk[16 * I + i][tid] = a[i];
-      }
-#pragma unroll
-      for (int i = 0; i < 16; ++i)
-        if (16 * I + i < T) u[out0 + (16 * I + i) * out_t + tid] = xk[16 * I + i][tid];
-    }
-  }
-  gdn::lds_barrier();
-
-  // --- o: two threads per column, 8 of every 16 nodes each ---
-  {
-    const int col = tid % D, half = tid / D;
+    wave_lds_order();
 #pragma unroll 1
-    for (int I = 0; 16 * I < T; ++I) {
-      const int t0 = 16 * I + 8 * half;
-      if (t0 >= T) break;
-      float a[8], us[16];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int t = t0 + i;
-        a[i] = t < T && link[min(t, T - 1)] != kUnused ? (scale * rq[t]) * total[t] * xq[t][col] : 0.0f;
-      }
-#pragma unroll 1
-      for (int J = 0; J <= I; ++J) {
-        if (J < I && !any_cu[I][J]) continue;
-#pragma unroll
-        for (int i = 0; i < 16; ++i) us[i] = xk[16 * J + i][col];
-        add_block(a, 1.0f, co, t0, 16 * J, us);
-      }
-      bool fine = true;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) fine &= finite(a[i]);
-      if (__any(!fine)) {
-#pragma unroll 1
-        for (int t = t0; t < min(T, t0 + 8); ++t) {
-          float x = 0.0f;
-          if (link[t] != kUnused) {
-            x = (scale * rq[t]) * total[t] * xq[t][col];
-            for (int s = t; s >= 0; s = link[s]) x = fmaf(co[t][s], xk[s][col], x);
-          }
-          o[out0 + t * out_t + col] = gdn::f2bf(x);
+    for (int t = 16 * I; t < min(T, 16 * I + 16); ++t) {
+      float x = 0.0f, y = 0.0f;
+      if (link[t] != kUnused) {
+        x = fv[t] * gdn::bf2f(v[b * v_b + t * v_t + static_cast<int64_t>(h) * D + mine]) + fk[t] * xk[t - 16 * I][mine];
+        y = fq[t] * xq[t - 16 * I][mine];
+        for (int s = link[t]; s >= 0; s = link[s]) {
+          const float us = u[out0 + s * out_t + mine];
+          x = fmaf(cu[t][s], us, x);
+          y = fmaf(co[t][s], us, y);
         }
-      } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-          if (t0 + i < T) o[out0 + (t0 + i) * out_t + col] = gdn::f2bf(a[i]);
+        y = fmaf(co[t][t], x, y);
+      }
+      if (lane < 32) {
+        u[out0 + t * out_t + mine] = x;
+        o[out0 + t * out_t + mine] = gdn::f2bf(y);
       }
     }
+    wave_lds_order();
   }
 }
 
 // ---- commit ----
 // The first `states` workgroups: the state tiles, one each.  Then the taps, 8 channels per
 // thread.
-template <int D, int NT>
+template <int D>
 __global__ __launch_bounds__(2 * D) void commit_tree_kernel(float* __restrict__ pool, int64_t s_slot,
                                                             uint16_t* __restrict__ cpool, int64_t sp_slot,
                                                             int64_t sp_ch, int64_t n_slots,
                                                             const int64_t* __restrict__ ids, RulePending pd,
                                                             ConvPending cd, int B, int Hk, int Hv, int C,
                                                             int states) {
-  constexpr int NW = D / 32, TM = 16 * NT;
-  __shared__ __align__(16) float wk[TM][D];
-  __shared__ __align__(16) float us[TM][D];
+  constexpr int NW = D / 32;
+  __shared__ __align__(16) float wk[kPathRows][D];
+  __shared__ __align__(16) float us[kPathRows][D];
+  __shared__ int raw[kMaxNodes], link[kMaxNodes];
   __shared__ Path path;
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -785,16 +839,16 @@ __global__ __launch_bounds__(2 * D) void commit_tree_kernel(float* __restrict__ 
     const int at = blockIdx.x - states, b = at / parts;
     const int64_t slot = ids[b];
     if (slot < 0 || slot >= n_slots) return;
-    if (wave == 0) tree_links(cd.parents[b * cd.p_b + min(lane, cd.T - 1)], cd.T, lane, path.raw, path.link);
+    if (wave == 0) tree_links(cd.parents[b * cd.p_b + min(lane, cd.T - 1)], cd.T, lane, raw, link);
     __syncthreads();
-    const int a = accepted_node(cd.accepted[b], cd.T, path.link);
+    const int a = accepted_node(cd.accepted[b], cd.T, link);
     const int c0 = (at % parts * 2 * D + tid) * 8;
     if (c0 >= C || a < 0) return;
     uint16_t* p = cpool + slot * sp_slot + c0 * sp_ch;
     const bool dense = dense_taps(cpool, sp_slot, sp_ch);
     Taps taps;
     taps.load(p, sp_ch, dense);
-    taps.advance(cd, b, c0, a, path.link);
+    taps.advance(cd, b, c0, a, link);
     taps.store(p, sp_ch, dense);
     return;
   }
@@ -804,25 +858,31 @@ __global__ __launch_bounds__(2 * D) void commit_tree_kernel(float* __restrict__ 
   const int lr = lane & 15, lg = lane >> 4;
   const int64_t slot = ids[b];
   if (slot < 0 || slot >= n_slots) return;
-  float* S0 = pool + slot * s_slot + static_cast<int64_t>(h) * D * D + 8 * lg * D + 32 * wave + 2 * lr;
+  const buf_t bs = buf_of(pool + slot * s_slot + static_cast<int64_t>(h) * D * D);
+  const int s_off = (8 * lg * D + 32 * wave + 2 * lr) * 4;
   PathIn pin = {-1, 0.0f, 0};
   if (wave == 0) pin.load(pd, b, h, Hv, lane);
   gdn::keep_loads_here();
   Tile<D> S;
-  S.load(S0);
+  S.load(bs, s_off);
   gdn::keep_loads_here();
   if (wave == 0) find_path(pin, pd.T, lane, path);
   gdn::lds_barrier();
   if (path.count == 0) return;  // (the whole workgroup)
-  stage_path<D, TM>(pd, path, b, h, h / (Hv / Hk), Hv, wave, NW, lane, wk, us);
-  gdn::lds_barrier();
-  S.advance(path.total, path.count, wk, us, wave, lr, lg);
-  S.store(S0);
+  for (int p = 0; p < path.count; p += kPathRows) {
+    if (p) gdn::lds_barrier();
+    stage_path<D>(pd, path, p, b, h, h / (Hv / Hk), Hv, wave, NW, lane, wk, us);
+    gdn::lds_barrier();
+    if (p == 0) S.scale(path.total);
+    S.advance(min(path.count - p, kPathRows), wk, us, wave, lr, lg);
+  }
+  S.store(bs, s_off);
 }
 
 bool rows_ok(const void* p, int64_t s_b, int64_t s_t, int width, int T) {
-  return p && reinterpret_cast<uintptr_t>(p) % 16 == 0 && s_b % 8 == 0 && s_t % 8 == 0 && s_t >= width && s_b >= 0 &&
-         T >= 1 && T <= kMaxNodes;
+  // (kMaxNodes rows of below 2^24 values: 32-bit byte offsets)
+  return p && reinterpret_cast<uintptr_t>(p) % 16 == 0 && s_b % 8 == 0 && s_t % 8 == 0 && s_t >= width &&
+         s_t < (1 << 24) && s_b >= 0 && T >= 1 && T <= kMaxNodes;
 }
 
 }  // namespace
@@ -869,15 +929,14 @@ extern "C" int gdn_rule_tree(const uint16_t* q, int64_t q_b, int64_t q_t, const 
   const RulePending pd{last_k, lk_b, lk_t, last_g, last_u, last_parents, lp_b, accepted, last_T};
   const dim3 grid(static_cast<unsigned>(gdn::kNumXcd * ((B * Hv + gdn::kNumXcd - 1) / gdn::kNumXcd)));
   hipStream_t st = static_cast<hipStream_t>(stream);
-  const int nodes = accepted ? std::max(T, last_T) : T;
 #define GDN_RULE(DD, NT)                                                                                            \
   rule_tree_kernel<DD, NT><<<grid, dim3(2 * DD), 0, st>>>(q, q_b, q_t, k, k_b, k_t, v, v_b, v_t, g, beta, s_pool,    \
                                                           s_slot, n_slots, ids, parents, p_b, pd, o, u, B, T, Hk, Hv, \
                                                           scale)
   if (D == 128)
-    nodes <= 16 ? GDN_RULE(128, 1) : nodes <= 32 ? GDN_RULE(128, 2) : nodes <= 48 ? GDN_RULE(128, 3) : GDN_RULE(128, 4);
+    T <= 16 ? GDN_RULE(128, 1) : T <= 32 ? GDN_RULE(128, 2) : T <= 48 ? GDN_RULE(128, 3) : GDN_RULE(128, 4);
   else
-    nodes <= 16 ? GDN_RULE(64, 1) : nodes <= 32 ? GDN_RULE(64, 2) : nodes <= 48 ? GDN_RULE(64, 3) : GDN_RULE(64, 4);
+    T <= 16 ? GDN_RULE(64, 1) : T <= 32 ? GDN_RULE(64, 2) : T <= 48 ? GDN_RULE(64, 3) : GDN_RULE(64, 4);
 #undef GDN_RULE
   return gdn_launch_status();
 }
@@ -902,13 +961,11 @@ extern "C" int gdn_commit_tree(float* s_pool, int64_t s_slot, uint16_t* conv_poo
   const int states = gdn::kNumXcd * ((B * Hv + gdn::kNumXcd - 1) / gdn::kNumXcd);
   const dim3 grid(static_cast<unsigned>(states + B * ((C + 8 * 2 * D - 1) / (8 * 2 * D))));
   hipStream_t st = static_cast<hipStream_t>(stream);
-#define GDN_COMMIT(DD, NT)                                                                                          \
-  commit_tree_kernel<DD, NT><<<grid, dim3(2 * DD), 0, st>>>(s_pool, s_slot, conv_pool, sp_slot, sp_ch, n_slots, ids, \
-                                                            pd, cd, B, Hk, Hv, C, states)
   if (D == 128)
-    T <= 16 ? GDN_COMMIT(128, 1) : GDN_COMMIT(128, 4);
+    commit_tree_kernel<128><<<grid, dim3(256), 0, st>>>(s_pool, s_slot, conv_pool, sp_slot, sp_ch, n_slots, ids, pd, cd,
+                                                        B, Hk, Hv, C, states);
   else
-    T <= 16 ? GDN_COMMIT(64, 1) : GDN_COMMIT(64, 4);
-#undef GDN_COMMIT
+    commit_tree_kernel<64><<<grid, dim3(128), 0, st>>>(s_pool, s_slot, conv_pool, sp_slot, sp_ch, n_slots, ids, pd, cd,
+                                                       B, Hk, Hv, C, states);
   return gdn_launch_status();
 }

@@ -891,7 +891,7 @@ def _tree_rows(t: torch.Tensor, name: str, shape: tuple):
     width = shape[2] if len(shape) == 3 else shape[2] * shape[3]
     st = t.stride()
     dense = st[-1] == 1 and (len(shape) == 3 or st[2] == shape[3] or shape[2] == 1)
-    if not dense or st[1] < width or st[0] % 8 or st[1] % 8 or t.data_ptr() % 16:
+    if not dense or not width <= st[1] < 1 << 24 or st[0] % 8 or st[1] % 8 or t.data_ptr() % 16:
         t = t.contiguous() if not t.is_contiguous() else t.clone(memory_format=torch.contiguous_format)
         return t, shape[1] * width, width
     return t, st[0], st[1]

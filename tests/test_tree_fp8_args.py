@@ -179,7 +179,7 @@ def test_c_entry_points_reject_before_launch(pkg):
         lib.gdn_rule_tree(q, 8 * 128, qt, P, 8 * 128, 128, P, 8 * 256, vt, g, P, s, st, 4, P, P, 8, P, 8 * 128, 128,
                           P, lu, P, 8, P, lT, o, u, B, T, Hk, Hv, D, 1.0, None))
     assert r(B=0) == ok and r(T=65) == uns and r(D=96) == uns and r(lT=65) == uns
-    for bad in (dict(q=None), dict(qt=120), dict(vt=248), dict(g=None), dict(s=odd), dict(st=slot - 4), dict(o=None),
+    for bad in (dict(q=None), dict(qt=120), dict(qt=1 << 24), dict(vt=248), dict(g=None), dict(s=odd), dict(st=slot - 4), dict(o=None),
                 dict(u=odd), dict(Hk=3), dict(Hk=0), dict(lu=None), dict(lT=0), dict(T=-1)):
         assert r(**bad) == inv, bad
     c = lambda s=P, st=slot, cp=P, cs=3 * C, x=P, k=P, u=P, acc=P, B=2, T=8, Hk=2, Hv=4, D=64, Cc=C: (  # noqa: E731
