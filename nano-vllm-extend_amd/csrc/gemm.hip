@@ -380,6 +380,10 @@ __global__ __launch_bounds__(kGemmThreads, kMinWG) void gemm_tn_kernel(const uin
 // 508 -> 425, 1949 x 12352 x 2048 100 -> 87, 1949 x 2048 x 4096 42.6 -> 38.
 constexpr int kPPThreads = 512;
 
+// s_waitcnt vmcnt(8) lgkmcnt(0): all but the newest 8 loads have landed and
+// every LDS read has returned
+constexpr int kWaitPP = 8 | (7 << 4);
+
 // grid = 8 * min(32, ...) workgroups of 512; tiles 0 .. whole - 1 run as 256 x
 // 256, the rest as quarters.  K is a multiple of 128.
 __global__ __launch_bounds__(kPPThreads, 2) void gemm_tn_pp_kernel(const uint16_t* __restrict__ A, int64_t lda,

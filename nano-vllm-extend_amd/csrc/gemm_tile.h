@@ -125,9 +125,6 @@ __device__ __forceinline__ void half_barrier() {
   asm volatile("" ::: "memory");
 }
 
-// s_waitcnt vmcnt(8) lgkmcnt(0): all but the newest 8 loads have landed and
-// every LDS read has returned
-constexpr int kWaitPP = 8 | (7 << 4);
 // s_waitcnt lgkmcnt(0) alone (vmcnt 63)
 constexpr int kWaitLds = 15 | (7 << 4) | (3 << 14);
 

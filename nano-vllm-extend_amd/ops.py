@@ -914,7 +914,7 @@ def _conv_pool_ok(pool: torch.Tensor, C: int) -> tuple:
 
 
 def _s_pool_ok(pool: torch.Tensor, Hv: int, D: int) -> None:
-    if not _state_view_ok(pool, Hv, D):
+    if pool.shape[1:] != (Hv, D, D) or pool.stride()[1:] != (D * D, D, 1) or pool.dtype != torch.float32:
         raise ValueError(f"s_pool must be an fp32 [slots, {Hv}, {D}, {D}] view with dense slots")
 
 
@@ -1348,6 +1348,18 @@ def rms_norm_gated_ranges(hidden_states: torch.Tensor, gate: torch.Tensor, weigh
               D, float(eps), _stream(dev))
 
 
+def _token_heads(t: torch.Tensor, H: int, D: int):
+    """[..., H, D] as tokens with dense heads that the kernel reads in 16-byte pieces
+    (else copied once), and their stride."""
+    if t.is_contiguous():
+        return (t if t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format)), H * D
+    t = t.reshape(-1, H, D)
+    st = t.stride()
+    if st[2] != 1 or st[1] != D or st[0] % 8 or t.data_ptr() % 16:
+        return t.contiguous() if not t.is_contiguous() else t.clone(memory_format=torch.contiguous_format), H * D
+    return t, st[0]
+
+
 def rms_norm_gated_fp8(hidden_states: torch.Tensor, gate: torch.Tensor, weight: torch.Tensor, eps: float):
     """rms_norm_gated written in e4m3 for an 8-bit out projection: y = x * rsqrt(mean(x^2)
     + eps) * w * silu(z) in fp32 over the last dim, then quantize_fp8's groups of 128
@@ -1365,20 +1377,11 @@ def rms_norm_gated_fp8(hidden_states: torch.Tensor, gate: torch.Tensor, weight: 
     if weight.numel() != D or H == 0 or H * D % FP8_GROUP:
         raise ValueError(f"weight must have {D} values and H * D = {H * D} be a multiple of {FP8_GROUP}")
 
-    def tokens(t):  # dense heads of a token, in 16-byte pieces
-        if t.is_contiguous():
-            return (t if t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format)), H * D
-        t = t.reshape(-1, H, D)
-        st = t.stride()
-        if st[2] != 1 or st[1] != D or st[0] % 8 or t.data_ptr() % 16:
-            return t.contiguous() if not t.is_contiguous() else t.clone(memory_format=torch.contiguous_format), H * D
-        return t, st[0]
-
-    x, x_tok = tokens(hidden_states)
-    z, z_tok = tokens(gate)
+    x, x_tok = _token_heads(hidden_states, H, D)
+    z, z_tok = _token_heads(gate, H, D)
     n_tok = hidden_states.numel() // (H * D)
-    y = torch.empty(hidden_states.shape, dtype=FP8, device=hidden_states.device)
-    scale = _fp8_scales(n_tok, H * D // FP8_GROUP, hidden_states.device)
+    y = x.new_empty(hidden_states.shape, dtype=FP8)
+    scale = _fp8_scales(n_tok, H * D // FP8_GROUP, x.device)
     _call_on(idx, "gdn_rmsnorm_gated_fp8", x.data_ptr(), x_tok, z.data_ptr(), z_tok, weight.data_ptr(), y.data_ptr(),
              scale.data_ptr(), 1, n_tok, n_tok, H, D, float(eps))
     return y, scale
