@@ -452,7 +452,12 @@ int gdn_quantize_fp8(const void* x, int x_is_fp32, int64_t sx, uint8_t* y, int64
  *      dead after the call
  *   B  [N, K] e4m3 (the weight), row stride ldb; sb [ceil(N / 128), K / 128] fp32, row
  *      stride sb_row
- *   C  bf16, n_parts column parts as gdn_gemm_bf16_cols
+ *   B2 [N2, K] bf16, row stride ldb2 (N2 == 0: none): columns N .. N + N2 - 1 of the output
+ *      with a weight that stays in bf16, on A's bf16 rows (a_is_bf16; N, N2 multiples of 16;
+ *      K in steps of 128, summed in fp32).  The GDN layer's gate projections, whose own
+ *      launch costs more than they do
+ *   C  bf16, n_parts column parts over the N + N2 columns as gdn_gemm_bf16_cols, one of
+ *      them ending at N
  * K a multiple of 128; lda a multiple of 16 (bf16: 8), ldb of 16, A and B 16-byte aligned.
  * The order in which the blocks' sums are added may depend on M, N and K (not on which of
  * the two A is: a call from bf16 rows has the bits of gdn_quantize_fp8 and one from its
@@ -460,9 +465,9 @@ int gdn_quantize_fp8(const void* x, int x_is_fp32, int64_t sx, uint8_t* y, int64
  * block the matrix cores drop what lies below 2^-13 of the block's largest products.
  */
 int gdn_gemm_fp8(const void* A, int a_is_bf16, int64_t lda, const float* sa, int64_t sa_row, int64_t sa_grp,
-                 const uint8_t* B, int64_t ldb, const float* sb, int64_t sb_row, int M, int N, int K, int n_parts,
-                 uint16_t* const* C, const int64_t* ldc, const int* col_end, void* workspace,
-                 int64_t workspace_bytes, void* stream);
+                 const uint8_t* B, int64_t ldb, const float* sb, int64_t sb_row, const uint16_t* B2, int64_t ldb2,
+                 int N2, int M, int N, int K, int n_parts, uint16_t* const* C, const int64_t* ldc, const int* col_end,
+                 void* workspace, int64_t workspace_bytes, void* stream);
 
 /* Workspace bytes of gdn_gemm_fp8; -1 on bad args. */
 int64_t gdn_gemm_fp8_workspace_size(int M, int N, int K, int a_is_bf16);

@@ -68,8 +68,8 @@ SIGNATURES: dict[str, list] = {
     "gdn_state_tile_copy": [_p, _p, _i64, _p, _i32, _i32, _i32, _p],
     "gdn_rmsnorm_gated_ranges": [_p, _i64, _p, _i64, _p, _p, _i64, _p, _i32, _i64, _i32, _i32, _f32, _p],
     "gdn_quantize_fp8": [_p, _i32, _i64, _p, _i64, _p, _i64, _i64, _i64, _i32, _i32, _p],
-    "gdn_gemm_fp8": [_p, _i32, _i64, _p, _i64, _i64, _p, _i64, _p, _i64, _i32, _i32, _i32, _i32, _p, _p, _p, _p, _i64,
-                     _p],
+    "gdn_gemm_fp8": [_p, _i32, _i64, _p, _i64, _i64, _p, _i64, _p, _i64, _p, _i64, _i32, _i32, _i32, _i32, _i32, _p, _p,
+                     _p, _p, _i64, _p],
     "gdn_gemm_fp8_workspace_size": [_i32, _i32, _i32, _i32],
     "gdn_rmsnorm_gated_fp8": [_p, _i64, _p, _i64, _p, _p, _p, _i64, _i64, _i64, _i32, _i32, _f32, _p],
     "gdn_conv_tree": [_p, _i64, _i64, _p, _i64, _i64, _i64, _p, _p, _p, _i64, _p, _i64, _i64, _p, _i64, _p, _i32, _p,

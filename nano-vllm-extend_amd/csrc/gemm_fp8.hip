@@ -14,6 +14,7 @@
 #include <algorithm>
 
 #include "gemm_tile.h"
+#include "quant_fp8.h"
 
 namespace {
 
@@ -358,6 +359,117 @@ __global__ __launch_bounds__(kPPThreads, 2) void gemm_fp8_pp_kernel(const uint8_
   __builtin_amdgcn_s_waitcnt(0);
 }
 
+// ---- columns with a bf16 weight beside the 8-bit ones ----
+// The layer's gate projections are a few columns whose weight stays in bf16, read with
+// the same rows.  A launch of their own costs more than they do (64 columns of 2048: 5
+// us), so the kernels that quantize the rows take them along: 16 rows x 16 columns per
+// workgroup, K-steps of 128 dealt to its waves, two stages per wave, as in the ring.
+struct Fp8Wide {
+  const uint16_t* b;  // [n, K] bf16, row stride ldb; columns N .. N + n - 1 of the output
+  int64_t ldb;
+  int n;              // a multiple of 16; 0: none
+};
+
+// Bytes of a stage of one wave: 16 rows of 256 bytes of each operand.
+constexpr int kWideStage = 2 * 16 * 256;
+
+template <int NW>
+__device__ __forceinline__ void wide_tile(const void* __restrict__ A, int64_t lda, const Fp8Wide& wide,
+                                          const GemmOut& out, int M, int N, int K, int m0, int n0, uint8_t* st0,
+                                          uint8_t* st1, int stage) {
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lr = lane & 15, lg = lane >> 4;
+  const __amdgpu_buffer_rsrc_t ra = rsrc_of(A), rb = rsrc_of(wide.b);
+  int voff[8];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    // 4 rows of 256 bytes; granule c of row r at slot c ^ r
+    const int r = 4 * i + (lane >> 4), at = 16 * ((lane & 15) ^ r);
+    voff[i] = static_cast<int>(min(m0 + r, M - 1) * lda * 2 + at);
+    voff[4 + i] = static_cast<int>((n0 + r) * wide.ldb * 2 + at);
+  }
+  const int nk = K / 128;
+  auto issue = [&](uint8_t* st, int step) {
+    uint8_t* w = st + wave * stage;
+    const int s = 256 * min(step, nk - 1);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) dma16(i < 4 ? ra : rb, w + i * 1024, voff[i], s);
+  };
+  gdn::f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
+  auto one = [&](uint8_t* st, int step) {
+    const uint8_t* a = st + wave * stage;
+    gdn::s16x8_t fa[4], fb[4];
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      fa[c] = *reinterpret_cast<const gdn::s16x8_t*>(a + lr * 256 + 16 * ((4 * c + lg) ^ lr));
+      fb[c] = *reinterpret_cast<const gdn::s16x8_t*>(a + 4096 + lr * 256 + 16 * ((4 * c + lg) ^ lr));
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_waitcnt(kWaitLds);
+    __builtin_amdgcn_sched_barrier(0);
+    issue(st, step + 2 * NW);
+#pragma unroll
+    for (int c = 0; c < 4; ++c) acc = gdn::mfma16x16x32(fb[c], fa[c], acc);
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_waitcnt(8 | (7 << 4) | (15 << 8));  // vmcnt(8): all but the newest stage
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  issue(st0, wave);
+  issue(st1, wave + NW);
+  __builtin_amdgcn_s_waitcnt(8 | (7 << 4) | (15 << 8));
+  int s = wave;
+  for (; s + NW < nk; s += 2 * NW) {
+    one(st0, s);
+    one(st1, s + NW);
+  }
+  if (s < nk) one(st0, s);
+  __builtin_amdgcn_s_waitcnt(0);  // the repeated loads past the last step
+  __syncthreads();
+  gdn::f32x4_t* red = reinterpret_cast<gdn::f32x4_t*>(st0);
+  red[wave * 64 + lane] = acc;
+  __syncthreads();
+  if (wave) return;
+  acc = red[lane];
+#pragma unroll
+  for (int w = 1; w < NW; ++w) acc += red[w * 64 + lane];
+  // lane (lr, lg): row m0 + lr, columns N + n0 + 4 lg .. + 3, all of one part
+  const int n = N + n0;
+  int p = 0;
+#pragma unroll
+  for (int i = 0; i + 1 < kMaxParts; ++i) p += n >= out.end[i] ? 1 : 0;
+  auto pick = [&](auto a0, auto a1, auto a2, auto a3) { return p == 0 ? a0 : p == 1 ? a1 : p == 2 ? a2 : a3; };
+  if (m0 + lr >= M) return;
+  uint16_t* c = pick(out.c[0], out.c[1], out.c[2], out.c[3]) +
+                static_cast<int64_t>(m0 + lr) * pick(out.ld[0], out.ld[1], out.ld[2], out.ld[3]) + n -
+                pick(0, out.end[0], out.end[1], out.end[2]) + 4 * lg;
+  const uint2 v = make_uint2(gdn::f2bf2(acc[0], acc[1]), gdn::f2bf2(acc[2], acc[3]));
+  if (pick(out.vec[0], out.vec[1], out.vec[2], out.vec[3])) {
+    *reinterpret_cast<uint2*>(c) = v;
+  } else {
+    c[0] = static_cast<uint16_t>(v.x);
+    c[1] = static_cast<uint16_t>(v.x >> 16);
+    c[2] = static_cast<uint16_t>(v.y);
+    c[3] = static_cast<uint16_t>(v.y >> 16);
+  }
+}
+
+// Rows to e4m3 for the kernels that take them so, and the bf16 columns: the first `groups`
+// workgroups 16 groups of 128 each, then 16 x 16 tiles.
+__global__ __launch_bounds__(256) void quant_wide_kernel(const uint16_t* __restrict__ A, int64_t lda,
+                                                         uint8_t* __restrict__ y, float* __restrict__ scale,
+                                                         Fp8Wide wide, GemmOut out, int M, int N, int K, int groups) {
+  __shared__ __align__(16) uint8_t st0[4 * kWideStage];
+  __shared__ __align__(16) uint8_t st1[4 * kWideStage];
+  if (static_cast<int>(blockIdx.x) < groups) {
+    quant_group<false>(A, lda, y, K, scale, 1, M, M, K / gdn::kFp8Group,
+                       static_cast<int64_t>(blockIdx.x) * 16 + threadIdx.x / 16, threadIdx.x % 16);
+    return;
+  }
+  const int t = blockIdx.x - groups, mb_n = (M + 15) / 16;
+  wide_tile<4>(A, lda, wide, out, M, N, K, 16 * (t % mb_n), 16 * (t / mb_n), st0, st1, kWideStage);
+}
+
 // the larger of each pair of 16-bit halves
 typedef uint16_t u16x2_t __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {
@@ -378,7 +490,8 @@ __device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {
 template <int BM, int BN, int NW, int NS, bool kQuant>
 __global__ __launch_bounds__(64 * NW) void gemm_fp8_ring_kernel(const void* __restrict__ A, int64_t lda,
                                                                 const uint8_t* __restrict__ B, int64_t ldb,
-                                                                Fp8Scales sc, GemmOut out, int M, int N, int K) {
+                                                                Fp8Scales sc, GemmOut out, int M, int N, int K,
+                                                                Fp8Wide wide) {
   constexpr int MT = BM / 16, NT = BN / 32;
   constexpr int kARow = kQuant ? 256 : 128;               // bytes of a row of A in LDS
   constexpr int kABytes = BM * kARow, kBBytes = BN * 128;
@@ -394,8 +507,16 @@ __global__ __launch_bounds__(64 * NW) void gemm_fp8_ring_kernel(const void* __re
   static_assert(MT * NT * 2048 <= kStage, "the partial sums fit a stage");
   const int mb_n = (M + BM - 1) / BM, nb_n = (N + BN - 1) / BN;
   // the row blocks of a column block on one XCD, so that its L2 reads the weights once
-  const int64_t L = gdn::xcd_remap(blockIdx.x, static_cast<int64_t>(mb_n) * nb_n);
+  const int64_t L = gdn::xcd_remap(blockIdx.x, static_cast<int64_t>(mb_n) * (nb_n + (kQuant ? wide.n / 16 : 0)));
   if (L < 0) return;
+  if constexpr (kQuant) {
+    static_assert(BM == 16 && kStage >= kWideStage, "wide tiles in the ring's stages");
+    if (L >= static_cast<int64_t>(mb_n) * nb_n) {
+      const int t = static_cast<int>(L - static_cast<int64_t>(mb_n) * nb_n);
+      wide_tile<NW>(A, lda, wide, out, M, N, K, 16 * (t % mb_n), 16 * (t / mb_n), st0, st1, kStage);
+      return;
+    }
+  }
   const int m0 = BM * static_cast<int>(L % mb_n), n0 = BN * static_cast<int>(L / mb_n);
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -737,10 +858,14 @@ Fp8Kernel fp8_plan(int M, int N, int K, bool quant) {
   return kPP;
 }
 
+// Rows up to which the quantizing launch takes the bf16 columns along (each 16 x 16 tile
+// reads its rows again).
+constexpr int kWideRows = 1024;
+
 bool fp8_quantizes(Fp8Kernel k) { return k >= kRingQ16x32; }
 
 int fp8_launch(Fp8Kernel kernel, const void* A, int64_t lda, const uint8_t* B, int64_t ldb, const Fp8Scales& sc,
-               const GemmOut& out, int M, int N, int K, hipStream_t st) {
+               const GemmOut& out, int M, int N, int K, const Fp8Wide& wide, hipStream_t st) {
   auto blocks = [&](int bm, int bn) { return static_cast<int64_t>((M + bm - 1) / bm) * ((N + bn - 1) / bn); };
   auto grid = [](int64_t wgs) {
     return dim3(static_cast<unsigned>(gdn::kNumXcd * ((wgs + gdn::kNumXcd - 1) / gdn::kNumXcd)));
@@ -765,10 +890,11 @@ int fp8_launch(Fp8Kernel kernel, const void* A, int64_t lda, const uint8_t* B, i
       gemm_fp8_deep_kernel<128, 3><<<grid(blocks(64, 128)), dim3(kFp8Threads), 0, st>>>(A8, lda, B, ldb, sc, out, M,
                                                                                        N, K);
       break;
-#define GDN_RING(name, BM, BN, NW, NS, Q)                                                                          \
-  case name:                                                                                                       \
-    gemm_fp8_ring_kernel<BM, BN, NW, NS, Q><<<grid(blocks(BM, BN)), dim3(64 * NW), 0, st>>>(A, lda, B, ldb, sc, out, \
-                                                                                           M, N, K);               \
+#define GDN_RING(name, BM, BN, NW, NS, Q)                                                                       \
+  case name:                                                                                                    \
+    gemm_fp8_ring_kernel<BM, BN, NW, NS, Q>                                                                     \
+        <<<grid(blocks(BM, BN) + (Q ? blocks(16, 16 * N) * (wide.n / 16) : 0)), dim3(64 * NW), 0, st>>>(        \
+            A, lda, B, ldb, sc, out, M, N, K, wide);                                                            \
     break
       GDN_RING(kRing16x32, 16, 32, 8, 2, false);
       GDN_RING(kRing16x64, 16, 64, 4, 3, false);
@@ -791,10 +917,11 @@ extern "C" int64_t gdn_gemm_fp8_workspace_size(int M, int N, int K, int a_is_bf1
 }
 
 extern "C" int gdn_gemm_fp8(const void* A, int a_is_bf16, int64_t lda, const float* sa, int64_t sa_row, int64_t sa_grp,
-                            const uint8_t* B, int64_t ldb, const float* sb, int64_t sb_row, int M, int N, int K,
-                            int n_parts, uint16_t* const* C, const int64_t* ldc, const int* col_end, void* workspace,
-                            int64_t workspace_bytes, void* stream) {
-  if (M < 0 || N < 0 || K < 0 || n_parts < 1 || n_parts > kMaxParts || !C || !ldc || !col_end)
+                            const uint8_t* B, int64_t ldb, const float* sb, int64_t sb_row, const uint16_t* B2,
+                            int64_t ldb2, int N2, int M, int N, int K, int n_parts, uint16_t* const* C,
+                            const int64_t* ldc, const int* col_end, void* workspace, int64_t workspace_bytes,
+                            void* stream) {
+  if (M < 0 || N < 0 || K < 0 || N2 < 0 || n_parts < 1 || n_parts > kMaxParts || !C || !ldc || !col_end)
     return GDN_ERR_INVALID_ARG;
   if (M == 0 || N == 0) return GDN_OK;
   if (!A || !B || !sb || (!a_is_bf16 && !sa)) return GDN_ERR_INVALID_ARG;
@@ -809,22 +936,46 @@ extern "C" int gdn_gemm_fp8(const void* A, int a_is_bf16, int64_t lda, const flo
   if (!a_is_bf16 && (sa_row < 0 || sa_grp < 0 || 4 * ((M - 1) * sa_row + (groups - 1) * sa_grp) >= kLimit))
     return GDN_ERR_INVALID_ARG;
   GemmOut out{};
-  if (!parts_of(out, n_parts, C, ldc, col_end, N)) return GDN_ERR_INVALID_ARG;
+  if (!parts_of(out, n_parts, C, ldc, col_end, N + N2)) return GDN_ERR_INVALID_ARG;
+  int first = n_parts;  // the first part of the bf16 columns
+  if (N2) {
+    if (!B2 || !a_is_bf16 || N2 % 16 || N % 16 || ldb2 % 8 || ldb2 < K || reinterpret_cast<uintptr_t>(B2) % 16 ||
+        N2 * ldb2 * 2 >= kLimit)
+      return GDN_ERR_INVALID_ARG;
+    first = 0;
+    while (first < n_parts && col_end[first] < N) ++first;
+    if (first == n_parts || col_end[first++] != N) return GDN_ERR_INVALID_ARG;  // a part ends at N
+  }
   const Fp8Kernel kernel = fp8_plan(M, N, K, a_is_bf16 != 0);
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  const Fp8Wide wide{B2, ldb2, N2};
   if (a_is_bf16 && !fp8_quantizes(kernel)) {
     if (workspace_bytes < gdn_gemm_fp8_workspace_size(M, N, K, 1) || !workspace ||
         reinterpret_cast<uintptr_t>(workspace) % 16)
       return GDN_ERR_INVALID_ARG;
     uint8_t* x8 = static_cast<uint8_t*>(workspace);
     float* scale = reinterpret_cast<float*>(x8 + static_cast<int64_t>(M) * K);
-    const int st = gdn_quantize_fp8(A, 0, lda, x8, K, scale, 1, M, M, K, 1, stream);
-    if (st != GDN_OK) return st;
+    int rc;
+    if (N2 && M <= kWideRows) {
+      const int64_t quant = (M * groups + 15) / 16;
+      quant_wide_kernel<<<dim3(static_cast<unsigned>(quant + (M + 15) / 16 * (N2 / 16))), dim3(256), 0, st>>>(
+          static_cast<const uint16_t*>(A), lda, x8, scale, wide, out, M, N, K, static_cast<int>(quant));
+      rc = gdn_launch_status();
+    } else {
+      rc = gdn_quantize_fp8(A, 0, lda, x8, K, scale, 1, M, M, K, 1, stream);
+      if (rc == GDN_OK && N2) {
+        int ends[kMaxParts];
+        for (int i = first; i < n_parts; ++i) ends[i - first] = col_end[i] - N;
+        rc = gdn_gemm_bf16_cols(static_cast<const uint16_t*>(A), lda, B2, ldb2, M, N2, K, n_parts - first, C + first,
+                                ldc + first, ends, nullptr, nullptr, nullptr, nullptr, 0, 0, 0, stream);
+      }
+    }
+    if (rc != GDN_OK) return rc;
     A = x8;
     lda = K;
     sa = scale;
     sa_row = 1;
     sa_grp = M;
   }
-  return fp8_launch(kernel, A, lda, B, ldb, Fp8Scales{sa, sa_row, sa_grp, sb, sb_row}, out, M, N, K,
-                    static_cast<hipStream_t>(stream));
+  return fp8_launch(kernel, A, lda, B, ldb, Fp8Scales{sa, sa_row, sa_grp, sb, sb_row}, out, M, N, K, wide, st);
 }

@@ -639,12 +639,10 @@ class GatedDeltaNetLayer:
         widths = [C, V, Hv, Hv]
         if self.fp8:
             with self._timed("in_proj"):
+                if Hv % 16 == 0 and not gates:
+                    return (*ops.linear_fp8_cols(hidden, self.w_in, self.w_in_scale, widths, wide=self.w_ba), None)
                 mixed, z = ops.linear_fp8_cols(hidden, self.w_in, self.w_in_scale, [C, V])
                 how = {"gate_col": 0, "A_log": c.A_log, "dt_bias": c.dt_bias} if gates else None
-                if Hv % 16 == 0:
-                    y = ops.linear_cols(hidden, self.w_ba, [Hv, Hv], gates=how)
-                    (b, a), gb = (y[0], y[1:]) if gates else (y, None)
-                    return mixed, z, b, a, gb
                 y = ops.linear(hidden, self.w_ba, gates=how)
                 y, gb = (y[0], y[1:]) if gates else (y, None)
                 return mixed, z, y[..., :Hv], y[..., Hv:], gb

@@ -1233,9 +1233,15 @@ def _check_fp8(x, weight, weight_scale, x_scale):
     return M, N, K
 
 
-def _linear_fp8(x, weight, weight_scale, x_scale, M, N, K, outs, widths):
-    """The product into outs, [M, widths[s]] each."""
-    idx = _device_of(x, weight, weight_scale, x_scale, *outs)
+def _linear_fp8(x, weight, weight_scale, x_scale, M, N, K, outs, widths, wide=None):
+    """The product into outs, [M, widths[s]] each; the columns past N from the bf16 weight
+    `wide`."""
+    idx = _device_of(x, weight, weight_scale, x_scale, wide, *outs)
+    wide_args = (None, 0, 0)
+    if wide is not None:
+        if wide.stride(1) != 1 or wide.stride(0) % 8 or wide.stride(0) < K or wide.data_ptr() % 16:
+            wide = wide.clone(memory_format=torch.contiguous_format)
+        wide_args = (wide.data_ptr(), wide.stride(0), wide.shape[0])
     w, w_st = weight, weight.stride()
     if w_st[1] != 1 or w_st[0] % 16 or w_st[0] < K or w.data_ptr() % 16:
         w = w.contiguous() if not w.is_contiguous() else w.clone(memory_format=torch.contiguous_format)
@@ -1262,7 +1268,7 @@ def _linear_fp8(x, weight, weight_scale, x_scale, M, N, K, outs, widths):
         tables = ((ctypes.c_void_p * n)(*[p.data_ptr() for p in outs]), (ctypes.c_int64 * n)(*widths),
                   (ctypes.c_int * n)(*ends))
     _call_on(idx, "gdn_gemm_fp8", x2.data_ptr(), int(bf16), x_row, *xs, w.data_ptr(), w_st[0], ws.data_ptr(),
-             ws.stride(0) if N > FP8_GROUP else G, M, N, K, n, *tables, _lib.ptr(work), ws_bytes)
+             ws.stride(0) if N > FP8_GROUP else G, *wide_args, M, N, K, n, *tables, _lib.ptr(work), ws_bytes)
 
 
 def linear_fp8(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor,
@@ -1286,14 +1292,30 @@ def linear_fp8(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor
 
 
 def linear_fp8_cols(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor, widths: list[int],
-                    x_scale: torch.Tensor | None = None) -> list[torch.Tensor]:
+                    x_scale: torch.Tensor | None = None, wide: torch.Tensor | None = None) -> list[torch.Tensor]:
     """linear_fp8 with the output's columns split into len(widths) (1-4) contiguous
-    tensors [..., widths[s]], every boundary a multiple of 16 (as linear_cols)."""
+    tensors [..., widths[s]], every boundary a multiple of 16 (as linear_cols).
+
+    wide: a bf16 weight [N2, K] (N2 and N multiples of 16) whose product with the bf16 x
+    follows as the last columns, N2 of the widths' sum, a boundary at N: the GDN layer's
+    gate projections, which stay in bf16, without a launch of their own where x is
+    quantized in the call's."""
     M, N, K = _check_fp8(x, weight, weight_scale, x_scale)
-    if not 1 <= len(widths) <= 4 or sum(widths) != N or min(widths) <= 0 or any(w % 16 for w in widths[:-1]):
-        raise ValueError(f"widths {widths}: 1 to 4 parts of {N} columns, boundaries at multiples of 16")
+    total = N
+    if wide is not None:
+        if wide.dtype != torch.bfloat16 or x.dtype != torch.bfloat16:
+            raise TypeError(f"wide and x must be bfloat16, got {wide.dtype} and {x.dtype}")
+        if wide.dim() != 2 or wide.shape[1] != K or wide.shape[0] % 16 or wide.shape[0] == 0 or N % 16:
+            raise ValueError(f"wide must be [N2, {K}] with N2 and N = {N} positive multiples of 16, got "
+                             f"{list(wide.shape)}")
+        total += wide.shape[0]
+    ends = [sum(widths[:i + 1]) for i in range(len(widths))]
+    if not 1 <= len(widths) <= 4 or ends[-1] != total or min(widths) <= 0 or any(w % 16 for w in widths[:-1]) \
+            or N not in ends:
+        raise ValueError(f"widths {widths}: 1 to 4 parts of {total} columns, boundaries at multiples of 16"
+                         + (f" and at {N}" if wide is not None else ""))
     parts = [torch.empty(M, w, dtype=torch.bfloat16, device=x.device) for w in widths]
-    _linear_fp8(x, weight, weight_scale, x_scale, M, N, K, parts, widths)
+    _linear_fp8(x, weight, weight_scale, x_scale, M, N, K, parts, widths, wide)
     return parts if x.dim() == 2 else [p.view(*x.shape[:-1], p.shape[1]) for p in parts]
 
 

@@ -133,6 +133,26 @@ def test_linear_fp8_cols(pkg, dev, M):
     assert torch.equal(torch.cat(parts, -1).view(M, N), y)
 
 
+@pytest.mark.parametrize("M,N,K,N2", [(1, 12288, 2048, 64), (1, 2048, 128, 16), (5, 256, 384, 32), (37, 12288, 2048, 64),
+                                      (37, 2048, 4096, 48), (200, 8192, 2048, 32), (1000, 512, 640, 64),
+                                      (1025, 1024, 512, 64), (3000, 2048, 2048, 64)])
+def test_linear_fp8_with_bf16_columns(pkg, dev, M, N, K, N2):
+    """The 8-bit columns are linear_fp8's; the bf16 ones within bf16's half step and fp32's
+    error (K products and K / 128 partial sums, each a rounding) of the 64-bit product."""
+    gen = torch.Generator().manual_seed(M + N2)
+    x = _rows(gen, M, K).to(BF16).to(dev)
+    w8, ws = (t.to(dev) for t in ref.to_e4m3(_rows(gen, N, K) * K ** -0.5, 128))
+    wide = (torch.randn(N2, 2 * K, generator=gen) * K ** -0.5).to(BF16).to(dev)[:, K:]
+    widths = [N - 16, 16, N2] if N2 < 32 else [N, N2 - 16, 16]
+    parts = pkg.ops.linear_fp8_cols(x, w8, ws, widths, wide=wide)
+    torch.cuda.synchronize()
+    y = torch.cat(parts, 1)
+    assert torch.equal(y[:, :N], pkg.linear_fp8(x, w8, ws))
+    a, b = x.double(), wide.double()
+    want, slack = a @ b.t(), (a.abs() @ b.abs().t()) * (K + K // 128) * ref.U32
+    _check(y[:, N:], want, slack, "bf16 columns")
+
+
 def test_linear_fp8_views_empty_and_non_finite(pkg, dev):
     gen = torch.Generator().manual_seed(8)
     M, N, K = 70, 300, 512
@@ -222,10 +242,14 @@ def test_mixer_with_8_bit_weights(pkg, dev, Hk, Hv, D, hidden):
         cu = torch.tensor([0] + lens).cumsum(0).to(torch.int32).to(dev)
         mine, theirs = [t.clone() for t in pools], [t.clone() for t in pools]
         y = layer.forward(hidden_rows, cu, max(lens), ids, mine[1], mine[0], lens_q=lens)
-        mixed, z = pkg.ops.linear_fp8_cols(hidden_rows, w_in8, w_in_s, [C, V])
-        ba = pkg.linear(hidden_rows, torch.cat([w_b, w_a]))
-        o = core.forward(mixed, z, ba[:, :Hv].contiguous(), ba[:, Hv:].contiguous(), cu, max(lens), ids, theirs[1],
-                         theirs[0], lens_q=lens, fp8=True)
+        if Hv % 16 == 0:
+            mixed, z, b, a = pkg.ops.linear_fp8_cols(hidden_rows, w_in8, w_in_s, [C, V, Hv, Hv],
+                                                     wide=torch.cat([w_b, w_a]))
+        else:
+            mixed, z = pkg.ops.linear_fp8_cols(hidden_rows, w_in8, w_in_s, [C, V])
+            ba = pkg.linear(hidden_rows, torch.cat([w_b, w_a]))
+            b, a = ba[:, :Hv].contiguous(), ba[:, Hv:].contiguous()
+        o = core.forward(mixed, z, b, a, cu, max(lens), ids, theirs[1], theirs[0], lens_q=lens, fp8=True)
         o, s = o if isinstance(o, tuple) else (o, None)
         want = pkg.linear_fp8(o.reshape(N, V), w_out8, w_out_s, x_scale=s)
         torch.cuda.synchronize()

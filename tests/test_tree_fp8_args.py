@@ -91,6 +91,10 @@ def test_8_bit_calls_refuse(ops):
              out=[out.float(), out[:4], out.t(), out.expand(M, N)[:, :100], out[:1].expand(M, N)])
     _refused(ops.linear_fp8_cols, dict(x=x, weight=w8, weight_scale=ws, widths=[96, 104]),
              widths=[[100, 100], [], [96, 96], [16] * 5 + [120], [-16, 216]])
+    w9, wide = torch.zeros(192, K, dtype=FP8), torch.zeros(32, K, dtype=BF16)
+    _refused(ops.linear_fp8_cols, dict(x=x, weight=w9, weight_scale=ws, widths=[192, 16, 16], wide=wide),
+             x=[x8], weight=[w8], widths=[[192], [176, 48], [192, 24, 8], [192, 48]],
+             wide=[wide.float(), wide[:24], wide[:, :128], wide[:0], wide[0]])
     n = torch.zeros(M, 4, 64, dtype=BF16)
     _refused(ops.rms_norm_gated_fp8, dict(hidden_states=n, gate=n, weight=torch.ones(64), eps=1e-6),
              hidden_states=[n.float(), n[:, :3], n[0, 0]], gate=[n.float(), n[:, :2]], weight=[torch.ones(32)])
@@ -143,8 +147,8 @@ def test_c_entry_points_reject_before_launch(pkg):
         assert q(**bad) == inv, bad
     # product
     C1, ld1, end1 = (ctypes.c_void_p * 1)(1 << 20), (ctypes.c_int64 * 1)(96), (ctypes.c_int * 1)(96)
-    f = lambda A=P, lda=256, sa=P, ar=1, B=P, ldb=256, sb=P, br=2, M=4, N=96, K=256, n=1, C=C1, ld=ld1, e=end1, q=0, ws=None, wb=0: (  # noqa: E731,E501
-        lib.gdn_gemm_fp8(A, q, lda, sa, ar, 4, B, ldb, sb, br, M, N, K, n, C, ld, e, ws, wb, None))
+    f = lambda A=P, lda=256, sa=P, ar=1, B=P, ldb=256, sb=P, br=2, M=4, N=96, K=256, n=1, C=C1, ld=ld1, e=end1, q=0, ws=None, wb=0, b2=None, l2=256, n2=0: (  # noqa: E731,E501
+        lib.gdn_gemm_fp8(A, q, lda, sa, ar, 4, B, ldb, sb, br, b2, l2, n2, M, N, K, n, C, ld, e, ws, wb, None))
     assert f(M=0) == ok and f(N=0) == ok
     for bad in (dict(A=None), dict(A=odd), dict(lda=248), dict(lda=128), dict(sa=None), dict(B=None), dict(B=odd),
                 dict(ldb=250), dict(sb=None), dict(br=1), dict(K=0), dict(K=192), dict(n=0), dict(n=5), dict(C=None),
@@ -159,6 +163,12 @@ def test_c_entry_points_reject_before_launch(pkg):
     assert need == 5000 * (256 + 8)
     for bad in (dict(ws=None, wb=need), dict(ws=odd, wb=need), dict(ws=P, wb=need - 1), dict(lda=252)):
         assert f(**{**dict(q=1, M=5000, ws=P, wb=need), **bad}) == inv, bad
+    # bf16 columns behind them: on bf16 rows, in 16s, with a part that ends at N
+    C2, ld2 = (ctypes.c_void_p * 2)(1 << 20, 1 << 20), (ctypes.c_int64 * 2)(96, 96)
+    wide = dict(q=1, b2=P, n2=32, n=2, C=C2, ld=ld2, e=(ctypes.c_int * 2)(96, 128), ws=P, wb=4 * 264)
+    for bad in (dict(q=0), dict(b2=None), dict(b2=odd), dict(n2=24), dict(l2=252), dict(l2=128), dict(n2=-16),
+                dict(e=(ctypes.c_int * 2)(80, 128)), dict(e=(ctypes.c_int * 2)(96, 112)), dict(n=1, e=end1)):
+        assert f(**{**wide, **bad}) == inv, bad
     # norm
     n = lambda x=P, sx=256, w=P, y=P, s=P, N=4, H=2, D=128: lib.gdn_rmsnorm_gated_fp8(  # noqa: E731
         x, sx, P, 256, w, y, s, 1, 4, N, H, D, 1e-6, None)
