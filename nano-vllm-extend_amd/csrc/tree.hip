@@ -14,7 +14,9 @@
 // so the states of the nodes are never stored: a verify reads S once, where the chain
 // form (gdn_recurrent) writes one D x D state per token, and a commit forms one state
 // from the path's k, g and u.  The weights are products of factors in [0, 1], never
-// differences of sums: no cancellation, and a decay of 0 stays 0.
+// differences of sums: no cancellation, and a decay of 0 stays 0.  What has weight 0 is
+// left out, not multiplied: a node sees nothing of what its path has forgotten, nor of
+// unused nodes and other branches, infinities and NaN included.
 #include "gdn_common.h"
 
 namespace {
@@ -332,6 +334,13 @@ struct Tile {
     __builtin_amdgcn_sched_barrier(0);
   }
   __device__ __forceinline__ void scale(float total) {
+    if (total == 0.0f) {  // forgotten, whatever it held
+#pragma unroll
+      for (int kk = 0; kk < D / 32; ++kk)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) s[kk][e] = f32x2_t{0.0f, 0.0f};
+      return;
+    }
 #pragma unroll
     for (int kk = 0; kk < D / 32; ++kk)
 #pragma unroll
@@ -441,8 +450,10 @@ __device__ __forceinline__ void stage_path(const RulePending& pd, const Path& pa
         v[e] = gdn::bf2f(kr[i][e]);
         ss = fmaf(v[e], v[e], ss);
       }
-      *reinterpret_cast<floats*>(&u[p][lane * E]) = ur[i];
-      *reinterpret_cast<floats*>(&wk[p][lane * E]) = v * (path.weight[first + p] * rsqrtf(gdn::wave_sum(ss) + kEps));
+      const float weight = path.weight[first + p], norm = rsqrtf(gdn::wave_sum(ss) + kEps);
+      const bool on = weight != 0.0f;
+      *reinterpret_cast<floats*>(&u[p][lane * E]) = on ? ur[i] : floats(0.0f);
+      *reinterpret_cast<floats*>(&wk[p][lane * E]) = on ? v * (weight * norm) : floats(0.0f);
     }
   }
 }
@@ -799,9 +810,11 @@ __global__ __launch_bounds__(2 * D, NT <= 2 ? 3 : NT == 3 || D == 128 ? 2 : 1) v
     for (int t = 16 * I; t < min(T, 16 * I + 16); ++t) {
       float x = 0.0f, y = 0.0f;
       if (link[t] != kUnused) {
-        x = fv[t] * gdn::bf2f(v[b * v_b + t * v_t + static_cast<int64_t>(h) * D + mine]) + fk[t] * xk[t - 16 * I][mine];
-        y = fq[t] * xq[t - 16 * I][mine];
+        if (fv[t] != 0.0f) x = fv[t] * gdn::bf2f(v[b * v_b + t * v_t + static_cast<int64_t>(h) * D + mine]);
+        if (fk[t] != 0.0f) x += fk[t] * xk[t - 16 * I][mine];
+        if (fq[t] != 0.0f) y = fq[t] * xq[t - 16 * I][mine];
         for (int s = link[t]; s >= 0; s = link[s]) {
+          if (wt[t][s] == 0.0f) continue;
           const float us = u[out0 + s * out_t + mine];
           x = fmaf(cu[t][s], us, x);
           y = fmaf(co[t][s], us, y);

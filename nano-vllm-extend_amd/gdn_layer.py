@@ -131,7 +131,10 @@ class TreeStep:
     accepted paths: the raw rows, the keys after the conv, the gates, the
     corrections and the trees (GatedDeltaNetCore.verify_tree).  accept() names the
     last accepted node of each sequence; the step is then the next verify's
-    `pending`, or goes to commit_tree."""
+    `pending`, for the same sequences in the same rows, or goes to commit_tree.
+    x, parents and accepted are the caller's tensors, not copies: they stay as they
+    are until the step is in the pools (two buffers in turn, where a graph replays
+    the steps)."""
     x: torch.Tensor          # [B, T, C]
     k: torch.Tensor          # [B, T, Hk, D]
     g: torch.Tensor          # [B, T, Hv]
@@ -685,12 +688,11 @@ class GatedDeltaNetLayer:
         """The mixer of one verify step over trees of T drafted tokens: hidden [B, T,
         hidden] bf16 -> ([B, T, hidden] bf16, TreeStep).  ids, parents and pending as
         GatedDeltaNetCore.verify_tree; in_proj, core and out_proj as forward."""
-        B, T, _ = hidden.shape
-        mixed, z, b, a, _ = self.project_in(hidden.reshape(B * T, -1))
+        B, T, width = hidden.shape
+        rows = self.project_in(hidden.reshape(B * T, width))[:4]
         self.core.timer = self.timer
-        core, step = self.core.verify_tree(mixed.reshape(B, T, -1), z.reshape(B, T, -1), b.reshape(B, T, -1),
-                                           a.reshape(B, T, -1), ids, conv_cache, s_cache, parents, pending=pending,
-                                           fp8=self.fp8)
+        core, step = self.core.verify_tree(*(t.reshape(B, T, t.shape[1]) for t in rows), ids, conv_cache, s_cache,
+                                           parents, pending=pending, fp8=self.fp8)
         if not isinstance(core, tuple):
             core = core.reshape(B, T, self.core.value_dim)
         return self._project_out(core, hidden.shape), step

@@ -928,8 +928,10 @@ def conv_tree_step(x: torch.Tensor, conv_pool: torch.Tensor, ids: torch.Tensor, 
     parent is neither -1 nor an earlier used node (-2 for padding) is unused and
     its output 0.  A sequence whose id is no slot has zero outputs.
 
-    pending = (x, parents, accepted) of the step before: the rows on the path to
-    node accepted[b] of each sequence (-1: none) go into the pool first.  Along a
+    pending = (x, parents, accepted) of the step before, for the same sequences in
+    the same rows: the rows on the path to node accepted[b] of each sequence (-1:
+    none) go into the pool first, so a slot is in ids at most once among the rows
+    with an accepted node (a padded batch's rows: id -1, or accepted -1).  Along a
     path the results are conv_decode_step's, bit for bit.  Returns y [B, T, C].
     (No reference counterpart: spec decode is disabled for qwen3_5,
     nanovllm/config.py:84.)"""
@@ -971,9 +973,11 @@ def recurrent_gdn_tree(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: tor
     Returns (o [B, T, Hv, D] bf16, u [B, T, Hv, D] fp32): the outputs, and the
     corrections from which, with k and g, the state after any node follows (no
     state of a node is stored).  pending = (k, g, u, parents, accepted) of the
-    step before: the states after the accepted nodes go into the pool first, in
-    the same pass over them, and the trees start from there (accepted[b] -1, or no
-    used node: the row's state stays).
+    step before, for the same sequences in the same rows: the states after the
+    accepted nodes go into the pool first, in the same pass over them, and the
+    trees start from there (accepted[b] -1, or no used node: the row's state stays;
+    slots as conv_tree_step's).  A decay of 0 (g = -inf) forgets what came before
+    it, also what is not finite.
     (No reference counterpart: spec decode is disabled for qwen3_5,
     nanovllm/config.py:84; one token: qwen3_5.py:575-594.)"""
     last_k, last_g, last_u, last_parents, accepted = pending if pending is not None else (None,) * 5
@@ -1019,7 +1023,8 @@ def commit_tree(s_pool: torch.Tensor, conv_pool: torch.Tensor, ids: torch.Tensor
     """The accepted path of a verified tree into both pools, for another user of the
     slots than the next verify (whose `pending` does the same): row ids[b] of
     s_pool becomes the state after node accepted[b], that of conv_pool the last
-    three raw rows on its path; -1 (or no used node) leaves both as they are.
+    three raw rows on its path; -1 (or no used node) leaves both as they are (slots
+    as conv_tree_step's).
     x [B, T, C] the raw rows, k [B, T, Hk, D], g [B, T, Hv], u [B, T, Hv, D] and
     parents those of the verified step."""
     idx = _device_of(s_pool, conv_pool, ids, parents, accepted, x, k, g, u)
@@ -1247,7 +1252,8 @@ def _linear_fp8(x, weight, weight_scale, x_scale, M, N, K, outs, widths, wide=No
         w = w.contiguous() if not w.is_contiguous() else w.clone(memory_format=torch.contiguous_format)
         w_st = (K, 1)
     G = K // FP8_GROUP
-    ws = weight_scale if weight_scale.stride(1) == 1 or G == 1 else weight_scale.contiguous()
+    ws_st = weight_scale.stride()
+    ws = weight_scale if (ws_st[1] == 1 or G == 1) and (ws_st[0] >= G or N <= FP8_GROUP) else weight_scale.contiguous()
     bf16 = x_scale is None
     x2, _, x_row = _rows_of(x, 8 if bf16 else 16)
     work, ws_bytes, xs = None, 0, (None, 0, 0)

@@ -255,3 +255,30 @@ def test_mixer_with_8_bit_weights(pkg, dev, Hk, Hv, D, hidden):
         torch.cuda.synchronize()
         assert (s is not None) == (1 not in lens)
         assert torch.equal(y, want) and torch.equal(mine[0], theirs[0]) and torch.equal(mine[1], theirs[1])
+
+
+def test_other_stream_and_one_scale_for_all(pkg, dev):
+    """On a second stream the same bits; a broadcast scale is its copies."""
+    gen = torch.Generator().manual_seed(53)
+    x, w = _rows(gen, 40, 384).to(BF16).to(dev), (torch.randn(300, 384, generator=gen) * 0.05).to(BF16).to(dev)
+    o, z = (torch.randn(33, 4, 128, generator=gen).to(BF16).to(dev) for _ in range(2))
+    weight = torch.rand(128, generator=gen).to(BF16).to(dev)
+
+    def run():
+        x8, xs = pkg.quantize_fp8(x)
+        w8, ws = pkg.quantize_weight_fp8(w)
+        one = torch.full((1, 1), 0.25, device=dev)
+        return (x8.view(torch.uint8), xs, pkg.linear_fp8(x, w8, ws), pkg.linear_fp8(x8, w8, ws, x_scale=xs),
+                pkg.linear_fp8(x8, w8, one.expand(3, 3), x_scale=one.expand(40, 3)),
+                pkg.linear_fp8(x8, w8, torch.full((3, 3), 0.25, device=dev),
+                               x_scale=torch.full((40, 3), 0.25, device=dev)),
+                pkg.rms_norm_gated_fp8(o, z, weight, 1e-6)[0].view(torch.uint8))
+
+    want = run()
+    torch.cuda.synchronize()
+    assert torch.equal(want[4], want[5])
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        got = run()
+    side.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))

@@ -372,3 +372,128 @@ def test_other_stream(pkg, dev):
         got = pkg.recurrent_gdn_tree(*args)
     side.synchronize()
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_not_finite_stays_on_its_branch(pkg, dev):
+    """Infinities and NaN in the rows of some nodes, of unused ones among them: every value
+    that the 64-bit form has finite is within its bound, the others are not finite."""
+    gen = torch.Generator().manual_seed(31)
+    B, T, Hk, Hv, D = 4, 40, 1, 2, 128
+    i = _inputs(gen, B, T, Hk, Hv, D, slow=True)
+    parents, _ = ref.tree(gen, B, T, 6)
+    parents[:, 1::9] = 0                                 # branches from the root's child on
+    parents[:, 20] = -2                                  # unused, and what follows it
+    q, k, v = _qkv(i["y"], Hk, Hv, D)
+    nan, inf = float("nan"), float("inf")
+    k[0, 3, 0, 5], v[0, 20], k[0, 20], q[0, 9, 0, 1] = nan, nan, inf, nan
+    v[1, 2, 1, 77], v[1, 18, 0, 3] = inf, nan
+    i["g"][2, 7], i["beta"][2, 30, 1] = nan, nan
+    k[3, 20], q[3, 20], v[3, 20], i["g"][3, 20], i["beta"][3, 20] = nan, nan, nan, nan, nan
+    pool = torch.randn(B, Hv, D, D, generator=gen) * 0.3
+    o, u = pkg.recurrent_gdn_tree(*_qkv(i["y"].to(dev), Hk, Hv, D), i["g"].to(dev), i["beta"].to(dev), pool.to(dev),
+                                  torch.arange(B, device=dev), parents.to(dev))
+    torch.cuda.synchronize()
+    o, u = o.cpu().double(), u.cpu().double()
+    for b in range(B):
+        ro, ru, _, eo, eu = ref.rule(q[b], k[b], v[b], i["g"][b], i["beta"][b], pool[b], parents[b])
+        for got, want, bound in ((u[b], ru, eu), (o[b], ro, eo + ref.HALF_BF16 * (ro.abs() + eo))):
+            ok = want.isfinite()
+            assert 0 < int(ok.sum()) and (b == 3) == bool(ok.all())
+            assert torch.equal(got.isfinite(), ok)
+            _close(got[ok], want[ok], bound[ok] + 1e-30, f"row {b}")
+
+
+def test_a_decay_of_zero_forgets_what_is_not_finite(pkg, dev):
+    """A state and corrections that are not finite, behind a decay of 0: outputs and committed
+    states are those of the 64-bit form on a state of zeros."""
+    gen = torch.Generator().manual_seed(37)
+    B, T, Hk, Hv, D = 2, 19, 1, 2, 128
+    i = _inputs(gen, B, T, Hk, Hv, D, slow=True)
+    parents = torch.arange(-1, T - 1, dtype=torch.int32)
+    parents[9] = -1                                      # a second root: 9, and the chain behind it
+    q, k, v = _qkv(i["y"], Hk, Hv, D)
+    i["g"][:, 9], i["g"][:, 4] = float("-inf"), float("-inf")
+    v[0, 2] = float("nan")                               # a correction that node 4 forgets
+    pool = torch.full((B, Hv, D, D), float("nan"))
+    ids, node = torch.arange(B), torch.tensor([T - 1, 6])
+    dv = lambda *ts: tuple(t.to(dev) for t in ts)  # noqa: E731
+    kd = _qkv(i["y"].to(dev), Hk, Hv, D)
+    pd, cd = pool.to(dev), torch.zeros(B, i["x"].shape[2], 3, dtype=BF16, device=dev)
+    o, u = pkg.recurrent_gdn_tree(*kd, *dv(i["g"], i["beta"]), pd, *dv(ids, parents))
+    pkg.commit_tree(pd, cd, *dv(ids, parents, node, i["x"]), kd[1], i["g"].to(dev), u)
+    torch.cuda.synchronize()
+    o, u, pd = o.cpu().double(), u.cpu().double(), pd.cpu()
+    v = v.clone()
+    v[0, 2] = 0
+    for b in range(B):
+        ro, ru, states, eo, eu = ref.rule(q[b], k[b], v[b], i["g"][b], i["beta"][b], torch.zeros(Hv, D, D), parents)
+        seen = torch.arange(T) >= 4
+        _close(u[b][seen], ru[seen], eu[seen], f"row {b}: u")
+        _close(o[b][seen], ro[seen], (eo + ref.HALF_BF16 * (ro.abs() + eo))[seen], f"row {b}: o")
+        assert not u[b][~seen].isfinite().any() and not o[b][~seen].isfinite().any()
+        P, A, depth = states[int(node[b])]
+        _close(pd[b], P, (2 * D + 3 * T + 64) * (depth + 2) * ref.U32 * A + 1e-30, f"row {b}: state")
+
+
+@pytest.mark.parametrize("taps,lead", [(4, 0), (3, 2), (8, 6), (3, 1)])
+def test_conv_pools_of_other_layouts(pkg, dev, taps, lead):
+    """Taps that lie apart, and pools that begin in the middle of a 16- or 4-byte piece."""
+    gen = torch.Generator().manual_seed(41)
+    B, T, C, slots = 3, 9, 264, 4
+    n = lambda *s: torch.randn(*s, generator=gen).to(BF16)  # noqa: E731
+    x, last_x, w = n(B, T, C), n(B, T, C), n(C, 4)
+    parents, _ = ref.tree(gen, B, T, 3)
+    accepted = torch.tensor([4, 8, 0])
+    flat = n(slots * C * taps + lead)
+    view = lambda t: t[lead:].view(slots, C, taps)[..., :3]  # noqa: E731
+    ids = torch.tensor([2, 0, 3])
+    flat_d, flat_2 = flat.to(dev), flat.to(dev)
+    dv = lambda *ts: tuple(t.to(dev) for t in ts)  # noqa: E731
+    y = pkg.conv_tree_step(*dv(x), view(flat_d), *dv(ids, w, parents), pending=dv(last_x, parents, accepted))
+    Hv, D = 1, 64                                        # commit_tree beside a small state
+    k, g, u = n(B, T, 1, D), torch.zeros(B, T, Hv), torch.zeros(B, T, Hv, D)
+    pkg.commit_tree(torch.zeros(slots, Hv, D, D, device=dev), view(flat_2),
+                    *dv(ids, parents, accepted, last_x, k, g, u))
+    torch.cuda.synchronize()
+    want = flat.clone()
+    for b in range(B):
+        view(want)[ids[b]] = ref.taps_after(view(want)[ids[b]], last_x[b], parents[b], int(accepted[b]))
+        ry, e = ref.conv(x[b], view(want)[ids[b]], w, parents[b])
+        _close(y[b], ry, e, f"row {b}")
+    assert torch.equal(flat_d.cpu(), want) and torch.equal(flat_2.cpu(), want)
+
+
+def test_no_sequences(pkg, dev):
+    gen = torch.Generator().manual_seed(43)
+    for weights in ("bf16", "fp8"):
+        layer = _mixer(pkg, gen, dev, weights, 2, 16, 64, 256)
+        pool, cpool = torch.ones(2, 16, 64, 64, device=dev), torch.ones(2, layer.core.conv_dim, 3, dtype=BF16, device=dev)
+        none = torch.empty(0, dtype=torch.int64, device=dev)
+        parents = torch.empty(0, 5, dtype=torch.int32, device=dev)
+        y, step = layer.verify_tree(torch.empty(0, 5, 256, dtype=BF16, device=dev), none, cpool, pool, parents)
+        y, step = layer.verify_tree(torch.empty(0, 5, 256, dtype=BF16, device=dev), none, cpool, pool, parents,
+                                    pending=step.accept(none))
+        layer.commit_tree(step.accept(none), none, cpool, pool)
+        torch.cuda.synchronize()
+        assert y.shape == (0, 5, 256) and bool((pool == 1).all()) and bool((cpool == 1).all())
+
+
+def test_rows_of_a_slot_that_is_read_only_twice(pkg, dev):
+    """The same slot in several rows, with nothing accepted in all but one of them."""
+    gen = torch.Generator().manual_seed(47)
+    B, T, Hk, Hv, D = 4, 6, 1, 2, 128
+    i, last = _inputs(gen, B, T, Hk, Hv, D), _inputs(gen, B, T, Hk, Hv, D)
+    parents, _ = ref.tree(gen, B, T, 2)
+    pool = torch.randn(2, Hv, D, D, generator=gen) * 0.3
+    ids, accepted = torch.tensor([1, 0, 0, 0]), torch.tensor([3, -1, -1, -1])
+    dv = lambda *ts: tuple(t.to(dev) for t in ts)  # noqa: E731
+    pd = pool.to(dev)
+    kk = _qkv(last["y"], Hk, Hv, D)[1]
+    o, _ = pkg.recurrent_gdn_tree(*_qkv(i["y"].to(dev), Hk, Hv, D), *dv(i["g"], i["beta"]), pd, *dv(ids, parents),
+                                  pending=dv(kk, last["g"], last["u"], parents, accepted))
+    torch.cuda.synchronize()
+    assert torch.equal(pd[0].cpu(), pool[0])
+    q, k, v = _qkv(i["y"], Hk, Hv, D)
+    for b in range(B):
+        ro, _, _, eo, _ = ref.rule(q[b], k[b], v[b], i["g"][b], i["beta"][b], pd[ids[b]].cpu(), parents[b])
+        _close(o[b], ro, eo + ref.HALF_BF16 * (ro.abs() + eo), f"row {b}")
