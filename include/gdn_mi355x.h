@@ -485,15 +485,17 @@ int gdn_rmsnorm_gated_fp8(const uint16_t* x, int64_t sx_tok, const uint16_t* z, 
 
 /*
  * Speculative verify over a tree of drafted tokens (no counterpart in the reference:
- * spec decode is disabled for qwen3_5, nanovllm/config.py:84).  Three entry points:
+ * spec decode is disabled for qwen3_5, nanovllm/config.py:84).  Four entry points:
  * the conv and the gated delta rule of T nodes (1 to 64) per sequence against the
- * pools, and the accepted paths' way into the pools.
+ * pools, the rule with the layer's gates and norm, and the accepted paths' way into
+ * the pools.
  *   parents  int32, of sequence b at parents + b p_b (0: one tree for all): the node
  *            before node t: -1 the sequence's own state (a tree may have several such
  *            nodes), else a node s < t.  Any other value (-2 for padding) or an unused
  *            parent makes node t unused: its outputs are 0 and it has no effect.
  *   ids      int64 [B] slots; a sequence whose slot is outside [0, n_slots) has outputs 0
- *            and nothing of it is written.  Duplicate ids (the dummy slot) are tolerated.
+ *            and nothing of it is written.  A slot may come more than once (the dummy slot)
+ *            as long as one of its rows at most has an accepted node.
  *   accepted int64 [B] or NULL: the node of the step before, last_*, up to which its
  *            tokens were accepted.  Its path from the root goes into the pool rows first
  *            (in place), and the new tree starts from there; a value that is no used
@@ -530,6 +532,24 @@ int gdn_rule_tree(const uint16_t* q, int64_t q_b, int64_t q_t, const uint16_t* k
                   const uint16_t* last_k, int64_t lk_b, int64_t lk_t, const float* last_g, const float* last_u,
                   const int32_t* last_parents, int64_t lp_b, const int64_t* accepted, int last_T, uint16_t* o,
                   float* u, int B, int T, int Hk, int Hv, int D, float scale, void* stream);
+
+/*
+ * gdn_rule_tree_layer: gdn_rule_tree with the layer's gates before it (gdn_g_beta on b,
+ * a [B, T, Hv] contiguous) and its gated norm behind it (z [B, T, Hv * D], strides z_b,
+ * z_t as q's; w [D]) in the same launch: y as gdn_rmsnorm_gated gives it from o, or, D =
+ * 128, y8 and y8_scale as gdn_rmsnorm_gated_fp8 (scale of token i = b T + t, head h at h B
+ * T + i); one of y and y8 is NULL.  g [B, T, Hv] fp32 is written for the next step's
+ * last_g.  Unused nodes give zeros; rows of a slot that is none zeros in u and g too.
+ */
+int gdn_rule_tree_layer(const uint16_t* q, int64_t q_b, int64_t q_t, const uint16_t* k, int64_t k_b, int64_t k_t,
+                        const uint16_t* v, int64_t v_b, int64_t v_t, const uint16_t* b, const uint16_t* a,
+                        const void* A_log, const void* dt_bias, int param_is_fp32, float* s_pool, int64_t s_slot,
+                        int64_t n_slots, const int64_t* ids, const int32_t* parents, int64_t p_b,
+                        const uint16_t* last_k, int64_t lk_b, int64_t lk_t, const float* last_g, const float* last_u,
+                        const int32_t* last_parents, int64_t lp_b, const int64_t* accepted, int last_T,
+                        const uint16_t* z, int64_t z_b, int64_t z_t, const uint16_t* w, float eps, uint16_t* y,
+                        uint8_t* y8, float* y8_scale, float* u, float* g, int B, int T, int Hk, int Hv, int D,
+                        float scale, void* stream);
 
 /* gdn_commit_tree: the accepted paths into the state and conv pools (x, k, g, u and
  * parents of the verified step). */

@@ -30,6 +30,7 @@ from .ops import (  # noqa: F401
     recurrent_gdn_inplace,
     recurrent_gdn_multitoken,
     recurrent_gdn_tree,
+    recurrent_tree_fused,
     rms_norm_gated,
     rms_norm_gated_fp8,
 )

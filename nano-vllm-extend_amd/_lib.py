@@ -76,6 +76,9 @@ SIGNATURES: dict[str, list] = {
                       _i32, _i32, _i32, _p],
     "gdn_rule_tree": [_p, _i64, _i64, _p, _i64, _i64, _p, _i64, _i64, _p, _p, _p, _i64, _i64, _p, _p, _i64, _p, _i64,
                       _i64, _p, _p, _p, _i64, _p, _i32, _p, _p, _i32, _i32, _i32, _i32, _i32, _f32, _p],
+    "gdn_rule_tree_layer": [_p, _i64, _i64, _p, _i64, _i64, _p, _i64, _i64, _p, _p, _p, _p, _i32, _p, _i64, _i64, _p,
+                            _p, _i64, _p, _i64, _i64, _p, _p, _p, _i64, _p, _i32, _p, _i64, _i64, _p, _f32, _p, _p, _p,
+                            _p, _p, _i32, _i32, _i32, _i32, _i32, _f32, _p],
     "gdn_commit_tree": [_p, _i64, _p, _i64, _i64, _i64, _p, _p, _i64, _p, _p, _i64, _i64, _p, _i64, _i64, _p, _p,
                         _i32, _i32, _i32, _i32, _i32, _i32, _p],
 }

@@ -280,6 +280,12 @@ __global__ __launch_bounds__(64) void conv_tree_kernel(const uint16_t* __restric
 // fp32 products of 16 x 16 x 4, in which a lane's results are its part of the next
 // operand (register r of lane group lg: node 4 lg + r), so that nothing goes through LDS.
 //
+// kLayer: the layer's gates before it and its gated norm behind it in the same launch.  Wave
+// 0 finds the gates of the head's nodes.  A tile's outputs, rounded to bf16 as without the
+// norm, meet in LDS, and D / 8 lanes per row take the norm in the order of its own kernel.
+// Two launches and the outputs' way out and in less: 64 trees of 16 nodes 65.7 us for the
+// 71.8 of three launches, one of 8 nodes 10.9 for 14.3 (32 heads of 128, with a pending path).
+//
 // What bounds it: the state's way in (and out, where a path is pending).  The tree's
 // weights, the nodes' norms and dot products (on the matrix cores as well) and the
 // pending path's rows are worked on while the state is on its way.
@@ -482,14 +488,28 @@ __device__ __forceinline__ gdn::f32x4_t mul16(const gdn::f32x4_t& a, const gdn::
 
 __device__ __forceinline__ const gdn::f32x4_t& four(const float* p) { return *reinterpret_cast<const gdn::f32x4_t*>(p); }
 
+// The layer around the rule: what the gates and the norm take and give.
+struct TreeLayer {
+  const uint16_t *b, *a;        // [B, T, Hv] contiguous
+  const void *A_log, *dt_bias;  // [Hv]
+  int param_f32;
+  float* g;                     // out, [B, T, Hv]
+  const uint16_t* z;            // [B, T, Hv D], strides z_b, z_t
+  int64_t z_b, z_t;
+  const uint16_t* w;            // [D]
+  float eps;
+  uint8_t* y8;                  // D = 128: [B, T, Hv, D] e4m3 in o's place (else NULL), with
+  float* scale;                 // a scale per row, row i of head h at h M + i, M = B T
+};
+
 // NT: 16-node tiles of the tree.
-template <int D, int NT>
+template <int D, int NT, bool kLayer>
 __global__ __launch_bounds__(2 * D, NT <= 2 ? 3 : NT == 3 || D == 128 ? 2 : 1) void rule_tree_kernel(
     const uint16_t* __restrict__ q, int64_t q_b, int64_t q_t, const uint16_t* __restrict__ k, int64_t k_b, int64_t k_t,
     const uint16_t* __restrict__ v, int64_t v_b, int64_t v_t, const float* __restrict__ g,
     const uint16_t* __restrict__ beta, float* __restrict__ pool, int64_t s_slot, int64_t n_slots,
     const int64_t* __restrict__ ids, const int32_t* __restrict__ parents, int64_t p_b, RulePending pd,
-    uint16_t* __restrict__ o, float* __restrict__ u, int B, int T, int Hk, int Hv, float scale) {
+    uint16_t* __restrict__ o, float* __restrict__ u, int B, int T, int Hk, int Hv, float scale, TreeLayer L) {
   constexpr int NW = D / 32, KK = D / 32, TM = 16 * NT;
   __shared__ __align__(16) float wt[TM][TM];    // weights w(t, s)
   __shared__ __align__(16) float cu[TM][TM];    // minus the coefficients of u_s in u_t
@@ -502,6 +522,8 @@ __global__ __launch_bounds__(2 * D, NT <= 2 ? 3 : NT == 3 || D == 128 ? 2 : 1) v
   __shared__ __align__(16) float fv[TM], fk[TM], fq[TM];  // factors of v, S^T k, S^T q: 0 for an unused node
   __shared__ int any_cu[NT][NT];                // whether a tile of coefficients holds an ancestor
   __shared__ Path path;
+  __shared__ __align__(16) uint16_t rows[kLayer ? 2 : 1][kLayer ? 16 : 1][D + 8];  // a tile's outputs, two in turn
+  __shared__ int bad;                           // a correction is not finite
 
   const int64_t wi = gdn::xcd_remap(blockIdx.x, static_cast<int64_t>(B) * Hv);
   if (wi < 0) return;
@@ -515,8 +537,13 @@ __global__ __launch_bounds__(2 * D, NT <= 2 ? 3 : NT == 3 || D == 128 ? 2 : 1) v
   const int64_t slot = ids[b];
   if (slot < 0 || slot >= n_slots) {  // (the whole workgroup)
     for (int t = tid / D; t < T; t += 2) {
-      o[out0 + t * out_t + tid % D] = 0;
+      if (kLayer && L.y8) L.y8[out0 + t * out_t + tid % D] = 0;
+      else o[out0 + t * out_t + tid % D] = 0;
       u[out0 + t * out_t + tid % D] = 0.0f;
+    }
+    if (kLayer && tid < T) {
+      L.g[(static_cast<int64_t>(b) * T + tid) * Hv + h] = 0.0f;
+      if (L.y8) L.scale[static_cast<int64_t>(h) * B * T + static_cast<int64_t>(b) * T + tid] = gdn::fp8_scale(0.0f);
     }
     return;
   }
@@ -529,12 +556,17 @@ __global__ __launch_bounds__(2 * D, NT <= 2 ? 3 : NT == 3 || D == 128 ? 2 : 1) v
   auto k_frag = [&](int I, int kk) { return buf_row(bk, min(16 * I + lr, T - 1) * k_row + 16 * lg + 64 * kk); };
   auto q_frag = [&](int I, int kk) { return buf_row(bq, min(16 * I + lr, T - 1) * q_row + 16 * lg + 64 * kk); };
   int my_parent = 0;
-  float my_g = 0.0f, my_beta = 0.0f;
+  float my_g = 0.0f, my_beta = 0.0f, A_log = 0.0f, dt_bias = 0.0f;
   PathIn pin = {-1, 0.0f, 0};
   if (wave == 0) {
     const int64_t at = (static_cast<int64_t>(b) * T + min(lane, T - 1)) * Hv + h;
-    my_g = g[at];
-    my_beta = gdn::bf2f(beta[at]);
+    // (with the layer: a and b as they are, until the loads are on their way)
+    my_g = kLayer ? gdn::bf2f(L.a[at]) : g[at];
+    my_beta = gdn::bf2f((kLayer ? L.b : beta)[at]);
+    if (kLayer) {
+      A_log = gdn::load_param(L.A_log, h, L.param_f32);
+      dt_bias = gdn::load_param(L.dt_bias, h, L.param_f32);
+    }
     my_parent = parents[b * p_b + min(lane, T - 1)];
   } else if (wave == 1 && pd.accepted) {
     pin.load(pd, b, h, Hv, lane);
@@ -574,6 +606,12 @@ __global__ __launch_bounds__(2 * D, NT <= 2 ? 3 : NT == 3 || D == 128 ? 2 : 1) v
   // --- the tree: lane t of wave 0 from node t up to the root; the pending path ---
   if (wave == 0) {
     for (int i = lane; i < TM * TM / 4; i += 64) reinterpret_cast<float4*>(wt)[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (kLayer) {
+      my_g = gdn::gate_g(my_g, A_log, dt_bias);
+      my_beta = gdn::bf2f(gdn::gate_beta(my_beta));
+      if (lane < T) L.g[(static_cast<int64_t>(b) * T + lane) * Hv + h] = my_g;
+      if (lane == 0) bad = 0;
+    }
     const float dec = expf(my_g);
     bool fine = lane < T && my_parent >= -1 && my_parent < lane;
     int s = fine ? my_parent : -1;
@@ -712,6 +750,59 @@ __global__ __launch_bounds__(2 * D, NT <= 2 ? 3 : NT == 3 || D == 128 ? 2 : 1) v
   // (the nodes' rows come again, from the caches, one product ahead: held in registers from
   // the start they would cost a workgroup per CU)
   const int tiles = (T + 15) / 16;
+  constexpr int kLanes = D / 8;  // of a row in the norm: 8 columns each
+  const int row = tid / kLanes, c8 = tid % kLanes * 8;
+  auto z_row = [&](int I) {
+    return *reinterpret_cast<const uint4*>(L.z + b * L.z_b + min(16 * I + row, T - 1) * L.z_t +
+                                           static_cast<int64_t>(h) * D + c8);
+  };
+  uint4 zv, wv;
+  if constexpr (kLayer) {
+    zv = z_row(0);
+    wv = *reinterpret_cast<const uint4*>(L.w + c8);
+  }
+  // the gated norm of tile I's rows, as its own kernels take it
+  auto norm_rows = [&](int I) {
+    const int t = 16 * I + row;
+    uint16_t xs[8], zs[8], ws[8];
+    __builtin_memcpy(xs, &rows[I & 1][kLayer ? row : 0][c8], 16);
+    __builtin_memcpy(zs, &zv, 16);
+    __builtin_memcpy(ws, &wv, 16);
+    float v[8], ss = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      v[i] = gdn::bf2f(xs[i]);
+      ss += v[i] * v[i];
+    }
+#pragma unroll
+    for (int m = kLanes / 2; m >= 1; m >>= 1) ss += __shfl_xor(ss, m, 64);
+    const float r = rsqrtf(ss / static_cast<float>(D) + L.eps);
+    const bool on = link[t] != kUnused;
+    const int64_t at = out0 + t * out_t + c8;
+    if (D == 128 && L.y8) {
+      float top = 0.0f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        v[i] = on ? v[i] * r * gdn::bf2f(ws[i]) * gdn::silu_ulp(gdn::bf2f(zs[i])) : 0.0f;
+        top = fmaxf(top, fabsf(v[i]));
+      }
+#pragma unroll
+      for (int m = 8; m >= 1; m >>= 1) top = fmaxf(top, __shfl_xor(top, m, 64));
+      const float s = gdn::fp8_scale(top), inv = 1.0f / s;
+      if (t < T) {
+        *reinterpret_cast<uint2*>(L.y8 + at) =
+            make_uint2(gdn::f2fp8x4(v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv),
+                       gdn::f2fp8x4(v[4] * inv, v[5] * inv, v[6] * inv, v[7] * inv));
+        if (c8 == 0) L.scale[static_cast<int64_t>(h) * B * T + static_cast<int64_t>(b) * T + t] = s;
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = on ? gdn::norm_gate(v[i], r, gdn::bf2f(ws[i]), gdn::bf2f(zs[i])) : 0.0f;
+      if (t < T)
+        *reinterpret_cast<uint4*>(o + at) = make_uint4(gdn::f2bf2(v[0], v[1]), gdn::f2bf2(v[2], v[3]),
+                                                       gdn::f2bf2(v[4], v[5]), gdn::f2bf2(v[6], v[7]));
+    }
+  };
   gdn::s16x8_t nk = k_frag(0, 0), nq = q_frag(0, 0);
 #pragma unroll
   for (int kk = 0; kk < KK; ++kk) {
@@ -783,13 +874,25 @@ __global__ __launch_bounds__(2 * D, NT <= 2 ? 3 : NT == 3 || D == 128 ? 2 : 1) v
     for (int r = 0; r < 4; ++r) {
       const int t = 16 * I + 4 * lg + r;
       fine &= finite(uu[I][0][r]) && finite(uu[I][1][r]);
-      if (t < T) {
-        *reinterpret_cast<f32x2_t*>(u + out0 + t * out_t + col) = f32x2_t{uu[I][0][r], uu[I][1][r]};
-        *reinterpret_cast<uint32_t*>(o + out0 + t * out_t + col) = gdn::f2bf2(out[0][r], out[1][r]);
-      }
+      if (t < T) *reinterpret_cast<f32x2_t*>(u + out0 + t * out_t + col) = f32x2_t{uu[I][0][r], uu[I][1][r]};
+      const uint32_t pair = gdn::f2bf2(out[0][r], out[1][r]);
+      if constexpr (kLayer) *reinterpret_cast<uint32_t*>(&rows[I & 1][4 * lg + r][col]) = pair;
+      else if (t < T) *reinterpret_cast<uint32_t*>(o + out0 + t * out_t + col) = pair;
+    }
+    if constexpr (kLayer) {
+      if (__any(!fine) && lane == 0) bad = 1;
+      gdn::lds_barrier();
+      const uint4 next = I + 1 < tiles ? z_row(I + 1) : zv;
+      norm_rows(I);
+      zv = next;
     }
   }
-  if (!__any(!fine)) return;
+  if constexpr (kLayer) {
+    if (!bad) return;  // (the whole workgroup)
+    gdn::lds_barrier();
+  } else if (!__any(!fine)) {
+    return;
+  }
 
   // --- where a correction is not finite (an infinity or a NaN in a row or in the state): the
   // products above let it into every node of its column, coefficient 0 or not.  So the
@@ -823,10 +926,16 @@ __global__ __launch_bounds__(2 * D, NT <= 2 ? 3 : NT == 3 || D == 128 ? 2 : 1) v
       }
       if (lane < 32) {
         u[out0 + t * out_t + mine] = x;
-        o[out0 + t * out_t + mine] = gdn::f2bf(y);
+        if constexpr (kLayer) rows[I & 1][t - 16 * I][mine] = gdn::f2bf(y);
+        else o[out0 + t * out_t + mine] = gdn::f2bf(y);
       }
     }
     wave_lds_order();
+    if constexpr (kLayer) {
+      gdn::lds_barrier();
+      zv = z_row(I);
+      norm_rows(I);
+    }
   }
 }
 
@@ -898,6 +1007,50 @@ bool rows_ok(const void* p, int64_t s_b, int64_t s_t, int width, int T) {
          s_t < (1 << 24) && s_b >= 0 && T >= 1 && T <= kMaxNodes;
 }
 
+struct RuleRows {
+  const uint16_t* q;
+  int64_t q_b, q_t;
+  const uint16_t* k;
+  int64_t k_b, k_t;
+  const uint16_t* v;
+  int64_t v_b, v_t;
+};
+
+int rule_check(const RuleRows& r, const float* s_pool, int64_t s_slot, int64_t n_slots, const int64_t* ids,
+               const int32_t* parents, int64_t p_b, const RulePending& pd, const float* u, int B, int T, int Hk, int Hv,
+               int D) {
+  if (B < 0 || T < 0 || Hk <= 0 || Hv <= 0 || Hv % Hk || n_slots < 0) return GDN_ERR_INVALID_ARG;
+  if (T > kMaxNodes || (pd.accepted && pd.T > kMaxNodes) || (D != 64 && D != 128)) return GDN_ERR_UNSUPPORTED;
+  if (B == 0 || T == 0) return GDN_OK;
+  if (!rows_ok(r.q, r.q_b, r.q_t, Hk * D, T) || !rows_ok(r.k, r.k_b, r.k_t, Hk * D, T) ||
+      !rows_ok(r.v, r.v_b, r.v_t, Hv * D, T) || !s_pool || !ids || !parents || !u || p_b < 0 ||
+      s_slot < static_cast<int64_t>(Hv) * D * D || s_slot % 4 || reinterpret_cast<uintptr_t>(s_pool) % 16 ||
+      reinterpret_cast<uintptr_t>(u) % 16)
+    return GDN_ERR_INVALID_ARG;
+  if (pd.accepted && (!rows_ok(pd.k, pd.k_b, pd.k_t, Hk * D, pd.T) || !pd.g || !pd.u || !pd.parents || pd.p_b < 0 ||
+                      reinterpret_cast<uintptr_t>(pd.u) % 16))
+    return GDN_ERR_INVALID_ARG;
+  return static_cast<int64_t>(B) * Hv >= (1LL << 24) ? GDN_ERR_UNSUPPORTED : GDN_OK;
+}
+
+template <bool kLayer>
+int rule_launch(const RuleRows& r, const float* g, const uint16_t* beta, float* s_pool, int64_t s_slot, int64_t n_slots,
+                const int64_t* ids, const int32_t* parents, int64_t p_b, const RulePending& pd, uint16_t* o, float* u,
+                int B, int T, int Hk, int Hv, int D, float scale, const TreeLayer& layer, void* stream) {
+  const dim3 grid(static_cast<unsigned>(gdn::kNumXcd * ((B * Hv + gdn::kNumXcd - 1) / gdn::kNumXcd)));
+  hipStream_t st = static_cast<hipStream_t>(stream);
+#define GDN_RULE(DD, NT)                                                                                           \
+  rule_tree_kernel<DD, NT, kLayer><<<grid, dim3(2 * DD), 0, st>>>(r.q, r.q_b, r.q_t, r.k, r.k_b, r.k_t, r.v, r.v_b,  \
+                                                                  r.v_t, g, beta, s_pool, s_slot, n_slots, ids,      \
+                                                                  parents, p_b, pd, o, u, B, T, Hk, Hv, scale, layer)
+  if (D == 128)
+    T <= 16 ? GDN_RULE(128, 1) : T <= 32 ? GDN_RULE(128, 2) : T <= 48 ? GDN_RULE(128, 3) : GDN_RULE(128, 4);
+  else
+    T <= 16 ? GDN_RULE(64, 1) : T <= 32 ? GDN_RULE(64, 2) : T <= 48 ? GDN_RULE(64, 3) : GDN_RULE(64, 4);
+#undef GDN_RULE
+  return gdn_launch_status();
+}
+
 }  // namespace
 
 extern "C" int gdn_conv_tree(const uint16_t* x, int64_t x_b, int64_t x_t, uint16_t* pool, int64_t sp_slot,
@@ -927,31 +1080,36 @@ extern "C" int gdn_rule_tree(const uint16_t* q, int64_t q_b, int64_t q_t, const 
                              const float* last_g, const float* last_u, const int32_t* last_parents, int64_t lp_b,
                              const int64_t* accepted, int last_T, uint16_t* o, float* u, int B, int T, int Hk, int Hv,
                              int D, float scale, void* stream) {
-  if (B < 0 || T < 0 || Hk <= 0 || Hv <= 0 || Hv % Hk || n_slots < 0) return GDN_ERR_INVALID_ARG;
-  if (T > kMaxNodes || (accepted && last_T > kMaxNodes) || (D != 64 && D != 128)) return GDN_ERR_UNSUPPORTED;
-  if (B == 0 || T == 0) return GDN_OK;
-  if (!rows_ok(q, q_b, q_t, Hk * D, T) || !rows_ok(k, k_b, k_t, Hk * D, T) || !rows_ok(v, v_b, v_t, Hv * D, T) || !g ||
-      !beta || !s_pool || !ids || !parents || !o || !u || p_b < 0 || s_slot < static_cast<int64_t>(Hv) * D * D ||
-      s_slot % 4 || reinterpret_cast<uintptr_t>(s_pool) % 16 || reinterpret_cast<uintptr_t>(o) % 16 ||
-      reinterpret_cast<uintptr_t>(u) % 16)
-    return GDN_ERR_INVALID_ARG;
-  if (accepted && (!rows_ok(last_k, lk_b, lk_t, Hk * D, last_T) || !last_g || !last_u || !last_parents || lp_b < 0 ||
-                   reinterpret_cast<uintptr_t>(last_u) % 16))
-    return GDN_ERR_INVALID_ARG;
-  if (static_cast<int64_t>(B) * Hv >= (1LL << 24)) return GDN_ERR_UNSUPPORTED;
   const RulePending pd{last_k, lk_b, lk_t, last_g, last_u, last_parents, lp_b, accepted, last_T};
-  const dim3 grid(static_cast<unsigned>(gdn::kNumXcd * ((B * Hv + gdn::kNumXcd - 1) / gdn::kNumXcd)));
-  hipStream_t st = static_cast<hipStream_t>(stream);
-#define GDN_RULE(DD, NT)                                                                                            \
-  rule_tree_kernel<DD, NT><<<grid, dim3(2 * DD), 0, st>>>(q, q_b, q_t, k, k_b, k_t, v, v_b, v_t, g, beta, s_pool,    \
-                                                          s_slot, n_slots, ids, parents, p_b, pd, o, u, B, T, Hk, Hv, \
-                                                          scale)
-  if (D == 128)
-    T <= 16 ? GDN_RULE(128, 1) : T <= 32 ? GDN_RULE(128, 2) : T <= 48 ? GDN_RULE(128, 3) : GDN_RULE(128, 4);
-  else
-    T <= 16 ? GDN_RULE(64, 1) : T <= 32 ? GDN_RULE(64, 2) : T <= 48 ? GDN_RULE(64, 3) : GDN_RULE(64, 4);
-#undef GDN_RULE
-  return gdn_launch_status();
+  const RuleRows r{q, q_b, q_t, k, k_b, k_t, v, v_b, v_t};
+  const int rc = rule_check(r, s_pool, s_slot, n_slots, ids, parents, p_b, pd, u, B, T, Hk, Hv, D);
+  if (rc != GDN_OK || B == 0 || T == 0) return rc;
+  if (!g || !beta || !o || reinterpret_cast<uintptr_t>(o) % 16) return GDN_ERR_INVALID_ARG;
+  return rule_launch<false>(r, g, beta, s_pool, s_slot, n_slots, ids, parents, p_b, pd, o, u, B, T, Hk, Hv, D, scale,
+                            TreeLayer{}, stream);
+}
+
+extern "C" int gdn_rule_tree_layer(const uint16_t* q, int64_t q_b, int64_t q_t, const uint16_t* k, int64_t k_b,
+                                   int64_t k_t, const uint16_t* v, int64_t v_b, int64_t v_t, const uint16_t* b,
+                                   const uint16_t* a, const void* A_log, const void* dt_bias, int param_is_fp32,
+                                   float* s_pool, int64_t s_slot, int64_t n_slots, const int64_t* ids,
+                                   const int32_t* parents, int64_t p_b, const uint16_t* last_k, int64_t lk_b,
+                                   int64_t lk_t, const float* last_g, const float* last_u, const int32_t* last_parents,
+                                   int64_t lp_b, const int64_t* accepted, int last_T, const uint16_t* z, int64_t z_b,
+                                   int64_t z_t, const uint16_t* w, float eps, uint16_t* y, uint8_t* y8, float* y8_scale,
+                                   float* u, float* g, int B, int T, int Hk, int Hv, int D, float scale, void* stream) {
+  const RulePending pd{last_k, lk_b, lk_t, last_g, last_u, last_parents, lp_b, accepted, last_T};
+  const RuleRows r{q, q_b, q_t, k, k_b, k_t, v, v_b, v_t};
+  const int rc = rule_check(r, s_pool, s_slot, n_slots, ids, parents, p_b, pd, u, B, T, Hk, Hv, D);
+  if (rc != GDN_OK || B == 0 || T == 0) return rc;
+  if (!rows_ok(z, z_b, z_t, Hv * D, T) || !b || !a || !A_log || !dt_bias || !w || !g || (!y == !y8) ||
+      reinterpret_cast<uintptr_t>(w) % 16 || reinterpret_cast<uintptr_t>(y) % 16 ||
+      reinterpret_cast<uintptr_t>(y8) % 16 || (y8 && !y8_scale))
+    return GDN_ERR_INVALID_ARG;
+  if (y8 && D != gdn::kFp8Group) return GDN_ERR_UNSUPPORTED;  // a head per scale
+  const TreeLayer layer{b, a, A_log, dt_bias, param_is_fp32 ? 1 : 0, g, z, z_b, z_t, w, eps, y8, y8_scale};
+  return rule_launch<true>(r, nullptr, nullptr, s_pool, s_slot, n_slots, ids, parents, p_b, pd, y, u, B, T, Hk, Hv, D,
+                           scale, layer, stream);
 }
 
 extern "C" int gdn_commit_tree(float* s_pool, int64_t s_slot, uint16_t* conv_pool, int64_t sp_slot, int64_t sp_ch,

@@ -297,16 +297,18 @@ class GatedDeltaNetCore:
             last_rule = (pending.k, pending.g, pending.u, pending.parents, pending.accepted)
         with self._timed("conv_tree"):
             y = ops.conv_tree_step(mixed, conv_cache, ids, self.conv_w, parents, pending=last_conv)
+        q, k, v = (y[..., :kd].unflatten(-1, (Hk, D)), y[..., kd:2 * kd].unflatten(-1, (Hk, D)),
+                   y[..., 2 * kd:].unflatten(-1, (Hv, D)))
+        if not fp8 or D == ops.FP8_GROUP:
+            with self._timed("recurrent_tree"):
+                out, u, g = ops.recurrent_tree_fused(q, k, v, b, a, self.A_log, self.dt_bias, z, self.norm_w, s_cache,
+                                                     ids, parents, self.eps, pending=last_rule, fp8=fp8)
+            return out, TreeStep(mixed, k, g, u, parents)
+        # (heads of 64: two share a scale, which the fused norm does not see)
         g, beta = self._g_beta(b.contiguous(), a.contiguous(), None)
-        k = y[..., kd:2 * kd].unflatten(-1, (Hk, D))
         with self._timed("recurrent_tree"):
-            o, u = ops.recurrent_gdn_tree(y[..., :kd].unflatten(-1, (Hk, D)), k, y[..., 2 * kd:].unflatten(-1, (Hv, D)),
-                                          g, beta, s_cache, ids, parents, pending=last_rule)
-        step = TreeStep(mixed, k, g, u, parents)
-        if z.stride(0) % 8 or z.stride(1) % 8 or z.data_ptr() % 16:
-            z = z.contiguous()      # (the norm reads 16-byte pieces)
-        z = z.reshape(B, T, Hv, D)
-        return (self._norm_fp8(o, z) if fp8 else self._norm(o, z)), step
+            o, u = ops.recurrent_gdn_tree(q, k, v, g, beta, s_cache, ids, parents, pending=last_rule)
+        return self._norm_fp8(o, z.reshape(B, T, Hv, D)), TreeStep(mixed, k, g, u, parents)
 
     def commit_tree(self, step: TreeStep, ids, conv_cache, s_cache) -> None:
         """The accepted paths of a verify step into both pools, for another user of

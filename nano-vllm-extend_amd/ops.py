@@ -961,6 +961,38 @@ def conv_tree_step(x: torch.Tensor, conv_pool: torch.Tensor, ids: torch.Tensor, 
     return y
 
 
+def _rule_args(q, k, v, s_pool, ids, parents, pending):
+    """The checked arguments of the rule over a tree: (B, T, Hk, Hv, D), those of the rows
+    and those from the pool on, and the tensors that they point into."""
+    if k.dim() != 4 or v.dim() != 4:
+        raise ValueError(f"q, k, v must be [B, T, heads, D], got {list(k.shape)} and {list(v.shape)}")
+    k_shape = B, T, Hk, D = k.shape
+    Hv = v.shape[2]
+    if Hk == 0 or Hv % Hk:
+        raise ValueError(f"{Hv} value heads are no multiple of {Hk} key heads")
+    q, q_b, q_t = _tree_rows(q, "q", k_shape)
+    k, k_b, k_t = _tree_rows(k, "k", k_shape)
+    v, v_b, v_t = _tree_rows(v, "v", (B, T, Hv, D))
+    _s_pool_ok(s_pool, Hv, D)
+    ids = _tree_ids(ids, B)
+    par, p_b = _tree_parents(parents, B, T)
+    last, keep = (None, 0, 0, None, None, None, 0, None, 0), None
+    if pending is not None:
+        last_k, last_g, last_u, last_parents, accepted = pending
+        last_T = last_k.shape[1]
+        last_k, lk_b, lk_t = _tree_rows(last_k, "pending k", (B, last_T, Hk, D))
+        last_g = _tree_f32(last_g, "pending g", (B, last_T, Hv))
+        last_u = _tree_f32(last_u, "pending u", (B, last_T, Hv, D))
+        last_parents, lp_b = _tree_parents(last_parents, B, last_T)
+        accepted = _tree_ids(accepted, B, "accepted")
+        last = (last_k.data_ptr(), lk_b, lk_t, last_g.data_ptr(), last_u.data_ptr(), last_parents.data_ptr(), lp_b,
+                accepted.data_ptr(), last_T)
+        keep = last_k, last_g, last_u, last_parents, accepted
+    return ((B, T, Hk, Hv, D), (q.data_ptr(), q_b, q_t, k.data_ptr(), k_b, k_t, v.data_ptr(), v_b, v_t),
+            (s_pool.data_ptr(), s_pool.stride(0), s_pool.shape[0], ids.data_ptr(), par.data_ptr(), p_b, *last),
+            (q, k, v, ids, par, keep))
+
+
 def recurrent_gdn_tree(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch.Tensor, beta: torch.Tensor,
                        s_pool: torch.Tensor, ids: torch.Tensor, parents: torch.Tensor,
                        pending: tuple | None = None):
@@ -980,42 +1012,60 @@ def recurrent_gdn_tree(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: tor
     it, also what is not finite.
     (No reference counterpart: spec decode is disabled for qwen3_5,
     nanovllm/config.py:84; one token: qwen3_5.py:575-594.)"""
-    last_k, last_g, last_u, last_parents, accepted = pending if pending is not None else (None,) * 5
-    idx = _device_of(k, q, v, g, beta, s_pool, ids, parents, last_k, last_g, last_u, last_parents, accepted)
-    if k.dim() != 4 or v.dim() != 4:
-        raise ValueError(f"q, k, v must be [B, T, heads, D], got {list(k.shape)} and {list(v.shape)}")
-    k_shape = B, T, Hk, D = k.shape
-    Hv = v.shape[2]
-    if Hk == 0 or Hv % Hk:
-        raise ValueError(f"{Hv} value heads are no multiple of {Hk} key heads")
-    v_shape, g_shape = (B, T, Hv, D), (B, T, Hv)
-    q, q_b, q_t = _tree_rows(q, "q", k_shape)
-    k, k_b, k_t = _tree_rows(k, "k", k_shape)
-    v, v_b, v_t = _tree_rows(v, "v", v_shape)
+    idx = _device_of(k, q, v, g, beta, s_pool, ids, parents, *(pending or ()))
+    dims, rows, state, keep = _rule_args(q, k, v, s_pool, ids, parents, pending)
+    B, T, Hk, Hv, D = dims
+    g_shape, v_shape = (B, T, Hv), (B, T, Hv, D)
     g = _tree_f32(g, "g", g_shape)
     _bf16(beta, "beta")
     if beta.shape != g_shape:
         raise ValueError(f"beta must be {list(g_shape)}, got {list(beta.shape)}")
     if not beta.is_contiguous():
         beta = beta.contiguous()
-    _s_pool_ok(s_pool, Hv, D)
-    ids = _tree_ids(ids, B)
-    par, p_b = _tree_parents(parents, B, T)
-    last = (None, 0, 0, None, None, None, 0, None, 0)
-    if pending is not None:
-        last_T = last_k.shape[1]
-        last_k, lk_b, lk_t = _tree_rows(last_k, "pending k", (B, last_T, Hk, D))
-        last_g = _tree_f32(last_g, "pending g", (B, last_T, Hv))
-        last_u = _tree_f32(last_u, "pending u", (B, last_T, Hv, D))
-        last_parents, lp_b = _tree_parents(last_parents, B, last_T)
-        accepted = _tree_ids(accepted, B, "accepted")
-        last = (last_k.data_ptr(), lk_b, lk_t, last_g.data_ptr(), last_u.data_ptr(), last_parents.data_ptr(), lp_b,
-                accepted.data_ptr(), last_T)
     o, u = v.new_empty(v_shape), g.new_empty(v_shape)
-    _call_on(idx, "gdn_rule_tree", q.data_ptr(), q_b, q_t, k.data_ptr(), k_b, k_t, v.data_ptr(), v_b, v_t,
-             g.data_ptr(), beta.data_ptr(), s_pool.data_ptr(), s_pool.stride(0), s_pool.shape[0], ids.data_ptr(),
-             par.data_ptr(), p_b, *last, o.data_ptr(), u.data_ptr(), B, T, Hk, Hv, D, D ** -0.5)
+    _call_on(idx, "gdn_rule_tree", *rows, g.data_ptr(), beta.data_ptr(), *state, o.data_ptr(), u.data_ptr(), *dims,
+             D ** -0.5)
     return o, u
+
+
+def recurrent_tree_fused(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, b: torch.Tensor, a: torch.Tensor,
+                         a_log: torch.Tensor, dt_bias: torch.Tensor, z: torch.Tensor, norm_weight: torch.Tensor,
+                         s_pool: torch.Tensor, ids: torch.Tensor, parents: torch.Tensor, eps: float = 1e-6,
+                         pending: tuple | None = None, fp8: bool = False):
+    """recurrent_gdn_tree with the layer's gates before it and its gated norm behind
+    it in one launch: fused_g_beta(b, a) -> recurrent_gdn_tree -> rms_norm_gated (or
+    with fp8, D = 128, rms_norm_gated_fp8), the same bits for every used node, and
+    zeros for the others (rows of a slot that is none: g too).  b, a [B, T, Hv] bf16,
+    a_log and dt_bias [Hv], z [B, T, Hv * D] bf16, norm_weight [D].  Returns (y [B, T,
+    Hv, D] bf16, or its (e4m3, scales); u; g), g for the next step's pending."""
+    idx = _device_of(k, q, v, b, a, a_log, dt_bias, z, norm_weight, s_pool, ids, parents, *(pending or ()))
+    dims, rows, state, keep = _rule_args(q, k, v, s_pool, ids, parents, pending)
+    B, T, Hk, Hv, D = dims
+    if fp8 and D != FP8_GROUP:
+        raise ValueError(f"fp8 outputs have a scale for each head of {FP8_GROUP}, got head dim {D}")
+    for t, name in ((b, "b"), (a, "a")):
+        _bf16(t, name)
+        if t.shape != (B, T, Hv):
+            raise ValueError(f"{name} must be {[B, T, Hv]}, got {list(t.shape)}")
+    b, a = b.contiguous(), a.contiguous()
+    if a_log.dtype != dt_bias.dtype or a_log.dtype not in (torch.bfloat16, torch.float32):
+        a_log, dt_bias = a_log.float(), dt_bias.float()
+    a_log, dt_bias = a_log.contiguous(), dt_bias.contiguous()
+    if a_log.numel() != Hv or dt_bias.numel() != Hv or norm_weight.numel() != D:
+        raise ValueError(f"a_log and dt_bias must have {Hv} values, norm_weight {D}")
+    z, z_b, z_t = _tree_rows(z, "z", (B, T, Hv * D))
+    w = norm_weight
+    if w.dtype != torch.bfloat16 or not w.is_contiguous() or w.data_ptr() % 16:
+        w = w.to(torch.bfloat16).clone(memory_format=torch.contiguous_format)
+    y = v.new_empty((B, T, Hv, D), dtype=FP8 if fp8 else torch.bfloat16)
+    scale = _fp8_scales(B * T, Hv, v.device) if fp8 else None
+    u = v.new_empty((B, T, Hv, D), dtype=torch.float32)
+    g = v.new_empty((B, T, Hv), dtype=torch.float32)
+    out = (None, y.data_ptr(), scale.data_ptr()) if fp8 else (y.data_ptr(), None, None)
+    _call_on(idx, "gdn_rule_tree_layer", *rows, b.data_ptr(), a.data_ptr(), a_log.data_ptr(), dt_bias.data_ptr(),
+             int(a_log.dtype == torch.float32), *state, z.data_ptr(), z_b, z_t, w.data_ptr(), float(eps), *out,
+             u.data_ptr(), g.data_ptr(), *dims, D ** -0.5)
+    return (y, scale) if fp8 else y, u, g
 
 
 def commit_tree(s_pool: torch.Tensor, conv_pool: torch.Tensor, ids: torch.Tensor, parents: torch.Tensor,

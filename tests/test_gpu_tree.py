@@ -497,3 +497,92 @@ def test_rows_of_a_slot_that_is_read_only_twice(pkg, dev):
     for b in range(B):
         ro, _, _, eo, _ = ref.rule(q[b], k[b], v[b], i["g"][b], i["beta"][b], pd[ids[b]].cpu(), parents[b])
         _close(o[b], ro, eo + ref.HALF_BF16 * (ro.abs() + eo), f"row {b}")
+
+
+def _layer_inputs(gen, B, T, Hk, Hv, D, f32=False):
+    """What stands around the rule in the layer: b, a, A_log, dt_bias, z's rows among 16 others, w."""
+    n = lambda *s: torch.randn(*s, generator=gen).to(BF16)  # noqa: E731
+    params = [torch.randn(Hv, generator=gen) for _ in range(2)]
+    return (n(B, T, Hv), n(B, T, Hv), *(p if f32 else p.to(BF16) for p in params), n(B, T, Hv * D + 16),
+            (1 + 0.1 * torch.randn(D, generator=gen)).to(BF16))
+
+
+@pytest.mark.parametrize("B,T,Hk,Hv,D,back", RULE)
+@pytest.mark.parametrize("pending", [False, True])
+def test_rule_with_gates_and_norm_is_the_three_calls(pkg, dev, B, T, Hk, Hv, D, back, pending):
+    """Bit for bit on used nodes, zeros on the others and on rows of a slot that is none."""
+    gen = torch.Generator().manual_seed(7 * B + T + Hv + pending)
+    i, last = _inputs(gen, B, T, Hk, Hv, D), _inputs(gen, B, T, Hk, Hv, D)
+    b, a, A_log, dt, z, w = (t.to(dev) for t in _layer_inputs(gen, B, T, Hk, Hv, D, f32=T % 2 == 0))
+    z = z[..., 8:-8]
+    parents, _ = ref.tree(gen, B, T, back, ragged=B > 1)
+    last_parents, accepted = ref.tree(gen, B, T, back, ragged=True)
+    pools = [(torch.randn(B + 1, Hv, D, D, generator=torch.Generator().manual_seed(3)) * 0.3).to(dev) for _ in range(3)]
+    ids = torch.randperm(B + 1, generator=gen)[:B]
+    if B > 2:
+        ids[1] = -1
+    q, k, v = _qkv(i["y"].to(dev), Hk, Hv, D)
+    pend = (tuple(t.to(dev) for t in (_qkv(last["y"], Hk, Hv, D)[1], last["g"], last["u"], last_parents, accepted))
+            if pending else None)
+    ids, par = ids.to(dev), parents.to(dev)
+    g, beta = pkg.fused_g_beta(b, a, A_log, dt, None)
+    o, u = pkg.recurrent_gdn_tree(q, k, v, g, beta, pools[0], ids, par, pending=pend)
+    want = pkg.rms_norm_gated(o, z.reshape(B, T, Hv, D), w, 1e-6)
+    on = torch.tensor([ref.used(p.tolist()) for p in parents], device=dev) & (ids >= 0)[:, None]
+
+    def same(got, ref_, tag):
+        assert torch.equal(got[on].contiguous().view(torch.uint8), ref_[on].contiguous().view(torch.uint8)), tag
+        assert bool((got[~on].float() == 0).all()), tag
+
+    y, u1, g1 = pkg.recurrent_tree_fused(q, k, v, b, a, A_log, dt, z, w, pools[1], ids, par, pending=pend)
+    same(y, want, "y")
+    same(u1, u, "u")
+    assert torch.equal(g1[ids >= 0], g[ids >= 0]) and bool((g1[ids < 0] == 0).all())
+    assert torch.equal(pools[0], pools[1])
+    if D == 128:
+        want, ws = pkg.rms_norm_gated_fp8(o, z.reshape(B, T, Hv, D), w, 1e-6)
+        (y, ys), u2, g2 = pkg.recurrent_tree_fused(q, k, v, b, a, A_log, dt, z, w, pools[2], ids, par, pending=pend,
+                                                   fp8=True)
+        same(y, want, "y8")
+        assert torch.equal(ys.view(B, T, Hv)[on], ws.view(B, T, Hv)[on]) and ys.shape == ws.shape
+        assert torch.equal(u1, u2) and torch.equal(g1, g2) and torch.equal(pools[0], pools[2])
+    torch.cuda.synchronize()
+
+
+def test_rule_with_gates_and_norm_where_not_finite(pkg, dev):
+    """A NaN in one head of one sequence: its rows are not finite in the norm, the other rows
+    are those of the separate calls, bit for bit elsewhere and within rounding in that head
+    (the rule takes another order of sums there)."""
+    gen = torch.Generator().manual_seed(59)
+    B, T, Hk, Hv, D = 2, 37, 1, 2, 128
+    i = _inputs(gen, B, T, Hk, Hv, D)
+    b, a, A_log, dt, z, w = _layer_inputs(gen, B, T, Hk, Hv, D)
+    z = z[..., 8:-8]
+    parents, _ = ref.tree(gen, B, T, 5)
+    parents[:, 5::7] = 0
+    q, k, v = _qkv(i["y"], Hk, Hv, D)
+    v[0, 3, 1, 70] = float("nan")
+    pool = torch.randn(B, Hv, D, D, generator=gen) * 0.3
+    dv = lambda *ts: tuple(t.to(dev) for t in ts)  # noqa: E731
+    ids = torch.arange(B)
+    y, u, g = pkg.recurrent_tree_fused(*_qkv(i["y"].to(dev), Hk, Hv, D), *dv(b, a, A_log, dt, z, w, pool, ids, parents))
+    g0, beta = pkg.fused_g_beta(*dv(b, a, A_log, dt), None)
+    o, u0 = pkg.recurrent_gdn_tree(*_qkv(i["y"].to(dev), Hk, Hv, D), g0, beta, *dv(pool, ids, parents))
+    want = pkg.rms_norm_gated(o, z.to(dev).reshape(B, T, Hv, D), w.to(dev), 1e-6)
+    torch.cuda.synchronize()
+    y, want, o, beta, g = (t.cpu() for t in (y, want, o, beta, g))
+    assert torch.equal(y[1], want[1]) and torch.equal(y[0, :, 0], want[0, :, 0])
+    hit = ~o[0, :, 1].float().isfinite().all(-1)
+    assert 1 < int(hit.sum()) < T - 5
+    assert torch.equal(y[0, :, 1].isnan().all(-1), hit) and torch.equal(y[0, :, 1].isfinite().all(-1), ~hit)
+    # both o are within eo and half a step of the 64-bit one, so 2 (eo + 2^-8 |o|) of each other; that
+    # through x r w silu(z), r from the row, and three roundings of the norm on either side
+    ro, _, _, eo, _ = ref.rule(q[0], k[0], v[0], g[0], beta[0], pool[0], parents[0])
+    ro, eo = ro[~hit, 1], eo[~hit, 1]
+    d = 2 * (eo + ref.HALF_BF16 * (ro.abs() + eo))
+    r = (ro.square().mean(-1, keepdim=True) + 1e-6).rsqrt()
+    zz = z.double().view(B, T, Hv, D)[0, ~hit, 1]
+    gain = (w.double() * zz * torch.sigmoid(zz)).abs()
+    rel = d.norm(dim=-1, keepdim=True) / ro.norm(dim=-1, keepdim=True)
+    bound = r * gain * (d + ro.abs() * rel) * 1.1 + 6 * ref.HALF_BF16 * (want[0, ~hit, 1].double().abs() + r * gain * d)
+    _close(y[0, ~hit, 1], want[0, ~hit, 1].double(), bound + 1e-30, "head 1")

@@ -65,6 +65,26 @@ def test_recurrent_gdn_tree_refuses(ops):
                       (q, g, u, par[:, :2], ids), (q, g, u, par, ids[:1])])
 
 
+def test_recurrent_tree_fused_refuses(ops):
+    B, T, Hk, Hv, D = 2, 4, 1, 2, 128
+    q, v = torch.zeros(B, T, Hk, D, dtype=BF16), torch.zeros(B, T, Hv, D, dtype=BF16)
+    b, z, w = torch.zeros(B, T, Hv, dtype=BF16), torch.zeros(B, T, Hv * D, dtype=BF16), torch.ones(D)
+    p, pool, ids = torch.zeros(Hv), torch.zeros(5, Hv, D, D), torch.arange(B)
+    par, g, u = torch.zeros(B, T, dtype=torch.int32), torch.zeros(B, T, Hv), torch.zeros(B, T, Hv, D)
+    good = dict(q=q, k=q, v=v, b=b, a=b, a_log=p, dt_bias=p.to(BF16), z=z, norm_weight=w, s_pool=pool, ids=ids,
+                parents=par, pending=(q, g, u, par, ids), fp8=True)
+    _refused(ops.recurrent_tree_fused, good,
+             q=[q.float()], v=[v[:, :3]], b=[b.float(), b[:1]], a=[b.float(), b[..., :1]], a_log=[p[:1]],
+             dt_bias=[p[:1]], z=[z.float(), z[..., :128], v], norm_weight=[w[:64]], s_pool=[pool.double()],
+             ids=[ids.float()], parents=[par[:1]], pending=[(q, g, u, par, ids[:1])])
+    half = dict(good, q=q[..., :64], k=q[..., :64], v=v[..., :64], z=z[..., :128], norm_weight=w[:64],
+                s_pool=torch.zeros(5, Hv, 64, 64), pending=None)
+    with pytest.raises(ValueError):      # heads of 64 share a scale
+        ops.recurrent_tree_fused(**half)
+    with pytest.raises(Launched):
+        ops.recurrent_tree_fused(**dict(half, fp8=False))
+
+
 def test_commit_tree_refuses(ops):
     B, T, Hk, Hv, D, C = 2, 4, 2, 4, 64, 512
     k, u = torch.zeros(B, T, Hk, D, dtype=BF16), torch.zeros(B, T, Hv, D)
@@ -192,6 +212,15 @@ def test_c_entry_points_reject_before_launch(pkg):
     for bad in (dict(q=None), dict(qt=120), dict(qt=1 << 24), dict(vt=248), dict(g=None), dict(s=odd), dict(st=slot - 4), dict(o=None),
                 dict(u=odd), dict(Hk=3), dict(Hk=0), dict(lu=None), dict(lT=0), dict(T=-1)):
         assert r(**bad) == inv, bad
+    f = lambda q=P, b=P, a=P, al=P, z=P, zt=256, w=P, y=P, y8=None, ys=None, u=P, g=P, B=2, T=8, D=64: (  # noqa: E731
+        lib.gdn_rule_tree_layer(q, 8 * 128, 128, P, 8 * 128, 128, P, 8 * 256, 256, b, a, al, P, 0, P, slot, 4, P, P, 8,
+                                None, 0, 0, None, None, None, 0, None, 0, z, 8 * 256, zt, w, 1e-6, y, y8, ys, u, g, B,
+                                T, 2, 4, D, 1.0, None))
+    assert f(B=0) == ok and f(T=65) == uns and f(y=None, y8=P, ys=P) == uns
+    for bad in (dict(q=None), dict(b=None), dict(a=None), dict(al=None), dict(z=None), dict(z=odd), dict(zt=248),
+                dict(w=odd), dict(y=None), dict(y8=P, ys=P), dict(y=None, y8=P), dict(y=odd), dict(u=odd),
+                dict(g=None)):
+        assert f(**bad) == inv, bad
     c = lambda s=P, st=slot, cp=P, cs=3 * C, x=P, k=P, u=P, acc=P, B=2, T=8, Hk=2, Hv=4, D=64, Cc=C: (  # noqa: E731
         lib.gdn_commit_tree(s, st, cp, cs, 3, 4, P, P, 8, acc, x, 8 * C, C, k, 8 * 128, 128, P, u, B, T, Hk, Hv, D,
                             Cc, None))
