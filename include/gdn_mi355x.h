@@ -558,6 +558,25 @@ int gdn_commit_tree(float* s_pool, int64_t s_slot, uint16_t* conv_pool, int64_t 
                     const uint16_t* x, int64_t x_b, int64_t x_t, const uint16_t* k, int64_t k_b, int64_t k_t,
                     const float* g, const float* u, int B, int T, int Hk, int Hv, int D, int C, void* stream);
 
+/*
+ * The calls above that are short enough for the cost of a foreign call to show (23 to 45
+ * arguments through ctypes 1.9 to 3.5 us, one array 0.5), with their arguments as 8-byte
+ * words: words[0] = GDN_CALL_x + (n << 32), then the n arguments in order, pointers and
+ * integers as int64 (an integer that its argument does not hold is refused), floats as
+ * double.  For GDN_CALL_GEMM_FP8 the C, ldc and col_end arguments are left out, and
+ * n_parts triples (C[s], ldc[s], col_end[s]) follow the others.
+ */
+enum {
+  GDN_CALL_QUANTIZE_FP8 = 1,
+  GDN_CALL_GEMM_FP8 = 2,
+  GDN_CALL_RMSNORM_GATED_FP8 = 3,
+  GDN_CALL_CONV_TREE = 4,
+  GDN_CALL_RULE_TREE = 5,
+  GDN_CALL_RULE_TREE_LAYER = 6,
+  GDN_CALL_COMMIT_TREE = 7
+};
+int gdn_call_words(const void* words);
+
 #ifdef __cplusplus
 }
 #endif

@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 from pathlib import Path
 
 import torch  # noqa: F401  (loads the HIP runtime the library binds to)
@@ -81,7 +82,24 @@ SIGNATURES: dict[str, list] = {
                             _p, _p, _i32, _i32, _i32, _i32, _i32, _f32, _p],
     "gdn_commit_tree": [_p, _i64, _p, _i64, _i64, _i64, _p, _p, _i64, _p, _p, _i64, _i64, _p, _i64, _i64, _p, _p,
                         _i32, _i32, _i32, _i32, _i32, _i32, _p],
+    "gdn_call_words": [ctypes.c_char_p],
 }
+
+# gdn_call_words: the packing of an entry point's arguments (the stream among them) and
+# the word before them.  Its arguments are 8-byte integers, a NULL pointer 0.
+_WORD_CALLS = ("gdn_quantize_fp8", "gdn_gemm_fp8", "gdn_rmsnorm_gated_fp8", "gdn_conv_tree", "gdn_rule_tree",
+               "gdn_rule_tree_layer", "gdn_commit_tree")
+
+
+def _words_of(name: str, types: list):
+    head = _WORD_CALLS.index(name) + 1 + (len(types) << 32)
+    return struct.Struct("=q" + "".join("d" if t is _f32 else "q" for t in types)).pack, head
+
+
+# (the GEMM's part tables go as triples behind the rest: one packing per number of parts)
+_GEMM = SIGNATURES["gdn_gemm_fp8"]
+WORDS = {name: _words_of(name, SIGNATURES[name]) for name in _WORD_CALLS if name != "gdn_gemm_fp8"}
+GEMM_FP8_WORDS = [None] + [_words_of("gdn_gemm_fp8", _GEMM[:17] + _GEMM[20:] + 3 * n * [_i64]) for n in range(1, 5)]
 
 # entry points whose return type is not int (status)
 RESTYPES = {"gdn_chunk_prefill_workspace_size": ctypes.c_int64,
@@ -135,6 +153,13 @@ def call(name: str, *args) -> None:
     """Invoke an entry point and raise on a non-zero status."""
     lib = load()
     check(name, getattr(lib, name)(*args))
+
+
+def call_words(name: str, words: bytes) -> None:
+    """Invoke the entry point `name` through gdn_call_words and raise on a non-zero status."""
+    status = load().gdn_call_words(words)
+    if status:
+        check(name, status)
 
 
 def ptr(t) -> int | None:

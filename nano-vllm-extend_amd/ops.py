@@ -10,6 +10,7 @@ CPU or eager fallback: a CPU tensor or a missing library raises.
 from __future__ import annotations
 
 import ctypes
+import functools
 import os
 
 import torch
@@ -61,15 +62,19 @@ def _device_of(first: torch.Tensor, *others: torch.Tensor | None) -> int:
 
 
 def _call_on(idx: int, name: str, *args) -> None:
-    """_lib.call on device idx's current stream, which is appended to args: a launch
-    goes to its stream's device, so that one is made current where it is not."""
+    """An entry point of _lib.WORDS on device idx's current stream, which is appended to
+    args (NULL is 0): a launch goes to its stream's device, so that one is made current
+    where it is not."""
+    pack, head = _lib.WORDS[name]
+    _launch_on(idx, name, pack(head, *args, _lib.stream_of(idx)))
+
+
+def _launch_on(idx: int, name: str, words: bytes) -> None:
     if idx == _current_device():
-        status = getattr(_lib.load(), name)(*args, _lib.stream_of(idx))
+        _lib.call_words(name, words)
     else:
         with torch.cuda.device(idx):
-            status = getattr(_lib.load(), name)(*args, _lib.stream_of(idx))
-    if status:
-        _lib.check(name, status)
+            _lib.call_words(name, words)
 
 
 # (0.2 us cheaper than the public call, which checks that CUDA is initialised: a tensor on
@@ -948,7 +953,7 @@ def conv_tree_step(x: torch.Tensor, conv_pool: torch.Tensor, ids: torch.Tensor, 
     w = weight if weight.is_contiguous() else weight.contiguous()
     ids = _tree_ids(ids, B)
     par, p_b = _tree_parents(parents, B, T)
-    last = (None, 0, 0, None, 0, None, 0)
+    last = (0, 0, 0, 0, 0, 0, 0)
     if pending is not None:
         last_T = last_x.shape[1]
         last_x, lx_b, lx_t = _tree_rows(last_x, "pending x", (B, last_T, C))
@@ -976,7 +981,7 @@ def _rule_args(q, k, v, s_pool, ids, parents, pending):
     _s_pool_ok(s_pool, Hv, D)
     ids = _tree_ids(ids, B)
     par, p_b = _tree_parents(parents, B, T)
-    last, keep = (None, 0, 0, None, None, None, 0, None, 0), None
+    last, keep = (0,) * 9, None
     if pending is not None:
         last_k, last_g, last_u, last_parents, accepted = pending
         last_T = last_k.shape[1]
@@ -1061,7 +1066,7 @@ def recurrent_tree_fused(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, b: t
     scale = _fp8_scales(B * T, Hv, v.device) if fp8 else None
     u = v.new_empty((B, T, Hv, D), dtype=torch.float32)
     g = v.new_empty((B, T, Hv), dtype=torch.float32)
-    out = (None, y.data_ptr(), scale.data_ptr()) if fp8 else (y.data_ptr(), None, None)
+    out = (0, y.data_ptr(), scale.data_ptr()) if fp8 else (y.data_ptr(), 0, 0)
     _call_on(idx, "gdn_rule_tree_layer", *rows, b.data_ptr(), a.data_ptr(), a_log.data_ptr(), dt_bias.data_ptr(),
              int(a_log.dtype == torch.float32), *state, z.data_ptr(), z_b, z_t, w.data_ptr(), float(eps), *out,
              u.data_ptr(), g.data_ptr(), *dims, D ** -0.5)
@@ -1223,7 +1228,7 @@ def _rows_of(x: torch.Tensor, align: int):
 
 def _fp8_scales(M: int, G: int, dev) -> torch.Tensor:
     """[M, G] fp32 with the rows of one group side by side (as the GEMM reads them)."""
-    return torch.empty(G, M, dtype=torch.float32, device=dev).t()
+    return torch.empty_strided((M, G), (1, M), dtype=torch.float32, device=dev)
 
 
 def quantize_fp8(x: torch.Tensor):
@@ -1288,11 +1293,16 @@ def _check_fp8(x, weight, weight_scale, x_scale):
     return M, N, K
 
 
+@functools.lru_cache(maxsize=256)
+def _fp8_workspace(M: int, N: int, K: int) -> int:
+    return _lib.load().gdn_gemm_fp8_workspace_size(M, N, K, 1)
+
+
 def _linear_fp8(x, weight, weight_scale, x_scale, M, N, K, outs, widths, wide=None):
     """The product into outs, [M, widths[s]] each; the columns past N from the bf16 weight
     `wide`."""
     idx = _device_of(x, weight, weight_scale, x_scale, wide, *outs)
-    wide_args = (None, 0, 0)
+    wide_args = (0, 0, 0)
     if wide is not None:
         if wide.stride(1) != 1 or wide.stride(0) % 8 or wide.stride(0) < K or wide.data_ptr() % 16:
             wide = wide.clone(memory_format=torch.contiguous_format)
@@ -1306,9 +1316,9 @@ def _linear_fp8(x, weight, weight_scale, x_scale, M, N, K, outs, widths, wide=No
     ws = weight_scale if (ws_st[1] == 1 or G == 1) and (ws_st[0] >= G or N <= FP8_GROUP) else weight_scale.contiguous()
     bf16 = x_scale is None
     x2, _, x_row = _rows_of(x, 8 if bf16 else 16)
-    work, ws_bytes, xs = None, 0, (None, 0, 0)
+    work, ws_bytes, xs = None, 0, (0, 0, 0)
     if bf16:
-        ws_bytes = _lib.load().gdn_gemm_fp8_workspace_size(M, N, K, 1)
+        ws_bytes = _fp8_workspace(M, N, K)
         if ws_bytes > 0:
             work = torch.empty(ws_bytes, dtype=torch.uint8, device=x.device)
     else:
@@ -1316,15 +1326,17 @@ def _linear_fp8(x, weight, weight_scale, x_scale, M, N, K, outs, widths, wide=No
     n = len(widths)
     if n == 1:
         y = outs[0]
-        ld = y.stride(0)
-        tables = (ctypes.byref(ctypes.c_void_p(y.data_ptr())), ctypes.byref(ctypes.c_int64(ld if ld >= N else N)),
-                  ctypes.byref(ctypes.c_int(N)))
+        parts = (y.data_ptr(), max(y.stride(0), N), N)
     else:
-        ends = [sum(widths[:i + 1]) for i in range(n)]
-        tables = ((ctypes.c_void_p * n)(*[p.data_ptr() for p in outs]), (ctypes.c_int64 * n)(*widths),
-                  (ctypes.c_int * n)(*ends))
-    _call_on(idx, "gdn_gemm_fp8", x2.data_ptr(), int(bf16), x_row, *xs, w.data_ptr(), w_st[0], ws.data_ptr(),
-             ws.stride(0) if N > FP8_GROUP else G, *wide_args, M, N, K, n, *tables, _lib.ptr(work), ws_bytes)
+        parts, end = [], 0
+        for y, width in zip(outs, widths):
+            end += width
+            parts += (y.data_ptr(), width, end)
+    pack, head = _lib.GEMM_FP8_WORDS[n]
+    _launch_on(idx, "gdn_gemm_fp8", pack(head, x2.data_ptr(), bf16, x_row, *xs, w.data_ptr(), w_st[0], ws.data_ptr(),
+                                         ws.stride(0) if N > FP8_GROUP else G, *wide_args, M, N, K, n,
+                                         0 if work is None else work.data_ptr(), ws_bytes, _lib.stream_of(idx),
+                                         *parts))
 
 
 def linear_fp8(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor,

@@ -20,6 +20,8 @@ def ops(pkg, monkeypatch):
 
     monkeypatch.setattr(pkg.ops, "_device_of", lambda *ts: 0)
     monkeypatch.setattr(pkg.ops, "_call_on", fake_call)
+    monkeypatch.setattr(pkg.ops, "_launch_on", fake_call)
+    monkeypatch.setattr(pkg._lib, "stream_of", lambda index: 0)
     return pkg.ops
 
 
@@ -228,3 +230,32 @@ def test_c_entry_points_reject_before_launch(pkg):
     for bad in (dict(s=None), dict(st=slot - 4), dict(cp=None), dict(cs=3 * C - 3), dict(x=None), dict(k=odd),
                 dict(u=None), dict(acc=None), dict(Hk=3)):
         assert c(**bad) == inv, bad
+
+
+def test_calls_by_words(pkg):
+    """An entry point's arguments as words: the same answers as the call itself; wrong heads,
+    counts and integers that do not fit are refused."""
+    lib, _lib = pkg._lib.load(), pkg._lib
+    inv, uns, ok = _lib.GDN_ERR_INVALID_ARG, _lib.GDN_ERR_UNSUPPORTED, _lib.GDN_OK
+    assert lib.gdn_call_words(None) == inv
+    for name, (pack, head) in _lib.WORDS.items():
+        n = head >> 32
+        types = _lib.SIGNATURES[name]
+        assert n == len(types)
+        zeros = [0.0 if t is ctypes.c_float else 0 for t in types]
+        assert lib.gdn_call_words(pack(head, *zeros)) == getattr(lib, name)(
+            *(None if t is ctypes.c_void_p else z for t, z in zip(types, zeros))), name
+        for wrong in (head + (1 << 32), head - (1 << 32), head & 0xffffffff, head + 64, n << 32):
+            assert lib.gdn_call_words(pack(wrong, *zeros)) == inv
+    pack, head = _lib.WORDS["gdn_conv_tree"]
+    conv = lambda B=0, T=8, C=64: lib.gdn_call_words(pack(head, *[0] * 19, B, T, C, 0))  # noqa: E731
+    assert conv() == ok and conv(T=65) == uns and conv(C=0) == inv and conv(B=1) == inv
+    assert conv(B=1 << 32) == inv and conv(T=(1 << 32) + 8) == inv       # 0 and 8 if they were cut
+    for n in range(1, 5):
+        pack, head = _lib.GEMM_FP8_WORDS[n]
+        args = lambda M, N, parts: [0] * 13 + [M, N, 128, parts, 0, 0, 0] + [0, 64, 64] * n  # noqa: E731
+        assert lib.gdn_call_words(pack(head, *args(0, 64, n))) == ok
+        assert lib.gdn_call_words(pack(head, *args(1 << 32, 64, n))) == inv
+        assert lib.gdn_call_words(pack(head, *args(0, 64, n % 4 + 1))) == inv
+        assert lib.gdn_call_words(pack(head, *args(0, 64, 0))) == inv
+        assert lib.gdn_call_words(pack(head, *args(2, 64, n))) == inv     # no operands
