@@ -23,27 +23,29 @@ namespace {
 
 constexpr int kMaxNodes = 64;
 
-// A tree's links, by the 64 lanes of one wave, lane t with node t's parent: link[t] the
-// parent (-1: the state), or kUnused.  (Each walk goes to smaller nodes, so it ends.)
+// The links of two trees, by the 64 lanes of one wave, lane t with node t's parents: the
+// parent (-1: the state), or kUnused (lanes past T too).  A node counts if the walk from it
+// ends at -1; every lane jumps over its ancestor's jumps, so that the rounds are as many as
+// the depth has bits.  (Jumps go to smaller nodes: they end.)
 constexpr int kUnused = -2;
-__device__ __forceinline__ void tree_links(int parent, int T, int lane, int* raw, int* link) {
-  if (lane < T) raw[lane] = parent;
-  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront", "local");
-  __builtin_amdgcn_wave_barrier();
-  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront", "local");
-  if (lane < T) {
-    int n = lane;
-    while (n >= 0) {
-      const int p = raw[n];
-      n = p >= -1 && p < n ? p : kUnused;
-    }
-    link[lane] = n == -1 ? raw[lane] : kUnused;
+__device__ __forceinline__ void tree_links(int lane, int T0, int& link0, int T1, int& link1) {
+  auto near = [&](int p, int T) { return lane < T && p >= -1 && p < lane ? p : kUnused; };
+  link0 = near(link0, T0);
+  link1 = near(link1, T1);
+  int a0 = link0, a1 = link1;
+  while (__any(a0 >= 0 || a1 >= 0)) {
+    const int n0 = __shfl(a0, max(a0, 0), 64), n1 = __shfl(a1, max(a1, 0), 64);
+    a0 = a0 >= 0 ? n0 : a0;
+    a1 = a1 >= 0 ? n1 : a1;
   }
+  if (a0 != -1) link0 = kUnused;
+  if (a1 != -1) link1 = kUnused;
 }
 
 // The accepted node of a row, or -1: nothing was accepted.
-__device__ __forceinline__ int accepted_node(int64_t a, int T, const int* link) {
-  return a >= 0 && a < T && link[a] != kUnused ? static_cast<int>(a) : -1;
+__device__ __forceinline__ int accepted_node(int64_t want, int T, int link) {
+  const int a = want >= 0 && want < T ? __builtin_amdgcn_readfirstlane(static_cast<int>(want)) : -1;
+  return a >= 0 && __builtin_amdgcn_readlane(link, a) != kUnused ? a : -1;
 }
 
 // A step that was verified and is not yet in the pools.
@@ -68,8 +70,11 @@ struct ConvPending {
 };
 
 // ---- conv ----
-// The row before row r of a tree: r >= 0 a node, -1, -2, -3 the taps from the newest.
-__device__ __forceinline__ int row_before(int r, const int* link) { return r >= 0 ? link[r] : r - 1; }
+// The row before row r (one for the wave) of a tree: r >= 0 a node, -1, -2, -3 the taps from
+// the newest.
+__device__ __forceinline__ int row_before(int r, int link) {
+  return r >= 0 ? __builtin_amdgcn_readlane(link, r) : r - 1;
+}
 
 // Eight channels' values (of a row, or of one tap).
 struct Row8 {
@@ -121,7 +126,7 @@ struct Taps {
     return r == -1 ? tap[2] : r == -2 ? tap[1] : tap[0];
   }
   // The taps after the accepted node: its row, its parent's and its grandparent's.
-  __device__ __forceinline__ void advance(const ConvPending& pd, int b, int c, int a, const int* link) {
+  __device__ __forceinline__ void advance(const ConvPending& pd, int b, int c, int a, int link) {
     const uint16_t* x = pd.x + b * pd.x_b + c;
     const int r1 = row_before(a, link), r0 = row_before(r1, link);
     const Row8 n2 = row8(x + a * pd.x_t);
@@ -154,7 +159,6 @@ __global__ __launch_bounds__(64) void conv_tree_kernel(const uint16_t* __restric
   // [3 + T][64], two channels per thread: the taps, oldest first, then the nodes' rows, so
   // that row r is at r + 3 (row_before)
   extern __shared__ uint32_t rows[];
-  __shared__ int raw[2][kMaxNodes], link[2][kMaxNodes];
   const int b = blockIdx.y, lane = threadIdx.x;
   const int c = 2 * (blockIdx.x * 64 + lane);
   const bool in = c < C;
@@ -165,11 +169,10 @@ __global__ __launch_bounds__(64) void conv_tree_kernel(const uint16_t* __restric
     return;
   }
   // what the links need first, then weights and rows, then the taps and the pending rows
-  const int parent = parents[b * p_b + min(lane, T - 1)];
-  int last_parent = 0;
+  int link = parents[b * p_b + min(lane, T - 1)], last_link = kUnused;
   int64_t want = -1;
   if (pd.accepted) {
-    last_parent = pd.parents[b * pd.p_b + min(lane, pd.T - 1)];
+    last_link = pd.parents[b * pd.p_b + min(lane, pd.T - 1)];
     want = pd.accepted[b];
   }
   const uint16_t* xb = x + b * x_b + (in ? c : 0);
@@ -191,18 +194,13 @@ __global__ __launch_bounds__(64) void conv_tree_kernel(const uint16_t* __restric
     for (int j = 0; j < 3; ++j) tap[j] = tp[j] | static_cast<uint32_t>(tp[sp_ch + j]) << 16;
   }
   gdn::keep_loads_here();
-  tree_links(parent, T, lane, raw[0], link[0]);
-  if (pd.accepted) tree_links(last_parent, pd.T, lane, raw[1], link[1]);
-  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront", "local");
-  __builtin_amdgcn_wave_barrier();
-  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront", "local");
-  auto before = [](int r, const int* l) { return __builtin_amdgcn_readfirstlane(row_before(r, l)); };
+  tree_links(lane, T, link, pd.T, last_link);
   auto old = [&](int r) { return r == -1 ? tap[2] : r == -2 ? tap[1] : tap[0]; };
-  const int a = pd.accepted ? __builtin_amdgcn_readfirstlane(accepted_node(want, pd.T, link[1])) : -1;
+  const int a = accepted_node(want, pd.T, last_link);
   if (a >= 0) {
     // the taps after the accepted node: its row, its parent's and its grandparent's
     const uint16_t* lx = pd.x + b * pd.x_b + (in ? c : 0);
-    const int r1 = before(a, link[1]), r0 = before(r1, link[1]);
+    const int r1 = row_before(a, last_link), r0 = row_before(r1, last_link);
     const uint32_t n2 = pair(lx + a * pd.x_t);
     const uint32_t n1 = r1 >= 0 ? pair(lx + r1 * pd.x_t) : old(r1);
     const uint32_t n0 = r0 >= 0 ? pair(lx + r0 * pd.x_t) : old(r0);
@@ -232,11 +230,12 @@ __global__ __launch_bounds__(64) void conv_tree_kernel(const uint16_t* __restric
 #pragma unroll
   for (int j = 0; j < 3; ++j) rows[j * 64 + lane] = tap[j];
   // lane t: the places of node t's three predecessors, a byte each; negative: unused
-  int places = -1;
-  if (lane < T && link[0][lane] != kUnused) {
-    const int r2 = link[0][lane], r1 = row_before(r2, link[0]), r0 = row_before(r1, link[0]);
-    places = (r2 + 3) | (r1 + 3) << 8 | (r0 + 3) << 16;
-  }
+  auto up = [&](int r) {
+    const int p = __shfl(link, max(r, 0), 64);
+    return r >= 0 ? p : r - 1;
+  };
+  const int r2 = link, r1 = up(r2), r0 = up(r1);
+  const int places = link == kUnused ? -1 : (r2 + 3) | (r1 + 3) << 8 | (r0 + 3) << 16;
   auto lo = [](uint32_t u) { return __uint_as_float(u << 16); };
   auto hi = [](uint32_t u) { return __uint_as_float(u & 0xffff0000u); };
   for (int t0 = 0; t0 < T; t0 += 8) {
@@ -250,16 +249,29 @@ __global__ __launch_bounds__(64) void conv_tree_kernel(const uint16_t* __restric
 #pragma unroll
     for (int i = 0; i < 8; ++i)
       if (t0 + i < T) rows[(3 + t0 + i) * 64 + lane] = now[i];
+    // (nodes together: their reads and chains of operations run side by side)
+    constexpr int kG = 4;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int t = t0 + i;
-      if (t >= T) break;
-      const int place = __builtin_amdgcn_readlane(places, t), at = max(place, 0);
-      const uint32_t x3 = now[i], x2 = rows[(at & 255) * 64 + lane], x1 = rows[(at >> 8 & 255) * 64 + lane],
-                     x0 = rows[(at >> 16 & 255) * 64 + lane];
-      const uint32_t out = gdn::f2bf2(gdn::conv_decode_silu(lo(x3), lo(x0), lo(x1), lo(x2), w0),
-                                      gdn::conv_decode_silu(hi(x3), hi(x0), hi(x1), hi(x2), w1));
-      if (in) yb[t * (C / 2)] = place < 0 ? 0 : out;
+    for (int i0 = 0; i0 < 8; i0 += kG) {
+      if (t0 + i0 >= T) break;
+      uint32_t x0[kG], x1[kG], x2[kG];
+      int place[kG];
+#pragma unroll
+      for (int i = 0; i < kG; ++i) {
+        place[i] = __builtin_amdgcn_readlane(places, t0 + i0 + i);
+        const int at = max(place[i], 0);
+        x2[i] = rows[(at & 255) * 64 + lane];
+        x1[i] = rows[(at >> 8 & 255) * 64 + lane];
+        x0[i] = rows[(at >> 16 & 255) * 64 + lane];
+      }
+#pragma unroll
+      for (int i = 0; i < kG; ++i) {
+        const int t = t0 + i0 + i;
+        const uint32_t x3 = now[i0 + i];
+        const uint32_t out = gdn::f2bf2(gdn::conv_decode_silu(lo(x3), lo(x0[i]), lo(x1[i]), lo(x2[i]), w0),
+                                        gdn::conv_decode_silu(hi(x3), hi(x0[i]), hi(x1[i]), hi(x2[i]), w1));
+        if (in && t < T) yb[t * (C / 2)] = place[i] < 0 ? 0 : out;
+      }
     }
   }
 }
@@ -952,7 +964,6 @@ __global__ __launch_bounds__(2 * D) void commit_tree_kernel(float* __restrict__ 
   constexpr int NW = D / 32;
   __shared__ __align__(16) float wk[kPathRows][D];
   __shared__ __align__(16) float us[kPathRows][D];
-  __shared__ int raw[kMaxNodes], link[kMaxNodes];
   __shared__ Path path;
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -961,8 +972,8 @@ __global__ __launch_bounds__(2 * D) void commit_tree_kernel(float* __restrict__ 
     const int at = blockIdx.x - states, b = at / parts;
     const int64_t slot = ids[b];
     if (slot < 0 || slot >= n_slots) return;
-    if (wave == 0) tree_links(cd.parents[b * cd.p_b + min(lane, cd.T - 1)], cd.T, lane, raw, link);
-    __syncthreads();
+    int link = cd.parents[b * cd.p_b + min(lane, cd.T - 1)], none = kUnused;
+    tree_links(lane, cd.T, link, 0, none);
     const int a = accepted_node(cd.accepted[b], cd.T, link);
     const int c0 = (at % parts * 2 * D + tid) * 8;
     if (c0 >= C || a < 0) return;
