@@ -69,6 +69,15 @@ struct ConvPending {
   int T;
 };
 
+// Rows and tiles move through buffer loads and stores: the base, which the workgroup
+// shares, in the descriptor, the lane's offset in one register, the rest in the
+// instruction, so that no address pairs sit in registers.  bytes: from where on a load gives
+// 0 and a store is dropped.
+typedef __amdgpu_buffer_rsrc_t buf_t;
+__device__ __forceinline__ buf_t buf_of(const void* base, int bytes = 0x7fffffff) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), static_cast<short>(0), bytes, 0x00020000);
+}
+
 // ---- conv ----
 // The row before row r (one for the wave) of a tree: r >= 0 a node, -1, -2, -3 the taps from
 // the newest.
@@ -145,27 +154,36 @@ __device__ __forceinline__ bool dense_taps(const uint16_t* pool, int64_t sp_slot
 // A workgroup is one wave: 128 channels of one sequence, two per thread, all nodes.  A
 // thread's rows go through its own column of LDS, where their children find them: every
 // row is read once, no wave waits for another, and a thread rolls its own channels' taps.
-// Rows come 8 at a time, the next ones on their way while these are worked on.  Bound by
-// the rows' way in and out (2 + 2 bytes per value) and the SiLU's two transcendentals per
-// value, with few sequences by the latency of links, rows and taps.  (256 threads of 8
-// channels that share the nodes of a sequence: 64 trees of 16 nodes, 8192 channels 17.7
-// us, one tree of 8 nodes 5.5.)
+// Rows come 4 at a time, the next 8 on their way while these are worked on, 4 nodes' chains of
+// operations side by side.  No branch in the loop: rows past T are past the buffers' ends, and
+// the counts by which a wave waits for its rows stay known (else it waits for its stores too).
+//
+// Bound by the rows' way in and out (2 + 2 bytes per value) and, with few waves, by each
+// node's own chain: 64 trees of 64 nodes, 8192 channels 35.3 us (4.1 TB/s), of 16 nodes 11.3,
+// one tree of 16 nodes 5.0, of 8 nodes 4.1.  Before: with a branch per node 49.7, 13.0, 6.8
+// and 5.1; four channels per thread in place of two 57.4, 14.2, 8.1, 5.9; 256 threads of 8
+// channels that share the nodes of a sequence 17.7 (64 x 16) and 5.5 (1 x 8).
 __global__ __launch_bounds__(64) void conv_tree_kernel(const uint16_t* __restrict__ x, int64_t x_b, int64_t x_t,
                                                        uint16_t* __restrict__ pool, int64_t sp_slot, int64_t sp_ch,
                                                        int64_t n_slots, const int64_t* __restrict__ ids,
                                                        const uint16_t* __restrict__ w,
                                                        const int32_t* __restrict__ parents, int64_t p_b,
                                                        ConvPending pd, uint16_t* __restrict__ y, int T, int C) {
-  // [3 + T][64], two channels per thread: the taps, oldest first, then the nodes' rows, so
-  // that row r is at r + 3 (row_before)
+  // [3 + T up to whole groups][64], two channels per thread: the taps, oldest first, then the
+  // nodes' rows, so that row r is at r + 3 (row_before)
   extern __shared__ uint32_t rows[];
   const int b = blockIdx.y, lane = threadIdx.x;
   const int c = 2 * (blockIdx.x * 64 + lane);
   const bool in = c < C;
-  uint32_t* yb = reinterpret_cast<uint32_t*>(y + static_cast<int64_t>(b) * T * C + c);
+  // (x_t < 2^24, C < 2^23: the rows of 64 nodes and a few more have 32-bit offsets, also from
+  // 2^31 on, where the stores of channels past C are dropped)
+  const buf_t by = buf_of(y + static_cast<int64_t>(b) * T * C, T * C * 2);
+  const buf_t bx = buf_of(x + b * x_b, ((T - 1) * static_cast<int>(x_t) + C) * 2);
+  const uint32_t y_row = 2 * C, x_row = 2 * static_cast<uint32_t>(x_t);
+  const uint32_t y_at = in ? 2 * c : 0x80000000u, x_at = 2 * c;
   const int64_t slot = ids[b];
   if (slot < 0 || slot >= n_slots) {  // (the whole workgroup)
-    for (int t = 0; t < T && in; ++t) yb[t * (C / 2)] = 0;
+    for (int t = 0; t < T; ++t) __builtin_amdgcn_raw_buffer_store_b32(0u, by, y_at + t * y_row, 0, 0);
     return;
   }
   // what the links need first, then weights and rows, then the taps and the pending rows
@@ -175,13 +193,21 @@ __global__ __launch_bounds__(64) void conv_tree_kernel(const uint16_t* __restric
     last_link = pd.parents[b * pd.p_b + min(lane, pd.T - 1)];
     want = pd.accepted[b];
   }
-  const uint16_t* xb = x + b * x_b + (in ? c : 0);
   uint16_t* tp = pool + slot * sp_slot + (in ? c : 0) * sp_ch;
   const uint4 wv = *reinterpret_cast<const uint4*>(w + (in ? c : 0) * 4);
   auto pair = [](const uint16_t* p) { return *reinterpret_cast<const uint32_t*>(p); };
-  uint32_t next[8];
+  constexpr int kG = 4;  // nodes at a time
+  struct Group {
+    uint32_t v[kG];
+  };
+  auto load = [&](int t0) {
+    Group r;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) next[i] = pair(xb + min(i, T - 1) * x_t);
+    for (int i = 0; i < kG; ++i)
+      r.v[i] = __builtin_amdgcn_raw_buffer_load_b32(bx, x_at + static_cast<uint32_t>(t0 + i) * x_row, 0, 0);
+    return r;
+  };
+  Group next[2] = {load(0), load(kG)};
   uint32_t tap[3];  // of both channels, oldest first
   const bool dense = sp_ch == 3 && sp_slot % 2 == 0 && reinterpret_cast<uintptr_t>(pool) % 4 == 0;
   if (dense) {
@@ -207,18 +233,6 @@ __global__ __launch_bounds__(64) void conv_tree_kernel(const uint16_t* __restric
     tap[0] = n0;
     tap[1] = n1;
     tap[2] = n2;
-    if (in && dense) {
-      uint32_t* q = reinterpret_cast<uint32_t*>(tp);
-      q[0] = (n0 & 0xffffu) | (n1 << 16);
-      q[1] = (n2 & 0xffffu) | (n0 & 0xffff0000u);
-      q[2] = (n1 >> 16) | (n2 & 0xffff0000u);
-    } else if (in) {
-#pragma unroll
-      for (int j = 0; j < 3; ++j) {
-        tp[j] = static_cast<uint16_t>(tap[j]);
-        tp[sp_ch + j] = static_cast<uint16_t>(tap[j] >> 16);
-      }
-    }
   }
   float w0[4], w1[4];
   const uint32_t ww[4] = {wv.x, wv.y, wv.z, wv.w};
@@ -238,40 +252,42 @@ __global__ __launch_bounds__(64) void conv_tree_kernel(const uint16_t* __restric
   const int places = link == kUnused ? -1 : (r2 + 3) | (r1 + 3) << 8 | (r0 + 3) << 16;
   auto lo = [](uint32_t u) { return __uint_as_float(u << 16); };
   auto hi = [](uint32_t u) { return __uint_as_float(u & 0xffff0000u); };
-  for (int t0 = 0; t0 < T; t0 += 8) {
-    uint32_t now[8];
+  for (int t0 = 0; t0 < T; t0 += kG) {
+    const Group now = next[0];
+    next[0] = next[1];
+    next[1] = load(t0 + 2 * kG);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) now[i] = next[i];
-    if (t0 + 8 < T) {
+    for (int i = 0; i < kG; ++i) rows[(3 + t0 + i) * 64 + lane] = now.v[i];
+    uint32_t x0[kG], x1[kG], x2[kG];
+    int place[kG];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) next[i] = pair(xb + min(t0 + 8 + i, T - 1) * x_t);
+    for (int i = 0; i < kG; ++i) {
+      place[i] = __builtin_amdgcn_readlane(places, t0 + i);
+      const int at = max(place[i], 0);
+      x2[i] = rows[(at & 255) * 64 + lane];
+      x1[i] = rows[(at >> 8 & 255) * 64 + lane];
+      x0[i] = rows[(at >> 16 & 255) * 64 + lane];
     }
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (t0 + i < T) rows[(3 + t0 + i) * 64 + lane] = now[i];
-    // (nodes together: their reads and chains of operations run side by side)
-    constexpr int kG = 4;
+    for (int i = 0; i < kG; ++i) {
+      const uint32_t x3 = now.v[i];
+      const uint32_t out = gdn::f2bf2(gdn::conv_decode_silu(lo(x3), lo(x0[i]), lo(x1[i]), lo(x2[i]), w0),
+                                      gdn::conv_decode_silu(hi(x3), hi(x0[i]), hi(x1[i]), hi(x2[i]), w1));
+      __builtin_amdgcn_raw_buffer_store_b32(place[i] < 0 ? 0u : out, by, y_at + static_cast<uint32_t>(t0 + i) * y_row,
+                                            0, 0);
+    }
+  }
+  if (a < 0 || !in) return;
+  if (dense) {
+    uint32_t* q = reinterpret_cast<uint32_t*>(tp);
+    q[0] = (tap[0] & 0xffffu) | (tap[1] << 16);
+    q[1] = (tap[2] & 0xffffu) | (tap[0] & 0xffff0000u);
+    q[2] = (tap[1] >> 16) | (tap[2] & 0xffff0000u);
+  } else {
 #pragma unroll
-    for (int i0 = 0; i0 < 8; i0 += kG) {
-      if (t0 + i0 >= T) break;
-      uint32_t x0[kG], x1[kG], x2[kG];
-      int place[kG];
-#pragma unroll
-      for (int i = 0; i < kG; ++i) {
-        place[i] = __builtin_amdgcn_readlane(places, t0 + i0 + i);
-        const int at = max(place[i], 0);
-        x2[i] = rows[(at & 255) * 64 + lane];
-        x1[i] = rows[(at >> 8 & 255) * 64 + lane];
-        x0[i] = rows[(at >> 16 & 255) * 64 + lane];
-      }
-#pragma unroll
-      for (int i = 0; i < kG; ++i) {
-        const int t = t0 + i0 + i;
-        const uint32_t x3 = now[i0 + i];
-        const uint32_t out = gdn::f2bf2(gdn::conv_decode_silu(lo(x3), lo(x0[i]), lo(x1[i]), lo(x2[i]), w0),
-                                        gdn::conv_decode_silu(hi(x3), hi(x0[i]), hi(x1[i]), hi(x2[i]), w1));
-        if (in && t < T) yb[t * (C / 2)] = place[i] < 0 ? 0 : out;
-      }
+    for (int j = 0; j < 3; ++j) {
+      tp[j] = static_cast<uint16_t>(tap[j]);
+      tp[sp_ch + j] = static_cast<uint16_t>(tap[j] >> 16);
     }
   }
 }
@@ -305,15 +321,7 @@ typedef float f32x2_t __attribute__((ext_vector_type(2)));
 constexpr float kEps = 1e-6f;
 constexpr int kPathRows = 16;  // of a pending path in LDS at a time
 
-// Rows and tiles move through buffer loads and stores: the base, which the workgroup
-// shares, in the descriptor, the lane's offset in one register, the rest in the
-// instruction, so that no address pairs sit in the registers beside the state.  The range
-// is left open: the offsets stay inside of the arrays.
-typedef __amdgpu_buffer_rsrc_t buf_t;
 constexpr int kNT = 2;  // cache policy: non-temporal
-__device__ __forceinline__ buf_t buf_of(const void* base) {
-  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), static_cast<short>(0), 0x7fffffff, 0x00020000);
-}
 __device__ __forceinline__ gdn::s16x8_t buf_row(buf_t r, int voff) {
   return __builtin_bit_cast(gdn::s16x8_t, __builtin_amdgcn_raw_buffer_load_b128(r, voff, 0, 0));
 }
@@ -1070,7 +1078,7 @@ extern "C" int gdn_conv_tree(const uint16_t* x, int64_t x_b, int64_t x_t, uint16
                              const int32_t* last_parents, int64_t lp_b, const int64_t* accepted, int last_T,
                              uint16_t* y, int B, int T, int C, void* stream) {
   if (B < 0 || T < 0 || C <= 0 || n_slots < 0) return GDN_ERR_INVALID_ARG;
-  if (T > kMaxNodes || (accepted && last_T > kMaxNodes) || C % 8) return GDN_ERR_UNSUPPORTED;
+  if (T > kMaxNodes || (accepted && last_T > kMaxNodes) || C % 8 || C >= 1 << 23) return GDN_ERR_UNSUPPORTED;
   if (B == 0 || T == 0) return GDN_OK;
   if (!rows_ok(x, x_b, x_t, C, T) || !pool || !ids || !w || !parents || !y || p_b < 0 || sp_ch < 3 ||
       sp_slot < static_cast<int64_t>(C - 1) * sp_ch + 3 || reinterpret_cast<uintptr_t>(w) % 16 ||
@@ -1079,7 +1087,7 @@ extern "C" int gdn_conv_tree(const uint16_t* x, int64_t x_b, int64_t x_t, uint16
   if (accepted && (!rows_ok(last_x, lx_b, lx_t, C, last_T) || !last_parents || lp_b < 0)) return GDN_ERR_INVALID_ARG;
   if (B > 65535) return GDN_ERR_UNSUPPORTED;
   const ConvPending pd{last_x, lx_b, lx_t, last_parents, lp_b, accepted, last_T};
-  conv_tree_kernel<<<dim3((C + 127) / 128, B), dim3(64), (T + 3) * 256, static_cast<hipStream_t>(stream)>>>(
+  conv_tree_kernel<<<dim3((C + 127) / 128, B), dim3(64), ((T + 3) / 4 * 4 + 3) * 256, static_cast<hipStream_t>(stream)>>>(
       x, x_b, x_t, pool, sp_slot, sp_ch, n_slots, ids, w, parents, p_b, pd, y, T, C);
   return gdn_launch_status();
 }

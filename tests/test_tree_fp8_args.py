@@ -249,7 +249,7 @@ def test_calls_by_words(pkg):
             assert lib.gdn_call_words(pack(wrong, *zeros)) == inv
     pack, head = _lib.WORDS["gdn_conv_tree"]
     conv = lambda B=0, T=8, C=64: lib.gdn_call_words(pack(head, *[0] * 19, B, T, C, 0))  # noqa: E731
-    assert conv() == ok and conv(T=65) == uns and conv(C=0) == inv and conv(B=1) == inv
+    assert conv() == ok and conv(T=65) == uns and conv(C=1 << 23) == uns and conv(C=0) == inv and conv(B=1) == inv
     assert conv(B=1 << 32) == inv and conv(T=(1 << 32) + 8) == inv       # 0 and 8 if they were cut
     for n in range(1, 5):
         pack, head = _lib.GEMM_FP8_WORDS[n]
