@@ -318,6 +318,8 @@ __global__ __launch_bounds__(64) void conv_tree_kernel(const uint16_t* __restric
 // weights, the nodes' norms and dot products (on the matrix cores as well) and the
 // pending path's rows are worked on while the state is on its way.
 typedef float f32x2_t __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
 constexpr float kEps = 1e-6f;
 constexpr int kPathRows = 16;  // of a pending path in LDS at a time
 
@@ -347,14 +349,13 @@ struct Tile {
             f32x2_t, __builtin_amdgcn_raw_buffer_load_b64(r, voff + e * D * 4, 32 * kk * D * 4, kNT));
   }
   __device__ __forceinline__ void store(buf_t r, int voff) const {
-    typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
     // (a region of its own: nothing overwrites a register whose store is being issued)
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int kk = 0; kk < D / 32; ++kk)
 #pragma unroll
       for (int e = 0; e < 8; ++e)
-        __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u32x2, s[kk][e]), r, voff + e * D * 4,
+        __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u32x2_t, s[kk][e]), r, voff + e * D * 4,
                                               32 * kk * D * 4, kNT);
     asm volatile("s_nop 1");
     __builtin_amdgcn_sched_barrier(0);
@@ -770,6 +771,11 @@ __global__ __launch_bounds__(2 * D, NT <= 2 ? 3 : NT == 3 || D == 128 ? 2 : 1) v
   // (the nodes' rows come again, from the caches, one product ahead: held in registers from
   // the start they would cost a workgroup per CU)
   const int tiles = (T + 15) / 16;
+  // What is written is dropped past the buffers' ends (rows past T): no branch, and the counts
+  // by which a wave waits for its loads stay known (else it waits for its stores too).
+  const int out_row = static_cast<int>(out_t), out_end = (T - 1) * out_row + D;
+  const buf_t bu = buf_of(u + out0, 4 * out_end);
+  const buf_t bo = kLayer && L.y8 ? buf_of(L.y8 + out0, out_end) : buf_of(o + out0, 2 * out_end);
   constexpr int kLanes = D / 8;  // of a row in the norm: 8 columns each
   const int row = tid / kLanes, c8 = tid % kLanes * 8;
   auto z_row = [&](int I) {
@@ -798,7 +804,7 @@ __global__ __launch_bounds__(2 * D, NT <= 2 ? 3 : NT == 3 || D == 128 ? 2 : 1) v
     for (int m = kLanes / 2; m >= 1; m >>= 1) ss += __shfl_xor(ss, m, 64);
     const float r = rsqrtf(ss / static_cast<float>(D) + L.eps);
     const bool on = link[t] != kUnused;
-    const int64_t at = out0 + t * out_t + c8;
+    const int at = t * out_row + c8;
     if (D == 128 && L.y8) {
       float top = 0.0f;
 #pragma unroll
@@ -809,25 +815,23 @@ __global__ __launch_bounds__(2 * D, NT <= 2 ? 3 : NT == 3 || D == 128 ? 2 : 1) v
 #pragma unroll
       for (int m = 8; m >= 1; m >>= 1) top = fmaxf(top, __shfl_xor(top, m, 64));
       const float s = gdn::fp8_scale(top), inv = 1.0f / s;
-      if (t < T) {
-        *reinterpret_cast<uint2*>(L.y8 + at) =
-            make_uint2(gdn::f2fp8x4(v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv),
-                       gdn::f2fp8x4(v[4] * inv, v[5] * inv, v[6] * inv, v[7] * inv));
-        if (c8 == 0) L.scale[static_cast<int64_t>(h) * B * T + static_cast<int64_t>(b) * T + t] = s;
-      }
+      const u32x2_t w8 = {gdn::f2fp8x4(v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv),
+                          gdn::f2fp8x4(v[4] * inv, v[5] * inv, v[6] * inv, v[7] * inv)};
+      __builtin_amdgcn_raw_buffer_store_b64(w8, bo, at, 0, 0);
+      const buf_t bs8 = buf_of(L.scale + (static_cast<int64_t>(h) * B + b) * T, 4 * T);
+      __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(s), bs8, c8 == 0 ? 4 * t : 4 * kMaxNodes, 0, 0);
     } else {
 #pragma unroll
       for (int i = 0; i < 8; ++i) v[i] = on ? gdn::norm_gate(v[i], r, gdn::bf2f(ws[i]), gdn::bf2f(zs[i])) : 0.0f;
-      if (t < T)
-        *reinterpret_cast<uint4*>(o + at) = make_uint4(gdn::f2bf2(v[0], v[1]), gdn::f2bf2(v[2], v[3]),
-                                                       gdn::f2bf2(v[4], v[5]), gdn::f2bf2(v[6], v[7]));
+      const u32x4_t w16 = {gdn::f2bf2(v[0], v[1]), gdn::f2bf2(v[2], v[3]), gdn::f2bf2(v[4], v[5]),
+                           gdn::f2bf2(v[6], v[7])};
+      __builtin_amdgcn_raw_buffer_store_b128(w16, bo, 2 * at, 0, 0);
     }
   };
   gdn::s16x8_t nk = k_frag(0, 0), nq = q_frag(0, 0);
 #pragma unroll
   for (int kk = 0; kk < KK; ++kk) {
-    typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-    u32x4 f[2][3];
+    u32x4_t f[2][3];
 #pragma unroll
     for (int e = 0; e < 4; ++e)
 #pragma unroll
@@ -894,10 +898,12 @@ __global__ __launch_bounds__(2 * D, NT <= 2 ? 3 : NT == 3 || D == 128 ? 2 : 1) v
     for (int r = 0; r < 4; ++r) {
       const int t = 16 * I + 4 * lg + r;
       fine &= finite(uu[I][0][r]) && finite(uu[I][1][r]);
-      if (t < T) *reinterpret_cast<f32x2_t*>(u + out0 + t * out_t + col) = f32x2_t{uu[I][0][r], uu[I][1][r]};
+      const int at = t * out_row + col;
+      __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u32x2_t, f32x2_t{uu[I][0][r], uu[I][1][r]}), bu, 4 * at,
+                                            0, 0);
       const uint32_t pair = gdn::f2bf2(out[0][r], out[1][r]);
       if constexpr (kLayer) *reinterpret_cast<uint32_t*>(&rows[I & 1][4 * lg + r][col]) = pair;
-      else if (t < T) *reinterpret_cast<uint32_t*>(o + out0 + t * out_t + col) = pair;
+      else __builtin_amdgcn_raw_buffer_store_b32(pair, bo, 2 * at, 0, 0);
     }
     if constexpr (kLayer) {
       if (__any(!fine) && lane == 0) bad = 1;
@@ -1049,7 +1055,9 @@ int rule_check(const RuleRows& r, const float* s_pool, int64_t s_slot, int64_t n
   if (pd.accepted && (!rows_ok(pd.k, pd.k_b, pd.k_t, Hk * D, pd.T) || !pd.g || !pd.u || !pd.parents || pd.p_b < 0 ||
                       reinterpret_cast<uintptr_t>(pd.u) % 16))
     return GDN_ERR_INVALID_ARG;
-  return static_cast<int64_t>(B) * Hv >= (1LL << 24) ? GDN_ERR_UNSUPPORTED : GDN_OK;
+  // (Hv D below 2^23: 64 rows of u have 32-bit byte offsets)
+  return static_cast<int64_t>(B) * Hv >= (1LL << 24) || static_cast<int64_t>(Hv) * D >= (1 << 23) ? GDN_ERR_UNSUPPORTED
+                                                                                                   : GDN_OK;
 }
 
 template <bool kLayer>
