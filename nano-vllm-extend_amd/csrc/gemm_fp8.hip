@@ -18,6 +18,7 @@
 // On normal data that is 2^-17 of the sum of magnitudes, far inside of the bf16 result's
 // half step.  Everything after a block's sum is fp32, and one rounding to bf16.
 #include <algorithm>
+#include <utility>
 
 #include "gemm_tile.h"
 #include "quant_fp8.h"
@@ -375,61 +376,66 @@ __global__ __launch_bounds__(kPPThreads, 2) void gemm_fp8_pp_kernel(const uint8_
 // The layer's gate projections are a few columns whose weight stays in bf16, read with
 // the same rows.  A launch of their own costs more than they do (64 columns of 2048: 5
 // us), so the kernels that quantize the rows take them along: 16 rows x 16 columns per
-// workgroup, K-steps of 128 dealt to its waves, two stages per wave, as in the ring.
+// workgroup, K-steps of 64 or 128 dealt to its waves, two stages per wave, as in the ring.
 struct Fp8Wide {
   const uint16_t* b;  // [n, K] bf16, row stride ldb; columns N .. N + n - 1 of the output
   int64_t ldb;
   int n;              // a multiple of 16; 0: none
 };
 
-// Bytes of a stage of one wave: 16 rows of 256 bytes of each operand.
-constexpr int kWideStage = 2 * 16 * 256;
+// Bytes of a stage of one wave: 16 rows of KS values of each operand.
+constexpr int wide_stage(int KS) { return 2 * 16 * 2 * KS; }
 
-template <int NW>
+template <int NW, int KS>
 __device__ __forceinline__ void wide_tile(const void* __restrict__ A, int64_t lda, const Fp8Wide& wide,
                                           const GemmOut& out, int M, int N, int K, int m0, int n0, uint8_t* st0,
-                                          uint8_t* st1, int stage) {
+                                          uint8_t* st1) {
+  constexpr int kRow = 2 * KS, kGran = kRow / 16;  // bytes and 16-byte granules of a row
+  constexpr int kLoads = 16 * kRow / 1024;         // of an operand's stage
+  constexpr int kWait = 2 * kLoads | (7 << 4) | (15 << 8);  // all but the newest stage
+  static_assert(2 * kLoads < 16, "vmcnt field");
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int lr = lane & 15, lg = lane >> 4;
   const __amdgpu_buffer_rsrc_t ra = rsrc_of(A), rb = rsrc_of(wide.b);
-  int voff[8];
+  int voff[2 * kLoads];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    // 4 rows of 256 bytes; granule c of row r at slot c ^ r
-    const int r = 4 * i + (lane >> 4), at = 16 * ((lane & 15) ^ r);
+  for (int i = 0; i < kLoads; ++i) {
+    // granule c of row r at slot c ^ (r % kGran)
+    const int r = 1024 / kRow * i + lane / kGran, at = 16 * ((lane % kGran) ^ (r % kGran));
     voff[i] = static_cast<int>(min(m0 + r, M - 1) * lda * 2 + at);
-    voff[4 + i] = static_cast<int>((n0 + r) * wide.ldb * 2 + at);
+    voff[kLoads + i] = static_cast<int>((n0 + r) * wide.ldb * 2 + at);
   }
-  const int nk = K / 128;
+  const int nk = K / KS;
   auto issue = [&](uint8_t* st, int step) {
-    uint8_t* w = st + wave * stage;
-    const int s = 256 * min(step, nk - 1);
+    uint8_t* w = st + wave * wide_stage(KS);
+    const int s = kRow * min(step, nk - 1);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) dma16(i < 4 ? ra : rb, w + i * 1024, voff[i], s);
+    for (int i = 0; i < 2 * kLoads; ++i) dma16(i < kLoads ? ra : rb, w + i * 1024, voff[i], s);
   };
   gdn::f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
   auto one = [&](uint8_t* st, int step) {
-    const uint8_t* a = st + wave * stage;
-    gdn::s16x8_t fa[4], fb[4];
+    const uint8_t* a = st + wave * wide_stage(KS) + lr * kRow;
+    gdn::s16x8_t fa[KS / 32], fb[KS / 32];
 #pragma unroll
-    for (int c = 0; c < 4; ++c) {
-      fa[c] = *reinterpret_cast<const gdn::s16x8_t*>(a + lr * 256 + 16 * ((4 * c + lg) ^ lr));
-      fb[c] = *reinterpret_cast<const gdn::s16x8_t*>(a + 4096 + lr * 256 + 16 * ((4 * c + lg) ^ lr));
+    for (int c = 0; c < KS / 32; ++c) {
+      const int at = 16 * ((4 * c + lg) ^ (lr % kGran));
+      fa[c] = *reinterpret_cast<const gdn::s16x8_t*>(a + at);
+      fb[c] = *reinterpret_cast<const gdn::s16x8_t*>(a + 16 * kRow + at);
     }
     __builtin_amdgcn_sched_barrier(0);
     __builtin_amdgcn_s_waitcnt(kWaitLds);
     __builtin_amdgcn_sched_barrier(0);
     issue(st, step + 2 * NW);
 #pragma unroll
-    for (int c = 0; c < 4; ++c) acc = gdn::mfma16x16x32(fb[c], fa[c], acc);
+    for (int c = 0; c < KS / 32; ++c) acc = gdn::mfma16x16x32(fb[c], fa[c], acc);
     __builtin_amdgcn_sched_barrier(0);
-    __builtin_amdgcn_s_waitcnt(8 | (7 << 4) | (15 << 8));  // vmcnt(8): all but the newest stage
+    __builtin_amdgcn_s_waitcnt(kWait);
     __builtin_amdgcn_sched_barrier(0);
   };
   issue(st0, wave);
   issue(st1, wave + NW);
-  __builtin_amdgcn_s_waitcnt(8 | (7 << 4) | (15 << 8));
+  __builtin_amdgcn_s_waitcnt(kWait);
   int s = wave;
   for (; s + NW < nk; s += 2 * NW) {
     one(st0, s);
@@ -471,15 +477,15 @@ __device__ __forceinline__ void wide_tile(const void* __restrict__ A, int64_t ld
 __global__ __launch_bounds__(256) void quant_wide_kernel(const uint16_t* __restrict__ A, int64_t lda,
                                                          uint8_t* __restrict__ y, float* __restrict__ scale,
                                                          Fp8Wide wide, GemmOut out, int M, int N, int K, int groups) {
-  __shared__ __align__(16) uint8_t st0[4 * kWideStage];
-  __shared__ __align__(16) uint8_t st1[4 * kWideStage];
+  __shared__ __align__(16) uint8_t st0[4 * wide_stage(128)];
+  __shared__ __align__(16) uint8_t st1[4 * wide_stage(128)];
   if (static_cast<int>(blockIdx.x) < groups) {
     quant_group<false>(A, lda, y, K, scale, 1, M, M, K / gdn::kFp8Group,
                        static_cast<int64_t>(blockIdx.x) * 16 + threadIdx.x / 16, threadIdx.x % 16);
     return;
   }
   const int t = blockIdx.x - groups, mb_n = (M + 15) / 16;
-  wide_tile<4>(A, lda, wide, out, M, N, K, 16 * (t % mb_n), 16 * (t / mb_n), st0, st1, kWideStage);
+  wide_tile<4, 128>(A, lda, wide, out, M, N, K, 16 * (t % mb_n), 16 * (t / mb_n), st0, st1);
 }
 
 // the larger of each pair of 16-bit halves
@@ -487,6 +493,31 @@ typedef uint16_t u16x2_t __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {
   const u16x2_t x = __builtin_bit_cast(u16x2_t, a), y = __builtin_bit_cast(u16x2_t, b);
   return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(x, y));
+}
+
+// The waves' partial sums, added in wave order, into C.  red: [wave][row tile][column
+// tile][lane], free of loads and readers.
+template <int MT, int NT, int NW>
+__device__ __forceinline__ void ring_store(const gdn::f32x4_t (&acc)[MT][NT][2], gdn::f32x4_t* red, const GemmOut& out,
+                                           int M, int N, int m0, int n0) {
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+#pragma unroll
+  for (int i = 0; i < MT; ++i)
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+      for (int t = 0; t < 2; ++t) red[(((wave * MT + i) * NT + j) * 2 + t) * 64 + lane] = acc[i][j][t];
+  __syncthreads();
+  for (int ij = wave; ij < MT * NT; ij += NW) {
+    gdn::f32x4_t c0 = red[(ij * 2) * 64 + lane], c1 = red[(ij * 2 + 1) * 64 + lane];
+#pragma unroll
+    for (int w = 1; w < NW; ++w) {
+      c0 += red[((w * MT * NT + ij) * 2) * 64 + lane];
+      c1 += red[((w * MT * NT + ij) * 2 + 1) * 64 + lane];
+    }
+    gemm_store16(c0, c1, out, M, N, m0 + 16 * (ij / NT), n0 + 32 * (ij % NT), lane, GemmGates{}, nullptr);
+  }
 }
 
 // ---- few rows: a load ring per wave ----
@@ -498,7 +529,8 @@ __device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {
 // kQuant: A is bf16 and is brought to e4m3 here (gdn::fp8_scale, the bits of
 // gdn_quantize_fp8), a lane's 32 values of a row in its registers and the largest
 // magnitude over the four lanes that share the row: no launch of its own and nothing
-// written.  Every workgroup repeats it for its rows, so it is for few of them.
+// written.  Every workgroup repeats it for its rows, so it is for few of them (fewer still:
+// gemm_fp8_rows_kernel).
 template <int BM, int BN, int NW, int NS, bool kQuant>
 __global__ __launch_bounds__(64 * NW) void gemm_fp8_ring_kernel(const void* __restrict__ A, int64_t lda,
                                                                 const uint8_t* __restrict__ B, int64_t ldb,
@@ -522,10 +554,10 @@ __global__ __launch_bounds__(64 * NW) void gemm_fp8_ring_kernel(const void* __re
   const int64_t L = gdn::xcd_remap(blockIdx.x, static_cast<int64_t>(mb_n) * (nb_n + (kQuant ? wide.n / 16 : 0)));
   if (L < 0) return;
   if constexpr (kQuant) {
-    static_assert(BM == 16 && kStage >= kWideStage, "wide tiles in the ring's stages");
+    static_assert(BM == 16 && kStage >= wide_stage(128), "wide tiles in the ring's stages");
     if (L >= static_cast<int64_t>(mb_n) * nb_n) {
       const int t = static_cast<int>(L - static_cast<int64_t>(mb_n) * nb_n);
-      wide_tile<NW>(A, lda, wide, out, M, N, K, 16 * (t % mb_n), 16 * (t / mb_n), st0, st1, kStage);
+      wide_tile<NW, 128>(A, lda, wide, out, M, N, K, 16 * (t % mb_n), 16 * (t / mb_n), st0, st1);
       return;
     }
   }
@@ -673,23 +705,179 @@ __global__ __launch_bounds__(64 * NW) void gemm_fp8_ring_kernel(const void* __re
   // the repeated loads past the last step land before the stages are reused
   __builtin_amdgcn_s_waitcnt(0);
   __syncthreads();
-  gdn::f32x4_t* red = reinterpret_cast<gdn::f32x4_t*>(st0);  // [wave][row tile][column tile][lane]
+  ring_store<MT, NT, NW>(acc, reinterpret_cast<gdn::f32x4_t*>(st0), out, M, N, m0, n0);
+}
+
+// v of the lane D places on, around each 16 lanes
+template <int D>
+__device__ __forceinline__ float row_ror(float v) {
+  return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x120 + D, 15, 15, false));
+}
+
+template <class F, int... I>
+__device__ __forceinline__ void each(const F& f, std::integer_sequence<int, I...>) {
+  (f(std::integral_constant<int, I>{}), ...);
+}
+
+// ---- up to 8 bf16 rows ----
+// The ring of 16 rows for R (4 or 8) of them that come in bf16.  A wave has at most S K-steps: it
+// asks for its rows' values of all of them first, 8 per lane, then for as many stages of B as LDS
+// holds, and quantizes while B is on its way, into LDS rows as the ring's loads would leave them:
+// R S / 4 passes of 55 instructions, where the ring's own way takes 140 for each of S steps,
+// whether its 16 rows are there or not, and between the waits.  1 x 12288 x 2048 5.2 us (ring 6.7,
+// e4m3 rows 5.1), 8 rows 5.7 (6.7), 1 x 2048 x 4096 4.7 (7.0), 8 rows 5.9 (7.2); for 16 rows 7.5 and
+// 8.2 (6.8, 7.2).
+template <int BN, int NW, int NS, int S, int R>
+__global__ __launch_bounds__(64 * NW) void gemm_fp8_rows_kernel(const uint16_t* __restrict__ A, int64_t lda,
+                                                                const uint8_t* __restrict__ B, int64_t ldb,
+                                                                Fp8Scales sc, GemmOut out, int M, int N, int K,
+                                                                Fp8Wide wide) {
+  constexpr int NT = BN / 32;
+  constexpr int kBBytes = BN * 128, kStage = kBBytes + 256;
+  constexpr int kBPer = kBBytes / 1024, kPer = kBPer + 1;  // loads of a stage
+  static_assert(NS <= 4 && NS <= S && (NS - 1) * kPer < 64, "stages, vmcnt field");
+  static_assert(kStage >= wide_stage(64) && NT * 2048 <= kStage, "wide tiles and partial sums fit a stage");
+  __shared__ __align__(16) uint8_t st0[NW * kStage];
+  __shared__ __align__(16) uint8_t st1[NW * kStage];
+  __shared__ __align__(16) uint8_t st2[NS > 2 ? NW * kStage : 16];
+  __shared__ __align__(16) uint8_t st3[NS > 3 ? NW * kStage : 16];
+  __shared__ __align__(16) uint8_t rows[NW * S * 2048];  // [wave][step] 16 rows of 128 bytes
+  __shared__ float scales[NW * S * 16];
+  const int mb_n = (M + 15) / 16, nb_n = (N + BN - 1) / BN;
+  const int64_t L = gdn::xcd_remap(blockIdx.x, static_cast<int64_t>(mb_n) * (nb_n + wide.n / 16));
+  if (L < 0) return;
+  if (L >= static_cast<int64_t>(mb_n) * nb_n) {
+    const int t = static_cast<int>(L - static_cast<int64_t>(mb_n) * nb_n);
+    wide_tile<NW, 64>(A, lda, wide, out, M, N, K, 16 * (t % mb_n), 16 * (t / mb_n), st0, st1);
+    return;
+  }
+  const int m0 = 16 * static_cast<int>(L % mb_n), n0 = BN * static_cast<int>(L / mb_n);
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lr = lane & 15, lg = lane >> 4;
+  const __amdgpu_buffer_rsrc_t ra = rsrc_of(A), rb = rsrc_of(B), rsb = rsrc_of(sc.b);
+  const int nk = K / 128;
+  // pass p: the 8 values l of step g % S of row g / S, g = 4 p + lane / 16
+  constexpr int P = R * S / 4;
+  static_assert(R * S % 4 == 0, "whole passes");
+  const int l = lane & 15;
+  auto row_of = [&](int p) { return (4 * p + lg) / S; };
+  auto step_of = [&](int p) { return (4 * p + lg) % S; };
+  i32x4_t raw[P];
 #pragma unroll
-  for (int i = 0; i < MT; ++i)
+  for (int p = 0; p < P; ++p)
+    raw[p] = __builtin_bit_cast(
+        i32x4_t, __builtin_amdgcn_raw_buffer_load_b128(
+                     ra, static_cast<int>(min(m0 + row_of(p), M - 1) * lda * 2) + 16 * l +
+                             256 * min(wave + NW * step_of(p), nk - 1), 0, 0));
+  gdn::keep_loads_here();
+  int goff[kBPer];
+#pragma unroll
+  for (int i = 0; i < kBPer; ++i) {
+    const int r = 8 * i + (lane >> 3);
+    goff[i] = static_cast<int>(min(n0 + r, N - 1) * ldb + 16 * ((lane & 7) ^ (((r >> 1) & 1) | (((r >> 3) & 3) << 1))));
+  }
+  const int vb = static_cast<int>(n0 / 128 * sc.b_row * 4);
+  auto issue = [&](uint8_t* st, int i) {
+    const int s = min(wave + NW * i, nk - 1);
+    uint8_t* w = st + wave * kStage;
+#pragma unroll
+    for (int k = 0; k < kBPer; ++k) dma16(rb, w + k * 1024, goff[k], 128 * s);
+    dma4(rsb, w + kBBytes, vb, 4 * s);
+  };
+  uint8_t* const st[4] = {st0, st1, st2, st3};
+#pragma unroll
+  for (int i = 0; i < NS; ++i) issue(st[i], i);
+  __builtin_amdgcn_sched_barrier(0);
+  // each group's largest magnitude, two values at a time in 16-bit integers (bf16 magnitudes
+  // are ordered as such), then as a float; one at a time where there is a NaN, which sorts
+  // above infinity there and must not count
+  auto lo = [&](int p, int w) { return __uint_as_float(static_cast<uint32_t>(raw[p][w]) << 16); };
+  auto hi = [&](int p, int w) { return __uint_as_float(raw[p][w] & 0xffff0000u); };
+  float f[P];
+  bool nan = false;
+#pragma unroll
+  for (int p = 0; p < P; ++p) {
+    uint32_t top = 0;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) top = max2(top, raw[p][w] & 0x7fff7fffu);
+    f[p] = __uint_as_float(max(top & 0xffffu, top >> 16) << 16);
+    nan |= f[p] != f[p];
+  }
+  if (__builtin_expect(__any(nan), 0)) {
+#pragma unroll
+    for (int p = 0; p < P; ++p) {
+      f[p] = 0.0f;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) f[p] = fmaxf(f[p], fmaxf(fabsf(lo(p, w)), fabsf(hi(p, w))));
+    }
+  }
+  uint8_t* my_rows = rows + wave * S * 2048;
+  float* my_scales = scales + wave * S * 16;
+#pragma unroll
+  for (int p = 0; p < P; ++p) {
+    float m = f[p];  // over the 16 lanes
+    m = fmaxf(m, row_ror<8>(m));
+    m = fmaxf(m, row_ror<4>(m));
+    m = fmaxf(m, row_ror<2>(m));
+    m = fmaxf(m, row_ror<1>(m));
+    const float s = gdn::fp8_scale(m), inv = 1.0f / s;
+    const int r = row_of(p), i = step_of(p);
+    *reinterpret_cast<uint2*>(my_rows + i * 2048 + sw_off(r, l >> 1) + 8 * (l & 1)) =
+        make_uint2(gdn::f2fp8x4(lo(p, 0) * inv, hi(p, 0) * inv, lo(p, 1) * inv, hi(p, 1) * inv),
+                   gdn::f2fp8x4(lo(p, 2) * inv, hi(p, 2) * inv, lo(p, 3) * inv, hi(p, 3) * inv));
+    if (l == 0) my_scales[i * 16 + r] = s;
+  }
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront", "local");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront", "local");
+  gdn::f32x4_t acc[1][NT][2];
+#pragma unroll
+  for (int j = 0; j < NT; ++j)
+#pragma unroll
+    for (int t = 0; t < 2; ++t) acc[0][j][t] = gdn::f32x4_t{0.f, 0.f, 0.f, 0.f};
+  auto step = [&](auto at) {
+    constexpr int i = decltype(at)::value;
+    // stages behind stage i that have been asked for
+    constexpr int behind = (i + NS <= S ? NS : S - i) - 1, vm = behind * kPer;
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_waitcnt((vm & 15) | (7 << 4) | (15 << 8) | ((vm >> 4) << 14));
+    __builtin_amdgcn_sched_barrier(0);
+    const uint8_t* b = st[i % NS] + wave * kStage;
+    Frag8 fa, fb[NT][2];
+    fa.lo = *reinterpret_cast<const i32x4_t*>(my_rows + i * 2048 + sw_off(lr, lg));
+    fa.hi = *reinterpret_cast<const i32x4_t*>(my_rows + i * 2048 + sw_off(lr, 4 + lg));
 #pragma unroll
     for (int j = 0; j < NT; ++j)
 #pragma unroll
-      for (int t = 0; t < 2; ++t) red[(((wave * MT + i) * NT + j) * 2 + t) * 64 + lane] = acc[i][j][t];
-  __syncthreads();
-  for (int ij = wave; ij < MT * NT; ij += NW) {
-    gdn::f32x4_t c0 = red[(ij * 2) * 64 + lane], c1 = red[(ij * 2 + 1) * 64 + lane];
-#pragma unroll
-    for (int w = 1; w < NW; ++w) {
-      c0 += red[((w * MT * NT + ij) * 2) * 64 + lane];
-      c1 += red[((w * MT * NT + ij) * 2 + 1) * 64 + lane];
+      for (int t = 0; t < 2; ++t) {
+        const int r = 8 * (lr >> 2) + 4 * t + (lr & 3);
+        fb[j][t].lo = *reinterpret_cast<const i32x4_t*>(b + 4096 * j + swb_off(r, lg));
+        fb[j][t].hi = *reinterpret_cast<const i32x4_t*>(b + 4096 * j + swb_off(r, 4 + lg));
+      }
+    const float sb = *reinterpret_cast<const float*>(b + kBBytes);
+    if constexpr (i + NS < S) {
+      // the reads have returned before the stage is loaded again
+      __builtin_amdgcn_sched_barrier(0);
+      __builtin_amdgcn_s_waitcnt(kWaitLds);
+      __builtin_amdgcn_sched_barrier(0);
+      issue(st[i % NS], i + NS);
     }
-    gemm_store16(c0, c1, out, M, N, m0 + 16 * (ij / NT), n0 + 32 * (ij % NT), lane, GemmGates{}, nullptr);
-  }
+    if (wave + NW * i < nk) {
+      const float s = my_scales[i * 16 + lr] * sb;
+#pragma unroll
+      for (int j = 0; j < NT; ++j)
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          const gdn::f32x4_t r = mfma_fp8(fb[j][t], fa);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[0][j][t][e] = fmaf(r[e], s, acc[0][j][t][e]);
+        }
+    }
+  };
+  each(step, std::make_integer_sequence<int, S>{});
+  __syncthreads();
+  ring_store<1, NT, NW>(acc, reinterpret_cast<gdn::f32x4_t*>(st0), out, M, N, m0, n0);
 }
 
 // ---- 64-row tiles with a deeper load pipeline ----
@@ -829,11 +1017,14 @@ __global__ __launch_bounds__(kFp8Threads, 2) void gemm_fp8_deep_kernel(const uin
   __builtin_amdgcn_s_waitcnt(0);  // the repeated loads past the last step
 }
 
-// The kernels (fp8_plan says which is taken); the last two take bf16 rows.  Those and the
-// two that take the same calls' e4m3 rows deal K to as many waves, so that a call from
+// The kernels (fp8_plan says which is taken); the last four take bf16 rows.  Those and
+// the two that take the same calls' e4m3 rows deal K to as many waves, so that a call from
 // bf16 rows has the bits of gdn_quantize_fp8 and a call from e4m3 ones.  (Four waves of
 // three stages for kRing16x32: 1 x 2048 3.6 us against 3.8, 64 x 2048 x 4096 4.8 / 5.1.)
-enum Fp8Kernel { kPP, kDeep64, kDeep128, kRing16x32, kRing16x64, kRing32x32, kRing64x32, kRingQ16x32, kRingQ16x64 };
+enum Fp8Kernel {
+  kPP, kDeep64, kDeep128, kRing16x32, kRing16x64, kRing32x32, kRing64x32,
+  kRingQ16x32, kRingQ16x64, kRows16x32, kRows16x64
+};
 
 // Times: one launch replayed from a graph, operands in the caches, K = 2048 unless
 // said.
@@ -847,13 +1038,15 @@ Fp8Kernel fp8_plan(int M, int N, int K, bool quant) {
   // 64 tiles 6.9), 1 x 16384 5.2 (5.6, 7.3); past one workgroup per CU 1 x 32768 14.3,
   // 64 x 64 tiles 12.4.
   if (quant && K <= 4096) {
-    // A bf16 A's own launch takes 2.0 to 2.4 us; in the ring it takes 0.5 per K-step of a
-    // wave (2048 columns: two of them for each of 8 waves): 1 x 2048 5.0 against 3.8 +
-    // 2.0, 64 x 2048 5.4 against 4.0 + 2.4, 37 x 2048 x 4096 6.8 against 4.6 + 2.3, 1 x
-    // 12288 6.3 against 4.8 + 2.1.  Longer rows take more, and so do row blocks past one
-    // workgroup per CU (64 x 8192 17.5 against 6.2 + 2.4).
-    if (blocks(16, 32) <= kCUs8) return kRingQ16x32;
-    if (M <= 16 && blocks(16, 64) <= kCUs8) return kRingQ16x64;
+    // A bf16 A's own launch takes 2.0 to 2.8 us; in the ring it takes 0.5 per K-step of a
+    // wave (2048 columns: two of them for each of 8 waves): 64 x 2048 5.9 against 7.0 in
+    // two launches, 37 x 2048 x 4096 7.4 against 7.8, 16 x 12288 6.9 against 7.7.  Longer
+    // rows take more, and so do row blocks past one workgroup per CU (64 x 8192 17.5
+    // against 8.6).
+    // Up to 8 rows quantize ahead, in at most 8 passes per wave (see there; with 16: 8 x 12288
+    // x 4096 12.3 against 11.7).
+    if (blocks(16, 32) <= kCUs8) return M <= 8 ? kRows16x32 : kRingQ16x32;
+    if (M <= 16 && blocks(16, 64) <= kCUs8) return M <= 4 || (M <= 8 && K <= 2048) ? kRows16x64 : kRingQ16x64;
   }
   if (blocks(16, 32) <= kCUs8) return kRing16x32;
   if (M <= 16 && blocks(16, 64) <= kCUs8) return kRing16x64;
@@ -883,6 +1076,8 @@ int fp8_launch(Fp8Kernel kernel, const void* A, int64_t lda, const uint8_t* B, i
     return dim3(static_cast<unsigned>(gdn::kNumXcd * ((wgs + gdn::kNumXcd - 1) / gdn::kNumXcd)));
   };
   const uint8_t* A8 = static_cast<const uint8_t*>(A);
+  const uint16_t* A16 = static_cast<const uint16_t*>(A);
+  auto rows_grid = [&](int bn) { return grid(blocks(16, bn) + blocks(16, 1 << 30) * (wide.n / 16)); };
   switch (kernel) {
     case kPP: {
       // whole 256 x 256 tiles for full rounds of the CUs, the rest (up to half a round)
@@ -902,11 +1097,10 @@ int fp8_launch(Fp8Kernel kernel, const void* A, int64_t lda, const uint8_t* B, i
       gemm_fp8_deep_kernel<128, 3><<<grid(blocks(64, 128)), dim3(kFp8Threads), 0, st>>>(A8, lda, B, ldb, sc, out, M,
                                                                                        N, K);
       break;
-#define GDN_RING(name, BM, BN, NW, NS, Q)                                                                       \
-  case name:                                                                                                    \
-    gemm_fp8_ring_kernel<BM, BN, NW, NS, Q>                                                                     \
-        <<<grid(blocks(BM, BN) + (Q ? blocks(16, 16 * N) * (wide.n / 16) : 0)), dim3(64 * NW), 0, st>>>(        \
-            A, lda, B, ldb, sc, out, M, N, K, wide);                                                            \
+#define GDN_RING(name, BM, BN, NW, NS, Q)                                                                            \
+  case name:                                                                                                         \
+    gemm_fp8_ring_kernel<BM, BN, NW, NS, Q>                                                                          \
+        <<<Q ? rows_grid(BN) : grid(blocks(BM, BN)), dim3(64 * NW), 0, st>>>(A, lda, B, ldb, sc, out, M, N, K, wide); \
     break
       GDN_RING(kRing16x32, 16, 32, 8, 2, false);
       GDN_RING(kRing16x64, 16, 64, 4, 3, false);
@@ -915,6 +1109,22 @@ int fp8_launch(Fp8Kernel kernel, const void* A, int64_t lda, const uint8_t* B, i
       GDN_RING(kRingQ16x32, 16, 32, 8, 2, true);
       GDN_RING(kRingQ16x64, 16, 64, 4, 2, true);
 #undef GDN_RING
+#define GDN_ROWS(BN, NW, NS, S, R)                                                                                  \
+  gemm_fp8_rows_kernel<BN, NW, NS, S, R><<<rows_grid(BN), dim3(64 * NW), 0, st>>>(A16, lda, B, ldb, sc, out, M, N, K, \
+                                                                                  wide)
+    case kRows16x32:
+      if (K <= 2048)
+        M <= 4 ? GDN_ROWS(32, 8, 2, 2, 4) : GDN_ROWS(32, 8, 2, 2, 8);
+      else
+        M <= 4 ? GDN_ROWS(32, 8, 2, 4, 4) : GDN_ROWS(32, 8, 2, 4, 8);
+      break;
+    case kRows16x64:
+      if (K <= 2048)
+        M <= 4 ? GDN_ROWS(64, 4, 3, 4, 4) : GDN_ROWS(64, 4, 3, 4, 8);
+      else
+        GDN_ROWS(64, 4, 2, 8, 4);
+      break;
+#undef GDN_ROWS
   }
   return gdn_launch_status();
 }

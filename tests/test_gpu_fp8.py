@@ -282,3 +282,37 @@ def test_other_stream_and_one_scale_for_all(pkg, dev):
         got = run()
     side.synchronize()
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("M", [1, 2, 4, 5, 8, 9, 16])
+@pytest.mark.parametrize("N,K", [(40, 128), (256, 896), (2048, 2048), (512, 2176), (1024, 4096), (64, 4224), (12288, 2048),
+                                 (8200, 640), (8320, 4096), (8320, 2304)])
+def test_linear_fp8_few_rows(pkg, dev, M, N, K):
+    """Few bf16 rows, also strided, with a NaN, an infinity and a row of zeros among them: the
+    bits of quantize_fp8 and a call with its result; rows past M are not there; bf16 columns."""
+    gen = torch.Generator().manual_seed(M + N + K)
+    big = _rows(gen, M + 1, K + 8).to(BF16)
+    w8, ws = (t.to(dev) for t in ref.to_e4m3(_rows(gen, N, K) * K ** -0.5, 128))
+    for bad in (False, True):
+        if bad:
+            big[0, 8 + K - 3] = float("nan")
+            big[M // 2, 9] = float("-inf")
+            big[M - 1] = 0
+        x = big.to(dev)[:M, 8:]
+        x8, xs = pkg.quantize_fp8(x)
+        want = pkg.linear_fp8(x8, w8, ws, x_scale=xs)
+        out = torch.full((M + 1, N + 3), 7.0, dtype=BF16, device=dev)
+        pkg.linear_fp8(x, w8, ws, out=out[:M, :N])
+        wide = torch.randn(32, K, generator=gen).to(BF16).to(dev)
+        parts = pkg.ops.linear_fp8_cols(x, w8, ws, [N, 16, 16], wide=wide) if N % 16 == 0 else None
+        torch.cuda.synchronize()
+        rows = [r for r in range(M) if not bad or r not in (0, M // 2)] + ([M - 1] if bad else [])
+        assert torch.equal(out[rows, :N], want[rows]) and bool(want[rows].isfinite().all())
+        if bad and M > 2:
+            assert bool(out[[0, M // 2], :N].isnan().all())
+        assert bool((out[M:] == 7).all()) and bool((out[:, N:] == 7).all())
+        if parts is not None:
+            assert torch.equal(parts[0][rows], want[rows])
+            a, b = x[rows].double(), wide.double()
+            slack = (a.abs() @ b.abs().t()) * (K + K // 64) * ref.U32
+            _check(torch.cat(parts[1:], 1)[rows], a @ b.t(), slack, "bf16 columns")
