@@ -484,6 +484,20 @@ int gdn_rmsnorm_gated_fp8(const uint16_t* x, int64_t sx_tok, const uint16_t* z, 
                           float eps, void* stream);
 
 /*
+ * The decode step of gdn_recurrent_decode_fused (with q and k) or gdn_decode_step (q and k
+ * NULL; Hv == Hk or 2 * Hk) with its gated norm written as gdn_rmsnorm_gated_fp8 writes it, for
+ * an 8-bit out projection: head dim 128, z required, y8 [B, Hv, D] e4m3 contiguous, the scale
+ * of row b, head h at y8_scale[h * ss + b] (ss >= B).  The other arguments are those entry
+ * points'; q and k NULL takes gdn_decode_step's rows.
+ */
+int gdn_decode_fp8(const uint16_t* q, int64_t sq_b, const uint16_t* k, int64_t sk_b, const uint16_t* x, int64_t sx_row,
+                   uint16_t* conv_pool, int64_t cp_slot, int64_t cp_ch, const uint16_t* conv_w, const uint16_t* a,
+                   const uint16_t* b, const void* A_log, const void* dt_bias, int param_is_fp32, float* s_pool,
+                   int64_t s_stride, const int64_t* ids, uint8_t* y8, float* y8_scale, int64_t ss, int B, int Hk,
+                   int Hv, int D, float scale, int l2norm, const uint16_t* z, int64_t sz_b, const uint16_t* norm_w,
+                   float eps, void* stream);
+
+/*
  * Speculative verify over a tree of drafted tokens (no counterpart in the reference:
  * spec decode is disabled for qwen3_5, nanovllm/config.py:84).  Four entry points:
  * the conv and the gated delta rule of T nodes (1 to 64) per sequence against the

@@ -73,6 +73,8 @@ SIGNATURES: dict[str, list] = {
                      _p, _p, _i64, _p],
     "gdn_gemm_fp8_workspace_size": [_i32, _i32, _i32, _i32],
     "gdn_rmsnorm_gated_fp8": [_p, _i64, _p, _i64, _p, _p, _p, _i64, _i64, _i64, _i32, _i32, _f32, _p],
+    "gdn_decode_fp8": [_p, _i64, _p, _i64, _p, _i64, _p, _i64, _i64, _p, _p, _p, _p, _p, _i32, _p, _i64, _p, _p, _p, _i64,
+                       _i32, _i32, _i32, _i32, _f32, _i32, _p, _i64, _p, _f32, _p],
     "gdn_conv_tree": [_p, _i64, _i64, _p, _i64, _i64, _i64, _p, _p, _p, _i64, _p, _i64, _i64, _p, _i64, _p, _i32, _p,
                       _i32, _i32, _i32, _p],
     "gdn_rule_tree": [_p, _i64, _i64, _p, _i64, _i64, _p, _i64, _i64, _p, _p, _p, _i64, _i64, _p, _p, _i64, _p, _i64,

@@ -95,7 +95,30 @@ struct NormIn {
   int64_t sz;
   const uint16_t* w;  // [D]
   float eps;
+  // instead of o (kFp8 instances, D = 128): [B, Hv, D] e4m3 with a scale per row, as
+  // gdn_rmsnorm_gated_fp8 writes it; that of row b, head h at scale[h * ss + b]
+  uint8_t* y8;
+  float* scale;
+  int64_t ss;
 };
+
+// 4 of a head's 128 columns per lane, 32 neighbouring lanes: the norm's row (r as norm_gate)
+// in e4m3 with its scale.
+__device__ __forceinline__ void norm_store_fp8(const NormIn& nin, const float (&x)[4], float r, const uint16_t* ws,
+                                               const uint16_t* zs, int64_t b, int h, int Hv, int c4) {
+  float v[4], top = 0.0f;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    v[i] = x[i] * r * gdn::bf2f(ws[i]) * gdn::silu_ulp(gdn::bf2f(zs[i]));
+    top = fmaxf(top, fabsf(v[i]));
+  }
+#pragma unroll
+  for (int m = 16; m >= 1; m >>= 1) top = fmaxf(top, __shfl_xor(top, m, 64));
+  const float s = gdn::fp8_scale(top), inv = 1.0f / s;
+  *reinterpret_cast<uint32_t*>(nin.y8 + (b * Hv + h) * gdn::kFp8Group + 4 * c4) =
+      gdn::f2fp8x4(v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv);
+  if (c4 == 0) nin.scale[h * nin.ss + b] = s;
+}
 
 // Initial states of a speculative-verify step taken from the previous step's
 // per-token states (deferred commit): row b starts from src[b, acc[b] - 1]
@@ -106,7 +129,7 @@ struct SrcIn {
   int T_src;
 };
 
-template <int D, int NVB, int NW, bool kFused, int kPolicy>
+template <int D, int NVB, int NW, bool kFused, int kPolicy, bool kFp8 = false>
 __global__ __launch_bounds__(64 * NW) void recurrent_kernel(
     const uint16_t* __restrict__ q, int64_t sq_b, int64_t sq_t, const uint16_t* __restrict__ k,
     int64_t sk_b, int64_t sk_t, const uint16_t* __restrict__ v, int64_t sv_b, int64_t sv_t,
@@ -396,6 +419,10 @@ __global__ __launch_bounds__(64 * NW) void recurrent_kernel(
         const float r = rsqrtf(ss / static_cast<float>(D) + nin.eps);
         const uint16_t* zs = reinterpret_cast<const uint16_t*>(&n_z);
         const uint16_t* ws = reinterpret_cast<const uint16_t*>(&n_w);
+        if constexpr (kFp8) {
+          norm_store_fp8(nin, x, r, ws, zs, b, h, Hv, c4);
+          continue;
+        }
         u.x = gdn::f2bf2(gdn::norm_gate(x[0], r, gdn::bf2f(ws[0]), gdn::bf2f(zs[0])),
                          gdn::norm_gate(x[1], r, gdn::bf2f(ws[1]), gdn::bf2f(zs[1])));
         u.y = gdn::f2bf2(gdn::norm_gate(x[2], r, gdn::bf2f(ws[2]), gdn::bf2f(zs[2])),
@@ -433,7 +460,7 @@ struct StepIn {
   int param_f32;
 };
 
-template <int D, int kR>
+template <int D, int kR, bool kFp8 = false>
 __global__ __launch_bounds__(4 * D, 4) void decode_step_kernel(StepIn in, NormIn nin, float* s_pool,
                                                                int64_t s_stride, const int64_t* __restrict__ ids,
                                                                uint16_t* __restrict__ o, int B, int Hk, float scale,
@@ -635,6 +662,10 @@ __global__ __launch_bounds__(4 * D, 4) void decode_step_kernel(StepIn in, NormIn
       const float rs = rsqrtf(ss / static_cast<float>(D) + nin.eps);
       const uint16_t* zs = reinterpret_cast<const uint16_t*>(&n_z);
       const uint16_t* ws = reinterpret_cast<const uint16_t*>(&n_w);
+      if constexpr (kFp8) {
+        norm_store_fp8(nin, x, rs, ws, zs, b, h0 + r0, Hv, c4);
+        return;
+      }
       u.x = gdn::f2bf2(gdn::norm_gate(x[0], rs, gdn::bf2f(ws[0]), gdn::bf2f(zs[0])),
                        gdn::norm_gate(x[1], rs, gdn::bf2f(ws[1]), gdn::bf2f(zs[1])));
       u.y = gdn::f2bf2(gdn::norm_gate(x[2], rs, gdn::bf2f(ws[2]), gdn::bf2f(zs[2])),
@@ -698,6 +729,14 @@ int launch_recurrent(const uint16_t* q, int64_t sq_b, int64_t sq_t, const uint16
   const int64_t work = static_cast<int64_t>(B) * Hv * NVB;
   const int64_t grid = gdn::kNumXcd * ((work + gdn::kNumXcd - 1) / gdn::kNumXcd);
   if constexpr (kPolicy == kLoadNT) {  // (the fused step is one token)
+    if constexpr (D == gdn::kFp8Group && NVB == 1) {
+      if (nin.y8) {
+        recurrent_kernel<D, NVB, NW, true, kPolicy, true><<<dim3(static_cast<unsigned>(grid)), dim3(64 * NW), 0, stream>>>(
+            q, sq_b, sq_t, k, sk_b, sk_t, v, sv_b, sv_t, g, beta, s_in, s_in_stride, s_out, s_out_stride,
+            ids, inter, o, B, T, Hk, Hv, scale, l2norm, din, nin, src);
+        return gdn_launch_status();
+      }
+    }
     if (din.xv) {
       recurrent_kernel<D, NVB, NW, true, kPolicy><<<dim3(static_cast<unsigned>(grid)), dim3(64 * NW), 0, stream>>>(
           q, sq_b, sq_t, k, sk_b, sk_t, v, sv_b, sv_t, g, beta, s_in, s_in_stride, s_out, s_out_stride,
@@ -833,7 +872,13 @@ int launch_decode_step(const StepIn& in, const NormIn& nin, float* s_pool, int64
   const dim3 grid(static_cast<unsigned>(gdn::kNumXcd * ((work + gdn::kNumXcd - 1) / gdn::kNumXcd)));
 #define GDN_STEP(D_, R_) \
   decode_step_kernel<D_, R_><<<grid, dim3(4 * D_), 0, stream>>>(in, nin, s_pool, s_stride, ids, o, B, Hk, scale, l2norm)
-  if (D == 128 && Hv == Hk) GDN_STEP(128, 1);
+  if (nin.y8 && Hv == Hk)
+    decode_step_kernel<128, 1, true><<<grid, dim3(512), 0, stream>>>(in, nin, s_pool, s_stride, ids, o, B, Hk, scale,
+                                                                     l2norm);
+  else if (nin.y8)
+    decode_step_kernel<128, 2, true><<<grid, dim3(512), 0, stream>>>(in, nin, s_pool, s_stride, ids, o, B, Hk, scale,
+                                                                     l2norm);
+  else if (D == 128 && Hv == Hk) GDN_STEP(128, 1);
   else if (D == 128) GDN_STEP(128, 2);
   else if (Hv == Hk) GDN_STEP(64, 1);
   else GDN_STEP(64, 2);
@@ -895,6 +940,38 @@ extern "C" int gdn_recurrent_decode_fused(const uint16_t* q, int64_t sq_b, const
   // the norm, and the q/k conv, need a head's D columns in one workgroup
   return launch_one_token(D, z || qk_fused ? 1 : recurrent_nvb(B, Hv, 1), GDN_REC_ARGS);
 #undef GDN_REC_ARGS
+}
+
+extern "C" int gdn_decode_fp8(const uint16_t* q, int64_t sq_b, const uint16_t* k, int64_t sk_b, const uint16_t* x,
+                              int64_t sx_row, uint16_t* conv_pool, int64_t cp_slot, int64_t cp_ch,
+                              const uint16_t* conv_w, const uint16_t* a, const uint16_t* b, const void* A_log,
+                              const void* dt_bias, int param_is_fp32, float* s_pool, int64_t s_stride,
+                              const int64_t* ids, uint8_t* y8, float* y8_scale, int64_t ss, int B, int Hk, int Hv,
+                              int D, float scale, int l2norm, const uint16_t* z, int64_t sz_b, const uint16_t* norm_w,
+                              float eps, void* stream) {
+  if (D != gdn::kFp8Group) return GDN_ERR_UNSUPPORTED;  // a head per scale
+  if (B < 0 || Hk <= 0 || Hv <= 0 || Hv % Hk || ss < B) return GDN_ERR_INVALID_ARG;
+  if (B == 0) return GDN_OK;
+  const bool whole = !q && !k;
+  if ((!q || !k) && !(whole && (Hv == Hk || Hv == 2 * Hk))) return GDN_ERR_INVALID_ARG;
+  if (!z || !y8_scale) return GDN_ERR_INVALID_ARG;
+  const int st = decode_check(x, sx_row, conv_pool, cp_slot, cp_ch, conv_w, a, b, A_log, dt_bias, s_pool, s_stride,
+                              ids, reinterpret_cast<uint16_t*>(y8), Hk, Hv, D, z, sz_b, norm_w);
+  if (st != GDN_OK) return st;
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  const NormIn nin{z, sz_b, norm_w, eps, y8, y8_scale, ss};
+  // the kernels that the bf16 entry points take, by their rules
+  if (whole && (Hv != Hk || static_cast<int64_t>(B) * Hv < kStepTiles)) {
+    if (sx_row % 8 || reinterpret_cast<uintptr_t>(x) % 16) return GDN_ERR_INVALID_ARG;
+    const StepIn in{x, sx_row, conv_pool, cp_slot, cp_ch, conv_w, a, b, A_log, dt_bias, param_is_fp32 ? 1 : 0};
+    return launch_decode_step(in, nin, s_pool, s_stride, ids, nullptr, B, Hk, Hv, D, scale, l2norm, s);
+  }
+  const int64_t vbase = 2LL * Hk * D;
+  const DecodeIn din{x + vbase, sx_row, conv_pool + vbase * cp_ch, cp_slot, cp_ch, conv_w + vbase * 4, a, b,
+                     A_log, dt_bias, param_is_fp32 ? 1 : 0, whole ? x : nullptr, conv_pool, conv_w, Hk * D};
+  return launch_recurrent<gdn::kFp8Group, 1, 8, kLoadNT>(q, sq_b, 0, k, sk_b, 0, nullptr, 0, 0, nullptr, nullptr, s_pool,
+                                                         s_stride, s_pool, s_stride, ids, nullptr, nullptr, B, 1, Hk,
+                                                         Hv, scale, l2norm, din, nin, SrcIn{}, s);
 }
 
 static int state_tile_pass(const float* src, float* dst, int64_t slot_stride, const int64_t* ids, int B, int Hv,

@@ -227,10 +227,11 @@ class GatedDeltaNetCore:
             return ops.rms_norm_gated_fp8(core, z, self.norm_w, self.eps)
 
     # --------------------------------------------------------------- decode --
-    def decode(self, mixed, z, b, a, ids, conv_cache, s_cache, gb=None, out=None):
+    def decode(self, mixed, z, b, a, ids, conv_cache, s_cache, gb=None, out=None, fp8=False):
         """One token per row (the T == 1 branch of _gdn_padded, qwen3_5.py:1008-1030).
         mixed [B, C], z [B, Hv*D], b/a [B, Hv]; pools are per-layer views.
-        Returns core [B, Hv, D] bf16 (in `out` where given)."""
+        Returns core [B, Hv, D] bf16 (in `out` where given); with fp8 (D == 128, no `out`)
+        its (e4m3 [B, 1, Hv, D], scales) where the fused decode kernels run."""
         self._to(mixed.device)
         B = mixed.shape[0]
         Hk, Hv, D = self.Hk, self.Hv, self.D
@@ -242,8 +243,9 @@ class GatedDeltaNetCore:
                 with self._timed("recurrent_decode"):
                     out = ops.recurrent_decode_fused(None, mixed, conv_cache, self.conv_w, b, a, self.A_log,
                                                      self.dt_bias, s_cache, ids, Hk, Hv, D, z=z,
-                                                     norm_weight=self.norm_w, eps=self.eps, grouped=True, out=out)
-                return out.view(B, Hv, D)
+                                                     norm_weight=self.norm_w, eps=self.eps, grouped=True, out=out,
+                                                     fp8=fp8)
+                return out if fp8 else out.view(B, Hv, D)
             # q/k conv, then gates + v conv + recurrent update + gated norm in
             # one kernel (the same results as the calls below)
             with self._timed("conv_decode"):
@@ -251,8 +253,8 @@ class GatedDeltaNetCore:
             with self._timed("recurrent_decode"):
                 out = ops.recurrent_decode_fused(qk, mixed, conv_cache, self.conv_w, b, a, self.A_log, self.dt_bias,
                                                  s_cache, ids, Hk, Hv, D, z=z, norm_weight=self.norm_w, eps=self.eps,
-                                                 out=out)
-            return out.view(B, Hv, D)
+                                                 out=out, fp8=fp8)
+            return out if fp8 else out.view(B, Hv, D)
         g, beta = self._g_beta(b.contiguous(), a.contiguous(), None, gb)
         if self.sw.conv_kernel:
             with self._timed("conv_decode"):
@@ -476,13 +478,14 @@ class GatedDeltaNetCore:
         mixed [N, C], z [N, Hv*D], b/a [N, Hv]; gb: optional (g [N, Hv] fp32,
         beta [N, Hv] bf16) already computed from b, a (used by the paths that
         would run the gate kernel).  Returns [N, Hv*D] bf16; with fp8, a step of
-        prompts alone returns (e4m3 [N, Hv, D], scales) instead where its norm is a
-        launch of its own (ops.rms_norm_gated_fp8)."""
+        prompts alone or of decode rows alone returns its (e4m3 [N, Hv, D] or [N, 1, Hv, D],
+        scales) instead where its kernels write that (ops.rms_norm_gated_fp8)."""
         rows = (lambda i, j: None) if gb is None else (lambda i, j: (gb[0][i:j], gb[1][i:j]))
         N = mixed.shape[0]
         T = int(max_seqlen_q)
         if T == 1:
-            return self.decode(mixed, z, b, a, ids, conv_cache, s_cache, gb=gb).view(N, self.value_dim)
+            core = self.decode(mixed, z, b, a, ids, conv_cache, s_cache, gb=gb, fp8=fp8 and self.D == ops.FP8_GROUP)
+            return core if isinstance(core, tuple) else core.view(N, self.value_dim)
         # per-sequence lengths on the device, formed only where a path reads
         # them (a decode step or a varlen prefill given lens_q launches nothing
         # for them)

@@ -651,7 +651,7 @@ def one_launch_decode(B: int, num_k_heads: int, num_v_heads: int) -> bool:
 
 def recurrent_decode_fused(qk, mixed, conv_pool, conv_weight, b, a, a_log, dt_bias, s_pool, ids, Hk, Hv, D,
                            scale=None, z=None, norm_weight=None, eps=1e-6, fuse_norm=None, grouped=False,
-                           out=None):
+                           out=None, fp8=False):
     """The decode step after the q/k conv, in one kernel: the gates from a, b,
     the v channels' conv1d + SiLU (their conv state rolled in place at `ids`)
     and the in-place recurrent update.  qk [B, 2*Hk*D] is conv_decode_step's
@@ -668,7 +668,10 @@ def recurrent_decode_fused(qk, mixed, conv_pool, conv_weight, b, a, a_log, dt_bi
     decode conv runs in the kernel as well, their conv states rolled there
     (the whole step in one launch); the same bits as conv_decode_step on
     those channels followed by the call above with its output.  out: a
-    contiguous bf16 tensor of B * Hv * D elements that takes the result."""
+    contiguous bf16 tensor of B * Hv * D elements that takes the result.
+
+    fp8 (with z, D == 128): the norm in e4m3 for an 8-bit out projection, the bits of
+    rms_norm_gated_fp8 on the core output.  Returns (e4m3 [B, 1, Hv, D], scales [B, Hv])."""
     dev = _check_cuda(qk, mixed, conv_pool, conv_weight, b, a, a_log, dt_bias, s_pool, ids, z, norm_weight)
     for t, nm in ((qk, "qk"), (mixed, "mixed"), (conv_pool, "conv_pool"), (b, "b"), (a, "a")):
         if t is not None:
@@ -694,6 +697,8 @@ def recurrent_decode_fused(qk, mixed, conv_pool, conv_weight, b, a, a_log, dt_bi
     assert _state_view_ok(s_pool, Hv, D)
     ids64 = ids.to(torch.int64).contiguous()
     assert ids64.shape == (B,), "one slot id per row"
+    if fp8 and (z is None or D != FP8_GROUP or out is not None or (fuse_norm is not None and not fuse_norm)):
+        raise ValueError(f"fp8 outputs need z, a head dim of {FP8_GROUP} and the norm in the kernel, and take no out")
     if z is not None and fuse_norm is not None and not fuse_norm:
         core = recurrent_decode_fused(qk, mixed, conv_pool, conv_weight, b, a, a_log, dt_bias, s_pool, ids, Hk, Hv,
                                       D, scale)
@@ -709,12 +714,27 @@ def recurrent_decode_fused(qk, mixed, conv_pool, conv_weight, b, a, a_log, dt_bi
         sz = z.stride(0) if B > 1 else Hv * D
         assert norm_weight is not None and norm_weight.numel() == D
         nw = norm_weight.to(torch.bfloat16).contiguous()
+    if scale is None:
+        scale = D ** -0.5
+    if fp8:
+        y = torch.empty(B, 1, Hv, D, dtype=FP8, device=mixed.device)
+        y_scale = _fp8_scales(B, Hv, mixed.device)
+        if qk is not None:
+            q_k = (_lib.ptr(qk), qk.stride(0), _lib.ptr(qk[:, kd:]), qk.stride(0))
+        else:
+            q_k = (None, 0, None, 0)
+            if mixed.stride(0) % 8 or mixed.data_ptr() % 16:
+                mixed = mixed.contiguous() if mixed.data_ptr() % 16 == 0 else mixed.clone()
+        _lib.call("gdn_decode_fp8", *q_k, _lib.ptr(mixed), mixed.stride(0), _lib.ptr(conv_pool), conv_pool.stride(0),
+                  conv_pool.stride(1), _lib.ptr(w), _lib.ptr(a), _lib.ptr(b), _lib.ptr(a_log), _lib.ptr(dt_bias),
+                  int(a_log.dtype == torch.float32), _lib.ptr(s_pool), s_pool.stride(0), _lib.ptr(ids64), _lib.ptr(y),
+                  _lib.ptr(y_scale), B, B, Hk, Hv, D, float(scale), 1, _lib.ptr(z), sz, _lib.ptr(nw), float(eps),
+                  _stream(dev))
+        return y, y_scale
     if out is None:
         out = torch.empty(B, 1, Hv, D, dtype=mixed.dtype, device=mixed.device)
     else:
         out = _out(out, B * Hv * D, dev).view(B, 1, Hv, D)
-    if scale is None:
-        scale = D ** -0.5
     entry, q_k = "gdn_recurrent_decode_fused", (None, 0, None, 0)
     if qk is not None:
         q_k = (_lib.ptr(qk), qk.stride(0), _lib.ptr(qk[:, kd:]), qk.stride(0))

@@ -259,3 +259,27 @@ def test_calls_by_words(pkg):
         assert lib.gdn_call_words(pack(head, *args(0, 64, n % 4 + 1))) == inv
         assert lib.gdn_call_words(pack(head, *args(0, 64, 0))) == inv
         assert lib.gdn_call_words(pack(head, *args(2, 64, n))) == inv     # no operands
+
+
+def test_decode_step_to_e4m3_refuses(pkg, monkeypatch):
+    monkeypatch.setattr(pkg.ops, "_check_cuda", lambda *ts: torch.device("cpu"))
+    monkeypatch.setattr(pkg._lib, "call", lambda *a: (_ for _ in ()).throw(Launched()))
+    monkeypatch.setattr(pkg.ops, "_stream", lambda dev: 0)
+    B, Hk, Hv, D = 2, 1, 2, 128
+    C = 2 * Hk * D + Hv * D
+    n = lambda *s: torch.zeros(*s, dtype=BF16)  # noqa: E731
+    good = dict(qk=None, mixed=n(B, C), conv_pool=n(4, C, 3), conv_weight=n(C, 4), b=n(B, Hv), a=n(B, Hv), a_log=n(Hv),
+                dt_bias=n(Hv), s_pool=torch.zeros(4, Hv, D, D), ids=torch.arange(B), Hk=Hk, Hv=Hv, D=D, z=n(B, Hv * D),
+                norm_weight=n(D), grouped=True, fp8=True)
+    _refused(pkg.ops.recurrent_decode_fused, good, z=[None], out=[n(B, Hv * D)])
+    with pytest.raises(ValueError):
+        pkg.ops.recurrent_decode_fused(**dict(good, qk=n(B, 2 * Hk * D), fuse_norm=False))
+    lib, _lib = pkg._lib.load(), pkg._lib
+    P, odd = 1 << 20, (1 << 20) + 2
+    f = lambda q=None, k=None, x=P, y=P, s=P, ss=8, B=4, Hk=2, Hv=4, D=128, z=P, w=P, sx=1024: (  # noqa: E731
+        lib.gdn_decode_fp8(q, 1024, k, 1024, x, sx, P, 3 * 1024, 3, P, P, P, P, P, 0, P, Hv * D * D, P, y, s, ss, B, Hk,
+                           Hv, D, 1.0, 1, z, 512, w, 1e-6, None))
+    assert f(B=0) == _lib.GDN_OK and f(D=64) == _lib.GDN_ERR_UNSUPPORTED
+    for bad in (dict(q=P), dict(k=P), dict(Hk=1), dict(Hv=5), dict(x=None), dict(x=odd), dict(y=None), dict(y=odd),
+                dict(s=None), dict(ss=3), dict(z=None), dict(z=odd), dict(w=None), dict(sx=1020), dict(B=-1)):
+        assert f(**bad) == _lib.GDN_ERR_INVALID_ARG, bad
