@@ -61,11 +61,13 @@ struct Fp8Scales {
 // that read a step's scales loads those of the step two later, so that two sections
 // in a row issue 9 loads.  An odd step past the last one repeats it with B's scale 0.
 //
-// 16384 x 12288 x 2048 396 us (2.09 PFLOP/s; the library's product with one scale for each
-// operand 399), 8192^3 431 us (2.55 PFLOP/s; library 2.65), 17001 x 2048 x 2048 80 us.  Bound
-// by power: the clock falls to 1.6-2.0 GHz with the matrix cores busy 0.49 (K = 2048) to 0.64
-// (8192^3) of the cycles, no LDS conflicts; for 17001 x 2048 by 536 tiles in rounds of 256.
-// Not kept: row-block groups of 2, 8 and 16 (4 is 1-3 % faster), non-temporal stores (slower).
+// 16384 x 12288 x 2048 363 us (2.27 PFLOP/s; the library's product with one scale for each
+// operand 399), 8192^3 418 us (2.63 PFLOP/s; library 2.65), 17001 x 2048 x 2048 70 us.  Bound
+// by power (the clock falls to 1.6-2.0 GHz), no LDS conflicts; for 17001 x 2048 by 536 tiles
+// in rounds of 256.  The 16 spilled registers that a first form reloaded between tiles, each
+// behind a wait for every load and store in flight, cost 385, 432 and 79 us.  Not kept:
+// row-block groups of 2, 8 and 16 (4 is 1-3 % faster), non-temporal stores (slower), a tile's
+// first sections that do not wait for the stores of the tile before (no faster).
 constexpr int kPPThreads = 512;
 constexpr int kWaitPP8 = 9 | (7 << 4);    // s_waitcnt vmcnt(9) lgkmcnt(0)
 constexpr int kWaitQ8 = 10 | (7 << 4);    // s_waitcnt vmcnt(10) lgkmcnt(0)
@@ -114,20 +116,31 @@ __global__ __launch_bounds__(kPPThreads, 2) void gemm_fp8_pp_kernel(const uint8_
   };
   const __amdgpu_buffer_rsrc_t ra = rsrc_of(A), rb = rsrc_of(B), rs = rsrc_of(wave < 4 ? sc.a : sc.b);
   const int s_step = wave < 4 ? static_cast<int>(sc.a_grp) * 4 : 4;
-  const int ldrow = 8 * wave + (lane >> 3);
-  const int gcol_a = 16 * ((lane & 7) ^ (((wave & 1) << 2) | (lane >> 4)));
-  const int gcol_b = 16 * ((lane & 7) ^ (((wave & 3) << 1) | ((lane >> 4) & 1)));
+  // the lane's number found anew: nothing that only a new tile's offsets or an epilogue needs
+  // is kept in registers across the loop (a spilled one comes back behind a wait for every
+  // load and store in flight)
+  auto new_lane = []() {
+    int zero = 0;
+    asm volatile("" : "+v"(zero));
+    return static_cast<int>(__builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, zero)));
+  };
+  // (all byte offsets are below 2^31)
+  const int a_ld = static_cast<int>(lda), b_ld = static_cast<int>(ldb);
+  const int a_row = static_cast<int>(sc.a_row) * 4, b_row = static_cast<int>(sc.b_row) * 4;
   int va[2][2], vb[2][2], vs;
   auto set_offsets = [&](int m0, int n0) {
+    const int l = new_lane();
+    const int ldrow = 8 * wave + (l >> 3);
+    const int gcol_a = 16 * ((l & 7) ^ (((wave & 1) << 2) | (l >> 4)));
+    const int gcol_b = 16 * ((l & 7) ^ (((wave & 3) << 1) | ((l >> 4) & 1)));
 #pragma unroll
     for (int h = 0; h < 2; ++h)
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        va[h][i] = static_cast<int>(min(m0 + 128 * h + 64 * i + ldrow, M - 1) * lda + gcol_a);
-        vb[h][i] = static_cast<int>(min(n0 + 128 * h + 64 * i + ldrow, N - 1) * ldb + gcol_b);
+        va[h][i] = min(m0 + 128 * h + 64 * i + ldrow, M - 1) * a_ld + gcol_a;
+        vb[h][i] = min(n0 + 128 * h + 64 * i + ldrow, N - 1) * b_ld + gcol_b;
       }
-    vs = wave < 4 ? static_cast<int>(min(m0 + 64 * wave + lane, M - 1) * sc.a_row * 4)
-                  : static_cast<int>(min(n0 / 128 + (wave & 1), (N - 1) / 128) * sc.b_row * 4);
+    vs = wave < 4 ? min(m0 + 64 * wave + l, M - 1) * a_row : min(n0 / 128 + (wave & 1), (N - 1) / 128) * b_row;
   };
   auto dma = [&](const __amdgpu_buffer_rsrc_t& r, uint8_t* dst, const int (&v)[2], int kbyte) {
 #pragma unroll
@@ -275,10 +288,7 @@ __global__ __launch_bounds__(kPPThreads, 2) void gemm_fp8_pp_kernel(const uint8_
         prod(acc[1], fa, fbn, fb1, sa[1]);
       }
       if (!wm) half_barrier();
-      // (the lane from an opaque copy, so that no address of the epilogue is
-      // kept in registers across the loop)
-      int tid_e = static_cast<int>(threadIdx.x);
-      asm volatile("" : "+v"(tid_e));
+      const int lane_e = new_lane();
 #pragma unroll
       for (int a = 0; a < 2; ++a)
 #pragma unroll
@@ -286,7 +296,7 @@ __global__ __launch_bounds__(kPPThreads, 2) void gemm_fp8_pp_kernel(const uint8_
 #pragma unroll
           for (int b = 0; b < 2; ++b)
             gemm_store16(acc[a][b][i][0], acc[a][b][i][1], out, M, N, m0c + 128 * a + 64 * wm + 16 * i,
-                         n0c + 128 * b + 32 * wn, tid_e & 63, GemmGates{}, nullptr);
+                         n0c + 128 * b + 32 * wn, lane_e, GemmGates{}, nullptr);
       if (Ln >= xend) break;
       L = Ln;
     }
@@ -367,7 +377,7 @@ __global__ __launch_bounds__(kPPThreads, 2) void gemm_fp8_pp_kernel(const uint8_
     if (!wm) half_barrier();
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-      gemm_store16(c[i][0], c[i][1], out, M, N, m0 + 64 * wm + 16 * i, n0 + 32 * wn, lane, GemmGates{}, nullptr);
+      gemm_store16(c[i][0], c[i][1], out, M, N, m0 + 64 * wm + 16 * i, n0 + 32 * wn, new_lane(), GemmGates{}, nullptr);
   }
   __builtin_amdgcn_s_waitcnt(0);
 }
