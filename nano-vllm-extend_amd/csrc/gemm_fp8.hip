@@ -1066,9 +1066,9 @@ Fp8Kernel fp8_plan(int M, int N, int K, bool quant) {
   // blocks 13.1), 1024 x 2048 9.0 (10.3, 13.2), 128 x 12288 8.6 (10.3, 13.3); with three
   // 256 x 12288 14.5 (12.4, 14.3).
   if (blocks(64, 64) <= 2 * kCUs8) return kDeep64;
-  // Up to nearly four 64 x 128 tiles per CU: 400 x 12288 22.2 (pp 25.9), 700 x 8192 22.4
-  // (25.8), 900 x 8192 26.7 (28.7), 1500 x 2048 13.1 (13.9); then the large tiles: 1024 x
-  // 8192 28.2 against 28.2, 700 x 12288 34.1 against 32.7, 1024 x 12288 40.0 against 34.4.
+  // Up to nearly four 64 x 128 tiles per CU: 400 x 12288 21.2 (pp 24.7), 700 x 8192 21.3
+  // (24.6), 600 x 12288 26.1 (28.3), 1500 x 2048 13.1 (14.1), 900 x 8192 26.0 (25.4); then
+  // the large tiles: 700 x 12288 31.7 against 28.4.
   if (blocks(64, 128) <= 15 * kCUs8 / 4) return kDeep128;
   return kPP;
 }
