@@ -135,7 +135,8 @@ def test_linear_fp8_cols(pkg, dev, M):
 
 @pytest.mark.parametrize("M,N,K,N2", [(1, 12288, 2048, 64), (1, 2048, 128, 16), (5, 256, 384, 32), (37, 12288, 2048, 64),
                                       (37, 2048, 4096, 48), (200, 8192, 2048, 32), (1000, 512, 640, 64),
-                                      (1025, 1024, 512, 64), (3000, 2048, 2048, 64)])
+                                      (1025, 1024, 512, 64), (3000, 2048, 2048, 64), (3, 80, 256, 32), (16, 48, 384, 16),
+                                      (40, 144, 512, 16), (70, 8208, 256, 32), (1100, 2064, 640, 48)])
 def test_linear_fp8_with_bf16_columns(pkg, dev, M, N, K, N2):
     """The 8-bit columns are linear_fp8's; the bf16 ones within bf16's half step and fp32's
     error (K products and K / 128 partial sums, each a rounding) of the 64-bit product."""
