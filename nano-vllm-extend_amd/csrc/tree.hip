@@ -160,10 +160,14 @@ __device__ __forceinline__ bool dense_taps(const uint16_t* pool, int64_t sp_slot
 //
 // Bound by the rows' way in and out (2 + 2 bytes per value) and, with few waves, by each
 // node's own chain: 64 trees of 64 nodes, 8192 channels 35.3 us (4.1 TB/s), of 16 nodes 11.3,
-// one tree of 16 nodes 5.0, of 8 nodes 4.1.  Before: with a branch per node 49.7, 13.0, 6.8
-// and 5.1; four channels per thread in place of two 57.4, 14.2, 8.1, 5.9; 256 threads of 8
-// channels that share the nodes of a sequence 17.7 (64 x 16) and 5.5 (1 x 8).
-__global__ __launch_bounds__(64) void conv_tree_kernel(const uint16_t* __restrict__ x, int64_t x_b, int64_t x_t,
+// one tree of 64 nodes 5.5, of 16 nodes 4.1, of 8 nodes 3.9.  Before: with a branch per node
+// 49.7 (64 x 64), 13.0 (64 x 16), 6.8 (1 x 16) and 5.1 (1 x 8); four channels per thread in
+// place of two 57.4, 14.2, 8.1, 5.9.
+//
+// W: with few sequences W waves share a workgroup's channels and deal the groups of 4 nodes
+// among them.  Wave 0 has the taps; every row is in LDS before the first node is worked on.
+template <int W>
+__global__ __launch_bounds__(64 * W) void conv_tree_kernel(const uint16_t* __restrict__ x, int64_t x_b, int64_t x_t,
                                                        uint16_t* __restrict__ pool, int64_t sp_slot, int64_t sp_ch,
                                                        int64_t n_slots, const int64_t* __restrict__ ids,
                                                        const uint16_t* __restrict__ w,
@@ -172,7 +176,8 @@ __global__ __launch_bounds__(64) void conv_tree_kernel(const uint16_t* __restric
   // [3 + T up to whole groups][64], two channels per thread: the taps, oldest first, then the
   // nodes' rows, so that row r is at r + 3 (row_before)
   extern __shared__ uint32_t rows[];
-  const int b = blockIdx.y, lane = threadIdx.x;
+  const int b = blockIdx.y, lane = threadIdx.x % 64;
+  const int wave = W == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
   const int c = 2 * (blockIdx.x * 64 + lane);
   const bool in = c < C;
   // (x_t < 2^24, C < 2^23: the rows of 64 nodes and a few more have 32-bit offsets, also from
@@ -183,7 +188,7 @@ __global__ __launch_bounds__(64) void conv_tree_kernel(const uint16_t* __restric
   const uint32_t y_at = in ? 2 * c : 0x80000000u, x_at = 2 * c;
   const int64_t slot = ids[b];
   if (slot < 0 || slot >= n_slots) {  // (the whole workgroup)
-    for (int t = 0; t < T; ++t) __builtin_amdgcn_raw_buffer_store_b32(0u, by, y_at + t * y_row, 0, 0);
+    for (int t = wave; t < T; t += W) __builtin_amdgcn_raw_buffer_store_b32(0u, by, y_at + t * y_row, 0, 0);
     return;
   }
   // what the links need first, then weights and rows, then the taps and the pending rows
@@ -207,10 +212,13 @@ __global__ __launch_bounds__(64) void conv_tree_kernel(const uint16_t* __restric
       r.v[i] = __builtin_amdgcn_raw_buffer_load_b32(bx, x_at + static_cast<uint32_t>(t0 + i) * x_row, 0, 0);
     return r;
   };
-  Group next[2] = {load(0), load(kG)};
-  uint32_t tap[3];  // of both channels, oldest first
+  Group next[W == 1 ? 2 : kMaxNodes / kG / W];
+#pragma unroll
+  for (int i = 0; i < static_cast<int>(sizeof(next) / sizeof(Group)); ++i) next[i] = load(kG * (wave + W * i));
+  uint32_t tap[3] = {0u, 0u, 0u};  // of both channels, oldest first
   const bool dense = sp_ch == 3 && sp_slot % 2 == 0 && reinterpret_cast<uintptr_t>(pool) % 4 == 0;
-  if (dense) {
+  if (W > 1 && wave) {
+  } else if (dense) {
     const uint32_t u0 = pair(tp), u1 = pair(tp + 2), u2 = pair(tp + 4);
     tap[0] = (u0 & 0xffffu) | (u1 & 0xffff0000u);
     tap[1] = (u0 >> 16) | (u2 << 16);
@@ -222,7 +230,7 @@ __global__ __launch_bounds__(64) void conv_tree_kernel(const uint16_t* __restric
   gdn::keep_loads_here();
   tree_links(lane, T, link, pd.T, last_link);
   auto old = [&](int r) { return r == -1 ? tap[2] : r == -2 ? tap[1] : tap[0]; };
-  const int a = accepted_node(want, pd.T, last_link);
+  const int a = wave ? -1 : accepted_node(want, pd.T, last_link);
   if (a >= 0) {
     // the taps after the accepted node: its row, its parent's and its grandparent's
     const uint16_t* lx = pd.x + b * pd.x_b + (in ? c : 0);
@@ -241,8 +249,10 @@ __global__ __launch_bounds__(64) void conv_tree_kernel(const uint16_t* __restric
     w0[j] = __uint_as_float(j % 2 ? ww[j / 2] & 0xffff0000u : ww[j / 2] << 16);
     w1[j] = __uint_as_float(j % 2 ? ww[2 + j / 2] & 0xffff0000u : ww[2 + j / 2] << 16);
   }
+  if (W == 1 || wave == 0) {
 #pragma unroll
-  for (int j = 0; j < 3; ++j) rows[j * 64 + lane] = tap[j];
+    for (int j = 0; j < 3; ++j) rows[j * 64 + lane] = tap[j];
+  }
   // lane t: the places of node t's three predecessors, a byte each; negative: unused
   auto up = [&](int r) {
     const int p = __shfl(link, max(r, 0), 64);
@@ -252,12 +262,11 @@ __global__ __launch_bounds__(64) void conv_tree_kernel(const uint16_t* __restric
   const int places = link == kUnused ? -1 : (r2 + 3) | (r1 + 3) << 8 | (r0 + 3) << 16;
   auto lo = [](uint32_t u) { return __uint_as_float(u << 16); };
   auto hi = [](uint32_t u) { return __uint_as_float(u & 0xffff0000u); };
-  for (int t0 = 0; t0 < T; t0 += kG) {
-    const Group now = next[0];
-    next[0] = next[1];
-    next[1] = load(t0 + 2 * kG);
+  auto put = [&](int t0, const Group& now) {
 #pragma unroll
     for (int i = 0; i < kG; ++i) rows[(3 + t0 + i) * 64 + lane] = now.v[i];
+  };
+  auto work = [&](int t0, const Group& now) {
     uint32_t x0[kG], x1[kG], x2[kG];
     int place[kG];
 #pragma unroll
@@ -276,6 +285,24 @@ __global__ __launch_bounds__(64) void conv_tree_kernel(const uint16_t* __restric
       __builtin_amdgcn_raw_buffer_store_b32(place[i] < 0 ? 0u : out, by, y_at + static_cast<uint32_t>(t0 + i) * y_row,
                                             0, 0);
     }
+  };
+  if constexpr (W == 1) {
+    for (int t0 = 0; t0 < T; t0 += kG) {
+      const Group now = next[0];
+      next[0] = next[1];
+      next[1] = load(t0 + 2 * kG);
+      put(t0, now);
+      work(t0, now);
+    }
+  } else {
+    constexpr int kGroups = kMaxNodes / kG / W;
+#pragma unroll
+    for (int i = 0; i < kGroups; ++i)
+      if (kG * (wave + W * i) < T) put(kG * (wave + W * i), next[i]);
+    gdn::lds_barrier();
+#pragma unroll
+    for (int i = 0; i < kGroups; ++i)
+      if (kG * (wave + W * i) < T) work(kG * (wave + W * i), next[i]);
   }
   if (a < 0 || !in) return;
   if (dense) {
@@ -756,6 +783,15 @@ __global__ __launch_bounds__(2 * D, NT <= 2 ? 3 : NT == 3 || D == 128 ? 2 : 1) v
   }
 
   // --- the state after the pending path; its products with the nodes' rows ---
+  // (the rows come again, from the caches, kAhead products ahead: as many as there are registers
+  // for beside the state; all of them held from the start would cost a workgroup per CU)
+  constexpr int kAhead = NT == 1 ? KK : 2;
+  gdn::s16x8_t nk[kAhead], nq[kAhead];
+#pragma unroll
+  for (int n = 0; n < kAhead; ++n) {
+    nk[n] = k_frag(n % NT, n / NT);
+    nq[n] = q_frag(n % NT, n / NT);
+  }
   gdn::lds_barrier();
   if (pending) {
     S.scale(path.total);
@@ -774,9 +810,6 @@ __global__ __launch_bounds__(2 * D, NT <= 2 ? 3 : NT == 3 || D == 128 ? 2 : 1) v
   for (int I = 0; I < NT; ++I)
 #pragma unroll
     for (int c = 0; c < 2; ++c) ak[I][c] = aq[I][c] = gdn::f32x4_t{0.f, 0.f, 0.f, 0.f};
-  // (the nodes' rows come again, from the caches, one product ahead: held in registers from
-  // the start they would cost a workgroup per CU)
-  const int tiles = (T + 15) / 16;
   // What is written is dropped past the buffers' ends (rows past T): no branch, and the counts
   // by which a wave waits for its loads stay known (else it waits for its stores too).
   const int out_row = static_cast<int>(out_t), out_end = (T - 1) * out_row + D;
@@ -834,7 +867,6 @@ __global__ __launch_bounds__(2 * D, NT <= 2 ? 3 : NT == 3 || D == 128 ? 2 : 1) v
       __builtin_amdgcn_raw_buffer_store_b128(w16, bo, 2 * at, 0, 0);
     }
   };
-  gdn::s16x8_t nk = k_frag(0, 0), nq = q_frag(0, 0);
 #pragma unroll
   for (int kk = 0; kk < KK; ++kk) {
     u32x4_t f[2][3];
@@ -850,12 +882,11 @@ __global__ __launch_bounds__(2 * D, NT <= 2 ? 3 : NT == 3 || D == 128 ? 2 : 1) v
       }
 #pragma unroll
     for (int I = 0; I < NT; ++I) {
-      if (I >= tiles) break;
-      const gdn::s16x8_t x = nk, y = nq;
-      const int In = I + 1 < tiles && I + 1 < NT ? I + 1 : 0, kn = In ? kk : kk + 1;
-      if (kn < KK) {
-        nk = k_frag(In, kn);
-        nq = q_frag(In, kn);
+      const int at = kk * NT + I, to = at + kAhead;
+      const gdn::s16x8_t x = nk[at % kAhead], y = nq[at % kAhead];
+      if (to < KK * NT) {
+        nk[at % kAhead] = k_frag(to % NT, to / NT);
+        nq[at % kAhead] = q_frag(to % NT, to / NT);
       }
 #pragma unroll
       for (int n = 2; n >= 0; --n)  // (the smallest terms first)
@@ -872,7 +903,6 @@ __global__ __launch_bounds__(2 * D, NT <= 2 ? 3 : NT == 3 || D == 128 ? 2 : 1) v
   bool fine = true;
 #pragma unroll
   for (int I = 0; I < NT; ++I) {
-    if (I >= tiles) break;
     const gdn::f32x4_t xv = four(&fv[16 * I + 4 * lg]), xk4 = four(&fk[16 * I + 4 * lg]), xq4 = four(&fq[16 * I + 4 * lg]);
     gdn::f32x4_t rhs[2], out[2];
 #pragma unroll
@@ -914,7 +944,7 @@ __global__ __launch_bounds__(2 * D, NT <= 2 ? 3 : NT == 3 || D == 128 ? 2 : 1) v
     if constexpr (kLayer) {
       if (__any(!fine) && lane == 0) bad = 1;
       gdn::lds_barrier();
-      const uint4 next = I + 1 < tiles ? z_row(I + 1) : zv;
+      const uint4 next = I + 1 < NT ? z_row(I + 1) : zv;
       norm_rows(I);
       zv = next;
     }
@@ -931,7 +961,7 @@ __global__ __launch_bounds__(2 * D, NT <= 2 ? 3 : NT == 3 || D == 128 ? 2 : 1) v
   // wave's columns again, a column per lane, each node from its ancestors alone. ---
   const int mine = 32 * wave + (lane & 31);
 #pragma unroll 1
-  for (int I = 0; I < tiles; ++I) {
+  for (int I = 0; I < NT; ++I) {
 #pragma unroll
     for (int J = 0; J < NT; ++J)
       if (J == I)
@@ -1102,8 +1132,18 @@ extern "C" int gdn_conv_tree(const uint16_t* x, int64_t x_b, int64_t x_t, uint16
   if (accepted && (!rows_ok(last_x, lx_b, lx_t, C, last_T) || !last_parents || lp_b < 0)) return GDN_ERR_INVALID_ARG;
   if (B > 65535) return GDN_ERR_UNSUPPORTED;
   const ConvPending pd{last_x, lx_b, lx_t, last_parents, lp_b, accepted, last_T};
-  conv_tree_kernel<<<dim3((C + 127) / 128, B), dim3(64), ((T + 3) / 4 * 4 + 3) * 256, static_cast<hipStream_t>(stream)>>>(
-      x, x_b, x_t, pool, sp_slot, sp_ch, n_slots, ids, w, parents, p_b, pd, y, T, C);
+  const dim3 grid((C + 127) / 128, B);
+  const int lds = ((T + 3) / 4 * 4 + 3) * 256;
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  // Up to six workgroups per CU and more than one group of nodes: 1 x 8 3.9 us (one wave 4.2), 1 x
+  // 64 5.5 (11.7), 8 x 64 7.4 (13.1), 16 x 16 5.6 (6.0); 1 x 4 3.8 against 3.6, 32 x 16 8.0 against
+  // 7.4, 64 x 16 12.8 against 11.2 (8192 channels).
+  if (T > 4 && static_cast<int64_t>(B) * ((C + 127) / 128) <= 6 * gdn::kNumCu)
+    conv_tree_kernel<4><<<grid, dim3(256), lds, st>>>(x, x_b, x_t, pool, sp_slot, sp_ch, n_slots, ids, w, parents, p_b, pd,
+                                                     y, T, C);
+  else
+    conv_tree_kernel<1><<<grid, dim3(64), lds, st>>>(x, x_b, x_t, pool, sp_slot, sp_ch, n_slots, ids, w, parents, p_b, pd,
+                                                    y, T, C);
   return gdn_launch_status();
 }
 

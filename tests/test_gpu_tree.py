@@ -96,7 +96,8 @@ def test_rule_states_follow_from_u(pkg, dev):
         _close(got[b], P, bound, f"row {b}")
 
 
-@pytest.mark.parametrize("B,T,C,back", [(1, 1, 64, 1), (3, 5, 384, 2), (2, 16, 1032, 4), (1, 64, 8192, 1), (7, 33, 200, 6)])
+@pytest.mark.parametrize("B,T,C,back", [(1, 1, 64, 1), (3, 5, 384, 2), (2, 16, 1032, 4), (1, 64, 8192, 1), (7, 33, 200, 6),
+                                        (25, 18, 8192, 3), (40, 64, 6152, 30), (1600, 4, 96, 2), (1600, 11, 96, 4)])
 @pytest.mark.parametrize("pending", [False, True])
 def test_conv_against_64_bits(pkg, dev, B, T, C, back, pending):
     gen = torch.Generator().manual_seed(B + T + C)
