@@ -17,6 +17,8 @@
 // differences of sums: no cancellation, and a decay of 0 stays 0.  What has weight 0 is
 // left out, not multiplied: a node sees nothing of what its path has forgotten, nor of
 // unused nodes and other branches, infinities and NaN included.
+#include <algorithm>
+
 #include "gdn_common.h"
 
 namespace {
@@ -540,6 +542,20 @@ __device__ __forceinline__ gdn::f32x4_t mul16(const gdn::f32x4_t& a, const gdn::
   return c;
 }
 
+// v added over N (8 or 16) neighbouring lanes
+template <int kPerm>
+__device__ __forceinline__ float lane_perm(float v) {
+  return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), kPerm, 15, 15, false));
+}
+template <int N>
+__device__ __forceinline__ float row_sum(float v) {
+  v += lane_perm<0xB1>(v);   // lane ^ 1
+  v += lane_perm<0x4E>(v);   // lane ^ 2
+  v += lane_perm<0x141>(v);  // the other half of 8
+  if (N == 16) v += lane_perm<0x140>(v);
+  return v;
+}
+
 __device__ __forceinline__ const gdn::f32x4_t& four(const float* p) { return *reinterpret_cast<const gdn::f32x4_t*>(p); }
 
 // The layer around the rule: what the gates and the norm take and give.
@@ -558,25 +574,36 @@ struct TreeLayer {
 
 // NT: 16-node tiles of the tree.
 template <int D, int NT, bool kLayer>
-__global__ __launch_bounds__(2 * D, NT <= 2 ? 3 : NT == 3 || D == 128 ? 2 : 1) void rule_tree_kernel(
+__global__ __launch_bounds__(2 * D, D == 128 ? (NT <= 2 ? 3 : 2) : NT == 1 ? 3 : NT == 2 ? 2 : 1) void rule_tree_kernel(
     const uint16_t* __restrict__ q, int64_t q_b, int64_t q_t, const uint16_t* __restrict__ k, int64_t k_b, int64_t k_t,
     const uint16_t* __restrict__ v, int64_t v_b, int64_t v_t, const float* __restrict__ g,
     const uint16_t* __restrict__ beta, float* __restrict__ pool, int64_t s_slot, int64_t n_slots,
     const int64_t* __restrict__ ids, const int32_t* __restrict__ parents, int64_t p_b, RulePending pd,
     uint16_t* __restrict__ o, float* __restrict__ u, int B, int T, int Hk, int Hv, float scale, TreeLayer L) {
   constexpr int NW = D / 32, KK = D / 32, TM = 16 * NT;
-  __shared__ __align__(16) float wt[TM][TM];    // weights w(t, s)
-  __shared__ __align__(16) float cu[TM][TM];    // minus the coefficients of u_s in u_t
-  __shared__ __align__(16) float co[TM][TM];    // the coefficients of u_s in o_t
-  __shared__ __align__(16) float inv[TM][16];   // the inverses of the 16-node triangles
-  __shared__ __align__(16) float xk[kPathRows][D];  // the pending path's keys
-  __shared__ __align__(16) float xq[kPathRows][D];  // and corrections (and see the end)
+  // 16 x 16 tiles (I, J), J <= I, of a node t's row and an earlier node s's column
+  constexpr int kTiles = NT * (NT + 1) / 2;
+  auto tile = [](int I, int J) { return I * (I + 1) / 2 + J; };
+  __shared__ __align__(16) float cu[kTiles][16][16];  // minus the coefficients of u_s in u_t
+  __shared__ __align__(16) float co[kTiles][16][16];  // the coefficients of u_s in o_t
+  __shared__ __align__(16) float inv[TM][16];         // the inverses of the 16-node triangles
+  // The pending path's keys and corrections (and see the end).  With 64 nodes, where two
+  // workgroups of a CU leave no room for both, in the weights' place once those are used.
+  constexpr bool kShare = NT == 4;
+  constexpr int kPathFloats = 2 * kPathRows * D;
+  __shared__ __align__(16) float xbuf[kShare ? std::max(kPathFloats, 256 * kTiles) : kPathFloats];
+  __shared__ __align__(16) float wbuf[kShare ? 4 : 256 * kTiles];
+  float(*wt)[16][16] = reinterpret_cast<float(*)[16][16]>(kShare ? xbuf : wbuf);  // weights w(t, s)
+  float(&xk)[kPathRows][D] = *reinterpret_cast<float(*)[kPathRows][D]>(xbuf);
+  float(&xq)[kPathRows][D] = *reinterpret_cast<float(*)[kPathRows][D]>(xbuf + kPathRows * D);
   __shared__ __align__(16) int link[TM];
   __shared__ __align__(16) float bt[TM], total[TM], rk[TM], rq[TM];
   __shared__ __align__(16) float fv[TM], fk[TM], fq[TM];  // factors of v, S^T k, S^T q: 0 for an unused node
   __shared__ int any_cu[NT][NT];                // whether a tile of coefficients holds an ancestor
   __shared__ Path path;
-  __shared__ __align__(16) uint16_t rows[kLayer ? 2 : 1][kLayer ? 16 : 1][D + 8];  // a tile's outputs, two in turn
+  __shared__ __align__(16) uint16_t kq[2 * TM][D + 8];  // the nodes' keys, then their queries
+  // (the layer's norm) a tile's outputs, two in turn, where the rows were
+  uint16_t(*rows)[16][D + 8] = reinterpret_cast<uint16_t(*)[16][D + 8]>(&kq[0][0]);
   __shared__ int bad;                           // a correction is not finite
 
   const int64_t wi = gdn::xcd_remap(blockIdx.x, static_cast<int64_t>(B) * Hv);
@@ -606,9 +633,6 @@ __global__ __launch_bounds__(2 * D, NT <= 2 ? 3 : NT == 3 || D == 128 ? 2 : 1) v
   const buf_t bk = buf_of(k + b * k_b + kh * D), bq = buf_of(q + b * q_b + kh * D);
   const buf_t bv = buf_of(v + b * v_b + static_cast<int64_t>(h) * D);
   const int k_row = static_cast<int>(k_t) * 2, q_row = static_cast<int>(q_t) * 2, v_row = static_cast<int>(v_t) * 2;
-  // the lane's 8 values of every 32 of node 16 I + lr
-  auto k_frag = [&](int I, int kk) { return buf_row(bk, min(16 * I + lr, T - 1) * k_row + 16 * lg + 64 * kk); };
-  auto q_frag = [&](int I, int kk) { return buf_row(bq, min(16 * I + lr, T - 1) * q_row + 16 * lg + 64 * kk); };
   int my_parent = 0;
   float my_g = 0.0f, my_beta = 0.0f, A_log = 0.0f, dt_bias = 0.0f;
   PathIn pin = {-1, 0.0f, 0};
@@ -625,24 +649,14 @@ __global__ __launch_bounds__(2 * D, NT <= 2 ? 3 : NT == 3 || D == 128 ? 2 : 1) v
   } else if (wave == 1 && pd.accepted) {
     pin.load(pd, b, h, Hv, lane);
   }
-  // the wave's units (I, k or q): the 16 nodes' rows of tile I, for their norms and, against
-  // the keys of tiles J <= I, their products.  From the last wave on: the first two have the
-  // trees to follow.
-  constexpr int kUnits = 2 * NT, UW = (kUnits + NW - 1) / NW;
-  auto unit = [&](int j) { return (NW - 1 - wave) + j * NW; };
-  gdn::s16x8_t fr[UW][KK], fc[NT][KK];
+  // the nodes' rows, each once, 8 values per lane: the wave's share, keys first
+  constexpr int kRowLanes = D / 8, kRowsPer = 64 / kRowLanes;
+  const int rl = lane % kRowLanes, rr = wave * kRowsPer + lane / kRowLanes;  // of rows NW kRowsPer = 16
+  gdn::s16x8_t raw[2 * NT];
 #pragma unroll
-  for (int j = 0; j < UW; ++j) {
-    if (unit(j) >= kUnits) break;
-#pragma unroll
-    for (int kk = 0; kk < KK; ++kk) fr[j][kk] = unit(j) & 1 ? q_frag(unit(j) >> 1, kk) : k_frag(unit(j) >> 1, kk);
-  }
-#pragma unroll
-  for (int J = 0; J < NT; ++J) {
-    // (up to the tile of the wave's last unit)
-    if (unit(0) >= kUnits || 2 * J > unit(unit(UW - 1) < kUnits ? UW - 1 : 0) || 16 * J >= T) break;
-#pragma unroll
-    for (int kk = 0; kk < KK; ++kk) fc[J][kk] = k_frag(J, kk);
+  for (int p = 0; p < 2 * NT; ++p) {
+    const int t = min(16 * (p % NT) + rr, T - 1);
+    raw[p] = p < NT ? buf_row(bk, t * k_row + 16 * rl) : buf_row(bq, t * q_row + 16 * rl);
   }
   uint32_t vv[NT][4];  // rows 16 I + 4 lg + r, both columns
 #pragma unroll
@@ -659,7 +673,7 @@ __global__ __launch_bounds__(2 * D, NT <= 2 ? 3 : NT == 3 || D == 128 ? 2 : 1) v
 
   // --- the tree: lane t of wave 0 from node t up to the root; the pending path ---
   if (wave == 0) {
-    for (int i = lane; i < TM * TM / 4; i += 64) reinterpret_cast<float4*>(wt)[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int i = lane; i < 64 * kTiles; i += 64) reinterpret_cast<float4*>(wt)[i] = make_float4(0.f, 0.f, 0.f, 0.f);
     if (kLayer) {
       my_g = gdn::gate_g(my_g, A_log, dt_bias);
       my_beta = gdn::bf2f(gdn::gate_beta(my_beta));
@@ -670,13 +684,13 @@ __global__ __launch_bounds__(2 * D, NT <= 2 ? 3 : NT == 3 || D == 128 ? 2 : 1) v
     bool fine = lane < T && my_parent >= -1 && my_parent < lane;
     int s = fine ? my_parent : -1;
     float w = dec;
-    if (fine) wt[lane][lane] = 1.0f;
+    if (fine) wt[tile(lane >> 4, lane >> 4)][lane & 15][lane & 15] = 1.0f;
     while (__any(s >= 0)) {
       const int at = max(s, 0);
       const float d = __shfl(dec, at, 64);
       const int p = __shfl(my_parent, at, 64);
       if (s >= 0) {
-        wt[lane][s] = w;
+        wt[tile(lane >> 4, s >> 4)][lane & 15][s & 15] = w;
         w *= d;
         fine = p >= -1 && p < s;  // (each step goes to an earlier node: the walk ends)
         s = fine ? p : -1;
@@ -691,24 +705,21 @@ __global__ __launch_bounds__(2 * D, NT <= 2 ? 3 : NT == 3 || D == 128 ? 2 : 1) v
     find_path(pin, pd.T, lane, path);
   }
 #pragma unroll
-  for (int j = 0; j < UW; ++j) {
-    // row 16 I + lr: the lane's 8 values of every 32, then the four lanes of the row
-    if (unit(j) >= kUnits) break;
+  for (int p = 0; p < 2 * NT; ++p) {
+    const int t = 16 * (p % NT) + rr;
+    *reinterpret_cast<gdn::s16x8_t*>(&kq[p < NT ? t : TM + t][8 * rl]) = raw[p];
     float ss = 0.0f;
 #pragma unroll
-    for (int kk = 0; kk < KK; ++kk)
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float x = gdn::bf2f(static_cast<uint16_t>(fr[j][kk][e]));
-        ss = fmaf(x, x, ss);
-      }
-    ss += __shfl_xor(ss, 16, 64);
-    ss += __shfl_xor(ss, 32, 64);
-    if (lg == 0) (unit(j) & 1 ? rq : rk)[16 * (unit(j) >> 1) + lr] = rsqrtf(ss + kEps);
+    for (int e = 0; e < 8; ++e) {
+      const float x = gdn::bf2f(static_cast<uint16_t>(raw[p][e]));
+      ss = fmaf(x, x, ss);
+    }
+    ss = row_sum<kRowLanes>(ss);
+    if (rl == 0) (p < NT ? rk : rq)[t] = rsqrtf(ss + kEps);
   }
   gdn::lds_barrier();
   const bool pending = pd.accepted && path.count > 0;  // (the whole workgroup)
-  if (pending) stage_path<D>(pd, path, 0, b, h, kh, Hv, wave, NW, lane, xk, xq);
+  if (pending && !kShare) stage_path<D>(pd, path, 0, b, h, kh, Hv, wave, NW, lane, xk, xq);
   if (tid < TM) {
     const bool on = link[tid] != kUnused;
     fv[tid] = on ? bt[tid] : 0.0f;
@@ -720,81 +731,84 @@ __global__ __launch_bounds__(2 * D, NT <= 2 ? 3 : NT == 3 || D == 128 ? 2 : 1) v
   // Tile (I, J), J <= I, of K K^T and of Q K^T: lane (lr, lg), register r: t = 16 I + 4 lg
   // + r, s = 16 J + lr.  A weight of 0 is not multiplied: nothing of an unused node, of
   // another branch or past T gets in.
+  auto frag = [&](int row, int kk) { return *reinterpret_cast<const gdn::s16x8_t*>(&kq[row][32 * kk + 8 * lg]); };
+  auto coefficients = [&](int I, int J, bool out) {  // of u_s in o_t, else in u_t
+    gdn::f32x4_t c = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-  for (int j = 0; j < UW; ++j) {
-    const int I = unit(j) >> 1, type = unit(j) & 1;
-    if (unit(j) >= kUnits || 16 * I >= T) break;
+    for (int kk = 0; kk < KK; ++kk) c = gdn::mfma16x16x32(frag((out ? TM : 0) + 16 * I + lr, kk), frag(16 * J + lr, kk), c);
+    const int s = 16 * J + lr;
+    const float rs = rk[s];
+    bool some = false;
 #pragma unroll
-    for (int J = 0; J < NT; ++J) {
-      if (J > I) break;
-      gdn::f32x4_t c = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int kk = 0; kk < KK; ++kk) c = gdn::mfma16x16x32(fr[j][kk], fc[J][kk], c);
-      const int s = 16 * J + lr;
-      const float rs = rk[s];
-      bool some = false;
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int t = 16 * I + 4 * lg + r;
-        const float w = wt[t][s];
-        const bool on = w != 0.0f && link[t] != kUnused;
-        if (type) {
-          co[t][s] = on ? (scale * rq[t]) * (rs * w) * c[r] : 0.0f;
-        } else {
-          cu[t][s] = on && s < t ? -(bt[t] * rk[t]) * (rs * w) * c[r] : 0.0f;
-          some |= on && s < t;
-        }
-      }
-      if (!type) {
-        some = __any(some);
-        if (lane == 0) any_cu[I][J] = some;
+    for (int r = 0; r < 4; ++r) {
+      const int t = 16 * I + 4 * lg + r;
+      const float w = wt[tile(I, J)][4 * lg + r][lr];
+      const bool on = w != 0.0f && link[t] != kUnused;
+      if (out) {
+        co[tile(I, J)][4 * lg + r][lr] = on ? (scale * rq[t]) * (rs * w) * c[r] : 0.0f;
+      } else {
+        cu[tile(I, J)][4 * lg + r][lr] = on && s < t ? -(bt[t] * rk[t]) * (rs * w) * c[r] : 0.0f;
+        some |= on && s < t;
       }
     }
-    if (!type) {
-      // the inverse of the triangle by substitution: lane (lr, lg) rows 4 lg .. + 3 of its
-      // column lr; four rows at a time are finished and handed to the later ones (in few
-      // registers: the state is on its way into most of them)
-      wave_lds_order();
-      gdn::f32x4_t x;
+    if (!out) {
+      some = __any(some);
+      if (lane == 0) any_cu[I][J] = some;
+    }
+  };
+  // the inverse of a triangle by substitution: lane (lr, lg) rows 4 lg .. + 3 of its column lr;
+  // four rows at a time are finished and handed to the later ones (in few registers: the state
+  // is on its way into most of them)
+  auto invert = [&](int I) {
+    wave_lds_order();
+    gdn::f32x4_t x;
 #pragma unroll
-      for (int r = 0; r < 4; ++r) x[r] = 4 * lg + r == lr ? 1.0f : 0.0f;
+    for (int r = 0; r < 4; ++r) x[r] = 4 * lg + r == lr ? 1.0f : 0.0f;
 #pragma unroll
-      for (int p = 0; p < 4; ++p) {
-        gdn::f32x4_t c[4], y = x;
+    for (int p = 0; p < 4; ++p) {
+      gdn::f32x4_t c[4], y = x;
 #pragma unroll
-        for (int r = 0; r < 4; ++r) c[r] = four(&cu[16 * I + 4 * lg + r][16 * I + 4 * p]);
-        y[1] = fmaf(c[1][0], y[0], y[1]);
-        y[2] = fmaf(c[2][1], y[1], fmaf(c[2][0], y[0], y[2]));
-        y[3] = fmaf(c[3][2], y[2], fmaf(c[3][1], y[1], fmaf(c[3][0], y[0], y[3])));
-        float z[4];
+      for (int r = 0; r < 4; ++r) c[r] = four(&cu[tile(I, I)][4 * lg + r][4 * p]);
+      y[1] = fmaf(c[1][0], y[0], y[1]);
+      y[2] = fmaf(c[2][1], y[1], fmaf(c[2][0], y[0], y[2]));
+      y[3] = fmaf(c[3][2], y[2], fmaf(c[3][1], y[1], fmaf(c[3][0], y[0], y[3])));
+      float z[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) z[e] = __shfl(y[e], 16 * p + lr, 64);
+      for (int e = 0; e < 4; ++e) z[e] = __shfl(y[e], 16 * p + lr, 64);
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          float n = x[r];
+      for (int r = 0; r < 4; ++r) {
+        float n = x[r];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) n = fmaf(c[r][e], z[e], n);
-          x[r] = lg == p ? y[r] : n;
-        }
+        for (int e = 0; e < 4; ++e) n = fmaf(c[r][e], z[e], n);
+        x[r] = lg == p ? y[r] : n;
       }
+    }
 #pragma unroll
-      for (int r = 0; r < 4; ++r) inv[16 * I + 4 * lg + r][lr] = x[r];
+    for (int r = 0; r < 4; ++r) inv[16 * I + 4 * lg + r][lr] = x[r];
+  };
+  // a triangle and its inverse to one wave (from the last one on), the other tiles dealt out
+  int turn = 0;
+#pragma unroll 1
+  for (int I = 0; I < NT; ++I) {
+    if (wave == NW - 1 - I % NW) {
+      coefficients(I, I, false);
+      invert(I);
+    }
+#pragma unroll 1
+    for (int J = 0; J <= I; ++J) {
+      if (J < I && turn++ % NW == wave) coefficients(I, J, false);
+      if (turn++ % NW == wave) coefficients(I, J, true);
     }
   }
 
   // --- the state after the pending path; its products with the nodes' rows ---
-  // (the rows come again, from the caches, kAhead products ahead: as many as there are registers
-  // for beside the state; all of them held from the start would cost a workgroup per CU)
-  constexpr int kAhead = NT == 1 ? KK : 2;
-  gdn::s16x8_t nk[kAhead], nq[kAhead];
-#pragma unroll
-  for (int n = 0; n < kAhead; ++n) {
-    nk[n] = k_frag(n % NT, n / NT);
-    nq[n] = q_frag(n % NT, n / NT);
-  }
   gdn::lds_barrier();
   if (pending) {
     S.scale(path.total);
+    if (kShare) {
+      stage_path<D>(pd, path, 0, b, h, kh, Hv, wave, NW, lane, xk, xq);
+      gdn::lds_barrier();
+    }
     S.advance(min(path.count, kPathRows), xk, xq, wave, lr, lg);
     for (int p = kPathRows; p < path.count; p += kPathRows) {
       gdn::lds_barrier();
@@ -830,7 +844,7 @@ __global__ __launch_bounds__(2 * D, NT <= 2 ? 3 : NT == 3 || D == 128 ? 2 : 1) v
   auto norm_rows = [&](int I) {
     const int t = 16 * I + row;
     uint16_t xs[8], zs[8], ws[8];
-    __builtin_memcpy(xs, &rows[I & 1][kLayer ? row : 0][c8], 16);
+    __builtin_memcpy(xs, &rows[I & 1][row][c8], 16);
     __builtin_memcpy(zs, &zv, 16);
     __builtin_memcpy(ws, &wv, 16);
     float v[8], ss = 0.0f;
@@ -882,12 +896,7 @@ __global__ __launch_bounds__(2 * D, NT <= 2 ? 3 : NT == 3 || D == 128 ? 2 : 1) v
       }
 #pragma unroll
     for (int I = 0; I < NT; ++I) {
-      const int at = kk * NT + I, to = at + kAhead;
-      const gdn::s16x8_t x = nk[at % kAhead], y = nq[at % kAhead];
-      if (to < KK * NT) {
-        nk[at % kAhead] = k_frag(to % NT, to / NT);
-        nq[at % kAhead] = q_frag(to % NT, to / NT);
-      }
+      const gdn::s16x8_t x = frag(16 * I + lr, kk), y = frag(TM + 16 * I + lr, kk);
 #pragma unroll
       for (int n = 2; n >= 0; --n)  // (the smallest terms first)
 #pragma unroll
@@ -899,6 +908,7 @@ __global__ __launch_bounds__(2 * D, NT <= 2 ? 3 : NT == 3 || D == 128 ? 2 : 1) v
   }
 
   // --- u and o, 16 nodes at a time ---
+  if constexpr (kLayer) gdn::lds_barrier();  // the rows have been read
   gdn::f32x4_t uu[NT][2];
   bool fine = true;
 #pragma unroll
@@ -917,14 +927,14 @@ __global__ __launch_bounds__(2 * D, NT <= 2 ? 3 : NT == 3 || D == 128 ? 2 : 1) v
 #pragma unroll
     for (int J = 0; J < I; ++J) {
       if (!any_cu[I][J]) continue;
-      const gdn::f32x4_t a = four(&cu[16 * I + lr][16 * J + 4 * lg]), e = four(&co[16 * I + lr][16 * J + 4 * lg]);
+      const gdn::f32x4_t a = four(&cu[tile(I, J)][lr][4 * lg]), e = four(&co[tile(I, J)][lr][4 * lg]);
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
         rhs[c] = mul16(a, uu[J][c], rhs[c]);
         out[c] = mul16(e, uu[J][c], out[c]);
       }
     }
-    const gdn::f32x4_t a = four(&inv[16 * I + lr][4 * lg]), e = four(&co[16 * I + lr][16 * I + 4 * lg]);
+    const gdn::f32x4_t a = four(&inv[16 * I + lr][4 * lg]), e = four(&co[tile(I, I)][lr][4 * lg]);
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
       uu[I][c] = mul16(a, rhs[c], gdn::f32x4_t{0.f, 0.f, 0.f, 0.f});
@@ -979,12 +989,12 @@ __global__ __launch_bounds__(2 * D, NT <= 2 ? 3 : NT == 3 || D == 128 ? 2 : 1) v
         if (fk[t] != 0.0f) x += fk[t] * xk[t - 16 * I][mine];
         if (fq[t] != 0.0f) y = fq[t] * xq[t - 16 * I][mine];
         for (int s = link[t]; s >= 0; s = link[s]) {
-          if (wt[t][s] == 0.0f) continue;
-          const float us = u[out0 + s * out_t + mine];
-          x = fmaf(cu[t][s], us, x);
-          y = fmaf(co[t][s], us, y);
+          const float us = u[out0 + s * out_t + mine], a = cu[tile(I, s >> 4)][t & 15][s & 15],
+                      e = co[tile(I, s >> 4)][t & 15][s & 15];
+          if (a != 0.0f) x = fmaf(a, us, x);
+          if (e != 0.0f) y = fmaf(e, us, y);
         }
-        y = fmaf(co[t][t], x, y);
+        y = fmaf(co[tile(I, I)][t & 15][t & 15], x, y);
       }
       if (lane < 32) {
         u[out0 + t * out_t + mine] = x;
