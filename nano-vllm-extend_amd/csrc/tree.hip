@@ -331,6 +331,11 @@ __global__ __launch_bounds__(64 * W) void conv_tree_kernel(const uint16_t* __res
 // up to it exactly (8 bits of the significand each), k and q are not normalised before
 // (their norms scale the results), so the products are those of fp32 operands.
 //
+// The nodes' rows are loaded once, 8 values per lane ahead of the state, and go to LDS, where
+// the coefficients (k_s . k_t, k_s . q_t, 16 x 16 nodes at a time, dealt to the waves) and the
+// products with the state find them.  (Rows read by each wave from the caches: 64 x 64 nodes
+// 120 us for 103, 1 x 64 21.4 for 17.8, 64 x 16 without a pending path 37.1 for 33.4.)
+//
 // The corrections u of 16 nodes are the product of the inverse of their 16 x 16 triangle
 // (found by substitution while the state is on its way) with what the state, v and the
 // nodes of earlier tiles give, and o adds the products of the second coefficients with u:
@@ -340,16 +345,17 @@ __global__ __launch_bounds__(64 * W) void conv_tree_kernel(const uint16_t* __res
 // kLayer: the layer's gates before it and its gated norm behind it in the same launch.  Wave
 // 0 finds the gates of the head's nodes.  A tile's outputs, rounded to bf16 as without the
 // norm, meet in LDS, and D / 8 lanes per row take the norm in the order of its own kernel.
-// Two launches and the outputs' way out and in less: 64 trees of 16 nodes 65.7 us for the
-// 71.8 of three launches, one of 8 nodes 10.9 for 14.3 (32 heads of 128, with a pending path).
+// Two launches and the outputs' way out and in less: 64 trees of 16 nodes 63 us for the 69
+// of three launches, one of 8 nodes 12.0 for 15.4 (32 heads of 128, with a pending path).
 //
 // What bounds it: the state's way in (and out, where a path is pending).  The tree's
 // weights, the nodes' norms and dot products (on the matrix cores as well) and the
 // pending path's rows are worked on while the state is on its way.  32 heads of 128: 64
-// trees of 16 nodes with a pending path 59 us (5.3 TB/s, a large copy's rate), without one
-// 39; 30 trees of 24 nodes 39, 16 of 48 28; one tree of 8 nodes 7.0, the latency of its
-// chain (ids, state, products, corrections).  Paths of 48 nodes cost more than the state:
-// 21 chains of 48 76 us, each row of the path a pass of the vector ALUs over the tile.
+// trees of 16 nodes with a pending path 57.5 us (5.5 TB/s, a large copy's rate), without one
+// 33.4; 30 trees of 24 nodes 33.7, 16 of 48 24.5; one tree of 8 nodes 6.6, the latency of its
+// chain (ids, state, products, corrections).  64 nodes cost more than the state (64 trees
+// 103 us, one 17.8: coefficients 4.3, products 2.2, corrections 3.3), and so do long paths: 21
+// chains of 48 70 us, each row of the path a pass of the vector ALUs over the tile.
 // Before: a thread per column of the state and one node at a time 249 us (64 x 16) and
 // 32 (1 x 8).
 typedef float f32x2_t __attribute__((ext_vector_type(2)));
