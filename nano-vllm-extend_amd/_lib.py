@@ -8,6 +8,8 @@ silent fallback.
 from __future__ import annotations
 
 import ctypes
+import importlib.machinery
+import importlib.util
 import os
 import struct
 from pathlib import Path
@@ -136,6 +138,27 @@ def load() -> ctypes.CDLL:
         fn.restype = RESTYPES.get(name, ctypes.c_int)
     _LIB = lib
     return lib
+
+
+QUICK_PATH = Path(__file__).resolve().parent / "lib" / "gdn_quick_calls.so"
+_QUICK = None
+
+
+def quick():
+    """The module of csrc/quick_calls.cpp: a call whose tensors the kernel takes as they are,
+    checked and launched in C++; None where the wrapper has to look at them itself."""
+    global _QUICK
+    if _QUICK is None:
+        load()   # (the module's calls are the library's)
+        if not QUICK_PATH.exists():
+            raise GDNLibraryError(f"{QUICK_PATH} not found: build it with `python nano-vllm-extend_amd/build.py` "
+                                  "(or __graft_entry__.build())")
+        loader = importlib.machinery.ExtensionFileLoader("gdn_quick_calls", str(QUICK_PATH))
+        module = importlib.util.module_from_spec(importlib.util.spec_from_loader("gdn_quick_calls", loader))
+        loader.exec_module(module)
+        module.set_check(check)
+        _QUICK = module
+    return _QUICK
 
 
 def check(name: str, status: int) -> None:

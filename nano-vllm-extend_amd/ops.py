@@ -960,6 +960,9 @@ def conv_tree_step(x: torch.Tensor, conv_pool: torch.Tensor, ids: torch.Tensor, 
     path the results are conv_decode_step's, bit for bit.  Returns y [B, T, C].
     (No reference counterpart: spec decode is disabled for qwen3_5,
     nanovllm/config.py:84.)"""
+    y = _lib.quick().conv_tree(x, conv_pool, ids, weight, parents, pending)
+    if y is not None:
+        return y
     last_x, last_parents, accepted = pending if pending is not None else (None, None, None)
     idx = _device_of(x, conv_pool, ids, weight, parents, last_x, last_parents, accepted)
     if x.dim() != 3:
@@ -1037,6 +1040,9 @@ def recurrent_gdn_tree(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: tor
     it, also what is not finite.
     (No reference counterpart: spec decode is disabled for qwen3_5,
     nanovllm/config.py:84; one token: qwen3_5.py:575-594.)"""
+    out = _lib.quick().rule_tree(q, k, v, g, beta, s_pool, ids, parents, pending)
+    if out is not None:
+        return out
     idx = _device_of(k, q, v, g, beta, s_pool, ids, parents, *(pending or ()))
     dims, rows, state, keep = _rule_args(q, k, v, s_pool, ids, parents, pending)
     B, T, Hk, Hv, D = dims
@@ -1063,6 +1069,11 @@ def recurrent_tree_fused(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, b: t
     zeros for the others (rows of a slot that is none: g too).  b, a [B, T, Hv] bf16,
     a_log and dt_bias [Hv], z [B, T, Hv * D] bf16, norm_weight [D].  Returns (y [B, T,
     Hv, D] bf16, or its (e4m3, scales); u; g), g for the next step's pending."""
+    out = _lib.quick().rule_tree_layer(q, k, v, b, a, a_log, dt_bias, z, norm_weight, s_pool, ids, parents, eps, pending,
+                                       fp8)
+    if out is not None:
+        y, scale, u, g = out
+        return (y, scale) if fp8 else y, u, g
     idx = _device_of(k, q, v, b, a, a_log, dt_bias, z, norm_weight, s_pool, ids, parents, *(pending or ()))
     dims, rows, state, keep = _rule_args(q, k, v, s_pool, ids, parents, pending)
     B, T, Hk, Hv, D = dims
@@ -1102,6 +1113,8 @@ def commit_tree(s_pool: torch.Tensor, conv_pool: torch.Tensor, ids: torch.Tensor
     as conv_tree_step's).
     x [B, T, C] the raw rows, k [B, T, Hk, D], g [B, T, Hv], u [B, T, Hv, D] and
     parents those of the verified step."""
+    if _lib.quick().commit_tree(s_pool, conv_pool, ids, parents, accepted, x, k, g, u):
+        return
     idx = _device_of(s_pool, conv_pool, ids, parents, accepted, x, k, g, u)
     if k.dim() != 4 or u.dim() != 4 or x.dim() != 3:
         raise ValueError(f"x, k, u must be [B, T, C], [B, T, Hk, D], [B, T, Hv, D], got {list(x.shape)}, "
@@ -1367,6 +1380,10 @@ def linear_fp8(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor
     a call with its result), or e4m3 with its x_scale [M, K / 128] (any strides).  K a
     multiple of 128.  fp32 accumulation; returns [..., N] bf16 (or writes `out`, a [M, N]
     view with contiguous rows)."""
+    if out is None:
+        y = _lib.quick().linear_fp8(x, weight, weight_scale, x_scale)
+        if y is not None:
+            return y
     M, N, K = _check_fp8(x, weight, weight_scale, x_scale)
     if out is None:
         y = torch.empty(M, N, dtype=torch.bfloat16, device=x.device)
@@ -1475,6 +1492,9 @@ def rms_norm_gated_fp8(hidden_states: torch.Tensor, gate: torch.Tensor, weight: 
     + eps) * w * silu(z) in fp32 over the last dim, then quantize_fp8's groups of 128
     over a token's H * D columns (a multiple of 128), rounded once.  hidden_states / gate
     [..., H, D] bf16.  Returns (e4m3 [..., H, D], scales [tokens, H * D / 128] fp32)."""
+    out = _lib.quick().norm_fp8(hidden_states, gate, weight, eps)
+    if out is not None:
+        return out
     idx = _device_of(hidden_states, gate, weight)
     _bf16(hidden_states, "hidden_states")
     _bf16(gate, "gate")

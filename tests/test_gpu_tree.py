@@ -587,3 +587,67 @@ def test_rule_with_gates_and_norm_where_not_finite(pkg, dev):
     rel = d.norm(dim=-1, keepdim=True) / ro.norm(dim=-1, keepdim=True)
     bound = r * gain * (d + ro.abs() * rel) * 1.1 + 6 * ref.HALF_BF16 * (want[0, ~hit, 1].double().abs() + r * gain * d)
     _close(y[0, ~hit, 1], want[0, ~hit, 1].double(), bound + 1e-30, "head 1")
+
+
+class _NoQuick:
+    def __getattr__(self, name):
+        return lambda *a: None
+
+
+def test_quick_and_checked_calls_agree(pkg, dev, monkeypatch):
+    """The calls by way of C++ and those by way of the Python wrappers: the same bits, errors of the
+    same type; memory that comes back; what the kernel does not take as it is goes the other way."""
+    gen = torch.Generator().manual_seed(61)
+    B, T, Hk, Hv, D, slots = 3, 9, 1, 2, 128, 5
+    C = 2 * Hk * D + Hv * D
+    i, last = _inputs(gen, B, T, Hk, Hv, D), _inputs(gen, B, T, Hk, Hv, D)
+    parents, accepted = (t.to(dev) for t in ref.tree(gen, B, T, 3))
+    ids = torch.tensor([4, 0, 2], device=dev)
+    x, y, g, beta = (i[n].to(dev) for n in ("x", "y", "g", "beta"))
+    q, k, v = _qkv(y, Hk, Hv, D)
+    lk, lg, lu, lx = _qkv(last["y"].to(dev), Hk, Hv, D)[1], last["g"].to(dev), last["u"].to(dev), last["x"].to(dev)
+    b, a, A_log, dt, z, w = (t.to(dev) for t in _layer_inputs(gen, B, T, Hk, Hv, D))
+    z, cw = z[..., 8:-8], torch.randn(C, 4, generator=gen).to(BF16).to(dev)
+    pend = (lk, lg, lu, parents, accepted)
+    pools = (torch.randn(slots, 2, Hv, D, D, generator=gen) * 0.3, torch.randn(slots, 2, C, 3, generator=gen).to(BF16))
+    x8, xs = pkg.quantize_fp8(torch.randn(40, 256, generator=gen).to(BF16).to(dev))
+    w8, ws = pkg.quantize_weight_fp8(torch.randn(300, 256, generator=gen).to(BF16).to(dev))
+    rows = torch.randn(5, 8, 256, generator=gen).to(BF16).to(dev)
+
+    def run():
+        s, c = (p.to(dev)[:, 1] for p in pools)
+        out = [pkg.conv_tree_step(x, c, ids, cw, parents, pending=(lx, parents, accepted)),
+               pkg.conv_tree_step(x, c, ids, cw, parents[0]),
+               *pkg.recurrent_gdn_tree(q, k, v, g, beta, s, ids, parents, pending=pend),
+               *pkg.recurrent_gdn_tree(q, k, v, g, beta, s, ids, parents)]
+        y8, *rest = pkg.recurrent_tree_fused(q, k, v, b, a, A_log, dt, z, w, s, ids, parents, 1e-6, pending=pend, fp8=True)
+        out += [*y8, *rest, *pkg.recurrent_tree_fused(q, k, v, b, a, A_log, dt, z, w, s, ids, parents)]
+        pkg.commit_tree(s, c, ids, parents, accepted, lx, lk, lg, lu)
+        out += [s, c, pkg.linear_fp8(x8, w8, ws, x_scale=xs), pkg.linear_fp8(rows, w8, ws), pkg.linear_fp8(rows[:1], w8, ws),
+                *pkg.rms_norm_gated_fp8(v, v, w, 1e-6)]
+        return [t.contiguous().view(torch.uint8).cpu() for t in out], [t.shape for t in out], [t.stride() for t in out]
+
+    quick = pkg._lib.quick()
+    assert quick.conv_tree(x, pools[1].to(dev)[:, 1], ids, cw, parents, None) is not None
+    assert quick.linear_fp8(rows, w8, ws, None) is not None and quick.norm_fp8(v.contiguous(), v.contiguous(), w, 1e-6)
+    got = run()
+    before = torch.cuda.memory_allocated()
+    for _ in range(50):
+        pkg.recurrent_tree_fused(q, k, v, b, a, A_log, dt, z, w, pools[0].to(dev)[:, 1], ids, parents, pending=pend)
+        pkg.linear_fp8(rows, w8, ws)
+    assert torch.cuda.memory_allocated() == before
+    # int32 ids, int64 parents, strided gates: the wrappers copy
+    for bad in (quick.conv_tree(x, pools[1].to(dev)[:, 1], ids.int(), cw, parents, None),
+                quick.conv_tree(x, pools[1].to(dev)[:, 1], ids, cw, parents.long(), None),
+                quick.rule_tree(q, k, v, torch.cat([g, g], 2)[..., :Hv], beta, pools[0].to(dev)[:, 1], ids, parents, None),
+                quick.rule_tree(q, k, v, g, beta, pools[0].to(dev)[:, 1], ids.cpu(), parents, None),
+                quick.linear_fp8(rows[..., :128], w8, ws, None), quick.linear_fp8(x8, w8, ws, None)):
+        assert bad is None
+    with pytest.raises(pkg._lib.GDNKernelError):         # head dim 32
+        pkg.recurrent_gdn_tree(q[..., :32].contiguous(), k[..., :32].contiguous(), v[..., :32].contiguous(), g, beta,
+                               torch.zeros(slots, Hv, 32, 32, device=dev), ids, parents)
+    monkeypatch.setattr(pkg._lib, "quick", lambda: _NoQuick())
+    want = run()
+    torch.cuda.synchronize()
+    assert got[1] == want[1] and got[2] == want[2]
+    assert all(torch.equal(p, r) for p, r in zip(got[0], want[0]))

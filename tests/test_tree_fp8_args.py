@@ -283,3 +283,17 @@ def test_decode_step_to_e4m3_refuses(pkg, monkeypatch):
     for bad in (dict(q=P), dict(k=P), dict(Hk=1), dict(Hv=5), dict(x=None), dict(x=odd), dict(y=None), dict(y=odd),
                 dict(s=None), dict(ss=3), dict(z=None), dict(z=odd), dict(w=None), dict(sx=1020), dict(B=-1)):
         assert f(**bad) == _lib.GDN_ERR_INVALID_ARG, bad
+
+
+def test_quick_calls_leave_the_rest_to_the_wrappers(pkg):
+    """What is not a tensor on the device as the kernel takes it is not taken, and said to be None."""
+    quick = pkg._lib.quick()
+    t, f = torch.zeros(1, 2, 8, dtype=BF16), torch.zeros(1, 2, 2, 64)
+    for name, n in (("conv_tree", 6), ("rule_tree", 9), ("rule_tree_layer", 15), ("commit_tree", 9), ("linear_fp8", 4),
+                    ("norm_fp8", 4)):
+        call = getattr(quick, name)
+        for arg in (t, f, None, 3, "x", (), torch.nn.Parameter(f), [t]):
+            assert call(*[arg] * n) is None, (name, arg)
+        for wrong in (0, n - 1, n + 1):
+            with pytest.raises(TypeError):
+                call(*[t] * wrong)
