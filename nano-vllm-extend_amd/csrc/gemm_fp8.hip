@@ -295,7 +295,7 @@ __global__ __launch_bounds__(kPPThreads, 2) void gemm_fp8_pp_kernel(const uint8_
         for (int i = 0; i < 4; ++i)
 #pragma unroll
           for (int b = 0; b < 2; ++b)
-            gemm_store16(acc[a][b][i][0], acc[a][b][i][1], out, M, N, m0c + 128 * a + 64 * wm + 16 * i,
+            gemm_store16<true>(acc[a][b][i][0], acc[a][b][i][1], out, M, N, m0c + 128 * a + 64 * wm + 16 * i,
                          n0c + 128 * b + 32 * wn, lane_e, GemmGates{}, nullptr);
       if (Ln >= xend) break;
       L = Ln;
@@ -377,7 +377,7 @@ __global__ __launch_bounds__(kPPThreads, 2) void gemm_fp8_pp_kernel(const uint8_
     if (!wm) half_barrier();
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-      gemm_store16(c[i][0], c[i][1], out, M, N, m0 + 64 * wm + 16 * i, n0 + 32 * wn, new_lane(), GemmGates{}, nullptr);
+      gemm_store16<true>(c[i][0], c[i][1], out, M, N, m0 + 64 * wm + 16 * i, n0 + 32 * wn, new_lane(), GemmGates{}, nullptr);
   }
   __builtin_amdgcn_s_waitcnt(0);
 }
@@ -526,7 +526,7 @@ __device__ __forceinline__ void ring_store(const gdn::f32x4_t (&acc)[MT][NT][2],
       c0 += red[((w * MT * NT + ij) * 2) * 64 + lane];
       c1 += red[((w * MT * NT + ij) * 2 + 1) * 64 + lane];
     }
-    gemm_store16(c0, c1, out, M, N, m0 + 16 * (ij / NT), n0 + 32 * (ij % NT), lane, GemmGates{}, nullptr);
+    gemm_store16<true>(c0, c1, out, M, N, m0 + 16 * (ij / NT), n0 + 32 * (ij % NT), lane, GemmGates{}, nullptr);
   }
 }
 
@@ -1022,7 +1022,7 @@ __global__ __launch_bounds__(kFp8Threads, 2) void gemm_fp8_deep_kernel(const uin
   for (int i = 0; i < 2; ++i)
 #pragma unroll
     for (int j = 0; j < NJ; ++j)
-      gemm_store16(acc[i][j][0], acc[i][j][1], out, M, N, m0 + 32 * wm + 16 * i, n0 + 32 * (NJ * wn + j), lane,
+      gemm_store16<true>(acc[i][j][0], acc[i][j][1], out, M, N, m0 + 32 * wm + 16 * i, n0 + 32 * (NJ * wn + j), lane,
                    GemmGates{}, nullptr);
   __builtin_amdgcn_s_waitcnt(0);  // the repeated loads past the last step
 }

@@ -56,7 +56,10 @@ __device__ __forceinline__ void dma16(__amdgpu_buffer_rsrc_t rsrc, uint8_t* lds,
 
 // ---- 16 rows x 32 columns of accumulators to the output (the 8-wave kernel) ----
 // Lane (lr, lg) holds C[row0 + lr][cb + 8 lg .. + 7] in c0 (the first four) and
-// c1: one 16-byte piece, four lanes filling 64 contiguous bytes of a row.
+// c1: one 16-byte piece, four lanes filling 64 contiguous bytes of a row.  kAnyRow: the piece
+// goes out whole in rows without 16-byte alignment too (the 8-bit GEMM's kernels: 8192 x
+// 4001 x 256 36 us, value by value 77; 4002 columns 26).
+template <bool kAnyRow = false>
 __device__ __forceinline__ void gemm_store16(const gdn::f32x4_t& c0, const gdn::f32x4_t& c1, const GemmOut& out,
                                              int M, int N, int row0, int cb, int lane, const GemmGates& gt,
                                              uint16_t* gs) {
@@ -82,7 +85,9 @@ __device__ __forceinline__ void gemm_store16(const gdn::f32x4_t& c0, const gdn::
     const int pb = pick(sp, 0, out.end[0], out.end[1], out.end[2]);
     uint16_t* crow = pick(sp, out.c[0], out.c[1], out.c[2], out.c[3]) +
                      static_cast<int64_t>(m) * pick(sp, out.ld[0], out.ld[1], out.ld[2], out.ld[3]) - pb;
-    if (pick(sp, out.vec[0], out.vec[1], out.vec[2], out.vec[3]) && n + 8 <= pe) {
+    if (kAnyRow && n + 8 <= pe) {
+      __builtin_memcpy(crow + n, &w, 16);
+    } else if (!kAnyRow && pick(sp, out.vec[0], out.vec[1], out.vec[2], out.vec[3]) && n + 8 <= pe) {
       *reinterpret_cast<uint4*>(crow + n) = w;
     } else {
       const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
