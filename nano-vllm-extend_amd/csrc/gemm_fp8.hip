@@ -895,8 +895,13 @@ __global__ __launch_bounds__(64 * NW) void gemm_fp8_rows_kernel(const uint16_t* 
 // loads of step s + NS - 1 at the start of step s, the barrier before it waiting for
 // step s alone.  The scales of a step come with its operands (wave 0 the rows', the
 // others B's: a load each).
-template <int BN, int NS>
-__global__ __launch_bounds__(kFp8Threads, 2) void gemm_fp8_deep_kernel(const uint8_t* __restrict__ A, int64_t lda,
+//
+// H = 2: two groups of four waves, each with stages of its own, take the first and the second
+// half of the K-steps (an odd one past the last repeats it with scale 0), which puts twice the
+// loads in flight where a CU has one tile; the second's sums
+// are added to the first's through LDS.
+template <int BN, int NS, int H>
+__global__ __launch_bounds__(kFp8Threads * H, 2) void gemm_fp8_deep_kernel(const uint8_t* __restrict__ A, int64_t lda,
                                                                        const uint8_t* __restrict__ B, int64_t ldb,
                                                                        Fp8Scales sc, GemmOut out, int M, int N,
                                                                        int K) {
@@ -907,10 +912,10 @@ __global__ __launch_bounds__(kFp8Threads, 2) void gemm_fp8_deep_kernel(const uin
   constexpr int kVm = (NS - 2) * kPer;
   static_assert(kVm < 64, "vmcnt field");
   constexpr int kWait = (kVm & 15) | (7 << 4) | ((kVm >> 4) << 14);
-  __shared__ __align__(16) uint8_t st0[kStage];
-  __shared__ __align__(16) uint8_t st1[kStage];
-  __shared__ __align__(16) uint8_t st2[kStage];
-  __shared__ __align__(16) uint8_t st3[NS == 4 ? kStage : 16];
+  __shared__ __align__(16) uint8_t st0[H * kStage];
+  __shared__ __align__(16) uint8_t st1[H * kStage];
+  __shared__ __align__(16) uint8_t st2[H * kStage];
+  __shared__ __align__(16) uint8_t st3[NS == 4 ? H * kStage : 16];
 
   const int mb_n = (M + BM - 1) / BM, nb_n = (N + BN - 1) / BN;
   const int64_t L = gdn::xcd_remap(blockIdx.x, static_cast<int64_t>(mb_n) * nb_n);
@@ -920,7 +925,8 @@ __global__ __launch_bounds__(kFp8Threads, 2) void gemm_fp8_deep_kernel(const uin
   const int gm = static_cast<int>(min<int64_t>(kGroupM8, mb_n - grp * kGroupM8));
   const int m0 = BM * static_cast<int>(grp * kGroupM8 + in_grp % gm), n0 = BN * static_cast<int>(in_grp / gm);
   const int lane = threadIdx.x & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6 & 3);
+  const int half = H == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 8);
   const int wm = wave >> 1, wn = wave & 1;
   const int lr = lane & 15, lg = lane >> 4;
   const __amdgpu_buffer_rsrc_t ra = rsrc_of(A), rb = rsrc_of(B), rs = rsrc_of(wave == 0 ? sc.a : sc.b);
@@ -935,9 +941,10 @@ __global__ __launch_bounds__(kFp8Threads, 2) void gemm_fp8_deep_kernel(const uin
   const int vs = wave == 0 ? static_cast<int>(min(m0 + lane, M - 1) * sc.a_row * 4)
                            : static_cast<int>(n0 / 128 * sc.b_row * 4);
   const int s_step = wave == 0 ? static_cast<int>(sc.a_grp) * 4 : 4;
-  const int nk = K / 128;
+  const int nk = K / 128, trips = (nk + H - 1) / H, first = half * trips;
   auto issue = [&](uint8_t* st, int step) {
-    const int s = min(step, nk - 1);
+    const int s = min(first + step, nk - 1);
+    st += half * kStage;
 #pragma unroll
     for (int i = 0; i < kAPer + kBPer; ++i)
       dma16(i < kAPer ? ra : rb, st + (i < kAPer ? 0 : BM * 128) + (wave + 4 * (i < kAPer ? i : i - kAPer)) * 1024,
@@ -960,6 +967,7 @@ __global__ __launch_bounds__(kFp8Threads, 2) void gemm_fp8_deep_kernel(const uin
     __builtin_amdgcn_sched_barrier(0);
     issue(nxt, step + NS - 1);
     __builtin_amdgcn_sched_barrier(0);
+    cur += half * kStage;
     const uint8_t* b = cur + BM * 128;
     const float* p = reinterpret_cast<const float*>(cur + (BM + BN) * 128);
     Frag8 fa[2], fb[NJ][2];
@@ -979,7 +987,7 @@ __global__ __launch_bounds__(kFp8Threads, 2) void gemm_fp8_deep_kernel(const uin
         fb[j][t].lo = *reinterpret_cast<const i32x4_t*>(b + swb_off(r, lg));
         fb[j][t].hi = *reinterpret_cast<const i32x4_t*>(b + swb_off(r, 4 + lg));
       }
-    const float sb = p[64];
+    const float sb = H == 1 || first + step < nk ? p[64] : 0.0f;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const float s = f[i] * sb;
@@ -1000,23 +1008,44 @@ __global__ __launch_bounds__(kFp8Threads, 2) void gemm_fp8_deep_kernel(const uin
   // loop head and wait there for loads that are meant to stay in flight)
   int s = 0;
   if constexpr (NS == 4) {
-    for (; s + 3 < nk; s += 4) {
+    for (; s + 3 < trips; s += 4) {
       one(st0, st3, s);
       one(st1, st0, s + 1);
       one(st2, st1, s + 2);
       one(st3, st2, s + 3);
     }
-    if (s < nk) one(st0, st3, s);
-    if (s + 1 < nk) one(st1, st0, s + 1);
-    if (s + 2 < nk) one(st2, st1, s + 2);
+    if (s < trips) one(st0, st3, s);
+    if (s + 1 < trips) one(st1, st0, s + 1);
+    if (s + 2 < trips) one(st2, st1, s + 2);
   } else {
-    for (; s + 2 < nk; s += 3) {
+    for (; s + 2 < trips; s += 3) {
       one(st0, st2, s);
       one(st1, st0, s + 1);
       one(st2, st1, s + 2);
     }
-    if (s < nk) one(st0, st2, s);
-    if (s + 1 < nk) one(st1, st0, s + 1);
+    if (s < trips) one(st0, st2, s);
+    if (s + 1 < trips) one(st1, st0, s + 1);
+  }
+  if constexpr (H == 2) {
+    static_assert(4 * NJ * 4096 <= H * kStage, "the second half's sums fit a stage");
+    __builtin_amdgcn_s_waitcnt(0);  // the repeated loads past the last step
+    __syncthreads();
+    gdn::f32x4_t* red = reinterpret_cast<gdn::f32x4_t*>(st0) + (threadIdx.x & 255);
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int j = 0; j < NJ; ++j)
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+          if (half) red[256 * ((i * NJ + j) * 2 + t)] = acc[i][j][t];
+    __syncthreads();
+    if (half) return;
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int j = 0; j < NJ; ++j)
+#pragma unroll
+        for (int t = 0; t < 2; ++t) acc[i][j][t] += red[256 * ((i * NJ + j) * 2 + t)];
   }
 #pragma unroll
   for (int i = 0; i < 2; ++i)
@@ -1032,7 +1061,7 @@ __global__ __launch_bounds__(kFp8Threads, 2) void gemm_fp8_deep_kernel(const uin
 // bf16 rows has the bits of gdn_quantize_fp8 and a call from e4m3 ones.  (Four waves of
 // three stages for kRing16x32: 1 x 2048 3.6 us against 3.8, 64 x 2048 x 4096 4.8 / 5.1.)
 enum Fp8Kernel {
-  kPP, kDeep64, kDeep128, kRing16x32, kRing16x64, kRing32x32, kRing64x32,
+  kPP, kDeep64, kDeep128, kDeep64x2, kRing16x32, kRing16x64, kRing32x32, kRing64x32,
   kRingQ16x32, kRingQ16x64, kRows16x32, kRows16x64
 };
 
@@ -1062,6 +1091,9 @@ Fp8Kernel fp8_plan(int M, int N, int K, bool quant) {
   if (M <= 16 && blocks(16, 64) <= kCUs8) return kRing16x64;
   if (blocks(32, 32) <= kCUs8) return kRing32x32;
   if (blocks(64, 32) <= kCUs8) return kRing64x32;
+  // At most one 64 x 64 tile per CU, in two halves of K: 512 x 2048 x 4096 9.8 us (whole 11.4),
+  // 512 x 2048 7.0 (7.5), 128 x 8192 7.2 (7.7); 300 x 2048 x 512 4.8 (4.3).
+  if (blocks(64, 64) <= kCUs8 && K >= 2048) return kDeep64x2;
   // Up to two 64 x 64 tiles per CU: 200 x 8192 8.5 us (64 x 128 tiles 10.4, 128 x 128
   // blocks 13.1), 1024 x 2048 9.0 (10.3, 13.2), 128 x 12288 8.6 (10.3, 13.3); with three
   // 256 x 12288 14.5 (12.4, 14.3).
@@ -1099,14 +1131,15 @@ int fp8_launch(Fp8Kernel kernel, const void* A, int64_t lda, const uint8_t* B, i
                                                                  static_cast<int>(whole));
       break;
     }
-    case kDeep64:
-      gemm_fp8_deep_kernel<64, 4><<<grid(blocks(64, 64)), dim3(kFp8Threads), 0, st>>>(A8, lda, B, ldb, sc, out, M, N,
-                                                                                     K);
-      break;
-    case kDeep128:
-      gemm_fp8_deep_kernel<128, 3><<<grid(blocks(64, 128)), dim3(kFp8Threads), 0, st>>>(A8, lda, B, ldb, sc, out, M,
-                                                                                       N, K);
-      break;
+#define GDN_DEEP(name, BN, NS, H)                                                                                       \
+  case name:                                                                                                           \
+    gemm_fp8_deep_kernel<BN, NS, H><<<grid(blocks(64, BN)), dim3(kFp8Threads * H), 0, st>>>(A8, lda, B, ldb, sc, out, M, \
+                                                                                           N, K);                      \
+    break
+      GDN_DEEP(kDeep64, 64, 4, 1);
+      GDN_DEEP(kDeep128, 128, 3, 1);
+      GDN_DEEP(kDeep64x2, 64, 4, 2);
+#undef GDN_DEEP
 #define GDN_RING(name, BM, BN, NW, NS, Q)                                                                            \
   case name:                                                                                                         \
     gemm_fp8_ring_kernel<BM, BN, NW, NS, Q>                                                                          \

@@ -94,7 +94,7 @@ def _check(y, want, slack, tag):
 SHAPES = [(1, 1, 128), (1, 2048, 2048), (1, 12288, 2048), (3, 200, 128), (16, 256, 384), (17, 2048, 4096),
           (33, 72, 640), (37, 8192, 2048), (64, 1000, 1152), (65, 130, 2048), (100, 520, 4992), (129, 2048, 2048),
           (200, 12288, 2048), (256, 2048, 4096), (257, 384, 256), (300, 8192, 2048), (511, 513, 896),
-          (700, 4096, 2048), (1024, 12288, 2048), (1025, 2048, 1920), (2049, 2048, 2048), (4100, 333, 640)]
+          (400, 2048, 4096), (129, 3000, 2176), (500, 2000, 2304), (65, 8192, 2048), (700, 4096, 2048), (1024, 12288, 2048), (1025, 2048, 1920), (2049, 2048, 2048), (4100, 333, 640)]
 
 
 @pytest.mark.parametrize("M,N,K", SHAPES)
