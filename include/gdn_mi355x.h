@@ -520,7 +520,8 @@ int gdn_decode_fp8(const uint16_t* q, int64_t sq_b, const uint16_t* k, int64_t s
  * ppp the ancestors, past the root the pool's taps from the newest: gdn_conv_decode's
  * arithmetic along each path.  x [B, T, C] bf16 strides x_b, x_t (multiples of 8, x_t
  * below 2^24), pool as
- * gdn_conv_decode, w [C, 4], y [B, T, C] contiguous; last_x like x with last_T nodes.
+ * gdn_conv_decode, w [C, 4], y [B, T, C] contiguous; last_x like x with last_T nodes.  B
+ * below 65536, C a multiple of 8 below 2^23.
  */
 int gdn_conv_tree(const uint16_t* x, int64_t x_b, int64_t x_t, uint16_t* pool, int64_t sp_slot, int64_t sp_ch,
                   int64_t n_slots, const int64_t* ids, const uint16_t* w, const int32_t* parents, int64_t p_b,
@@ -538,7 +539,8 @@ int gdn_conv_tree(const uint16_t* x, int64_t x_b, int64_t x_t, uint16_t* pool, i
  *   q, k [B, T, Hk, D], v [B, T, Hv, D] bf16, strides per sequence and token (multiples of
  *   8, the token's below 2^24; head stride D); g [B, T, Hv] fp32 and beta [B, T, Hv] bf16 contiguous; s_pool, s_slot
  *   as gdn_recurrent; o [B, T, Hv, D] bf16 and u [B, T, Hv, D] fp32 contiguous; last_k,
- *   last_g, last_u: k, g and u of the step before (last_T nodes).  D 64 or 128.
+ *   last_g, last_u: k, g and u of the step before (last_T nodes).  D 64 or 128, B Hv below
+ *   2^24, Hv D below 2^23.
  */
 int gdn_rule_tree(const uint16_t* q, int64_t q_b, int64_t q_t, const uint16_t* k, int64_t k_b, int64_t k_t,
                   const uint16_t* v, int64_t v_b, int64_t v_t, const float* g, const uint16_t* beta, float* s_pool,

@@ -651,3 +651,39 @@ def test_quick_and_checked_calls_agree(pkg, dev, monkeypatch):
     torch.cuda.synchronize()
     assert got[1] == want[1] and got[2] == want[2]
     assert all(torch.equal(p, r) for p, r in zip(got[0], want[0]))
+
+
+def test_slots_past_four_gigabytes(pkg, dev):
+    """Slots whose bytes begin past 2^32 (and past 2^31 values): the results of the same slots in
+    small pools."""
+    gen = torch.Generator().manual_seed(67)
+    B, T, Hk, Hv, D = 2, 5, 16, 32, 128
+    C = 2 * Hk * D + Hv * D
+    slots = [2 ** 32 // (4 * Hv * D * D) + 3, 2 ** 32 // (2 * 3 * C) + 3]
+    i, last = _inputs(gen, B, T, Hk, Hv, D), _inputs(gen, B, T, Hk, Hv, D)
+    parents, accepted = ref.tree(gen, B, T, 2)
+    accepted[:] = torch.tensor([3, 2])
+    dv = lambda *ts: tuple(t.to(dev) for t in ts)  # noqa: E731
+    parents, accepted = dv(parents, accepted)
+    S = torch.randn(B, Hv, D, D, generator=gen) * 0.3
+    taps = torch.randn(B, C, 3, generator=gen).to(BF16)
+    w = torch.randn(C, 4, generator=gen).to(BF16).to(dev)
+    lk = _qkv(last["y"].to(dev), Hk, Hv, D)[1]
+    kk = _qkv(i["y"].to(dev), Hk, Hv, D)
+    lx, lg, lu, x, g, beta = dv(last["x"], last["g"], last["u"], i["x"], i["g"], i["beta"])
+    results = []
+    for far in (False, True):
+        n = slots if far else [B, B]
+        s_pool = torch.zeros(n[0], Hv, D, D, device=dev)
+        c_pool = torch.zeros(n[1], C, 3, dtype=BF16, device=dev)
+        s_ids, c_ids = (torch.arange(m - B, m, device=dev) for m in n)
+        s_pool[s_ids], c_pool[c_ids] = dv(S, taps)
+        y = pkg.conv_tree_step(x, c_pool, c_ids, w, parents, pending=(lx, parents, accepted))
+        o, u = pkg.recurrent_gdn_tree(*kk, g, beta, s_pool, s_ids, parents, pending=(lk, lg, lu, parents, accepted))
+        pkg.commit_tree(s_pool, c_pool[:n[0]], s_ids, parents, accepted, x, kk[1], g, u)
+        results.append([t.cpu() for t in (y, o, u, s_pool[s_ids], c_pool[c_ids], c_pool[s_ids])])
+        if far:
+            assert not s_pool[:8].any() and not c_pool[:8].any()
+        del s_pool, c_pool
+    near, far = results
+    assert all(torch.equal(a, b) for a, b in zip(near[:4], far[:4]))
