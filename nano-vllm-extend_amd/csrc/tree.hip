@@ -18,6 +18,7 @@
 // left out, not multiplied: a node sees nothing of what its path has forgotten, nor of
 // unused nodes and other branches, infinities and NaN included.
 #include <algorithm>
+#include <type_traits>
 
 #include "gdn_common.h"
 
@@ -334,7 +335,7 @@ __global__ __launch_bounds__(64 * W) void conv_tree_kernel(const uint16_t* __res
 // The nodes' rows are loaded once, 8 values per lane ahead of the state, and go to LDS, where
 // the coefficients (k_s . k_t, k_s . q_t, 16 x 16 nodes at a time, dealt to the waves) and the
 // products with the state find them.  (Rows read by each wave from the caches: 64 x 64 nodes
-// 120 us for 103, 1 x 64 21.4 for 17.8, 64 x 16 without a pending path 37.1 for 33.4.)
+// 120 us for 99, 1 x 64 21.4 for 17.7, 64 x 16 without a pending path 37.1 for 33.4.)
 //
 // The corrections u of 16 nodes are the product of the inverse of their 16 x 16 triangle
 // (found by substitution while the state is on its way) with what the state, v and the
@@ -352,10 +353,10 @@ __global__ __launch_bounds__(64 * W) void conv_tree_kernel(const uint16_t* __res
 // weights, the nodes' norms and dot products (on the matrix cores as well) and the
 // pending path's rows are worked on while the state is on its way.  32 heads of 128: 64
 // trees of 16 nodes with a pending path 57.5 us (5.5 TB/s, a large copy's rate), without one
-// 33.4; 30 trees of 24 nodes 33.7, 16 of 48 24.5; one tree of 8 nodes 6.6, the latency of its
+// 33.4; 30 trees of 24 nodes 33.5, 16 of 48 24.0; one tree of 8 nodes 6.6, the latency of its
 // chain (ids, state, products, corrections).  64 nodes cost more than the state (64 trees
-// 103 us, one 17.8: coefficients 4.3, products 2.2, corrections 3.3), and so do long paths: 21
-// chains of 48 70 us, each row of the path a pass of the vector ALUs over the tile.
+// 99 us, one 17.7: coefficients 4, products 2.2, corrections 3.3), and so do long paths: 21
+// chains of 48 69 us, each row of the path a pass of the vector ALUs over the tile.
 // Before: a thread per column of the state and one node at a time 249 us (64 x 16) and
 // 32 (1 x 8).
 typedef float f32x2_t __attribute__((ext_vector_type(2)));
@@ -738,10 +739,15 @@ __global__ __launch_bounds__(2 * D, D == 128 ? (NT <= 2 ? 3 : 2) : NT == 1 ? 3 :
   // + r, s = 16 J + lr.  A weight of 0 is not multiplied: nothing of an unused node, of
   // another branch or past T gets in.
   auto frag = [&](int row, int kk) { return *reinterpret_cast<const gdn::s16x8_t*>(&kq[row][32 * kk + 8 * lg]); };
-  auto coefficients = [&](int I, int J, bool out) {  // of u_s in o_t, else in u_t
-    gdn::f32x4_t c = {0.f, 0.f, 0.f, 0.f};
+  // of u_s in u_t, in o_t, or in both
+  auto coefficients = [&](int I, int J, auto in_u, auto in_o) {
+    gdn::f32x4_t c = {0.f, 0.f, 0.f, 0.f}, d = c;
 #pragma unroll
-    for (int kk = 0; kk < KK; ++kk) c = gdn::mfma16x16x32(frag((out ? TM : 0) + 16 * I + lr, kk), frag(16 * J + lr, kk), c);
+    for (int kk = 0; kk < KK; ++kk) {
+      const gdn::s16x8_t key = frag(16 * J + lr, kk);
+      if constexpr (in_u.value) c = gdn::mfma16x16x32(frag(16 * I + lr, kk), key, c);
+      if constexpr (in_o.value) d = gdn::mfma16x16x32(frag(TM + 16 * I + lr, kk), key, d);
+    }
     const int s = 16 * J + lr;
     const float rs = rk[s];
     bool some = false;
@@ -750,18 +756,19 @@ __global__ __launch_bounds__(2 * D, D == 128 ? (NT <= 2 ? 3 : 2) : NT == 1 ? 3 :
       const int t = 16 * I + 4 * lg + r;
       const float w = wt[tile(I, J)][4 * lg + r][lr];
       const bool on = w != 0.0f && link[t] != kUnused;
-      if (out) {
-        co[tile(I, J)][4 * lg + r][lr] = on ? (scale * rq[t]) * (rs * w) * c[r] : 0.0f;
-      } else {
+      if constexpr (in_o.value) co[tile(I, J)][4 * lg + r][lr] = on ? (scale * rq[t]) * (rs * w) * d[r] : 0.0f;
+      if constexpr (in_u.value) {
         cu[tile(I, J)][4 * lg + r][lr] = on && s < t ? -(bt[t] * rk[t]) * (rs * w) * c[r] : 0.0f;
         some |= on && s < t;
       }
     }
-    if (!out) {
+    if constexpr (in_u.value) {
       some = __any(some);
       if (lane == 0) any_cu[I][J] = some;
     }
   };
+  constexpr std::true_type yes;
+  constexpr std::false_type no;
   // the inverse of a triangle by substitution: lane (lr, lg) rows 4 lg .. + 3 of its column lr;
   // four rows at a time are finished and handed to the later ones (in few registers: the state
   // is on its way into most of them)
@@ -797,14 +804,13 @@ __global__ __launch_bounds__(2 * D, D == 128 ? (NT <= 2 ? 3 : 2) : NT == 1 ? 3 :
 #pragma unroll 1
   for (int I = 0; I < NT; ++I) {
     if (wave == NW - 1 - I % NW) {
-      coefficients(I, I, false);
+      coefficients(I, I, yes, no);
       invert(I);
     }
 #pragma unroll 1
-    for (int J = 0; J <= I; ++J) {
-      if (J < I && turn++ % NW == wave) coefficients(I, J, false);
-      if (turn++ % NW == wave) coefficients(I, J, true);
-    }
+    for (int J = 0; J < I; ++J)
+      if (turn++ % NW == wave) coefficients(I, J, yes, yes);
+    if (turn++ % NW == wave) coefficients(I, I, no, yes);
   }
 
   // --- the state after the pending path; its products with the nodes' rows ---
