@@ -64,7 +64,7 @@ struct Fp8Scales {
 // 16384 x 12288 x 2048 363 us (2.27 PFLOP/s; the library's product with one scale for each
 // operand 399), 8192^3 418 us (2.63 PFLOP/s; library 2.65), 17001 x 2048 x 2048 70-75 us.  Bound
 // by power (the clock falls to 1.6-2.0 GHz), no LDS conflicts; for 17001 x 2048 by 536 tiles
-// in rounds of 256.  The 16 spilled registers that a first form reloaded between tiles, each
+// in rounds of 256.  The 12 spilled registers that a first form reloaded between tiles, each
 // behind a wait for every load and store in flight, cost 385, 432 and 79 us.  Not kept:
 // row-block groups of 2, 8 and 16 (4 is 1-3 % faster), non-temporal stores (slower), a tile's
 // first sections that do not wait for the stores of the tile before (no faster).
