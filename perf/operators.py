@@ -30,6 +30,7 @@ import torch
 own = False
 
 HK = 16          # key heads
+HIDDEN = 2048
 LAYERS = 2       # layers in a pool; the calls use the last one
 EPS = 1e-6
 BF16, F32, F64 = torch.bfloat16, torch.float32, torch.float64
@@ -198,14 +199,8 @@ def run(state):
     return (_own if own else _plain)[state["op"]](state)
 
 
-_package = None
-
-
 def _ops():
-    global _package
-    if _package is None:    # (a program imports it once)
-        _package = importlib.import_module("nano-vllm-extend_amd")
-    return _package.ops
+    return importlib.import_module("nano-vllm-extend_amd").ops
 
 
 def _own_linear(s):
