@@ -134,19 +134,22 @@ struct Taps {
         for (int j = 0; j < 3; ++j) p[i * sp_ch + j] = tap[j].v[i];
     }
   }
-  __device__ __forceinline__ const Row8& before(int r) const {  // r in -1, -2, -3
-    return r == -1 ? tap[2] : r == -2 ? tap[1] : tap[0];
-  }
-  // The taps after the accepted node: its row, its parent's and its grandparent's.
-  __device__ __forceinline__ void advance(const ConvPending& pd, int b, int c, int a, int link) {
+  // The taps after the accepted node: its row (a), its parent's (r1) and its grandparent's (r0),
+  // each a node or, below 0, one of the taps.
+  __device__ __forceinline__ void advance(const ConvPending& pd, int b, int c, int a, int r1, int r0) {
     const uint16_t* x = pd.x + b * pd.x_b + c;
-    const int r1 = row_before(a, link), r0 = row_before(r1, link);
-    const Row8 n2 = row8(x + a * pd.x_t);
-    const Row8 n1 = r1 >= 0 ? row8(x + r1 * pd.x_t) : before(r1);
-    const Row8 n0 = r0 >= 0 ? row8(x + r0 * pd.x_t) : before(r0);
-    tap[0] = n0;
-    tap[1] = n1;
-    tap[2] = n2;
+    // (masks: a choice among the taps becomes one among their addresses, with all of them in memory)
+    typedef uint32_t words __attribute__((ext_vector_type(4)));
+    const words t0 = __builtin_bit_cast(words, tap[0]), t1 = __builtin_bit_cast(words, tap[1]),
+                t2 = __builtin_bit_cast(words, tap[2]);
+    auto row = [&](int r) {
+      words v = (t2 & (r == -1 ? ~0u : 0u)) | (t1 & (r == -2 ? ~0u : 0u)) | (t0 & (r == -3 ? ~0u : 0u));
+      if (r >= 0) v = *reinterpret_cast<const words*>(x + r * pd.x_t);
+      return __builtin_bit_cast(Row8, v);
+    };
+    tap[0] = row(r0);
+    tap[1] = row(r1);
+    tap[2] = row(a);
   }
 };
 
@@ -1048,13 +1051,16 @@ __global__ __launch_bounds__(2 * D) void commit_tree_kernel(float* __restrict__ 
     int link = cd.parents[b * cd.p_b + min(lane, cd.T - 1)], none = kUnused;
     tree_links(lane, cd.T, link, 0, none);
     const int a = accepted_node(cd.accepted[b], cd.T, link);
+    if (a < 0) return;
+    // (the path's rows while every lane, and with it every node's link, is there)
+    const int r1 = row_before(a, link), r0 = row_before(r1, link);
     const int c0 = (at % parts * 2 * D + tid) * 8;
-    if (c0 >= C || a < 0) return;
+    if (c0 >= C) return;
     uint16_t* p = cpool + slot * sp_slot + c0 * sp_ch;
     const bool dense = dense_taps(cpool, sp_slot, sp_ch);
     Taps taps;
     taps.load(p, sp_ch, dense);
-    taps.advance(cd, b, c0, a, link);
+    taps.advance(cd, b, c0, a, r1, r0);
     taps.store(p, sp_ch, dense);
     return;
   }

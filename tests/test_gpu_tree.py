@@ -687,3 +687,27 @@ def test_slots_past_four_gigabytes(pkg, dev):
         del s_pool, c_pool
     near, far = results
     assert all(torch.equal(a, b) for a, b in zip(near[:4], far[:4]))
+
+
+@pytest.mark.parametrize("C,T,accepted", [(192, 64, 63), (200, 40, 35), (8, 34, 33), (264, 64, 50)])
+@pytest.mark.parametrize("taps", [3, 4])                      # (channels' taps side by side, and apart)
+def test_commit_of_few_channels_and_far_nodes(pkg, dev, C, T, accepted, taps):
+    """The accepted node and its path lie past the lanes that have channels: the taps bit for bit."""
+    gen = torch.Generator().manual_seed(C + T)
+    B, Hk, Hv, D = 3, 1, 1, 64
+    n = lambda *s: torch.randn(*s, generator=gen)  # noqa: E731
+    x, cpool = n(B, T, C).to(BF16), n(B, C, taps).to(BF16)
+    k, g, u = n(B, T, Hk, D).to(BF16), -n(B, T, Hv).abs(), n(B, T, Hv, D)
+    pool = n(B, Hv, D, D)
+    parents = torch.arange(-1, T - 1, dtype=torch.int32).expand(B, T).clone()
+    parents[1, accepted] = accepted - 3
+    parents[2, accepted] = -1                                 # (a root: two of the old taps stay)
+    nodes = torch.full((B,), accepted)
+    cd = cpool.to(dev)
+    pkg.commit_tree(pool.to(dev), cd[..., :3], torch.arange(B, device=dev), parents.to(dev), nodes.to(dev), x.to(dev),
+                    k.to(dev), g.to(dev), u.to(dev))
+    torch.cuda.synchronize()
+    want = cpool.clone()
+    for b in range(B):
+        want[b, :, :3] = ref.taps_after(cpool[b, :, :3], x[b], parents[b], accepted)
+    assert torch.equal(cd.cpu().view(torch.int16), want.view(torch.int16))
