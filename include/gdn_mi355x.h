@@ -26,7 +26,7 @@
 extern "C" {
 #endif
 
-#define GDN_ABI_VERSION 6
+#define GDN_ABI_VERSION 7
 
 #define GDN_OK 0
 #define GDN_ERR_INVALID_ARG (-1) /* shape / stride / pointer rejected */
@@ -37,8 +37,14 @@ extern "C" {
  * (one per GPU, held until the process ends). */
 #define GDN_NOALLOC_SCRATCH_BYTES (128LL << 20)
 
+/* In the place of the stream of gdn_conv_tree, gdn_rule_tree, gdn_rule_tree_layer,
+ * gdn_commit_tree and gdn_rmsnorm_gated_fp8: the arguments are checked as the call would, and
+ * nothing is launched.  For calls of which all or none are to be made: gdn_conv_tree moves the
+ * conv pool on, and what gdn_rule_tree refuses after it would leave the two pools a step apart. */
+#define GDN_CHECK_ONLY ((void*)-1)
+
 /* ABI version of the loaded library (GDN_ABI_VERSION; 5 added gdn_decode_step, 6 the
- * 8-bit projections and the tree verify). */
+ * 8-bit projections and the tree verify, 7 GDN_CHECK_ONLY). */
 int gdn_abi_version(void);
 
 /*

@@ -17,9 +17,10 @@ from pathlib import Path
 import torch  # noqa: F401  (loads the HIP runtime the library binds to)
 
 LIB_PATH = Path(os.environ.get("GDN_MI355X_LIB", Path(__file__).resolve().parent / "lib" / "libgdn_mi355x.so"))
-ABI_VERSION = 6
+ABI_VERSION = 7
 
 GDN_OK = 0
+CHECK_ONLY = -1   # in a stream's place: the arguments are checked, nothing is launched
 GDN_ERR_INVALID_ARG = -1
 GDN_ERR_UNSUPPORTED = -2
 GDN_ERR_SCRATCH = -3

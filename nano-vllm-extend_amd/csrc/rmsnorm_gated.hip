@@ -207,6 +207,7 @@ extern "C" int gdn_rmsnorm_gated_fp8(const uint16_t* x, int64_t sx_tok, const ui
   const int G = H * D / gdn::kFp8Group;
   const int64_t nb = (n_tok + 15) / 16 * G;
   if (nb >= (1LL << 31)) return GDN_ERR_UNSUPPORTED;
+  if (stream == GDN_CHECK_ONLY) return GDN_OK;
   const dim3 grid(static_cast<unsigned>(nb)), block(256);
   hipStream_t s = static_cast<hipStream_t>(stream);
   if (D == 128)

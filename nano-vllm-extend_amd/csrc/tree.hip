@@ -1129,6 +1129,7 @@ template <bool kLayer>
 int rule_launch(const RuleRows& r, const float* g, const uint16_t* beta, float* s_pool, int64_t s_slot, int64_t n_slots,
                 const int64_t* ids, const int32_t* parents, int64_t p_b, const RulePending& pd, uint16_t* o, float* u,
                 int B, int T, int Hk, int Hv, int D, float scale, const TreeLayer& layer, void* stream) {
+  if (stream == GDN_CHECK_ONLY) return GDN_OK;
   const dim3 grid(static_cast<unsigned>(gdn::kNumXcd * ((B * Hv + gdn::kNumXcd - 1) / gdn::kNumXcd)));
   hipStream_t st = static_cast<hipStream_t>(stream);
 #define GDN_RULE(DD, NT)                                                                                           \
@@ -1159,6 +1160,7 @@ extern "C" int gdn_conv_tree(const uint16_t* x, int64_t x_b, int64_t x_t, uint16
     return GDN_ERR_INVALID_ARG;
   if (accepted && (!rows_ok(last_x, lx_b, lx_t, C, last_T) || !last_parents || lp_b < 0)) return GDN_ERR_INVALID_ARG;
   if (B > 65535) return GDN_ERR_UNSUPPORTED;
+  if (stream == GDN_CHECK_ONLY) return GDN_OK;
   const ConvPending pd{last_x, lx_b, lx_t, last_parents, lp_b, accepted, last_T};
   const dim3 grid((C + 127) / 128, B);
   const int lds = ((T + 3) / 4 * 4 + 3) * 256;
@@ -1228,6 +1230,7 @@ extern "C" int gdn_commit_tree(float* s_pool, int64_t s_slot, uint16_t* conv_poo
       reinterpret_cast<uintptr_t>(u) % 16)
     return GDN_ERR_INVALID_ARG;
   if (static_cast<int64_t>(B) * (Hv + (C + D - 1) / D) >= (1LL << 24)) return GDN_ERR_UNSUPPORTED;
+  if (stream == GDN_CHECK_ONLY) return GDN_OK;
   const RulePending pd{k, k_b, k_t, g, u, parents, p_b, accepted, T};
   const ConvPending cd{x, x_b, x_t, parents, p_b, accepted, T};
   // (the conv workgroups after the states')

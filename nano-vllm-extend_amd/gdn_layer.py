@@ -285,32 +285,22 @@ class GatedDeltaNetCore:
         parents [B, T] or [T] (ops.conv_tree_step); the pools' rows ids [B] are
         read, and stay, except that pending (the step before, with its accepted
         nodes) goes into them first.  Returns (core [B, T, Hv, D] bf16, or with fp8
-        its (e4m3, scales) as the 8-bit out projection reads it; TreeStep)."""
+        its (e4m3, scales) as the 8-bit out projection reads it; TreeStep).  A call
+        that is refused leaves both pools as they were."""
         self._to(mixed.device)
         if not self.sw.gbeta or not self.sw.conv_kernel or self.K != 4:
             raise NotImplementedError("verify_tree runs the gate and conv kernels (conv width 4) only")
         if pending is not None and pending.accepted is None:
             raise ValueError("pending has no accepted nodes: accept() follows each verify")
-        B, T, _ = mixed.shape
-        Hk, Hv, D, kd = self.Hk, self.Hv, self.D, self.key_dim
         last_conv = last_rule = None
         if pending is not None:
             last_conv = (pending.x, pending.parents, pending.accepted)
             last_rule = (pending.k, pending.g, pending.u, pending.parents, pending.accepted)
-        with self._timed("conv_tree"):
-            y = ops.conv_tree_step(mixed, conv_cache, ids, self.conv_w, parents, pending=last_conv)
-        q, k, v = (y[..., :kd].unflatten(-1, (Hk, D)), y[..., kd:2 * kd].unflatten(-1, (Hk, D)),
-                   y[..., 2 * kd:].unflatten(-1, (Hv, D)))
-        if not fp8 or D == ops.FP8_GROUP:
-            with self._timed("recurrent_tree"):
-                out, u, g = ops.recurrent_tree_fused(q, k, v, b, a, self.A_log, self.dt_bias, z, self.norm_w, s_cache,
-                                                     ids, parents, self.eps, pending=last_rule, fp8=fp8)
-            return out, TreeStep(mixed, k, g, u, parents)
-        # (heads of 64: two share a scale, which the fused norm does not see)
-        g, beta = self._g_beta(b.contiguous(), a.contiguous(), None)
-        with self._timed("recurrent_tree"):
-            o, u = ops.recurrent_gdn_tree(q, k, v, g, beta, s_cache, ids, parents, pending=last_rule)
-        return self._norm_fp8(o, z.reshape(B, T, Hv, D)), TreeStep(mixed, k, g, u, parents)
+        out, k, u, g = ops._verify_tree(
+            mixed, conv_cache, self.conv_w, b, a, self.A_log, self.dt_bias, z, self.norm_w, s_cache, ids, parents,
+            self.Hk, self.Hv, self.D, self.eps, last_conv, last_rule, fp8,
+            lambda: self._g_beta(b.contiguous(), a.contiguous(), None), None if self.timer is None else self._timed)
+        return out, TreeStep(mixed, k, g, u, parents)
 
     def commit_tree(self, step: TreeStep, ids, conv_cache, s_cache) -> None:
         """The accepted paths of a verify step into both pools, for another user of

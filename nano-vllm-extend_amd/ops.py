@@ -9,6 +9,7 @@ CPU or eager fallback: a CPU tensor or a missing library raises.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import functools
 import os
@@ -75,6 +76,24 @@ def _launch_on(idx: int, name: str, words: bytes) -> None:
     else:
         with torch.cuda.device(idx):
             _lib.call_words(name, words)
+
+
+class _Ready:
+    """A call whose arguments are checked and whose outputs are there: launch() makes it.  keep: the
+    tensors that the arguments point into."""
+    __slots__ = ("idx", "name", "args", "out", "keep")
+
+    def __init__(self, idx, name, args, out, keep):
+        self.idx, self.name, self.args, self.out, self.keep = idx, name, args, out, keep
+
+    def check(self):
+        """What the entry point itself would refuse, without a launch."""
+        pack, head = _lib.WORDS[self.name]
+        _lib.call_words(self.name, pack(head, *self.args, _lib.CHECK_ONLY))
+
+    def launch(self):
+        _call_on(self.idx, self.name, *self.args)
+        return self.out
 
 
 # (0.2 us cheaper than the public call, which checks that CUDA is initialised: a tensor on
@@ -961,8 +980,11 @@ def conv_tree_step(x: torch.Tensor, conv_pool: torch.Tensor, ids: torch.Tensor, 
     (No reference counterpart: spec decode is disabled for qwen3_5,
     nanovllm/config.py:84.)"""
     y = _lib.quick().conv_tree(x, conv_pool, ids, weight, parents, pending)
-    if y is not None:
-        return y
+    return y if y is not None else _conv_tree_ready(x, conv_pool, ids, weight, parents, pending).launch()
+
+
+def _conv_tree_ready(x, conv_pool, ids, weight, parents, pending, y=None) -> _Ready:
+    """conv_tree_step's call, checked; y: a contiguous tensor that takes the result."""
     last_x, last_parents, accepted = pending if pending is not None else (None, None, None)
     idx = _device_of(x, conv_pool, ids, weight, parents, last_x, last_parents, accepted)
     if x.dim() != 3:
@@ -983,10 +1005,11 @@ def conv_tree_step(x: torch.Tensor, conv_pool: torch.Tensor, ids: torch.Tensor, 
         last_parents, lp_b = _tree_parents(last_parents, B, last_T)
         accepted = _tree_ids(accepted, B, "accepted")
         last = (last_x.data_ptr(), lx_b, lx_t, last_parents.data_ptr(), lp_b, accepted.data_ptr(), last_T)
-    y = x.new_empty(shape)
-    _call_on(idx, "gdn_conv_tree", x.data_ptr(), x_b, x_t, conv_pool.data_ptr(), pool_st[0], pool_st[1],
-             conv_pool.shape[0], ids.data_ptr(), w.data_ptr(), par.data_ptr(), p_b, *last, y.data_ptr(), B, T, C)
-    return y
+    if y is None:
+        y = x.new_empty(shape)
+    args = (x.data_ptr(), x_b, x_t, conv_pool.data_ptr(), pool_st[0], pool_st[1], conv_pool.shape[0], ids.data_ptr(),
+            w.data_ptr(), par.data_ptr(), p_b, *last, y.data_ptr(), B, T, C)
+    return _Ready(idx, "gdn_conv_tree", args, y, (x, ids, w, par, last_x, last_parents, accepted))
 
 
 def _rule_args(q, k, v, s_pool, ids, parents, pending):
@@ -1041,8 +1064,11 @@ def recurrent_gdn_tree(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: tor
     (No reference counterpart: spec decode is disabled for qwen3_5,
     nanovllm/config.py:84; one token: qwen3_5.py:575-594.)"""
     out = _lib.quick().rule_tree(q, k, v, g, beta, s_pool, ids, parents, pending)
-    if out is not None:
-        return out
+    return out if out is not None else _rule_tree_ready(q, k, v, g, beta, s_pool, ids, parents, pending).launch()
+
+
+def _rule_tree_ready(q, k, v, g, beta, s_pool, ids, parents, pending) -> _Ready:
+    """recurrent_gdn_tree's call, checked."""
     idx = _device_of(k, q, v, g, beta, s_pool, ids, parents, *(pending or ()))
     dims, rows, state, keep = _rule_args(q, k, v, s_pool, ids, parents, pending)
     B, T, Hk, Hv, D = dims
@@ -1054,9 +1080,8 @@ def recurrent_gdn_tree(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: tor
     if not beta.is_contiguous():
         beta = beta.contiguous()
     o, u = v.new_empty(v_shape), g.new_empty(v_shape)
-    _call_on(idx, "gdn_rule_tree", *rows, g.data_ptr(), beta.data_ptr(), *state, o.data_ptr(), u.data_ptr(), *dims,
-             D ** -0.5)
-    return o, u
+    args = (*rows, g.data_ptr(), beta.data_ptr(), *state, o.data_ptr(), u.data_ptr(), *dims, D ** -0.5)
+    return _Ready(idx, "gdn_rule_tree", args, (o, u), (g, beta, keep))
 
 
 def recurrent_tree_fused(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, b: torch.Tensor, a: torch.Tensor,
@@ -1074,6 +1099,13 @@ def recurrent_tree_fused(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, b: t
     if out is not None:
         y, scale, u, g = out
         return (y, scale) if fp8 else y, u, g
+    return _rule_tree_layer_ready(q, k, v, b, a, a_log, dt_bias, z, norm_weight, s_pool, ids, parents, eps, pending,
+                                  fp8).launch()
+
+
+def _rule_tree_layer_ready(q, k, v, b, a, a_log, dt_bias, z, norm_weight, s_pool, ids, parents, eps, pending,
+                           fp8) -> _Ready:
+    """recurrent_tree_fused's call, checked."""
     idx = _device_of(k, q, v, b, a, a_log, dt_bias, z, norm_weight, s_pool, ids, parents, *(pending or ()))
     dims, rows, state, keep = _rule_args(q, k, v, s_pool, ids, parents, pending)
     B, T, Hk, Hv, D = dims
@@ -1098,10 +1130,59 @@ def recurrent_tree_fused(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, b: t
     u = v.new_empty((B, T, Hv, D), dtype=torch.float32)
     g = v.new_empty((B, T, Hv), dtype=torch.float32)
     out = (0, y.data_ptr(), scale.data_ptr()) if fp8 else (y.data_ptr(), 0, 0)
-    _call_on(idx, "gdn_rule_tree_layer", *rows, b.data_ptr(), a.data_ptr(), a_log.data_ptr(), dt_bias.data_ptr(),
-             int(a_log.dtype == torch.float32), *state, z.data_ptr(), z_b, z_t, w.data_ptr(), float(eps), *out,
-             u.data_ptr(), g.data_ptr(), *dims, D ** -0.5)
-    return (y, scale) if fp8 else y, u, g
+    args = (*rows, b.data_ptr(), a.data_ptr(), a_log.data_ptr(), dt_bias.data_ptr(), int(a_log.dtype == torch.float32),
+            *state, z.data_ptr(), z_b, z_t, w.data_ptr(), float(eps), *out, u.data_ptr(), g.data_ptr(), *dims, D ** -0.5)
+    return _Ready(idx, "gdn_rule_tree_layer", args, ((y, scale) if fp8 else y, u, g), (b, a, a_log, dt_bias, z, w, keep))
+
+
+def _verify_tree(x, conv_pool, weight, b, a, a_log, dt_bias, z, norm_weight, s_pool, ids, parents, Hk, Hv, D, eps,
+                 last_conv, last_rule, fp8, gates, timed):
+    """conv_tree_step and the rule with the layer's gates and norm (recurrent_tree_fused, or where heads
+    of 64 share a scale its three calls, gates() giving g and beta), of which all are launched or none:
+    each is checked, and all memory allocated, before the conv moves its pool on.  timed(name): a
+    context around a launch, or None.  Returns (out, k, u, g)."""
+    conv = (x, conv_pool, ids, weight, parents, last_conv)
+    layer = (b, a, a_log, dt_bias, z, norm_weight, s_pool, ids, parents, eps, last_rule, fp8)
+    fused = not fp8 or D == FP8_GROUP
+    g = beta = None
+    if not fused:
+        g, beta = gates()
+    if timed is None:
+        quick = _lib.quick()
+        if fused:
+            out = quick.verify_tree(*conv, Hk, D, *layer)
+            if out is not None:
+                y, scale, k, u, g = out
+                return (y, scale) if fp8 else y, k, u, g
+        else:
+            out = quick.verify_tree_norm(*conv, Hk, D, g, beta, s_pool, ids, parents, last_rule, z, norm_weight, eps)
+            if out is not None:
+                y, scale, k, u = out
+                return (y, scale), k, u, g
+    B, T, C = x.shape
+    kd = Hk * D
+    if C != 2 * kd + Hv * D:
+        raise ValueError(f"x must have {2 * kd + Hv * D} channels, got {C}")
+    y = x.new_empty(x.shape)
+    q, k, v = (y[..., :kd].unflatten(-1, (Hk, D)), y[..., kd:2 * kd].unflatten(-1, (Hk, D)),
+               y[..., 2 * kd:].unflatten(-1, (Hv, D)))
+    if conv_pool.shape[0] != s_pool.shape[0]:     # (a slot of one of them alone)
+        raise ValueError(f"the pools have {s_pool.shape[0]} and {conv_pool.shape[0]} slots")
+    calls = [("conv_tree", _conv_tree_ready(*conv, y))]
+    if fused:
+        calls.append(("recurrent_tree", _rule_tree_layer_ready(q, k, v, *layer)))
+        out, u, g = calls[1][1].out
+    else:
+        calls.append(("recurrent_tree", _rule_tree_ready(q, k, v, g, beta, s_pool, ids, parents, last_rule)))
+        o, u = calls[1][1].out
+        calls.append(("rmsnorm_gated", _norm_fp8_ready(o, z.reshape(B, T, Hv, D), norm_weight, eps)))
+        out = calls[2][1].out
+    for _, call in calls:
+        call.check()
+    for name, call in calls:
+        with contextlib.nullcontext() if timed is None else timed(name):
+            call.launch()
+    return out, k, u, g
 
 
 def commit_tree(s_pool: torch.Tensor, conv_pool: torch.Tensor, ids: torch.Tensor, parents: torch.Tensor,
@@ -1493,8 +1574,11 @@ def rms_norm_gated_fp8(hidden_states: torch.Tensor, gate: torch.Tensor, weight: 
     over a token's H * D columns (a multiple of 128), rounded once.  hidden_states / gate
     [..., H, D] bf16.  Returns (e4m3 [..., H, D], scales [tokens, H * D / 128] fp32)."""
     out = _lib.quick().norm_fp8(hidden_states, gate, weight, eps)
-    if out is not None:
-        return out
+    return out if out is not None else _norm_fp8_ready(hidden_states, gate, weight, eps).launch()
+
+
+def _norm_fp8_ready(hidden_states, gate, weight, eps) -> _Ready:
+    """rms_norm_gated_fp8's call, checked."""
     idx = _device_of(hidden_states, gate, weight)
     _bf16(hidden_states, "hidden_states")
     _bf16(gate, "gate")
@@ -1512,9 +1596,9 @@ def rms_norm_gated_fp8(hidden_states: torch.Tensor, gate: torch.Tensor, weight: 
     n_tok = hidden_states.numel() // (H * D)
     y = x.new_empty(hidden_states.shape, dtype=FP8)
     scale = _fp8_scales(n_tok, H * D // FP8_GROUP, x.device)
-    _call_on(idx, "gdn_rmsnorm_gated_fp8", x.data_ptr(), x_tok, z.data_ptr(), z_tok, weight.data_ptr(), y.data_ptr(),
-             scale.data_ptr(), 1, n_tok, n_tok, H, D, float(eps))
-    return y, scale
+    args = (x.data_ptr(), x_tok, z.data_ptr(), z_tok, weight.data_ptr(), y.data_ptr(), scale.data_ptr(), 1, n_tok, n_tok,
+            H, D, float(eps))
+    return _Ready(idx, "gdn_rmsnorm_gated_fp8", args, (y, scale), (x, z, weight))
 
 
 class Qwen3_5RMSNormGated(torch.nn.Module):

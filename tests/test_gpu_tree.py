@@ -711,3 +711,48 @@ def test_commit_of_few_channels_and_far_nodes(pkg, dev, C, T, accepted, taps):
     for b in range(B):
         want[b, :, :3] = ref.taps_after(cpool[b, :, :3], x[b], parents[b], accepted)
     assert torch.equal(cd.cpu().view(torch.int16), want.view(torch.int16))
+
+
+@pytest.mark.parametrize("Hk,Hv,D,fp8,timed", [(2, 4, 128, False, False), (2, 4, 128, True, False), (2, 4, 64, True, False),
+                                               (2, 4, 128, True, True), (1, 1, 64, False, True)])
+def test_a_refused_verify_leaves_the_pools(pkg, dev, monkeypatch, Hk, Hv, D, fp8, timed):
+    """A verify whose rule is refused leaves the taps too, so that the call repeated with what was
+    wrong mended is commit_tree followed by a verify (which goes through the Python wrappers)."""
+    gen = torch.Generator().manual_seed(71 + D)
+    B, T = 3, 7
+    C = (2 * Hk + Hv) * D
+    n = lambda *s: torch.randn(*s, generator=gen).to(BF16).to(dev)  # noqa: E731
+    core = pkg.GatedDeltaNetCore(Hk, Hv, D, n(C, 4), n(Hv), n(Hv), torch.ones(D, dtype=BF16, device=dev))
+    if timed:
+        class Timer:
+            names = []
+            start = lambda self, name: self.names.append(name)  # noqa: E731
+            stop = lambda self, *a: None  # noqa: E731
+        core.timer = Timer()
+    s1, c1 = (torch.randn(B + 1, Hv, D, D, generator=gen) * 0.1).to(dev), n(B + 1, C, 3)
+    ids = torch.tensor([3, 0, 2], device=dev)
+    rows = [(n(B, T, C), n(B, T, Hv * D), n(B, T, Hv), n(B, T, Hv)) for _ in range(2)]
+    trees = [ref.tree(gen, B, T, 3) for _ in range(2)]
+    _, step = core.verify_tree(*rows[0], ids, c1, s1, trees[0][0].to(dev), fp8=fp8)
+    step.accept(torch.tensor([2, -1, T - 1], device=dev))
+    before = s1.clone(), c1.clone()
+    x, z, b, a = rows[1]
+    par = trees[1][0].to(dev)
+    whole = torch.zeros(s1.numel() + 1, device=dev)[1:].view(s1.shape)      # not 16-byte aligned: the entry point's refusal
+    wrong = pkg.TreeStep(step.x, step.k, step.g, step.u[..., :D // 2], step.parents, step.accepted)
+    for args, pending in (((x, z[..., 8:], b, a, ids, c1, s1), step), ((x, z, b.float(), a, ids, c1, s1), step),
+                          ((x, z, b, a, ids, c1, whole), step), ((x, z, b, a, ids, c1, s1[:B]), step),
+                          ((x, z, b, a, ids, c1, s1), wrong)):
+        with pytest.raises((ValueError, TypeError, RuntimeError, AssertionError)):
+            core.verify_tree(*args, par, pending=pending, fp8=fp8)
+        torch.cuda.synchronize()
+        assert torch.equal(s1, before[0]) and torch.equal(c1, before[1])
+    got, after = core.verify_tree(x, z, b, a, ids, c1, s1, par, pending=step, fp8=fp8)
+    monkeypatch.setattr(pkg._lib, "quick", lambda: _NoQuick())
+    core.commit_tree(step, ids, before[1], before[0])
+    want, other = core.verify_tree(x, z, b, a, ids, before[1], before[0], par, fp8=fp8)
+    torch.cuda.synchronize()
+    pairs = [(s1, before[0]), (c1, before[1]), (after.u, other.u), (after.k, other.k), (after.g, other.g)]
+    pairs += [(got[0].float(), want[0].float()), (got[1], want[1])] if fp8 else [(got, want)]
+    assert all(torch.equal(p, r) for p, r in pairs)
+    assert not timed or {"conv_tree", "recurrent_tree"} <= set(core.timer.names)

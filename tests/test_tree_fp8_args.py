@@ -297,3 +297,82 @@ def test_quick_calls_leave_the_rest_to_the_wrappers(pkg):
         for wrong in (0, n - 1, n + 1):
             with pytest.raises(TypeError):
                 call(*[t] * wrong)
+
+
+@pytest.mark.parametrize("D,fp8", [(128, False), (128, True), (64, False), (64, True)])
+def test_a_refused_verify_launches_nothing(pkg, monkeypatch, D, fp8):
+    """The conv of a verify step moves the conv pool on: it is not launched where a later call of the
+    same step is refused, by its wrapper or by its entry point."""
+    launched = []
+    monkeypatch.setattr(pkg.ops, "_device_of", lambda *ts: 0)
+    monkeypatch.setattr(pkg.ops, "_call_on", lambda idx, name, *a: launched.append(name))
+    none = type("Nothing", (), {"__getattr__": lambda self, name: lambda *a: None})()
+    monkeypatch.setattr(pkg._lib, "quick", lambda: none)
+    B, T, Hk, Hv, slots = 2, 5, 1, 2, 6
+    C = (2 * Hk + Hv) * D
+    n = lambda *s: torch.zeros(*s, dtype=BF16)  # noqa: E731
+    f = lambda *s: torch.zeros(*s)  # noqa: E731
+    core = pkg.GatedDeltaNetCore(Hk, Hv, D, n(C, 4), f(Hv), f(Hv), n(D))
+    core._g_beta = lambda b, a, mask: (f(*b.shape), b)
+    step = lambda **kw: pkg.TreeStep(**{**dict(x=n(B, T, C), k=n(B, T, Hk, D), g=f(B, T, Hv), u=f(B, T, Hv, D),  # noqa: E731
+                                               parents=torch.zeros(T, dtype=torch.int32)), **kw})
+    acc = torch.zeros(B, dtype=torch.int64)
+    good = dict(mixed=n(B, T, C), z=n(B, T, Hv * D), b=n(B, T, Hv), a=n(B, T, Hv), ids=torch.arange(B),
+                conv_cache=n(slots, C, 3), s_cache=f(slots, Hv, D, D), parents=torch.zeros(B, T, dtype=torch.int32),
+                pending=step().accept(acc), fp8=fp8)
+    fused = not fp8 or D == 128
+    core.verify_tree(**good)
+    assert launched == ["gdn_conv_tree", "gdn_rule_tree_layer"] if fused else \
+        launched == ["gdn_conv_tree", "gdn_rule_tree", "gdn_rmsnorm_gated_fp8"]
+    bad = dict(z=[n(B, T, Hv * D + 8), n(B, T + 1, Hv * D)], b=[n(B, T, Hv + 1)[..., 1:].float()],
+               s_cache=[f(slots, Hv, D, D).double(), f(slots, Hv + 1, D, D), f(slots, Hv, D, D).transpose(2, 3),
+                        f(slots * Hv * D * D + 1)[1:].view(slots, Hv, D, D),                # not 16-byte aligned
+                        f(slots, Hv * D * D + 2)[:, :-2].unflatten(1, (Hv, D, D)),          # slots neither
+                        f(0, Hv, D, D)],
+               pending=[step(k=n(B, T, Hk + 1, D)).accept(acc), step(u=f(B, T, Hv, D).double()).accept(acc),
+                        step(g=f(B, T + 1, Hv)).accept(acc)],
+               mixed=[n(B, T, C + 64), n(B, T, C).float()], parents=[torch.zeros(B, T + 1, dtype=torch.int32)],
+               conv_cache=[n(slots + 1, C, 3)])
+    for name, values in bad.items():
+        for value in values:
+            launched.clear()
+            with pytest.raises((ValueError, TypeError, RuntimeError)):
+                core.verify_tree(**{**good, name: value})
+            assert launched == [], name
+    small = pkg.GatedDeltaNetCore(Hk, Hv, 32, n(4 * 32, 4), f(Hv), f(Hv), n(32))     # no such head dim
+    launched.clear()
+    with pytest.raises(pkg._lib.GDNKernelError):
+        small.verify_tree(n(B, T, 4 * 32), n(B, T, Hv * 32), n(B, T, Hv), n(B, T, Hv), torch.arange(B),
+                          n(slots, 4 * 32, 3), f(slots, Hv, 32, 32), good["parents"])
+    assert launched == []
+
+
+def test_checks_without_a_launch(pkg):
+    """CHECK_ONLY in the stream's place: the entry point's own answers, for arguments that it takes as
+    well (dummy addresses: nothing is launched)."""
+    lib, _lib = pkg._lib.load(), pkg._lib
+    inv, uns, ok, only = _lib.GDN_ERR_INVALID_ARG, _lib.GDN_ERR_UNSUPPORTED, _lib.GDN_OK, ctypes.c_void_p(-1)
+    P, odd, C, slot = ctypes.c_void_p(1 << 20), ctypes.c_void_p((1 << 20) + 8), 512, 4 * 64 * 64
+    cv = lambda x=P, B=2, T=8, Cc=C: lib.gdn_conv_tree(  # noqa: E731
+        x, 8 * C, C, P, 3 * C, 3, 4, P, P, P, 8, P, 8 * C, C, P, 8, P, 8, P, B, T, Cc, only)
+    assert cv() == ok and cv(B=0) == ok and cv(x=odd) == inv and cv(T=65) == uns and cv(B=65536) == uns
+    r = lambda q=P, s=P, st=slot, T=8, Hv=4: lib.gdn_rule_tree(  # noqa: E731
+        q, 8 * 128, 128, P, 8 * 128, 128, P, 8 * 256, 256, P, P, s, st, 4, P, P, 8, P, 8 * 128, 128, P, P, P, 8, P, 8, P, P,
+        2, T, 2, Hv, 64, 1.0, only)
+    assert r() == ok and r(q=None) == inv and r(s=odd) == inv and r(st=slot + 2) == inv and r(T=65) == uns
+    f = lambda z=P, w=P, D=64: lib.gdn_rule_tree_layer(  # noqa: E731
+        P, 8 * 128, 128, P, 8 * 128, 128, P, 8 * 256, 256, P, P, P, P, 0, P, slot, 4, P, P, 8, None, 0, 0, None, None, None,
+        0, None, 0, z, 8 * 256, 256, w, 1e-6, P, None, None, P, P, 2, 8, 2, 4, D, 1.0, only)
+    assert f() == ok and f(z=None) == inv and f(w=odd) == inv and f(D=32) == uns
+    c = lambda s=P, T=8: lib.gdn_commit_tree(s, slot, P, 3 * C, 3, 4, P, P, 8, P, P, 8 * C, C, P, 8 * 128, 128, P, P, 2, T,  # noqa: E731
+                                             2, 4, 64, C, only)
+    assert c() == ok and c(s=None) == inv and c(T=65) == uns
+    n = lambda w=P, H=2: lib.gdn_rmsnorm_gated_fp8(P, 256, P, 256, w, P, P, 1, 4, 4, H, 128, 1e-6, only)  # noqa: E731
+    assert n() == ok and n(w=odd) == inv and n(H=0) == inv
+    quick, t = pkg._lib.quick(), torch.zeros(1, 2, 8, dtype=BF16)
+    for arg in (t, None, 3, (), [t]):
+        assert quick.verify_tree(*[arg] * 20) is None and quick.verify_tree_norm(*[arg] * 17) is None
+    for call, n in ((quick.verify_tree, 20), (quick.verify_tree_norm, 17)):
+        for wrong in (0, n - 1, n + 1):
+            with pytest.raises(TypeError):
+                call(*[t] * wrong)
