@@ -515,7 +515,9 @@ int gdn_decode_fp8(const uint16_t* q, int64_t sq_b, const uint16_t* k, int64_t s
  *            parent makes node t unused: its outputs are 0 and it has no effect.
  *   ids      int64 [B] slots; a sequence whose slot is outside [0, n_slots) has outputs 0
  *            and nothing of it is written.  A slot may come more than once (the dummy slot)
- *            as long as one of its rows at most has an accepted node.
+ *            as long as none of its rows has an accepted node: a row that has one writes the
+ *            slot while the others read it, and their outputs would be of the old state, of
+ *            the new one or of parts of both.
  *   accepted int64 [B] or NULL: the node of the step before, last_*, up to which its
  *            tokens were accepted.  Its path from the root goes into the pool rows first
  *            (in place), and the new tree starts from there; a value that is no used

@@ -974,8 +974,9 @@ def conv_tree_step(x: torch.Tensor, conv_pool: torch.Tensor, ids: torch.Tensor, 
 
     pending = (x, parents, accepted) of the step before, for the same sequences in
     the same rows: the rows on the path to node accepted[b] of each sequence (-1:
-    none) go into the pool first, so a slot is in ids at most once among the rows
-    with an accepted node (a padded batch's rows: id -1, or accepted -1).  Along a
+    none) go into the pool first, so the slot of a row with an accepted node is in no
+    other row (which would read it while it is written); a slot of which nothing is
+    accepted may be in several (a padded batch's rows: the dummy slot, or id -1).  Along a
     path the results are conv_decode_step's, bit for bit.  Returns y [B, T, C].
     (No reference counterpart: spec decode is disabled for qwen3_5,
     nanovllm/config.py:84.)"""

@@ -756,3 +756,32 @@ def test_a_refused_verify_leaves_the_pools(pkg, dev, monkeypatch, Hk, Hv, D, fp8
     pairs += [(got[0].float(), want[0].float()), (got[1], want[1])] if fp8 else [(got, want)]
     assert all(torch.equal(p, r) for p, r in pairs)
     assert not timed or {"conv_tree", "recurrent_tree"} <= set(core.timer.names)
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+def test_padded_rows_share_a_slot_of_which_nothing_is_accepted(pkg, dev, fp8):
+    """The rows of a padded batch on the dummy slot, between rows that commit their last step: the
+    slot stays, and every row's outputs are those that it has alone."""
+    gen = torch.Generator().manual_seed(73)
+    B, T, Hk, Hv, D, slots = 6, 9, 2, 4, 128, 5
+    C = (2 * Hk + Hv) * D
+    n = lambda *s: torch.randn(*s, generator=gen).to(BF16).to(dev)  # noqa: E731
+    core = pkg.GatedDeltaNetCore(Hk, Hv, D, n(C, 4), n(Hv), n(Hv), n(D))
+    pools = (torch.randn(slots, Hv, D, D, generator=gen) * 0.1).to(dev), n(slots, C, 3)
+    ids, accepted = torch.tensor([4, 1, 4, 0, 4, 4], device=dev), torch.tensor([-1, 5, -1, 2, -1, T], device=dev)
+    rows = [(n(B, T, C), n(B, T, Hv * D), n(B, T, Hv), n(B, T, Hv)) for _ in range(2)]
+    par = [ref.tree(gen, B, T, 3)[0].to(dev) for _ in range(2)]
+
+    def steps(at):
+        s, c = (p.clone() for p in pools)
+        pick = lambda r: [t[at] for t in r]  # noqa: E731
+        _, step = core.verify_tree(*pick(rows[0]), ids[at], c, s, par[0][at], fp8=fp8)
+        out, after = core.verify_tree(*pick(rows[1]), ids[at], c, s, par[1][at], pending=step.accept(accepted[at]), fp8=fp8)
+        return [t.float() for t in ((out[0], out[1].unflatten(0, (-1, T))) if fp8 else (out,))] + [after.u, after.k], s, c
+
+    got, s, c = steps(slice(0, B))
+    for b in range(B):
+        want, s1, c1 = steps(slice(b, b + 1))
+        assert all(torch.equal(g[b:b + 1], w) for g, w in zip(got, want)), b
+        assert torch.equal(s[ids[b]], s1[ids[b]]) and torch.equal(c[ids[b]], c1[ids[b]])
+    assert all(torch.equal(a[[2, 3, 4]], p[[2, 3, 4]]) for a, p in zip((s, c), pools))
