@@ -463,7 +463,8 @@ int gdn_quantize_fp8(const void* x, int x_is_fp32, int64_t sx, uint8_t* y, int64
  *      K in steps of 128, summed in fp32).  The GDN layer's gate projections, whose own
  *      launch costs more than they do
  *   C  bf16, n_parts column parts over the N + N2 columns as gdn_gemm_bf16_cols, one of
- *      them ending at N
+ *      them ending at N; parts of the N columns may have any alignment (16-byte rows are the
+ *      fastest)
  * K a multiple of 128; lda a multiple of 16 (bf16: 8), ldb of 16, A and B 16-byte aligned.
  * The order in which the blocks' sums are added may depend on M, N and K (not on which of
  * the two A is: a call from bf16 rows has the bits of gdn_quantize_fp8 and one from its

@@ -1201,7 +1201,7 @@ extern "C" int gdn_gemm_fp8(const void* A, int a_is_bf16, int64_t lda, const flo
   if (!a_is_bf16 && (sa_row < 0 || sa_grp < 0 || 4 * ((M - 1) * sa_row + (groups - 1) * sa_grp) >= kLimit))
     return GDN_ERR_INVALID_ARG;
   GemmOut out{};
-  if (!parts_of(out, n_parts, C, ldc, col_end, N + N2)) return GDN_ERR_INVALID_ARG;
+  if (!parts_of(out, n_parts, C, ldc, col_end, N + N2, true)) return GDN_ERR_INVALID_ARG;
   int first = n_parts;  // the first part of the bf16 columns
   if (N2) {
     if (!B2 || !a_is_bf16 || N2 % 16 || N % 16 || ldb2 % 8 || ldb2 < K || reinterpret_cast<uintptr_t>(B2) % 16 ||
@@ -1210,6 +1210,8 @@ extern "C" int gdn_gemm_fp8(const void* A, int a_is_bf16, int64_t lda, const flo
     first = 0;
     while (first < n_parts && col_end[first] < N) ++first;
     if (first == n_parts || col_end[first++] != N) return GDN_ERR_INVALID_ARG;  // a part ends at N
+    for (int i = first; i < n_parts; ++i)  // (the bf16 GEMM's rows, which writes them where M is large)
+      if (!part_ok(C[i], ldc[i], 0)) return GDN_ERR_INVALID_ARG;
   }
   const Fp8Kernel kernel = fp8_plan(M, N, K, a_is_bf16 != 0);
   hipStream_t st = static_cast<hipStream_t>(stream);

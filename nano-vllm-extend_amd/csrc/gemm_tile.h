@@ -147,17 +147,20 @@ bool part_ok(const uint16_t* c, int64_t ld, int width) {
 }
 
 // The n_parts (1 to kMaxParts) column parts of an output of N columns: increasing
-// boundaries at multiples of 16, the last one at N.
-bool parts_of(GemmOut& out, int n_parts, uint16_t* const* C, const int64_t* ldc, const int* col_end, int N) {
+// boundaries at multiples of 16, the last one at N.  any_row: rows of any alignment are taken
+// (gemm_store16<true>), those with 16-byte stores among them.
+bool parts_of(GemmOut& out, int n_parts, uint16_t* const* C, const int64_t* ldc, const int* col_end, int N,
+              bool any_row = false) {
   int beg = 0;
   for (int s = 0; s < kMaxParts; ++s) {
     const int e = s < n_parts ? col_end[s] : N;
     if (s < n_parts) {
       if (e <= beg || (s + 1 < n_parts ? e % 16 != 0 || e >= N : e != N)) return false;
-      if (!part_ok(C[s], ldc[s], e - beg)) return false;
+      const uintptr_t at = reinterpret_cast<uintptr_t>(C[s]);
+      if (any_row ? !at || at % 2 || ldc[s] < e - beg : !part_ok(C[s], ldc[s], e - beg)) return false;
       out.c[s] = C[s];
       out.ld[s] = ldc[s];
-      out.vec[s] = ldc[s] % 8 == 0;
+      out.vec[s] = ldc[s] % 8 == 0 && at % 16 == 0;
     } else {
       out.c[s] = out.c[n_parts - 1];
       out.ld[s] = out.ld[n_parts - 1];

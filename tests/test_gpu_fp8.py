@@ -351,3 +351,18 @@ def test_decode_step_to_e4m3(pkg, dev, B, Hk, Hv, params):
         assert y.shape == (B, 1, Hv, D) and torch.equal(y.view(torch.uint8), want.view(torch.uint8))
         assert torch.equal(scale, ws) and scale.shape == (B, Hv)
         assert torch.equal(s_pool, pools[0][0]) and torch.equal(c_pool.view(torch.int16), pools[0][1].view(torch.int16))
+
+
+@pytest.mark.parametrize("M,N,K", [(1, 2048, 256), (3, 72, 128), (16, 520, 384), (37, 2048, 4096), (300, 512, 2048),
+                                   (600, 2048, 256), (1500, 2048, 384), (4100, 2056, 128)])
+@pytest.mark.parametrize("lead", [1, 2, 4, 8])
+def test_linear_fp8_into_columns_that_begin_anywhere(pkg, dev, M, N, K, lead):
+    """out: columns of a wider buffer, its rows of 16-byte pieces, that begin between them."""
+    gen = torch.Generator().manual_seed(M + N + lead)
+    x = _rows(gen, M, K).to(BF16).to(dev)
+    w8, ws = (t.to(dev) for t in ref.to_e4m3(_rows(gen, N, K) * K ** -0.5, 128))
+    buf = torch.full((M, N + 16), 7.0, dtype=BF16, device=dev)
+    pkg.linear_fp8(x, w8, ws, out=buf[:, lead:lead + N])
+    torch.cuda.synchronize()
+    assert torch.equal(buf[:, lead:lead + N], pkg.linear_fp8(x, w8, ws))
+    assert bool((buf[:, :lead] == 7).all()) and bool((buf[:, lead + N:] == 7).all())
