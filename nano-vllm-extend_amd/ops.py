@@ -996,7 +996,9 @@ def _conv_tree_ready(x, conv_pool, ids, weight, parents, pending, y=None) -> _Re
     _bf16(weight, "weight")
     if weight.numel() != 4 * C or weight.shape[-1] != 4 or C % 8:
         raise ValueError(f"weight must be [{C}, 4] (conv width 4) and C a multiple of 8")
-    w = weight if weight.is_contiguous() else weight.contiguous()
+    w = weight
+    if not w.is_contiguous() or w.data_ptr() % 16:
+        w = w.clone(memory_format=torch.contiguous_format)
     ids = _tree_ids(ids, B)
     par, p_b = _tree_parents(parents, B, T)
     last = (0, 0, 0, 0, 0, 0, 0)

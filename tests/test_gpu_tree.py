@@ -785,3 +785,18 @@ def test_padded_rows_share_a_slot_of_which_nothing_is_accepted(pkg, dev, fp8):
         assert all(torch.equal(g[b:b + 1], w) for g, w in zip(got, want)), b
         assert torch.equal(s[ids[b]], s1[ids[b]]) and torch.equal(c[ids[b]], c1[ids[b]])
     assert all(torch.equal(a[[2, 3, 4]], p[[2, 3, 4]]) for a, p in zip((s, c), pools))
+
+
+@pytest.mark.parametrize("lead", [1, 4])
+def test_conv_weight_that_begins_anywhere(pkg, dev, lead):
+    """A contiguous weight that is not 16-byte aligned (a view into a flat buffer) is copied."""
+    gen = torch.Generator().manual_seed(79)
+    B, T, C = 2, 5, 264
+    n = lambda *s: torch.randn(*s, generator=gen).to(BF16).to(dev)  # noqa: E731
+    x, pool, w = n(B, T, C), n(B, C, 3), n(C, 4)
+    flat = torch.cat([n(lead), w.flatten()])[lead:].view(C, 4)
+    assert flat.is_contiguous() and flat.data_ptr() % 16
+    args = torch.arange(B, device=dev), torch.arange(-1, T - 1, dtype=torch.int32, device=dev)
+    got, want = pkg.conv_tree_step(x, pool, args[0], flat, args[1]), pkg.conv_tree_step(x, pool, args[0], w, args[1])
+    torch.cuda.synchronize()
+    assert torch.equal(got, want)

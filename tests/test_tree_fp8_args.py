@@ -376,3 +376,18 @@ def test_checks_without_a_launch(pkg):
         for wrong in (0, n - 1, n + 1):
             with pytest.raises(TypeError):
                 call(*[t] * wrong)
+
+
+def _between(t):
+    """The same values at an address that is no multiple of 16."""
+    flat = torch.cat([t.new_zeros(1), t.flatten()])[1:].view(t.shape)
+    assert flat.is_contiguous() and flat.data_ptr() % 16
+    return flat
+
+
+def test_conv_weight_reaches_the_kernel_aligned(pkg, monkeypatch):
+    monkeypatch.setattr(pkg.ops, "_device_of", lambda *ts: 0)
+    B, T, C = 2, 3, 64
+    z = lambda *s: torch.zeros(*s, dtype=BF16)  # noqa: E731
+    pkg.ops._conv_tree_ready(z(B, T, C), z(4, C, 3), torch.arange(B), _between(z(C, 1, 4)),
+                             torch.zeros(T, dtype=torch.int32), None).check()
