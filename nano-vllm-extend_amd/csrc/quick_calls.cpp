@@ -158,7 +158,8 @@ struct Conv {
     ids = &t.ids(a[2], B);
     w = &t.tensor(a[3], kBf16, -1);
     par = &t.parents(a[4], B, T, p_b);
-    if (!t.ok || w->numel() != 4 * C || w->dim() == 0 || w->size(-1) != 4 || !w->is_contiguous() || C % 8) return false;
+    if (!t.ok || w->numel() != 4 * C || w->dim() == 0 || w->size(-1) != 4 || !w->is_contiguous() || !aligned(*w) || C % 8)
+      return false;
     if (PyObject* p = t.pending(a[5], 3)) {
       lx = &t.tensor(PyTuple_GET_ITEM(p, 0), kBf16, 3);
       if (!t.ok) return false;
