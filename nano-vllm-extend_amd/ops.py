@@ -1589,8 +1589,8 @@ def _norm_fp8_ready(hidden_states, gate, weight, eps) -> _Ready:
         raise ValueError(f"hidden_states and gate must be [..., H, D] alike, got {list(hidden_states.shape)} and "
                          f"{list(gate.shape)}")
     H, D = hidden_states.shape[-2:]
-    if weight.dtype != torch.bfloat16 or not weight.is_contiguous():
-        weight = weight.to(torch.bfloat16).contiguous()
+    if weight.dtype != torch.bfloat16 or not weight.is_contiguous() or weight.data_ptr() % 16:
+        weight = weight.to(torch.bfloat16).clone(memory_format=torch.contiguous_format)
     if weight.numel() != D or H == 0 or H * D % FP8_GROUP:
         raise ValueError(f"weight must have {D} values and H * D = {H * D} be a multiple of {FP8_GROUP}")
 

@@ -366,3 +366,14 @@ def test_linear_fp8_into_columns_that_begin_anywhere(pkg, dev, M, N, K, lead):
     torch.cuda.synchronize()
     assert torch.equal(buf[:, lead:lead + N], pkg.linear_fp8(x, w8, ws))
     assert bool((buf[:, :lead] == 7).all()) and bool((buf[:, lead + N:] == 7).all())
+
+
+@pytest.mark.parametrize("lead", [1, 4])
+def test_norm_weight_that_begins_anywhere(pkg, dev, lead):
+    gen = torch.Generator().manual_seed(83)
+    x, z, w = (torch.randn(*s, generator=gen).to(BF16).to(dev) for s in ((5, 2, 128), (5, 2, 128), (128,)))
+    flat = torch.cat([w[:lead], w])[lead:]
+    assert flat.is_contiguous() and flat.data_ptr() % 16
+    got, want = pkg.rms_norm_gated_fp8(x, z, flat, 1e-6), pkg.rms_norm_gated_fp8(x, z, w, 1e-6)
+    torch.cuda.synchronize()
+    assert torch.equal(_bits(got[0]), _bits(want[0])) and torch.equal(got[1], want[1])

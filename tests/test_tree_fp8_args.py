@@ -391,3 +391,9 @@ def test_conv_weight_reaches_the_kernel_aligned(pkg, monkeypatch):
     z = lambda *s: torch.zeros(*s, dtype=BF16)  # noqa: E731
     pkg.ops._conv_tree_ready(z(B, T, C), z(4, C, 3), torch.arange(B), _between(z(C, 1, 4)),
                              torch.zeros(T, dtype=torch.int32), None).check()
+
+
+def test_norm_weight_reaches_the_kernel_aligned(pkg, monkeypatch):
+    monkeypatch.setattr(pkg.ops, "_device_of", lambda *ts: 0)
+    n = torch.zeros(5, 2, 128, dtype=BF16)
+    pkg.ops._norm_fp8_ready(n, n, _between(torch.ones(128, dtype=BF16)), 1e-6).check()
