@@ -141,22 +141,27 @@ def load() -> ctypes.CDLL:
     return lib
 
 
-QUICK_PATH = Path(__file__).resolve().parent / "lib" / "gdn_quick_calls.so"
+QUICK_NAME = "gdn_quick_calls.so"
 _QUICK = None
 
 
 def quick():
     """The module of csrc/quick_calls.cpp: a call whose tensors the kernel takes as they are,
-    checked and launched in C++; None where the wrapper has to look at them itself."""
+    checked and launched in C++; None where the wrapper has to look at them itself.  It lies beside
+    the library, whose entry points it calls, and is of the same version."""
     global _QUICK
     if _QUICK is None:
         load()   # (the module's calls are the library's)
-        if not QUICK_PATH.exists():
-            raise GDNLibraryError(f"{QUICK_PATH} not found: build it with `python nano-vllm-extend_amd/build.py` "
+        path = LIB_PATH.parent / QUICK_NAME
+        if not path.exists():
+            raise GDNLibraryError(f"{path} not found: build it with `python nano-vllm-extend_amd/build.py` "
                                   "(or __graft_entry__.build())")
-        loader = importlib.machinery.ExtensionFileLoader("gdn_quick_calls", str(QUICK_PATH))
+        loader = importlib.machinery.ExtensionFileLoader("gdn_quick_calls", str(path))
         module = importlib.util.module_from_spec(importlib.util.spec_from_loader("gdn_quick_calls", loader))
         loader.exec_module(module)
+        v = getattr(module, "ABI_VERSION", None)
+        if v != ABI_VERSION:
+            raise GDNLibraryError(f"ABI mismatch: {path} {v}, bindings {ABI_VERSION}")
         module.set_check(check)
         _QUICK = module
     return _QUICK

@@ -531,4 +531,9 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "gdn_quick_calls", nullptr, -1, met
 
 }  // namespace
 
-extern "C" __attribute__((visibility("default"))) PyObject* PyInit_gdn_quick_calls() { return PyModule_Create(&module); }
+extern "C" __attribute__((visibility("default"))) PyObject* PyInit_gdn_quick_calls() {
+  PyObject* m = PyModule_Create(&module);
+  // (of the header that the calls above were compiled with)
+  if (m && PyModule_AddIntConstant(m, "ABI_VERSION", GDN_ABI_VERSION) != 0) Py_CLEAR(m);
+  return m;
+}

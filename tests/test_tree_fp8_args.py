@@ -397,3 +397,35 @@ def test_norm_weight_reaches_the_kernel_aligned(pkg, monkeypatch):
     monkeypatch.setattr(pkg.ops, "_device_of", lambda *ts: 0)
     n = torch.zeros(5, 2, 128, dtype=BF16)
     pkg.ops._norm_fp8_ready(n, n, _between(torch.ones(128, dtype=BF16)), 1e-6).check()
+
+
+def test_quick_calls_of_another_version_or_place_are_refused(pkg, tmp_path):
+    """The module is the one beside the library that is loaded, and of the bindings' version: its calls
+    are compiled against a header's argument lists."""
+    import shutil
+    import subprocess
+    import sys
+    import sysconfig
+    from pathlib import Path
+
+    lib = pkg._lib.LIB_PATH
+    shutil.copy(lib, tmp_path / lib.name)
+    code = ("import os, sys; sys.path.insert(0, %r); os.environ['GDN_MI355X_LIB'] = %r\n"
+            "import __graft_entry__ as ge\npkg = ge.load_package()\n"
+            "try:\n    print('TAKEN', pkg._lib.quick().__file__)\nexcept pkg._lib.GDNLibraryError as e:\n    print('LOUD', e)\n"
+            % (str(Path(__file__).resolve().parents[1]), str(tmp_path / lib.name)))
+    run = lambda: subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=120).stdout  # noqa: E731
+    assert "LOUD" in run()                                           # none beside it
+    module = tmp_path / pkg._lib.QUICK_NAME
+    for constant in ("", f'if (m) PyModule_AddIntConstant(m, "ABI_VERSION", {pkg._lib.ABI_VERSION - 1});'):
+        src = tmp_path / "old.c"
+        src.write_text('#include <Python.h>\nstatic struct PyModuleDef d = {PyModuleDef_HEAD_INIT, "gdn_quick_calls", 0, -1};\n'
+                       "PyMODINIT_FUNC PyInit_gdn_quick_calls(void) {\n  PyObject* m = PyModule_Create(&d);\n"
+                       f"  {constant}\n  return m;\n}}\n")
+        subprocess.run(["gcc", "-shared", "-fPIC", f"-I{sysconfig.get_paths()['include']}", str(src), "-o", str(module)],
+                       check=True)
+        out = run()
+        assert "LOUD ABI mismatch" in out, out
+    shutil.copy(lib.parent / module.name, module)
+    out = run()
+    assert f"TAKEN {module}" in out, out
