@@ -59,7 +59,8 @@ struct Fp8Scales {
 // like its operands: one 4-byte load per lane and wave (waves 0 to 3 a quarter of the
 // rows each, wave 4 + h the column half h), two steps ahead.  The section after the one
 // that read a step's scales loads those of the step two later, so that two sections
-// in a row issue 9 loads.  An odd step past the last one repeats it with B's scale 0.
+// in a row issue 9 loads.  An odd step past the last one repeats it with scales of 0 (both: a row's
+// may be infinite).
 //
 // 16384 x 12288 x 2048 363 us (2.27 PFLOP/s; the library's product with one scale for each
 // operand 399), 8192^3 418 us (2.63 PFLOP/s; library 2.65), 17001 x 2048 x 2048 70-75 us.  Bound
@@ -76,6 +77,8 @@ __device__ __forceinline__ void dma4(__amdgpu_buffer_rsrc_t rsrc, void* lds, int
   __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_ptr_t)lds, 4, voff, soff, 0, 0);
 }
 
+// kOdd: K is an odd number of steps.
+template <bool kOdd>
 __global__ __launch_bounds__(kPPThreads, 2) void gemm_fp8_pp_kernel(const uint8_t* __restrict__ A, int64_t lda,
                                                                     const uint8_t* __restrict__ B, int64_t ldb,
                                                                     Fp8Scales sc, GemmOut out, int M, int N, int K,
@@ -175,15 +178,21 @@ __global__ __launch_bounds__(kPPThreads, 2) void gemm_fp8_pp_kernel(const uint8_
       sb[h] = s < nk ? p[256 + 64 * h] : 0.0f;
     }
   };
+  // a product of scales of step s, or 0 past the last one (a mask: of a choice the compiler makes two
+  // bodies of the loop, and spills).  In an instance of its own: it costs 1 to 2 % (8192^3 423 us
+  // for 413), and so does the even one without the choice of sb above (426 for 420).
+  auto kept = [&](float v, int s) {
+    return kOdd ? __uint_as_float(__float_as_uint(v) & static_cast<uint32_t>((s - nk) >> 31)) : v;
+  };
   gdn::f32x4_t acc[2][2][4][2];  // [row half][column half][16-row tile][column tile]
-  // one row half of A against both column halves of B
+  // one row half of A against both column halves of B, in step `at`; odd: which may be past the last
   auto prod = [&](gdn::f32x4_t (&c)[2][4][2], const Frag8 (&fa)[4], const Frag8 (&f0)[2], const Frag8 (&f1)[2],
-                  const float (&s)[4]) {
+                  const float (&s)[4], int at, auto odd) {
     float f[2][4];
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
-      for (int b = 0; b < 2; ++b) f[b][i] = s[i] * sb[b];
+      for (int b = 0; b < 2; ++b) f[b][i] = odd.value ? kept(s[i] * sb[b], at) : s[i] * sb[b];
     __builtin_amdgcn_s_setprio(1);
     // product j is scaled into its sum behind the issue of product j + 2, when its
     // result is there
@@ -197,7 +206,7 @@ __global__ __launch_bounds__(kPPThreads, 2) void gemm_fp8_pp_kernel(const uint8_
         for (int e = 0; e < 4; ++e) c[b][i][t][e] = fmaf(p[d % 3][e], f[b][i], c[b][i][t][e]);
       }
     }
-    __builtin_amdgcn_sched_group_barrier(0x002, 8, 0);  // the scales
+    __builtin_amdgcn_sched_group_barrier(0x002, kOdd && odd.value ? 16 : 8, 0);  // the scales
     __builtin_amdgcn_sched_group_barrier(0x008, 2, 0);
 #pragma unroll
     for (int j = 2; j < 16; ++j) {
@@ -208,6 +217,8 @@ __global__ __launch_bounds__(kPPThreads, 2) void gemm_fp8_pp_kernel(const uint8_
     __builtin_amdgcn_s_setprio(0);
     half_barrier();
   };
+  constexpr std::true_type yes;
+  constexpr std::false_type no;
   auto mem_end = [&]() {
     __builtin_amdgcn_sched_barrier(0);
     __builtin_amdgcn_s_waitcnt(kWaitPP8);
@@ -264,28 +275,28 @@ __global__ __launch_bounds__(kPPThreads, 2) void gemm_fp8_pp_kernel(const uint8_
         read_b(b01, fb1);
         read_sc(sc0, s);
         mem_end();
-        prod(acc[0], fa, fb0, fb1, sa[0]);
+        prod(acc[0], fa, fb0, fb1, sa[0], s, no);
         dma(ra, a00, va[0], k2);
         dma(rb, b01, vb[1], k2);
         dma_sc(sc0, s2);
         read_a(a01, fa);
         read_b(b10, fbn);
         mem_end();
-        prod(acc[1], fa, fb0, fb1, sa[1]);
+        prod(acc[1], fa, fb0, fb1, sa[1], s, no);
         dma(rb, b10, vb[0], k3);
         dma(ra, a01, va[1], k2);
         read_a(a10, fa);
         read_b(b11, fb1);
         read_sc(sc1, s + 1);
         mem_end();
-        prod(acc[0], fa, fbn, fb1, sa[0]);
+        prod(acc[0], fa, fbn, fb1, sa[0], s + 1, yes);
         dma(ra, a10, va[0], k3);
         dma(rb, b11, vb[1], k3);
         dma_sc(sc1, s2 + 1);
         read_a(a11, fa);
         read_b(b00, fb0);
         mem_end();
-        prod(acc[1], fa, fbn, fb1, sa[1]);
+        prod(acc[1], fa, fbn, fb1, sa[1], s + 1, yes);
       }
       if (!wm) half_barrier();
       const int lane_e = new_lane();
@@ -353,7 +364,7 @@ __global__ __launch_bounds__(kPPThreads, 2) void gemm_fp8_pp_kernel(const uint8_
       __builtin_amdgcn_s_setprio(1);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const float fg = f[i] * g;
+        const float fg = kept(f[i] * g, s);
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
           const gdn::f32x4_t r = mfma_fp8(fb[t], fa[i]);
@@ -897,10 +908,10 @@ __global__ __launch_bounds__(64 * NW) void gemm_fp8_rows_kernel(const uint16_t* 
 // others B's: a load each).
 //
 // H = 2: two groups of four waves, each with stages of its own, take the first and the second
-// half of the K-steps (an odd one past the last repeats it with scale 0), which puts twice the
+// half of the K-steps (kOdd: one past the last repeats it with scale 0), which puts twice the
 // loads in flight where a CU has one tile; the second's sums
 // are added to the first's through LDS.
-template <int BN, int NS, int H>
+template <int BN, int NS, int H, bool kOdd>
 __global__ __launch_bounds__(kFp8Threads * H, 2) void gemm_fp8_deep_kernel(const uint8_t* __restrict__ A, int64_t lda,
                                                                        const uint8_t* __restrict__ B, int64_t ldb,
                                                                        Fp8Scales sc, GemmOut out, int M, int N,
@@ -987,10 +998,11 @@ __global__ __launch_bounds__(kFp8Threads * H, 2) void gemm_fp8_deep_kernel(const
         fb[j][t].lo = *reinterpret_cast<const i32x4_t*>(b + swb_off(r, lg));
         fb[j][t].hi = *reinterpret_cast<const i32x4_t*>(b + swb_off(r, 4 + lg));
       }
-    const float sb = H == 1 || first + step < nk ? p[64] : 0.0f;
+    const float sb = p[64];
+    const bool on = !kOdd || first + step < nk;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      const float s = f[i] * sb;
+      const float s = on ? f[i] * sb : 0.0f;
 #pragma unroll
       for (int j = 0; j < NJ; ++j)
 #pragma unroll
@@ -1127,18 +1139,16 @@ int fp8_launch(Fp8Kernel kernel, const void* A, int64_t lda, const uint8_t* B, i
       const int64_t t256 = blocks(256, 256), rem = t256 % kCUs8;
       const int64_t whole = rem <= kCUs8 / 2 ? t256 - rem : t256;
       const int64_t wgs = std::min<int64_t>(kCUs8, whole ? std::max(whole, 4 * (t256 - whole)) : blocks(128, 128));
-      gemm_fp8_pp_kernel<<<grid(wgs), dim3(kPPThreads), 0, st>>>(A8, lda, B, ldb, sc, out, M, N, K,
-                                                                 static_cast<int>(whole));
+      auto pp = K / gdn::kFp8Group % 2 ? gemm_fp8_pp_kernel<true> : gemm_fp8_pp_kernel<false>;
+      pp<<<grid(wgs), dim3(kPPThreads), 0, st>>>(A8, lda, B, ldb, sc, out, M, N, K, static_cast<int>(whole));
       break;
     }
-#define GDN_DEEP(name, BN, NS, H)                                                                                       \
-  case name:                                                                                                           \
-    gemm_fp8_deep_kernel<BN, NS, H><<<grid(blocks(64, BN)), dim3(kFp8Threads * H), 0, st>>>(A8, lda, B, ldb, sc, out, M, \
-                                                                                           N, K);                      \
-    break
-      GDN_DEEP(kDeep64, 64, 4, 1);
-      GDN_DEEP(kDeep128, 128, 3, 1);
-      GDN_DEEP(kDeep64x2, 64, 4, 2);
+#define GDN_DEEP(BN, NS, H, odd)                                                                                        \
+  gemm_fp8_deep_kernel<BN, NS, H, odd><<<grid(blocks(64, BN)), dim3(kFp8Threads * H), 0, st>>>(A8, lda, B, ldb, sc, out, \
+                                                                                               M, N, K)
+    case kDeep64: GDN_DEEP(64, 4, 1, false); break;
+    case kDeep128: GDN_DEEP(128, 3, 1, false); break;
+    case kDeep64x2: K / gdn::kFp8Group % 2 ? GDN_DEEP(64, 4, 2, true) : GDN_DEEP(64, 4, 2, false); break;
 #undef GDN_DEEP
 #define GDN_RING(name, BM, BN, NW, NS, Q)                                                                            \
   case name:                                                                                                         \

@@ -377,3 +377,24 @@ def test_norm_weight_that_begins_anywhere(pkg, dev, lead):
     got, want = pkg.rms_norm_gated_fp8(x, z, flat, 1e-6), pkg.rms_norm_gated_fp8(x, z, w, 1e-6)
     torch.cuda.synchronize()
     assert torch.equal(_bits(got[0]), _bits(want[0])) and torch.equal(got[1], want[1])
+
+
+# odd numbers of 128-column blocks: a ring, tiles in two halves of K, 256-row tiles with whole ones and quarters alone
+@pytest.mark.parametrize("M,N,K", [(3, 512, 384), (500, 2000, 2176), (4100, 2056, 640), (8492, 2304, 384), (200, 8192, 640),
+                                   (1500, 2048, 640)])
+def test_linear_fp8_infinite_row_scales(pkg, dev, M, N, K):
+    """A caller's infinite scale of a row's last block, whose values are positive as the weight's are,
+    makes the row infinite, not NaN; the other rows are what they were."""
+    gen = torch.Generator().manual_seed(M + K)
+    x8, xs = (t.to(dev) for t in ref.to_e4m3(_rows(gen, M, K), 1))
+    w8, ws = (t.to(dev) for t in ref.to_e4m3(_rows(gen, N, K).abs() + 0.1, 128))
+    x8.view(torch.uint8)[:, -128:] = 0x38                      # 1.0
+    y = pkg.linear_fp8(x8, w8, ws, x_scale=xs)
+    rows = torch.randperm(M, generator=gen)[:max(1, M // 7)].to(dev)
+    xs[rows, -1] = float("inf")
+    z = pkg.linear_fp8(x8, w8, ws, x_scale=xs)
+    torch.cuda.synchronize()
+    assert bool((z[rows] == float("inf")).all())
+    others = torch.ones(M, dtype=torch.bool, device=dev)
+    others[rows] = False
+    assert torch.equal(z[others], y[others]) and bool(y.isfinite().all())
