@@ -9,9 +9,11 @@
 #include <ATen/ops/empty.h>
 #include <ATen/ops/empty_strided.h>
 #include <c10/hip/HIPFunctions.h>
+#include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <cmath>
+#include <exception>
 #include <tuple>
 
 #include "../../include/gdn_mi355x.h"
@@ -125,7 +127,8 @@ bool failed(const char* name, int status) {
   return true;
 }
 
-// What a call of one function gives: its C++ exceptions become Python's.
+// What a call of one function gives: its C++ exceptions become what torch makes of them in Python
+// (no memory: torch.OutOfMemoryError).
 template <class F>
 PyObject* guarded(Py_ssize_t n, Py_ssize_t want, F&& f) {
   if (n != want) {
@@ -134,8 +137,8 @@ PyObject* guarded(Py_ssize_t n, Py_ssize_t want, F&& f) {
   }
   try {
     return f();
-  } catch (const std::exception& e) {
-    PyErr_SetString(PyExc_RuntimeError, e.what());
+  } catch (...) {
+    torch::translate_exception_to_python(std::current_exception());
     return nullptr;
   }
 }
