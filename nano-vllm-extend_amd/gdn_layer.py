@@ -222,6 +222,11 @@ class GatedDeltaNetCore:
         with self._timed("rmsnorm_gated"):
             return ops.rms_norm_gated(core, z, self.norm_w, self.eps, out)
 
+    def _check_fp8(self, fp8: bool):
+        """Before a call's first launch: whether its e4m3 rows have whole groups."""
+        if fp8 and self.value_dim % ops.FP8_GROUP:
+            raise ValueError(f"fp8 rows have a scale for each {ops.FP8_GROUP} of their {self.value_dim} columns")
+
     def _norm_fp8(self, core, z):
         with self._timed("rmsnorm_gated"):
             return ops.rms_norm_gated_fp8(core, z, self.norm_w, self.eps)
@@ -233,6 +238,8 @@ class GatedDeltaNetCore:
         Returns core [B, Hv, D] bf16 (in `out` where given); with fp8 (D == 128, no `out`)
         its (e4m3 [B, 1, Hv, D], scales) where the fused decode kernels run."""
         self._to(mixed.device)
+        if fp8 and (self.D != ops.FP8_GROUP or out is not None):
+            raise ValueError(f"fp8 outputs need a head dim of {ops.FP8_GROUP} and take no out")
         B = mixed.shape[0]
         Hk, Hv, D = self.Hk, self.Hv, self.D
         kd = self.key_dim
@@ -290,6 +297,7 @@ class GatedDeltaNetCore:
         self._to(mixed.device)
         if not self.sw.gbeta or not self.sw.conv_kernel or self.K != 4:
             raise NotImplementedError("verify_tree runs the gate and conv kernels (conv width 4) only")
+        self._check_fp8(fp8)
         if pending is not None and pending.accepted is None:
             raise ValueError("pending has no accepted nodes: accept() follows each verify")
         last_conv = last_rule = None
@@ -321,6 +329,7 @@ class GatedDeltaNetCore:
         `out` where given, except with the split state pass); with fp8 (and no
         `out`) its (e4m3, scales), except with the split state pass."""
         self._to(mixed.device)
+        self._check_fp8(fp8)
         N = mixed.shape[0]
         Hk, Hv, D = self.Hk, self.Hv, self.D
         if self.sw.fused_prefill and self.sw.gbeta and self.sw.conv_kernel and self.K == 4:
@@ -470,6 +479,7 @@ class GatedDeltaNetCore:
         would run the gate kernel).  Returns [N, Hv*D] bf16; with fp8, a step of
         prompts alone or of decode rows alone returns its (e4m3 [N, Hv, D] or [N, 1, Hv, D],
         scales) instead where its kernels write that (ops.rms_norm_gated_fp8)."""
+        self._check_fp8(fp8)
         rows = (lambda i, j: None) if gb is None else (lambda i, j: (gb[0][i:j], gb[1][i:j]))
         N = mixed.shape[0]
         T = int(max_seqlen_q)

@@ -429,3 +429,29 @@ def test_quick_calls_of_another_version_or_place_are_refused(pkg, tmp_path):
     shutil.copy(lib.parent / module.name, module)
     out = run()
     assert f"TAKEN {module}" in out, out
+
+
+def test_e4m3_rows_without_whole_groups_launch_nothing(pkg, monkeypatch):
+    """Three value heads of 64: 192 columns.  The core refuses them before its conv and rule have moved
+    the pools on, not in the norm behind them."""
+    launched = []
+    for where, name in ((pkg._lib, "call"), (pkg.ops, "_call_on"), (pkg.ops, "_launch_on")):
+        monkeypatch.setattr(where, name, lambda *a: launched.append(a))
+    monkeypatch.setattr(pkg.ops, "_device_of", lambda *ts: 0)
+    monkeypatch.setattr(pkg.ops, "_check_cuda", lambda *ts: torch.device("cpu"))
+    Hk, Hv, D, N = 1, 3, 64, 6
+    C, V = (2 * Hk + Hv) * D, Hv * D
+    n = lambda *s: torch.zeros(*s, dtype=BF16)  # noqa: E731
+    core = pkg.GatedDeltaNetCore(Hk, Hv, D, n(C, 4), n(Hv), n(Hv), n(D))
+    pools, cu = (n(2, C, 3), torch.zeros(2, Hv, D, D)), torch.tensor([0, 4, 6], dtype=torch.int32)
+    rows, ids = (n(N, C), n(N, V), n(N, Hv), n(N, Hv)), torch.arange(2)
+    for call in (lambda: core.forward(*rows, cu, 4, ids, *pools, lens_q=[4, 2], fp8=True),
+                 lambda: core.forward(*rows, torch.arange(7), 1, torch.arange(6), *pools, lens_q=[1] * 6, fp8=True),
+                 lambda: core.prefill_varlen(*rows, [4, 2], ids, *pools, fp8=True),
+                 lambda: core.verify_tree(*(t.view(2, 3, -1) for t in rows), ids, *pools, torch.zeros(3, dtype=torch.int32),
+                                          fp8=True)):
+        with pytest.raises(ValueError, match="192 columns"):
+            call()
+    with pytest.raises(ValueError, match="head dim of 128"):       # (two launches: the conv's is the first)
+        core.decode(*rows, torch.arange(6), *pools, fp8=True)
+    assert launched == []
