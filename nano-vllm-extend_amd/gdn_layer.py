@@ -614,7 +614,8 @@ class GatedDeltaNetLayer:
                 raise ValueError(f"w_qkv and w_z must have {c.conv_dim} and {c.value_dim} rows")
             self.w_in, self.w_in_scale = ops.quantize_weight_fp8(torch.cat([w_qkv, w_z], 0))
         self.hidden = self.w_in.shape[1]
-        self.w_out, self.w_out_scale = pair(w_out, self.hidden, "w_out")
+        # (laid out once: a view would be copied in every call)
+        self.w_out, self.w_out_scale = (t.contiguous() for t in pair(w_out, self.hidden, "w_out"))
         if self.w_out.shape[1] != c.value_dim or w_b.shape != (c.Hv, self.hidden) or w_a.shape != w_b.shape:
             raise ValueError(f"w_out must be [{self.hidden}, {c.value_dim}], w_b and w_a [{c.Hv}, {self.hidden}]")
         self.w_ba = torch.cat([w_b, w_a], 0).contiguous()

@@ -455,3 +455,17 @@ def test_e4m3_rows_without_whole_groups_launch_nothing(pkg, monkeypatch):
     with pytest.raises(ValueError, match="head dim of 128"):       # (two launches: the conv's is the first)
         core.decode(*rows, torch.arange(6), *pools, fp8=True)
     assert launched == []
+
+
+def test_a_checkpoints_out_projection_is_laid_out_once(pkg):
+    """An e4m3 w_out that comes as a view (columns of a wider tensor, a transposed one) is contiguous in the
+    layer, which would copy it in every call else."""
+    Hk = Hv = 1
+    D, hidden, C = 128, 256, 384
+    z = lambda *s: torch.zeros(*s, dtype=BF16)  # noqa: E731
+    e = lambda *s: z(*s).to(FP8)  # noqa: E731
+    rest = (z(Hv, hidden), z(Hv, hidden))
+    for w8, scale in ((e(hidden, 136)[:, :D], torch.ones(2, 1)), (e(D, hidden).t(), torch.ones(1, 2).t())):
+        layer = pkg.GatedDeltaNetLayer((e(C, hidden), torch.ones(3, 2)), (e(D, hidden), torch.ones(1, 2)), *rest, (w8, scale),
+                                       Hk, Hv, D, z(C, 4), z(Hv), z(Hv), z(D), weights="fp8")
+        assert layer.w_out.is_contiguous() and layer.w_out_scale.is_contiguous() and layer.w_in.is_contiguous()
