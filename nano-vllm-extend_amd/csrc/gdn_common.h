@@ -154,7 +154,8 @@ __device__ __forceinline__ float norm_gate(float x, float r, float w, float z) {
 
 // ---- e4m3 values with one fp32 scale for each group of 128 ----
 // scale = amax * fp32(1 / 448), at least 2^-126 so that its reciprocal is finite
-// (a group of zeros; magnitudes below 2^-117 go to zero); a value is
+// (a group of zeros; a group whose largest magnitude is below about 2^-117 has that scale, so
+// that its values lose steps, and those of 2^-136 and less are 0); a value is
 // e4m3(x * fp32(1 / scale)), to nearest, ties to even.  The product is at most 448
 // times 1 + 2^-22, which rounds to 448, the largest e4m3 value.  A NaN does not
 // count in amax and stays NaN; an infinity makes the scale infinite, itself NaN

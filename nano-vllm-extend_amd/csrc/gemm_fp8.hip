@@ -15,8 +15,13 @@
 // Rounding: the matrix cores add a block's 128 products after shifting them to the
 // exponent of the largest, and what lies below 2^-13 of that one is lost (measured: two
 // large products that cancel leave a third of 2^-13 of them whole and lose one of 2^-14).
-// On normal data that is 2^-17 of the sum of magnitudes, far inside of the bf16 result's
-// half step.  Everything after a block's sum is fp32, and one rounding to bf16.
+// What a result is off by beyond its rounding, of the sum of its products' magnitudes (the
+// largest of 64 x 1024 results): normal data 2^-17.2 for K = 128 and 2^-19.4 for 2048; with 2 %
+// of the columns 30 times as loud 2^-13.8 and 2^-14.5; values spread over 2^14 2^-12.8 and 2^-15.1.
+// bf16's half step is 2^-9 of the result, so that a result of which most cancels can lose more
+// to the products than to its rounding.  The instruction with 32 products per sum loses the same
+// (in each of its parts) and runs at half the rate (2.4 against 4.8 PFLOP/s from registers); the
+// alternative is the bf16 GEMM.  Everything after a block's sum is fp32, and one rounding to bf16.
 #include <algorithm>
 #include <utility>
 
@@ -747,7 +752,8 @@ __device__ __forceinline__ void each(const F& f, std::integer_sequence<int, I...
 // R S / 4 passes of 55 instructions, where the ring's own way takes 140 for each of S steps,
 // whether its 16 rows are there or not, and between the waits.  1 x 12288 x 2048 5.2 us (ring 6.7,
 // e4m3 rows 5.1), 8 rows 5.7 (6.7), 1 x 2048 x 4096 4.7 (7.0), 8 rows 5.9 (7.2); for 16 rows 7.5 and
-// 8.2 (6.8, 7.2).
+// 8.2 (6.8, 7.2).  Those are with the weights in the last-level cache; from memory 1 x 12288 x 2048
+// takes 7.8, 8 rows 8.1, 1 x 2048 x 4096 6.1, 8 rows 7.1.
 template <int BN, int NW, int NS, int S, int R>
 __global__ __launch_bounds__(64 * NW) void gemm_fp8_rows_kernel(const uint16_t* __restrict__ A, int64_t lda,
                                                                 const uint8_t* __restrict__ B, int64_t ldb,
@@ -1096,6 +1102,9 @@ Fp8Kernel fp8_plan(int M, int N, int K, bool quant) {
     // against 8.6).
     // Up to 8 rows quantize ahead, in at most 8 passes per wave (see there; with 16: 8 x 12288
     // x 4096 12.3 against 11.7).
+    // K past 4096, in the ring against two launches: 2048 columns lose (1 row x 5120 7.7 against 6.9, x
+    // 8192 10.2 / 8.1; 16 rows 7.8 / 8.0, 10.4 / 9.0), 8192 and 12288 ones would gain up to a
+    // tenth (1 x 8192 x 5120 10.4 / 10.9, 16 x 12288 x 8192 18.8 / 20.2): the limit is for all.
     if (blocks(16, 32) <= kCUs8) return M <= 8 ? kRows16x32 : kRingQ16x32;
     if (M <= 16 && blocks(16, 64) <= kCUs8) return M <= 4 || (M <= 8 && K <= 2048) ? kRows16x64 : kRingQ16x64;
   }

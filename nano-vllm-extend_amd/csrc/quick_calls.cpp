@@ -1,7 +1,7 @@
 // The short calls' way from Python without its cost: a call whose tensors the kernel takes
 // as they are (types, shapes, strides, alignment, one device, the current one) is checked,
-// allocated and launched here, in about 5 us where the Python wrapper and ctypes take 9 to
-// 14.  Anything else returns None: the wrapper's own checks then say what is wrong, or copy.
+// allocated and launched here, in 4 to 10 us (by the call and the box) where the Python wrapper
+// and ctypes take 9 to 18.  Anything else returns None: the wrapper's own checks then say what is wrong, or copy.
 #include <Python.h>
 
 #include <ATen/core/Tensor.h>
