@@ -329,7 +329,6 @@ class GatedDeltaNetCore:
         `out` where given, except with the split state pass); with fp8 (and no
         `out`) its (e4m3, scales), except with the split state pass."""
         self._to(mixed.device)
-        self._check_fp8(fp8)
         N = mixed.shape[0]
         Hk, Hv, D = self.Hk, self.Hv, self.D
         if self.sw.fused_prefill and self.sw.gbeta and self.sw.conv_kernel and self.K == 4:
@@ -340,6 +339,7 @@ class GatedDeltaNetCore:
             if split is not None:
                 return self._prefill_split(mixed, z, b, a, lens_q, ids, conv_cache, s_cache, fresh, cu64_cpu,
                                            cu64_gpu, split)
+            self._check_fp8(fp8 and out is None)
             with self._timed("conv_chunk_prefill"):
                 o = ops.conv_chunk_prefill_varlen(mixed, conv_cache, self.conv_w, b, a, self.A_log, self.dt_bias,
                                                   cu64_gpu, s_cache, ids, Hk, Hv, D, fresh=fresh,
@@ -347,6 +347,7 @@ class GatedDeltaNetCore:
             if fp8 and out is None:
                 return self._norm_fp8(o, z.view(N, Hv, D))
             return self._norm(o, z.view(N, Hv, D), out).view(N, Hv, D)
+        self._check_fp8(fp8 and out is None)
         if fresh is not None:
             zero = ids[fresh.to(device=ids.device, dtype=torch.bool)]
             conv_cache[zero] = 0
@@ -479,7 +480,6 @@ class GatedDeltaNetCore:
         would run the gate kernel).  Returns [N, Hv*D] bf16; with fp8, a step of
         prompts alone or of decode rows alone returns its (e4m3 [N, Hv, D] or [N, 1, Hv, D],
         scales) instead where its kernels write that (ops.rms_norm_gated_fp8)."""
-        self._check_fp8(fp8)
         rows = (lambda i, j: None) if gb is None else (lambda i, j: (gb[0][i:j], gb[1][i:j]))
         N = mixed.shape[0]
         T = int(max_seqlen_q)

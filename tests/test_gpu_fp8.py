@@ -398,3 +398,23 @@ def test_linear_fp8_infinite_row_scales(pkg, dev, M, N, K):
     others = torch.ones(M, dtype=torch.bool, device=dev)
     others[rows] = False
     assert torch.equal(z[others], y[others]) and bool(y.isfinite().all())
+
+
+@pytest.mark.parametrize("lens", [[1] * 4, [1, 1, 30, 70]])
+def test_steps_that_write_bf16_take_any_heads(pkg, dev, lens):
+    """Three value heads of 64 (no whole groups of 128): decode rows, and decode rows ahead of prompts,
+    give bf16 with fp8 too, and the same."""
+    gen = torch.Generator().manual_seed(97)
+    Hk, Hv, D, N = 1, 3, 64, sum(lens)
+    C = (2 * Hk + Hv) * D
+    n = lambda *s: torch.randn(*s, generator=gen).to(BF16).to(dev)  # noqa: E731
+    core = pkg.GatedDeltaNetCore(Hk, Hv, D, n(C, 4), n(Hv), n(Hv), n(D))
+    rows = n(N, C), n(N, Hv * D), n(N, Hv), n(N, Hv)
+    pools = torch.randn(4, Hv, D, D, generator=gen).to(dev) * 0.1, n(4, C, 3)
+    cu = torch.tensor([0] + lens).cumsum(0).to(torch.int32).to(dev)
+    got = []
+    for fp8 in (False, True):
+        s, c = (p.clone() for p in pools)
+        got.append((core.forward(*rows, cu, max(lens), torch.arange(4, device=dev), c, s, lens_q=lens, fp8=fp8), s, c))
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(*got)) and got[0][0].dtype == BF16

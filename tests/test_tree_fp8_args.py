@@ -446,7 +446,6 @@ def test_e4m3_rows_without_whole_groups_launch_nothing(pkg, monkeypatch):
     pools, cu = (n(2, C, 3), torch.zeros(2, Hv, D, D)), torch.tensor([0, 4, 6], dtype=torch.int32)
     rows, ids = (n(N, C), n(N, V), n(N, Hv), n(N, Hv)), torch.arange(2)
     for call in (lambda: core.forward(*rows, cu, 4, ids, *pools, lens_q=[4, 2], fp8=True),
-                 lambda: core.forward(*rows, torch.arange(7), 1, torch.arange(6), *pools, lens_q=[1] * 6, fp8=True),
                  lambda: core.prefill_varlen(*rows, [4, 2], ids, *pools, fp8=True),
                  lambda: core.verify_tree(*(t.view(2, 3, -1) for t in rows), ids, *pools, torch.zeros(3, dtype=torch.int32),
                                           fp8=True)):
@@ -455,6 +454,10 @@ def test_e4m3_rows_without_whole_groups_launch_nothing(pkg, monkeypatch):
     with pytest.raises(ValueError, match="head dim of 128"):       # (two launches: the conv's is the first)
         core.decode(*rows, torch.arange(6), *pools, fp8=True)
     assert launched == []
+    monkeypatch.setattr(pkg.ops, "_stream", lambda dev: 0)
+    # decode rows are bf16 with heads of 64: nothing to refuse
+    out = core.forward(*rows, torch.arange(7), 1, torch.arange(6) % 2, *pools, lens_q=[1] * 6, fp8=True)
+    assert out.dtype == BF16 and out.shape == (N, V) and launched
 
 
 def test_a_checkpoints_out_projection_is_laid_out_once(pkg):
