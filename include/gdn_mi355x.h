@@ -465,7 +465,8 @@ int gdn_quantize_fp8(const void* x, int x_is_fp32, int64_t sx, uint8_t* y, int64
  *   C  bf16, n_parts column parts over the N + N2 columns as gdn_gemm_bf16_cols, one of
  *      them ending at N; parts of the N columns may have any alignment (16-byte rows are the
  *      fastest)
- * K a multiple of 128; lda a multiple of 16 (bf16: 8), ldb of 16, A and B 16-byte aligned.
+ * K a multiple of 128; lda a multiple of 16 (bf16: 8), ldb of 16, A and B 16-byte aligned; A, B,
+ * B2 and the scales span less than 2^31 bytes each (32-bit offsets; C may be larger).
  * The order in which the blocks' sums are added may depend on M, N and K (not on which of
  * the two A is: a call from bf16 rows has the bits of gdn_quantize_fp8 and one from its
  * rows).  Inside of a block the matrix cores drop what lies below 2^-13 of the block's largest

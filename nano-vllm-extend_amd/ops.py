@@ -1462,8 +1462,9 @@ def linear_fp8(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor
     K / 128] fp32, one for each 128 x 128 block (quantize_weight_fp8's, or a
     checkpoint's).  x [..., K] bf16, quantized in the call (the bits of quantize_fp8 and
     a call with its result), or e4m3 with its x_scale [M, K / 128] (any strides).  K a
-    multiple of 128.  fp32 accumulation; returns [..., N] bf16 (or writes `out`, a [M, N]
-    view with contiguous rows)."""
+    multiple of 128; x and weight below 2 GiB each (more rows in several calls).  fp32
+    accumulation; returns [..., N] bf16 (or writes `out`, a [M, N] view with contiguous
+    rows of any alignment)."""
     if out is None:
         y = _lib.quick().linear_fp8(x, weight, weight_scale, x_scale)
         if y is not None:
