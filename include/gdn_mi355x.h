@@ -26,7 +26,7 @@
 extern "C" {
 #endif
 
-#define GDN_ABI_VERSION 7
+#define GDN_ABI_VERSION 8
 
 #define GDN_OK 0
 #define GDN_ERR_INVALID_ARG (-1) /* shape / stride / pointer rejected */
@@ -38,13 +38,14 @@ extern "C" {
 #define GDN_NOALLOC_SCRATCH_BYTES (128LL << 20)
 
 /* In the place of the stream of gdn_conv_tree, gdn_rule_tree, gdn_rule_tree_layer,
- * gdn_commit_tree and gdn_rmsnorm_gated_fp8: the arguments are checked as the call would, and
+ * gdn_commit_tree, gdn_rmsnorm_gated_fp8 and gdn_add_rms_norm: the arguments are checked as the call would, and
  * nothing is launched.  For calls of which all or none are to be made: gdn_conv_tree moves the
  * conv pool on, and what gdn_rule_tree refuses after it would leave the two pools a step apart. */
 #define GDN_CHECK_ONLY ((void*)-1)
 
 /* ABI version of the loaded library (GDN_ABI_VERSION; 5 added gdn_decode_step, 6 the
- * 8-bit projections and the tree verify, 7 GDN_CHECK_ONLY). */
+ * 8-bit projections and the tree verify, 7 GDN_CHECK_ONLY, 8 the block norms and the
+ * adapters). */
 int gdn_abi_version(void);
 
 /*
@@ -586,6 +587,73 @@ int gdn_commit_tree(float* s_pool, int64_t s_slot, uint16_t* conv_pool, int64_t 
                     const float* g, const float* u, int B, int T, int Hk, int Hv, int D, int C, void* stream);
 
 /*
+ * The residual stream between two blocks of the model: it takes a block's output x, and
+ * the next block reads its RMSNorm (the decoder layer's norms,
+ * nanovllm/models/qwen3_5.py:99-118, :674-689; the norm behind a block, the gate and the
+ * scale are other models').
+ *   h = x;  h = h rsqrt(mean(h^2) + eps) (offset + post_w)  if post_w;
+ *   h = h gate, or h sigmoid(gate) with gate_sigmoid        if gate;
+ *   r = residual + scale h  (scale h if residual is NULL);
+ *   y = r rsqrt(mean(r^2) + eps) (offset + w)
+ * in fp32; y comes from the r that is not rounded.
+ *   x         [M, H] bf16, row stride sx; residual [M, H] fp32 (stream_is_fp32) or bf16, row
+ *             stride sr, or NULL
+ *   w, post_w [H] fp32 (w_is_fp32) or bf16; post_w NULL: none; offset 1 for weights that are
+ *             held as their distance from 1 (the reference's), 0 for others
+ *   gate      fp32 (gate_is_fp32) or bf16, NULL: none; of row m and column n at gate[m g_row +
+ *             n g_col], g_col 0 (one per row) or 1 (g_row 0: one per column)
+ *   stream_out [M, H] contiguous, the type of residual: r (NULL: not written). It may be
+ *             residual itself, where that is contiguous
+ *   y         [M, H] bf16 contiguous, y8 [M, H] e4m3 contiguous with the scale of row m and
+ *             columns 128 g .. at y8_scale[m ss_row + g ss_grp] as gdn_quantize_fp8 of the
+ *             fp32 values (H a multiple of 128 then); one of the two may be NULL
+ * H to 16384. Rows of any alignment; 16-byte aligned ones with H a multiple of 8 are read in
+ * whole pieces, and y8 asks for such.
+ */
+int gdn_add_rms_norm(const uint16_t* x, int64_t sx, const void* residual, int64_t sr, int stream_is_fp32, const void* w,
+                     const void* post_w, int w_is_fp32, float offset, const void* gate, int gate_is_fp32,
+                     int64_t g_row, int64_t g_col, int gate_sigmoid, float scale, float eps, void* stream_out,
+                     uint16_t* y, uint8_t* y8, float* y8_scale, int64_t ss_row, int64_t ss_grp, int64_t M, int H,
+                     void* stream);
+
+/*
+ * Low-rank adapters of many requests beside a projection with shared weights (no counterpart
+ * in the reference), in two calls: the rows shrunk to their adapters' rank, then the
+ * projection with the other half in its sums:
+ *   v[m][p][r] = scale[s] sum over k of x[m][k] a[s][p rank + r][k]
+ *   C[m][n]    = bf16(sum over k of A[m][k] B[n][k] + sum over r of v[m][p(n)][r] lb[s][n][r])
+ * with s = ids[m]; a row whose s is outside of 0 .. slots - 1 has no adapter and takes the
+ * projection alone.  A projection's columns may be those of several side by side, its
+ * slices (1 to 4), each with an a of its own: slice p is columns slice_end[p - 1] ..
+ * slice_end[p] - 1, its boundaries multiples of 16.
+ *   rank  a multiple of 8, at most 256 (smaller ranks are padded with zeros)
+ *   a     [slots][slices rank, K] bf16, slot stride a_slot (a multiple of 8), 16-byte aligned;
+ *         scale [slots] fp32; ids int32 [M]
+ *   v     [M, slices, 2, rank] bf16, row stride ldv (a multiple of 8), 16-byte aligned: each value as the sum
+ *         of two.  Rows without an adapter are not written, and not read by what follows
+ *   lb    [slots][N, rank] bf16, slot stride lb_slot (a multiple of 8), 16-byte aligned
+ * x as the GEMM's A: bf16 with K in steps of 64, or e4m3 with its scales (K in steps of
+ * 128).  An adapter's rows do not change the bits of others, whatever it holds.
+ */
+int gdn_lora_shrink(const void* x, int x_is_bf16, int64_t ldx, const float* xs, int64_t xs_row, int64_t xs_grp,
+                    const uint16_t* a, int64_t a_slot, const float* scale, const int32_t* ids, int slots, int slices,
+                    int rank, int M, int K, uint16_t* v, int64_t ldv, void* stream);
+
+/* gdn_gemm_bf16_cols with the adapters' part. */
+int gdn_gemm_bf16_lora(const uint16_t* A, int64_t lda, const uint16_t* B, int64_t ldb, int M, int N, int K, int n_parts,
+                       uint16_t* const* C, const int64_t* ldc, const int* col_end, float* g, uint16_t* beta,
+                       const void* A_log, const void* dt_bias, int param_is_fp32, int gate_col, int Hv,
+                       const uint16_t* v, int64_t ldv, const uint16_t* lb, int64_t lb_slot, const int32_t* ids, int slots,
+                       int rank, int slices, const int* slice_end, void* stream);
+
+/* gdn_gemm_fp8 from e4m3 rows with the adapters' part. */
+int gdn_gemm_fp8_lora(const uint8_t* A, int64_t lda, const float* sa, int64_t sa_row, int64_t sa_grp, const uint8_t* B,
+                      int64_t ldb, const float* sb, int64_t sb_row, int M, int N, int K, int n_parts, uint16_t* const* C,
+                      const int64_t* ldc, const int* col_end, const uint16_t* v, int64_t ldv, const uint16_t* lb,
+                      int64_t lb_slot, const int32_t* ids, int slots, int rank, int slices, const int* slice_end,
+                      void* stream);
+
+/*
  * The calls above that are short enough for the cost of a foreign call to show (23 to 45
  * arguments through ctypes 1.9 to 3.5 us, one array 0.5), with their arguments as 8-byte
  * words: words[0] = GDN_CALL_x + (n << 32), then the n arguments in order, pointers and
@@ -600,7 +668,9 @@ enum {
   GDN_CALL_CONV_TREE = 4,
   GDN_CALL_RULE_TREE = 5,
   GDN_CALL_RULE_TREE_LAYER = 6,
-  GDN_CALL_COMMIT_TREE = 7
+  GDN_CALL_COMMIT_TREE = 7,
+  GDN_CALL_ADD_RMS_NORM = 8,
+  GDN_CALL_LORA_SHRINK = 9
 };
 int gdn_call_words(const void* words);
 

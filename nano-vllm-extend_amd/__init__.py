@@ -11,7 +11,11 @@ that installs the kernels into the reference model module (integration).
 """
 from . import _lib, ops, state_pool, gdn_layer, integration  # noqa: F401
 from .ops import (  # noqa: F401
+    LoraPool,
     Qwen3_5RMSNormGated,
+    adapter_rows,
+    add_rms_norm,
+    add_rms_norm_fp8,
     causal_conv_silu,
     causal_conv_silu_varlen,
     causal_conv_silu_varlen_parts,
@@ -24,6 +28,8 @@ from .ops import (  # noqa: F401
     fused_g_beta,
     linear,
     linear_fp8,
+    linear_fp8_lora,
+    linear_lora,
     quantize_fp8,
     quantize_weight_fp8,
     recurrent_gated_delta_rule,

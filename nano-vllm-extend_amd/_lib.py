@@ -17,7 +17,7 @@ from pathlib import Path
 import torch  # noqa: F401  (loads the HIP runtime the library binds to)
 
 LIB_PATH = Path(os.environ.get("GDN_MI355X_LIB", Path(__file__).resolve().parent / "lib" / "libgdn_mi355x.so"))
-ABI_VERSION = 7
+ABI_VERSION = 8
 
 GDN_OK = 0
 CHECK_ONLY = -1   # in a stream's place: the arguments are checked, nothing is launched
@@ -87,13 +87,20 @@ SIGNATURES: dict[str, list] = {
                             _p, _p, _i32, _i32, _i32, _i32, _i32, _f32, _p],
     "gdn_commit_tree": [_p, _i64, _p, _i64, _i64, _i64, _p, _p, _i64, _p, _p, _i64, _i64, _p, _i64, _i64, _p, _p,
                         _i32, _i32, _i32, _i32, _i32, _i32, _p],
+    "gdn_add_rms_norm": [_p, _i64, _p, _i64, _i32, _p, _p, _i32, _f32, _p, _i32, _i64, _i64, _i32, _f32, _f32, _p, _p, _p,
+                         _p, _i64, _i64, _i64, _i32, _p],
+    "gdn_lora_shrink": [_p, _i32, _i64, _p, _i64, _i64, _p, _i64, _p, _p, _i32, _i32, _i32, _i32, _i32, _p, _i64, _p],
+    "gdn_gemm_bf16_lora": [_p, _i64, _p, _i64, _i32, _i32, _i32, _i32, _p, _p, _p, _p, _p, _p, _p, _i32, _i32, _i32, _p,
+                           _i64, _p, _i64, _p, _i32, _i32, _i32, _p, _p],
+    "gdn_gemm_fp8_lora": [_p, _i64, _p, _i64, _i64, _p, _i64, _p, _i64, _i32, _i32, _i32, _i32, _p, _p, _p, _p, _i64, _p,
+                          _i64, _p, _i32, _i32, _i32, _p, _p],
     "gdn_call_words": [ctypes.c_char_p],
 }
 
 # gdn_call_words: the packing of an entry point's arguments (the stream among them) and
 # the word before them.  Its arguments are 8-byte integers, a NULL pointer 0.
 _WORD_CALLS = ("gdn_quantize_fp8", "gdn_gemm_fp8", "gdn_rmsnorm_gated_fp8", "gdn_conv_tree", "gdn_rule_tree",
-               "gdn_rule_tree_layer", "gdn_commit_tree")
+               "gdn_rule_tree_layer", "gdn_commit_tree", "gdn_add_rms_norm", "gdn_lora_shrink")
 
 
 def _words_of(name: str, types: list):

@@ -1,0 +1,258 @@
+// The residual stream between two blocks: the stream takes a block's output, and the next
+// block reads the stream's RMSNorm (the decoder layer's norms, nanovllm/models/qwen3_5.py:99-118,
+// :674-689; the norm behind a block, its gate and the scales are other models').
+//
+//   h = x                                                     the block's output
+//   h = h rsqrt(mean(h^2) + eps) (offset + post_w)            where the block has a norm behind it
+//   h = h gate, or h sigmoid(gate)                            per row, column or value
+//   r = residual + scale h                                    the stream; scale h without a residual
+//   y = r rsqrt(mean(r^2) + eps) (offset + w)                 in bf16, in e4m3 (gdn::fp8_scale), or both
+//
+// All of it in fp32 from the inputs' values; r is rounded once, to the stream's type, and y
+// is formed from the r that was not rounded (as the reference forms it), so that y has one
+// rounding.
+#include <type_traits>
+
+#include "gdn_common.h"
+
+namespace {
+
+struct NormArgs {
+  const uint16_t* x;
+  int64_t sx;
+  const void* residual;  // NULL: none
+  int64_t sr;
+  const void* w;
+  const void* post_w;    // NULL: none
+  const void* gate;      // NULL: none
+  int64_t g_row, g_col;
+  void* stream;          // r, dense; NULL: not written
+  uint16_t* y;           // dense; NULL: not written
+  uint8_t* y8;           // dense (kFp8)
+  float* y8_scale;
+  int64_t ss_row, ss_grp;
+  int64_t M;
+  int H;
+  int stream_f32, w_f32, gate_f32, gate_sigmoid;
+  float offset, scale, eps;
+};
+
+// 1 / (1 + e^-g): the hardware reciprocal and one Newton step; 0 below -88, where it is less
+// than 2^-126.
+__device__ __forceinline__ float sigmoid_ulp(float g) {
+  const float d = 1.0f + gdn::exp_acc(fminf(0.0f - g, 88.0f));
+  const float rc = __builtin_amdgcn_rcpf(d);
+  return g < -88.0f ? 0.0f : g != g ? g : fmaf(rc, fmaf(-d, rc, 1.0f), rc);
+}
+
+// V (8 or 1) values at p[at], bf16 or fp32
+template <int V>
+__device__ __forceinline__ void load(const void* p, int64_t at, bool f32, float (&v)[V]) {
+  if constexpr (V == 8) {
+    if (f32) {
+      const float4 a = *reinterpret_cast<const float4*>(static_cast<const float*>(p) + at);
+      const float4 b = *reinterpret_cast<const float4*>(static_cast<const float*>(p) + at + 4);
+      v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+      v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+    } else {
+      const uint4 a = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p) + at);
+      const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        v[2 * i] = __uint_as_float(w[i] << 16);
+        v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+      }
+    }
+  } else {
+    v[0] = f32 ? static_cast<const float*>(p)[at] : gdn::bf2f(static_cast<const uint16_t*>(p)[at]);
+  }
+}
+
+template <int V>
+__device__ __forceinline__ void store(void* p, int64_t at, bool f32, const float (&v)[V]) {
+  if constexpr (V == 8) {
+    if (f32) {
+      float4* q = reinterpret_cast<float4*>(static_cast<float*>(p) + at);
+      q[0] = make_float4(v[0], v[1], v[2], v[3]);
+      q[1] = make_float4(v[4], v[5], v[6], v[7]);
+    } else {
+      *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p) + at) =
+          make_uint4(gdn::f2bf2(v[0], v[1]), gdn::f2bf2(v[2], v[3]), gdn::f2bf2(v[4], v[5]), gdn::f2bf2(v[6], v[7]));
+    }
+  } else {
+    if (f32) static_cast<float*>(p)[at] = v[0];
+    else static_cast<uint16_t*>(p)[at] = gdn::f2bf(v[0]);
+  }
+}
+
+// The sum over the T threads of a row (T: 64, or the whole workgroup).
+template <int T>
+__device__ __forceinline__ float row_sum(float v, float* part) {
+  v = gdn::wave_sum(v);
+  if constexpr (T > 64) {
+    constexpr int W = T / 64;
+    if (threadIdx.x % 64 == 0) part[threadIdx.x / 64] = v;
+    __syncthreads();
+    v = part[0];
+#pragma unroll
+    for (int i = 1; i < W; ++i) v += part[i];
+  }
+  return v;
+}
+
+// T threads per row, N pieces of V values per thread: piece i of thread t is columns V (T i +
+// t) .., so that 16 neighbouring lanes hold a group of 128.
+template <int V, int N, int T, bool kFp8>
+__global__ __launch_bounds__(T > 256 ? T : 256) void block_norm_kernel(NormArgs a) {
+  __shared__ float part[2][T > 64 ? T / 64 : 1];
+  constexpr int kRows = T > 256 ? 1 : 256 / T;
+  static_assert(T == 64 || kRows == 1, "a row's threads are a wave or the workgroup");
+  const int t = threadIdx.x % T;
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * kRows + threadIdx.x / T;
+  if (row >= a.M) return;  // (a wave, or the workgroup)
+  auto col = [&](int i) { return V * (T * i + t); };
+  float h[N][V];
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+#pragma unroll
+    for (int e = 0; e < V; ++e) h[i][e] = 0.0f;
+    if (col(i) < a.H) load<V>(a.x, row * a.sx + col(i), false, h[i]);
+  }
+  float res[N][V];
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+#pragma unroll
+    for (int e = 0; e < V; ++e) res[i][e] = 0.0f;
+    if (a.residual && col(i) < a.H) load<V>(a.residual, row * a.sr + col(i), a.stream_f32, res[i]);
+  }
+  const float inv_h = 1.0f / static_cast<float>(a.H);
+  if (a.post_w) {
+    float ss = 0.0f;
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+#pragma unroll
+      for (int e = 0; e < V; ++e) ss = fmaf(h[i][e], h[i][e], ss);
+    const float r = rsqrtf(row_sum<T>(ss, part[0]) * inv_h + a.eps);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      if (col(i) >= a.H) continue;
+      float w[V];
+      load<V>(a.post_w, col(i), a.w_f32, w);
+#pragma unroll
+      for (int e = 0; e < V; ++e) h[i][e] *= r * (a.offset + w[e]);
+    }
+  }
+  if (a.gate) {
+    if (a.g_col == 0) {
+      float g[1];
+      load<1>(a.gate, row * a.g_row, a.gate_f32, g);
+      if (a.gate_sigmoid) g[0] = sigmoid_ulp(g[0]);
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+#pragma unroll
+        for (int e = 0; e < V; ++e) h[i][e] *= g[0];
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        if (col(i) >= a.H) continue;
+        float g[V];
+        load<V>(a.gate, row * a.g_row + col(i), a.gate_f32, g);
+#pragma unroll
+        for (int e = 0; e < V; ++e) h[i][e] *= a.gate_sigmoid ? sigmoid_ulp(g[e]) : g[e];
+      }
+    }
+  }
+  float ss = 0.0f;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      // (what lies past the row stays 0: a gate of infinity is one per row there)
+      h[i][e] = col(i) < a.H ? fmaf(h[i][e], a.scale, res[i][e]) : 0.0f;
+      ss = fmaf(h[i][e], h[i][e], ss);
+    }
+    if (a.stream && col(i) < a.H) store<V>(a.stream, row * a.H + col(i), a.stream_f32, h[i]);
+  }
+  const float r = rsqrtf(row_sum<T>(ss, part[1]) * inv_h + a.eps);
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const bool in = col(i) < a.H;
+    if (!kFp8 && !in) continue;
+    float w[V];
+#pragma unroll
+    for (int e = 0; e < V; ++e) w[e] = 0.0f;
+    if (in) load<V>(a.w, col(i), a.w_f32, w);
+#pragma unroll
+    for (int e = 0; e < V; ++e) h[i][e] *= r * (a.offset + w[e]);
+    if (a.y && in) store<V>(a.y, row * a.H + col(i), false, h[i]);
+    if constexpr (kFp8) {
+      float top = 0.0f;
+#pragma unroll
+      for (int e = 0; e < V; ++e) top = fmaxf(top, fabsf(h[i][e]));
+#pragma unroll
+      for (int m = 8; m >= 1; m >>= 1) top = fmaxf(top, __shfl_xor(top, m, 64));
+      const float s = gdn::fp8_scale(top), inv = 1.0f / s;
+      if (in) {
+        *reinterpret_cast<uint2*>(a.y8 + row * a.H + col(i)) =
+            make_uint2(gdn::f2fp8x4(h[i][0] * inv, h[i][1] * inv, h[i][2] * inv, h[i][3] * inv),
+                       gdn::f2fp8x4(h[i][4] * inv, h[i][5] * inv, h[i][6] * inv, h[i][7] * inv));
+        if (t % 16 == 0) a.y8_scale[row * a.ss_row + col(i) / gdn::kFp8Group * a.ss_grp] = s;
+      }
+    }
+  }
+}
+
+template <int V, int T, bool kFp8, int... N>
+int launch(const NormArgs& a, hipStream_t st) {
+  constexpr int kRows = T > 256 ? 1 : 256 / T;
+  const dim3 grid(static_cast<unsigned>((a.M + kRows - 1) / kRows)), block(T > 256 ? T : 256);
+  bool done = false;
+  auto one = [&](auto n) {
+    if (done || a.H > V * T * n.value) return;
+    block_norm_kernel<V, n.value, T, kFp8><<<grid, block, 0, st>>>(a);
+    done = true;
+  };
+  (one(std::integral_constant<int, N>{}), ...);
+  return done ? gdn_launch_status() : GDN_ERR_UNSUPPORTED;
+}
+
+template <bool kFp8>
+int launch_rows(const NormArgs& a, hipStream_t st) {
+  if (a.M >= 2048 && a.H <= 4096) return launch<8, 64, kFp8, 1, 2, 4, 8>(a, st);
+  return launch<8, 256, kFp8, 1, 2, 4, 8>(a, st);
+}
+
+constexpr int kMostColumns = 16384;
+
+}  // namespace
+
+extern "C" int gdn_add_rms_norm(const uint16_t* x, int64_t sx, const void* residual, int64_t sr, int stream_is_fp32,
+                                const void* w, const void* post_w, int w_is_fp32, float offset, const void* gate,
+                                int gate_is_fp32, int64_t g_row, int64_t g_col, int gate_sigmoid, float scale, float eps,
+                                void* stream_out, uint16_t* y, uint8_t* y8, float* y8_scale, int64_t ss_row,
+                                int64_t ss_grp, int64_t M, int H, void* stream) {
+  if (M < 0 || H <= 0 || g_col < 0 || g_col > 1 || g_row < 0) return GDN_ERR_INVALID_ARG;
+  if (H > kMostColumns || M >= (1LL << 31)) return GDN_ERR_UNSUPPORTED;
+  if (y8 && H % gdn::kFp8Group) return GDN_ERR_INVALID_ARG;
+  if (M == 0) return GDN_OK;
+  if (!x || !w || (!y && !y8) || (y8 && !y8_scale) || sx < H || (residual && sr < H)) return GDN_ERR_INVALID_ARG;
+  if (gate && g_col == 1 && g_row != 0 && g_row < H) return GDN_ERR_INVALID_ARG;
+  auto aligned = [](const void* p, uintptr_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; };
+  auto natural = [&](const void* p, int f32) { return aligned(p, f32 ? 4 : 2); };
+  if (!aligned(x, 2) || !natural(residual, stream_is_fp32) || !natural(w, w_is_fp32) || !natural(post_w, w_is_fp32) ||
+      !natural(gate, gate_is_fp32) || !natural(stream_out, stream_is_fp32) || !aligned(y, 2) || !aligned(y8_scale, 4))
+    return GDN_ERR_INVALID_ARG;
+  const NormArgs a{x, sx, residual, sr, w, post_w, gate, g_row, g_col, stream_out, y, y8, y8_scale, ss_row, ss_grp, M, H,
+                   stream_is_fp32 ? 1 : 0, w_is_fp32 ? 1 : 0, gate_is_fp32 ? 1 : 0, gate_sigmoid ? 1 : 0, offset, scale,
+                   eps};
+  // rows of whole 16-byte pieces
+  const bool whole = H % 8 == 0 && sx % 8 == 0 && (!residual || sr % 8 == 0) && aligned(x, 16) && aligned(residual, 16) &&
+                     aligned(w, 16) && aligned(post_w, 16) && aligned(stream_out, 16) && aligned(y, 16) && aligned(y8, 8) &&
+                     (!gate || g_col == 0 || (aligned(gate, 16) && g_row % 8 == 0));
+  if (y8 && !whole) return GDN_ERR_INVALID_ARG;
+  if (stream == GDN_CHECK_ONLY) return GDN_OK;
+  const hipStream_t st = static_cast<hipStream_t>(stream);
+  if (y8) return launch_rows<true>(a, st);
+  if (whole) return launch_rows<false>(a, st);
+  return H <= 1024 ? launch<1, 256, false, 4>(a, st) : launch<1, 1024, false, 4, 16>(a, st);
+}

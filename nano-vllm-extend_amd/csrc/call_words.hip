@@ -81,6 +81,8 @@ extern "C" int gdn_call_words(const void* words) {
     case GDN_CALL_RULE_TREE: return call(gdn_rule_tree, w, count);
     case GDN_CALL_RULE_TREE_LAYER: return call(gdn_rule_tree_layer, w, count);
     case GDN_CALL_COMMIT_TREE: return call(gdn_commit_tree, w, count);
+    case GDN_CALL_ADD_RMS_NORM: return call(gdn_add_rms_norm, w, count);
+    case GDN_CALL_LORA_SHRINK: return call(gdn_lora_shrink, w, count);
     default: return GDN_ERR_INVALID_ARG;
   }
 }

@@ -59,8 +59,10 @@
 // bf16-rounded values with the gate kernel's arithmetic (gdn::gate_beta,
 // gdn::gate_g), so they equal gdn_g_beta applied to C.
 #include <algorithm>
+#include <type_traits>
 
 #include "gemm_tile.h"
+#include "lora_tile.h"
 
 namespace {
 
@@ -386,10 +388,11 @@ constexpr int kWaitPP = 8 | (7 << 4);
 
 // grid = 8 * min(32, ...) workgroups of 512; tiles 0 .. whole - 1 run as 256 x
 // 256, the rest as quarters.  K is a multiple of 128.
+template <bool kLora>
 __global__ __launch_bounds__(kPPThreads, 2) void gemm_tn_pp_kernel(const uint16_t* __restrict__ A, int64_t lda,
                                                                   const uint16_t* __restrict__ B, int64_t ldb,
                                                                   GemmOut out, int M, int N, int K, GemmGates gt,
-                                                                  int whole) {
+                                                                  int whole, LoraArg<kLora> lo) {
   constexpr int kHalf = 128 * 128;  // bytes of a half tile: 128 rows of 64 values
   __shared__ __align__(16) uint8_t a00[kHalf];
   __shared__ __align__(16) uint8_t a01[kHalf];
@@ -553,6 +556,14 @@ __global__ __launch_bounds__(kPPThreads, 2) void gemm_tn_pp_kernel(const uint16_
     // kept in registers across the loop)
     int tid_e = static_cast<int>(threadIdx.x);
     asm volatile("" : "+v"(tid_e));
+    if constexpr (kLora) {
+#pragma unroll
+      for (int a = 0; a < 2; ++a) {
+        const int cb[2] = {n0c + 32 * wn, n0c + 128 + 32 * wn};
+        lora_add<4, 2, 1>(lo, M, N, m0c + 128 * a + 64 * wm, cb, tid_e & 63, 0, 1,
+                          [&](int i, int j, int t) -> gdn::f32x4_t& { return acc[a][j][i][t]; });
+      }
+    }
 #pragma unroll
     for (int a = 0; a < 2; ++a)
 #pragma unroll
@@ -633,6 +644,11 @@ __global__ __launch_bounds__(kPPThreads, 2) void gemm_tn_pp_kernel(const uint16_
       step(a11, b11, a10, b10, s + 3);
     }
     if (!wm) half_barrier();
+    if constexpr (kLora) {
+      const int cb[1] = {n0 + 32 * wn};
+      lora_add<4, 1, 2>(lo, M, N, m0 + 64 * wm, cb, lane, 0, 1,
+                        [&](int i, int, int t) -> gdn::f32x4_t& { return c[i][t]; });
+    }
 #pragma unroll
     for (int i = 0; i < 4; ++i)
       gemm_store16(c[i][0], c[i][1], out, M, N, m0 + 64 * wm + 16 * i, n0 + 32 * wn, lane, gt, gscr[wave]);
@@ -651,10 +667,11 @@ __global__ __launch_bounds__(kPPThreads, 2) void gemm_tn_pp_kernel(const uint16_
 // unit pays per row.)  Against the 64 x 64 deep kernel: 1 x 2048 x 4096 16.8 ->
 // 6.2 us, 64 rows 17.1 -> 7.9, 200 rows 17.2 -> 11.7; 256 x 2048 x 2048 10.5 ->
 // 8.1.
-template <int BM>
+template <int BM, bool kLora>
 __global__ __launch_bounds__(kGemmThreads) void gemm_tn_ring_kernel(const uint16_t* __restrict__ A, int64_t lda,
                                                                     const uint16_t* __restrict__ B, int64_t ldb,
-                                                                    GemmOut out, int M, int N, int K, GemmGates gt) {
+                                                                    GemmOut out, int M, int N, int K, GemmGates gt,
+                                                                    LoraArg<kLora> lo) {
   constexpr int NW = kGemmThreads / 64, NS = 3;
   constexpr int MT = BM / 16, BN = 32;
   constexpr int kStage = (BM + BN) * 128;   // one wave's stage
@@ -734,6 +751,11 @@ __global__ __launch_bounds__(kGemmThreads) void gemm_tn_ring_kernel(const uint16
   issue(st0, wave);
   issue(st1, wave + NW);
   issue(st2, wave + 2 * NW);
+  if constexpr (kLora) {
+    const int cb[1] = {n0};
+    lora_add<MT, 1, 4>(lo, M, N, m0, cb, lane, wave, NW,
+                       [&](int i, int, int t) -> gdn::f32x4_t& { return acc[i][t]; });
+  }
   __builtin_amdgcn_s_waitcnt(kWait);
   int s = wave;
   for (; s + (NS - 1) * NW < nk; s += NS * NW) {
@@ -763,6 +785,61 @@ __global__ __launch_bounds__(kGemmThreads) void gemm_tn_ring_kernel(const uint16
   }
 }
 
+// lora_add for products of 32 x 32 x 16: 32 rows from row0 against NJ blocks of 32 columns from
+// col0, acc[j] register 4 q + r of lane (li, lg) being C[row0 + li][col0 + 32 j + 8 q + 4 lg + r].
+template <int NJ, int DEPTH>
+__device__ __forceinline__ void lora_add32(const Lora& lo, int M, int N, int row0, int col0, int lane,
+                                           f32x16_t (&acc)[NJ]) {
+  const int li = lane & 31, lg = lane >> 5;
+  const int r = row0 + li, rc = min(r, M - 1);
+  const int s0 = lo.ids[rc];
+  const int mine = r < M && static_cast<unsigned>(s0) < static_cast<unsigned>(lo.slots) ? s0 : -1;
+  const uint64_t all = __ballot(mine >= 0 && lane < 32);
+  if (!all) return;
+  const int voff = static_cast<int>(rc * lo.ldv * 2);
+  const int half = lo.rank / 8, terms = 2 * half;
+  for (int p = 0, beg = 0; p < lo.slices; beg = lo.end[p++]) {
+    const int end = lo.end[p];
+    if (col0 >= end || col0 + 32 * NJ <= beg) continue;
+    const __amdgpu_buffer_rsrc_t rv = rsrc_of(lo.v + 2 * p * lo.rank);
+    for (int c = 0; c < terms; c += 2) {
+      const int q = c + lg, qb = q < half ? q : q - half;  // (terms is even: every granule is there)
+      const gdn::s16x8_t va = lora_load(rv, voff + 16 * q);
+      LoraIds it{all, 0, 1, 0};
+      gdn::s16x8_t fb[DEPTH][NJ];
+      int sid[DEPTH];
+      auto fetch = [&](int d) {
+        sid[d] = it.next(mine);
+        if (sid[d] < 0) return;
+        const __amdgpu_buffer_rsrc_t rb = lora_b(lo, sid[d], N);
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) fb[d][j] = lora_load(rb, (col0 + 32 * j + li) * lo.rank * 2 + 16 * qb);
+      };
+#pragma unroll
+      for (int d = 0; d < DEPTH; ++d) fetch(d);
+      while (sid[0] >= 0) {
+#pragma unroll
+        for (int d = 0; d < DEPTH; ++d) {
+          if (sid[d] < 0) continue;
+#pragma unroll
+          for (int j = 0; j < NJ; ++j) {
+            const int cb = col0 + 32 * j;
+            const f32x16_t sum = mfma_bf16(fb[d][j], va, acc[j]);
+            // (slices end at multiples of 16)
+            const bool take0 = mine == sid[d] && cb >= beg && cb < end;
+            const bool take1 = mine == sid[d] && cb + 16 >= beg && cb + 16 < end;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) acc[j][e] = take0 ? sum[e] : acc[j][e];
+#pragma unroll
+            for (int e = 8; e < 16; ++e) acc[j][e] = take1 ? sum[e] : acc[j][e];
+          }
+          fetch(d);
+        }
+      }
+    }
+  }
+}
+
 // ---- small M (decode batches): a deeper load pipeline ----
 // gemm_tn_kernel's two stages let a step's loads arrive during one step's
 // products, which at 64-row tiles are four to eight products: every step then
@@ -777,11 +854,11 @@ __global__ __launch_bounds__(kGemmThreads) void gemm_tn_ring_kernel(const uint16
 // stages (every path issues the same loads), drained before the epilogue.
 // (Graph-replayed, without an exit inside a loop trip: 37 x 12352 x 2048 11.2
 // -> 10.5 us, 128 rows 15.2 -> 14.4, 200 rows 21.9 -> 21.3.)
-template <int BN, int NS>
+template <int BN, int NS, bool kLora>
 __global__ __launch_bounds__(kGemmThreads, 2) void gemm_tn_deep_kernel(const uint16_t* __restrict__ A, int64_t lda,
                                                                     const uint16_t* __restrict__ B, int64_t ldb,
                                                                     GemmOut out, int M,
-                                                                    int N, int K, GemmGates gt) {
+                                                                    int N, int K, GemmGates gt, LoraArg<kLora> lo) {
   static_assert(NS == 3 || NS == 4, "three or four stages");
   constexpr int BM = 64, MI = 1, NJ = BN / 64;
   constexpr int kStage = (BM + BN) * 128;
@@ -867,6 +944,7 @@ __global__ __launch_bounds__(kGemmThreads, 2) void gemm_tn_deep_kernel(const uin
   issue(st0, 0);
   issue(st1, 1);
   if constexpr (NS == 4) issue(st2, 2);
+  if constexpr (kLora) lora_add32<NJ, 4>(lo, M, N, m0 + 32 * wm, n0 + (BN / 2) * wn, lane, acc[0]);
   // (no exit inside a trip: with one, the compiler's load counting merges its
   // states at the loop head and waits there for loads that are meant to stay
   // in flight)
@@ -902,8 +980,12 @@ namespace {
 
 // Tile choice and launch for C = A B^T into `out` (arguments checked by the
 // entry points).
+//
+// With adapters (kLora) the kernels with their products are fewer: the general one has none, and
+// what it would take goes to the kernel with 64-row tiles.
+template <bool kLora>
 int gemm_launch(const uint16_t* A, int64_t lda, const uint16_t* B, int64_t ldb, const GemmOut& out, int M, int N,
-                int K, const GemmGates& gt, void* stream) {
+                int K, const GemmGates& gt, const LoraArg<kLora>& lo, void* stream) {
   const int64_t nb256 = (N + 255) / 256;
   const int64_t t256 = ((M + 255) / 256) * nb256, t192 = ((M + 191) / 192) * nb256;
   const int64_t t128 = static_cast<int64_t>((M + 127) / 128) * ((N + 127) / 128);
@@ -932,15 +1014,15 @@ int gemm_launch(const uint16_t* A, int64_t lda, const uint16_t* B, int64_t ldb, 
   // 4096 x 512 7.7 -> 9.7; two rounds of blocks, 400 x 12352 x 2048 35.0 -> 38.1).
   const bool blocks = !wide && t128 <= kCUs && t64x128 > kCUs && 2 * t64x128 > 3 * t128 &&
                       K * t64x128 >= 1600 * kCUs;
-  if (K % (2 * kBK) == 0 && (wide ? !one192 : blocks)) {
+  if (K % (2 * kBK) == 0 && (wide ? kLora || !one192 : blocks)) {
     const int64_t rem = t256 % kCUs;
     const int64_t whole = rem <= kCUs / 2 ? t256 - rem : t256;
     const int64_t wgs = std::min<int64_t>(kCUs, whole ? std::max(whole, 4 * (t256 - whole)) : t128);
-    gemm_tn_pp_kernel<<<grid(wgs), dim3(kPPThreads), 0, st>>>(A, lda, B, ldb, out, M, N, K, gt,
-                                                              static_cast<int>(whole));
+    gemm_tn_pp_kernel<kLora><<<grid(wgs), dim3(kPPThreads), 0, st>>>(A, lda, B, ldb, out, M, N, K, gt,
+                                                                     static_cast<int>(whole), lo);
     return gdn_launch_status();
   }
-  if (wide) {
+  if (wide && !kLora) {
     // Odd multiples of 64, and one round of 192-row tiles: a launch runs in
     // ceil(tiles / CUs) waves of tiles, each taking time in proportion to the
     // tile's rows; 192 x 256 is taken when its waves x rows is smaller (a short
@@ -955,7 +1037,7 @@ int gemm_launch(const uint16_t* A, int64_t lda, const uint16_t* B, int64_t ldb, 
   // Small M.  The deeper load pipelines pay when K has at least 16 steps (with
   // fewer their prologue and the repeated last loads cost more than they save:
   // 1000 x 2080 x 512: 6.5 -> 7.0 us).
-  const bool deep = K / kBK >= 16;
+  const bool deep = kLora || K / kBK >= 16;
   // Ring tiles of 16, 32 or 64 rows x 32 columns, the smallest with at most one
   // workgroup per CU (with more, the 64-row tiles below move fewer bytes: 64 x
   // 12352 x 2048 11.2 us against 16-19; 500 x 2048 x 2048 13.7 against 13.9), and
@@ -970,23 +1052,23 @@ int gemm_launch(const uint16_t* A, int64_t lda, const uint16_t* B, int64_t ldb, 
   if (deep && rows <= (tall ? 32 : 64)) {
     const dim3 gr = grid((M + rows - 1) / rows * nb32);
     if (rows == 16)
-      gemm_tn_ring_kernel<16><<<gr, b3, 0, st>>>(A, lda, B, ldb, out, M, N, K, gt);
+      gemm_tn_ring_kernel<16, kLora><<<gr, b3, 0, st>>>(A, lda, B, ldb, out, M, N, K, gt, lo);
     else if (rows == 32)
-      gemm_tn_ring_kernel<32><<<gr, b3, 0, st>>>(A, lda, B, ldb, out, M, N, K, gt);
+      gemm_tn_ring_kernel<32, kLora><<<gr, b3, 0, st>>>(A, lda, B, ldb, out, M, N, K, gt, lo);
     else
-      gemm_tn_ring_kernel<64><<<gr, b3, 0, st>>>(A, lda, B, ldb, out, M, N, K, gt);
+      gemm_tn_ring_kernel<64, kLora><<<gr, b3, 0, st>>>(A, lda, B, ldb, out, M, N, K, gt, lo);
     return gdn_launch_status();
   }
   // 64 x 128 tiles, two or more workgroups per CU, spread the work over the
   // whole chip; 64 x 64 when even those would not.
   if (t64x128 >= kCUs / 2) {
     if (deep)
-      gemm_tn_deep_kernel<128, 3><<<grid(t64x128), b3, 0, st>>>(A, lda, B, ldb, out, M, N, K, gt);
+      gemm_tn_deep_kernel<128, 3, kLora><<<grid(t64x128), b3, 0, st>>>(A, lda, B, ldb, out, M, N, K, gt, lo);
     else
       gemm_tn_kernel<64, 128, 2><<<grid(t64x128), b3, 0, st>>>(A, lda, B, ldb, out, M, N, K, gt);
   } else {
     if (deep)
-      gemm_tn_deep_kernel<64, 4><<<grid(t64), b3, 0, st>>>(A, lda, B, ldb, out, M, N, K, gt);
+      gemm_tn_deep_kernel<64, 4, kLora><<<grid(t64), b3, 0, st>>>(A, lda, B, ldb, out, M, N, K, gt, lo);
     else
       gemm_tn_kernel<64, 64, 2><<<grid(t64), b3, 0, st>>>(A, lda, B, ldb, out, M, N, K, gt);
   }
@@ -1019,7 +1101,7 @@ extern "C" int gdn_gemm_bf16(const uint16_t* A, int64_t lda, const uint16_t* B, 
   const int v = ldc % 8 == 0;
   const GemmOut out{{C, C, C, C}, {ldc, ldc, ldc, ldc}, {N, N, N, N}, {v, v, v, v}};
   const GemmGates gt{g, beta, A_log, dt_bias, param_is_fp32 ? 1 : 0, gate_col, Hv};
-  return gemm_launch(A, lda, B, ldb, out, M, N, K, gt, stream);
+  return gemm_launch<false>(A, lda, B, ldb, out, M, N, K, gt, NoLora{}, stream);
 }
 
 extern "C" int gdn_gemm_bf16_cols(const uint16_t* A, int64_t lda, const uint16_t* B, int64_t ldb, int M, int N, int K,
@@ -1035,5 +1117,25 @@ extern "C" int gdn_gemm_bf16_cols(const uint16_t* A, int64_t lda, const uint16_t
   GemmOut out{};
   if (!parts_of(out, n_parts, C, ldc, col_end, N)) return GDN_ERR_INVALID_ARG;
   const GemmGates gt{g, beta, A_log, dt_bias, param_is_fp32 ? 1 : 0, gate_col, Hv};
-  return gemm_launch(A, lda, B, ldb, out, M, N, K, gt, stream);
+  return gemm_launch<false>(A, lda, B, ldb, out, M, N, K, gt, NoLora{}, stream);
+}
+
+extern "C" int gdn_gemm_bf16_lora(const uint16_t* A, int64_t lda, const uint16_t* B, int64_t ldb, int M, int N, int K,
+                                  int n_parts, uint16_t* const* C, const int64_t* ldc, const int* col_end, float* g,
+                                  uint16_t* beta, const void* A_log, const void* dt_bias, int param_is_fp32,
+                                  int gate_col, int Hv, const uint16_t* v, int64_t ldv, const uint16_t* lb,
+                                  int64_t lb_slot, const int32_t* ids, int slots, int rank, int slices,
+                                  const int* slice_end, void* stream) {
+  if (M < 0 || N < 0 || K < 0 || n_parts < 1 || n_parts > kMaxParts || !C || !ldc || !col_end)
+    return GDN_ERR_INVALID_ARG;
+  if (M == 0 || N == 0) return GDN_OK;
+  if (!A || !B) return GDN_ERR_INVALID_ARG;
+  const int st = gemm_check(A, lda, B, ldb, M, N, K, g, beta, A_log, dt_bias, gate_col, Hv);
+  if (st != GDN_OK) return st;
+  GemmOut out{};
+  if (!parts_of(out, n_parts, C, ldc, col_end, N)) return GDN_ERR_INVALID_ARG;
+  Lora lo{};
+  if (!lora_of(lo, v, ldv, lb, lb_slot, ids, slots, rank, slices, slice_end, M, N)) return GDN_ERR_INVALID_ARG;
+  const GemmGates gt{g, beta, A_log, dt_bias, param_is_fp32 ? 1 : 0, gate_col, Hv};
+  return gemm_launch<true>(A, lda, B, ldb, out, M, N, K, gt, lo, stream);
 }

@@ -26,6 +26,7 @@
 #include <utility>
 
 #include "gemm_tile.h"
+#include "lora_tile.h"
 #include "quant_fp8.h"
 
 namespace {
@@ -83,11 +84,11 @@ __device__ __forceinline__ void dma4(__amdgpu_buffer_rsrc_t rsrc, void* lds, int
 }
 
 // kOdd: K is an odd number of steps.
-template <bool kOdd>
+template <bool kOdd, bool kLora>
 __global__ __launch_bounds__(kPPThreads, 2) void gemm_fp8_pp_kernel(const uint8_t* __restrict__ A, int64_t lda,
                                                                     const uint8_t* __restrict__ B, int64_t ldb,
                                                                     Fp8Scales sc, GemmOut out, int M, int N, int K,
-                                                                    int whole) {
+                                                                    int whole, LoraArg<kLora> lo) {
   constexpr int kHalf = 128 * 128;  // bytes of a half tile
   __shared__ __align__(16) uint8_t a00[kHalf];
   __shared__ __align__(16) uint8_t a01[kHalf];
@@ -305,6 +306,14 @@ __global__ __launch_bounds__(kPPThreads, 2) void gemm_fp8_pp_kernel(const uint8_
       }
       if (!wm) half_barrier();
       const int lane_e = new_lane();
+      if constexpr (kLora) {
+#pragma unroll
+        for (int a = 0; a < 2; ++a) {
+          const int cb[2] = {n0c + 32 * wn, n0c + 128 + 32 * wn};
+          lora_add<4, 2, 1>(lo, M, N, m0c + 128 * a + 64 * wm, cb, lane_e, 0, 1,
+                            [&](int i, int j, int t) -> gdn::f32x4_t& { return acc[a][j][i][t]; });
+        }
+      }
 #pragma unroll
       for (int a = 0; a < 2; ++a)
 #pragma unroll
@@ -391,6 +400,11 @@ __global__ __launch_bounds__(kPPThreads, 2) void gemm_fp8_pp_kernel(const uint8_
       step(a11, b11, sc3, a10, b10, sc2, s + 3);
     }
     if (!wm) half_barrier();
+    if constexpr (kLora) {
+      const int cb[1] = {n0 + 32 * wn};
+      lora_add<4, 1, 2>(lo, M, N, m0 + 64 * wm, cb, new_lane(), 0, 1,
+                        [&](int i, int, int t) -> gdn::f32x4_t& { return c[i][t]; });
+    }
 #pragma unroll
     for (int i = 0; i < 4; ++i)
       gemm_store16<true>(c[i][0], c[i][1], out, M, N, m0 + 64 * wm + 16 * i, n0 + 32 * wn, new_lane(), GemmGates{}, nullptr);
@@ -557,11 +571,11 @@ __device__ __forceinline__ void ring_store(const gdn::f32x4_t (&acc)[MT][NT][2],
 // magnitude over the four lanes that share the row: no launch of its own and nothing
 // written.  Every workgroup repeats it for its rows, so it is for few of them (fewer still:
 // gemm_fp8_rows_kernel).
-template <int BM, int BN, int NW, int NS, bool kQuant>
+template <int BM, int BN, int NW, int NS, bool kQuant, bool kLora>
 __global__ __launch_bounds__(64 * NW) void gemm_fp8_ring_kernel(const void* __restrict__ A, int64_t lda,
                                                                 const uint8_t* __restrict__ B, int64_t ldb,
                                                                 Fp8Scales sc, GemmOut out, int M, int N, int K,
-                                                                Fp8Wide wide) {
+                                                                Fp8Wide wide, LoraArg<kLora> lo) {
   constexpr int MT = BM / 16, NT = BN / 32;
   constexpr int kARow = kQuant ? 256 : 128;               // bytes of a row of A in LDS
   constexpr int kABytes = BM * kARow, kBBytes = BN * 128;
@@ -719,6 +733,13 @@ __global__ __launch_bounds__(64 * NW) void gemm_fp8_ring_kernel(const void* __re
   issue(st0, wave);
   issue(st1, wave + NW);
   if constexpr (NS == 3) issue(st2, wave + 2 * NW);
+  if constexpr (kLora) {
+    int cb[NT];
+#pragma unroll
+    for (int j = 0; j < NT; ++j) cb[j] = n0 + 32 * j;
+    lora_add<MT, NT, 4>(lo, M, N, m0, cb, lane, wave, NW,
+                        [&](int i, int j, int t) -> gdn::f32x4_t& { return acc[i][j][t]; });
+  }
   __builtin_amdgcn_s_waitcnt(kWait);
   int s = wave;
   for (; s + (NS - 1) * NW < nk; s += NS * NW) {
@@ -917,11 +938,11 @@ __global__ __launch_bounds__(64 * NW) void gemm_fp8_rows_kernel(const uint16_t* 
 // half of the K-steps (kOdd: one past the last repeats it with scale 0), which puts twice the
 // loads in flight where a CU has one tile; the second's sums
 // are added to the first's through LDS.
-template <int BN, int NS, int H, bool kOdd>
+template <int BN, int NS, int H, bool kOdd, bool kLora>
 __global__ __launch_bounds__(kFp8Threads * H, 2) void gemm_fp8_deep_kernel(const uint8_t* __restrict__ A, int64_t lda,
                                                                        const uint8_t* __restrict__ B, int64_t ldb,
                                                                        Fp8Scales sc, GemmOut out, int M, int N,
-                                                                       int K) {
+                                                                       int K, LoraArg<kLora> lo) {
   static_assert(NS == 3 || NS == 4, "three or four stages");
   constexpr int BM = 64, NJ = BN / 64;  // column pairs of 32 per wave
   constexpr int kStage = (BM + BN) * 128 + 1024;
@@ -1022,6 +1043,13 @@ __global__ __launch_bounds__(kFp8Threads * H, 2) void gemm_fp8_deep_kernel(const
   issue(st0, 0);
   issue(st1, 1);
   if constexpr (NS == 4) issue(st2, 2);
+  if constexpr (kLora) {
+    int cb[NJ];
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) cb[j] = n0 + 32 * (NJ * wn + j);
+    lora_add<2, NJ, 4>(lo, M, N, m0 + 32 * wm, cb, lane, half, H,
+                       [&](int i, int j, int t) -> gdn::f32x4_t& { return acc[i][j][t]; });
+  }
   // (no exit inside a trip: the compiler's load counting would merge its states at the
   // loop head and wait there for loads that are meant to stay in flight)
   int s = 0;
@@ -1130,10 +1158,18 @@ Fp8Kernel fp8_plan(int M, int N, int K, bool quant) {
 // reads its rows again).
 constexpr int kWideRows = 1024;
 
+template <bool kWant, class T>
+LoraArg<kWant> ring_arg(const T& lo) {
+  if constexpr (kWant) return lo;
+  else return {};
+}
+
 bool fp8_quantizes(Fp8Kernel k) { return k >= kRingQ16x32; }
 
+// kLora: e4m3 rows.
+template <bool kLora>
 int fp8_launch(Fp8Kernel kernel, const void* A, int64_t lda, const uint8_t* B, int64_t ldb, const Fp8Scales& sc,
-               const GemmOut& out, int M, int N, int K, const Fp8Wide& wide, hipStream_t st) {
+               const GemmOut& out, int M, int N, int K, const Fp8Wide& wide, const LoraArg<kLora>& lo, hipStream_t st) {
   auto blocks = [&](int bm, int bn) { return static_cast<int64_t>((M + bm - 1) / bm) * ((N + bn - 1) / bn); };
   auto grid = [](int64_t wgs) {
     return dim3(static_cast<unsigned>(gdn::kNumXcd * ((wgs + gdn::kNumXcd - 1) / gdn::kNumXcd)));
@@ -1148,21 +1184,23 @@ int fp8_launch(Fp8Kernel kernel, const void* A, int64_t lda, const uint8_t* B, i
       const int64_t t256 = blocks(256, 256), rem = t256 % kCUs8;
       const int64_t whole = rem <= kCUs8 / 2 ? t256 - rem : t256;
       const int64_t wgs = std::min<int64_t>(kCUs8, whole ? std::max(whole, 4 * (t256 - whole)) : blocks(128, 128));
-      auto pp = K / gdn::kFp8Group % 2 ? gemm_fp8_pp_kernel<true> : gemm_fp8_pp_kernel<false>;
-      pp<<<grid(wgs), dim3(kPPThreads), 0, st>>>(A8, lda, B, ldb, sc, out, M, N, K, static_cast<int>(whole));
+      auto pp = K / gdn::kFp8Group % 2 ? gemm_fp8_pp_kernel<true, kLora> : gemm_fp8_pp_kernel<false, kLora>;
+      pp<<<grid(wgs), dim3(kPPThreads), 0, st>>>(A8, lda, B, ldb, sc, out, M, N, K, static_cast<int>(whole), lo);
       break;
     }
 #define GDN_DEEP(BN, NS, H, odd)                                                                                        \
-  gemm_fp8_deep_kernel<BN, NS, H, odd><<<grid(blocks(64, BN)), dim3(kFp8Threads * H), 0, st>>>(A8, lda, B, ldb, sc, out, \
-                                                                                               M, N, K)
+  gemm_fp8_deep_kernel<BN, NS, H, odd, kLora><<<grid(blocks(64, BN)), dim3(kFp8Threads * H), 0, st>>>(A8, lda, B, ldb,   \
+                                                                                                      sc, out, M, N, K, \
+                                                                                                      lo)
     case kDeep64: GDN_DEEP(64, 4, 1, false); break;
     case kDeep128: GDN_DEEP(128, 3, 1, false); break;
     case kDeep64x2: K / gdn::kFp8Group % 2 ? GDN_DEEP(64, 4, 2, true) : GDN_DEEP(64, 4, 2, false); break;
 #undef GDN_DEEP
 #define GDN_RING(name, BM, BN, NW, NS, Q)                                                                            \
   case name:                                                                                                         \
-    gemm_fp8_ring_kernel<BM, BN, NW, NS, Q>                                                                          \
-        <<<Q ? rows_grid(BN) : grid(blocks(BM, BN)), dim3(64 * NW), 0, st>>>(A, lda, B, ldb, sc, out, M, N, K, wide); \
+    gemm_fp8_ring_kernel<BM, BN, NW, NS, Q, kLora && !Q>                                                             \
+        <<<Q ? rows_grid(BN) : grid(blocks(BM, BN)), dim3(64 * NW), 0, st>>>(A, lda, B, ldb, sc, out, M, N, K, wide,  \
+                                                                             ring_arg<kLora && !Q>(lo));             \
     break
       GDN_RING(kRing16x32, 16, 32, 8, 2, false);
       GDN_RING(kRing16x64, 16, 64, 4, 3, false);
@@ -1191,6 +1229,19 @@ int fp8_launch(Fp8Kernel kernel, const void* A, int64_t lda, const uint8_t* B, i
   return gdn_launch_status();
 }
 
+// K in whole groups; 16-byte row pieces of A and B; 32-bit buffer offsets.
+bool fp8_operands_ok(const void* A, bool a_is_bf16, int64_t lda, int64_t sa_row, int64_t sa_grp, const uint8_t* B,
+                     int64_t ldb, int64_t sb_row, int M, int N, int K) {
+  const int64_t kLimit = 1LL << 31;
+  const int64_t groups = K / gdn::kFp8Group;
+  if (K == 0 || K % gdn::kFp8Group || lda % (a_is_bf16 ? 8 : 16) || ldb % 16 || lda < K || ldb < K ||
+      reinterpret_cast<uintptr_t>(A) % 16 || reinterpret_cast<uintptr_t>(B) % 16 ||
+      M * lda * (a_is_bf16 ? 2 : 1) >= kLimit || N * ldb >= kLimit || sb_row < groups ||
+      4 * ((N + 127) / 128 * sb_row) >= kLimit)
+    return false;
+  return a_is_bf16 || (sa_row >= 0 && sa_grp >= 0 && 4 * ((M - 1) * sa_row + (groups - 1) * sa_grp) < kLimit);
+}
+
 }  // namespace
 
 // x's rows in e4m3 and their scales, of a call from bf16 rows that no kernel above quantizes itself.
@@ -1209,16 +1260,8 @@ extern "C" int gdn_gemm_fp8(const void* A, int a_is_bf16, int64_t lda, const flo
     return GDN_ERR_INVALID_ARG;
   if (M == 0 || N == 0) return GDN_OK;
   if (!A || !B || !sb || (!a_is_bf16 && !sa)) return GDN_ERR_INVALID_ARG;
-  // K in whole groups; 16-byte row pieces of A and B; 32-bit buffer offsets
-  const int64_t kLimit = 1LL << 31;
-  const int64_t groups = K / gdn::kFp8Group;
-  if (K == 0 || K % gdn::kFp8Group || lda % (a_is_bf16 ? 8 : 16) || ldb % 16 || lda < K || ldb < K ||
-      reinterpret_cast<uintptr_t>(A) % 16 || reinterpret_cast<uintptr_t>(B) % 16 ||
-      M * lda * (a_is_bf16 ? 2 : 1) >= kLimit || N * ldb >= kLimit || sb_row < groups ||
-      4 * ((N + 127) / 128 * sb_row) >= kLimit)
-    return GDN_ERR_INVALID_ARG;
-  if (!a_is_bf16 && (sa_row < 0 || sa_grp < 0 || 4 * ((M - 1) * sa_row + (groups - 1) * sa_grp) >= kLimit))
-    return GDN_ERR_INVALID_ARG;
+  if (!fp8_operands_ok(A, a_is_bf16 != 0, lda, sa_row, sa_grp, B, ldb, sb_row, M, N, K)) return GDN_ERR_INVALID_ARG;
+  const int64_t kLimit = 1LL << 31, groups = K / gdn::kFp8Group;
   GemmOut out{};
   if (!parts_of(out, n_parts, C, ldc, col_end, N + N2, true)) return GDN_ERR_INVALID_ARG;
   int first = n_parts;  // the first part of the bf16 columns
@@ -1263,5 +1306,24 @@ extern "C" int gdn_gemm_fp8(const void* A, int a_is_bf16, int64_t lda, const flo
     sa_row = 1;
     sa_grp = M;
   }
-  return fp8_launch(kernel, A, lda, B, ldb, Fp8Scales{sa, sa_row, sa_grp, sb, sb_row}, out, M, N, K, wide, st);
+  return fp8_launch<false>(kernel, A, lda, B, ldb, Fp8Scales{sa, sa_row, sa_grp, sb, sb_row}, out, M, N, K, wide,
+                           NoLora{}, st);
+}
+
+extern "C" int gdn_gemm_fp8_lora(const uint8_t* A, int64_t lda, const float* sa, int64_t sa_row, int64_t sa_grp,
+                                 const uint8_t* B, int64_t ldb, const float* sb, int64_t sb_row, int M, int N, int K,
+                                 int n_parts, uint16_t* const* C, const int64_t* ldc, const int* col_end,
+                                 const uint16_t* v, int64_t ldv, const uint16_t* lb, int64_t lb_slot, const int32_t* ids,
+                                 int slots, int rank, int slices, const int* slice_end, void* stream) {
+  if (M < 0 || N < 0 || K < 0 || n_parts < 1 || n_parts > kMaxParts || !C || !ldc || !col_end)
+    return GDN_ERR_INVALID_ARG;
+  if (M == 0 || N == 0) return GDN_OK;
+  if (!A || !B || !sb || !sa || !fp8_operands_ok(A, false, lda, sa_row, sa_grp, B, ldb, sb_row, M, N, K))
+    return GDN_ERR_INVALID_ARG;
+  GemmOut out{};
+  if (!parts_of(out, n_parts, C, ldc, col_end, N, true)) return GDN_ERR_INVALID_ARG;
+  Lora lo{};
+  if (!lora_of(lo, v, ldv, lb, lb_slot, ids, slots, rank, slices, slice_end, M, N)) return GDN_ERR_INVALID_ARG;
+  return fp8_launch<true>(fp8_plan(M, N, K, false), A, lda, B, ldb, Fp8Scales{sa, sa_row, sa_grp, sb, sb_row}, out, M, N,
+                          K, Fp8Wide{}, lo, static_cast<hipStream_t>(stream));
 }

@@ -1,0 +1,265 @@
+// The first half of low-rank adapters beside a projection: the rows shrunk to their adapters'
+// rank, v[m][j] = scale_s sum over k of x[m][k] A_s[j][k], s = ids[m] the row's adapter (none
+// outside of 0 .. slots - 1: nothing is written for the row), j over the slices' ranks one
+// after the other.  The GEMMs take v from there (lora_tile.h).  No counterpart in the
+// reference.
+//
+// v is summed in fp32 and held as two bf16 values, high and low part (2^-16 of it is lost): one
+// would cost the result as much again as its own rounding where an adapter's share is as large
+// as the projection's.
+//
+// A workgroup has 16 MT rows and 16 NT of the columns j.  It goes through the adapters of its
+// rows, each once: all rows times the adapter's A, K-steps dealt to the waves, each with a ring of
+// NS stages of its own in LDS that loads fill directly (as in the GEMM's ring kernel), the
+// waves' sums added in wave order, and the rows that have the adapter stored.  With gridDim.y > 1
+// workgroups share a tile's adapters: few rows, most of them with adapters of their own, are
+// bound by the reading of A and want it spread over the chip; a prompt's tile has one.
+//
+// x comes in bf16 (steps of 64 values) or in e4m3 with a scale for each row and 128 columns
+// (steps of 128): e4m3 values are bf16 ones, so a group's sum is the matrix cores' and the
+// scale is applied to it in fp32.
+#include <algorithm>
+
+#include "lora_tile.h"
+
+namespace {
+
+typedef int i32x2_t __attribute__((ext_vector_type(2)));
+
+struct Shrink {
+  const void* x;
+  int64_t ldx;
+  const float* xs;  // kFp8: scale of row m, group g at xs[m xs_row + g xs_grp]
+  int64_t xs_row, xs_grp;
+  const uint16_t* a;  // [slots][cols, K] bf16
+  int64_t a_slot;
+  const float* scale;  // [slots]
+  const int* ids;
+  int slots, cols, rank, M, K;
+  uint16_t* v;
+  int64_t ldv;
+};
+
+// 8 e4m3 values as bf16
+__device__ __forceinline__ gdn::s16x8_t e4m3_to_bf16(const i32x2_t& w) {
+  typedef float f2 __attribute__((ext_vector_type(2)));
+  uint32_t d[4];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const f2 lo = __builtin_amdgcn_cvt_pk_f32_fp8(w[i], false), hi = __builtin_amdgcn_cvt_pk_f32_fp8(w[i], true);
+    d[2 * i] = gdn::f2bf2(lo[0], lo[1]);
+    d[2 * i + 1] = gdn::f2bf2(hi[0], hi[1]);
+  }
+  typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+  return __builtin_bit_cast(gdn::s16x8_t, u4{d[0], d[1], d[2], d[3]});
+}
+
+template <int MT, int NT, int NW, int NS, bool kFp8>
+__global__ __launch_bounds__(64 * NW) void lora_shrink_kernel(Shrink p) {
+  constexpr int BM = 16 * MT, BN = 16 * NT;
+  constexpr int kStep = kFp8 ? 128 : 64;                   // values of a K-step
+  constexpr int kHalves = kFp8 ? 2 : 1;                    // 128-byte rows of A in it
+  constexpr int kXBytes = BM * 128, kABytes = BN * 128;    // (of one half)
+  constexpr int kStage = kXBytes + kHalves * kABytes + (kFp8 ? 256 : 0);
+  constexpr int kXPer = kXBytes / 1024, kAPer = kABytes / 1024;
+  constexpr int kPer = kXPer + kHalves * kAPer + (kFp8 ? 1 : 0);
+  constexpr int kVm = (NS - 1) * kPer;
+  static_assert(kVm < 64 && (NS == 2 || NS == 3), "vmcnt field");
+  constexpr int kWait = (kVm & 15) | (7 << 4) | (15 << 8) | ((kVm >> 4) << 14);
+  static_assert(MT * NT * 1024 <= kStage, "the partial sums fit a stage");
+  __shared__ __align__(16) uint8_t st0[NW * kStage];
+  __shared__ __align__(16) uint8_t st1[NW * kStage];
+  __shared__ __align__(16) uint8_t st2[NS > 2 ? NW * kStage : 16];
+  const int tiles_n = (p.cols + BN - 1) / BN;
+  const int m0 = BM * static_cast<int>(blockIdx.x / tiles_n), c0 = BN * static_cast<int>(blockIdx.x % tiles_n);
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lr = lane & 15, lg = lane >> 4;
+  int id[MT];
+#pragma unroll
+  for (int i = 0; i < MT; ++i) {
+    const int r = m0 + 16 * i + lr;
+    const int s = p.ids[min(r, p.M - 1)];
+    id[i] = r < p.M && static_cast<unsigned>(s) < static_cast<unsigned>(p.slots) ? s : -1;
+  }
+  int mine = BM > lane ? id[0] : -1;  // row m0 + lane's
+#pragma unroll
+  for (int i = 1; i < MT; ++i) mine = lg == i ? id[i] : mine;
+  LoraIds it{__ballot(mine >= 0), static_cast<int>(blockIdx.y), static_cast<int>(gridDim.y), 0};
+  int s = it.next(mine);
+  if (s < 0) return;  // (the workgroup)
+
+  const __amdgpu_buffer_rsrc_t rx = rsrc_of(p.x), rs = rsrc_of(p.xs);
+  int goff[kXPer + kAPer];
+#pragma unroll
+  for (int i = 0; i < kXPer + kAPer; ++i) {
+    const int r = 8 * (i < kXPer ? i : i - kXPer) + (lane >> 3);
+    const int gran = 16 * ((lane & 7) ^ ((r >> 1) & 7));
+    goff[i] = i < kXPer ? static_cast<int>(min(m0 + r, p.M - 1) * p.ldx * (kFp8 ? 1 : 2)) + gran
+                        : min(c0 + r, p.cols - 1) * p.K * 2 + gran;
+  }
+  const int vs = kFp8 ? static_cast<int>(min(m0 + lane % BM, p.M - 1) * p.xs_row * 4) : 0;
+  const int nk = p.K / kStep;
+  while (s >= 0) {
+    const __amdgpu_buffer_rsrc_t ra = rsrc_of(p.a + s * p.a_slot);
+    auto issue = [&](uint8_t* st, int step) {
+      const int k = min(step, nk - 1);
+      uint8_t* w = st + wave * kStage;
+#pragma unroll
+      for (int i = 0; i < kXPer; ++i) dma16(rx, w + i * 1024, goff[i], 128 * k);
+#pragma unroll
+      for (int h = 0; h < kHalves; ++h)
+#pragma unroll
+        for (int i = 0; i < kAPer; ++i)
+          dma16(ra, w + kXBytes + h * kABytes + i * 1024, goff[kXPer + i], 128 * (kHalves * k + h));
+      if constexpr (kFp8)
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_ptr_t)(w + kXBytes + kHalves * kABytes), 4, vs,
+                                                 static_cast<int>(p.xs_grp) * 4 * k, 0, 0);
+    };
+    gdn::f32x4_t acc[MT][NT];
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+      for (int j = 0; j < NT; ++j) acc[i][j] = gdn::f32x4_t{0.f, 0.f, 0.f, 0.f};
+    auto one = [&](uint8_t* st, int step) {
+      const uint8_t* x = st + wave * kStage;
+      const uint8_t* a = x + kXBytes;
+      constexpr int kSub = kStep / 32;
+      gdn::s16x8_t fa[kSub][NT];
+      gdn::s16x8_t fx[kSub][MT];
+      float f[MT];
+#pragma unroll
+      for (int ks = 0; ks < kSub; ++ks) {
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+          const int r = 16 * i + lr;
+          if constexpr (kFp8)
+            fx[ks][i] = e4m3_to_bf16(*reinterpret_cast<const i32x2_t*>(x + sw_off(r, 2 * ks + (lg >> 1)) + 8 * (lg & 1)));
+          else
+            fx[ks][i] = *reinterpret_cast<const gdn::s16x8_t*>(x + sw_off(r, 4 * ks + lg));
+        }
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+          fa[ks][j] = *reinterpret_cast<const gdn::s16x8_t*>(a + (ks >> 1) * kABytes + sw_off(16 * j + lr, 4 * (ks & 1) + lg));
+      }
+      if constexpr (kFp8)
+#pragma unroll
+        for (int i = 0; i < MT; ++i) f[i] = reinterpret_cast<const float*>(a + kHalves * kABytes)[16 * i + lr];
+      // the reads have returned before the stage is loaded again
+      __builtin_amdgcn_sched_barrier(0);
+      __builtin_amdgcn_s_waitcnt(kWaitLds);
+      __builtin_amdgcn_sched_barrier(0);
+      issue(st, step + NS * NW);
+#pragma unroll
+      for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+          gdn::f32x4_t sum = kFp8 ? gdn::f32x4_t{0.f, 0.f, 0.f, 0.f} : acc[i][j];
+#pragma unroll
+          for (int ks = 0; ks < kSub; ++ks) sum = gdn::mfma16x16x32(fa[ks][j], fx[ks][i], sum);
+          if constexpr (kFp8) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[i][j][e] = fmaf(sum[e], f[i], acc[i][j][e]);
+          } else {
+            acc[i][j] = sum;
+          }
+        }
+      __builtin_amdgcn_sched_barrier(0);
+      __builtin_amdgcn_s_waitcnt(kWait);
+      __builtin_amdgcn_sched_barrier(0);
+    };
+    issue(st0, wave);
+    issue(st1, wave + NW);
+    if constexpr (NS == 3) issue(st2, wave + 2 * NW);
+    __builtin_amdgcn_s_waitcnt(kWait);
+    int k = wave;
+    for (; k + (NS - 1) * NW < nk; k += NS * NW) {
+      one(st0, k);
+      one(st1, k + NW);
+      if constexpr (NS == 3) one(st2, k + 2 * NW);
+    }
+    if (k < nk) one(st0, k);
+    if (NS == 3 && k + NW < nk) one(st1, k + NW);
+    // the repeated loads past the last step land before the stages are reused
+    __builtin_amdgcn_s_waitcnt(0);
+    __syncthreads();
+    gdn::f32x4_t* red = reinterpret_cast<gdn::f32x4_t*>(st0);  // [wave][row tile][column tile][lane]
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+      for (int j = 0; j < NT; ++j) red[((wave * MT + i) * NT + j) * 64 + lane] = acc[i][j];
+    __syncthreads();
+    const float scale = p.scale[s];
+#pragma unroll
+    for (int ij = 0; ij < MT * NT; ++ij) {
+      if (ij % NW != wave) continue;
+      const int i = ij / NT, j = ij % NT;
+      gdn::f32x4_t sum = red[ij * 64 + lane];
+#pragma unroll
+      for (int w = 1; w < NW; ++w) sum += red[(w * MT * NT + ij) * 64 + lane];
+      // columns c .. c + 3 of row m0 + 16 i + lr (a slice's ranks are a multiple of 8)
+      const int c = c0 + 16 * j + 4 * lg;
+      if (id[i] != s || c >= p.cols) continue;
+      float hi[4], lo[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float val = sum[e] * scale;
+        hi[e] = gdn::bf2f(gdn::f2bf(val));
+        // (what bf16 does not hold is infinite in the one part and has none in the other)
+        lo[e] = fabsf(hi[e]) < __builtin_inff() ? val - hi[e] : 0.0f;
+      }
+      const int slice = c / p.rank;
+      uint16_t* at = p.v + static_cast<int64_t>(m0 + 16 * i + lr) * p.ldv + slice * p.rank + c;
+      *reinterpret_cast<uint2*>(at) = make_uint2(gdn::f2bf2(hi[0], hi[1]), gdn::f2bf2(hi[2], hi[3]));
+      *reinterpret_cast<uint2*>(at + p.rank) = make_uint2(gdn::f2bf2(lo[0], lo[1]), gdn::f2bf2(lo[2], lo[3]));
+    }
+    s = it.next(mine);
+    if (s >= 0) __syncthreads();  // the sums have been read
+  }
+}
+
+template <bool kFp8>
+int launch(const Shrink& p, hipStream_t st) {
+  auto tiles = [](int n, int of) { return (n + of - 1) / of; };
+  // one wave's rows: prompts fill the chip with 64-row tiles
+  if (p.M > 2048) {
+    const int nt = tiles(p.cols, p.cols > 32 ? 64 : 32);
+    const dim3 grid(static_cast<unsigned>(tiles(p.M, 64) * nt));
+    if (p.cols > 32)
+      lora_shrink_kernel<4, 4, kFp8 ? 2 : 4, 2, kFp8><<<grid, dim3(kFp8 ? 128 : 256), 0, st>>>(p);
+    else
+      lora_shrink_kernel<4, 2, 4, 2, kFp8><<<grid, dim3(256), 0, st>>>(p);
+    return gdn_launch_status();
+  }
+  const int t = tiles(p.M, 16) * tiles(p.cols, 16);
+  // a tile's adapters over so many workgroups (those that find none end)
+  const int share = std::max(1, std::min(std::min(16, p.M), 1024 / t));
+  lora_shrink_kernel<1, 1, 8, 3, kFp8><<<dim3(static_cast<unsigned>(t), static_cast<unsigned>(share)), dim3(512), 0, st>>>(p);
+  return gdn_launch_status();
+}
+
+}  // namespace
+
+extern "C" int gdn_lora_shrink(const void* x, int x_is_bf16, int64_t ldx, const float* xs, int64_t xs_row, int64_t xs_grp,
+                               const uint16_t* a, int64_t a_slot, const float* scale, const int32_t* ids, int slots,
+                               int slices, int rank, int M, int K, uint16_t* v, int64_t ldv, void* stream) {
+  const int64_t kLimit = 1LL << 31;
+  if (M < 0 || slots < 0 || slices < 1 || slices > kMaxParts || rank < 8 || rank > kMaxRank || rank % 8 || K <= 0 ||
+      K % (x_is_bf16 ? 64 : gdn::kFp8Group))
+    return GDN_ERR_INVALID_ARG;
+  if (M == 0 || slots == 0) return GDN_OK;
+  const int cols = slices * rank;
+  if (!x || !a || !scale || !ids || !v || (!x_is_bf16 && !xs)) return GDN_ERR_INVALID_ARG;
+  if (reinterpret_cast<uintptr_t>(x) % 16 || reinterpret_cast<uintptr_t>(a) % 16 || reinterpret_cast<uintptr_t>(v) % 8 ||
+      reinterpret_cast<uintptr_t>(scale) % 4 || reinterpret_cast<uintptr_t>(ids) % 4 || ldx < K ||
+      ldx % (x_is_bf16 ? 8 : 16) || M * ldx * (x_is_bf16 ? 2 : 1) >= kLimit || a_slot % 8 ||
+      (slots > 1 && a_slot < static_cast<int64_t>(cols) * K) || static_cast<int64_t>(cols) * K * 2 >= kLimit ||
+      ldv % 4 || ldv < 2LL * cols)
+    return GDN_ERR_INVALID_ARG;
+  if (!x_is_bf16 && (reinterpret_cast<uintptr_t>(xs) % 4 || xs_row < 0 || xs_grp < 0 ||
+                     4 * ((M - 1) * xs_row + (K / gdn::kFp8Group - 1) * xs_grp) >= kLimit))
+    return GDN_ERR_INVALID_ARG;
+  const Shrink p{x, ldx, xs, xs_row, xs_grp, a, a_slot, scale, ids, slots, cols, rank, M, K, v, ldv};
+  const hipStream_t st = static_cast<hipStream_t>(stream);
+  return x_is_bf16 ? launch<false>(p, st) : launch<true>(p, st);
+}

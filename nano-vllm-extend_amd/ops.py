@@ -1509,6 +1509,371 @@ def linear_fp8_cols(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.T
     return parts if x.dim() == 2 else [p.view(*x.shape[:-1], p.shape[1]) for p in parts]
 
 
+# ------------------------------------------------------ low-rank adapters --
+LORA_MAX_RANK = 256
+
+
+class LoraPool:
+    """The low-rank adapters of one projection, or of several side by side, that are
+    loaded together: slot s adds scale[s] * (x A_s^T) B_s^T to the rows that name it.
+
+    widths: the columns of each projection (1 to 4 of them, boundaries at multiples of
+    16), each with an A of its own.  a [slots, len(widths) * rank, in_features] bf16, b
+    [slots, sum(widths), rank] bf16 and scale [slots] fp32 are laid out once and filled
+    in place (captured graphs see an adapter that is loaded later); `rank` is brought up
+    to a multiple of 8, and adapters of a smaller one are padded with zeros."""
+
+    def __init__(self, slots: int, rank: int, in_features: int, widths: list[int], device="cuda"):
+        self.widths, self.in_features = list(widths), in_features
+        self.rank = -(-rank // 8) * 8
+        if slots < 0 or not 1 <= rank <= LORA_MAX_RANK:
+            raise ValueError(f"slots = {slots} (0 or more) and rank = {rank} (1 to {LORA_MAX_RANK})")
+        if not 1 <= len(self.widths) <= 4 or min(self.widths) <= 0 or any(w % 16 for w in self.widths[:-1]):
+            raise ValueError(f"widths {widths}: 1 to 4 projections, boundaries at multiples of 16")
+        self.a = torch.zeros(slots, len(self.widths) * self.rank, in_features, dtype=torch.bfloat16, device=device)
+        self.b = torch.zeros(slots, sum(self.widths), self.rank, dtype=torch.bfloat16, device=device)
+        self.scale = torch.zeros(slots, dtype=torch.float32, device=device)
+
+    def load(self, slot: int, parts, scale: float) -> None:
+        """An adapter into a slot: for each projection (A [r, in_features], B [width, r]),
+        r at most the pool's rank, or None where the adapter has nothing for it; scale as
+        the checkpoint defines it (alpha / r)."""
+        if not 0 <= slot < self.a.shape[0]:
+            raise ValueError(f"slot {slot} of {self.a.shape[0]}")
+        if len(parts) != len(self.widths):
+            raise ValueError(f"{len(parts)} parts for {len(self.widths)} projections")
+        for part, width in zip(parts, self.widths):
+            if part is not None:
+                r = part[0].shape[0]
+                if r > self.rank or part[0].shape != (r, self.in_features) or part[1].shape != (width, r):
+                    raise ValueError(f"A must be [r, {self.in_features}] and B [{width}, r] with r <= {self.rank}, got "
+                                     f"{list(part[0].shape)} and {list(part[1].shape)}")
+        self.clear(slot)
+        col = 0
+        for p, (part, width) in enumerate(zip(parts, self.widths)):
+            if part is not None:
+                r = part[0].shape[0]
+                self.a[slot, p * self.rank:p * self.rank + r].copy_(part[0])
+                self.b[slot, col:col + width, :r].copy_(part[1])
+            col += width
+        self.scale[slot] = scale
+
+    def clear(self, slot: int) -> None:
+        """An empty adapter (its rows get the projection alone)."""
+        self.a[slot].zero_()
+        self.b[slot].zero_()
+        self.scale[slot] = 0.0
+
+
+def adapter_rows(adapters: torch.Tensor, cu_seqlens: torch.Tensor, rows: int) -> torch.Tensor:
+    """The adapter of each of `rows` rows, int32 [rows], from those of the sequences,
+    adapters [n] (-1: none), and the sequences' offsets cu_seqlens [n + 1] (device; the
+    last one is `rows`): once per step, for all of its layers."""
+    lens = cu_seqlens[1:] - cu_seqlens[:-1]
+    return adapters.to(torch.int32).repeat_interleave(lens, output_size=rows)
+
+
+def _lora_check(x, N, K, widths, lora_a, lora_b, lora_scale, ids):
+    """The adapters' shapes beside a product with N columns: (M, P, R)."""
+    M = x.numel() // K
+    P = len(widths)
+    if not 1 <= P <= 4 or sum(widths) != N or min(widths) <= 0 or any(w % 16 for w in widths[:-1]):
+        raise ValueError(f"widths {list(widths)}: 1 to 4 parts of {N} columns, boundaries at multiples of 16")
+    for t, nm in ((lora_a, "lora_a"), (lora_b, "lora_b")):
+        _bf16(t, nm)
+        if t.dim() != 3:
+            raise ValueError(f"{nm} must have 3 dims, got {list(t.shape)}")
+    S, R = lora_b.shape[0], lora_b.shape[2]
+    if R % 8 or not 8 <= R <= LORA_MAX_RANK:
+        raise ValueError(f"the rank must be a multiple of 8 up to {LORA_MAX_RANK} (LoraPool pads), got {R}")
+    if lora_a.shape != (S, P * R, K) or lora_b.shape[1] != N:
+        raise ValueError(f"lora_a must be {[S, P * R, K]} and lora_b {[S, N, R]}, got {list(lora_a.shape)} and "
+                         f"{list(lora_b.shape)}")
+    for t, nm in ((lora_a, "lora_a"), (lora_b, "lora_b")):
+        rows, cols = t.shape[1:]
+        if S and (t.stride(2) != 1 or t.stride(1) != cols or t.data_ptr() % 16
+                  or (S > 1 and (t.stride(0) % 8 or t.stride(0) < rows * cols))):
+            raise ValueError(f"{nm}'s slots must be contiguous and 16-byte aligned (they are not copied)")
+    if lora_scale.dtype != torch.float32 or lora_scale.shape != (S,) or not (lora_scale.is_contiguous() or S < 2):
+        raise ValueError(f"lora_scale must be float32 {[S]} contiguous, got {lora_scale.dtype} {list(lora_scale.shape)}")
+    if ids.dtype != torch.int32 or ids.numel() != M or ids.shape not in ((M,), x.shape[:-1]):
+        raise ValueError(f"ids must be int32 {[M]}, got {ids.dtype} {list(ids.shape)}")
+    return M, P, R
+
+
+def _lora_shrink(idx, rows, stride, x_scale, lora_a, lora_scale, ids, M, K, P, R):
+    """v [M, P, 2, R] of the rows with an adapter."""
+    v = torch.empty(M, P * 2 * R, dtype=torch.bfloat16, device=rows.device)
+    xs = (0, 0, 0) if x_scale is None else (x_scale.data_ptr(), *x_scale.stride())
+    _call_on(idx, "gdn_lora_shrink", rows.data_ptr(), int(x_scale is None), stride, *xs, lora_a.data_ptr(),
+             lora_a.stride(0), lora_scale.data_ptr(), ids.data_ptr(), lora_a.shape[0], P, R, M, K, v.data_ptr(), 2 * P * R)
+    return v
+
+
+def _tables(outs, widths, slices):
+    """The GEMMs' part and slice tables."""
+    n, ends = len(widths), [sum(widths[:i + 1]) for i in range(len(widths))]
+    return ((ctypes.c_void_p * n)(*[t.data_ptr() for t in outs]),
+            (ctypes.c_int64 * n)(*[max(t.stride(0), w) for t, w in zip(outs, widths)]), (ctypes.c_int * n)(*ends),
+            (ctypes.c_int * len(slices))(*[sum(slices[:i + 1]) for i in range(len(slices))]))
+
+
+def _gemm_bf16_lora(idx, rows, stride, weight, outs, widths, slices, first, col, v, lora_b, ids, gates=None):
+    """The bf16 product and the adapters' part into outs: its columns are lora_b's from `col` on, its
+    slices v's from `first` on.  With gates, (g, beta)."""
+    M, (N, K) = v.shape[0], weight.shape
+    R = lora_b.shape[2]
+    c, ld, ends, slice_ends = _tables(outs, widths, slices)
+    g = beta = a_log = dt_bias = None
+    gate_col = Hv = 0
+    if gates is not None:
+        a_log, dt_bias = gates["A_log"], gates["dt_bias"]
+        if a_log.dtype != dt_bias.dtype or a_log.dtype not in (torch.bfloat16, torch.float32):
+            a_log, dt_bias = a_log.float(), dt_bias.float()
+        a_log, dt_bias = a_log.contiguous(), dt_bias.contiguous()
+        Hv, gate_col = a_log.numel(), int(gates["gate_col"])
+        g = torch.empty(M, Hv, dtype=torch.float32, device=v.device)
+        beta = torch.empty(M, Hv, dtype=torch.bfloat16, device=v.device)
+    with torch.cuda.device(idx):
+        _lib.call("gdn_gemm_bf16_lora", rows.data_ptr(), stride, weight.data_ptr(), weight.stride(0), M, N, K, len(widths),
+                  c, ld, ends, _lib.ptr(g), _lib.ptr(beta), _lib.ptr(a_log), _lib.ptr(dt_bias),
+                  int(a_log is not None and a_log.dtype == torch.float32), gate_col, Hv, v.data_ptr() + 4 * first * R,
+                  v.stride(0), lora_b.data_ptr() + 2 * col * R, lora_b.stride(0), ids.data_ptr(), lora_b.shape[0], R,
+                  len(slices), slice_ends, _lib.stream_of(idx))
+    return g, beta
+
+
+def _weight_rows(w: torch.Tensor, align: int) -> torch.Tensor:
+    """A weight [N, K] whose rows the kernels read in 16-byte pieces."""
+    if w.stride(1) != 1 or w.stride(0) % align or w.stride(0) < w.shape[1] or w.data_ptr() % 16:
+        w = w.contiguous() if not w.is_contiguous() else w.clone(memory_format=torch.contiguous_format)
+    return w
+
+
+def linear_lora(x: torch.Tensor, weight: torch.Tensor, lora_a: torch.Tensor, lora_b: torch.Tensor,
+                lora_scale: torch.Tensor, ids: torch.Tensor, widths: list[int] | None = None,
+                gates: dict | None = None):
+    """linear(x, weight) with a low-rank adapter for each row beside the shared weight:
+    y[m] = x[m] W^T + lora_scale[s] * (x[m] A_s^T) B_s^T, s = ids[m]; a row whose s is
+    outside of 0 .. slots - 1 has no adapter.  x [..., K] bf16, weight [N, K] bf16 (K in
+    steps of 64); ids int32, one per row, in any order.
+
+    widths: y comes as len(widths) (1-4) contiguous tensors (as linear_cols), each part a
+    projection of its own with an A of its own; None is one part.  lora_a [slots,
+    parts * R, K] and lora_b [slots, N, R] bf16 (R a multiple of 8 up to 256), lora_scale
+    [slots] fp32: a LoraPool's.  gates: as linear_cols; they are of the adapted columns.
+
+    fp32 accumulation of both, one rounding; x A_s^T is held to 2^-16 in between.  A row's
+    result does not depend on the adapters of the others, whatever these hold.  Two
+    launches; x, weight and one slot of the adapters below 2 GiB each.  Returns [..., N], or the list of
+    parts, with gates (that, g, beta)."""
+    parts = [weight.shape[0]] if widths is None else list(widths)
+    if weight.dim() != 2:
+        raise ValueError(f"weight must be [N, K], got {list(weight.shape)}")
+    N, K = weight.shape
+    _bf16(x, "x")
+    _bf16(weight, "weight")
+    if K == 0 or K % 64 or x.shape[-1] != K:
+        raise ValueError(f"x [..., {x.shape[-1]}] and weight [{N}, {K}]: equal last dims, a positive multiple of 64")
+    M, P, R = _lora_check(x, N, K, parts, lora_a, lora_b, lora_scale, ids)
+    idx = _device_of(x, weight, lora_a, lora_b, lora_scale, ids)
+    rows, _, stride = _rows_of(x, 8)
+    weight, ids = _weight_rows(weight, 8), ids.contiguous()
+    outs = [torch.empty(M, w, dtype=torch.bfloat16, device=x.device) for w in parts]
+    v = _lora_shrink(idx, rows, stride, None, lora_a, lora_scale, ids, M, K, P, R)
+    g, beta = _gemm_bf16_lora(idx, rows, stride, weight, outs, parts, parts, 0, 0, v, lora_b, ids, gates)
+    y = [t.view(*x.shape[:-1], t.shape[1]) for t in outs]
+    y = y[0] if widths is None else y
+    return y if gates is None else (y, g, beta)
+
+
+def linear_fp8_lora(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor, lora_a: torch.Tensor,
+                    lora_b: torch.Tensor, lora_scale: torch.Tensor, ids: torch.Tensor,
+                    x_scale: torch.Tensor | None = None, widths: list[int] | None = None,
+                    wide: torch.Tensor | None = None, gates: dict | None = None):
+    """linear_fp8(x, weight, weight_scale) with a low-rank adapter for each row, as
+    linear_lora: the shared weight in e4m3 with its block scales, the adapters in bf16.  x
+    [..., K] bf16 is quantized for the shared weight (quantize_fp8) and read as it is by
+    the adapters; e4m3 with its x_scale both read as the values it stands for.
+
+    wide: a bf16 weight [N2, K] (N2 and N multiples of 16) whose product with the bf16 x
+    follows as the last columns, a boundary of widths at N; the adapters' columns then go
+    on over these (lora_b [slots, N + N2, R]).  gates: of the wide columns (gate_col
+    counted from N).  Returns as linear_lora."""
+    M, N, K = _check_fp8(x, weight, weight_scale, x_scale)
+    total = N
+    if wide is not None:
+        if wide.dtype != torch.bfloat16 or x.dtype != torch.bfloat16:
+            raise TypeError(f"wide and x must be bfloat16, got {wide.dtype} and {x.dtype}")
+        if wide.dim() != 2 or wide.shape[1] != K or wide.shape[0] % 16 or wide.shape[0] == 0 or N % 16:
+            raise ValueError(f"wide must be [N2, {K}] with N2 and N = {N} positive multiples of 16, got "
+                             f"{list(wide.shape)}")
+        total += wide.shape[0]
+    elif gates is not None:
+        raise ValueError("gates are of the wide columns")
+    parts = [total] if widths is None else list(widths)
+    M, P, R = _lora_check(x, total, K, parts, lora_a, lora_b, lora_scale, ids)
+    narrow = [i for i in range(1, P + 1) if sum(parts[:i]) == N]
+    if not narrow:
+        raise ValueError(f"widths {parts}: a boundary at {N}")
+    n = narrow[0]
+    idx = _device_of(x, weight, weight_scale, x_scale, wide, lora_a, lora_b, lora_scale, ids)
+    rows, _, stride = _rows_of(x, 8 if x_scale is None else 16)
+    weight, ids = _weight_rows(weight, 16), ids.contiguous()
+    G = K // FP8_GROUP
+    if not weight_scale.is_contiguous():
+        weight_scale = weight_scale.contiguous()
+    outs = [torch.empty(M, w, dtype=torch.bfloat16, device=x.device) for w in parts]
+    v = _lora_shrink(idx, rows, stride, x_scale, lora_a, lora_scale, ids, M, K, P, R)
+    x8, x8_stride, xs = rows, stride, x_scale
+    if x_scale is None:
+        x8 = torch.empty(M, K, dtype=FP8, device=x.device)
+        xs, x8_stride = _fp8_scales(M, G, x.device), K
+        _call_on(idx, "gdn_quantize_fp8", rows.data_ptr(), 0, stride, x8.data_ptr(), K, xs.data_ptr(), 1, M, M, K, 1)
+    c, ld, ends, slice_ends = _tables(outs[:n], parts[:n], parts[:n])
+    with torch.cuda.device(idx):
+        _lib.call("gdn_gemm_fp8_lora", x8.data_ptr(), x8_stride, xs.data_ptr(), *xs.stride(), weight.data_ptr(),
+                  weight.stride(0), weight_scale.data_ptr(), G, M, N, K, n, c, ld, ends, v.data_ptr(), v.stride(0),
+                  lora_b.data_ptr(), lora_b.stride(0), ids.data_ptr(), lora_b.shape[0], R, n, slice_ends,
+                  _lib.stream_of(idx))
+    g = beta = None
+    if wide is not None:
+        g, beta = _gemm_bf16_lora(idx, rows, stride, _weight_rows(wide, 8), outs[n:], parts[n:], parts[n:], n, N, v,
+                                  lora_b, ids, gates)
+    y = [t.view(*x.shape[:-1], t.shape[1]) for t in outs]
+    y = y[0] if widths is None else y
+    return y if gates is None else (y, g, beta)
+
+
+# ----------------------------------------------------- norms around blocks --
+NORM_MAX_COLUMNS = 16384
+
+
+def add_rms_norm(x: torch.Tensor, residual: torch.Tensor | None, weight: torch.Tensor, eps: float, *,
+                 post_weight: torch.Tensor | None = None, gate: torch.Tensor | None = None, gate_sigmoid: bool = False,
+                 scale: float = 1.0, offset: float = 1.0, residual_out: torch.Tensor | None = None):
+    """The seam between two blocks: the residual stream takes a block's output x, and the
+    next block reads its RMSNorm.  Over the last dim, in fp32:
+
+      h = x; with post_weight, the block's own norm: h rsqrt(mean(h^2) + eps) (offset +
+      post_weight); with gate, h * gate (gate_sigmoid: h * sigmoid(gate));
+      r = residual + scale * h;  y = r rsqrt(mean(r^2) + eps) (offset + weight)
+
+    x [..., H] bf16; residual like x in bf16 or fp32, or None (the stream begins: r is
+    scale * h); weight, post_weight [H] bf16 or fp32, held as their distance from 1 with
+    offset = 1 (the reference's), as they are with offset = 0; gate bf16 or fp32: [..., 1]
+    (per row), [H] (per column) or like x.  H up to 16384.
+
+    Returns (y bf16, r in the residual's type, bf16 without one).  y is formed before r is
+    rounded.  r goes into residual_out where that is given (contiguous, r's type; residual
+    itself is allowed); where r is x (no residual, nothing else either), it is x that is
+    returned.
+    Reference: _gemma_rms_forward, _gemma_add_rms_forward,
+    nanovllm/models/qwen3_5.py:99-118 (x and residual alone)."""
+    y, _, _, r = _add_rms_norm(x, residual, weight, eps, post_weight, gate, gate_sigmoid, scale, offset, residual_out,
+                               True, False)
+    return y, r
+
+
+def add_rms_norm_fp8(x: torch.Tensor, residual: torch.Tensor | None, weight: torch.Tensor, eps: float, *,
+                     post_weight: torch.Tensor | None = None, gate: torch.Tensor | None = None,
+                     gate_sigmoid: bool = False, scale: float = 1.0, offset: float = 1.0,
+                     residual_out: torch.Tensor | None = None, keep: bool = False):
+    """add_rms_norm with y in e4m3 for an 8-bit projection: quantize_fp8's groups of 128
+    of the fp32 values, rounded once (H a multiple of 128).  Returns (y8 [..., H], its
+    scales [rows, H / 128], r), with keep also the bf16 y (for what reads the same rows in
+    bf16: the layer's gate projections)."""
+    y, y8, y_scale, r = _add_rms_norm(x, residual, weight, eps, post_weight, gate, gate_sigmoid, scale, offset,
+                                      residual_out, keep, True)
+    return (y8, y_scale, r, y) if keep else (y8, y_scale, r)
+
+
+def _add_rms_norm(x, residual, weight, eps, post_weight, gate, gate_sigmoid, scale, offset, residual_out, bf16, fp8):
+    idx = _device_of(x, residual, weight, post_weight, gate, residual_out)
+    _bf16(x, "x")
+    if x.dim() < 1:
+        raise ValueError("x must be [..., H]")
+    H = x.shape[-1]
+    if not 1 <= H <= NORM_MAX_COLUMNS or (fp8 and H % FP8_GROUP):
+        raise ValueError(f"rows of 1 to {NORM_MAX_COLUMNS} columns" + (f" in multiples of {FP8_GROUP}" if fp8 else "")
+                         + f", got {H}")
+    floats = (torch.bfloat16, torch.float32)
+    for t, nm in ((residual, "residual"), (weight, "weight"), (post_weight, "post_weight"), (gate, "gate")):
+        if t is not None and t.dtype not in floats:
+            raise TypeError(f"{nm} must be bfloat16 or float32, got {t.dtype}")
+    if residual is not None and residual.shape != x.shape:
+        raise ValueError(f"residual must be {list(x.shape)}, got {list(residual.shape)}")
+    if post_weight is not None and post_weight.dtype != weight.dtype:
+        weight, post_weight = weight.float(), post_weight.float()
+    for t, nm in ((weight, "weight"), (post_weight, "post_weight")):
+        if t is not None and t.shape != (H,):
+            raise ValueError(f"{nm} must be [{H}], got {list(t.shape)}")
+    weight = weight.contiguous()
+    post_weight = None if post_weight is None else post_weight.contiguous()
+    M = x.numel() // H
+
+    def rows(t):
+        """[..., H] as rows with dense columns, and their stride."""
+        if t.is_contiguous():
+            return t, H
+        t = t.reshape(-1, H)
+        return (t, t.stride(0)) if (t.stride(1) == 1 or H == 1) and (t.stride(0) >= H or M < 2) else (t.contiguous(), H)
+
+    x2, sx = rows(x)
+    r2, sr = (None, 0) if residual is None else rows(residual)
+    g_row = g_col = 0
+    if gate is not None:
+        if gate.shape == (*x.shape[:-1], 1) and H > 1:
+            gate = gate.reshape(-1)
+            g_row = gate.stride(0) if gate.numel() > 1 else 0
+        elif gate.shape == x.shape:
+            gate, g_row = rows(gate)
+            g_col = 1
+        elif gate.shape == (H,):
+            gate, g_col = gate.contiguous(), 1
+        else:
+            raise ValueError(f"gate must be {[*x.shape[:-1], 1]}, {[H]} or {list(x.shape)}, got {list(gate.shape)}")
+    kind = torch.bfloat16 if residual is None else residual.dtype
+    same = residual is None and post_weight is None and gate is None and scale == 1.0   # r is x
+    if residual_out is not None:
+        r = residual_out
+        if r.dtype != kind or r.shape != x.shape or not r.is_contiguous():
+            raise ValueError(f"residual_out must be {kind} {list(x.shape)} contiguous, got {r.dtype} {list(r.shape)}")
+    else:
+        r = x if same else torch.empty(x.shape, dtype=kind, device=x.device)
+    written = residual_out is not None or not same
+    y = torch.empty(x.shape, dtype=torch.bfloat16, device=x.device) if bf16 else None
+    y8 = y_scale = None
+    if fp8:
+        # (the rows that the kernel reads in whole pieces)
+        x2, sx = _pieces(x2, sx, H, 8)
+        if r2 is not None:
+            r2, sr = _pieces(r2, sr, H, 8)
+        if gate is not None and g_col:
+            gate, g_row = _pieces(gate, g_row, H, 8)
+        weight = weight if weight.data_ptr() % 16 == 0 else weight.clone()
+        if post_weight is not None and post_weight.data_ptr() % 16:
+            post_weight = post_weight.clone()
+        if written and r.data_ptr() % 16:
+            raise ValueError("residual_out must be 16-byte aligned")
+        y8 = torch.empty(x.shape, dtype=FP8, device=x.device)
+        y_scale = _fp8_scales(M, H // FP8_GROUP, x.device)
+    ptr = lambda t: 0 if t is None else t.data_ptr()  # noqa: E731
+    f32 = lambda t: int(t is not None and t.dtype == torch.float32)  # noqa: E731
+    _call_on(idx, "gdn_add_rms_norm", x2.data_ptr(), sx, ptr(r2), sr, int(kind == torch.float32), weight.data_ptr(),
+             ptr(post_weight), f32(weight), float(offset), ptr(gate), f32(gate), g_row, g_col, int(bool(gate_sigmoid)),
+             float(scale), float(eps), r.data_ptr() if written else 0, ptr(y), ptr(y8), ptr(y_scale), 1, max(M, 1), M, H)
+    return y, y8, y_scale, r
+
+
+def _pieces(t, stride, H, align):
+    """Rows that are read in 16-byte pieces (else copied), and their stride; stride 0: one row for all."""
+    if t.data_ptr() % 16 or stride % align:
+        t = t.contiguous() if not t.is_contiguous() else t.clone(memory_format=torch.contiguous_format)
+        return t, H if stride else 0
+    return t, stride
+
+
 # -------------------------------------------------------------- gated norm --
 def rms_norm_gated(hidden_states: torch.Tensor, gate: torch.Tensor, weight: torch.Tensor,
                    eps: float, out: torch.Tensor | None = None) -> torch.Tensor:
