@@ -630,27 +630,29 @@ int gdn_add_rms_norm(const uint16_t* x, int64_t sx, const void* residual, int64_
  *   a     [slots][slices rank, K] bf16, slot stride a_slot (a multiple of 8), 16-byte aligned;
  *         scale [slots] fp32; ids int32 [M]
  *   v     [M, slices, 2, rank] bf16, row stride ldv (a multiple of 8), 16-byte aligned: each value as the sum
- *         of two.  Rows without an adapter are not written, and not read by what follows
+ *         of two.  Rows without an adapter are not written, and count for nothing in what follows
+ *   groups int32 [ceil(M / 16)], written by the first call for the second: the adapter of 16
+ *         rows (-1: none of them has one, -2: they differ)
  *   lb    [slots][N, rank] bf16, slot stride lb_slot (a multiple of 8), 16-byte aligned
  * x as the GEMM's A: bf16 with K in steps of 64, or e4m3 with its scales (K in steps of
  * 128).  An adapter's rows do not change the bits of others, whatever it holds.
  */
 int gdn_lora_shrink(const void* x, int x_is_bf16, int64_t ldx, const float* xs, int64_t xs_row, int64_t xs_grp,
                     const uint16_t* a, int64_t a_slot, const float* scale, const int32_t* ids, int slots, int slices,
-                    int rank, int M, int K, uint16_t* v, int64_t ldv, void* stream);
+                    int rank, int M, int K, uint16_t* v, int64_t ldv, int32_t* groups, void* stream);
 
 /* gdn_gemm_bf16_cols with the adapters' part. */
 int gdn_gemm_bf16_lora(const uint16_t* A, int64_t lda, const uint16_t* B, int64_t ldb, int M, int N, int K, int n_parts,
                        uint16_t* const* C, const int64_t* ldc, const int* col_end, float* g, uint16_t* beta,
                        const void* A_log, const void* dt_bias, int param_is_fp32, int gate_col, int Hv,
-                       const uint16_t* v, int64_t ldv, const uint16_t* lb, int64_t lb_slot, const int32_t* ids, int slots,
-                       int rank, int slices, const int* slice_end, void* stream);
+                       const uint16_t* v, int64_t ldv, const int32_t* groups, const uint16_t* lb, int64_t lb_slot,
+                       const int32_t* ids, int slots, int rank, int slices, const int* slice_end, void* stream);
 
 /* gdn_gemm_fp8 from e4m3 rows with the adapters' part. */
 int gdn_gemm_fp8_lora(const uint8_t* A, int64_t lda, const float* sa, int64_t sa_row, int64_t sa_grp, const uint8_t* B,
                       int64_t ldb, const float* sb, int64_t sb_row, int M, int N, int K, int n_parts, uint16_t* const* C,
-                      const int64_t* ldc, const int* col_end, const uint16_t* v, int64_t ldv, const uint16_t* lb,
-                      int64_t lb_slot, const int32_t* ids, int slots, int rank, int slices, const int* slice_end,
+                      const int64_t* ldc, const int* col_end, const uint16_t* v, int64_t ldv, const int32_t* groups,
+                      const uint16_t* lb, int64_t lb_slot, const int32_t* ids, int slots, int rank, int slices, const int* slice_end,
                       void* stream);
 
 /*

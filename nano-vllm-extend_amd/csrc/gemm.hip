@@ -59,6 +59,7 @@
 // bf16-rounded values with the gate kernel's arithmetic (gdn::gate_beta,
 // gdn::gate_g), so they equal gdn_g_beta applied to C.
 #include <algorithm>
+#include <cstddef>
 #include <type_traits>
 
 #include "gemm_tile.h"
@@ -392,7 +393,7 @@ template <bool kLora>
 __global__ __launch_bounds__(kPPThreads, 2) void gemm_tn_pp_kernel(const uint16_t* __restrict__ A, int64_t lda,
                                                                   const uint16_t* __restrict__ B, int64_t ldb,
                                                                   GemmOut out, int M, int N, int K, GemmGates gt,
-                                                                  int whole, LoraArg<kLora> lo) {
+                                                                  int whole, LoraArg<kLora>) {
   constexpr int kHalf = 128 * 128;  // bytes of a half tile: 128 rows of 64 values
   __shared__ __align__(16) uint8_t a00[kHalf];
   __shared__ __align__(16) uint8_t a01[kHalf];
@@ -403,7 +404,20 @@ __global__ __launch_bounds__(kPPThreads, 2) void gemm_tn_pp_kernel(const uint16_
   __shared__ __align__(16) uint8_t b10[kHalf];
   __shared__ __align__(16) uint8_t b11[kHalf];
   __shared__ __align__(16) uint16_t gscr[8][16 * 32];
+  __shared__ std::conditional_t<kLora, LoraTiles, int> tiles_l;
 
+  struct Args {  // the kernel's
+    const uint16_t* A;
+    int64_t lda;
+    const uint16_t* B;
+    int64_t ldb;
+    GemmOut out;
+    int M, N, K;
+    GemmGates gt;
+    int whole;
+    Lora lo;
+  };
+  constexpr int kLoraAt = static_cast<int>(offsetof(Args, lo));
   const int mb_n = (M + 255) / 256, nb_n = (N + 255) / 256;
   // XCD x (workgroups b % 8 == x) walks a contiguous range of the tiles
   const int xcd = blockIdx.x % gdn::kNumXcd, slot = blockIdx.x / gdn::kNumXcd, stride = gridDim.x / gdn::kNumXcd;
@@ -430,7 +444,28 @@ __global__ __launch_bounds__(kPPThreads, 2) void gemm_tn_pp_kernel(const uint16_
   const int gcol_a = 8 * ((lane & 7) ^ (((wave & 1) << 2) | (lane >> 4)));
   const int gcol_b = 8 * ((lane & 7) ^ (((wave & 3) << 1) | ((lane >> 4) & 1)));
   int va[2][2], vb[2][2];
+  // (kLora) the lane's number found anew where a new tile's offsets need it: a register kept for that
+  // across the loop is spilled, and comes back behind a wait for every load and store in flight
+  auto new_lane = []() {
+    int zero = 0;
+    asm volatile("" : "+v"(zero));
+    return static_cast<int>(__builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, zero)));
+  };
   auto set_offsets = [&](int m0, int n0) {
+    if constexpr (kLora) {
+      const int l = new_lane(), r = 8 * wave + (l >> 3);
+      const int ca = 16 * ((l & 7) ^ (((wave & 1) << 2) | (l >> 4)));
+      const int cb = 16 * ((l & 7) ^ (((wave & 3) << 1) | ((l >> 4) & 1)));
+      const int sa = 2 * static_cast<int>(lda), sb = 2 * static_cast<int>(ldb);  // (all offsets are below 2^31)
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          va[h][i] = min(m0 + 128 * h + 64 * i + r, M - 1) * sa + ca;
+          vb[h][i] = min(n0 + 128 * h + 64 * i + r, N - 1) * sb + cb;
+        }
+      return;
+    }
 #pragma unroll
     for (int h = 0; h < 2; ++h)
 #pragma unroll
@@ -458,6 +493,7 @@ __global__ __launch_bounds__(kPPThreads, 2) void gemm_tn_pp_kernel(const uint16_
       for (int ks = 0; ks < 2; ++ks)
         f[t][ks] = *reinterpret_cast<const frag_t*>(h + swb_off(32 * wn + 8 * (lr >> 2) + 4 * t + (lr & 3), 4 * ks + lg));
   };
+  int lora_lo = 0;  // (kLora) bytes to the low parts in a row of v
   gdn::f32x4_t acc[2][2][4][2];  // [row half][column half][16-row tile][column tile]
   // one row half of A against both column halves of B
   auto prod = [&](gdn::f32x4_t (&c0)[4][2], gdn::f32x4_t (&c1)[4][2], const frag_t (&fa)[4][2],
@@ -477,6 +513,24 @@ __global__ __launch_bounds__(kPPThreads, 2) void gemm_tn_pp_kernel(const uint16_
     __builtin_amdgcn_s_setprio(0);
     half_barrier();
   };
+  // the same of the adapters' steps: of ranks up to 32 the first half of a step
+  auto prod_lora = [&](gdn::f32x4_t (&c0)[4][2], gdn::f32x4_t (&c1)[4][2], const frag_t (&fa)[4][2],
+                       const frag_t (&f0)[2][2], const frag_t (&f1)[2][2]) {
+    if constexpr (kLora) {
+      auto half = [&](int ks) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int t = 0; t < 2; ++t) {
+            c0[i][t] = gdn::mfma16x16x32(f0[t][ks], fa[i][ks], c0[i][t]);
+            c1[i][t] = gdn::mfma16x16x32(f1[t][ks], fa[i][ks], c1[i][t]);
+          }
+      };
+      half(0);
+      if (lora_lo > 64) half(1);
+      half_barrier();
+    }
+  };
   auto mem_end = [&]() {
     __builtin_amdgcn_sched_barrier(0);
     __builtin_amdgcn_s_waitcnt(kWaitPP);
@@ -484,7 +538,13 @@ __global__ __launch_bounds__(kPPThreads, 2) void gemm_tn_pp_kernel(const uint16_
   };
   const int nk = K / kBK;  // even
   int L = xcd * per_xcd + slot;
-  if (L < xend) {
+  int n_whole = 0, n_quarters = 0;
+  if constexpr (kLora) {
+    lora_tiles(tiles_l, kernel_arg<Lora>(kLoraAt), M, N, xcd * per_xcd, xend, slot, stride, tile_of);
+    n_whole = __builtin_amdgcn_readfirstlane(tiles_l.whole);
+    if (n_whole) L = __builtin_amdgcn_readfirstlane(tiles_l.tile[0]);
+  }
+  if (kLora ? n_whole > 0 : L < xend) {
   int m0, n0;
   tile_of(L, m0, n0);
   set_offsets(m0, n0);
@@ -496,12 +556,26 @@ __global__ __launch_bounds__(kPPThreads, 2) void gemm_tn_pp_kernel(const uint16_
   dma(ra, a10, va[0], 128);
   dma(rb, b11, vb[1], 128);
   frag_t fa[4][2], fb0[2][2], fb1[2][2], fbn[2][2];
+  // (kLora) the pairs of steps behind K: v's rows and the adapters' B in A's and B's place
+  LoraBase na(A), nb(B);
+  LoraSteps lt{LoraTiles::kNone, 0, false};
+  auto set_lora_offsets = [&](int e, int m, int n) {
+    if constexpr (kLora) {
+      const Lora lo = kernel_arg<Lora>(kLoraAt);
+      lora_offsets(lo, lt, lora_pair(tiles_l, lo, lt, e, N, n), M, N, m, n, wave, new_lane(), va, vb, na, nb, lora_lo);
+    }
+  };
+  int at = 0;
   __builtin_amdgcn_s_waitcnt(12 | (7 << 4));
   half_barrier();
   read_b(b00, fb0);
   mem_end();
   for (;;) {
-    const int Ln = L + stride;
+    int Ln = L + stride;
+    if constexpr (kLora) {
+      lt = lora_steps(tiles_l, at);
+      Ln = ++at < n_whole ? __builtin_amdgcn_readfirstlane(tiles_l.tile[at]) : xend;
+    }
     const int m0c = m0, n0c = n0;
 #pragma unroll
     for (int a = 0; a < 2; ++a)
@@ -516,62 +590,121 @@ __global__ __launch_bounds__(kPPThreads, 2) void gemm_tn_pp_kernel(const uint16_
     for (int s = 0; s < nk; s += 2) {
       const int ka = kb - 128;  // of step s + 1: the current tile's
       int v1[2] = {va[1][0], va[1][1]};
+      if constexpr (kLora) dma(ra, a11, v1, ka);  // (here for two registers less)
       if (s + 2 == nk) {
         // the next loads are the next tile's first steps (past the last tile
         // they repeat this one's)
-        if (Ln < xend) {
+        if (kLora && lt.pairs) {
+          set_lora_offsets(0, m0, n0);
+        } else if (Ln < xend) {
           tile_of(Ln, m0, n0);
           set_offsets(m0, n0);
         }
         kb = 0;
       }
-      dma(rb, b00, vb[0], kb);
-      dma(ra, a11, v1, ka);
+      // step s + 3 of A and B behind step s + 2
+      const int k3a = kLora && s + 2 == nk && lt.pairs ? lora_lo : kb + 128;
+      const int k3b = kLora && s + 2 == nk && lt.pairs ? 0 : kb + 128;
+      __amdgpu_buffer_rsrc_t ra_n = ra, rb_n = rb;
+      if constexpr (kLora) ra_n = na.rsrc(), rb_n = nb.rsrc();
+      dma(rb_n, b00, vb[0], kb);
+      if constexpr (!kLora) dma(ra, a11, v1, ka);
       read_a(a00, fa);
       read_b(b01, fb1);
       mem_end();
       prod(acc[0][0], acc[0][1], fa, fb0, fb1);
-      dma(ra, a00, va[0], kb);
-      dma(rb, b01, vb[1], kb);
+      dma(ra_n, a00, va[0], kb);
+      dma(rb_n, b01, vb[1], kb);
       read_a(a01, fa);
       read_b(b10, fbn);
       mem_end();
       prod(acc[1][0], acc[1][1], fa, fb0, fb1);
-      dma(rb, b10, vb[0], kb + 128);
-      dma(ra, a01, va[1], kb);
+      dma(rb_n, b10, vb[0], k3b);
+      dma(ra_n, a01, va[1], kb);
       read_a(a10, fa);
       read_b(b11, fb1);
       mem_end();
       prod(acc[0][0], acc[0][1], fa, fbn, fb1);
-      dma(ra, a10, va[0], kb + 128);
-      dma(rb, b11, vb[1], kb + 128);
+      dma(ra_n, a10, va[0], k3a);
+      dma(rb_n, b11, vb[1], k3b);
       read_a(a11, fa);
       read_b(b00, fb0);
       mem_end();
       prod(acc[1][0], acc[1][1], fa, fbn, fb1);
       kb += 256;
     }
+    if constexpr (kLora) {
+      // the adapters' pairs of steps, as the loop's; the next loads are the next pair's or tile's
+      for (int e = 0; e < lt.pairs; ++e) {
+        dma(na.rsrc(), a11, va[1], lora_lo);
+        int k3a = 128, k3b = 128;
+        if (e + 1 < lt.pairs) {
+          set_lora_offsets(e + 1, m0, n0);
+          k3a = lora_lo;
+          k3b = 0;
+        } else if (Ln < xend) {
+          tile_of(Ln, m0, n0);
+          set_offsets(m0, n0);
+          na = LoraBase(A);
+          nb = LoraBase(B);
+        } else {
+          k3a = k3b = 0;
+        }
+        const __amdgpu_buffer_rsrc_t ra_n = na.rsrc(), rb_n = nb.rsrc();
+        dma(rb_n, b00, vb[0], 0);
+        read_a(a00, fa);
+        read_b(b01, fb1);
+        mem_end();
+        prod_lora(acc[0][0], acc[0][1], fa, fb0, fb1);
+        dma(ra_n, a00, va[0], 0);
+        dma(rb_n, b01, vb[1], 0);
+        read_a(a01, fa);
+        read_b(b10, fbn);
+        mem_end();
+        prod_lora(acc[1][0], acc[1][1], fa, fb0, fb1);
+        dma(rb_n, b10, vb[0], k3b);
+        dma(ra_n, a01, va[1], 0);
+        read_a(a10, fa);
+        read_b(b11, fb1);
+        mem_end();
+        prod_lora(acc[0][0], acc[0][1], fa, fbn, fb1);
+        dma(ra_n, a10, va[0], k3a);
+        dma(rb_n, b11, vb[1], k3b);
+        read_a(a11, fa);
+        read_b(b00, fb0);
+        mem_end();
+        prod_lora(acc[1][0], acc[1][1], fa, fbn, fb1);
+      }
+      if (lt.part) {
+        float bad = 0.0f;
+#pragma unroll
+        for (int a = 0; a < 2; ++a)
+#pragma unroll
+          for (int b = 0; b < 2; ++b)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+              for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int x = 0; x < 4; ++x) bad = fmaf(acc[a][b][i][t][x], 0.0f, bad);
+        if (bad != 0.0f) tiles_l.again[at - 1] = 1;
+      }
+    }
     if (!wm) half_barrier();
     // (the lane from an opaque copy, so that no address of the epilogue is
     // kept in registers across the loop)
     int tid_e = static_cast<int>(threadIdx.x);
     asm volatile("" : "+v"(tid_e));
-    if constexpr (kLora) {
-#pragma unroll
-      for (int a = 0; a < 2; ++a) {
-        const int cb[2] = {n0c + 32 * wn, n0c + 128 + 32 * wn};
-        lora_add<4, 2, 1>(lo, M, N, m0c + 128 * a + 64 * wm, cb, tid_e & 63, 0, 1,
-                          [&](int i, int j, int t) -> gdn::f32x4_t& { return acc[a][j][i][t]; });
-      }
-    }
+    const GemmOut out_e = kLora ? kernel_arg<GemmOut>(offsetof(Args, out)) : out;
+    const GemmGates gt_e = kLora ? kernel_arg<GemmGates>(offsetof(Args, gt)) : gt;
 #pragma unroll
     for (int a = 0; a < 2; ++a)
 #pragma unroll
       for (int i = 0; i < 4; ++i)
 #pragma unroll
         for (int b = 0; b < 2; ++b)
-          gemm_store16(acc[a][b][i][0], acc[a][b][i][1], out, M, N, m0c + 128 * a + 64 * wm + 16 * i,
-                       n0c + 128 * b + 32 * wn, tid_e & 63, gt, gscr[wave]);
+          gemm_store16(acc[a][b][i][0], acc[a][b][i][1], out_e, M, N, m0c + 128 * a + 64 * wm + 16 * i,
+                       n0c + 128 * b + 32 * wn, tid_e & 63, gt_e, gscr[wave]);
     if (Ln >= xend) break;
     L = Ln;
   }
@@ -586,9 +719,26 @@ __global__ __launch_bounds__(kPPThreads, 2) void gemm_tn_pp_kernel(const uint16_
   const int nq = whole ? 4 * (tiles - whole) : mq_n * nq_n;
   const int q_xcd = (nq + gdn::kNumXcd - 1) / gdn::kNumXcd;
   const int qend = min((xcd + 1) * q_xcd, nq);
-  for (int q = xcd * q_xcd + slot; q < qend; q += stride) {
-    int m0, n0;
-    if (whole) {
+  // (kLora) the quarters of the workgroup's own tiles first: ql of them, then q as without
+  int ql = 0;
+  if constexpr (kLora) n_quarters = lora_quarters(tiles_l);
+  for (int q = xcd * q_xcd + slot; q < qend || (kLora && ql < n_quarters); q += stride) {
+    int m0 = 0, n0 = 0;
+    bool own = false;
+    if constexpr (kLora) {
+      own = ql < n_quarters;
+      if (own) {
+        q -= stride;
+        tile_of(__builtin_amdgcn_readfirstlane(tiles_l.in_quarters[ql >> 2]), m0, n0);
+        m0 += 128 * ((ql >> 1) & 1);
+        n0 += 128 * (ql & 1);
+        ++ql;
+        if (m0 >= M || n0 >= N) continue;  // (the whole workgroup)
+      }
+    }
+    if (own) {
+      // (m0 and n0 are there)
+    } else if (whole) {
       tile_of(whole + (q >> 2), m0, n0);
       m0 += 128 * ((q >> 1) & 1);
       n0 += 128 * (q & 1);
@@ -644,14 +794,14 @@ __global__ __launch_bounds__(kPPThreads, 2) void gemm_tn_pp_kernel(const uint16_
       step(a11, b11, a10, b10, s + 3);
     }
     if (!wm) half_barrier();
-    if constexpr (kLora) {
-      const int cb[1] = {n0 + 32 * wn};
-      lora_add<4, 1, 2>(lo, M, N, m0 + 64 * wm, cb, lane, 0, 1,
-                        [&](int i, int, int t) -> gdn::f32x4_t& { return c[i][t]; });
-    }
+    if constexpr (kLora)
+      lora_add<4>(kernel_arg<Lora>(kLoraAt), M, N, m0 + 64 * wm, n0 + 32 * wn, new_lane(),
+                  [&](int i, int t) -> gdn::f32x4_t& { return c[i][t]; });
+    const GemmOut out_q = kLora ? kernel_arg<GemmOut>(offsetof(Args, out)) : out;
+    const GemmGates gt_q = kLora ? kernel_arg<GemmGates>(offsetof(Args, gt)) : gt;
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-      gemm_store16(c[i][0], c[i][1], out, M, N, m0 + 64 * wm + 16 * i, n0 + 32 * wn, lane, gt, gscr[wave]);
+      gemm_store16(c[i][0], c[i][1], out_q, M, N, m0 + 64 * wm + 16 * i, n0 + 32 * wn, lane, gt_q, gscr[wave]);
   }
   __builtin_amdgcn_s_waitcnt(0);
 }
@@ -753,7 +903,7 @@ __global__ __launch_bounds__(kGemmThreads) void gemm_tn_ring_kernel(const uint16
   issue(st2, wave + 2 * NW);
   if constexpr (kLora) {
     const int cb[1] = {n0};
-    lora_add<MT, 1, 4>(lo, M, N, m0, cb, lane, wave, NW,
+    lora_init<MT, 1, 4>(lo, M, N, m0, cb, lane, wave, NW,
                        [&](int i, int, int t) -> gdn::f32x4_t& { return acc[i][t]; });
   }
   __builtin_amdgcn_s_waitcnt(kWait);
@@ -785,35 +935,38 @@ __global__ __launch_bounds__(kGemmThreads) void gemm_tn_ring_kernel(const uint16
   }
 }
 
-// lora_add for products of 32 x 32 x 16: 32 rows from row0 against NJ blocks of 32 columns from
+// lora_init for products of 32 x 32 x 16: 32 rows from row0 against NJ blocks of 32 columns from
 // col0, acc[j] register 4 q + r of lane (li, lg) being C[row0 + li][col0 + 32 j + 8 q + 4 lg + r].
-template <int NJ, int DEPTH>
-__device__ __forceinline__ void lora_add32(const Lora& lo, int M, int N, int row0, int col0, int lane,
-                                           f32x16_t (&acc)[NJ]) {
+template <int NJ, int DEPTH, bool kSelect>
+__device__ __forceinline__ void lora_pass32(const Lora& lo, int N, int mine, uint64_t all, int voff, int col0, int lane,
+                                            f32x16_t (&acc)[NJ]) {
   const int li = lane & 31, lg = lane >> 5;
-  const int r = row0 + li, rc = min(r, M - 1);
-  const int s0 = lo.ids[rc];
-  const int mine = r < M && static_cast<unsigned>(s0) < static_cast<unsigned>(lo.slots) ? s0 : -1;
-  const uint64_t all = __ballot(mine >= 0 && lane < 32);
-  if (!all) return;
-  const int voff = static_cast<int>(rc * lo.ldv * 2);
-  const int half = lo.rank / 8, terms = 2 * half;
-  for (int p = 0, beg = 0; p < lo.slices; beg = lo.end[p++]) {
-    const int end = lo.end[p];
+  const int half = lo.rank / 8;
+  for (int p = 0, beg = 0, end = 0; p < lo.slices; ++p, beg = end) {
+    end = lora_end(lo, p);
     if (col0 >= end || col0 + 32 * NJ <= beg) continue;
     const __amdgpu_buffer_rsrc_t rv = rsrc_of(lo.v + 2 * p * lo.rank);
-    for (int c = 0; c < terms; c += 2) {
-      const int q = c + lg, qb = q < half ? q : q - half;  // (terms is even: every granule is there)
-      const gdn::s16x8_t va = lora_load(rv, voff + 16 * q);
+    for (int c = 0; c < half; c += 2) {
+      const int q = c + lg;
+      const int off = q < half ? 0 : kNoOffset;
+      const gdn::s16x8_t vh = lora_load(rv, (voff + 16 * q) | off);
+      const gdn::s16x8_t vl = lora_load(rv, (voff + 16 * (half + q)) | off);
+      int boff[NJ];
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) {
+        const int n = col0 + 32 * j + li;
+        boff[j] = (n * lo.rank * 2 + 16 * q) | off | (n >= beg && n < end ? 0 : kNoOffset);
+      }
       LoraIds it{all, 0, 1, 0};
       gdn::s16x8_t fb[DEPTH][NJ];
       int sid[DEPTH];
       auto fetch = [&](int d) {
-        sid[d] = it.next(mine);
+        uint64_t rows;
+        sid[d] = it.next(mine, rows);
         if (sid[d] < 0) return;
         const __amdgpu_buffer_rsrc_t rb = lora_b(lo, sid[d], N);
 #pragma unroll
-        for (int j = 0; j < NJ; ++j) fb[d][j] = lora_load(rb, (col0 + 32 * j + li) * lo.rank * 2 + 16 * qb);
+        for (int j = 0; j < NJ; ++j) fb[d][j] = lora_load(rb, boff[j]);
       };
 #pragma unroll
       for (int d = 0; d < DEPTH; ++d) fetch(d);
@@ -821,22 +974,43 @@ __device__ __forceinline__ void lora_add32(const Lora& lo, int M, int N, int row
 #pragma unroll
         for (int d = 0; d < DEPTH; ++d) {
           if (sid[d] < 0) continue;
+          const bool own = mine == sid[d];
+          const gdn::s16x8_t h = kSelect ? vh : lora_mask(vh, own), l = kSelect ? vl : lora_mask(vl, own);
 #pragma unroll
           for (int j = 0; j < NJ; ++j) {
-            const int cb = col0 + 32 * j;
-            const f32x16_t sum = mfma_bf16(fb[d][j], va, acc[j]);
+            f32x16_t sum = mfma_bf16(fb[d][j], h, acc[j]);
+            sum = mfma_bf16(fb[d][j], l, sum);
             // (slices end at multiples of 16)
-            const bool take0 = mine == sid[d] && cb >= beg && cb < end;
-            const bool take1 = mine == sid[d] && cb + 16 >= beg && cb + 16 < end;
+            const int cb = col0 + 32 * j;
+            const bool take0 = !kSelect || (own && cb >= beg && cb < end);
+            const bool take1 = !kSelect || (own && cb + 16 >= beg && cb + 16 < end);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) acc[j][e] = take0 ? sum[e] : acc[j][e];
-#pragma unroll
-            for (int e = 8; e < 16; ++e) acc[j][e] = take1 ? sum[e] : acc[j][e];
+            for (int e = 0; e < 16; ++e) acc[j][e] = (e < 8 ? take0 : take1) ? sum[e] : acc[j][e];
           }
           fetch(d);
         }
       }
     }
+  }
+}
+template <int NJ, int DEPTH>
+__device__ __forceinline__ void lora_init32(const Lora& lo, int M, int N, int row0, int col0, int lane,
+                                            f32x16_t (&acc)[NJ]) {
+  const int r = row0 + (lane & 31);
+  const int mine = lora_id(lo, r, M);
+  const uint64_t all = __ballot(mine >= 0 && lane < 32);
+  if (!all) return;
+  const int voff = static_cast<int>(min(r, M - 1) * lo.ldv * 2);
+  lora_pass32<NJ, DEPTH, false>(lo, N, mine, all, voff, col0, lane, acc);
+  float bad = 0.0f;
+#pragma unroll
+  for (int j = 0; j < NJ; ++j)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) bad = fmaf(acc[j][e], 0.0f, bad);
+  if (__builtin_expect(__any(bad != 0.0f || bad != bad), 0)) {
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) acc[j] = zero16();
+    lora_pass32<NJ, 1, true>(lo, N, mine, all, voff, col0, lane, acc);
   }
 }
 
@@ -944,7 +1118,7 @@ __global__ __launch_bounds__(kGemmThreads, 2) void gemm_tn_deep_kernel(const uin
   issue(st0, 0);
   issue(st1, 1);
   if constexpr (NS == 4) issue(st2, 2);
-  if constexpr (kLora) lora_add32<NJ, 4>(lo, M, N, m0 + 32 * wm, n0 + (BN / 2) * wn, lane, acc[0]);
+  if constexpr (kLora) lora_init32<NJ, NJ == 1 ? 12 : 6>(lo, M, N, m0 + 32 * wm, n0 + (BN / 2) * wn, lane, acc[0]);
   // (no exit inside a trip: with one, the compiler's load counting merges its
   // states at the loop head and waits there for loads that are meant to stay
   // in flight)
@@ -1014,7 +1188,8 @@ int gemm_launch(const uint16_t* A, int64_t lda, const uint16_t* B, int64_t ldb, 
   // 4096 x 512 7.7 -> 9.7; two rounds of blocks, 400 x 12352 x 2048 35.0 -> 38.1).
   const bool blocks = !wide && t128 <= kCUs && t64x128 > kCUs && 2 * t64x128 > 3 * t128 &&
                       K * t64x128 >= 1600 * kCUs;
-  if (K % (2 * kBK) == 0 && (wide ? kLora || !one192 : blocks)) {
+  const bool fits = !kLora || lora_tiles_fit(t256);
+  if (K % (2 * kBK) == 0 && fits && (wide ? kLora || !one192 : blocks)) {
     const int64_t rem = t256 % kCUs;
     const int64_t whole = rem <= kCUs / 2 ? t256 - rem : t256;
     const int64_t wgs = std::min<int64_t>(kCUs, whole ? std::max(whole, 4 * (t256 - whole)) : t128);
@@ -1123,7 +1298,7 @@ extern "C" int gdn_gemm_bf16_cols(const uint16_t* A, int64_t lda, const uint16_t
 extern "C" int gdn_gemm_bf16_lora(const uint16_t* A, int64_t lda, const uint16_t* B, int64_t ldb, int M, int N, int K,
                                   int n_parts, uint16_t* const* C, const int64_t* ldc, const int* col_end, float* g,
                                   uint16_t* beta, const void* A_log, const void* dt_bias, int param_is_fp32,
-                                  int gate_col, int Hv, const uint16_t* v, int64_t ldv, const uint16_t* lb,
+                                  int gate_col, int Hv, const uint16_t* v, int64_t ldv, const int32_t* groups, const uint16_t* lb,
                                   int64_t lb_slot, const int32_t* ids, int slots, int rank, int slices,
                                   const int* slice_end, void* stream) {
   if (M < 0 || N < 0 || K < 0 || n_parts < 1 || n_parts > kMaxParts || !C || !ldc || !col_end)
@@ -1135,7 +1310,8 @@ extern "C" int gdn_gemm_bf16_lora(const uint16_t* A, int64_t lda, const uint16_t
   GemmOut out{};
   if (!parts_of(out, n_parts, C, ldc, col_end, N)) return GDN_ERR_INVALID_ARG;
   Lora lo{};
-  if (!lora_of(lo, v, ldv, lb, lb_slot, ids, slots, rank, slices, slice_end, M, N)) return GDN_ERR_INVALID_ARG;
+  if (!lora_of(lo, v, ldv, groups, lb, lb_slot, ids, slots, rank, slices, slice_end, M, N)) return GDN_ERR_INVALID_ARG;
   const GemmGates gt{g, beta, A_log, dt_bias, param_is_fp32 ? 1 : 0, gate_col, Hv};
+  if (slots == 0) return gemm_launch<false>(A, lda, B, ldb, out, M, N, K, gt, NoLora{}, stream);
   return gemm_launch<true>(A, lda, B, ldb, out, M, N, K, gt, lo, stream);
 }

@@ -23,6 +23,7 @@
 // (in each of its parts) and runs at half the rate (2.4 against 4.8 PFLOP/s from registers); the
 // alternative is the bf16 GEMM.  Everything after a block's sum is fp32, and one rounding to bf16.
 #include <algorithm>
+#include <cstddef>
 #include <utility>
 
 #include "gemm_tile.h"
@@ -88,7 +89,7 @@ template <bool kOdd, bool kLora>
 __global__ __launch_bounds__(kPPThreads, 2) void gemm_fp8_pp_kernel(const uint8_t* __restrict__ A, int64_t lda,
                                                                     const uint8_t* __restrict__ B, int64_t ldb,
                                                                     Fp8Scales sc, GemmOut out, int M, int N, int K,
-                                                                    int whole, LoraArg<kLora> lo) {
+                                                                    int whole, LoraArg<kLora>) {
   constexpr int kHalf = 128 * 128;  // bytes of a half tile
   __shared__ __align__(16) uint8_t a00[kHalf];
   __shared__ __align__(16) uint8_t a01[kHalf];
@@ -103,7 +104,19 @@ __global__ __launch_bounds__(kPPThreads, 2) void gemm_fp8_pp_kernel(const uint8_
   __shared__ __align__(16) float sc1[512];
   __shared__ __align__(16) float sc2[512];
   __shared__ __align__(16) float sc3[512];
+  __shared__ std::conditional_t<kLora, LoraTiles, int> tiles_l;
 
+  struct Args {  // the kernel's
+    const uint8_t* A;
+    int64_t lda;
+    const uint8_t* B;
+    int64_t ldb;
+    Fp8Scales sc;
+    GemmOut out;
+    int M, N, K, whole;
+    Lora lo;
+  };
+  constexpr int kLoraAt = static_cast<int>(offsetof(Args, lo));
   const int mb_n = (M + 255) / 256, nb_n = (N + 255) / 256;
   const int xcd = blockIdx.x % gdn::kNumXcd, slot = blockIdx.x / gdn::kNumXcd, stride = gridDim.x / gdn::kNumXcd;
   const int tiles = mb_n * nb_n;
@@ -157,6 +170,7 @@ __global__ __launch_bounds__(kPPThreads, 2) void gemm_fp8_pp_kernel(const uint8_
   };
   const int nk = K / 128;
   const int steps = (nk + 1) & ~1;
+  if constexpr (kLora) __builtin_assume(steps >= 2);
   auto kbyte = [&](int s) { return 128 * min(s, nk - 1); };
   auto dma_sc = [&](float* dst, int s) { dma4(rs, dst + 64 * wave, vs, s_step * min(s, nk - 1)); };
   auto read_a = [&](const uint8_t* h, Frag8 (&f)[4]) {
@@ -191,6 +205,10 @@ __global__ __launch_bounds__(kPPThreads, 2) void gemm_fp8_pp_kernel(const uint8_
     return kOdd ? __uint_as_float(__float_as_uint(v) & static_cast<uint32_t>((s - nk) >> 31)) : v;
   };
   gdn::f32x4_t acc[2][2][4][2];  // [row half][column half][16-row tile][column tile]
+  // (kLora, which is short of registers: in a scalar one)
+  auto uniform = [](float v) {
+    return kLora ? __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(v))) : v;
+  };
   // one row half of A against both column halves of B, in step `at`; odd: which may be past the last
   auto prod = [&](gdn::f32x4_t (&c)[2][4][2], const Frag8 (&fa)[4], const Frag8 (&f0)[2], const Frag8 (&f1)[2],
                   const float (&s)[4], int at, auto odd) {
@@ -198,7 +216,7 @@ __global__ __launch_bounds__(kPPThreads, 2) void gemm_fp8_pp_kernel(const uint8_
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
-      for (int b = 0; b < 2; ++b) f[b][i] = odd.value ? kept(s[i] * sb[b], at) : s[i] * sb[b];
+      for (int b = 0; b < 2; ++b) f[b][i] = odd.value ? kept(s[i] * uniform(sb[b]), at) : s[i] * uniform(sb[b]);
     __builtin_amdgcn_s_setprio(1);
     // product j is scaled into its sum behind the issue of product j + 2, when its
     // result is there
@@ -231,7 +249,13 @@ __global__ __launch_bounds__(kPPThreads, 2) void gemm_fp8_pp_kernel(const uint8_
     half_barrier();
   };
   int L = xcd * per_xcd + slot;
-  if (L < xend) {
+  int n_whole = 0, n_quarters = 0;
+  if constexpr (kLora) {
+    lora_tiles(tiles_l, kernel_arg<Lora>(kLoraAt), M, N, xcd * per_xcd, xend, slot, stride, tile_of);
+    n_whole = __builtin_amdgcn_readfirstlane(tiles_l.whole);
+    if (n_whole) L = __builtin_amdgcn_readfirstlane(tiles_l.tile[0]);
+  }
+  if (kLora ? n_whole > 0 : L < xend) {
     int m0, n0;
     tile_of(L, m0, n0);
     set_offsets(m0, n0);
@@ -245,12 +269,52 @@ __global__ __launch_bounds__(kPPThreads, 2) void gemm_fp8_pp_kernel(const uint8_
     dma(ra, a10, va[0], kbyte(1));
     dma(rb, b11, vb[1], kbyte(1));
     Frag8 fa[4], fb0[2], fb1[2], fbn[2];
+    // (kLora) the pairs of bf16 steps behind K, as in the bf16 GEMM: v's rows and the adapters' B in
+    // A's and B's place, 64 values of a row in its 128 bytes
+    LoraBase na(A), nb(B);
+    int lora_lo = 0;  // bytes to the low parts in a row of v
+    LoraSteps lt{LoraTiles::kNone, 0, false};
+    auto set_lora_offsets = [&](int e, int m, int n) {
+      if constexpr (kLora) {
+        const Lora lo = kernel_arg<Lora>(kLoraAt);
+        lora_offsets(lo, lt, lora_pair(tiles_l, lo, lt, e, N, n), M, N, m, n, wave, new_lane(), va, vb, na, nb, lora_lo);
+      }
+    };
+    int at = 0;
+    // one row half of v against both column halves of the adapter's B; of ranks up to 32 the first half
+    // of a step
+    auto prod_lora = [&](gdn::f32x4_t (&c)[2][4][2], const Frag8 (&fa)[4], const Frag8 (&f0)[2], const Frag8 (&f1)[2]) {
+      if constexpr (kLora) {
+        auto bits = [](const i32x4_t& v) { return __builtin_bit_cast(gdn::s16x8_t, v); };
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+              c[b][i][t] = gdn::mfma16x16x32(bits(b ? f1[t].lo : f0[t].lo), bits(fa[i].lo), c[b][i][t]);
+        if (lora_lo > 64) {
+#pragma unroll
+          for (int b = 0; b < 2; ++b)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+              for (int t = 0; t < 2; ++t)
+                c[b][i][t] = gdn::mfma16x16x32(bits(b ? f1[t].hi : f0[t].hi), bits(fa[i].hi), c[b][i][t]);
+        }
+        half_barrier();
+      }
+    };
     __builtin_amdgcn_s_waitcnt(14 | (7 << 4));
     half_barrier();
     read_b(b00, fb0);
     mem_end();
     for (;;) {
-      const int Ln = L + stride;
+      int Ln = L + stride;
+      if constexpr (kLora) {
+        lt = lora_steps(tiles_l, at);
+        Ln = ++at < n_whole ? __builtin_amdgcn_readfirstlane(tiles_l.tile[at]) : xend;
+      }
       const int m0c = m0, n0c = n0;
 #pragma unroll
       for (int a = 0; a < 2; ++a)
@@ -264,63 +328,121 @@ __global__ __launch_bounds__(kPPThreads, 2) void gemm_fp8_pp_kernel(const uint8_
       for (int s = 0; s < steps; s += 2) {
         const int ka = kbyte(s + 1);  // the current tile's
         const int v1[2] = {va[1][0], va[1][1]};
+        if constexpr (kLora) dma(ra, a11, v1, ka);  // (here for two registers less)
         int s2 = s + 2;
+        const bool lora_next = kLora && s2 == steps && lt.pairs;
         if (s2 == steps) {
           // the next loads are the next tile's first steps (past the last tile
           // they repeat this one's)
-          if (Ln < xend) {
+          if (lora_next) {
+            set_lora_offsets(0, m0, n0);
+          } else if (Ln < xend) {
             tile_of(Ln, m0, n0);
             set_offsets(m0, n0);
           }
           s2 = 0;
         }
-        const int k2 = kbyte(s2), k3 = kbyte(s2 + 1);
-        dma(rb, b00, vb[0], k2);
-        dma(ra, a11, v1, ka);
+        const int k2 = kbyte(s2), k3 = lora_next ? lora_lo : kbyte(s2 + 1), k3b = lora_next ? 0 : k3;
+        __amdgpu_buffer_rsrc_t ra_n = ra, rb_n = rb;
+        if constexpr (kLora) ra_n = na.rsrc(), rb_n = nb.rsrc();
+        dma(rb_n, b00, vb[0], k2);
+        if constexpr (!kLora) dma(ra, a11, v1, ka);
         read_a(a00, fa);
         read_b(b01, fb1);
         read_sc(sc0, s);
         mem_end();
         prod(acc[0], fa, fb0, fb1, sa[0], s, no);
-        dma(ra, a00, va[0], k2);
-        dma(rb, b01, vb[1], k2);
+        dma(ra_n, a00, va[0], k2);
+        dma(rb_n, b01, vb[1], k2);
         dma_sc(sc0, s2);
         read_a(a01, fa);
         read_b(b10, fbn);
         mem_end();
         prod(acc[1], fa, fb0, fb1, sa[1], s, no);
-        dma(rb, b10, vb[0], k3);
-        dma(ra, a01, va[1], k2);
+        dma(rb_n, b10, vb[0], k3b);
+        dma(ra_n, a01, va[1], k2);
         read_a(a10, fa);
         read_b(b11, fb1);
         read_sc(sc1, s + 1);
         mem_end();
         prod(acc[0], fa, fbn, fb1, sa[0], s + 1, yes);
-        dma(ra, a10, va[0], k3);
-        dma(rb, b11, vb[1], k3);
+        dma(ra_n, a10, va[0], k3);
+        dma(rb_n, b11, vb[1], k3b);
         dma_sc(sc1, s2 + 1);
         read_a(a11, fa);
         read_b(b00, fb0);
         mem_end();
         prod(acc[1], fa, fbn, fb1, sa[1], s + 1, yes);
       }
-      if (!wm) half_barrier();
-      const int lane_e = new_lane();
       if constexpr (kLora) {
+        // the adapters' pairs of steps, as the loop's; the next loads are the next pair's or tile's
+        for (int e = 0; e < lt.pairs; ++e) {
+          dma(na.rsrc(), a11, va[1], lora_lo);
+          int k3a = kbyte(1), k3b = k3a;
+          if (e + 1 < lt.pairs) {
+            set_lora_offsets(e + 1, m0, n0);
+            k3a = lora_lo;
+            k3b = 0;
+          } else if (Ln < xend) {
+            tile_of(Ln, m0, n0);
+            set_offsets(m0, n0);
+            na = LoraBase(A);
+            nb = LoraBase(B);
+          } else {
+            k3a = k3b = 0;
+          }
+          const __amdgpu_buffer_rsrc_t ra_n = na.rsrc(), rb_n = nb.rsrc();
+          dma(rb_n, b00, vb[0], 0);
+          read_a(a00, fa);
+          read_b(b01, fb1);
+          mem_end();
+          prod_lora(acc[0], fa, fb0, fb1);
+          dma(ra_n, a00, va[0], 0);
+          dma(rb_n, b01, vb[1], 0);
+          dma_sc(sc0, 0);
+          read_a(a01, fa);
+          read_b(b10, fbn);
+          mem_end();
+          prod_lora(acc[1], fa, fb0, fb1);
+          dma(rb_n, b10, vb[0], k3b);
+          dma(ra_n, a01, va[1], 0);
+          read_a(a10, fa);
+          read_b(b11, fb1);
+          mem_end();
+          prod_lora(acc[0], fa, fbn, fb1);
+          dma(ra_n, a10, va[0], k3a);
+          dma(rb_n, b11, vb[1], k3b);
+          dma_sc(sc1, 1);
+          read_a(a11, fa);
+          read_b(b00, fb0);
+          mem_end();
+          prod_lora(acc[1], fa, fbn, fb1);
+        }
+        if (lt.part) {
+          float bad = 0.0f;
 #pragma unroll
-        for (int a = 0; a < 2; ++a) {
-          const int cb[2] = {n0c + 32 * wn, n0c + 128 + 32 * wn};
-          lora_add<4, 2, 1>(lo, M, N, m0c + 128 * a + 64 * wm, cb, lane_e, 0, 1,
-                            [&](int i, int j, int t) -> gdn::f32x4_t& { return acc[a][j][i][t]; });
+          for (int a = 0; a < 2; ++a)
+#pragma unroll
+            for (int b = 0; b < 2; ++b)
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int t = 0; t < 2; ++t)
+#pragma unroll
+                  for (int x = 0; x < 4; ++x) bad = fmaf(acc[a][b][i][t][x], 0.0f, bad);
+          if (bad != 0.0f) tiles_l.again[at - 1] = 1;
         }
       }
+      if (!wm) half_barrier();
+      const int lane_e = new_lane();
+      const GemmOut out_e = kLora ? kernel_arg<GemmOut>(offsetof(Args, out)) : out;
 #pragma unroll
       for (int a = 0; a < 2; ++a)
 #pragma unroll
         for (int i = 0; i < 4; ++i)
 #pragma unroll
           for (int b = 0; b < 2; ++b)
-            gemm_store16<true>(acc[a][b][i][0], acc[a][b][i][1], out, M, N, m0c + 128 * a + 64 * wm + 16 * i,
+            gemm_store16<true>(acc[a][b][i][0], acc[a][b][i][1], out_e, M, N, m0c + 128 * a + 64 * wm + 16 * i,
                          n0c + 128 * b + 32 * wn, lane_e, GemmGates{}, nullptr);
       if (Ln >= xend) break;
       L = Ln;
@@ -332,9 +454,26 @@ __global__ __launch_bounds__(kPPThreads, 2) void gemm_fp8_pp_kernel(const uint8_
   const int nq = whole ? 4 * (tiles - whole) : mq_n * nq_n;
   const int q_xcd = (nq + gdn::kNumXcd - 1) / gdn::kNumXcd;
   const int qend = min((xcd + 1) * q_xcd, nq);
-  for (int q = xcd * q_xcd + slot; q < qend; q += stride) {
-    int m0, n0;
-    if (whole) {
+  // (kLora) the quarters of the workgroup's own tiles first: ql of them, then q as without
+  int ql = 0;
+  if constexpr (kLora) n_quarters = lora_quarters(tiles_l);
+  for (int q = xcd * q_xcd + slot; q < qend || (kLora && ql < n_quarters); q += stride) {
+    int m0 = 0, n0 = 0;
+    bool own = false;
+    if constexpr (kLora) {
+      own = ql < n_quarters;
+      if (own) {
+        q -= stride;
+        tile_of(__builtin_amdgcn_readfirstlane(tiles_l.in_quarters[ql >> 2]), m0, n0);
+        m0 += 128 * ((ql >> 1) & 1);
+        n0 += 128 * (ql & 1);
+        ++ql;
+        if (m0 >= M || n0 >= N) continue;  // (the whole workgroup)
+      }
+    }
+    if (own) {
+      // (m0 and n0 are there)
+    } else if (whole) {
       tile_of(whole + (q >> 2), m0, n0);
       m0 += 128 * ((q >> 1) & 1);
       n0 += 128 * (q & 1);
@@ -400,14 +539,13 @@ __global__ __launch_bounds__(kPPThreads, 2) void gemm_fp8_pp_kernel(const uint8_
       step(a11, b11, sc3, a10, b10, sc2, s + 3);
     }
     if (!wm) half_barrier();
-    if constexpr (kLora) {
-      const int cb[1] = {n0 + 32 * wn};
-      lora_add<4, 1, 2>(lo, M, N, m0 + 64 * wm, cb, new_lane(), 0, 1,
-                        [&](int i, int, int t) -> gdn::f32x4_t& { return c[i][t]; });
-    }
+    if constexpr (kLora)
+      lora_add<4>(kernel_arg<Lora>(kLoraAt), M, N, m0 + 64 * wm, n0 + 32 * wn, new_lane(),
+                  [&](int i, int t) -> gdn::f32x4_t& { return c[i][t]; });
+    const GemmOut out_q = kLora ? kernel_arg<GemmOut>(offsetof(Args, out)) : out;
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-      gemm_store16<true>(c[i][0], c[i][1], out, M, N, m0 + 64 * wm + 16 * i, n0 + 32 * wn, new_lane(), GemmGates{}, nullptr);
+      gemm_store16<true>(c[i][0], c[i][1], out_q, M, N, m0 + 64 * wm + 16 * i, n0 + 32 * wn, new_lane(), GemmGates{}, nullptr);
   }
   __builtin_amdgcn_s_waitcnt(0);
 }
@@ -737,7 +875,7 @@ __global__ __launch_bounds__(64 * NW) void gemm_fp8_ring_kernel(const void* __re
     int cb[NT];
 #pragma unroll
     for (int j = 0; j < NT; ++j) cb[j] = n0 + 32 * j;
-    lora_add<MT, NT, 4>(lo, M, N, m0, cb, lane, wave, NW,
+    lora_init<MT, NT, 4>(lo, M, N, m0, cb, lane, wave, NW,
                         [&](int i, int j, int t) -> gdn::f32x4_t& { return acc[i][j][t]; });
   }
   __builtin_amdgcn_s_waitcnt(kWait);
@@ -1047,7 +1185,7 @@ __global__ __launch_bounds__(kFp8Threads * H, 2) void gemm_fp8_deep_kernel(const
     int cb[NJ];
 #pragma unroll
     for (int j = 0; j < NJ; ++j) cb[j] = n0 + 32 * (NJ * wn + j);
-    lora_add<2, NJ, 4>(lo, M, N, m0 + 32 * wm, cb, lane, half, H,
+    lora_init<2, NJ, 4>(lo, M, N, m0 + 32 * wm, cb, lane, half, H,
                        [&](int i, int j, int t) -> gdn::f32x4_t& { return acc[i][j][t]; });
   }
   // (no exit inside a trip: the compiler's load counting would merge its states at the
@@ -1174,6 +1312,7 @@ int fp8_launch(Fp8Kernel kernel, const void* A, int64_t lda, const uint8_t* B, i
   auto grid = [](int64_t wgs) {
     return dim3(static_cast<unsigned>(gdn::kNumXcd * ((wgs + gdn::kNumXcd - 1) / gdn::kNumXcd)));
   };
+  if (kLora && kernel == kPP && !lora_tiles_fit(blocks(256, 256))) kernel = kDeep128;
   const uint8_t* A8 = static_cast<const uint8_t*>(A);
   const uint16_t* A16 = static_cast<const uint16_t*>(A);
   auto rows_grid = [&](int bn) { return grid(blocks(16, bn) + blocks(16, 1 << 30) * (wide.n / 16)); };
@@ -1313,8 +1452,8 @@ extern "C" int gdn_gemm_fp8(const void* A, int a_is_bf16, int64_t lda, const flo
 extern "C" int gdn_gemm_fp8_lora(const uint8_t* A, int64_t lda, const float* sa, int64_t sa_row, int64_t sa_grp,
                                  const uint8_t* B, int64_t ldb, const float* sb, int64_t sb_row, int M, int N, int K,
                                  int n_parts, uint16_t* const* C, const int64_t* ldc, const int* col_end,
-                                 const uint16_t* v, int64_t ldv, const uint16_t* lb, int64_t lb_slot, const int32_t* ids,
-                                 int slots, int rank, int slices, const int* slice_end, void* stream) {
+                                 const uint16_t* v, int64_t ldv, const int32_t* groups, const uint16_t* lb,
+                                 int64_t lb_slot, const int32_t* ids, int slots, int rank, int slices, const int* slice_end, void* stream) {
   if (M < 0 || N < 0 || K < 0 || n_parts < 1 || n_parts > kMaxParts || !C || !ldc || !col_end)
     return GDN_ERR_INVALID_ARG;
   if (M == 0 || N == 0) return GDN_OK;
@@ -1323,7 +1462,10 @@ extern "C" int gdn_gemm_fp8_lora(const uint8_t* A, int64_t lda, const float* sa,
   GemmOut out{};
   if (!parts_of(out, n_parts, C, ldc, col_end, N, true)) return GDN_ERR_INVALID_ARG;
   Lora lo{};
-  if (!lora_of(lo, v, ldv, lb, lb_slot, ids, slots, rank, slices, slice_end, M, N)) return GDN_ERR_INVALID_ARG;
+  if (!lora_of(lo, v, ldv, groups, lb, lb_slot, ids, slots, rank, slices, slice_end, M, N)) return GDN_ERR_INVALID_ARG;
+  if (slots == 0)
+    return fp8_launch<false>(fp8_plan(M, N, K, false), A, lda, B, ldb, Fp8Scales{sa, sa_row, sa_grp, sb, sb_row}, out, M, N,
+                             K, Fp8Wide{}, NoLora{}, static_cast<hipStream_t>(stream));
   return fp8_launch<true>(fp8_plan(M, N, K, false), A, lda, B, ldb, Fp8Scales{sa, sa_row, sa_grp, sb, sb_row}, out, M, N,
                           K, Fp8Wide{}, lo, static_cast<hipStream_t>(stream));
 }

@@ -38,6 +38,7 @@ struct Shrink {
   int slots, cols, rank, M, K;
   uint16_t* v;
   int64_t ldv;
+  int* groups;      // [ceil(M / 16)]: the adapter of 16 rows, -1 none, -2 not one for all
 };
 
 // 8 e4m3 values as bf16
@@ -81,12 +82,16 @@ __global__ __launch_bounds__(64 * NW) void lora_shrink_kernel(Shrink p) {
     const int r = m0 + 16 * i + lr;
     const int s = p.ids[min(r, p.M - 1)];
     id[i] = r < p.M && static_cast<unsigned>(s) < static_cast<unsigned>(p.slots) ? s : -1;
+    const int first = __builtin_amdgcn_readfirstlane(id[i]);
+    const bool alike = !__any(r < p.M && id[i] != first);
+    if (c0 == 0 && blockIdx.y == 0 && threadIdx.x == 0 && r < p.M) p.groups[m0 / 16 + i] = alike ? first : -2;
   }
   int mine = BM > lane ? id[0] : -1;  // row m0 + lane's
 #pragma unroll
   for (int i = 1; i < MT; ++i) mine = lg == i ? id[i] : mine;
   LoraIds it{__ballot(mine >= 0), static_cast<int>(blockIdx.y), static_cast<int>(gridDim.y), 0};
-  int s = it.next(mine);
+  uint64_t rows;
+  int s = it.next(mine, rows);
   if (s < 0) return;  // (the workgroup)
 
   const __amdgpu_buffer_rsrc_t rx = rsrc_of(p.x), rs = rsrc_of(p.xs);
@@ -213,7 +218,7 @@ __global__ __launch_bounds__(64 * NW) void lora_shrink_kernel(Shrink p) {
       *reinterpret_cast<uint2*>(at) = make_uint2(gdn::f2bf2(hi[0], hi[1]), gdn::f2bf2(hi[2], hi[3]));
       *reinterpret_cast<uint2*>(at + p.rank) = make_uint2(gdn::f2bf2(lo[0], lo[1]), gdn::f2bf2(lo[2], lo[3]));
     }
-    s = it.next(mine);
+    s = it.next(mine, rows);
     if (s >= 0) __syncthreads();  // the sums have been read
   }
 }
@@ -242,16 +247,17 @@ int launch(const Shrink& p, hipStream_t st) {
 
 extern "C" int gdn_lora_shrink(const void* x, int x_is_bf16, int64_t ldx, const float* xs, int64_t xs_row, int64_t xs_grp,
                                const uint16_t* a, int64_t a_slot, const float* scale, const int32_t* ids, int slots,
-                               int slices, int rank, int M, int K, uint16_t* v, int64_t ldv, void* stream) {
+                               int slices, int rank, int M, int K, uint16_t* v, int64_t ldv, int32_t* groups,
+                               void* stream) {
   const int64_t kLimit = 1LL << 31;
   if (M < 0 || slots < 0 || slices < 1 || slices > kMaxParts || rank < 8 || rank > kMaxRank || rank % 8 || K <= 0 ||
       K % (x_is_bf16 ? 64 : gdn::kFp8Group))
     return GDN_ERR_INVALID_ARG;
   if (M == 0 || slots == 0) return GDN_OK;
   const int cols = slices * rank;
-  if (!x || !a || !scale || !ids || !v || (!x_is_bf16 && !xs)) return GDN_ERR_INVALID_ARG;
+  if (!x || !a || !scale || !ids || !v || !groups || (!x_is_bf16 && !xs)) return GDN_ERR_INVALID_ARG;
   if (reinterpret_cast<uintptr_t>(x) % 16 || reinterpret_cast<uintptr_t>(a) % 16 || reinterpret_cast<uintptr_t>(v) % 8 ||
-      reinterpret_cast<uintptr_t>(scale) % 4 || reinterpret_cast<uintptr_t>(ids) % 4 || ldx < K ||
+      reinterpret_cast<uintptr_t>(scale) % 4 || reinterpret_cast<uintptr_t>(ids) % 4 || reinterpret_cast<uintptr_t>(groups) % 4 || ldx < K ||
       ldx % (x_is_bf16 ? 8 : 16) || M * ldx * (x_is_bf16 ? 2 : 1) >= kLimit || a_slot % 8 ||
       (slots > 1 && a_slot < static_cast<int64_t>(cols) * K) || static_cast<int64_t>(cols) * K * 2 >= kLimit ||
       ldv % 4 || ldv < 2LL * cols)
@@ -259,7 +265,7 @@ extern "C" int gdn_lora_shrink(const void* x, int x_is_bf16, int64_t ldx, const 
   if (!x_is_bf16 && (reinterpret_cast<uintptr_t>(xs) % 4 || xs_row < 0 || xs_grp < 0 ||
                      4 * ((M - 1) * xs_row + (K / gdn::kFp8Group - 1) * xs_grp) >= kLimit))
     return GDN_ERR_INVALID_ARG;
-  const Shrink p{x, ldx, xs, xs_row, xs_grp, a, a_slot, scale, ids, slots, cols, rank, M, K, v, ldv};
+  const Shrink p{x, ldx, xs, xs_row, xs_grp, a, a_slot, scale, ids, slots, cols, rank, M, K, v, ldv, groups};
   const hipStream_t st = static_cast<hipStream_t>(stream);
   return x_is_bf16 ? launch<false>(p, st) : launch<true>(p, st);
 }

@@ -1602,12 +1602,14 @@ def _lora_check(x, N, K, widths, lora_a, lora_b, lora_scale, ids):
 
 
 def _lora_shrink(idx, rows, stride, x_scale, lora_a, lora_scale, ids, M, K, P, R):
-    """v [M, P, 2, R] of the rows with an adapter."""
+    """(v [M, P, 2, R] of the rows with an adapter, the adapters of their groups of 16)."""
     v = torch.empty(M, P * 2 * R, dtype=torch.bfloat16, device=rows.device)
+    groups = torch.empty(-(-M // 16), dtype=torch.int32, device=rows.device)
     xs = (0, 0, 0) if x_scale is None else (x_scale.data_ptr(), *x_scale.stride())
     _call_on(idx, "gdn_lora_shrink", rows.data_ptr(), int(x_scale is None), stride, *xs, lora_a.data_ptr(),
-             lora_a.stride(0), lora_scale.data_ptr(), ids.data_ptr(), lora_a.shape[0], P, R, M, K, v.data_ptr(), 2 * P * R)
-    return v
+             lora_a.stride(0), lora_scale.data_ptr(), ids.data_ptr(), lora_a.shape[0], P, R, M, K, v.data_ptr(), 2 * P * R,
+             groups.data_ptr())
+    return v, groups
 
 
 def _tables(outs, widths, slices):
@@ -1618,9 +1620,10 @@ def _tables(outs, widths, slices):
             (ctypes.c_int * len(slices))(*[sum(slices[:i + 1]) for i in range(len(slices))]))
 
 
-def _gemm_bf16_lora(idx, rows, stride, weight, outs, widths, slices, first, col, v, lora_b, ids, gates=None):
+def _gemm_bf16_lora(idx, rows, stride, weight, outs, widths, slices, first, col, shrunk, lora_b, ids, gates=None):
     """The bf16 product and the adapters' part into outs: its columns are lora_b's from `col` on, its
     slices v's from `first` on.  With gates, (g, beta)."""
+    v, groups = shrunk
     M, (N, K) = v.shape[0], weight.shape
     R = lora_b.shape[2]
     c, ld, ends, slice_ends = _tables(outs, widths, slices)
@@ -1638,7 +1641,7 @@ def _gemm_bf16_lora(idx, rows, stride, weight, outs, widths, slices, first, col,
         _lib.call("gdn_gemm_bf16_lora", rows.data_ptr(), stride, weight.data_ptr(), weight.stride(0), M, N, K, len(widths),
                   c, ld, ends, _lib.ptr(g), _lib.ptr(beta), _lib.ptr(a_log), _lib.ptr(dt_bias),
                   int(a_log is not None and a_log.dtype == torch.float32), gate_col, Hv, v.data_ptr() + 4 * first * R,
-                  v.stride(0), lora_b.data_ptr() + 2 * col * R, lora_b.stride(0), ids.data_ptr(), lora_b.shape[0], R,
+                  v.stride(0), groups.data_ptr(), lora_b.data_ptr() + 2 * col * R, lora_b.stride(0), ids.data_ptr(), lora_b.shape[0], R,
                   len(slices), slice_ends, _lib.stream_of(idx))
     return g, beta
 
@@ -1680,8 +1683,8 @@ def linear_lora(x: torch.Tensor, weight: torch.Tensor, lora_a: torch.Tensor, lor
     rows, _, stride = _rows_of(x, 8)
     weight, ids = _weight_rows(weight, 8), ids.contiguous()
     outs = [torch.empty(M, w, dtype=torch.bfloat16, device=x.device) for w in parts]
-    v = _lora_shrink(idx, rows, stride, None, lora_a, lora_scale, ids, M, K, P, R)
-    g, beta = _gemm_bf16_lora(idx, rows, stride, weight, outs, parts, parts, 0, 0, v, lora_b, ids, gates)
+    shrunk = _lora_shrink(idx, rows, stride, None, lora_a, lora_scale, ids, M, K, P, R)
+    g, beta = _gemm_bf16_lora(idx, rows, stride, weight, outs, parts, parts, 0, 0, shrunk, lora_b, ids, gates)
     y = [t.view(*x.shape[:-1], t.shape[1]) for t in outs]
     y = y[0] if widths is None else y
     return y if gates is None else (y, g, beta)
@@ -1724,7 +1727,7 @@ def linear_fp8_lora(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.T
     if not weight_scale.is_contiguous():
         weight_scale = weight_scale.contiguous()
     outs = [torch.empty(M, w, dtype=torch.bfloat16, device=x.device) for w in parts]
-    v = _lora_shrink(idx, rows, stride, x_scale, lora_a, lora_scale, ids, M, K, P, R)
+    shrunk = v, groups = _lora_shrink(idx, rows, stride, x_scale, lora_a, lora_scale, ids, M, K, P, R)
     x8, x8_stride, xs = rows, stride, x_scale
     if x_scale is None:
         x8 = torch.empty(M, K, dtype=FP8, device=x.device)
@@ -1734,11 +1737,11 @@ def linear_fp8_lora(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.T
     with torch.cuda.device(idx):
         _lib.call("gdn_gemm_fp8_lora", x8.data_ptr(), x8_stride, xs.data_ptr(), *xs.stride(), weight.data_ptr(),
                   weight.stride(0), weight_scale.data_ptr(), G, M, N, K, n, c, ld, ends, v.data_ptr(), v.stride(0),
-                  lora_b.data_ptr(), lora_b.stride(0), ids.data_ptr(), lora_b.shape[0], R, n, slice_ends,
+                  groups.data_ptr(), lora_b.data_ptr(), lora_b.stride(0), ids.data_ptr(), lora_b.shape[0], R, n, slice_ends,
                   _lib.stream_of(idx))
     g = beta = None
     if wide is not None:
-        g, beta = _gemm_bf16_lora(idx, rows, stride, _weight_rows(wide, 8), outs[n:], parts[n:], parts[n:], n, N, v,
+        g, beta = _gemm_bf16_lora(idx, rows, stride, _weight_rows(wide, 8), outs[n:], parts[n:], parts[n:], n, N, shrunk,
                                   lora_b, ids, gates)
     y = [t.view(*x.shape[:-1], t.shape[1]) for t in outs]
     y = y[0] if widths is None else y

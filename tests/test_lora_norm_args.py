@@ -129,7 +129,7 @@ def test_c_entries_refuse(pkg):
     assert norm() == bad and norm(M=-1) == bad and norm(H=0) == bad and norm(g_col=2) == bad
     assert norm(H=16385) == pkg._lib.GDN_ERR_UNSUPPORTED and norm(M=0) == 0
     shrink = lambda slots=2, slices=1, rank=16, M=4, K=128: lib.gdn_lora_shrink(  # noqa: E731
-        None, 1, K, None, 0, 0, None, 0, None, None, slots, slices, rank, M, K, None, 32, None)
+        None, 1, K, None, 0, 0, None, 0, None, None, slots, slices, rank, M, K, None, 32, None, None)
     for kw in (dict(), dict(slots=-1), dict(slices=0), dict(slices=5), dict(rank=12), dict(rank=264), dict(rank=0), dict(K=96),
                dict(M=-1), dict(K=0)):
         assert shrink(**kw) == bad, kw
@@ -140,17 +140,17 @@ def test_c_entries_refuse(pkg):
         pytest.skip("dummy device addresses are passed only where no GPU is visible")
     P = ctypes.c_void_p(1 << 20)
 
-    def bf16(M=4, N=96, K=64, ends=(96,), slice_ends=(96,), v=P, ldv=32, lb=P, lb_slot=96 * 16, ids=P, slots=2, rank=16):
+    def bf16(M=4, N=96, K=64, ends=(96,), slice_ends=(96,), v=P, ldv=32, groups=P, lb=P, lb_slot=96 * 16, ids=P, slots=2, rank=16):
         return lib.gdn_gemm_bf16_lora(P, K, P, K, M, N, K, len(ends), *parts, n(*ends), None, None, None, None, 0, 0, 0, v, ldv,
-                                      lb, lb_slot, ids, slots, rank, len(slice_ends), n(*slice_ends), None)
+                                      groups, lb, lb_slot, ids, slots, rank, len(slice_ends), n(*slice_ends), None)
 
-    def fp8(M=4, N=96, K=128, ends=(96,), slice_ends=(96,), v=P, ldv=32, lb=P, lb_slot=96 * 16, ids=P, slots=2, rank=16):
-        return lib.gdn_gemm_fp8_lora(P, K, P, 1, M, P, K, P, 1, M, N, K, len(ends), *parts, n(*ends), v, ldv, lb, lb_slot, ids,
+    def fp8(M=4, N=96, K=128, ends=(96,), slice_ends=(96,), v=P, ldv=32, groups=P, lb=P, lb_slot=96 * 16, ids=P, slots=2, rank=16):
+        return lib.gdn_gemm_fp8_lora(P, K, P, 1, M, P, K, P, 1, M, N, K, len(ends), *parts, n(*ends), v, ldv, groups, lb, lb_slot, ids,
                                      slots, rank, len(slice_ends), n(*slice_ends), None)
 
-    odd = ctypes.c_void_p((1 << 20) + 2)
+    odd, byte = ctypes.c_void_p((1 << 20) + 2), ctypes.c_void_p((1 << 20) + 1)
     for call in (bf16, fp8):
-        for kw in (dict(v=None), dict(v=odd), dict(lb=None), dict(lb=odd), dict(ids=None), dict(ids=odd), dict(slots=-1),
+        for kw in (dict(v=None), dict(v=odd), dict(groups=None), dict(groups=byte), dict(lb=None), dict(lb=odd), dict(ids=None), dict(ids=odd), dict(slots=-1),
                    dict(rank=12), dict(rank=264), dict(ldv=24), dict(ldv=36), dict(lb_slot=95 * 16), dict(lb_slot=96 * 16 + 4),
                    dict(slice_ends=(90,)), dict(slice_ends=(24, 96)), dict(slice_ends=(96, 96), ldv=64), dict(slice_ends=()),
                    dict(slice_ends=(48, 96)), dict(M=1 << 30), dict(K=100), dict(ends=(90,))):
@@ -164,7 +164,6 @@ def test_c_entries_refuse(pkg):
                                     a["g_col"], 0, 1.0, 1e-6, a["out"], a["y"], a["y8"], a["ys"], 1, 4, 4, a["H"],
                                     ctypes.c_void_p(-1))
     assert norm() == 0 and norm(y8=P, ys=P) == 0 and norm(y=None, y8=P, ys=P) == 0     # (checked only: nothing is launched)
-    byte = ctypes.c_void_p((1 << 20) + 1)
     for kw in (dict(x=None), dict(w=None), dict(y=None), dict(y8=P), dict(sx=255), dict(sr=255), dict(x=byte), dict(res=byte),
                dict(gate=P, g_col=1, g_row=255), dict(gate=byte), dict(y8=P, ys=P, H=200), dict(y8=P, ys=P, x=odd),
                dict(y8=P, ys=P, sx=260), dict(y8=odd, ys=P), dict(y8=P, ys=P, gate=odd, g_col=1)):
