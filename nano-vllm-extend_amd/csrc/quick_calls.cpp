@@ -512,6 +512,217 @@ PyObject* norm_fp8(PyObject*, PyObject* const* a, Py_ssize_t n) {
   });
 }
 
+// (x, residual or None, weight, eps, post_weight or None, gate or None, gate_sigmoid, scale, offset, bf16, fp8)
+// -> (y or None, y8 or None, scales or None, r)
+PyObject* add_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded(n, 11, [&]() -> PyObject* {
+    Taken t;
+    const Tensor& x = t.tensor(a[0], kBf16, -1);
+    if (!t.ok || x.dim() < 1 || !x.is_contiguous() || x.numel() == 0 || !PyFloat_CheckExact(a[3]) || !PyBool_Check(a[6]) ||
+        !PyFloat_CheckExact(a[7]) || !PyFloat_CheckExact(a[8]) || !PyBool_Check(a[9]) || !PyBool_Check(a[10]) ||
+        !THPVariable_CheckExact(a[2]))
+      return none();
+    const int64_t H = x.size(-1), M = x.numel() / H;
+    const bool want = a[9] == Py_True, fp8 = a[10] == Py_True;
+    const double scale = PyFloat_AS_DOUBLE(a[7]);
+    const ScalarType wt = THPVariable_Unpack(a[2]).scalar_type();
+    t.need((wt == kBf16 || wt == kF32) && H <= 16384 && M < (int64_t{1} << 31) && (!fp8 || H % kGroup == 0));
+    const int64_t align = fp8 ? 16 : 2;
+    const Tensor& w = t.dense(a[2], wt, {H}, align);
+    t.need(aligned(x, align));
+    const Tensor* post = a[4] == Py_None ? nullptr : &t.dense(a[4], wt, {H}, align);
+    const Tensor* res = nullptr;
+    ScalarType rt = kBf16;
+    if (a[1] != Py_None) {
+      if (!THPVariable_CheckExact(a[1])) return none();
+      rt = THPVariable_Unpack(a[1]).scalar_type();
+      t.need(rt == kBf16 || rt == kF32);
+      res = &t.dense(a[1], rt, x.sizes(), align);
+    }
+    const Tensor* gate = nullptr;
+    int64_t g_row = 0, g_col = 0;
+    if (a[5] != Py_None && t.ok) {
+      if (!THPVariable_CheckExact(a[5])) return none();
+      const ScalarType gt = THPVariable_Unpack(a[5]).scalar_type();
+      t.need(gt == kBf16 || gt == kF32);
+      gate = &t.tensor(a[5], gt, -1);
+      if (!t.ok || !gate->is_contiguous()) return none();
+      at::DimVector rows(x.sizes().begin(), x.sizes().end());
+      rows.back() = 1;
+      if (H > 1 && gate->sizes() == IntArrayRef(rows)) g_row = 1;
+      else if (gate->sizes() == x.sizes()) g_row = H, g_col = 1;
+      else if (gate->dim() == 1 && gate->size(0) == H) g_col = 1;
+      else return none();
+      t.need(g_col == 0 || aligned(*gate, align));
+    }
+    if (!t.here()) return none();
+    const bool same = !res && !post && !gate && scale == 1.0;  // r is x
+    Tensor r = same ? x : at::empty(x.sizes(), x.options().dtype(rt));
+    Tensor y, y8, ys;
+    if (want) y = at::empty(x.sizes(), x.options());
+    if (fp8) {
+      y8 = at::empty(x.sizes(), x.options().dtype(kFp8));
+      ys = at::empty_strided({M, H / kGroup}, {1, M}, x.options().dtype(kF32));
+    }
+    const int status = gdn_add_rms_norm(
+        bf(x), H, res ? res->data_ptr() : nullptr, H, rt == kF32 ? 1 : 0, w.data_ptr(), post ? post->data_ptr() : nullptr,
+        wt == kF32 ? 1 : 0, static_cast<float>(PyFloat_AS_DOUBLE(a[8])), gate ? gate->data_ptr() : nullptr,
+        gate && gate->scalar_type() == kF32 ? 1 : 0, g_row, g_col, a[6] == Py_True ? 1 : 0, static_cast<float>(scale),
+        static_cast<float>(PyFloat_AS_DOUBLE(a[3])), same ? nullptr : r.data_ptr(), want ? bf(y) : nullptr,
+        fp8 ? ptr<uint8_t>(y8) : nullptr, fp8 ? ptr<float>(ys) : nullptr, 1, M, M, static_cast<int>(H), t.stream());
+    if (failed("gdn_add_rms_norm", status)) return nullptr;
+    auto given = [](bool is, Tensor& v) { return is ? THPVariable_Wrap(std::move(v)) : none(); };
+    PyObject *oy = given(want, y), *o8 = given(fp8, y8), *os = given(fp8, ys);
+    PyObject* o = same ? (Py_INCREF(a[0]), a[0]) : THPVariable_Wrap(std::move(r));
+    return Py_BuildValue("(NNNN)", oy, o8, os, o);
+  });
+}
+
+// The adapters of a product with N columns and its parts.
+struct Adapters {
+  int64_t S = 0, P = 0, R = 0;
+  int n = 0, end[4] = {};
+  int64_t width[4] = {};
+  const Tensor *a = nullptr, *b = nullptr, *scale = nullptr, *ids = nullptr;
+  Tensor work, parts[4];
+  int64_t M = 0;
+
+  // arguments lora_a, lora_b, lora_scale, ids; widths: a list, or None for one part
+  bool take(Taken& t, PyObject* const* o, PyObject* widths, int64_t rows, int64_t N, int64_t K, IntArrayRef lead) {
+    M = rows;
+    if (widths == Py_None) {
+      n = 1, width[0] = N, end[0] = static_cast<int>(N);
+    } else {
+      if (!PyList_CheckExact(widths) || PyList_GET_SIZE(widths) < 1 || PyList_GET_SIZE(widths) > 4) return false;
+      int64_t sum = 0;
+      for (n = 0; n < PyList_GET_SIZE(widths); ++n) {
+        PyObject* w = PyList_GET_ITEM(widths, n);
+        if (!PyLong_CheckExact(w)) return false;
+        width[n] = PyLong_AsLongLong(w);
+        if (width[n] <= 0 || width[n] > N - sum) {
+          PyErr_Clear();
+          return false;
+        }
+        sum += width[n];
+        end[n] = static_cast<int>(sum);
+        if (n + 1 < PyList_GET_SIZE(widths) && sum % 16) return false;
+      }
+      if (sum != N) return false;
+    }
+    a = &t.tensor(o[0], kBf16, 3);
+    b = &t.tensor(o[1], kBf16, 3);
+    if (!t.ok) return false;
+    S = b->size(0), R = b->size(2), P = n;
+    t.need(S > 0 && R >= 8 && R <= 256 && R % 8 == 0 && b->size(1) == N && a->size(0) == S && a->size(1) == P * R &&
+           a->size(2) == K && S < (int64_t{1} << 31));
+    for (const Tensor* v : {a, b})
+      t.need(v->stride(2) == 1 && v->stride(1) == v->size(2) && aligned(*v) &&
+             (S == 1 || (v->stride(0) % 8 == 0 && v->stride(0) >= v->size(1) * v->size(2))));
+    scale = &t.dense(o[2], kF32, {S}, 4);
+    ids = &t.tensor(o[3], ScalarType::Int, -1);
+    if (!t.ok) return false;
+    t.need(ids->is_contiguous() && ((ids->dim() == 1 && ids->size(0) == M) || ids->sizes() == lead));
+    return t.ok;
+  }
+  uint16_t* v() const { return static_cast<uint16_t*>(work.data_ptr()); }
+  int64_t ldv() const { return 2 * P * R; }
+  int32_t* groups() const { return reinterpret_cast<int32_t*>(v() + M * ldv()); }
+  void allocate(const Tensor& x, IntArrayRef lead) {
+    work = at::empty({M * ldv() * 2 + (M + 15) / 16 * 4}, x.options().dtype(ScalarType::Byte));
+    for (int i = 0; i < n; ++i) {
+      at::DimVector shape(lead.begin(), lead.end());
+      shape.push_back(width[i]);
+      parts[i] = at::empty(shape, x.options().dtype(kBf16));
+    }
+  }
+  int shrink(const Tensor& x, const Tensor* xs, int64_t K, void* stream) const {
+    return gdn_lora_shrink(x.data_ptr(), xs ? 0 : 1, K, xs ? ptr<float>(*xs) : nullptr, xs ? xs->stride(0) : 0,
+                           xs ? xs->stride(1) : 0, bf(*a), a->stride(0), ptr<float>(*scale), ptr<int32_t>(*ids),
+                           static_cast<int>(S), static_cast<int>(P), static_cast<int>(R), static_cast<int>(M),
+                           static_cast<int>(K), v(), ldv(), groups(), stream);
+  }
+  PyObject* given(PyObject* widths) {
+    if (widths == Py_None) return THPVariable_Wrap(std::move(parts[0]));
+    PyObject* list = PyList_New(n);
+    if (!list) return nullptr;
+    for (int i = 0; i < n; ++i) PyList_SET_ITEM(list, i, THPVariable_Wrap(std::move(parts[i])));
+    return list;
+  }
+};
+
+// (x, weight, lora_a, lora_b, lora_scale, ids, widths or None) -> y, or the list of its parts
+PyObject* linear_lora(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded(n, 7, [&]() -> PyObject* {
+    Taken t;
+    const Tensor& x = t.tensor(a[0], kBf16, -1);
+    const Tensor& w = t.tensor(a[1], kBf16, 2);
+    if (!t.ok || x.dim() < 2 || x.numel() == 0) return none();
+    const int64_t N = w.size(0), K = w.size(1);
+    if (N == 0 || K == 0 || K % 64 || x.size(-1) != K) return none();
+    const int64_t M = x.numel() / K;
+    const IntArrayRef lead = x.sizes().slice(0, x.dim() - 1);
+    t.need(x.is_contiguous() && aligned(x) && w.stride(1) == 1 && w.stride(0) % 8 == 0 && w.stride(0) >= K && aligned(w) &&
+           M < (int64_t{1} << 31) && N < (int64_t{1} << 31));
+    Adapters l;
+    if (!t.ok || !l.take(t, a + 2, a[6], M, N, K, lead) || !t.here()) return none();
+    l.allocate(x, lead);
+    uint16_t* c[4];
+    for (int i = 0; i < l.n; ++i) c[i] = bf(l.parts[i]);
+    void* stream = t.stream();
+    if (failed("gdn_lora_shrink", l.shrink(x, nullptr, K, stream))) return nullptr;
+    const int status = gdn_gemm_bf16_lora(
+        bf(x), K, bf(w), w.stride(0), static_cast<int>(M), static_cast<int>(N), static_cast<int>(K), l.n, c, l.width, l.end,
+        nullptr, nullptr, nullptr, nullptr, 0, 0, 0, l.v(), l.ldv(), l.groups(), bf(*l.b), l.b->stride(0),
+        ptr<int32_t>(*l.ids), static_cast<int>(l.S), static_cast<int>(l.R), l.n, l.end, stream);
+    return failed("gdn_gemm_bf16_lora", status) ? nullptr : l.given(a[6]);
+  });
+}
+
+// (x, weight, weight_scale, lora_a, lora_b, lora_scale, ids, x_scale or None, widths or None) -> the same
+PyObject* linear_fp8_lora(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded(n, 9, [&]() -> PyObject* {
+    Taken t;
+    const bool ready = a[7] != Py_None;
+    const Tensor& x = t.tensor(a[0], ready ? kFp8 : kBf16, -1);
+    const Tensor& w = t.tensor(a[1], kFp8, 2);
+    if (!t.ok || x.dim() < 2 || x.numel() == 0) return none();
+    const int64_t N = w.size(0), K = w.size(1), G = K / kGroup;
+    if (N == 0 || K == 0 || K % kGroup || x.size(-1) != K) return none();
+    const int64_t M = x.numel() / K;
+    const IntArrayRef lead = x.sizes().slice(0, x.dim() - 1);
+    t.need(x.is_contiguous() && aligned(x) && w.stride(1) == 1 && w.stride(0) % 16 == 0 && w.stride(0) >= K && aligned(w) &&
+           M < (int64_t{1} << 31) && N < (int64_t{1} << 31));
+    const Tensor& ws = t.dense(a[2], kF32, {(N + kGroup - 1) / kGroup, G}, 4);
+    const Tensor* xs = nullptr;
+    if (t.ok && ready) {
+      xs = &t.tensor(a[7], kF32, 2);
+      if (t.ok) t.need(xs->size(0) == M && xs->size(1) == G);
+    }
+    Adapters l;
+    if (!t.ok || !l.take(t, a + 3, a[8], M, N, K, lead) || !t.here()) return none();
+    l.allocate(x, lead);
+    uint16_t* c[4];
+    for (int i = 0; i < l.n; ++i) c[i] = bf(l.parts[i]);
+    void* stream = t.stream();
+    if (failed("gdn_lora_shrink", l.shrink(x, xs, K, stream))) return nullptr;
+    Tensor x8, made;
+    if (!ready) {
+      x8 = at::empty({M, K}, x.options().dtype(kFp8));
+      made = at::empty_strided({M, G}, {1, M}, x.options().dtype(kF32));
+      if (failed("gdn_quantize_fp8", gdn_quantize_fp8(x.data_ptr(), 0, K, ptr<uint8_t>(x8), K, ptr<float>(made), 1, M, M,
+                                                       static_cast<int>(K), 1, stream)))
+        return nullptr;
+      xs = &made;
+    }
+    const int status = gdn_gemm_fp8_lora(
+        ptr<uint8_t>(ready ? x : x8), K, ptr<float>(*xs), xs->stride(0), xs->stride(1), ptr<uint8_t>(w), w.stride(0),
+        ptr<float>(ws), G, static_cast<int>(M), static_cast<int>(N), static_cast<int>(K), l.n, c, l.width, l.end, l.v(),
+        l.ldv(), l.groups(), bf(*l.b), l.b->stride(0), ptr<int32_t>(*l.ids), static_cast<int>(l.S), static_cast<int>(l.R),
+        l.n, l.end, stream);
+    return failed("gdn_gemm_fp8_lora", status) ? nullptr : l.given(a[8]);
+  });
+}
+
 // (check): check(name, status) raises
 PyObject* set_check(PyObject*, PyObject* check) {
   Py_INCREF(check);
@@ -528,6 +739,9 @@ PyMethodDef methods[] = {{"conv_tree", GDN_FAST(conv_tree)},
                          {"commit_tree", GDN_FAST(commit_tree)},
                          {"linear_fp8", GDN_FAST(linear_fp8)},
                          {"norm_fp8", GDN_FAST(norm_fp8)},
+                         {"add_norm", GDN_FAST(add_norm)},
+                         {"linear_lora", GDN_FAST(linear_lora)},
+                         {"linear_fp8_lora", GDN_FAST(linear_fp8_lora)},
                          {"set_check", set_check, METH_O, nullptr},
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "gdn_quick_calls", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

@@ -1670,6 +1670,10 @@ def linear_lora(x: torch.Tensor, weight: torch.Tensor, lora_a: torch.Tensor, lor
     result does not depend on the adapters of the others, whatever these hold.  Two
     launches; x, weight and one slot of the adapters below 2 GiB each.  Returns [..., N], or the list of
     parts, with gates (that, g, beta)."""
+    if gates is None:
+        y = _lib.quick().linear_lora(x, weight, lora_a, lora_b, lora_scale, ids, widths)
+        if y is not None:
+            return y
     parts = [weight.shape[0]] if widths is None else list(widths)
     if weight.dim() != 2:
         raise ValueError(f"weight must be [N, K], got {list(weight.shape)}")
@@ -1703,6 +1707,10 @@ def linear_fp8_lora(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.T
     follows as the last columns, a boundary of widths at N; the adapters' columns then go
     on over these (lora_b [slots, N + N2, R]).  gates: of the wide columns (gate_col
     counted from N).  Returns as linear_lora."""
+    if wide is None and gates is None:
+        y = _lib.quick().linear_fp8_lora(x, weight, weight_scale, lora_a, lora_b, lora_scale, ids, x_scale, widths)
+        if y is not None:
+            return y
     M, N, K = _check_fp8(x, weight, weight_scale, x_scale)
     total = N
     if wide is not None:
@@ -1792,6 +1800,10 @@ def add_rms_norm_fp8(x: torch.Tensor, residual: torch.Tensor | None, weight: tor
 
 
 def _add_rms_norm(x, residual, weight, eps, post_weight, gate, gate_sigmoid, scale, offset, residual_out, bf16, fp8):
+    if residual_out is None:
+        out = _lib.quick().add_norm(x, residual, weight, eps, post_weight, gate, gate_sigmoid, scale, offset, bf16, fp8)
+        if out is not None:
+            return out
     idx = _device_of(x, residual, weight, post_weight, gate, residual_out)
     _bf16(x, "x")
     if x.dim() < 1:

@@ -296,3 +296,85 @@ def test_adapter_rows(pkg, dev):
     cu = torch.tensor([0, 3, 3, 7, 8], device=dev)
     rows = pkg.adapter_rows(torch.tensor([2, 5, -1, 0], device=dev), cu, 8)
     assert rows.dtype == torch.int32 and rows.tolist() == [2, 2, 2, -1, -1, -1, -1, 0]
+
+
+class _NoQuick:
+    def __getattr__(self, name):
+        return lambda *a: None
+
+
+def _bits(out):
+    return [t.view(torch.uint8) if t.dtype == FP8 else t for t in (out if isinstance(out, (list, tuple)) else [out])]
+
+
+def test_quick_and_checked_calls_agree(pkg, dev, monkeypatch):
+    """The calls by way of C++ and those by way of the Python wrappers: the same bits, shapes and
+    strides; memory that comes back; what the kernels do not take as it is goes the other way."""
+    gen = torch.Generator().manual_seed(47)
+    M, N, K, R, S = 37, 96, 256, 16, 3
+    x, w = torch.randn(M, K, generator=gen).to(BF16).to(dev), (torch.randn(N, K, generator=gen) * 0.1).to(BF16).to(dev)
+    w8, ws = pkg.quantize_weight_fp8(w)
+    x8, xs = pkg.quantize_fp8(x)
+    ids = _ids(gen, M, S, "mixed").to(dev)
+    one = [t.to(dev) for t in _adapters(gen, S, [N], K, R)]
+    two = [t.to(dev) for t in _adapters(gen, S, [64, 32], K, R)]
+    res, nw = torch.randn(M, K, generator=gen).to(dev), torch.randn(K, generator=gen).to(BF16).to(dev)
+    gates = torch.randn(M, 1, generator=gen).to(dev), torch.randn(K, generator=gen).to(BF16).to(dev), x.clone()
+    calls = [lambda: pkg.linear_lora(x, w, *one, ids), lambda: pkg.linear_lora(x, w, *two, ids, widths=[64, 32]),
+             lambda: pkg.linear_lora(x.view(1, M, K), w, *two, ids.view(1, M), widths=[64, 32]),
+             lambda: pkg.linear_fp8_lora(x, w8, ws, *one, ids), lambda: pkg.linear_fp8_lora(x, w8, ws, *two, ids, widths=[64, 32]),
+             lambda: pkg.linear_fp8_lora(x8, w8, ws, *two, ids, x_scale=xs, widths=[64, 32]),
+             lambda: pkg.linear_fp8_lora(x8, w8, ws, *one, ids, x_scale=xs.contiguous()),
+             lambda: pkg.add_rms_norm(x, None, nw, 1e-6), lambda: pkg.add_rms_norm(x, res, nw.float(), 1e-6),
+             lambda: pkg.add_rms_norm(x, x, nw, 1e-6, post_weight=nw, gate=gates[0], gate_sigmoid=True, scale=0.5, offset=0.0),
+             *(lambda g=g: pkg.add_rms_norm(x, res, nw, 1e-6, gate=g) for g in gates),
+             lambda: pkg.add_rms_norm(x[0], x[1], nw, 1e-6),
+             *(lambda k=k: pkg.add_rms_norm_fp8(x, res, nw, 1e-6, post_weight=nw, keep=k) for k in (False, True))]
+    got = [call() for call in calls]
+    quick = pkg._lib.quick()
+    q = lambda t: t[:, :128]  # noqa: E731
+    taken = [quick.linear_lora(x, w, *one, ids, None), quick.linear_fp8_lora(x8, w8, ws, *one, ids, xs, None),
+             quick.add_norm(x, res, nw, 1e-6, nw, None, False, 1.0, 1.0, True, True)]
+    assert all(t is not None for t in taken)
+    left = [quick.linear_lora(q(x), q(w), *one, ids, None), quick.linear_lora(x, w, *one, ids.long(), None),
+            quick.linear_lora(x, w, *one, ids[1:], None), quick.linear_lora(x, w, *two, ids, None),
+            quick.linear_lora(x, w, *two, ids, [64, 31]), quick.linear_lora(x, w, *two, ids, [60, 36]),
+            quick.linear_lora(x, w, one[0], one[1], one[2].cpu(), ids, None), quick.linear_lora(x[:0], w, *one, ids[:0], None),
+            quick.linear_fp8_lora(x, w8, ws[:, :1], *one, ids, None, None), quick.linear_fp8_lora(x8, w8, ws, *one, ids, None, None),
+            quick.linear_fp8_lora(x8, w8, ws, *one, ids, xs[1:], None),
+            quick.add_norm(q(x), None, nw[:128], 1e-6, None, None, False, 1.0, 1.0, True, False),
+            quick.add_norm(x, res[1:], nw, 1e-6, None, None, False, 1.0, 1.0, True, False),
+            quick.add_norm(x, res, nw, 1e-6, nw.float(), None, False, 1.0, 1.0, True, False),
+            quick.add_norm(x, res, nw, 1e-6, None, ids.view(M, 1), False, 1.0, 1.0, True, False)]
+    assert all(t is None for t in left), [t is None for t in left]
+    before = torch.cuda.memory_allocated(dev)
+    for _ in range(3):
+        for call in calls:
+            call()
+    assert torch.cuda.memory_allocated(dev) == before
+    monkeypatch.setattr(pkg._lib, "quick", lambda: _NoQuick())
+    for i, (call, g) in enumerate(zip(calls, got)):
+        for a, b in zip(_bits(g), _bits(call()), strict=True):
+            assert a.dtype == b.dtype and a.shape == b.shape and a.stride() == b.stride() and torch.equal(a, b), i
+    assert calls[7]()[1] is x and got[7][1] is x
+
+
+def test_out_of_memory_is_torchs_error(pkg, dev):
+    """Outputs that do not fit raise torch's own error, and the next call is right."""
+    from test_gpu_no_memory import _memory_left
+    S, R, K = 1, 8, 128
+    x, w = torch.ones(16384, K, dtype=BF16, device=dev), torch.ones(8192, K, dtype=BF16, device=dev)
+    w8, ws = torch.ones(8192, K, device=dev).to(FP8), torch.ones(64, 1, device=dev)
+    a, b = torch.ones(S, R, K, dtype=BF16, device=dev), torch.ones(S, 8192, R, dtype=BF16, device=dev)
+    scale, ids = torch.ones(S, device=dev), torch.zeros(16384, dtype=torch.int32, device=dev)
+    rows = torch.zeros(8192, 8192, dtype=BF16, device=dev)
+    norm_w = torch.ones(8192, dtype=BF16, device=dev)
+    calls = (lambda: pkg.linear_lora(x, w, a, b, scale, ids),                     # 256 MiB
+             lambda: pkg.linear_fp8_lora(x, w8, ws, a, b, scale, ids),
+             lambda: pkg.add_rms_norm(rows, rows, norm_w, 1e-6),                  # twice 128 MiB
+             lambda: pkg.add_rms_norm_fp8(rows, rows, norm_w, 1e-6))
+    with _memory_left(dev, 32):
+        for call in calls:
+            with pytest.raises(torch.OutOfMemoryError):
+                call()
+    assert bool((calls[0]() == K + K * R).all())

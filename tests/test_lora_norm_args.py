@@ -168,3 +168,17 @@ def test_c_entries_refuse(pkg):
                dict(gate=P, g_col=1, g_row=255), dict(gate=byte), dict(y8=P, ys=P, H=200), dict(y8=P, ys=P, x=odd),
                dict(y8=P, ys=P, sx=260), dict(y8=odd, ys=P), dict(y8=P, ys=P, gate=odd, g_col=1)):
         assert norm(**kw) == bad, kw
+
+
+def test_quick_calls_leave_the_rest_to_the_wrappers(pkg):
+    """What is not a tensor on the device as the kernel takes it is not taken, and said to be None."""
+    quick = pkg._lib.quick()
+    t, f = torch.zeros(2, 128, dtype=BF16), torch.zeros(128)
+    for name, n in (("add_norm", 11), ("linear_lora", 7), ("linear_fp8_lora", 9)):
+        call = getattr(quick, name)
+        for arg in (t, f, None, 3, "x", (), torch.nn.Parameter(f), [t], [1 << 70], 1.5, True):
+            assert call(*[arg] * n) is None, (name, arg)
+        for wrong in (0, n - 1, n + 1):
+            with pytest.raises(TypeError):
+                call(*[t] * wrong)
+    assert quick.add_norm(t, t, f, 1e-6, None, None, False, 1.0, 1.0, True, False) is None   # (not on the device)
