@@ -90,10 +90,10 @@ __device__ __forceinline__ f32x16_t zero16() {
 // Epilogue of a BM x BN tile, straight from the accumulators of wave
 // (wm, wn).  `scratch`: (BM / 2) x 32 bf16 per wave of LDS that nothing reads
 // any more (the gate outputs go through it).
-template <int BM, int BN>
+template <int BM, int BN, class Order = SameRow>
 __device__ __forceinline__ void gemm_store(const f32x16_t (&acc)[BM / 64][BN / 64], const GemmOut& out, int M,
                                            int N, int m0, int n0, int wave, int lane, const GemmGates& gt,
-                                           uint8_t* scratch) {
+                                           uint8_t* scratch, const Order& order = {}) {
   constexpr int MI = BM / 64, NJ = BN / 64;
   const int wm = wave >> 1, wn = wave & 1;
   const int li = lane & 31, lg = lane >> 5;
@@ -105,8 +105,9 @@ __device__ __forceinline__ void gemm_store(const f32x16_t (&acc)[BM / 64][BN / 6
   // 16-byte store per pair, two lanes filling 32 bytes of a row.
 #pragma unroll
   for (int i = 0; i < MI; ++i) {
-    const int m = m0 + (BM / 2) * wm + 32 * i + li;
-    const bool row_ok = m < M;  // (no early exit: the gate loop below spans every lane)
+    const int at = m0 + (BM / 2) * wm + 32 * i + li;
+    const bool row_ok = at < M;  // (no early exit: the gate loop below spans every lane)
+    const int m = row_ok ? order(at) : 0;
 #pragma unroll
     for (int j = 0; j < NJ; ++j) {
       const int cb = n0 + (BN / 2) * wn + 32 * j;  // wave-uniform
@@ -120,7 +121,7 @@ __device__ __forceinline__ void gemm_store(const f32x16_t (&acc)[BM / 64][BN / 6
       int cend = pick(out.end[0], out.end[1], out.end[2], out.end[3]);
       bool vec = pick(out.vec[0], out.vec[1], out.vec[2], out.vec[3]) != 0;
       uint16_t* crow = pick(out.c[0], out.c[1], out.c[2], out.c[3]) +
-                       static_cast<int64_t>(row_ok ? m : 0) * pick(out.ld[0], out.ld[1], out.ld[2], out.ld[3]) - cbeg;
+                       static_cast<int64_t>(m) * pick(out.ld[0], out.ld[1], out.ld[2], out.ld[3]) - cbeg;
 #pragma unroll
       for (int p = 0; p < 2; ++p) {
         if (p == 1 && cend == cb + 16 && cend < N) {
@@ -131,7 +132,7 @@ __device__ __forceinline__ void gemm_store(const f32x16_t (&acc)[BM / 64][BN / 6
           cend = pick(out.end[0], out.end[1], out.end[2], out.end[3]);
           vec = pick(out.vec[0], out.vec[1], out.vec[2], out.vec[3]) != 0;
           crow = pick(out.c[0], out.c[1], out.c[2], out.c[3]) +
-                 static_cast<int64_t>(row_ok ? m : 0) * pick(out.ld[0], out.ld[1], out.ld[2], out.ld[3]) - cbeg;
+                 static_cast<int64_t>(m) * pick(out.ld[0], out.ld[1], out.ld[2], out.ld[3]) - cbeg;
         }
         const int q = 2 * p;
         const auto lo = __builtin_amdgcn_permlane32_swap(gdn::f2bf2(acc[i][j][4 * q], acc[i][j][4 * q + 1]),
@@ -170,7 +171,8 @@ __device__ __forceinline__ void gemm_store(const f32x16_t (&acc)[BM / 64][BN / 6
 #pragma unroll 1
         for (int e = lane; e < 32 * 32; e += 64) {
           const int r = e >> 5, c = e & 31;
-          const int mm = m - li + r, n = cb + c, col = n - gt.gate_col;
+          const int n = cb + c, col = n - gt.gate_col;
+          const int mm = at - li + r < M ? order(at - li + r) : M;
           if (mm >= M || n >= N || col < 0 || col >= 2 * gt.Hv) continue;
           const float v = gdn::bf2f(gs[32 * (32 * i + r) + c]);
           if (col < gt.Hv) {
@@ -852,7 +854,7 @@ __global__ __launch_bounds__(kGemmThreads) void gemm_tn_ring_kernel(const uint16
   for (int i = 0; i < kPer; ++i) {
     if (i < BM / 8) {
       const int gcol = 8 * ((lane & 7) ^ (((i & 1) << 2) | (lane >> 4)));
-      goff[i] = static_cast<int>((min(m0 + 8 * i + (lane >> 3), M - 1) * lda + gcol) * 2);
+      goff[i] = static_cast<int>((lora_row<kLora>(lo, m0 + 8 * i + (lane >> 3), M) * lda + gcol) * 2);
     } else {
       const int b = i - BM / 8;
       const int gcol = 8 * ((lane & 7) ^ (((b & 3) << 1) | ((lane >> 4) & 1)));
@@ -931,7 +933,7 @@ __global__ __launch_bounds__(kGemmThreads) void gemm_tn_ring_kernel(const uint16
       c0 += red[((w * MT + i) * 2) * 64 + lane];
       c1 += red[((w * MT + i) * 2 + 1) * 64 + lane];
     }
-    gemm_store16(c0, c1, out, M, N, m0 + 16 * i, n0, lane, gt, gscr[wave]);
+    gemm_store16(c0, c1, out, M, N, m0 + 16 * i, n0, lane, gt, gscr[wave], LoraOrder<kLora, LoraArg<kLora>>{lo, M});
   }
 }
 
@@ -957,7 +959,7 @@ __device__ __forceinline__ void lora_pass32(const Lora& lo, int N, int mine, uin
         const int n = col0 + 32 * j + li;
         boff[j] = (n * lo.rank * 2 + 16 * q) | off | (n >= beg && n < end ? 0 : kNoOffset);
       }
-      LoraIds it{all, 0, 1, 0};
+      LoraIds it{all, 0, 1};
       gdn::s16x8_t fb[DEPTH][NJ];
       int sid[DEPTH];
       auto fetch = [&](int d) {
@@ -997,10 +999,10 @@ template <int NJ, int DEPTH>
 __device__ __forceinline__ void lora_init32(const Lora& lo, int M, int N, int row0, int col0, int lane,
                                             f32x16_t (&acc)[NJ]) {
   const int r = row0 + (lane & 31);
-  const int mine = lora_id(lo, r, M);
+  const int mine = lo.order ? r < M ? lo.order[M + r] : -1 : lora_id(lo, r, M);
   const uint64_t all = __ballot(mine >= 0 && lane < 32);
   if (!all) return;
-  const int voff = static_cast<int>(min(r, M - 1) * lo.ldv * 2);
+  const int voff = static_cast<int>(lora_row<true>(lo, r, M) * lo.ldv * 2);
   lora_pass32<NJ, DEPTH, false>(lo, N, mine, all, voff, col0, lane, acc);
   float bad = 0.0f;
 #pragma unroll
@@ -1072,7 +1074,7 @@ __global__ __launch_bounds__(kGemmThreads, 2) void gemm_tn_deep_kernel(const uin
     const int b = wave + 4 * i;
     const int gcol = 8 * ((lane & 7) ^ (((b & 1) << 2) | (lane >> 4)));
     if (i < kAPer) {
-      goff[i] = static_cast<int>((min(m0 + 8 * b + (lane >> 3), M - 1) * lda + gcol) * 2);
+      goff[i] = static_cast<int>((lora_row<kLora>(lo, m0 + 8 * b + (lane >> 3), M) * lda + gcol) * 2);
     } else {
       goff[i] = static_cast<int>((min(n0 + 8 * (b - BM / 8) + (lane >> 3), N - 1) * ldb + gcol) * 2);
     }
@@ -1145,7 +1147,7 @@ __global__ __launch_bounds__(kGemmThreads, 2) void gemm_tn_deep_kernel(const uin
   // the repeated loads land before a stage is reused as the gates' scratch
   __builtin_amdgcn_s_waitcnt(0);
   __syncthreads();
-  gemm_store<BM, BN>(acc, out, M, N, m0, n0, wave, lane, gt, st0);
+  gemm_store<BM, BN>(acc, out, M, N, m0, n0, wave, lane, gt, st0, LoraOrder<kLora, LoraArg<kLora>>{lo, M});
 }
 
 }  // namespace

@@ -675,9 +675,9 @@ __device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {
 
 // The waves' partial sums, added in wave order, into C.  red: [wave][row tile][column
 // tile][lane], free of loads and readers.
-template <int MT, int NT, int NW>
+template <int MT, int NT, int NW, class Order = SameRow>
 __device__ __forceinline__ void ring_store(const gdn::f32x4_t (&acc)[MT][NT][2], gdn::f32x4_t* red, const GemmOut& out,
-                                           int M, int N, int m0, int n0) {
+                                           int M, int N, int m0, int n0, const Order& order = {}) {
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
 #pragma unroll
@@ -694,7 +694,8 @@ __device__ __forceinline__ void ring_store(const gdn::f32x4_t (&acc)[MT][NT][2],
       c0 += red[((w * MT * NT + ij) * 2) * 64 + lane];
       c1 += red[((w * MT * NT + ij) * 2 + 1) * 64 + lane];
     }
-    gemm_store16<true>(c0, c1, out, M, N, m0 + 16 * (ij / NT), n0 + 32 * (ij % NT), lane, GemmGates{}, nullptr);
+    gemm_store16<true>(c0, c1, out, M, N, m0 + 16 * (ij / NT), n0 + 32 * (ij % NT), lane, GemmGates{}, nullptr,
+                       order);
   }
 }
 
@@ -753,7 +754,7 @@ __global__ __launch_bounds__(64 * NW) void gemm_fp8_ring_kernel(const void* __re
       goff[i] = static_cast<int>(min(m0 + r, M - 1) * lda * 2 + 16 * ((lane & 15) ^ (r & 15)));
     } else {
       const int r = 8 * i + (lane >> 3);
-      goff[i] = static_cast<int>(min(m0 + r, M - 1) * lda + 16 * ((lane & 7) ^ ((r >> 1) & 7)));
+      goff[i] = static_cast<int>(lora_row<kLora>(lo, m0 + r, M) * lda + 16 * ((lane & 7) ^ ((r >> 1) & 7)));
     }
   }
 #pragma unroll
@@ -762,7 +763,7 @@ __global__ __launch_bounds__(64 * NW) void gemm_fp8_ring_kernel(const void* __re
     goff[kAPer + i] = static_cast<int>(min(n0 + r, N - 1) * ldb +
                                        16 * ((lane & 7) ^ (((r >> 1) & 1) | (((r >> 3) & 3) << 1))));
   }
-  const int va = kQuant ? 0 : static_cast<int>(min(m0 + lane % BM, M - 1) * sc.a_row * 4);
+  const int va = kQuant ? 0 : static_cast<int>(lora_row<kLora>(lo, m0 + lane % BM, M) * sc.a_row * 4);
   const int vb = static_cast<int>(n0 / 128 * sc.b_row * 4);
   const int nk = K / 128;
   auto issue = [&](uint8_t* st, int step) {
@@ -890,7 +891,8 @@ __global__ __launch_bounds__(64 * NW) void gemm_fp8_ring_kernel(const void* __re
   // the repeated loads past the last step land before the stages are reused
   __builtin_amdgcn_s_waitcnt(0);
   __syncthreads();
-  ring_store<MT, NT, NW>(acc, reinterpret_cast<gdn::f32x4_t*>(st0), out, M, N, m0, n0);
+  ring_store<MT, NT, NW>(acc, reinterpret_cast<gdn::f32x4_t*>(st0), out, M, N, m0, n0,
+                         LoraOrder<kLora, LoraArg<kLora>>{lo, M});
 }
 
 // v of the lane D places on, around each 16 lanes
@@ -1110,11 +1112,11 @@ __global__ __launch_bounds__(kFp8Threads * H, 2) void gemm_fp8_deep_kernel(const
 #pragma unroll
   for (int i = 0; i < kAPer + kBPer; ++i) {
     const int r = 8 * wave + 32 * (i < kAPer ? i : i - kAPer) + (lane >> 3);
-    goff[i] = i < kAPer ? static_cast<int>(min(m0 + r, M - 1) * lda + 16 * ((lane & 7) ^ ((r >> 1) & 7)))
+    goff[i] = i < kAPer ? static_cast<int>(lora_row<kLora>(lo, m0 + r, M) * lda + 16 * ((lane & 7) ^ ((r >> 1) & 7)))
                         : static_cast<int>(min(n0 + r, N - 1) * ldb +
                                            16 * ((lane & 7) ^ (((r >> 1) & 1) | (((r >> 3) & 3) << 1))));
   }
-  const int vs = wave == 0 ? static_cast<int>(min(m0 + lane, M - 1) * sc.a_row * 4)
+  const int vs = wave == 0 ? static_cast<int>(lora_row<kLora>(lo, m0 + lane, M) * sc.a_row * 4)
                            : static_cast<int>(n0 / 128 * sc.b_row * 4);
   const int s_step = wave == 0 ? static_cast<int>(sc.a_grp) * 4 : 4;
   const int nk = K / 128, trips = (nk + H - 1) / H, first = half * trips;
@@ -1236,7 +1238,7 @@ __global__ __launch_bounds__(kFp8Threads * H, 2) void gemm_fp8_deep_kernel(const
 #pragma unroll
     for (int j = 0; j < NJ; ++j)
       gemm_store16<true>(acc[i][j][0], acc[i][j][1], out, M, N, m0 + 32 * wm + 16 * i, n0 + 32 * (NJ * wn + j), lane,
-                   GemmGates{}, nullptr);
+                         GemmGates{}, nullptr, LoraOrder<kLora, LoraArg<kLora>>{lo, M});
   __builtin_amdgcn_s_waitcnt(0);  // the repeated loads past the last step
 }
 

@@ -59,10 +59,14 @@ __device__ __forceinline__ void dma16(__amdgpu_buffer_rsrc_t rsrc, uint8_t* lds,
 // c1: one 16-byte piece, four lanes filling 64 contiguous bytes of a row.  kAnyRow: the piece
 // goes out whole in rows without 16-byte alignment too (the 8-bit GEMM's kernels: 8192 x
 // 4001 x 256 36 us, value by value 77; 4002 columns 26).
-template <bool kAnyRow = false>
+// order(r): the row of the output that the tile's row r is.
+struct SameRow {
+  __device__ __forceinline__ int operator()(int r) const { return r; }
+};
+template <bool kAnyRow = false, class Order = SameRow>
 __device__ __forceinline__ void gemm_store16(const gdn::f32x4_t& c0, const gdn::f32x4_t& c1, const GemmOut& out,
                                              int M, int N, int row0, int cb, int lane, const GemmGates& gt,
-                                             uint16_t* gs) {
+                                             uint16_t* gs, const Order& order = {}) {
   const int lr = lane & 15, lg = lane >> 4;
   if (cb >= N || row0 >= M) return;  // wave-uniform
   auto pick = [](int t, auto a0, auto a1, auto a2, auto a3) { return t == 0 ? a0 : t == 1 ? a1 : t == 2 ? a2 : a3; };
@@ -71,7 +75,8 @@ __device__ __forceinline__ void gemm_store16(const gdn::f32x4_t& c0, const gdn::
   // the part of the block's first 16 columns (wave-uniform)
   const int s = cb < out.end[0] ? 0 : cb < out.end[1] ? 1 : cb < out.end[2] ? 2 : 3;
   const int cend = pick(s, out.end[0], out.end[1], out.end[2], out.end[3]);
-  const int m = row0 + lr, n = cb + 8 * lg;
+  const int n = cb + 8 * lg;
+  const int m = row0 + lr < M ? order(row0 + lr) : M;
   if (pick(s, out.vec[0], out.vec[1], out.vec[2], out.vec[3]) && cb + 32 <= cend) {
     // the whole block in one part with 16-byte rows
     uint16_t* c = pick(s, out.c[0], out.c[1], out.c[2], out.c[3]) - pick(s, 0, out.end[0], out.end[1], out.end[2]);
@@ -106,7 +111,8 @@ __device__ __forceinline__ void gemm_store16(const gdn::f32x4_t& c0, const gdn::
 #pragma unroll 1
     for (int e = lane; e < 16 * 32; e += 64) {
       const int r = e >> 5, c = e & 31;
-      const int mm = row0 + r, nn = cb + c, col = nn - gt.gate_col;
+      const int nn = cb + c, col = nn - gt.gate_col;
+      const int mm = row0 + r < M ? order(row0 + r) : M;
       if (mm >= M || nn >= N || col < 0 || col >= 2 * gt.Hv) continue;
       const float v = gdn::bf2f(gs[32 * r + c]);
       if (col < gt.Hv) {

@@ -8,12 +8,17 @@
 // would cost the result as much again as its own rounding where an adapter's share is as large
 // as the projection's.
 //
-// A workgroup has 16 MT rows and 16 NT of the columns j.  It goes through the adapters of its
-// rows, each once: all rows times the adapter's A, K-steps dealt to the waves, each with a ring of
-// NS stages of its own in LDS that loads fill directly (as in the GEMM's ring kernel), the
-// waves' sums added in wave order, and the rows that have the adapter stored.  With gridDim.y > 1
-// workgroups share a tile's adapters: few rows, most of them with adapters of their own, are
-// bound by the reading of A and want it spread over the chip; a prompt's tile has one.
+// Prompts (lora_shrink_kernel): a workgroup has 16 MT rows and 16 NT of the columns j.  It goes
+// through the adapters of its rows, each once: all rows times the adapter's A, K-steps dealt to
+// the waves, each with a ring of NS stages of its own in LDS that loads fill directly (as in the
+// GEMM's ring kernel), the waves' sums added in wave order, and the rows that have the adapter
+// stored.
+//
+// Few rows (lora_few_kernel), most of them with adapters of their own, are bound by the reading
+// of A: 16 rows and 16 columns to a workgroup, K dealt to its waves, all of their
+// loads on their way at once.  Up to kLoraSort rows are taken in the order of their
+// adapters, so that an adapter's A is read once for each 16 of its rows and not once for each 16
+// rows that it is among; the GEMM takes its rows in the same order.
 //
 // x comes in bf16 (steps of 64 values) or in e4m3 with a scale for each row and 128 columns
 // (steps of 128): e4m3 values are bf16 ones, so a group's sum is the matrix cores' and the
@@ -38,7 +43,8 @@ struct Shrink {
   int slots, cols, rank, M, K;
   uint16_t* v;
   int64_t ldv;
-  int* groups;      // [ceil(M / 16)]: the adapter of 16 rows, -1 none, -2 not one for all
+  int* groups;  // [ceil(M / 16)]: the adapter of 16 rows, -1 none, -2 not one for all; up to kLoraSort rows: [M] the
+                // rows in the order of their adapters, [M] these
 };
 
 // 8 e4m3 values as bf16
@@ -53,6 +59,196 @@ __device__ __forceinline__ gdn::s16x8_t e4m3_to_bf16(const i32x2_t& w) {
   }
   typedef uint32_t u4 __attribute__((ext_vector_type(4)));
   return __builtin_bit_cast(gdn::s16x8_t, u4{d[0], d[1], d[2], d[3]});
+}
+
+// Columns c .. c + 3 of row m (a slice's ranks are a multiple of 8).
+__device__ __forceinline__ void store_v(const Shrink& p, int m, int c, const gdn::f32x4_t& sum, float scale) {
+  if (c >= p.cols) return;
+  float hi[4], lo[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const float val = sum[e] * scale;
+    hi[e] = gdn::bf2f(gdn::f2bf(val));
+    // (what bf16 does not hold is infinite in the one part and has none in the other)
+    lo[e] = fabsf(hi[e]) < __builtin_inff() ? val - hi[e] : 0.0f;
+  }
+  const int slice = c / p.rank;
+  uint16_t* at = p.v + static_cast<int64_t>(m) * p.ldv + slice * p.rank + c;
+  *reinterpret_cast<uint2*>(at) = make_uint2(gdn::f2bf2(hi[0], hi[1]), gdn::f2bf2(hi[2], hi[3]));
+  *reinterpret_cast<uint2*>(at + p.rank) = make_uint2(gdn::f2bf2(lo[0], lo[1]), gdn::f2bf2(lo[2], lo[3]));
+}
+
+// A wave's share of 16 rows times 16 columns of one adapter: the K-steps wave, wave + NW, ...  Of C
+// steps the loads are on their way at once, 8 lanes to a row's 128 bytes (straight in the
+// matrix cores' layout, a row to a lane, they took 4 times as long); each step then goes through the wave's own rows of
+// LDS.  A lane asks for rows (-1: none) and columns lane / 8 and 8 + lane / 8; steps past the end load zeros.
+template <int NW, bool kFp8>
+__device__ __forceinline__ gdn::f32x4_t few_product(const Shrink& p, __amdgpu_buffer_rsrc_t rx, __amdgpu_buffer_rsrc_t ra,
+                                                    __amdgpu_buffer_rsrc_t rs, const int (&row)[2], int own_row, int c0, int wave,
+                                                    int lane, uint8_t* lds) {
+  constexpr int C = kFp8 ? 2 : 4, kStep = kFp8 ? 128 : 64, kHalves = kFp8 ? 2 : 1;
+  const int nk = p.K / kStep, lr = lane & 15, lg = lane >> 4;
+  int xoff[2], aoff[2], at[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int r = 8 * i + (lane >> 3);
+    xoff[i] = row[i] < 0 ? kNoOffset : static_cast<int>(row[i] * p.ldx * (kFp8 ? 1 : 2)) + 16 * (lane & 7);
+    aoff[i] = min(c0 + r, p.cols - 1) * p.K * 2 + 16 * (lane & 7);
+    at[i] = sw_off(r, lane & 7);
+  }
+  const int soff = kFp8 ? static_cast<int>(own_row * p.xs_row * 4) : 0;
+  gdn::f32x4_t acc = {0.f, 0.f, 0.f, 0.f};
+  for (int k0 = wave; k0 < nk; k0 += C * NW) {
+    gdn::s16x8_t x[C][2], a[C][2 * kHalves];
+    float f[C];
+#pragma unroll
+    for (int i = 0; i < C; ++i) {
+      const int k = k0 + i * NW, off = k < nk ? 0 : kNoOffset;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) x[i][h] = lora_load(rx, (xoff[h] + 128 * k) | off | (xoff[h] & kNoOffset));
+#pragma unroll
+      for (int h = 0; h < 2 * kHalves; ++h) a[i][h] = lora_load(ra, (aoff[h & 1] + 128 * (kHalves * k + (h >> 1))) | off);
+      if constexpr (kFp8)
+        f[i] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(
+                                             rs, (soff + static_cast<int>(p.xs_grp) * 4 * k) | off, 0, 0));
+    }
+#pragma unroll
+    for (int i = 0; i < C; ++i) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) *reinterpret_cast<gdn::s16x8_t*>(lds + at[h]) = x[i][h];
+#pragma unroll
+      for (int h = 0; h < 2 * kHalves; ++h)
+        *reinterpret_cast<gdn::s16x8_t*>(lds + 2048 * (1 + (h >> 1)) + at[h & 1]) = a[i][h];
+      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront", "local");
+      __builtin_amdgcn_wave_barrier();
+      __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront", "local");
+      gdn::f32x4_t sum = kFp8 ? gdn::f32x4_t{0.f, 0.f, 0.f, 0.f} : acc;
+#pragma unroll
+      for (int ks = 0; ks < 2 * kHalves; ++ks) {
+        const gdn::s16x8_t fa = *reinterpret_cast<const gdn::s16x8_t*>(lds + 2048 * (1 + (ks >> 1)) + sw_off(lr, 4 * (ks & 1) + lg));
+        gdn::s16x8_t fx;
+        if constexpr (kFp8)
+          fx = e4m3_to_bf16(*reinterpret_cast<const i32x2_t*>(lds + sw_off(lr, 2 * ks + (lg >> 1)) + 8 * (lg & 1)));
+        else
+          fx = *reinterpret_cast<const gdn::s16x8_t*>(lds + sw_off(lr, 4 * ks + lg));
+        sum = gdn::mfma16x16x32(fa, fx, sum);
+      }
+      if constexpr (kFp8) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[e] = fmaf(sum[e], f[i], acc[e]);
+      } else {
+        acc = sum;
+      }
+      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront", "local");
+      __builtin_amdgcn_wave_barrier();
+      __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront", "local");
+    }
+  }
+  return acc;
+}
+
+// kSort: 17 to kLoraSort rows in the order of their adapters, blockIdx.y and on every gridDim.y-th
+// of the runs of one adapter in 16 places of that order; the order is written for the GEMM.  Every
+// workgroup finds it for itself: a row's place is the number of rows before it, counted by all
+// threads (256 rows: under 1 us, and none of it waits for memory).  Else: blockIdx.x has 16 rows and, of
+// their adapters, blockIdx.y and on every gridDim.y-th.
+template <int NW, bool kFp8, bool kSort>
+__global__ __launch_bounds__(64 * NW) void lora_few_kernel(Shrink p) {
+  constexpr int kStepBytes = kFp8 ? 6144 : 4096;
+  __shared__ __align__(16) int key[kLoraSort];
+  __shared__ int place[kLoraSort], s_row[kLoraSort], s_id[kLoraSort], s_item[kLoraSort], s_count[4];
+  __shared__ __align__(16) uint8_t steps[NW * kStepBytes];
+  gdn::f32x4_t* red = reinterpret_cast<gdn::f32x4_t*>(steps);
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int lr = lane & 15, lg = lane >> 4;
+  const int tiles_n = (p.cols + 15) / 16;
+  const int c0 = 16 * static_cast<int>(blockIdx.x % tiles_n), m0 = 16 * static_cast<int>(blockIdx.x / tiles_n);
+  const __amdgpu_buffer_rsrc_t rx = rsrc_of(p.x), rs = rsrc_of(p.xs);
+  // rows: the ones that the lane loads
+  auto run = [&](int s, const int (&rows)[2], int row, bool own) {
+    const gdn::f32x4_t acc = few_product<NW, kFp8>(p, rx, rsrc_of(p.a + s * p.a_slot), rs, rows, row, c0, wave, lane,
+                                                   steps + wave * kStepBytes);
+    const float scale = p.scale[s];
+    __syncthreads();
+    red[64 * wave + lane] = acc;
+    __syncthreads();
+    if (wave == 0) {
+      gdn::f32x4_t sum = acc;
+#pragma unroll
+      for (int w = 1; w < NW; ++w) sum += red[64 * w + lane];
+      if (own) store_v(p, row, c0 + 4 * lg, sum, scale);
+    }
+    __syncthreads();
+  };
+  if constexpr (kSort) {
+    const int P = p.M <= 64 ? 64 : p.M <= 128 ? 128 : 256, span = P * P / (64 * NW);  // keys to a thread
+    if (tid < P) {
+      const int s = p.ids[min(tid, p.M - 1)];
+      key[tid] = tid >= p.M ? 0x7fffffff : static_cast<unsigned>(s) < static_cast<unsigned>(p.slots) ? s : -1;
+      place[tid] = 0;
+    }
+    __syncthreads();
+    const int m = tid & (P - 1), mine = key[m];
+    if (m < p.M) {
+      const int from = __builtin_amdgcn_readfirstlane(tid / P * span);
+      int count = 0;
+      for (int j = from; j < from + span; j += 4) {
+        const int4 k = *reinterpret_cast<const int4*>(key + j);
+        count += k.x < mine + (j < m) ? 1 : 0;
+        count += k.y < mine + (j + 1 < m) ? 1 : 0;
+        count += k.z < mine + (j + 2 < m) ? 1 : 0;
+        count += k.w < mine + (j + 3 < m) ? 1 : 0;
+      }
+      atomicAdd(&place[m], count);
+    }
+    const uint64_t differ = __ballot(m < p.M && mine != key[m & ~15]);
+    __syncthreads();
+    if (tid < p.M) {
+      s_row[place[tid]] = tid;
+      s_id[place[tid]] = mine;
+    }
+    __syncthreads();
+    const bool first = tid < p.M && s_id[tid] >= 0 && (tid % 16 == 0 || s_id[tid] != s_id[tid - 1]);
+    const uint64_t firsts = __ballot(first);
+    if (wave < 4 && lane == 0) s_count[wave] = __builtin_popcountll(firsts);
+    if (blockIdx.x == 0 && blockIdx.y == 0 && tid < p.M) {
+      if (lr == 0) p.groups[tid / 16] = (differ >> lane) & 0xffff ? -2 : mine;
+      int* order = p.groups + (p.M + 15) / 16;
+      order[tid] = s_row[tid];
+      order[p.M + tid] = s_id[tid];
+    }
+    __syncthreads();
+    int before = 0, items = 0;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      before += w < wave ? s_count[w] : 0;
+      items += s_count[w];
+    }
+    if (first) s_item[before + __builtin_popcountll(firsts & ((1ull << lane) - 1))] = tid;
+    __syncthreads();
+    for (int it = blockIdx.y; it < items; it += gridDim.y) {
+      const int at = s_item[it], to = min(at | 15, p.M - 1);
+      const int s = __builtin_amdgcn_readfirstlane(s_id[at]);
+      auto has = [&](int i) { return at + i <= to && s_id[min(at + i, to)] == s; };
+      auto row = [&](int i) { return has(i) ? s_row[at + i] : -1; };
+      const int rows[2] = {row(lane >> 3), row(8 + (lane >> 3))};
+      run(s, rows, max(row(lr), 0), has(lr));
+    }
+  } else {
+    const int r = m0 + lr, s0 = p.ids[min(r, p.M - 1)];
+    const int id = r < p.M && static_cast<unsigned>(s0) < static_cast<unsigned>(p.slots) ? s0 : -1;
+    const int first = __builtin_amdgcn_readfirstlane(id);
+    const bool alike = !__any(r < p.M && id != first);
+    if (c0 == 0 && blockIdx.y == 0 && tid == 0) p.groups[m0 / 16] = alike ? first : -2;
+    LoraIds it{__ballot(id >= 0 && lane < 16), static_cast<int>(blockIdx.y), static_cast<int>(gridDim.y)};
+    uint64_t rows;
+    for (int s = it.next(id, rows); s >= 0; s = it.next(id, rows)) {
+      auto row = [&](int i) { return (rows >> i) & 1 ? m0 + i : -1; };
+      const int mine[2] = {row(lane >> 3), row(8 + (lane >> 3))};
+      run(s, mine, min(r, p.M - 1), id == s);
+    }
+  }
 }
 
 template <int MT, int NT, int NW, int NS, bool kFp8>
@@ -71,8 +267,11 @@ __global__ __launch_bounds__(64 * NW) void lora_shrink_kernel(Shrink p) {
   __shared__ __align__(16) uint8_t st0[NW * kStage];
   __shared__ __align__(16) uint8_t st1[NW * kStage];
   __shared__ __align__(16) uint8_t st2[NS > 2 ? NW * kStage : 16];
+  // (the column tiles of a row tile one after the other on one XCD: x comes from its L2)
   const int tiles_n = (p.cols + BN - 1) / BN;
-  const int m0 = BM * static_cast<int>(blockIdx.x / tiles_n), c0 = BN * static_cast<int>(blockIdx.x % tiles_n);
+  const int64_t tile = gdn::xcd_remap(blockIdx.x, static_cast<int64_t>((p.M + BM - 1) / BM) * tiles_n);
+  if (tile < 0) return;
+  const int m0 = BM * static_cast<int>(tile / tiles_n), c0 = BN * static_cast<int>(tile % tiles_n);
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int lr = lane & 15, lg = lane >> 4;
@@ -84,12 +283,12 @@ __global__ __launch_bounds__(64 * NW) void lora_shrink_kernel(Shrink p) {
     id[i] = r < p.M && static_cast<unsigned>(s) < static_cast<unsigned>(p.slots) ? s : -1;
     const int first = __builtin_amdgcn_readfirstlane(id[i]);
     const bool alike = !__any(r < p.M && id[i] != first);
-    if (c0 == 0 && blockIdx.y == 0 && threadIdx.x == 0 && r < p.M) p.groups[m0 / 16 + i] = alike ? first : -2;
+    if (c0 == 0 && threadIdx.x == 0 && r < p.M) p.groups[m0 / 16 + i] = alike ? first : -2;
   }
   int mine = BM > lane ? id[0] : -1;  // row m0 + lane's
 #pragma unroll
   for (int i = 1; i < MT; ++i) mine = lg == i ? id[i] : mine;
-  LoraIds it{__ballot(mine >= 0), static_cast<int>(blockIdx.y), static_cast<int>(gridDim.y), 0};
+  LoraIds it{__ballot(mine >= 0), 0, 1};
   uint64_t rows;
   int s = it.next(mine, rows);
   if (s < 0) return;  // (the workgroup)
@@ -202,21 +401,7 @@ __global__ __launch_bounds__(64 * NW) void lora_shrink_kernel(Shrink p) {
       gdn::f32x4_t sum = red[ij * 64 + lane];
 #pragma unroll
       for (int w = 1; w < NW; ++w) sum += red[(w * MT * NT + ij) * 64 + lane];
-      // columns c .. c + 3 of row m0 + 16 i + lr (a slice's ranks are a multiple of 8)
-      const int c = c0 + 16 * j + 4 * lg;
-      if (id[i] != s || c >= p.cols) continue;
-      float hi[4], lo[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float val = sum[e] * scale;
-        hi[e] = gdn::bf2f(gdn::f2bf(val));
-        // (what bf16 does not hold is infinite in the one part and has none in the other)
-        lo[e] = fabsf(hi[e]) < __builtin_inff() ? val - hi[e] : 0.0f;
-      }
-      const int slice = c / p.rank;
-      uint16_t* at = p.v + static_cast<int64_t>(m0 + 16 * i + lr) * p.ldv + slice * p.rank + c;
-      *reinterpret_cast<uint2*>(at) = make_uint2(gdn::f2bf2(hi[0], hi[1]), gdn::f2bf2(hi[2], hi[3]));
-      *reinterpret_cast<uint2*>(at + p.rank) = make_uint2(gdn::f2bf2(lo[0], lo[1]), gdn::f2bf2(lo[2], lo[3]));
+      if (id[i] == s) store_v(p, m0 + 16 * i + lr, c0 + 16 * j + 4 * lg, sum, scale);
     }
     s = it.next(mine, rows);
     if (s >= 0) __syncthreads();  // the sums have been read
@@ -228,18 +413,29 @@ int launch(const Shrink& p, hipStream_t st) {
   auto tiles = [](int n, int of) { return (n + of - 1) / of; };
   // one wave's rows: prompts fill the chip with 64-row tiles
   if (p.M > 2048) {
-    const int nt = tiles(p.cols, p.cols > 32 ? 64 : 32);
-    const dim3 grid(static_cast<unsigned>(tiles(p.M, 64) * nt));
-    if (p.cols > 32)
-      lora_shrink_kernel<4, 4, kFp8 ? 2 : 4, 2, kFp8><<<grid, dim3(kFp8 ? 128 : 256), 0, st>>>(p);
-    else
-      lora_shrink_kernel<4, 2, 4, 2, kFp8><<<grid, dim3(256), 0, st>>>(p);
+    const int bn = !kFp8 && p.cols > 32 ? 64 : 32, nt = tiles(p.cols, bn);
+    const dim3 grid(static_cast<unsigned>(gdn::kNumXcd * tiles(tiles(p.M, 64) * nt, gdn::kNumXcd)));
+    if constexpr (!kFp8)
+      if (bn == 64) {
+        lora_shrink_kernel<4, 4, 4, 2, false><<<grid, dim3(256), 0, st>>>(p);
+        return gdn_launch_status();
+      }
+    lora_shrink_kernel<4, 2, 4, 2, kFp8><<<grid, dim3(256), 0, st>>>(p);
     return gdn_launch_status();
   }
-  const int t = tiles(p.M, 16) * tiles(p.cols, 16);
-  // a tile's adapters over so many workgroups (those that find none end)
-  const int share = std::max(1, std::min(std::min(16, p.M), 1024 / t));
-  lora_shrink_kernel<1, 1, 8, 3, kFp8><<<dim3(static_cast<unsigned>(t), static_cast<unsigned>(share)), dim3(512), 0, st>>>(p);
+  // so many workgroups share the adapters (those that find none end); 16 waves where 8 would have more
+  // than one round of loads
+  const int n = tiles(p.cols, 16), most = std::max(1, 1024 / n);
+  const bool sort = lora_sorted(p.M), wide = p.K > 2048;
+  const int share = sort ? std::min(most, std::min(p.M, tiles(p.M, 16) + std::min(p.slots, p.M)))
+                         : std::max(1, std::min(std::min(std::min(16, p.M), p.slots), 1024 / (n * tiles(p.M, 16))));
+  const dim3 grid(static_cast<unsigned>(sort ? n : n * tiles(p.M, 16)), static_cast<unsigned>(share));
+  if (sort)
+    wide ? lora_few_kernel<16, kFp8, true><<<grid, dim3(1024), 0, st>>>(p)
+         : lora_few_kernel<8, kFp8, true><<<grid, dim3(512), 0, st>>>(p);
+  else
+    wide ? lora_few_kernel<16, kFp8, false><<<grid, dim3(1024), 0, st>>>(p)
+         : lora_few_kernel<8, kFp8, false><<<grid, dim3(512), 0, st>>>(p);
   return gdn_launch_status();
 }
 

@@ -20,6 +20,12 @@
 namespace {
 
 constexpr int kMaxRank = 256;
+// Up to so many rows, and more than one tile's, are sorted by their adapters (lora.hip), and the kernels
+// of few rows take them in that order.  200 rows of 32 adapters at random, 12352 columns of e4m3 x 2048, rank 32: 32 us,
+// as they come 42.  (One tile's have nothing to gain: 1 row 16.0 us, sorted 17.3.  The counting grows
+// with the square of the rows: 512 would take 3 us of every workgroup.)
+constexpr int kLoraSort = GDN_LORA_SORT;
+__host__ __device__ constexpr bool lora_sorted(int M) { return M > 16 && M <= kLoraSort; }
 
 struct Lora {
   const uint16_t* v;    // [M, slices, 2, rank] bf16, row stride ldv
@@ -28,6 +34,7 @@ struct Lora {
   int64_t b_slot;
   const int* ids;       // [M]
   const int* groups;    // [ceil(M / 16)]: the adapter of 16 rows, -1 none, -2 not one for all (lora.hip)
+  const int* order;     // lora_sorted: [M] the rows in the order of their adapters, [M] the adapters
   int slots, rank, slices;
   int end[kMaxParts];   // slice p: columns end[p - 1] .. end[p] - 1; multiples of 16
 };
@@ -88,17 +95,18 @@ __device__ __forceinline__ gdn::s16x8_t lora_mask(const gdn::s16x8_t& v, bool ke
 }
 
 // The adapters of a wave's rows, each once, in the rows' order: `mine` is the lane's row's, -1
-// for none.  With `turns` waves that share the rows, wave `turn` takes every turns-th.
+// for none.  With `turns` waves that share the rows, wave `turn` takes every turns-th adapter (by its
+// number, and not by its place among the rows': which wave adds it shows in the result's last bits).
 struct LoraIds {
   uint64_t todo;
-  int turn, turns, at;
+  int turn, turns;
   // the next one and the lanes whose rows have it, or -1 (wave-uniform)
   __device__ __forceinline__ int next(int mine, uint64_t& rows) {
     while (todo) {
       const int s = __builtin_amdgcn_readlane(mine, __builtin_ctzll(todo));
       rows = __ballot(mine == s);
       todo &= ~rows;
-      if (at++ % turns == turn) return s;
+      if (turns == 1 || s % turns == turn) return s;
     }
     rows = 0;
     return -1;
@@ -110,6 +118,22 @@ __device__ __forceinline__ int lora_id(const Lora& lo, int r, int M) {
   const int s = lo.ids[min(r, M - 1)];
   return r < M && static_cast<unsigned>(s) < static_cast<unsigned>(lo.slots) ? s : -1;
 }
+
+// What the kernels of few rows have as their r-th row, at most the last one: rows in the order of
+// their adapters have few in a tile, and each is loaded and multiplied once there.
+template <bool kOrder, class L>
+__device__ __forceinline__ int lora_row(const L& lo, int r, int M) {
+  r = min(r, M - 1);
+  if constexpr (kOrder) r = lo.order ? lo.order[r] : r;
+  return r;
+}
+
+template <bool kOrder, class L>
+struct LoraOrder {
+  const L& lo;
+  int M;
+  __device__ __forceinline__ int operator()(int r) const { return lora_row<kOrder>(lo, r, M); }
+};
 
 // One past the last column of slice p.
 __device__ __forceinline__ int lora_end(const Lora& lo, int p) {
@@ -155,7 +179,7 @@ __device__ __forceinline__ void lora_pass(const Lora& lo, int N, const int (&id)
           // (a column of another slice: 0, as its value of v is not this slice's)
           boff[j][t] = ((cb[j] + brow + 4 * t) * lo.rank * 2 + 16 * qb) | off |
                        (cb[j] + brow + 4 * t >= beg && cb[j] + brow + 4 * t < end ? 0 : kNoOffset);
-      LoraIds it{all, turn, turns, 0};
+      LoraIds it{all, turn, turns};
       gdn::s16x8_t fb[DEPTH][CT][2];
       int sid[DEPTH];
       uint64_t rows[DEPTH];
@@ -204,7 +228,7 @@ __device__ __forceinline__ void lora_pass(const Lora& lo, int N, const int (&id)
 
 // The adapters of a lane's rows row0 + 16 i + lr and where their values are in v; `mine` is that of
 // row0 + lane, `all` the lanes that have one.
-template <int RT>
+template <int RT, bool kOrder>
 struct LoraRows {
   int id[RT], voff[RT], mine;
   uint64_t all;
@@ -212,8 +236,12 @@ struct LoraRows {
     const int lr = lane & 15, lg = lane >> 4;
 #pragma unroll
     for (int i = 0; i < RT; ++i) {
-      id[i] = lora_id(lo, row0 + 16 * i + lr, M);
-      voff[i] = static_cast<int>(min(row0 + 16 * i + lr, M - 1) * lo.ldv * 2);
+      const int r = row0 + 16 * i + lr;
+      if (kOrder && lo.order)
+        id[i] = r < M ? lo.order[M + r] : -1;
+      else
+        id[i] = lora_id(lo, r, M);
+      voff[i] = static_cast<int>(lora_row<kOrder>(lo, r, M) * lo.ldv * 2);
     }
     mine = RT * 16 > lane ? id[0] : -1;
 #pragma unroll
@@ -227,7 +255,7 @@ struct LoraRows {
 // of the rank the high parts, then the low ones.
 template <int DEPTH, class At>
 __device__ __forceinline__ void lora_add(const Lora& lo, int M, int N, int row0, int cb, int lane, const At& at) {
-  const LoraRows<4> r(lo, M, row0, lane);
+  const LoraRows<4, false> r(lo, M, row0, lane);
   if (!r.all || cb >= N) return;
   const int lr = lane & 15, lg = lane >> 4, half = lo.rank / 8;
   const bool both = half <= 4;  // high and low parts meet the same values of b at once
@@ -249,7 +277,7 @@ __device__ __forceinline__ void lora_add(const Lora& lo, int M, int N, int row0,
 #pragma unroll
         for (int i = 0; i < 4; ++i) vl[i] = lora_load(rv, (r.voff[i] + 16 * (q + half)) | off);
       }
-      LoraIds it{r.all, 0, 1, 0};
+      LoraIds it{r.all, 0, 1};
       gdn::s16x8_t fb[DEPTH][2];
       int sid[DEPTH];
       uint64_t rows[DEPTH];
@@ -292,7 +320,7 @@ __device__ __forceinline__ void lora_add(const Lora& lo, int M, int N, int row0,
 template <int RT, int CT, int DEPTH, class At>
 __device__ __forceinline__ void lora_init(const Lora& lo, int M, int N, int row0, const int (&cb)[CT], int lane, int turn,
                                           int turns, const At& at) {
-  const LoraRows<RT> r(lo, M, row0, lane);
+  const LoraRows<RT, true> r(lo, M, row0, lane);
   if (!r.all) return;
   lora_pass<RT, CT, DEPTH, false>(lo, N, r.id, r.mine, r.all, r.voff, cb, lane, turn, turns, at);
   float bad = 0.0f;
@@ -501,7 +529,7 @@ bool lora_of(Lora& lo, const uint16_t* v, int64_t ldv, const int* groups, const 
       b_slot % 8 || (slots > 1 && b_slot < static_cast<int64_t>(N) * rank) ||
       static_cast<int64_t>(N + 256) * rank * 2 >= kLimit)
     return false;
-  lo = Lora{v, ldv, b, b_slot, ids, groups, slots, rank, slices, {N, N, N, N}};
+  lo = Lora{v, ldv, b, b_slot, ids, groups, lora_sorted(M) ? groups + (M + 15) / 16 : nullptr, slots, rank, slices, {N, N, N, N}};
   for (int p = 0, beg = 0; p < slices; beg = slice_end[p++]) {
     const bool last = p + 1 == slices;
     if (slice_end[p] <= beg || (last ? slice_end[p] != N : slice_end[p] % 16 != 0 || slice_end[p] >= N)) return false;

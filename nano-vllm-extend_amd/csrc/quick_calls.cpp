@@ -628,7 +628,7 @@ struct Adapters {
   int64_t ldv() const { return 2 * P * R; }
   int32_t* groups() const { return reinterpret_cast<int32_t*>(v() + M * ldv()); }
   void allocate(const Tensor& x, IntArrayRef lead) {
-    work = at::empty({M * ldv() * 2 + (M + 15) / 16 * 4}, x.options().dtype(ScalarType::Byte));
+    work = at::empty({M * ldv() * 2 + (M + 15) / 16 * 4 + (M <= GDN_LORA_SORT ? 8 * M : 0)}, x.options().dtype(ScalarType::Byte));
     for (int i = 0; i < n; ++i) {
       at::DimVector shape(lead.begin(), lead.end());
       shape.push_back(width[i]);

@@ -1511,6 +1511,7 @@ def linear_fp8_cols(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.T
 
 # ------------------------------------------------------ low-rank adapters --
 LORA_MAX_RANK = 256
+LORA_SORT = 256       # GDN_LORA_SORT
 
 
 class LoraPool:
@@ -1602,9 +1603,10 @@ def _lora_check(x, N, K, widths, lora_a, lora_b, lora_scale, ids):
 
 
 def _lora_shrink(idx, rows, stride, x_scale, lora_a, lora_scale, ids, M, K, P, R):
-    """(v [M, P, 2, R] of the rows with an adapter, the adapters of their groups of 16)."""
+    """(v [M, P, 2, R] of the rows with an adapter, the adapters of their groups of 16 and, of few
+    rows, their order)."""
     v = torch.empty(M, P * 2 * R, dtype=torch.bfloat16, device=rows.device)
-    groups = torch.empty(-(-M // 16), dtype=torch.int32, device=rows.device)
+    groups = torch.empty(-(-M // 16) + (2 * M if M <= LORA_SORT else 0), dtype=torch.int32, device=rows.device)
     xs = (0, 0, 0) if x_scale is None else (x_scale.data_ptr(), *x_scale.stride())
     _call_on(idx, "gdn_lora_shrink", rows.data_ptr(), int(x_scale is None), stride, *xs, lora_a.data_ptr(),
              lora_a.stride(0), lora_scale.data_ptr(), ids.data_ptr(), lora_a.shape[0], P, R, M, K, v.data_ptr(), 2 * P * R,

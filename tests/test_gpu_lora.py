@@ -378,3 +378,40 @@ def test_out_of_memory_is_torchs_error(pkg, dev):
             with pytest.raises(torch.OutOfMemoryError):
                 call()
     assert bool((calls[0]() == K + K * R).all())
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("M", [2, 15, 16, 17, 63, 64, 65, 127, 129, 200, 255, 256, 257, 300])
+@pytest.mark.parametrize("N,S,how", [(96, 3, "mixed"), (96, 300, "mixed"), (12352, 8, "mixed"), (96, 5, "one"), (160, 1, "mixed"), (2048, 30, "mixed")])
+def test_rows_in_the_order_of_their_adapters(pkg, dev, M, N, S, how, fp8):
+    """Few rows are taken in their adapters' order: at the sizes where that begins, ends and changes, with more
+    adapters than rows and with one, each row stays its own, and the gates with it."""
+    gen = torch.Generator().manual_seed(M + N + S)
+    K, R = 256, 8
+    x = torch.randn(M, K, generator=gen).to(BF16).to(dev)
+    w = (torch.randn(N, K, generator=gen) * K ** -0.5).to(BF16).to(dev)
+    a, b, scale = (t.to(dev) for t in _adapters(gen, S, [N], K, R))
+    ids = _ids(gen, M, S, how).to(dev)
+    delta, slack = _delta(x, a, b, scale, ids, [N], K)
+    if fp8:
+        w8, ws = pkg.quantize_weight_fp8(w)
+        x8, xs = pkg.quantize_fp8(x)
+        y = pkg.linear_fp8_lora(x, w8, ws, a, b, scale, ids)
+        want, base = ref.linear(x8, xs, w8, ws)
+        base = base + 4 * R * U * (want.abs() + delta.abs())
+    else:
+        y = pkg.linear_lora(x, w, a, b, scale, ids)
+        want, base = x.double() @ w.double().t(), 2 * (K + 2 * R) * U * (x.double().abs() @ w.double().abs().t())
+    _check(y, want + delta, slack + base)
+    # an adapter's rows alone, at the same size: the same bits
+    for s in ids[[0, M // 2, M - 1]].tolist():
+        rows = ids == s
+        only = torch.where(rows, ids, -1)
+        again = pkg.linear_fp8_lora(x, w8, ws, a, b, scale, only) if fp8 else pkg.linear_lora(x, w, a, b, scale, only)
+        assert torch.equal(again[rows], y[rows])
+    if not fp8 and N == 96:
+        gates = dict(A_log=torch.randn(16, generator=gen).to(dev), dt_bias=torch.randn(16, generator=gen).to(dev), gate_col=64)
+        y2, g, beta = pkg.linear_lora(x, w, a, b, scale, ids, gates=gates)
+        assert torch.equal(y2, y)
+        eg, eb = pkg.fused_g_beta(y[:, 64:80].contiguous(), y[:, 80:].contiguous(), gates["A_log"], gates["dt_bias"], None)
+        assert torch.equal(g, eg) and torch.equal(beta, eb)
