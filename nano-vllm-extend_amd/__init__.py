@@ -2,8 +2,8 @@
 
 The GDN kernels of the Qwen3.5 hybrid model -- varlen / decode / padded
 causal conv + SiLU, fused g/beta, chunked gated delta rule, recurrent
-decode (single- and multi-token), gated RMSNorm, the projection GEMMs -- as
-hand-written HIP for
+decode (single- and multi-token), gated RMSNorm, the projection GEMMs with the
+requests' low-rank adapters, the norms around the mixer -- as hand-written HIP for
 gfx950 behind the C ABI of include/gdn_mi355x.h, with Python wrappers that
 keep the reference's call signatures (ops), a host mirror of the layer
 dispatch (gdn_layer), the slot-pool bookkeeping (state_pool) and the hook
@@ -40,5 +40,5 @@ from .ops import (  # noqa: F401
     rms_norm_gated,
     rms_norm_gated_fp8,
 )
-from .gdn_layer import GatedDeltaNetCore, GatedDeltaNetLayer, Switches, TreeStep  # noqa: F401
+from .gdn_layer import GatedDeltaNetBlock, GatedDeltaNetCore, GatedDeltaNetLayer, Switches, TreeStep  # noqa: F401
 from .state_pool import LinearStatePool, allocate_state_pools, reset_linear_states, varlen_meta  # noqa: F401

@@ -566,7 +566,12 @@ class GatedDeltaNetLayer:
     hidden and Hv*D are then multiples of 128.  Those three come in bf16 (they are
     converted here, once) or as a checkpoint's (e4m3, scales) pairs.  in_proj_b and
     in_proj_a, the gates' inputs, stay bf16: they are 2 Hv rows, and an error in
-    them is an error in every decay."""
+    them is an error in every decay.
+
+    add_adapters makes room for low-rank adapters beside the projections (qkv, z, b and a
+    each with an A of its own, and out); a call's `adapters` then names each row's slot."""
+
+    lora_in = lora_out = None   # LoraPool, once add_adapters has made them
 
     def __init__(self, w_qkv, w_z, w_b, w_a, w_out, num_k_heads: int, num_v_heads: int, head_dim: int,
                  conv_weight, A_log, dt_bias, norm_weight, eps: float = 1e-6, switches: Switches | None = None,
@@ -624,6 +629,39 @@ class GatedDeltaNetLayer:
     def n_in(self) -> int:
         return self.w_in.shape[0] + (self.w_ba.shape[0] if self.fp8 else 0)
 
+    def add_adapters(self, slots: int, rank: int) -> None:
+        """Room for `slots` low-rank adapters of at most `rank`, all of them empty, in the
+        place of those that were there.  (The value heads are a multiple of 16: where a
+        product's columns change from one projection to the next.)"""
+        c, dev = self.core, self.w_in.device
+        if c.Hv % 16 or self.hidden % 64 or c.value_dim % 64:
+            raise ValueError(f"adapters need value heads in multiples of 16 and rows in multiples of 64, got {c.Hv} heads, "
+                             f"{self.hidden} and {c.value_dim} columns")
+        pools = (ops.LoraPool(slots, rank, self.hidden, [c.conv_dim, c.value_dim, c.Hv, c.Hv], dev),
+                 ops.LoraPool(slots, rank, c.value_dim, [self.hidden], dev))
+        self.lora_in, self.lora_out = pools
+
+    def load_adapter(self, slot: int, scale: float, qkv=None, z=None, b=None, a=None, out=None) -> None:
+        """An adapter into a slot: (A [r, in], B [rows, r]) for the projections that it has one for, as the
+        checkpoint names them; scale is its alpha / r."""
+        self._pools()
+        self.lora_in.check(slot, [qkv, z, b, a])
+        self.lora_out.check(slot, [out])
+        self.lora_in.load(slot, [qkv, z, b, a], scale)
+        self.lora_out.load(slot, [out], scale)
+
+    def clear_adapter(self, slot: int) -> None:
+        for pool in self._pools():
+            pool.clear(slot)
+
+    def _pools(self):
+        if self.lora_in is None:
+            raise ValueError("the layer has no room for adapters: add_adapters first")
+        return self.lora_in, self.lora_out
+
+    def _lora(self, pool, adapters):
+        return pool.a, pool.b, pool.scale, adapters
+
     def _timed(self, name):
         return _NOT_TIMED if self.timer is None else _timing(self.timer, name)
 
@@ -635,74 +673,151 @@ class GatedDeltaNetLayer:
         fused_ok = sw.gbeta and sw.conv_kernel and c.K == 4
         return sw.gbeta and not (fused_ok and sw.fused_prefill and sw.varlen and sw.fused_decode and sw.inplace)
 
-    def project_in(self, hidden, gates: bool = False):
+    def project_in(self, hidden, gates: bool = False, adapters=None, fp8=None):
         """hidden [N, hidden] -> (mixed, z, b, a): one GEMM over the four
         concatenated weights whose output goes to four contiguous tensors,
         mixed [N, C], z [N, Hv*D], b and a [N, Hv] (rows of contiguous tensors
         read faster than columns of one wide buffer, and the gate readers take
         them without a copy); with gates, also (g, beta) of the b and a
         columns from the GEMM's epilogue (bit-equal to the gate kernel on
-        them, qwen3_5.py:933-934), else None."""
+        them, qwen3_5.py:933-934), else None.  adapters: each row's (forward).  fp8: hidden's
+        (e4m3, scales), for 8-bit weights, where what made hidden made those too."""
         c = self.core
         C, V, Hv = c.conv_dim, c.value_dim, c.Hv
         widths = [C, V, Hv, Hv]
+        how = {"gate_col": 0 if self.fp8 else C + V, "A_log": c.A_log, "dt_bias": c.dt_bias} if gates else None
+        if adapters is not None:
+            lora = self._lora(self._pools()[0], adapters)
+            with self._timed("in_proj"):
+                if self.fp8:
+                    y = ops.linear_fp8_lora(hidden, self.w_in, self.w_in_scale, *lora, widths=widths, wide=self.w_ba, gates=how)
+                else:
+                    y = ops.linear_lora(hidden, self.w_in, *lora, widths=widths, gates=how)
+            return (*y[0], y[1:]) if gates else (*y, None)
+        if self.fp8 and fp8 is not None:
+            with self._timed("in_proj"):
+                mixed, z = ops.linear_fp8_cols(fp8[0], self.w_in, self.w_in_scale, [C, V], x_scale=fp8[1])
+                y = ops.linear(hidden, self.w_ba, gates=how)
+                y, gb = (y[0], y[1:]) if gates else (y, None)
+                return mixed, z, y[..., :Hv], y[..., Hv:], gb
         if self.fp8:
             with self._timed("in_proj"):
                 if Hv % 16 == 0 and not gates:
                     return (*ops.linear_fp8_cols(hidden, self.w_in, self.w_in_scale, widths, wide=self.w_ba), None)
                 mixed, z = ops.linear_fp8_cols(hidden, self.w_in, self.w_in_scale, [C, V])
-                how = {"gate_col": 0, "A_log": c.A_log, "dt_bias": c.dt_bias} if gates else None
                 y = ops.linear(hidden, self.w_ba, gates=how)
                 y, gb = (y[0], y[1:]) if gates else (y, None)
                 return mixed, z, y[..., :Hv], y[..., Hv:], gb
         with self._timed("in_proj"):
             if all(w % 16 == 0 for w in widths[:-1]):
                 if gates:
-                    (mixed, z, b, a), g, beta = ops.linear_cols(hidden, self.w_in, widths,
-                                                                gates={"gate_col": C + V, "A_log": c.A_log,
-                                                                       "dt_bias": c.dt_bias})
+                    (mixed, z, b, a), g, beta = ops.linear_cols(hidden, self.w_in, widths, gates=how)
                     gb = (g, beta)
                 else:
                     (mixed, z, b, a), gb = ops.linear_cols(hidden, self.w_in, widths), None
                 return mixed, z, b, a, gb
             if gates:
-                y, g, beta = ops.linear(hidden, self.w_in, gates={"gate_col": C + V, "A_log": c.A_log,
-                                                                  "dt_bias": c.dt_bias})
+                y, g, beta = ops.linear(hidden, self.w_in, gates=how)
                 gb = (g, beta)
             else:
                 y, gb = ops.linear(hidden, self.w_in), None
         return y[:, :C], y[:, C:C + V], y[:, C + V:C + V + Hv], y[:, C + V + Hv:], gb
 
-    def forward(self, hidden, cu_seqlens_q, max_seqlen_q, ids, conv_cache, s_cache, lens_q=None):
+    def forward(self, hidden, cu_seqlens_q, max_seqlen_q, ids, conv_cache, s_cache, lens_q=None, adapters=None, fp8=None):
         """Qwen3_5GatedDeltaNet.forward for one varlen step (qwen3_5.py:864-920):
-        hidden [N, hidden] bf16 -> [N, hidden] bf16."""
-        mixed, z, b, a, gb = self.project_in(hidden, gates=self.gates_in_gemm())
+        hidden [N, hidden] bf16 -> [N, hidden] bf16.  adapters: int32 [N], the slot of each
+        row's adapter (-1 and what is no slot: none), from the sequences' by
+        ops.adapter_rows once for all layers; None: no row has one."""
+        mixed, z, b, a, gb = self.project_in(hidden, gates=self.gates_in_gemm(), adapters=adapters, fp8=fp8)
         self.core.timer = self.timer
         core = self.core.forward(mixed, z, b.contiguous(), a.contiguous(), cu_seqlens_q, max_seqlen_q, ids,
                                  conv_cache, s_cache, lens_q=lens_q, gb=gb, fp8=self.fp8)
-        return self._project_out(core, hidden.shape)
+        return self._project_out(core, hidden.shape, adapters)
 
-    def _project_out(self, core, shape):
+    def _project_out(self, core, shape, adapters=None):
         with self._timed("out_proj"):
+            lora = None if adapters is None else self._lora(self._pools()[1], adapters)
             if not self.fp8:
-                return ops.linear(core, self.w_out)
+                return ops.linear(core, self.w_out) if lora is None else ops.linear_lora(core, self.w_out, *lora)
             core, scale = core if isinstance(core, tuple) else (core, None)
-            return ops.linear_fp8(core.reshape(*shape[:-1], self.core.value_dim), self.w_out, self.w_out_scale,
-                                  x_scale=scale)
+            core = core.reshape(*shape[:-1], self.core.value_dim)
+            if lora is not None:
+                return ops.linear_fp8_lora(core, self.w_out, self.w_out_scale, *lora, x_scale=scale)
+            return ops.linear_fp8(core, self.w_out, self.w_out_scale, x_scale=scale)
 
-    def verify_tree(self, hidden, ids, conv_cache, s_cache, parents, pending: TreeStep | None = None):
+    def verify_tree(self, hidden, ids, conv_cache, s_cache, parents, pending: TreeStep | None = None, adapters=None,
+                    fp8=None):
         """The mixer of one verify step over trees of T drafted tokens: hidden [B, T,
         hidden] bf16 -> ([B, T, hidden] bf16, TreeStep).  ids, parents and pending as
-        GatedDeltaNetCore.verify_tree; in_proj, core and out_proj as forward."""
+        GatedDeltaNetCore.verify_tree; in_proj, core and out_proj as forward; adapters
+        int32 [B * T]."""
         B, T, width = hidden.shape
-        rows = self.project_in(hidden.reshape(B * T, width))[:4]
+        rows = self.project_in(hidden.reshape(B * T, width), adapters=adapters, fp8=fp8)[:4]
         self.core.timer = self.timer
         core, step = self.core.verify_tree(*(t.reshape(B, T, t.shape[1]) for t in rows), ids, conv_cache, s_cache,
                                            parents, pending=pending, fp8=self.fp8)
         if not isinstance(core, tuple):
             core = core.reshape(B, T, self.core.value_dim)
-        return self._project_out(core, hidden.shape), step
+        return self._project_out(core, hidden.shape, adapters), step
 
     def commit_tree(self, step: TreeStep, ids, conv_cache, s_cache) -> None:
         self.core.timer = self.timer
         self.core.commit_tree(step, ids, conv_cache, s_cache)
+
+
+class GatedDeltaNetBlock:
+    """The mixer's half of a decoder layer: the residual stream's norm, the mixer, and the norm
+    that the layer's other half reads (the layer around it, nanovllm/models/qwen3_5.py:99-118,
+    :674-689).  Per step
+
+      y, stream = add_rms_norm(hidden, residual, input_norm)   what came before joins the stream
+      out       = layer(y)
+      y, stream = add_rms_norm(out, stream, post_norm)         the mixer's output joins it
+
+    and y and stream are returned: y is what the other half reads, and its output with the
+    stream goes into the next block.  input_norm, post_norm [hidden], held as their distance
+    from 1 (offset = 0: as they are).  residual is None where the stream begins; it may be bf16 or fp32
+    and stays what it is.
+
+    Where the layer has 8-bit weights and many rows, the first norm writes e4m3 with its scales
+    beside the bf16 rows, and in_proj quantizes nothing."""
+
+    def __init__(self, layer: GatedDeltaNetLayer, input_norm: torch.Tensor, post_norm: torch.Tensor, eps: float = 1e-6,
+                 offset: float = 1.0):
+        for t, name in ((input_norm, "input_norm"), (post_norm, "post_norm")):
+            if t.shape != (layer.hidden,):
+                raise ValueError(f"{name} must be [{layer.hidden}], got {list(t.shape)}")
+        self.layer, self.input_norm, self.post_norm, self.eps, self.offset = layer, input_norm, post_norm, eps, offset
+
+    def _input(self, hidden, residual, adapters):
+        """(what the mixer reads, its e4m3 form or None, the stream)."""
+        rows = hidden.numel() // hidden.shape[-1]
+        with self.layer._timed("input_norm"):
+            if self.layer.fp8 and adapters is None and rows > ops.FP8_WIDE_ROWS:
+                y8, scale, residual, y = ops.add_rms_norm_fp8(hidden, residual, self.input_norm, self.eps, offset=self.offset,
+                                                              keep=True)
+                return y, (y8.view(rows, y8.shape[-1]), scale), residual
+            y, residual = ops.add_rms_norm(hidden, residual, self.input_norm, self.eps, offset=self.offset)
+            return y, None, residual
+
+    def _post(self, out, residual):
+        with self.layer._timed("post_norm"):
+            return ops.add_rms_norm(out, residual, self.post_norm, self.eps, offset=self.offset)
+
+    def forward(self, hidden, residual, cu_seqlens_q, max_seqlen_q, ids, conv_cache, s_cache, lens_q=None, adapters=None):
+        """hidden, residual [N, hidden] -> (y [N, hidden] bf16, stream [N, hidden]); the rest as
+        GatedDeltaNetLayer.forward."""
+        y, fp8, residual = self._input(hidden, residual, adapters)
+        out = self.layer.forward(y, cu_seqlens_q, max_seqlen_q, ids, conv_cache, s_cache, lens_q=lens_q, adapters=adapters,
+                                 fp8=fp8)
+        return self._post(out, residual)
+
+    def verify_tree(self, hidden, residual, ids, conv_cache, s_cache, parents, pending: TreeStep | None = None, adapters=None):
+        """hidden, residual [B, T, hidden] -> (y, stream, TreeStep); the rest as
+        GatedDeltaNetLayer.verify_tree."""
+        y, fp8, residual = self._input(hidden, residual, adapters)
+        out, step = self.layer.verify_tree(y, ids, conv_cache, s_cache, parents, pending=pending, adapters=adapters, fp8=fp8)
+        return (*self._post(out, residual), step)
+
+    def commit_tree(self, step: TreeStep, ids, conv_cache, s_cache) -> None:
+        self.layer.commit_tree(step, ids, conv_cache, s_cache)

@@ -1326,6 +1326,9 @@ def linear_cols(x: torch.Tensor, weight: torch.Tensor, widths: list[int],
 # ------------------------------------------------------- 8-bit projections --
 FP8 = torch.float8_e4m3fn
 FP8_GROUP = 128   # values with one scale
+# Up to so many rows the bf16 columns beside an 8-bit product come with the launch that quantizes
+# its rows (linear_fp8_cols' wide); past it they are a product of their own.
+FP8_WIDE_ROWS = 1024
 
 
 def _rows_of(x: torch.Tensor, align: int):
@@ -1535,10 +1538,8 @@ class LoraPool:
         self.b = torch.zeros(slots, sum(self.widths), self.rank, dtype=torch.bfloat16, device=device)
         self.scale = torch.zeros(slots, dtype=torch.float32, device=device)
 
-    def load(self, slot: int, parts, scale: float) -> None:
-        """An adapter into a slot: for each projection (A [r, in_features], B [width, r]),
-        r at most the pool's rank, or None where the adapter has nothing for it; scale as
-        the checkpoint defines it (alpha / r)."""
+    def check(self, slot: int, parts) -> None:
+        """Raises where load would."""
         if not 0 <= slot < self.a.shape[0]:
             raise ValueError(f"slot {slot} of {self.a.shape[0]}")
         if len(parts) != len(self.widths):
@@ -1549,6 +1550,12 @@ class LoraPool:
                 if r > self.rank or part[0].shape != (r, self.in_features) or part[1].shape != (width, r):
                     raise ValueError(f"A must be [r, {self.in_features}] and B [{width}, r] with r <= {self.rank}, got "
                                      f"{list(part[0].shape)} and {list(part[1].shape)}")
+
+    def load(self, slot: int, parts, scale: float) -> None:
+        """An adapter into a slot: for each projection (A [r, in_features], B [width, r]),
+        r at most the pool's rank, or None where the adapter has nothing for it; scale as
+        the checkpoint defines it (alpha / r)."""
+        self.check(slot, parts)
         self.clear(slot)
         col = 0
         for p, (part, width) in enumerate(zip(parts, self.widths)):
