@@ -411,16 +411,23 @@ __global__ __launch_bounds__(64 * NW) void lora_shrink_kernel(Shrink p) {
 template <bool kFp8>
 int launch(const Shrink& p, hipStream_t st) {
   auto tiles = [](int n, int of) { return (n + of - 1) / of; };
-  // one wave's rows: prompts fill the chip with 64-row tiles
+  // Prompts: 64-row tiles, all columns up to 64 (32 of them where x is e4m3: its stages are the larger ones).
+  // Four waves have a CU's LDS for themselves; with more tiles than CUs two waves and a
+  // half of it, so that a second tile runs beside the first.  us, four waves / two, 2048 columns of bf16 x, all rows one
+  // adapter's: 17001 x 64 (266 tiles) 26.3 / 21.5, 16384 x 128 (512) 25.9 / 20.9, 16384 x 64 (256) 18.1 / 18.0, 4096 x 128
+  // (128) 12.5 / 15.1; e4m3, 16384 x 64 (512) 21.2 / 17.0, 16384 x 16 (256) 11.9 / 13.7, 4096 x 128 (256) 10.9 / 13.3.
   if (p.M > 2048) {
-    const int bn = !kFp8 && p.cols > 32 ? 64 : 32, nt = tiles(p.cols, bn);
-    const dim3 grid(static_cast<unsigned>(gdn::kNumXcd * tiles(tiles(p.M, 64) * nt, gdn::kNumXcd)));
+    const int bn = !kFp8 && p.cols > 32 ? 64 : 32, n = tiles(p.M, 64) * tiles(p.cols, bn);
+    const dim3 grid(static_cast<unsigned>(gdn::kNumXcd * tiles(n, gdn::kNumXcd)));
+    const bool two = n > gdn::kNumCu;
     if constexpr (!kFp8)
       if (bn == 64) {
-        lora_shrink_kernel<4, 4, 4, 2, false><<<grid, dim3(256), 0, st>>>(p);
+        two ? lora_shrink_kernel<4, 4, 2, 2, false><<<grid, dim3(128), 0, st>>>(p)
+            : lora_shrink_kernel<4, 4, 4, 2, false><<<grid, dim3(256), 0, st>>>(p);
         return gdn_launch_status();
       }
-    lora_shrink_kernel<4, 2, 4, 2, kFp8><<<grid, dim3(256), 0, st>>>(p);
+    two ? lora_shrink_kernel<4, 2, 2, 2, kFp8><<<grid, dim3(128), 0, st>>>(p)
+        : lora_shrink_kernel<4, 2, 4, 2, kFp8><<<grid, dim3(256), 0, st>>>(p);
     return gdn_launch_status();
   }
   // so many workgroups share the adapters (those that find none end); 16 waves where 8 would have more

@@ -780,7 +780,9 @@ class GatedDeltaNetBlock:
     and stays what it is.
 
     Where the layer has 8-bit weights and many rows, the first norm writes e4m3 with its scales
-    beside the bf16 rows, and in_proj quantizes nothing."""
+    beside the bf16 rows, and in_proj quantizes nothing: norm and in_proj of 16384 rows (hidden 2048,
+    32 value heads) 494 us against 501, of 2048 85 against 87; of 256 26 against 25, where in_proj's own
+    launch takes the bf16 columns along."""
 
     def __init__(self, layer: GatedDeltaNetLayer, input_norm: torch.Tensor, post_norm: torch.Tensor, eps: float = 1e-6,
                  offset: float = 1.0):
