@@ -697,16 +697,18 @@ __global__ __launch_bounds__(kPPThreads, 2) void gemm_tn_pp_kernel(const uint16_
     // kept in registers across the loop)
     int tid_e = static_cast<int>(threadIdx.x);
     asm volatile("" : "+v"(tid_e));
-    const GemmOut out_e = kLora ? kernel_arg<GemmOut>(offsetof(Args, out)) : out;
-    const GemmGates gt_e = kLora ? kernel_arg<GemmGates>(offsetof(Args, gt)) : gt;
+    if constexpr (kLora)
+      gemm_store_tile<false>(acc, kernel_arg<GemmOut>(offsetof(Args, out)), M, N, m0c, n0c, wm, wn, tid_e & 63,
+                             kernel_arg<GemmGates>(offsetof(Args, gt)), gscr[wave]);
+    else
 #pragma unroll
-    for (int a = 0; a < 2; ++a)
+      for (int a = 0; a < 2; ++a)
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < 4; ++i)
 #pragma unroll
-        for (int b = 0; b < 2; ++b)
-          gemm_store16(acc[a][b][i][0], acc[a][b][i][1], out_e, M, N, m0c + 128 * a + 64 * wm + 16 * i,
-                       n0c + 128 * b + 32 * wn, tid_e & 63, gt_e, gscr[wave]);
+          for (int b = 0; b < 2; ++b)
+            gemm_store16(acc[a][b][i][0], acc[a][b][i][1], out, M, N, m0c + 128 * a + 64 * wm + 16 * i,
+                         n0c + 128 * b + 32 * wn, tid_e & 63, gt, gscr[wave]);
     if (Ln >= xend) break;
     L = Ln;
   }

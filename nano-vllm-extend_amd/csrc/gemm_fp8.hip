@@ -435,15 +435,18 @@ __global__ __launch_bounds__(kPPThreads, 2) void gemm_fp8_pp_kernel(const uint8_
       }
       if (!wm) half_barrier();
       const int lane_e = new_lane();
-      const GemmOut out_e = kLora ? kernel_arg<GemmOut>(offsetof(Args, out)) : out;
+      if constexpr (kLora)
+        gemm_store_tile<true>(acc, kernel_arg<GemmOut>(offsetof(Args, out)), M, N, m0c, n0c, wm, wn, lane_e, GemmGates{},
+                              nullptr);
+      else
 #pragma unroll
-      for (int a = 0; a < 2; ++a)
+        for (int a = 0; a < 2; ++a)
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+          for (int i = 0; i < 4; ++i)
 #pragma unroll
-          for (int b = 0; b < 2; ++b)
-            gemm_store16<true>(acc[a][b][i][0], acc[a][b][i][1], out_e, M, N, m0c + 128 * a + 64 * wm + 16 * i,
-                         n0c + 128 * b + 32 * wn, lane_e, GemmGates{}, nullptr);
+            for (int b = 0; b < 2; ++b)
+              gemm_store16<true>(acc[a][b][i][0], acc[a][b][i][1], out, M, N, m0c + 128 * a + 64 * wm + 16 * i,
+                           n0c + 128 * b + 32 * wn, lane_e, GemmGates{}, nullptr);
       if (Ln >= xend) break;
       L = Ln;
     }

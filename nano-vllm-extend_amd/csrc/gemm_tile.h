@@ -128,6 +128,51 @@ __device__ __forceinline__ void gemm_store16(const gdn::f32x4_t& c0, const gdn::
   }
 }
 
+// A wave's part of a 256 x 256 tile, by gemm_store16's blocks: those of the columns that lie in one part
+// with 16-byte rows share what is found out about them (one by one, 1 us more a tile).
+template <bool kAnyRow>
+__device__ __forceinline__ void gemm_store_tile(const gdn::f32x4_t (&acc)[2][2][4][2], const GemmOut& out, int M, int N,
+                                                int m0, int n0, int wm, int wn, int lane, const GemmGates& gt,
+                                                uint16_t* gs) {
+  const int row = m0 + 64 * wm + (lane & 15);
+#pragma unroll
+  for (int b = 0; b < 2; ++b) {
+    const int cb = n0 + 128 * b + 32 * wn;
+    int s = 0;
+#pragma unroll
+    for (int i = 0; i + 1 < kMaxParts; ++i) s += cb >= out.end[i] ? 1 : 0;
+    int end = out.end[0], beg = 0, vec = out.vec[0];
+    uint16_t* c = out.c[0];
+    int64_t ld = out.ld[0];
+#pragma unroll
+    for (int i = 1; i < kMaxParts; ++i) {
+      end = s == i ? out.end[i] : end;
+      beg = s == i ? out.end[i - 1] : beg;
+      vec = s == i ? out.vec[i] : vec;
+      c = s == i ? out.c[i] : c;
+      ld = s == i ? out.ld[i] : ld;
+    }
+    if (vec && cb + 32 <= end && !(gt.g && cb + 32 > gt.gate_col && cb < gt.gate_col + 2 * gt.Hv)) {
+      uint16_t* at = c + row * ld + (cb - beg + 8 * (lane >> 4));
+#pragma unroll
+      for (int a = 0; a < 2; ++a)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const gdn::f32x4_t &c0 = acc[a][b][i][0], &c1 = acc[a][b][i][1];
+          const uint4 w = make_uint4(gdn::f2bf2(c0[0], c0[1]), gdn::f2bf2(c0[2], c0[3]), gdn::f2bf2(c1[0], c1[1]),
+                                     gdn::f2bf2(c1[2], c1[3]));
+          if (row + 128 * a + 16 * i < M) *reinterpret_cast<uint4*>(at + (128 * a + 16 * i) * ld) = w;
+        }
+    } else {
+#pragma unroll
+      for (int a = 0; a < 2; ++a)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          gemm_store16<kAnyRow>(acc[a][b][i][0], acc[a][b][i][1], out, M, N, m0 + 128 * a + 64 * wm + 16 * i, cb, lane, gt, gs);
+    }
+  }
+}
+
 __device__ __forceinline__ void half_barrier() {
   asm volatile("" ::: "memory");
   __builtin_amdgcn_sched_barrier(0);

@@ -283,14 +283,22 @@ __global__ __launch_bounds__(64 * NW) void lora_shrink_kernel(Shrink p) {
     id[i] = r < p.M && static_cast<unsigned>(s) < static_cast<unsigned>(p.slots) ? s : -1;
     const int first = __builtin_amdgcn_readfirstlane(id[i]);
     const bool alike = !__any(r < p.M && id[i] != first);
-    if (c0 == 0 && threadIdx.x == 0 && r < p.M) p.groups[m0 / 16 + i] = alike ? first : -2;
+    if (c0 == 0 && blockIdx.y == 0 && threadIdx.x == 0 && r < p.M) p.groups[m0 / 16 + i] = alike ? first : -2;
   }
   int mine = BM > lane ? id[0] : -1;  // row m0 + lane's
 #pragma unroll
   for (int i = 1; i < MT; ++i) mine = lg == i ? id[i] : mine;
   LoraIds it{__ballot(mine >= 0), 0, 1};
   uint64_t rows;
-  int s = it.next(mine, rows);
+  int turn = static_cast<int>(blockIdx.y);  // adapters before this workgroup's next
+  auto next = [&]() {
+    int s;
+    do s = it.next(mine, rows);
+    while (s >= 0 && turn-- > 0);
+    turn = static_cast<int>(gridDim.y) - 1;
+    return s;
+  };
+  int s = next();
   if (s < 0) return;  // (the workgroup)
 
   const __amdgpu_buffer_rsrc_t rx = rsrc_of(p.x), rs = rsrc_of(p.xs);
@@ -403,7 +411,7 @@ __global__ __launch_bounds__(64 * NW) void lora_shrink_kernel(Shrink p) {
       for (int w = 1; w < NW; ++w) sum += red[(w * MT * NT + ij) * 64 + lane];
       if (id[i] == s) store_v(p, m0 + 16 * i + lr, c0 + 16 * j + 4 * lg, sum, scale);
     }
-    s = it.next(mine, rows);
+    s = next();
     if (s >= 0) __syncthreads();  // the sums have been read
   }
 }
@@ -418,8 +426,13 @@ int launch(const Shrink& p, hipStream_t st) {
   // (128) 12.5 / 15.1; e4m3, 16384 x 64 (512) 21.2 / 17.0, 16384 x 16 (256) 11.9 / 13.7, 4096 x 128 (256) 10.9 / 13.3.
   if (p.M > 2048) {
     const int bn = !kFp8 && p.cols > 32 ? 64 : 32, n = tiles(p.M, 64) * tiles(p.cols, bn);
-    const dim3 grid(static_cast<unsigned>(gdn::kNumXcd * tiles(n, gdn::kNumXcd)));
     const bool two = n > gdn::kNumCu;
+    // Workgroups share a tile's adapters where that leaves no more of them than find room at once (one that finds
+    // none ends): 17001 x 64 in 21 sequences 34.0 alone, 25.5 in two; 4096 x 16 in sequences of 700 12.7 and 8.7; 16384 x
+    // 16 (256 tiles) 15.4 and 16.8.
+    const int room = (two ? 2 : 1) * gdn::kNumCu;
+    const int share = std::max(1, std::min(16, (room + n / 2) / n));
+    const dim3 grid(static_cast<unsigned>(gdn::kNumXcd * tiles(n, gdn::kNumXcd)), static_cast<unsigned>(share));
     if constexpr (!kFp8)
       if (bn == 64) {
         two ? lora_shrink_kernel<4, 4, 2, 2, false><<<grid, dim3(128), 0, st>>>(p)

@@ -42,6 +42,30 @@ struct NoLora {};
 template <bool kLora>
 using LoraArg = std::conditional_t<kLora, Lora, NoLora>;
 
+// A pointer that is known to be one to global memory: by any other a store is a flat one, which
+// the LDS reads behind it wait for as well (a tile's stores: 2.3 us of the next tile's products).
+template <class T>
+__device__ __forceinline__ void in_global(T*& p) {
+  p = (T*)(__attribute__((address_space(1))) T*)reinterpret_cast<uintptr_t>(p);
+}
+__device__ __forceinline__ void in_global(GemmOut& o) {
+#pragma unroll
+  for (int i = 0; i < kMaxParts; ++i) in_global(o.c[i]);
+}
+__device__ __forceinline__ void in_global(GemmGates& g) {
+  in_global(g.g);
+  in_global(g.beta);
+  in_global(g.A_log);
+  in_global(g.dt_bias);
+}
+__device__ __forceinline__ void in_global(Lora& lo) {
+  in_global(lo.v);
+  in_global(lo.b);
+  in_global(lo.ids);
+  in_global(lo.groups);
+  in_global(lo.order);
+}
+
 // A kernel's argument read from where the launch put it, `offset` bytes into its arguments: at the
 // few places between tiles that need it, and not held in scalar registers across a loop that has
 // none to spare (spilled ones made its loads late: 15 % of a large product).
@@ -57,6 +81,7 @@ __device__ __forceinline__ T kernel_arg(int offset) {
   for (unsigned i = 0; i < sizeof(T) / 4; ++i) w[i] = ((words_t)p)[i];
   T value;
   __builtin_memcpy(&value, w, sizeof(T));
+  in_global(value);
   return value;
 }
 
