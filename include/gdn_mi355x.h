@@ -636,12 +636,14 @@ int gdn_add_rms_norm(const uint16_t* x, int64_t sx, const void* residual, int64_
  *         the rows in the order of their adapters, and these
  *   lb    [slots][N, rank] bf16, slot stride lb_slot (a multiple of 8), 16-byte aligned
  * x as the GEMM's A: bf16 with K in steps of 64, or e4m3 with its scales (K in steps of
- * 128).  An adapter's rows do not change the bits of others, whatever it holds.
+ * 128).  x8 (NULL: not wanted; x bf16, K in steps of 128) takes gdn_quantize_fp8 of x, one scale for
+ * each row's group, for the product that reads e4m3 rows.  An adapter's rows do not change the bits of others, whatever it holds.
  */
 #define GDN_LORA_SORT 256
 int gdn_lora_shrink(const void* x, int x_is_bf16, int64_t ldx, const float* xs, int64_t xs_row, int64_t xs_grp,
                     const uint16_t* a, int64_t a_slot, const float* scale, const int32_t* ids, int slots, int slices,
-                    int rank, int M, int K, uint16_t* v, int64_t ldv, int32_t* groups, void* stream);
+                    int rank, int M, int K, uint16_t* v, int64_t ldv, int32_t* groups, uint8_t* x8, int64_t sx8,
+                    float* x8_scale, int64_t s8_row, int64_t s8_grp, void* stream);
 
 /* gdn_gemm_bf16_cols with the adapters' part. */
 int gdn_gemm_bf16_lora(const uint16_t* A, int64_t lda, const uint16_t* B, int64_t ldb, int M, int N, int K, int n_parts,

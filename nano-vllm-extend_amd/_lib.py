@@ -90,7 +90,7 @@ SIGNATURES: dict[str, list] = {
     "gdn_add_rms_norm": [_p, _i64, _p, _i64, _i32, _p, _p, _i32, _f32, _p, _i32, _i64, _i64, _i32, _f32, _f32, _p, _p, _p,
                          _p, _i64, _i64, _i64, _i32, _p],
     "gdn_lora_shrink": [_p, _i32, _i64, _p, _i64, _i64, _p, _i64, _p, _p, _i32, _i32, _i32, _i32, _i32, _p, _i64, _p,
-                        _p],
+                        _p, _i64, _p, _i64, _i64, _p],
     "gdn_gemm_bf16_lora": [_p, _i64, _p, _i64, _i32, _i32, _i32, _i32, _p, _p, _p, _p, _p, _p, _p, _i32, _i32, _i32, _p,
                            _i64, _p, _p, _i64, _p, _i32, _i32, _i32, _p, _p],
     "gdn_gemm_fp8_lora": [_p, _i64, _p, _i64, _i64, _p, _i64, _p, _i64, _i32, _i32, _i32, _i32, _p, _p, _p, _p, _i64, _p,

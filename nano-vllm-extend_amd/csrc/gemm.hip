@@ -907,7 +907,7 @@ __global__ __launch_bounds__(kGemmThreads) void gemm_tn_ring_kernel(const uint16
   issue(st2, wave + 2 * NW);
   if constexpr (kLora) {
     const int cb[1] = {n0};
-    lora_init<MT, 1, 4>(lo, M, N, m0, cb, lane, wave, NW,
+    lora_init<MT, 1>(lo, M, N, m0, cb, lane, wave, NW,
                        [&](int i, int, int t) -> gdn::f32x4_t& { return acc[i][t]; });
   }
   __builtin_amdgcn_s_waitcnt(kWait);
@@ -941,7 +941,7 @@ __global__ __launch_bounds__(kGemmThreads) void gemm_tn_ring_kernel(const uint16
 
 // lora_init for products of 32 x 32 x 16: 32 rows from row0 against NJ blocks of 32 columns from
 // col0, acc[j] register 4 q + r of lane (li, lg) being C[row0 + li][col0 + 32 j + 8 q + 4 lg + r].
-template <int NJ, int DEPTH, bool kSelect>
+template <int NJ, int DEPTH, int CH, bool kSelect>
 __device__ __forceinline__ void lora_pass32(const Lora& lo, int N, int mine, uint64_t all, int voff, int col0, int lane,
                                             f32x16_t (&acc)[NJ]) {
   const int li = lane & 31, lg = lane >> 5;
@@ -950,19 +950,24 @@ __device__ __forceinline__ void lora_pass32(const Lora& lo, int N, int mine, uin
     end = lora_end(lo, p);
     if (col0 >= end || col0 + 32 * NJ <= beg) continue;
     const __amdgpu_buffer_rsrc_t rv = rsrc_of(lo.v + 2 * p * lo.rank);
-    for (int c = 0; c < half; c += 2) {
-      const int q = c + lg;
-      const int off = q < half ? 0 : kNoOffset;
-      const gdn::s16x8_t vh = lora_load(rv, (voff + 16 * q) | off);
-      const gdn::s16x8_t vl = lora_load(rv, (voff + 16 * (half + q)) | off);
+    for (int c0 = 0; c0 < half; c0 += 2 * CH) {
+      gdn::s16x8_t vh[CH], vl[CH];
+      int off[CH];
+#pragma unroll
+      for (int c = 0; c < CH; ++c) {
+        const int q = c0 + 2 * c + lg;
+        off[c] = q < half ? 0 : kNoOffset;
+        vh[c] = lora_load(rv, (voff + 16 * q) | off[c]);
+        vl[c] = lora_load(rv, (voff + 16 * (half + q)) | off[c]);
+      }
       int boff[NJ];
 #pragma unroll
       for (int j = 0; j < NJ; ++j) {
         const int n = col0 + 32 * j + li;
-        boff[j] = (n * lo.rank * 2 + 16 * q) | off | (n >= beg && n < end ? 0 : kNoOffset);
+        boff[j] = (n * lo.rank * 2 + 16 * (c0 + lg)) | (n >= beg && n < end ? 0 : kNoOffset);
       }
       LoraIds it{all, 0, 1};
-      gdn::s16x8_t fb[DEPTH][NJ];
+      gdn::s16x8_t fb[DEPTH][CH][NJ];
       int sid[DEPTH];
       auto fetch = [&](int d) {
         uint64_t rows;
@@ -970,7 +975,9 @@ __device__ __forceinline__ void lora_pass32(const Lora& lo, int N, int mine, uin
         if (sid[d] < 0) return;
         const __amdgpu_buffer_rsrc_t rb = lora_b(lo, sid[d], N);
 #pragma unroll
-        for (int j = 0; j < NJ; ++j) fb[d][j] = lora_load(rb, boff[j]);
+        for (int j = 0; j < NJ; ++j)
+#pragma unroll
+          for (int c = 0; c < CH; ++c) fb[d][c][j] = lora_load(rb, (boff[j] + 32 * c) | (boff[j] & kNoOffset) | off[c]);
       };
 #pragma unroll
       for (int d = 0; d < DEPTH; ++d) fetch(d);
@@ -979,17 +986,21 @@ __device__ __forceinline__ void lora_pass32(const Lora& lo, int N, int mine, uin
         for (int d = 0; d < DEPTH; ++d) {
           if (sid[d] < 0) continue;
           const bool own = mine == sid[d];
-          const gdn::s16x8_t h = kSelect ? vh : lora_mask(vh, own), l = kSelect ? vl : lora_mask(vl, own);
 #pragma unroll
-          for (int j = 0; j < NJ; ++j) {
-            f32x16_t sum = mfma_bf16(fb[d][j], h, acc[j]);
-            sum = mfma_bf16(fb[d][j], l, sum);
-            // (slices end at multiples of 16)
-            const int cb = col0 + 32 * j;
-            const bool take0 = !kSelect || (own && cb >= beg && cb < end);
-            const bool take1 = !kSelect || (own && cb + 16 >= beg && cb + 16 < end);
+          for (int c = 0; c < CH; ++c) {
+            if (c > 0 && c0 + 2 * c >= half) continue;
+            const gdn::s16x8_t h = kSelect ? vh[c] : lora_mask(vh[c], own), l = kSelect ? vl[c] : lora_mask(vl[c], own);
 #pragma unroll
-            for (int e = 0; e < 16; ++e) acc[j][e] = (e < 8 ? take0 : take1) ? sum[e] : acc[j][e];
+            for (int j = 0; j < NJ; ++j) {
+              f32x16_t sum = mfma_bf16(fb[d][c][j], h, acc[j]);
+              sum = mfma_bf16(fb[d][c][j], l, sum);
+              // (slices end at multiples of 16)
+              const int cb = col0 + 32 * j;
+              const bool take0 = !kSelect || (own && cb >= beg && cb < end);
+              const bool take1 = !kSelect || (own && cb + 16 >= beg && cb + 16 < end);
+#pragma unroll
+              for (int e = 0; e < 16; ++e) acc[j][e] = (e < 8 ? take0 : take1) ? sum[e] : acc[j][e];
+            }
           }
           fetch(d);
         }
@@ -997,7 +1008,9 @@ __device__ __forceinline__ void lora_pass32(const Lora& lo, int N, int mine, uin
     }
   }
 }
-template <int NJ, int DEPTH>
+// B of the next adapters is on its way: of 12 / NJ of a rank up to 16 (64 rows of 41 adapters, 12352
+// columns: 16.1 us, of four 16.8), else of two, 64 values of a row of B at once: its whole line.
+template <int NJ>
 __device__ __forceinline__ void lora_init32(const Lora& lo, int M, int N, int row0, int col0, int lane,
                                             f32x16_t (&acc)[NJ]) {
   const int r = row0 + (lane & 31);
@@ -1005,7 +1018,10 @@ __device__ __forceinline__ void lora_init32(const Lora& lo, int M, int N, int ro
   const uint64_t all = __ballot(mine >= 0 && lane < 32);
   if (!all) return;
   const int voff = static_cast<int>(lora_row<true>(lo, r, M) * lo.ldv * 2);
-  lora_pass32<NJ, DEPTH, false>(lo, N, mine, all, voff, col0, lane, acc);
+  if (lo.rank <= 16)
+    lora_pass32<NJ, 12 / NJ, 1, false>(lo, N, mine, all, voff, col0, lane, acc);
+  else
+    lora_pass32<NJ, 2, 4, false>(lo, N, mine, all, voff, col0, lane, acc);
   float bad = 0.0f;
 #pragma unroll
   for (int j = 0; j < NJ; ++j)
@@ -1014,7 +1030,7 @@ __device__ __forceinline__ void lora_init32(const Lora& lo, int M, int N, int ro
   if (__builtin_expect(__any(bad != 0.0f || bad != bad), 0)) {
 #pragma unroll
     for (int j = 0; j < NJ; ++j) acc[j] = zero16();
-    lora_pass32<NJ, 1, true>(lo, N, mine, all, voff, col0, lane, acc);
+    lora_pass32<NJ, 1, 1, true>(lo, N, mine, all, voff, col0, lane, acc);
   }
 }
 
@@ -1122,7 +1138,7 @@ __global__ __launch_bounds__(kGemmThreads, 2) void gemm_tn_deep_kernel(const uin
   issue(st0, 0);
   issue(st1, 1);
   if constexpr (NS == 4) issue(st2, 2);
-  if constexpr (kLora) lora_init32<NJ, NJ == 1 ? 12 : 6>(lo, M, N, m0 + 32 * wm, n0 + (BN / 2) * wn, lane, acc[0]);
+  if constexpr (kLora) lora_init32<NJ>(lo, M, N, m0 + 32 * wm, n0 + (BN / 2) * wn, lane, acc[0]);
   // (no exit inside a trip: with one, the compiler's load counting merges its
   // states at the loop head and waits there for loads that are meant to stay
   // in flight)
@@ -1192,7 +1208,7 @@ int gemm_launch(const uint16_t* A, int64_t lda, const uint16_t* B, int64_t ldb, 
   // 4096 x 512 7.7 -> 9.7; two rounds of blocks, 400 x 12352 x 2048 35.0 -> 38.1).
   const bool blocks = !wide && t128 <= kCUs && t64x128 > kCUs && 2 * t64x128 > 3 * t128 &&
                       K * t64x128 >= 1600 * kCUs;
-  const bool fits = !kLora || lora_tiles_fit(t256);
+  const bool fits = !kLora || (lora_tiles_fit(t256) && !lora_sorted(M));
   if (K % (2 * kBK) == 0 && fits && (wide ? kLora || !one192 : blocks)) {
     const int64_t rem = t256 % kCUs;
     const int64_t whole = rem <= kCUs / 2 ? t256 - rem : t256;

@@ -879,7 +879,7 @@ __global__ __launch_bounds__(64 * NW) void gemm_fp8_ring_kernel(const void* __re
     int cb[NT];
 #pragma unroll
     for (int j = 0; j < NT; ++j) cb[j] = n0 + 32 * j;
-    lora_init<MT, NT, 4>(lo, M, N, m0, cb, lane, wave, NW,
+    lora_init<MT, NT>(lo, M, N, m0, cb, lane, wave, NW,
                         [&](int i, int j, int t) -> gdn::f32x4_t& { return acc[i][j][t]; });
   }
   __builtin_amdgcn_s_waitcnt(kWait);
@@ -1190,7 +1190,7 @@ __global__ __launch_bounds__(kFp8Threads * H, 2) void gemm_fp8_deep_kernel(const
     int cb[NJ];
 #pragma unroll
     for (int j = 0; j < NJ; ++j) cb[j] = n0 + 32 * (NJ * wn + j);
-    lora_init<2, NJ, 4>(lo, M, N, m0 + 32 * wm, cb, lane, half, H,
+    lora_init<2, NJ>(lo, M, N, m0 + 32 * wm, cb, lane, half, H,
                        [&](int i, int j, int t) -> gdn::f32x4_t& { return acc[i][j][t]; });
   }
   // (no exit inside a trip: the compiler's load counting would merge its states at the
@@ -1317,7 +1317,7 @@ int fp8_launch(Fp8Kernel kernel, const void* A, int64_t lda, const uint8_t* B, i
   auto grid = [](int64_t wgs) {
     return dim3(static_cast<unsigned>(gdn::kNumXcd * ((wgs + gdn::kNumXcd - 1) / gdn::kNumXcd)));
   };
-  if (kLora && kernel == kPP && !lora_tiles_fit(blocks(256, 256))) kernel = kDeep128;
+  if (kLora && kernel == kPP && (!lora_tiles_fit(blocks(256, 256)) || lora_sorted(M))) kernel = kDeep128;
   const uint8_t* A8 = static_cast<const uint8_t*>(A);
   const uint16_t* A16 = static_cast<const uint16_t*>(A);
   auto rows_grid = [&](int bn) { return grid(blocks(16, bn) + blocks(16, 1 << 30) * (wide.n / 16)); };

@@ -26,6 +26,7 @@
 #include <algorithm>
 
 #include "lora_tile.h"
+#include "quant_fp8.h"
 
 namespace {
 
@@ -45,6 +46,13 @@ struct Shrink {
   int64_t ldv;
   int* groups;  // [ceil(M / 16)]: the adapter of 16 rows, -1 none, -2 not one for all; up to kLoraSort rows: [M] the
                 // rows in the order of their adapters, [M] these
+  // lora_few_kernel: where x is bf16 and an 8-bit product reads it next, its e4m3 rows, by workgroups of their own
+  // behind the `share` of the adapters' (one launch less: 2.3 us)
+  uint8_t* x8;
+  int64_t sx8;
+  float* s8;
+  int64_t s8_row, s8_grp;
+  int share;
 };
 
 // 8 e4m3 values as bf16
@@ -147,11 +155,11 @@ __device__ __forceinline__ gdn::f32x4_t few_product(const Shrink& p, __amdgpu_bu
   return acc;
 }
 
-// kSort: 17 to kLoraSort rows in the order of their adapters, blockIdx.y and on every gridDim.y-th
+// kSort: 17 to kLoraSort rows in the order of their adapters, blockIdx.y and on every share-th
 // of the runs of one adapter in 16 places of that order; the order is written for the GEMM.  Every
 // workgroup finds it for itself: a row's place is the number of rows before it, counted by all
 // threads (256 rows: under 1 us, and none of it waits for memory).  Else: blockIdx.x has 16 rows and, of
-// their adapters, blockIdx.y and on every gridDim.y-th.
+// their adapters, the blockIdx.y-th and on every share-th.
 template <int NW, bool kFp8, bool kSort>
 __global__ __launch_bounds__(64 * NW) void lora_few_kernel(Shrink p) {
   constexpr int kStepBytes = kFp8 ? 6144 : 4096;
@@ -164,6 +172,13 @@ __global__ __launch_bounds__(64 * NW) void lora_few_kernel(Shrink p) {
   const int lr = lane & 15, lg = lane >> 4;
   const int tiles_n = (p.cols + 15) / 16;
   const int c0 = 16 * static_cast<int>(blockIdx.x % tiles_n), m0 = 16 * static_cast<int>(blockIdx.x / tiles_n);
+  if constexpr (!kFp8)
+    if (static_cast<int>(blockIdx.y) >= p.share) {
+      const int64_t b = static_cast<int64_t>(blockIdx.y - p.share) * gridDim.x + blockIdx.x;
+      quant_group<false>(p.x, p.ldx, p.x8, p.sx8, p.s8, p.s8_row, p.s8_grp, p.M, p.K / gdn::kFp8Group, b * (4 * NW) + tid / 16,
+                         tid % 16);
+      return;
+    }
   const __amdgpu_buffer_rsrc_t rx = rsrc_of(p.x), rs = rsrc_of(p.xs);
   // rows: the ones that the lane loads
   auto run = [&](int s, const int (&rows)[2], int row, bool own) {
@@ -227,7 +242,7 @@ __global__ __launch_bounds__(64 * NW) void lora_few_kernel(Shrink p) {
     }
     if (first) s_item[before + __builtin_popcountll(firsts & ((1ull << lane) - 1))] = tid;
     __syncthreads();
-    for (int it = blockIdx.y; it < items; it += gridDim.y) {
+    for (int it = blockIdx.y; it < items; it += p.share) {
       const int at = s_item[it], to = min(at | 15, p.M - 1);
       const int s = __builtin_amdgcn_readfirstlane(s_id[at]);
       auto has = [&](int i) { return at + i <= to && s_id[min(at + i, to)] == s; };
@@ -241,7 +256,7 @@ __global__ __launch_bounds__(64 * NW) void lora_few_kernel(Shrink p) {
     const int first = __builtin_amdgcn_readfirstlane(id);
     const bool alike = !__any(r < p.M && id != first);
     if (c0 == 0 && blockIdx.y == 0 && tid == 0) p.groups[m0 / 16] = alike ? first : -2;
-    LoraIds it{__ballot(id >= 0 && lane < 16), static_cast<int>(blockIdx.y), static_cast<int>(gridDim.y)};
+    LoraIds it{__ballot(id >= 0 && lane < 16), static_cast<int>(blockIdx.y), p.share};
     uint64_t rows;
     for (int s = it.next(id, rows); s >= 0; s = it.next(id, rows)) {
       auto row = [&](int i) { return (rows >> i) & 1 ? m0 + i : -1; };
@@ -416,15 +431,18 @@ __global__ __launch_bounds__(64 * NW) void lora_shrink_kernel(Shrink p) {
   }
 }
 
+// Rows up to which x is quantized by the same launch.
+constexpr int kFewRows = 2048;
+
 template <bool kFp8>
-int launch(const Shrink& p, hipStream_t st) {
+int launch(Shrink p, hipStream_t st) {
   auto tiles = [](int n, int of) { return (n + of - 1) / of; };
   // Prompts: 64-row tiles, all columns up to 64 (32 of them where x is e4m3: its stages are the larger ones).
   // Four waves have a CU's LDS for themselves; with more tiles than CUs two waves and a
   // half of it, so that a second tile runs beside the first.  us, four waves / two, 2048 columns of bf16 x, all rows one
   // adapter's: 17001 x 64 (266 tiles) 26.3 / 21.5, 16384 x 128 (512) 25.9 / 20.9, 16384 x 64 (256) 18.1 / 18.0, 4096 x 128
   // (128) 12.5 / 15.1; e4m3, 16384 x 64 (512) 21.2 / 17.0, 16384 x 16 (256) 11.9 / 13.7, 4096 x 128 (256) 10.9 / 13.3.
-  if (p.M > 2048) {
+  if (p.M > kFewRows) {
     const int bn = !kFp8 && p.cols > 32 ? 64 : 32, n = tiles(p.M, 64) * tiles(p.cols, bn);
     const bool two = n > gdn::kNumCu;
     // Workgroups share a tile's adapters where that leaves no more of them than find room at once (one that finds
@@ -447,9 +465,11 @@ int launch(const Shrink& p, hipStream_t st) {
   // than one round of loads
   const int n = tiles(p.cols, 16), most = std::max(1, 1024 / n);
   const bool sort = lora_sorted(p.M), wide = p.K > 2048;
-  const int share = sort ? std::min(most, std::min(p.M, tiles(p.M, 16) + std::min(p.slots, p.M)))
+  p.share = sort ? std::min(most, std::min(p.M, tiles(p.M, 16) + std::min(p.slots, p.M)))
                          : std::max(1, std::min(std::min(std::min(16, p.M), p.slots), 1024 / (n * tiles(p.M, 16))));
-  const dim3 grid(static_cast<unsigned>(sort ? n : n * tiles(p.M, 16)), static_cast<unsigned>(share));
+  const int across = sort ? n : n * tiles(p.M, 16);
+  const int64_t quant = p.x8 ? (static_cast<int64_t>(p.M) * (p.K / gdn::kFp8Group) + (wide ? 63 : 31)) / (wide ? 64 : 32) : 0;
+  const dim3 grid(static_cast<unsigned>(across), static_cast<unsigned>(p.share + (quant + across - 1) / across));
   if (sort)
     wide ? lora_few_kernel<16, kFp8, true><<<grid, dim3(1024), 0, st>>>(p)
          : lora_few_kernel<8, kFp8, true><<<grid, dim3(512), 0, st>>>(p);
@@ -464,12 +484,15 @@ int launch(const Shrink& p, hipStream_t st) {
 extern "C" int gdn_lora_shrink(const void* x, int x_is_bf16, int64_t ldx, const float* xs, int64_t xs_row, int64_t xs_grp,
                                const uint16_t* a, int64_t a_slot, const float* scale, const int32_t* ids, int slots,
                                int slices, int rank, int M, int K, uint16_t* v, int64_t ldv, int32_t* groups,
-                               void* stream) {
+                               uint8_t* x8, int64_t sx8, float* x8_scale, int64_t s8_row, int64_t s8_grp, void* stream) {
   const int64_t kLimit = 1LL << 31;
+  const hipStream_t st = static_cast<hipStream_t>(stream);
   if (M < 0 || slots < 0 || slices < 1 || slices > kMaxParts || rank < 8 || rank > kMaxRank || rank % 8 || K <= 0 ||
       K % (x_is_bf16 ? 64 : gdn::kFp8Group))
     return GDN_ERR_INVALID_ARG;
-  if (M == 0 || slots == 0) return GDN_OK;
+  if (x8 && !x_is_bf16) return GDN_ERR_INVALID_ARG;
+  if (M == 0) return GDN_OK;
+  if (slots == 0) return x8 ? gdn_quantize_fp8(x, 0, ldx, x8, sx8, x8_scale, s8_row, s8_grp, M, K, 1, stream) : GDN_OK;
   const int cols = slices * rank;
   if (!x || !a || !scale || !ids || !v || !groups || (!x_is_bf16 && !xs)) return GDN_ERR_INVALID_ARG;
   if (reinterpret_cast<uintptr_t>(x) % 16 || reinterpret_cast<uintptr_t>(a) % 16 || reinterpret_cast<uintptr_t>(v) % 8 ||
@@ -481,7 +504,13 @@ extern "C" int gdn_lora_shrink(const void* x, int x_is_bf16, int64_t ldx, const 
   if (!x_is_bf16 && (reinterpret_cast<uintptr_t>(xs) % 4 || xs_row < 0 || xs_grp < 0 ||
                      4 * ((M - 1) * xs_row + (K / gdn::kFp8Group - 1) * xs_grp) >= kLimit))
     return GDN_ERR_INVALID_ARG;
-  const Shrink p{x, ldx, xs, xs_row, xs_grp, a, a_slot, scale, ids, slots, cols, rank, M, K, v, ldv, groups};
-  const hipStream_t st = static_cast<hipStream_t>(stream);
+  if (x8 && (K % gdn::kFp8Group || !x8_scale || reinterpret_cast<uintptr_t>(x8) % 8 || sx8 % 8 || sx8 < K ||
+             reinterpret_cast<uintptr_t>(x8_scale) % 4))
+    return GDN_ERR_INVALID_ARG;
+  if (x8 && M > kFewRows) {
+    const int status = gdn_quantize_fp8(x, 0, ldx, x8, sx8, x8_scale, s8_row, s8_grp, M, K, 1, stream);
+    if (status != GDN_OK) return status;
+  }
+  const Shrink p{x, ldx, xs, xs_row, xs_grp, a, a_slot, scale, ids, slots, cols, rank, M, K, v, ldv, groups, x8, sx8, x8_scale, s8_row, s8_grp, 0};
   return x_is_bf16 ? launch<false>(p, st) : launch<true>(p, st);
 }

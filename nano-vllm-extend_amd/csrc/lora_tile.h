@@ -165,8 +165,8 @@ __device__ __forceinline__ int lora_end(const Lora& lo, int p) {
   return p == 0 ? lo.end[0] : p == 1 ? lo.end[1] : p == 2 ? lo.end[2] : lo.end[3];
 }
 
-// lora_init's products.  kSelect: the sums kept apart per row.
-template <int RT, int CT, int DEPTH, bool kSelect, class At>
+// lora_init's products, CH times 32 values of the rank at once.  kSelect: the sums kept apart per row.
+template <int RT, int CT, int DEPTH, int CH, bool kSelect, class At>
 __device__ __forceinline__ void lora_pass(const Lora& lo, int N, const int (&id)[RT], int mine, uint64_t all,
                                           const int (&voff)[RT], const int (&cb)[CT], int lane, int turn, int turns,
                                           const At& at) {
@@ -185,27 +185,31 @@ __device__ __forceinline__ void lora_pass(const Lora& lo, int N, const int (&id)
     }
     if (!any) continue;
     const __amdgpu_buffer_rsrc_t rv = rsrc_of(lo.v + 2 * p * lo.rank);
-    for (int c = 0; c < half; c += 4) {
-      const int q = c + lg;
-      const int off = q < (packed ? 2 * half : half) ? 0 : kNoOffset;  // (or'ed: no branches)
-      const int qb = packed && q >= half ? q - half : q;
-      gdn::s16x8_t vh[RT], vl[RT];
+    for (int c0 = 0; c0 < half; c0 += 4 * CH) {
+      gdn::s16x8_t vh[CH][RT], vl[CH][RT];
+      int off[CH];
 #pragma unroll
-      for (int i = 0; i < RT; ++i) vh[i] = lora_load(rv, (voff[i] + 16 * q) | off);
-      if (!packed) {
+      for (int c = 0; c < CH; ++c) {
+        const int q = c0 + 4 * c + lg;
+        off[c] = q < (packed ? 2 * half : half) ? 0 : kNoOffset;  // (or'ed: no branches)
 #pragma unroll
-        for (int i = 0; i < RT; ++i) vl[i] = lora_load(rv, (voff[i] + 16 * (half + q)) | off);
+        for (int i = 0; i < RT; ++i) vh[c][i] = lora_load(rv, (voff[i] + 16 * q) | off[c]);
+        if (!packed) {
+#pragma unroll
+          for (int i = 0; i < RT; ++i) vl[c][i] = lora_load(rv, (voff[i] + 16 * (half + q)) | off[c]);
+        }
       }
+      const int q0 = c0 + lg, qb = packed && q0 >= half ? q0 - half : q0;
       int boff[CT][2];
 #pragma unroll
       for (int j = 0; j < CT; ++j)
 #pragma unroll
         for (int t = 0; t < 2; ++t)
           // (a column of another slice: 0, as its value of v is not this slice's)
-          boff[j][t] = ((cb[j] + brow + 4 * t) * lo.rank * 2 + 16 * qb) | off |
+          boff[j][t] = ((cb[j] + brow + 4 * t) * lo.rank * 2 + 16 * qb) |
                        (cb[j] + brow + 4 * t >= beg && cb[j] + brow + 4 * t < end ? 0 : kNoOffset);
       LoraIds it{all, turn, turns};
-      gdn::s16x8_t fb[DEPTH][CT][2];
+      gdn::s16x8_t fb[DEPTH][CH][CT][2];
       int sid[DEPTH];
       uint64_t rows[DEPTH];
       auto fetch = [&](int d) {
@@ -213,10 +217,12 @@ __device__ __forceinline__ void lora_pass(const Lora& lo, int N, const int (&id)
         if (sid[d] < 0) return;
         const __amdgpu_buffer_rsrc_t rb = lora_b(lo, sid[d], N);
 #pragma unroll
-        for (int j = 0; j < CT; ++j)
+        for (int c = 0; c < CH; ++c)
 #pragma unroll
-          for (int t = 0; t < 2; ++t)
-            if (in[j]) fb[d][j][t] = lora_load(rb, boff[j][t]);
+          for (int j = 0; j < CT; ++j)
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+              if (in[j]) fb[d][c][j][t] = lora_load(rb, (boff[j][t] + 64 * c) | (boff[j][t] & kNoOffset) | off[c]);
       };
 #pragma unroll
       for (int d = 0; d < DEPTH; ++d) fetch(d);
@@ -228,19 +234,23 @@ __device__ __forceinline__ void lora_pass(const Lora& lo, int N, const int (&id)
           for (int i = 0; i < RT; ++i) {
             if (!((rows[d] >> (16 * i)) & 0xffff)) continue;
             const bool own = id[i] == sid[d];
-            const gdn::s16x8_t h = kSelect ? vh[i] : lora_mask(vh[i], own);
-            gdn::s16x8_t l;
-            if (!packed) l = kSelect ? vl[i] : lora_mask(vl[i], own);
 #pragma unroll
-            for (int j = 0; j < CT; ++j) {
-              if (!in[j]) continue;
+            for (int c = 0; c < CH; ++c) {
+              if (c > 0 && c0 + 4 * c >= half) continue;
+              const gdn::s16x8_t h = kSelect ? vh[c][i] : lora_mask(vh[c][i], own);
+              gdn::s16x8_t l;
+              if (!packed) l = kSelect ? vl[c][i] : lora_mask(vl[c][i], own);
 #pragma unroll
-              for (int t = 0; t < 2; ++t) {
-                gdn::f32x4_t& acc = at(i, j, t);
-                gdn::f32x4_t sum = gdn::mfma16x16x32(fb[d][j][t], h, acc);
-                if (!packed) sum = gdn::mfma16x16x32(fb[d][j][t], l, sum);
+              for (int j = 0; j < CT; ++j) {
+                if (!in[j]) continue;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) acc[e] = !kSelect || (own && sel[j]) ? sum[e] : acc[e];
+                for (int t = 0; t < 2; ++t) {
+                  gdn::f32x4_t& acc = at(i, j, t);
+                  gdn::f32x4_t sum = gdn::mfma16x16x32(fb[d][c][j][t], h, acc);
+                  if (!packed) sum = gdn::mfma16x16x32(fb[d][c][j][t], l, sum);
+#pragma unroll
+                  for (int e = 0; e < 4; ++e) acc[e] = !kSelect || (own && sel[j]) ? sum[e] : acc[e];
+                }
               }
             }
           }
@@ -341,13 +351,17 @@ __device__ __forceinline__ void lora_add(const Lora& lo, int M, int N, int row0,
 
 // RT tiles of 16 rows from row0 against CT blocks of 32 columns from cb[j], into accumulators
 // that are 0: at(i, j, t) is that of row tile i, block j and half t, C[row0 + 16 i + lr][cb[j] + 8
-// lg + 4 t .. + 3] in lane (lr, lg) (gemm_store16).  B of the next DEPTH adapters is on its way.
-template <int RT, int CT, int DEPTH, class At>
+// lg + 4 t .. + 3] in lane (lr, lg) (gemm_store16).  B of the next adapters is on its way: of four,
+// of ranks past 32 of two, 64 values of a row of B at once, which is its whole line.
+template <int RT, int CT, class At>
 __device__ __forceinline__ void lora_init(const Lora& lo, int M, int N, int row0, const int (&cb)[CT], int lane, int turn,
                                           int turns, const At& at) {
   const LoraRows<RT, true> r(lo, M, row0, lane);
   if (!r.all) return;
-  lora_pass<RT, CT, DEPTH, false>(lo, N, r.id, r.mine, r.all, r.voff, cb, lane, turn, turns, at);
+  if (lo.rank <= 32)
+    lora_pass<RT, CT, 4, 1, false>(lo, N, r.id, r.mine, r.all, r.voff, cb, lane, turn, turns, at);
+  else
+    lora_pass<RT, CT, 2, 2, false>(lo, N, r.id, r.mine, r.all, r.voff, cb, lane, turn, turns, at);
   float bad = 0.0f;
 #pragma unroll
   for (int i = 0; i < RT; ++i)
@@ -364,7 +378,7 @@ __device__ __forceinline__ void lora_init(const Lora& lo, int M, int N, int row0
       for (int j = 0; j < CT; ++j)
 #pragma unroll
         for (int t = 0; t < 2; ++t) at(i, j, t) = gdn::f32x4_t{0.f, 0.f, 0.f, 0.f};
-    lora_pass<RT, CT, 1, true>(lo, N, r.id, r.mine, r.all, r.voff, cb, lane, turn, turns, at);
+    lora_pass<RT, CT, 1, 1, true>(lo, N, r.id, r.mine, r.all, r.voff, cb, lane, turn, turns, at);
   }
 }
 
@@ -383,7 +397,7 @@ constexpr int kLoraMix = 6, kLoraPairs = 12, kLoraTiles = 448, kLoraMixed = 48;
 // before: 5 us a tile.)  Tile j of workgroup `slot` is number stride j + (slot + j) % stride of its
 // XCD, so that a row block's tiles go to different workgroups.
 struct LoraTiles {
-  int whole, quarters, mixed;
+  int whole, quarters;
   // code: the one adapter of all rows, kNone, or kMixed - i for entry i of mix
   int tile[kLoraTiles], code[kLoraTiles], in_quarters[kLoraTiles];
   int mix[kLoraMixed][kLoraMix + 1];  // how many, and which

@@ -635,11 +635,12 @@ struct Adapters {
       parts[i] = at::empty(shape, x.options().dtype(kBf16));
     }
   }
-  int shrink(const Tensor& x, const Tensor* xs, int64_t K, void* stream) const {
+  // x8, s8: x in e4m3 too, and its scales
+  int shrink(const Tensor& x, const Tensor* xs, int64_t K, void* stream, uint8_t* x8 = nullptr, float* s8 = nullptr) const {
     return gdn_lora_shrink(x.data_ptr(), xs ? 0 : 1, K, xs ? ptr<float>(*xs) : nullptr, xs ? xs->stride(0) : 0,
                            xs ? xs->stride(1) : 0, bf(*a), a->stride(0), ptr<float>(*scale), ptr<int32_t>(*ids),
                            static_cast<int>(S), static_cast<int>(P), static_cast<int>(R), static_cast<int>(M),
-                           static_cast<int>(K), v(), ldv(), groups(), stream);
+                           static_cast<int>(K), v(), ldv(), groups(), x8, K, s8, 1, M, stream);
   }
   PyObject* given(PyObject* widths) {
     if (widths == Py_None) return THPVariable_Wrap(std::move(parts[0]));
@@ -704,16 +705,14 @@ PyObject* linear_fp8_lora(PyObject*, PyObject* const* a, Py_ssize_t n) {
     uint16_t* c[4];
     for (int i = 0; i < l.n; ++i) c[i] = bf(l.parts[i]);
     void* stream = t.stream();
-    if (failed("gdn_lora_shrink", l.shrink(x, xs, K, stream))) return nullptr;
     Tensor x8, made;
     if (!ready) {
       x8 = at::empty({M, K}, x.options().dtype(kFp8));
       made = at::empty_strided({M, G}, {1, M}, x.options().dtype(kF32));
-      if (failed("gdn_quantize_fp8", gdn_quantize_fp8(x.data_ptr(), 0, K, ptr<uint8_t>(x8), K, ptr<float>(made), 1, M, M,
-                                                       static_cast<int>(K), 1, stream)))
-        return nullptr;
-      xs = &made;
     }
+    const int shrunk = ready ? l.shrink(x, xs, K, stream) : l.shrink(x, nullptr, K, stream, ptr<uint8_t>(x8), ptr<float>(made));
+    if (failed("gdn_lora_shrink", shrunk)) return nullptr;
+    if (!ready) xs = &made;
     const int status = gdn_gemm_fp8_lora(
         ptr<uint8_t>(ready ? x : x8), K, ptr<float>(*xs), xs->stride(0), xs->stride(1), ptr<uint8_t>(w), w.stride(0),
         ptr<float>(ws), G, static_cast<int>(M), static_cast<int>(N), static_cast<int>(K), l.n, c, l.width, l.end, l.v(),

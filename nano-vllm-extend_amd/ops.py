@@ -1609,15 +1609,16 @@ def _lora_check(x, N, K, widths, lora_a, lora_b, lora_scale, ids):
     return M, P, R
 
 
-def _lora_shrink(idx, rows, stride, x_scale, lora_a, lora_scale, ids, M, K, P, R):
+def _lora_shrink(idx, rows, stride, x_scale, lora_a, lora_scale, ids, M, K, P, R, x8=None, x8_scale=None):
     """(v [M, P, 2, R] of the rows with an adapter, the adapters of their groups of 16 and, of few
-    rows, their order)."""
+    rows, their order); x8 and its scales [M, K / 128] take quantize_fp8 of the rows."""
     v = torch.empty(M, P * 2 * R, dtype=torch.bfloat16, device=rows.device)
     groups = torch.empty(-(-M // 16) + (2 * M if M <= LORA_SORT else 0), dtype=torch.int32, device=rows.device)
     xs = (0, 0, 0) if x_scale is None else (x_scale.data_ptr(), *x_scale.stride())
+    to = (0, K, 0, 0, 0) if x8 is None else (x8.data_ptr(), K, x8_scale.data_ptr(), *x8_scale.stride())
     _call_on(idx, "gdn_lora_shrink", rows.data_ptr(), int(x_scale is None), stride, *xs, lora_a.data_ptr(),
              lora_a.stride(0), lora_scale.data_ptr(), ids.data_ptr(), lora_a.shape[0], P, R, M, K, v.data_ptr(), 2 * P * R,
-             groups.data_ptr())
+             groups.data_ptr(), *to)
     return v, groups
 
 
@@ -1744,12 +1745,14 @@ def linear_fp8_lora(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.T
     if not weight_scale.is_contiguous():
         weight_scale = weight_scale.contiguous()
     outs = [torch.empty(M, w, dtype=torch.bfloat16, device=x.device) for w in parts]
-    shrunk = v, groups = _lora_shrink(idx, rows, stride, x_scale, lora_a, lora_scale, ids, M, K, P, R)
     x8, x8_stride, xs = rows, stride, x_scale
     if x_scale is None:
         x8 = torch.empty(M, K, dtype=FP8, device=x.device)
         xs, x8_stride = _fp8_scales(M, G, x.device), K
-        _call_on(idx, "gdn_quantize_fp8", rows.data_ptr(), 0, stride, x8.data_ptr(), K, xs.data_ptr(), 1, M, M, K, 1)
+        shrunk = _lora_shrink(idx, rows, stride, None, lora_a, lora_scale, ids, M, K, P, R, x8, xs)
+    else:
+        shrunk = _lora_shrink(idx, rows, stride, x_scale, lora_a, lora_scale, ids, M, K, P, R)
+    v, groups = shrunk
     c, ld, ends, slice_ends = _tables(outs[:n], parts[:n], parts[:n])
     with torch.cuda.device(idx):
         _lib.call("gdn_gemm_fp8_lora", x8.data_ptr(), x8_stride, xs.data_ptr(), *xs.stride(), weight.data_ptr(),

@@ -415,3 +415,24 @@ def test_rows_in_the_order_of_their_adapters(pkg, dev, M, N, S, how, fp8):
         assert torch.equal(y2, y)
         eg, eb = pkg.fused_g_beta(y[:, 64:80].contiguous(), y[:, 80:].contiguous(), gates["A_log"], gates["dt_bias"], None)
         assert torch.equal(g, eg) and torch.equal(beta, eb)
+
+
+@pytest.mark.parametrize("M", [1, 40, 300, 2500])
+def test_no_slots_and_the_rows_quantized_on_the_way(pkg, dev, M):
+    """A pool without slots: the products alone, bit for bit, bf16 rows for 8-bit weights quantized all the same;
+    and the e4m3 rows that come out of the adapters' launch are quantize_fp8's."""
+    gen = torch.Generator().manual_seed(M)
+    N, K, R = 96, 384, 16
+    x = torch.randn(M, K, generator=gen).to(BF16).to(dev)
+    w = (torch.randn(N, K, generator=gen) * K ** -0.5).to(BF16).to(dev)
+    w8, ws = pkg.quantize_weight_fp8(w)
+    empty = pkg.LoraPool(0, R, K, [N], dev)
+    ids = torch.zeros(M, dtype=torch.int32, device=dev)
+    assert torch.equal(pkg.linear_lora(x, w, empty.a, empty.b, empty.scale, ids), pkg.linear(x, w))
+    assert torch.equal(pkg.linear_fp8_lora(x, w8, ws, empty.a, empty.b, empty.scale, ids), pkg.linear_fp8(x, w8, ws))
+    a, b, scale = (t.to(dev) for t in _adapters(gen, 2, [N], K, R))
+    x8, xs = pkg.quantize_fp8(x)
+    to, to_s = torch.zeros_like(x8), torch.zeros_like(xs)
+    v, _ = pkg.ops._lora_shrink(dev.index or 0, x, K, None, a, scale, ids, M, K, 1, R, to, to_s)
+    alone, _ = pkg.ops._lora_shrink(dev.index or 0, x, K, None, a, scale, ids, M, K, 1, R)
+    assert torch.equal(to.view(torch.uint8), x8.view(torch.uint8)) and torch.equal(to_s, xs) and torch.equal(v, alone)

@@ -129,7 +129,7 @@ def test_c_entries_refuse(pkg):
     assert norm() == bad and norm(M=-1) == bad and norm(H=0) == bad and norm(g_col=2) == bad
     assert norm(H=16385) == pkg._lib.GDN_ERR_UNSUPPORTED and norm(M=0) == 0
     shrink = lambda slots=2, slices=1, rank=16, M=4, K=128: lib.gdn_lora_shrink(  # noqa: E731
-        None, 1, K, None, 0, 0, None, 0, None, None, slots, slices, rank, M, K, None, 32, None, None)
+        None, 1, K, None, 0, 0, None, 0, None, None, slots, slices, rank, M, K, None, 32, None, None, 0, None, 0, 0, None)
     for kw in (dict(), dict(slots=-1), dict(slices=0), dict(slices=5), dict(rank=12), dict(rank=264), dict(rank=0), dict(K=96),
                dict(M=-1), dict(K=0)):
         assert shrink(**kw) == bad, kw
@@ -148,6 +148,12 @@ def test_c_entries_refuse(pkg):
         return lib.gdn_gemm_fp8_lora(P, K, P, 1, M, P, K, P, 1, M, N, K, len(ends), *parts, n(*ends), v, ldv, groups, lb, lb_slot, ids,
                                      slots, rank, len(slice_ends), n(*slice_ends), None)
 
+    def shrink(x_is_bf16=1, M=4, K=128, x8=P, sx8=128, s8=P, ids=P):
+        return lib.gdn_lora_shrink(P, x_is_bf16, K, P, 1, M, P, 16 * K, P, ids, 2, 1, 16, M, K, P, 32, P, x8, sx8, s8, 1, M, None)
+
+    for kw in (dict(x_is_bf16=0), dict(K=64), dict(x8=ctypes.c_void_p((1 << 20) + 4)), dict(sx8=120), dict(sx8=132), dict(s8=None),
+               dict(s8=ctypes.c_void_p((1 << 20) + 2)), dict(ids=None)):
+        assert shrink(**kw) == bad, kw
     odd, byte = ctypes.c_void_p((1 << 20) + 2), ctypes.c_void_p((1 << 20) + 1)
     for call in (bf16, fp8):
         for kw in (dict(v=None), dict(v=odd), dict(groups=None), dict(groups=byte), dict(lb=None), dict(lb=odd), dict(ids=None), dict(ids=odd), dict(slots=-1),
