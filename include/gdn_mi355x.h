@@ -632,7 +632,7 @@ int gdn_add_rms_norm(const uint16_t* x, int64_t sx, const void* residual, int64_
  *   v     [M, slices, 2, rank] bf16, row stride ldv (a multiple of 8), 16-byte aligned: each value as the sum
  *         of two.  Rows without an adapter are not written, and count for nothing in what follows
  *   groups int32 [ceil(M / 16)], written by the first call for the second: the adapter of 16
- *         rows (-1: none of them has one, -2: they differ); with 16 < M <= GDN_LORA_SORT 2 M more:
+ *         rows (-1: none of them has one, -2: they differ); with M <= GDN_LORA_SORT 2 M more:
  *         the rows in the order of their adapters, and these
  *   lb    [slots][N, rank] bf16, slot stride lb_slot (a multiple of 8), 16-byte aligned
  * x as the GEMM's A: bf16 with K in steps of 64, or e4m3 with its scales (K in steps of

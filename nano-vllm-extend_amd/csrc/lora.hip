@@ -158,12 +158,12 @@ __device__ __forceinline__ gdn::f32x4_t few_product(const Shrink& p, __amdgpu_bu
 // kSort: 17 to kLoraSort rows in the order of their adapters, blockIdx.y and on every share-th
 // of the runs of one adapter in 16 places of that order; the order is written for the GEMM.  Every
 // workgroup finds it for itself: a row's place is the number of rows before it, counted by all
-// threads (256 rows: under 1 us, and none of it waits for memory).  Else: blockIdx.x has 16 rows and, of
+// threads (256 rows: 1 us, and none of it waits for memory).  Else: blockIdx.x has 16 rows and, of
 // their adapters, the blockIdx.y-th and on every share-th.
 template <int NW, bool kFp8, bool kSort>
 __global__ __launch_bounds__(64 * NW) void lora_few_kernel(Shrink p) {
   constexpr int kStepBytes = kFp8 ? 6144 : 4096;
-  __shared__ __align__(16) int key[kLoraSort];
+  __shared__ __align__(16) unsigned key[kLoraSort];
   __shared__ int place[kLoraSort], s_row[kLoraSort], s_id[kLoraSort], s_item[kLoraSort], s_count[4];
   __shared__ __align__(16) uint8_t steps[NW * kStepBytes];
   gdn::f32x4_t* red = reinterpret_cast<gdn::f32x4_t*>(steps);
@@ -197,27 +197,33 @@ __global__ __launch_bounds__(64 * NW) void lora_few_kernel(Shrink p) {
     __syncthreads();
   };
   if constexpr (kSort) {
-    const int P = p.M <= 64 ? 64 : p.M <= 128 ? 128 : 256, span = P * P / (64 * NW);  // keys to a thread
+    // a row's key: its adapter (0: none) and its number; the keys of P rows, T / P parts of them to a row
+    const int P = p.M <= 64 ? 64 : p.M <= 128 ? 128 : 256, parts = 64 * NW / P;
     if (tid < P) {
       const int s = p.ids[min(tid, p.M - 1)];
-      key[tid] = tid >= p.M ? 0x7fffffff : static_cast<unsigned>(s) < static_cast<unsigned>(p.slots) ? s : -1;
+      const unsigned id = static_cast<unsigned>(s) < static_cast<unsigned>(p.slots) ? s + 1 : 0;
+      key[tid] = tid < p.M ? id * kLoraSort + tid : ~0u;
       place[tid] = 0;
     }
     __syncthreads();
-    const int m = tid & (P - 1), mine = key[m];
+    const int m = tid & (P - 1), per = (p.M + 4 * parts - 1) / (4 * parts);
+    const unsigned own_key = key[m];
+    const int mine = static_cast<int>(own_key / kLoraSort) - 1;
     if (m < p.M) {
-      const int from = __builtin_amdgcn_readfirstlane(tid / P * span);
       int count = 0;
-      for (int j = from; j < from + span; j += 4) {
-        const int4 k = *reinterpret_cast<const int4*>(key + j);
-        count += k.x < mine + (j < m) ? 1 : 0;
-        count += k.y < mine + (j + 1 < m) ? 1 : 0;
-        count += k.z < mine + (j + 2 < m) ? 1 : 0;
-        count += k.w < mine + (j + 3 < m) ? 1 : 0;
+      const uint4* keys = reinterpret_cast<const uint4*>(key);
+      const int from = __builtin_amdgcn_readfirstlane(tid / P * per), to = min(from + per, P / 4);
+#pragma unroll 8
+      for (int j = from; j < to; ++j) {
+        const uint4 k = keys[j];
+        count += k.x < own_key ? 1 : 0;
+        count += k.y < own_key ? 1 : 0;
+        count += k.z < own_key ? 1 : 0;
+        count += k.w < own_key ? 1 : 0;
       }
       atomicAdd(&place[m], count);
     }
-    const uint64_t differ = __ballot(m < p.M && mine != key[m & ~15]);
+    const uint64_t differ = __ballot(m < p.M && mine != static_cast<int>(key[m & ~15] / kLoraSort) - 1);
     __syncthreads();
     if (tid < p.M) {
       s_row[place[tid]] = tid;
@@ -256,9 +262,12 @@ __global__ __launch_bounds__(64 * NW) void lora_few_kernel(Shrink p) {
     const int first = __builtin_amdgcn_readfirstlane(id);
     const bool alike = !__any(r < p.M && id != first);
     if (c0 == 0 && blockIdx.y == 0 && tid == 0) p.groups[m0 / 16] = alike ? first : -2;
-    LoraIds it{__ballot(id >= 0 && lane < 16), static_cast<int>(blockIdx.y), p.share};
+    LoraIds it{__ballot(id >= 0 && lane < 16), 0, 1};
     uint64_t rows;
+    int turn = static_cast<int>(blockIdx.y);
     for (int s = it.next(id, rows); s >= 0; s = it.next(id, rows)) {
+      if (turn-- > 0) continue;
+      turn = p.share - 1;
       auto row = [&](int i) { return (rows >> i) & 1 ? m0 + i : -1; };
       const int mine[2] = {row(lane >> 3), row(8 + (lane >> 3))};
       run(s, mine, min(r, p.M - 1), id == s);
@@ -463,8 +472,8 @@ int launch(Shrink p, hipStream_t st) {
   }
   // so many workgroups share the adapters (those that find none end); 16 waves where 8 would have more
   // than one round of loads
-  const int n = tiles(p.cols, 16), most = std::max(1, 1024 / n);
-  const bool sort = lora_sorted(p.M), wide = p.K > 2048;
+  const int n = tiles(p.cols, 16), most = std::max(1, 512 / n);
+  const bool sort = lora_sorted(p.M, p.slots), wide = p.K > 2048;
   p.share = sort ? std::min(most, std::min(p.M, tiles(p.M, 16) + std::min(p.slots, p.M)))
                          : std::max(1, std::min(std::min(std::min(16, p.M), p.slots), 1024 / (n * tiles(p.M, 16))));
   const int across = sort ? n : n * tiles(p.M, 16);

@@ -23,9 +23,11 @@ constexpr int kMaxRank = 256;
 // Up to so many rows, and more than one tile's, are sorted by their adapters (lora.hip), and the kernels
 // of few rows take them in that order.  200 rows of 32 adapters at random, 12352 columns of e4m3 x 2048, rank 32: 32 us,
 // as they come 42.  (One tile's have nothing to gain: 1 row 16.0 us, sorted 17.3.  The counting grows
-// with the square of the rows: 512 would take 3 us of every workgroup.)
+// with the square of the rows: 1.3 us for 256, 5 for 512.)
 constexpr int kLoraSort = GDN_LORA_SORT;
-__host__ __device__ constexpr bool lora_sorted(int M) { return M > 16 && M <= kLoraSort; }
+__host__ __device__ constexpr bool lora_sorted(int M, int slots) {
+  return M > 16 && M <= kLoraSort && slots < (1 << 23);  // (an adapter and a row in 32 bits)
+}
 
 struct Lora {
   const uint16_t* v;    // [M, slices, 2, rank] bf16, row stride ldv
@@ -568,7 +570,7 @@ bool lora_of(Lora& lo, const uint16_t* v, int64_t ldv, const int* groups, const 
       b_slot % 8 || (slots > 1 && b_slot < static_cast<int64_t>(N) * rank) ||
       static_cast<int64_t>(N + 256) * rank * 2 >= kLimit)
     return false;
-  lo = Lora{v, ldv, b, b_slot, ids, groups, lora_sorted(M) ? groups + (M + 15) / 16 : nullptr, slots, rank, slices, {N, N, N, N}};
+  lo = Lora{v, ldv, b, b_slot, ids, groups, lora_sorted(M, slots) ? groups + (M + 15) / 16 : nullptr, slots, rank, slices, {N, N, N, N}};
   for (int p = 0, beg = 0; p < slices; beg = slice_end[p++]) {
     const bool last = p + 1 == slices;
     if (slice_end[p] <= beg || (last ? slice_end[p] != N : slice_end[p] % 16 != 0 || slice_end[p] >= N)) return false;
