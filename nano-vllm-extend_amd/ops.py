@@ -1793,6 +1793,10 @@ def add_rms_norm(x: torch.Tensor, residual: torch.Tensor | None, weight: torch.T
     returned.
     Reference: _gemma_rms_forward, _gemma_add_rms_forward,
     nanovllm/models/qwen3_5.py:99-118 (x and residual alone)."""
+    if residual_out is None:
+        out = _lib.quick().add_norm(x, residual, weight, eps, post_weight, gate, gate_sigmoid, scale, offset, True, False)
+        if out is not None:
+            return out[0], out[3]
     y, _, _, r = _add_rms_norm(x, residual, weight, eps, post_weight, gate, gate_sigmoid, scale, offset, residual_out,
                                True, False)
     return y, r
@@ -1806,16 +1810,15 @@ def add_rms_norm_fp8(x: torch.Tensor, residual: torch.Tensor | None, weight: tor
     of the fp32 values, rounded once (H a multiple of 128).  Returns (y8 [..., H], its
     scales [rows, H / 128], r), with keep also the bf16 y (for what reads the same rows in
     bf16: the layer's gate projections)."""
-    y, y8, y_scale, r = _add_rms_norm(x, residual, weight, eps, post_weight, gate, gate_sigmoid, scale, offset,
-                                      residual_out, keep, True)
+    out = None
+    if residual_out is None:
+        out = _lib.quick().add_norm(x, residual, weight, eps, post_weight, gate, gate_sigmoid, scale, offset, bool(keep), True)
+    y, y8, y_scale, r = out or _add_rms_norm(x, residual, weight, eps, post_weight, gate, gate_sigmoid, scale, offset,
+                                             residual_out, keep, True)
     return (y8, y_scale, r, y) if keep else (y8, y_scale, r)
 
 
 def _add_rms_norm(x, residual, weight, eps, post_weight, gate, gate_sigmoid, scale, offset, residual_out, bf16, fp8):
-    if residual_out is None:
-        out = _lib.quick().add_norm(x, residual, weight, eps, post_weight, gate, gate_sigmoid, scale, offset, bf16, fp8)
-        if out is not None:
-            return out
     idx = _device_of(x, residual, weight, post_weight, gate, residual_out)
     _bf16(x, "x")
     if x.dim() < 1:
