@@ -1575,10 +1575,14 @@ class LoraPool:
 
 def adapter_rows(adapters: torch.Tensor, cu_seqlens: torch.Tensor, rows: int) -> torch.Tensor:
     """The adapter of each of `rows` rows, int32 [rows], from those of the sequences,
-    adapters [n] (-1: none), and the sequences' offsets cu_seqlens [n + 1] (device; the
-    last one is `rows`): once per step, for all of its layers."""
-    lens = cu_seqlens[1:] - cu_seqlens[:-1]
-    return adapters.to(torch.int32).repeat_interleave(lens, output_size=rows)
+    adapters [n] (-1: none), and the sequences' offsets cu_seqlens [n + 1] on the same
+    device: once per step, for all of its layers.  Rows behind the last sequence have none."""
+    if adapters.dim() != 1 or cu_seqlens.shape != (adapters.shape[0] + 1,) or adapters.device != cu_seqlens.device:
+        raise ValueError(f"adapters [n] and cu_seqlens [n + 1] on one device, got {list(adapters.shape)} on {adapters.device} "
+                         f"and {list(cu_seqlens.shape)} on {cu_seqlens.device}")
+    at = torch.searchsorted(cu_seqlens[1:].contiguous(), torch.arange(rows, dtype=cu_seqlens.dtype, device=adapters.device),
+                            right=True)
+    return torch.cat([adapters.to(torch.int32), adapters.new_full((1,), -1, dtype=torch.int32)])[at]
 
 
 def _lora_check(x, N, K, widths, lora_a, lora_b, lora_scale, ids):

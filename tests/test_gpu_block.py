@@ -300,3 +300,28 @@ def test_adapters_refused(pkg, dev):
     for norms in ((torch.zeros(64), torch.zeros(128)), (torch.zeros(128), torch.zeros(1, 128))):
         with pytest.raises(ValueError):
             pkg.GatedDeltaNetBlock(layer, *norms)
+
+
+@pytest.mark.parametrize("lens", [[1, 1, 40, 300], [700, 600, 50]], ids=["mixed", "prompts"])
+def test_block_with_gates_from_the_product(pkg, dev, lens):
+    """8-bit weights and a path that takes its gates from in_proj: the e4m3 rows of the first norm give
+    the same gates as its bf16 rows."""
+    gen = torch.Generator().manual_seed(96)
+    Hk, Hv, D, hidden = 8, 16, 128, 512
+    layer, _ = _layer(pkg, dev, gen, hidden, Hk, Hv, D, "fp8", switches=pkg.Switches(fused_prefill=False, fused_decode=False))
+    assert layer.gates_in_gemm()
+    n1, n2 = ((torch.randn(hidden, generator=gen) * 0.1).to(BF16).to(dev) for _ in range(2))
+    block = pkg.GatedDeltaNetBlock(layer, n1, n2)
+    N, cu, ids = sum(lens), _cu(lens, dev), torch.tensor([4, 1, 6, 0][:len(lens)], device=dev)
+    x, res = (torch.randn(N, hidden, generator=gen).to(BF16).to(dev) for _ in range(2))
+    conv0, s0 = _state(pkg, dev, gen, layer, 8)
+    pools = [conv0.clone(), s0.clone()], [conv0.clone(), s0.clone()]
+    y, stream = block.forward(x, res, cu, max(lens), ids, *pools[0], lens_q=lens)
+    y8, scale, r, h = pkg.add_rms_norm_fp8(x, res, n1, 1e-6, keep=True)
+    rows = layer.project_in(h, gates=True, fp8=(y8, scale) if N > 1024 else None)
+    g, beta = pkg.fused_g_beta(rows[2].contiguous(), rows[3].contiguous(), layer.core.A_log, layer.core.dt_bias, None)
+    assert torch.equal(rows[4][0], g) and torch.equal(rows[4][1], beta)
+    core = layer.core.forward(*(t.contiguous() for t in rows[:4]), cu, max(lens), ids, *pools[1], lens_q=lens, gb=rows[4],
+                              fp8=True)
+    want = pkg.add_rms_norm(layer._project_out(core, x.shape), r, n2, 1e-6)
+    assert torch.equal(y, want[0]) and torch.equal(stream, want[1]) and all(torch.equal(p, q) for p, q in zip(*pools))

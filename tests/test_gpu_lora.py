@@ -436,3 +436,61 @@ def test_no_slots_and_the_rows_quantized_on_the_way(pkg, dev, M):
     v, _ = pkg.ops._lora_shrink(dev.index or 0, x, K, None, a, scale, ids, M, K, 1, R, to, to_s)
     alone, _ = pkg.ops._lora_shrink(dev.index or 0, x, K, None, a, scale, ids, M, K, 1, R)
     assert torch.equal(to.view(torch.uint8), x8.view(torch.uint8)) and torch.equal(to_s, xs) and torch.equal(v, alone)
+
+
+def test_slots_past_32_bits(pkg, dev):
+    """Slots whose offsets pass 2^32 bytes, of A and of B: the same bits as from a pool of two.  (Which wave adds
+    an adapter goes by its slot's number modulo 8 at most: 8 for 0 and 33 for 1.)"""
+    gen = torch.Generator().manual_seed(53)
+    N, K, R, S = 384, 128, 16, 34
+    two = _adapters(gen, 2, [N], K, R)
+    far = [torch.empty(S, 1 << 26, dtype=BF16, device=dev) for _ in range(2)]
+    views = [t.as_strided((S, *s.shape[1:]), (1 << 26, s.shape[2], 1)) for t, s in zip(far, two)]
+    for t, s in zip(views, two):
+        t[8].copy_(s[0])
+        t[33].copy_(s[1])
+    scale = torch.zeros(S, device=dev)
+    scale[8], scale[33] = two[2][0], two[2][1]
+    near = [t.to(dev) for t in two]
+    assert 33 * (2 << 26) > 1 << 32
+    for M in (1, 20, 300, 2500, 5000):
+        x = torch.randn(M, K, generator=gen).to(BF16).to(dev)
+        w = torch.randn(N, K, generator=gen).to(BF16).to(dev)
+        ids = torch.randint(0, 2, (M,), generator=gen).sort().values.to(torch.int32).to(dev)
+        moved = torch.where(ids == 0, 8, 33).to(torch.int32)
+        assert torch.equal(pkg.linear_lora(x, w, *views, scale, moved), pkg.linear_lora(x, w, *near, ids)), M
+        w8, ws = pkg.quantize_weight_fp8(w)
+        assert torch.equal(pkg.linear_fp8_lora(x, w8, ws, *views, scale, moved), pkg.linear_fp8_lora(x, w8, ws, *near, ids)), M
+
+
+def test_two_streams_at_once(pkg, dev):
+    """Calls that overlap on two streams, and two graphs replayed in turn and at once: each has rows of its own."""
+    gen = torch.Generator().manual_seed(59)
+    N, K, R, S = 2048, 1024, 16, 8
+    w = torch.randn(N, K, generator=gen).to(BF16).to(dev)
+    lora = [t.to(dev) for t in _adapters(gen, S, [N], K, R)]
+    sides = [torch.cuda.Stream(dev) for _ in range(2)]
+    for M in (37, 3000):
+        xs = [torch.randn(M, K, generator=gen).to(BF16).to(dev) for _ in range(2)]
+        ids = [_ids(gen, M, S, how).to(dev) for how in ("mixed", "sequences")]
+        want = [pkg.linear_lora(x, w, *lora, i) for x, i in zip(xs, ids)]
+        torch.cuda.synchronize()
+        for _ in range(5):
+            got = []
+            for side, x, i in zip(sides, xs, ids):
+                with torch.cuda.stream(side):
+                    got.append(pkg.linear_lora(x, w, *lora, i))
+            torch.cuda.synchronize()
+            assert all(torch.equal(a, b) for a, b in zip(got, want))
+        graphs, out = [], []
+        for x, i in zip(xs, ids):
+            graphs.append(torch.cuda.CUDAGraph())
+            with torch.cuda.graph(graphs[-1]):
+                out.append(pkg.linear_lora(x, w, *lora, i))
+        for _ in range(3):
+            for side, g, y in zip(sides, graphs, out):
+                with torch.cuda.stream(side):
+                    y.zero_()
+                    g.replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(a, b) for a, b in zip(out, want))

@@ -188,3 +188,14 @@ def test_quick_calls_leave_the_rest_to_the_wrappers(pkg):
             with pytest.raises(TypeError):
                 call(*[t] * wrong)
     assert quick.add_norm(t, t, f, 1e-6, None, None, False, 1.0, 1.0, True, False) is None   # (not on the device)
+
+
+def test_adapter_rows(pkg):
+    """Each row its sequence's adapter, empty sequences none of them; rows behind the last one none."""
+    cu = torch.tensor([0, 3, 3, 4, 9], dtype=I32)
+    got = pkg.adapter_rows(torch.tensor([5, 7, -1, 2]), cu, 11)
+    assert got.dtype == I32 and got.tolist() == [5, 5, 5, -1, 2, 2, 2, 2, 2, -1, -1]
+    assert pkg.adapter_rows(torch.zeros(0, dtype=I32), cu[:1], 2).tolist() == [-1, -1]
+    for bad in ((torch.zeros(3), cu), (torch.zeros(4, 1), cu), (torch.zeros(4), cu[None])):
+        with pytest.raises(ValueError):
+            pkg.adapter_rows(*bad, 9)
