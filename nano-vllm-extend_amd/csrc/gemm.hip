@@ -495,7 +495,8 @@ __global__ __launch_bounds__(kPPThreads, 2) void gemm_tn_pp_kernel(const uint16_
       for (int ks = 0; ks < 2; ++ks)
         f[t][ks] = *reinterpret_cast<const frag_t*>(h + swb_off(32 * wn + 8 * (lr >> 2) + 4 * t + (lr & 3), 4 * ks + lg));
   };
-  int lora_lo = 0;  // (kLora) bytes to the low parts in a row of v
+  int lora_lo = 0;        // (kLora) bytes to the low parts in a row of v; 0: none in the second step
+  bool lora_all = false;  // a step's second half has values
   gdn::f32x4_t acc[2][2][4][2];  // [row half][column half][16-row tile][column tile]
   // one row half of A against both column halves of B
   auto prod = [&](gdn::f32x4_t (&c0)[4][2], gdn::f32x4_t (&c1)[4][2], const frag_t (&fa)[4][2],
@@ -515,9 +516,9 @@ __global__ __launch_bounds__(kPPThreads, 2) void gemm_tn_pp_kernel(const uint16_
     __builtin_amdgcn_s_setprio(0);
     half_barrier();
   };
-  // the same of the adapters' steps: of ranks up to 32 the first half of a step
+  // the same of the adapters' steps, if there is any of it
   auto prod_lora = [&](gdn::f32x4_t (&c0)[4][2], gdn::f32x4_t (&c1)[4][2], const frag_t (&fa)[4][2],
-                       const frag_t (&f0)[2][2], const frag_t (&f1)[2][2]) {
+                       const frag_t (&f0)[2][2], const frag_t (&f1)[2][2], bool any) {
     if constexpr (kLora) {
       auto half = [&](int ks) {
 #pragma unroll
@@ -528,8 +529,8 @@ __global__ __launch_bounds__(kPPThreads, 2) void gemm_tn_pp_kernel(const uint16_
             c1[i][t] = gdn::mfma16x16x32(f1[t][ks], fa[i][ks], c1[i][t]);
           }
       };
-      half(0);
-      if (lora_lo > 64) half(1);
+      if (any) half(0);
+      if (any && lora_all) half(1);
       half_barrier();
     }
   };
@@ -564,7 +565,7 @@ __global__ __launch_bounds__(kPPThreads, 2) void gemm_tn_pp_kernel(const uint16_
   auto set_lora_offsets = [&](int e, int m, int n) {
     if constexpr (kLora) {
       const Lora lo = kernel_arg<Lora>(kLoraAt);
-      lora_offsets(lo, lt, lora_pair(tiles_l, lo, lt, e, N, n), M, N, m, n, wave, new_lane(), va, vb, na, nb, lora_lo);
+      lora_offsets(lo, lt, lora_pair(tiles_l, lo, lt, e, N, n), M, N, m, n, wave, new_lane(), va, vb, na, nb, lora_lo, lora_all);
     }
   };
   int at = 0;
@@ -657,25 +658,27 @@ __global__ __launch_bounds__(kPPThreads, 2) void gemm_tn_pp_kernel(const uint16_
         read_a(a00, fa);
         read_b(b01, fb1);
         mem_end();
-        prod_lora(acc[0][0], acc[0][1], fa, fb0, fb1);
+        prod_lora(acc[0][0], acc[0][1], fa, fb0, fb1, true);
         dma(ra_n, a00, va[0], 0);
         dma(rb_n, b01, vb[1], 0);
         read_a(a01, fa);
-        read_b(b10, fbn);
+        if (lora_lo) read_b(b10, fbn);
         mem_end();
-        prod_lora(acc[1][0], acc[1][1], fa, fb0, fb1);
+        prod_lora(acc[1][0], acc[1][1], fa, fb0, fb1, true);
         dma(rb_n, b10, vb[0], k3b);
         dma(ra_n, a01, va[1], 0);
-        read_a(a10, fa);
-        read_b(b11, fb1);
+        if (lora_lo) {
+          read_a(a10, fa);
+          read_b(b11, fb1);
+        }
         mem_end();
-        prod_lora(acc[0][0], acc[0][1], fa, fbn, fb1);
+        prod_lora(acc[0][0], acc[0][1], fa, fbn, fb1, lora_lo);
         dma(ra_n, a10, va[0], k3a);
         dma(rb_n, b11, vb[1], k3b);
-        read_a(a11, fa);
+        if (lora_lo) read_a(a11, fa);
         read_b(b00, fb0);
         mem_end();
-        prod_lora(acc[1][0], acc[1][1], fa, fbn, fb1);
+        prod_lora(acc[1][0], acc[1][1], fa, fbn, fb1, lora_lo);
       }
       if (lt.part) {
         float bad = 0.0f;

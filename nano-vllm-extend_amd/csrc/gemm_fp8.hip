@@ -272,20 +272,23 @@ __global__ __launch_bounds__(kPPThreads, 2) void gemm_fp8_pp_kernel(const uint8_
     // (kLora) the pairs of bf16 steps behind K, as in the bf16 GEMM: v's rows and the adapters' B in
     // A's and B's place, 64 values of a row in its 128 bytes
     LoraBase na(A), nb(B);
-    int lora_lo = 0;  // bytes to the low parts in a row of v
+    int lora_lo = 0;        // bytes to the low parts in a row of v; 0: none in the second step
+    bool lora_all = false;  // a step's second half has values
     LoraSteps lt{LoraTiles::kNone, 0, false};
     auto set_lora_offsets = [&](int e, int m, int n) {
       if constexpr (kLora) {
         const Lora lo = kernel_arg<Lora>(kLoraAt);
-        lora_offsets(lo, lt, lora_pair(tiles_l, lo, lt, e, N, n), M, N, m, n, wave, new_lane(), va, vb, na, nb, lora_lo);
+        lora_offsets(lo, lt, lora_pair(tiles_l, lo, lt, e, N, n), M, N, m, n, wave, new_lane(), va, vb, na, nb, lora_lo, lora_all);
       }
     };
     int at = 0;
     // one row half of v against both column halves of the adapter's B; of ranks up to 32 the first half
     // of a step
-    auto prod_lora = [&](gdn::f32x4_t (&c)[2][4][2], const Frag8 (&fa)[4], const Frag8 (&f0)[2], const Frag8 (&f1)[2]) {
+    auto prod_lora = [&](gdn::f32x4_t (&c)[2][4][2], const Frag8 (&fa)[4], const Frag8 (&f0)[2], const Frag8 (&f1)[2],
+                         bool any) {
       if constexpr (kLora) {
         auto bits = [](const i32x4_t& v) { return __builtin_bit_cast(gdn::s16x8_t, v); };
+        if (any) {
 #pragma unroll
         for (int b = 0; b < 2; ++b)
 #pragma unroll
@@ -293,7 +296,8 @@ __global__ __launch_bounds__(kPPThreads, 2) void gemm_fp8_pp_kernel(const uint8_
 #pragma unroll
             for (int t = 0; t < 2; ++t)
               c[b][i][t] = gdn::mfma16x16x32(bits(b ? f1[t].lo : f0[t].lo), bits(fa[i].lo), c[b][i][t]);
-        if (lora_lo > 64) {
+        }
+        if (any && lora_all) {
 #pragma unroll
           for (int b = 0; b < 2; ++b)
 #pragma unroll
@@ -396,27 +400,29 @@ __global__ __launch_bounds__(kPPThreads, 2) void gemm_fp8_pp_kernel(const uint8_
           read_a(a00, fa);
           read_b(b01, fb1);
           mem_end();
-          prod_lora(acc[0], fa, fb0, fb1);
+          prod_lora(acc[0], fa, fb0, fb1, true);
           dma(ra_n, a00, va[0], 0);
           dma(rb_n, b01, vb[1], 0);
           dma_sc(sc0, 0);
           read_a(a01, fa);
-          read_b(b10, fbn);
+          if (lora_lo) read_b(b10, fbn);
           mem_end();
-          prod_lora(acc[1], fa, fb0, fb1);
+          prod_lora(acc[1], fa, fb0, fb1, true);
           dma(rb_n, b10, vb[0], k3b);
           dma(ra_n, a01, va[1], 0);
-          read_a(a10, fa);
-          read_b(b11, fb1);
+          if (lora_lo) {
+            read_a(a10, fa);
+            read_b(b11, fb1);
+          }
           mem_end();
-          prod_lora(acc[0], fa, fbn, fb1);
+          prod_lora(acc[0], fa, fbn, fb1, lora_lo);
           dma(ra_n, a10, va[0], k3a);
           dma(rb_n, b11, vb[1], k3b);
           dma_sc(sc1, 1);
-          read_a(a11, fa);
+          if (lora_lo) read_a(a11, fa);
           read_b(b00, fb0);
           mem_end();
-          prod_lora(acc[1], fa, fbn, fb1);
+          prod_lora(acc[1], fa, fbn, fb1, lora_lo);
         }
         if (lt.part) {
           float bad = 0.0f;

@@ -289,31 +289,28 @@ struct LoraRows {
 
 // 64 rows from row0 against the 32 columns from cb, onto sums that are kept apart per row: at(i, t)
 // as lora_init's at(i, 0, t).  A row's products in the order of the 256 x 256 tiles' steps: of each 64
-// of the rank the high parts, then the low ones.
+// of the rank the high parts, then the low ones, of ranks up to 32 both one behind the other.
 template <int DEPTH, class At>
 __device__ __forceinline__ void lora_add(const Lora& lo, int M, int N, int row0, int cb, int lane, const At& at) {
   const LoraRows<4, false> r(lo, M, row0, lane);
   if (!r.all || cb >= N) return;
   const int lr = lane & 15, lg = lane >> 4, half = lo.rank / 8;
-  const bool both = half <= 4;  // high and low parts meet the same values of b at once
+  const bool one = half <= 4;
   const int col = cb + 8 * (lr >> 2) + (lr & 3);
   for (int p = 0, beg = 0, end = 0; p < lo.slices; ++p, beg = end) {
     end = lora_end(lo, p);
     if (cb >= end || cb + 32 <= beg) continue;
     const bool sel = cb + 8 * lg >= beg && cb + 8 * lg < end;
     const __amdgpu_buffer_rsrc_t rv = rsrc_of(lo.v + 2 * p * lo.rank);
-    for (int sub = 0; sub < (both ? 1 : (half + 7) / 8 * 4); ++sub) {
-      // granules q0 .. q0 + 3 of the high (or low) parts
-      const int q0 = 8 * (sub >> 2) + 4 * (sub & 1), low = (sub >> 1) & 1;
-      if (q0 >= half) continue;
-      const int q = q0 + lg, off = q < half ? 0 : kNoOffset;
-      gdn::s16x8_t vh[4], vl[4];
+    for (int sub = 0; sub < (one ? (half + 1) / 2 : (half + 7) / 8 * 4); ++sub) {
+      // granules q0 .. q0 + 3 of both parts, or of the high (or low) ones
+      const int q0 = one ? 4 * sub : 8 * (sub >> 2) + 4 * (sub & 1), low = one ? 0 : (sub >> 1) & 1;
+      if (!one && q0 >= half) continue;
+      const int q = q0 + lg, off = q < (one ? 2 * half : half) ? 0 : kNoOffset;
+      const int qb = one && q >= half ? q - half : q;
+      gdn::s16x8_t v[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) vh[i] = lora_load(rv, (r.voff[i] + 16 * (q + (low ? half : 0))) | off);
-      if (both) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) vl[i] = lora_load(rv, (r.voff[i] + 16 * (q + half)) | off);
-      }
+      for (int i = 0; i < 4; ++i) v[i] = lora_load(rv, (r.voff[i] + 16 * (q + (low ? half : 0))) | off);
       LoraIds it{r.all, 0, 1};
       gdn::s16x8_t fb[DEPTH][2];
       int sid[DEPTH];
@@ -323,7 +320,7 @@ __device__ __forceinline__ void lora_add(const Lora& lo, int M, int N, int row0,
         if (sid[d] < 0) return;
         const __amdgpu_buffer_rsrc_t rb = lora_b(lo, sid[d], N);
 #pragma unroll
-        for (int t = 0; t < 2; ++t) fb[d][t] = lora_load(rb, ((col + 4 * t) * lo.rank * 2 + 16 * q) | off);
+        for (int t = 0; t < 2; ++t) fb[d][t] = lora_load(rb, ((col + 4 * t) * lo.rank * 2 + 16 * qb) | off);
       };
 #pragma unroll
       for (int d = 0; d < DEPTH; ++d) fetch(d);
@@ -338,8 +335,7 @@ __device__ __forceinline__ void lora_add(const Lora& lo, int M, int N, int row0,
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
               gdn::f32x4_t& acc = at(i, t);
-              gdn::f32x4_t sum = gdn::mfma16x16x32(fb[d][t], vh[i], acc);
-              if (both) sum = gdn::mfma16x16x32(fb[d][t], vl[i], sum);
+              const gdn::f32x4_t sum = gdn::mfma16x16x32(fb[d][t], v[i], acc);
 #pragma unroll
               for (int e = 0; e < 4; ++e) acc[e] = take ? sum[e] : acc[e];
             }
@@ -387,7 +383,8 @@ __device__ __forceinline__ void lora_init(const Lora& lo, int M, int N, int row0
 // ---- 256 x 256 tiles ----
 // A tile takes its rows' adapters as more steps of 64 values behind K, in pairs: the high parts of
 // 64 of the rank's values, then the low ones, for each adapter among its rows, each slice among
-// its columns and each 64 of the rank.  Rows of other adapters and columns of other slices come as
+// its columns and each 64 of the rank; of ranks up to 32 both parts are in the first step, B's values
+// twice, and the second one is empty.  Rows of other adapters and columns of other slices come as
 // zeros.  Where that is not all of the tile, a result that is not finite may be the zeros' fault:
 // the tile is then done again as quarters of 128 x 128, whose sums are kept apart per row
 // (lora_add, the same products in the same order: a row has the same bits).  So are the tiles with
@@ -522,13 +519,18 @@ __device__ __forceinline__ LoraPair lora_pair(const LoraTiles& list, const Lora&
   return q;
 }
 // Offsets of the wave's loads for a pair (rows m0 .., columns n0 ..; va and vb as the products'),
-// the pointers in A's and B's place, and the bytes from the high parts to the low ones.
+// the pointers in A's and B's place, the bytes from the high parts to the low ones (0: both are in the first
+// step), and whether a step's second half has values.
 __device__ __forceinline__ void lora_offsets(const Lora& lo, const LoraSteps& t, const LoraPair& q, int M, int N, int m0,
                                              int n0, int wave, int lane, int (&va)[2][2], int (&vb)[2][2], LoraBase& na,
-                                             LoraBase& nb, int& low) {
+                                             LoraBase& nb, int& low, bool& all) {
   const int half = lo.rank / 8, r = 8 * wave + (lane >> 3);
-  const int ga = (lane & 7) ^ (((wave & 1) << 2) | (lane >> 4)), gb = (lane & 7) ^ (((wave & 3) << 1) | ((lane >> 4) & 1));
-  const int oa = q.r0 / 8 + ga < half ? 0 : kNoOffset, ob = q.r0 / 8 + gb < half ? 0 : kNoOffset;
+  const bool one = half <= 4;
+  const int ga = (lane & 7) ^ (((wave & 1) << 2) | (lane >> 4));
+  int gb = (lane & 7) ^ (((wave & 3) << 1) | ((lane >> 4) & 1));
+  const int to = one ? 2 * half : half - q.r0 / 8;
+  const int oa = ga < to ? 0 : kNoOffset, ob = gb < to ? 0 : kNoOffset;
+  gb -= one && gb >= half ? half : 0;
 #pragma unroll
   for (int h = 0; h < 2; ++h)
 #pragma unroll
@@ -540,7 +542,8 @@ __device__ __forceinline__ void lora_offsets(const Lora& lo, const LoraSteps& t,
     }
   na = LoraBase(lo.v + 2 * q.p * lo.rank + q.r0);
   nb = LoraBase(lo.b + q.s * lo.b_slot + q.r0);
-  low = 2 * lo.rank;
+  low = one ? 0 : 2 * lo.rank;
+  all = half > 2;
 }
 // The tiles to be done again, behind the others' quarters; returns how many quarters.
 __device__ __forceinline__ int lora_quarters(LoraTiles& list) {
