@@ -45,43 +45,64 @@ __device__ __forceinline__ float sigmoid_ulp(float g) {
   return g < -88.0f ? 0.0f : g != g ? g : fmaf(rc, fmaf(-d, rc, 1.0f), rc);
 }
 
-// V (8 or 1) values at p[at], bf16 or fp32
-template <int V>
-__device__ __forceinline__ void load(const void* p, int64_t at, bool f32, float (&v)[V]) {
-  if constexpr (V == 8) {
-    if (f32) {
-      const float4 a = *reinterpret_cast<const float4*>(static_cast<const float*>(p) + at);
-      const float4 b = *reinterpret_cast<const float4*>(static_cast<const float*>(p) + at + 4);
+constexpr int V = 8;  // values to a piece
+
+// One value at p[at], bf16 or fp32.
+__device__ __forceinline__ float load1(const void* p, int64_t at, bool f32) {
+  return f32 ? static_cast<const float*>(p)[at] : gdn::bf2f(static_cast<const uint16_t*>(p)[at]);
+}
+
+// A piece at p[at].  kAny: at any address, its first n values (the others 0); else whole and aligned.
+template <bool kAny>
+__device__ __forceinline__ void load(const void* p, int64_t at, int n, bool f32, float (&v)[V]) {
+  if (kAny && n < V) {
+#pragma unroll
+    for (int e = 0; e < V; ++e) v[e] = e < n ? load1(p, at + e, f32) : 0.0f;
+  } else if (f32) {
+    const float* q = static_cast<const float*>(p) + at;
+    if constexpr (kAny) {
+      __builtin_memcpy(v, q, sizeof(v));
+    } else {
+      const float4 a = *reinterpret_cast<const float4*>(q), b = *reinterpret_cast<const float4*>(q + 4);
       v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
       v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-    } else {
-      const uint4 a = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p) + at);
-      const uint32_t w[4] = {a.x, a.y, a.z, a.w};
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        v[2 * i] = __uint_as_float(w[i] << 16);
-        v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-      }
     }
   } else {
-    v[0] = f32 ? static_cast<const float*>(p)[at] : gdn::bf2f(static_cast<const uint16_t*>(p)[at]);
+    const uint16_t* q = static_cast<const uint16_t*>(p) + at;
+    uint4 a;
+    if constexpr (kAny) __builtin_memcpy(&a, q, sizeof(a));
+    else a = *reinterpret_cast<const uint4*>(q);
+    const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      v[2 * i] = __uint_as_float(w[i] << 16);
+      v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    }
   }
 }
 
-template <int V>
-__device__ __forceinline__ void store(void* p, int64_t at, bool f32, const float (&v)[V]) {
-  if constexpr (V == 8) {
-    if (f32) {
-      float4* q = reinterpret_cast<float4*>(static_cast<float*>(p) + at);
-      q[0] = make_float4(v[0], v[1], v[2], v[3]);
-      q[1] = make_float4(v[4], v[5], v[6], v[7]);
+template <bool kAny>
+__device__ __forceinline__ void store(void* p, int64_t at, int n, bool f32, const float (&v)[V]) {
+  if (kAny && n < V) {
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      if (e >= n) continue;
+      if (f32) static_cast<float*>(p)[at + e] = v[e];
+      else static_cast<uint16_t*>(p)[at + e] = gdn::f2bf(v[e]);
+    }
+  } else if (f32) {
+    float* q = static_cast<float*>(p) + at;
+    if constexpr (kAny) {
+      __builtin_memcpy(q, v, sizeof(v));
     } else {
-      *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p) + at) =
-          make_uint4(gdn::f2bf2(v[0], v[1]), gdn::f2bf2(v[2], v[3]), gdn::f2bf2(v[4], v[5]), gdn::f2bf2(v[6], v[7]));
+      reinterpret_cast<float4*>(q)[0] = make_float4(v[0], v[1], v[2], v[3]);
+      reinterpret_cast<float4*>(q)[1] = make_float4(v[4], v[5], v[6], v[7]);
     }
   } else {
-    if (f32) static_cast<float*>(p)[at] = v[0];
-    else static_cast<uint16_t*>(p)[at] = gdn::f2bf(v[0]);
+    uint16_t* q = static_cast<uint16_t*>(p) + at;
+    const uint4 w = make_uint4(gdn::f2bf2(v[0], v[1]), gdn::f2bf2(v[2], v[3]), gdn::f2bf2(v[4], v[5]), gdn::f2bf2(v[6], v[7]));
+    if constexpr (kAny) __builtin_memcpy(q, &w, sizeof(w));
+    else *reinterpret_cast<uint4*>(q) = w;
   }
 }
 
@@ -104,9 +125,9 @@ __device__ __forceinline__ float row_sum(float v, float* part) {
 // TB/s; 4 bytes read and 4 written a value), with a norm behind the block and a gate 44, in bf16 and e4m3 55; a few rows one
 // launch's latency (1 x 2048 2.8, 201 rows with both norms 3.8).
 //
-// T threads per row, N pieces of V values per thread: piece i of thread t is columns V (T i +
+// T threads per row, N pieces of 8 values per thread: piece i of thread t is columns V (T i +
 // t) .., so that 16 neighbouring lanes hold a group of 128.
-template <int V, int N, int T, bool kFp8>
+template <bool kAny, int N, int T, bool kFp8>
 __global__ __launch_bounds__(T > 256 ? T : 256) void block_norm_kernel(NormArgs a) {
   __shared__ float part[2][T > 64 ? T / 64 : 1];
   constexpr int kRows = T > 256 ? 1 : 256 / T;
@@ -115,19 +136,20 @@ __global__ __launch_bounds__(T > 256 ? T : 256) void block_norm_kernel(NormArgs 
   const int64_t row = static_cast<int64_t>(blockIdx.x) * kRows + threadIdx.x / T;
   if (row >= a.M) return;  // (a wave, or the workgroup)
   auto col = [&](int i) { return V * (T * i + t); };
+  auto left = [&](int i) { return a.H - col(i); };  // values of the row from the piece on
   float h[N][V];
 #pragma unroll
   for (int i = 0; i < N; ++i) {
 #pragma unroll
     for (int e = 0; e < V; ++e) h[i][e] = 0.0f;
-    if (col(i) < a.H) load<V>(a.x, row * a.sx + col(i), false, h[i]);
+    if (col(i) < a.H) load<kAny>(a.x, row * a.sx + col(i), left(i), false, h[i]);
   }
   float res[N][V];
 #pragma unroll
   for (int i = 0; i < N; ++i) {
 #pragma unroll
     for (int e = 0; e < V; ++e) res[i][e] = 0.0f;
-    if (a.residual && col(i) < a.H) load<V>(a.residual, row * a.sr + col(i), a.stream_f32, res[i]);
+    if (a.residual && col(i) < a.H) load<kAny>(a.residual, row * a.sr + col(i), left(i), a.stream_f32, res[i]);
   }
   const float inv_h = 1.0f / static_cast<float>(a.H);
   if (a.post_w) {
@@ -141,26 +163,25 @@ __global__ __launch_bounds__(T > 256 ? T : 256) void block_norm_kernel(NormArgs 
     for (int i = 0; i < N; ++i) {
       if (col(i) >= a.H) continue;
       float w[V];
-      load<V>(a.post_w, col(i), a.w_f32, w);
+      load<kAny>(a.post_w, col(i), left(i), a.w_f32, w);
 #pragma unroll
       for (int e = 0; e < V; ++e) h[i][e] *= r * (a.offset + w[e]);
     }
   }
   if (a.gate) {
     if (a.g_col == 0) {
-      float g[1];
-      load<1>(a.gate, row * a.g_row, a.gate_f32, g);
-      if (a.gate_sigmoid) g[0] = sigmoid_ulp(g[0]);
+      float g = load1(a.gate, row * a.g_row, a.gate_f32);
+      if (a.gate_sigmoid) g = sigmoid_ulp(g);
 #pragma unroll
       for (int i = 0; i < N; ++i)
 #pragma unroll
-        for (int e = 0; e < V; ++e) h[i][e] *= g[0];
+        for (int e = 0; e < V; ++e) h[i][e] *= g;
     } else {
 #pragma unroll
       for (int i = 0; i < N; ++i) {
         if (col(i) >= a.H) continue;
         float g[V];
-        load<V>(a.gate, row * a.g_row + col(i), a.gate_f32, g);
+        load<kAny>(a.gate, row * a.g_row + col(i), left(i), a.gate_f32, g);
 #pragma unroll
         for (int e = 0; e < V; ++e) h[i][e] *= a.gate_sigmoid ? sigmoid_ulp(g[e]) : g[e];
       }
@@ -172,10 +193,10 @@ __global__ __launch_bounds__(T > 256 ? T : 256) void block_norm_kernel(NormArgs 
 #pragma unroll
     for (int e = 0; e < V; ++e) {
       // (what lies past the row stays 0: a gate of infinity is one per row there)
-      h[i][e] = col(i) < a.H ? fmaf(h[i][e], a.scale, res[i][e]) : 0.0f;
+      h[i][e] = (kAny ? e : 0) < left(i) ? fmaf(h[i][e], a.scale, res[i][e]) : 0.0f;
       ss = fmaf(h[i][e], h[i][e], ss);
     }
-    if (a.stream && col(i) < a.H) store<V>(a.stream, row * a.H + col(i), a.stream_f32, h[i]);
+    if (a.stream && col(i) < a.H) store<kAny>(a.stream, row * a.H + col(i), left(i), a.stream_f32, h[i]);
   }
   const float r = rsqrtf(row_sum<T>(ss, part[1]) * inv_h + a.eps);
 #pragma unroll
@@ -185,10 +206,10 @@ __global__ __launch_bounds__(T > 256 ? T : 256) void block_norm_kernel(NormArgs 
     float w[V];
 #pragma unroll
     for (int e = 0; e < V; ++e) w[e] = 0.0f;
-    if (in) load<V>(a.w, col(i), a.w_f32, w);
+    if (in) load<kAny>(a.w, col(i), left(i), a.w_f32, w);
 #pragma unroll
     for (int e = 0; e < V; ++e) h[i][e] *= r * (a.offset + w[e]);
-    if (a.y && in) store<V>(a.y, row * a.H + col(i), false, h[i]);
+    if (a.y && in) store<kAny>(a.y, row * a.H + col(i), left(i), false, h[i]);
     if constexpr (kFp8) {
       float top = 0.0f;
 #pragma unroll
@@ -206,31 +227,31 @@ __global__ __launch_bounds__(T > 256 ? T : 256) void block_norm_kernel(NormArgs 
   }
 }
 
-template <int V, int T, bool kFp8, int... N>
+template <bool kAny, int T, bool kFp8, int... N>
 int launch(const NormArgs& a, hipStream_t st) {
   constexpr int kRows = T > 256 ? 1 : 256 / T;
   const dim3 grid(static_cast<unsigned>((a.M + kRows - 1) / kRows)), block(T > 256 ? T : 256);
   bool done = false;
   auto one = [&](auto n) {
     if (done || a.H > V * T * n.value) return;
-    block_norm_kernel<V, n.value, T, kFp8><<<grid, block, 0, st>>>(a);
+    block_norm_kernel<kAny, n.value, T, kFp8><<<grid, block, 0, st>>>(a);
     done = true;
   };
   (one(std::integral_constant<int, N>{}), ...);
   return done ? gdn_launch_status() : GDN_ERR_UNSUPPORTED;
 }
 
-template <bool kFp8>
+template <bool kAny, bool kFp8>
 int launch_rows(const NormArgs& a, hipStream_t st) {
   // One piece of 8 to a thread (past 8192 columns two), and so a row's workgroup grows with it: what is in flight is then
   // bounded by the rows that run at once and not by a thread's chain (us, replayed; 256 threads for all: 16 x 4096
   // 4.2, in 512 3.9; 16 x 16384 8.6, in 1024 4.7; 8192 x 16384 317 and 188, 8192 x 8192 107 and 97).  Many short
   // rows go to a wave each, without a barrier: 16384 x 1024 22.1 (256 threads 24.5), 4096 x 1024 7.4 (7.8); 16384 x 2048 45.3
   // (41.1), 1024 x 1024 4.7 (4.3).
-  if (a.M >= 2048 && a.H <= 1024) return launch<8, 64, kFp8, 1, 2>(a, st);
-  if (a.H <= 2048) return launch<8, 256, kFp8, 1>(a, st);
-  if (a.H <= 4096) return launch<8, 512, kFp8, 1>(a, st);
-  return launch<8, 1024, kFp8, 1, 2>(a, st);
+  if (a.M >= 2048 && a.H <= 1024) return launch<kAny, 64, kFp8, 1, 2>(a, st);
+  if (a.H <= 2048) return launch<kAny, 256, kFp8, 1>(a, st);
+  if (a.H <= 4096) return launch<kAny, 512, kFp8, 1>(a, st);
+  return launch<kAny, 1024, kFp8, 1, 2>(a, st);
 }
 
 constexpr int kMostColumns = 16384;
@@ -263,8 +284,8 @@ extern "C" int gdn_add_rms_norm(const uint16_t* x, int64_t sx, const void* resid
   if (y8 && !whole) return GDN_ERR_INVALID_ARG;
   if (stream == GDN_CHECK_ONLY) return GDN_OK;
   const hipStream_t st = static_cast<hipStream_t>(stream);
-  if (y8) return launch_rows<true>(a, st);
-  if (whole) return launch_rows<false>(a, st);
-  // a row in pieces of one value: 8192 x 1001 25.1 us, with 1024 threads 40.7 (one row 4.3 and 3.5); 1024 x 500 4.5 / 6.4
-  return H <= 1024 ? launch<1, 256, false, 4>(a, st) : launch<1, 1024, false, 4, 16>(a, st);
+  if (y8) return launch_rows<false, true>(a, st);
+  // (any other row goes by the same pieces, which straddle lines, its last one value by value: value by value
+  // throughout, 8192 x 1001 25.1 us, 1031 x 4299 360)
+  return whole ? launch_rows<false, false>(a, st) : launch_rows<true, false>(a, st);
 }
