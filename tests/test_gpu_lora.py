@@ -417,7 +417,7 @@ def test_rows_in_the_order_of_their_adapters(pkg, dev, M, N, S, how, fp8):
         assert torch.equal(g, eg) and torch.equal(beta, eb)
 
 
-@pytest.mark.parametrize("M", [1, 40, 300, 2500])
+@pytest.mark.parametrize("M", [1, 40, 300, 2000, 2500])
 def test_no_slots_and_the_rows_quantized_on_the_way(pkg, dev, M):
     """A pool without slots: the products alone, bit for bit, bf16 rows for 8-bit weights quantized all the same;
     and the e4m3 rows that come out of the adapters' launch are quantize_fp8's."""
