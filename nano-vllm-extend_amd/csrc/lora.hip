@@ -90,11 +90,13 @@ __device__ __forceinline__ void store_v(const Shrink& p, int m, int c, const gdn
 // steps the loads are on their way at once, 8 lanes to a row's 128 bytes (straight in the
 // matrix cores' layout, a row to a lane, they took 4 times as long); each step then goes through the wave's own rows of
 // LDS.  A lane asks for rows (-1: none) and columns lane / 8 and 8 + lane / 8; steps past the end load zeros.
-template <int NW, bool kFp8>
+constexpr int kFewWaves = 8;  // (16 take as long, K up to 16384, and longer where there are more tiles than CUs)
+
+template <bool kFp8>
 __device__ __forceinline__ gdn::f32x4_t few_product(const Shrink& p, __amdgpu_buffer_rsrc_t rx, __amdgpu_buffer_rsrc_t ra,
                                                     __amdgpu_buffer_rsrc_t rs, const int (&row)[2], int own_row, int c0, int wave,
                                                     int lane, uint8_t* lds) {
-  constexpr int C = kFp8 ? 2 : 4, kStep = kFp8 ? 128 : 64, kHalves = kFp8 ? 2 : 1;
+  constexpr int NW = kFewWaves, C = kFp8 ? 2 : 4, kStep = kFp8 ? 128 : 64, kHalves = kFp8 ? 2 : 1;
   const int nk = p.K / kStep, lr = lane & 15, lg = lane >> 4;
   int xoff[2], aoff[2], at[2];
 #pragma unroll
@@ -160,8 +162,9 @@ __device__ __forceinline__ gdn::f32x4_t few_product(const Shrink& p, __amdgpu_bu
 // workgroup finds it for itself: a row's place is the number of rows before it, counted by all
 // threads (256 rows: 1 us, and none of it waits for memory).  Else: blockIdx.x has 16 rows and, of
 // their adapters, the blockIdx.y-th and on every share-th.
-template <int NW, bool kFp8, bool kSort>
-__global__ __launch_bounds__(64 * NW) void lora_few_kernel(Shrink p) {
+template <bool kFp8, bool kSort>
+__global__ __launch_bounds__(64 * kFewWaves) void lora_few_kernel(Shrink p) {
+  constexpr int NW = kFewWaves;
   constexpr int kStepBytes = kFp8 ? 6144 : 4096;
   __shared__ __align__(16) unsigned key[kLoraSort];
   __shared__ int place[kLoraSort], s_row[kLoraSort], s_id[kLoraSort], s_item[kLoraSort], s_count[4];
@@ -182,7 +185,7 @@ __global__ __launch_bounds__(64 * NW) void lora_few_kernel(Shrink p) {
   const __amdgpu_buffer_rsrc_t rx = rsrc_of(p.x), rs = rsrc_of(p.xs);
   // rows: the ones that the lane loads
   auto run = [&](int s, const int (&rows)[2], int row, bool own) {
-    const gdn::f32x4_t acc = few_product<NW, kFp8>(p, rx, rsrc_of(p.a + s * p.a_slot), rs, rows, row, c0, wave, lane,
+    const gdn::f32x4_t acc = few_product<kFp8>(p, rx, rsrc_of(p.a + s * p.a_slot), rs, rows, row, c0, wave, lane,
                                                    steps + wave * kStepBytes);
     const float scale = p.scale[s];
     __syncthreads();
@@ -473,21 +476,18 @@ int launch(Shrink p, hipStream_t st) {
         : lora_shrink_kernel<4, 2, 4, 2, kFp8><<<grid, dim3(256), 0, st>>>(p);
     return gdn_launch_status();
   }
-  // so many workgroups share the adapters (those that find none end); 16 waves where 8 would have more
-  // than one round of loads
+  // So many workgroups share the adapters (those that find none end).
   const int n = tiles(p.cols, 16), most = std::max(1, 512 / n);
-  const bool sort = lora_sorted(p.M, p.slots), wide = p.K > 2048;
+  const bool sort = lora_sorted(p.M, p.slots);
   p.share = sort ? std::min(most, std::min(p.M, tiles(p.M, 16) + std::min(p.slots, p.M)))
-                         : std::max(1, std::min(std::min(std::min(16, p.M), p.slots), 1024 / (n * tiles(p.M, 16))));
+                 : std::max(1, std::min(std::min(std::min(16, p.M), p.slots), 1024 / (n * tiles(p.M, 16))));
   const int across = sort ? n : n * tiles(p.M, 16);
-  const int64_t quant = p.x8 ? (static_cast<int64_t>(p.M) * (p.K / gdn::kFp8Group) + (wide ? 63 : 31)) / (wide ? 64 : 32) : 0;
+  const int64_t quant = p.x8 ? (static_cast<int64_t>(p.M) * (p.K / gdn::kFp8Group) + 31) / 32 : 0;
   const dim3 grid(static_cast<unsigned>(across), static_cast<unsigned>(p.share + (quant + across - 1) / across));
   if (sort)
-    wide ? lora_few_kernel<16, kFp8, true><<<grid, dim3(1024), 0, st>>>(p)
-         : lora_few_kernel<8, kFp8, true><<<grid, dim3(512), 0, st>>>(p);
+    lora_few_kernel<kFp8, true><<<grid, dim3(64 * kFewWaves), 0, st>>>(p);
   else
-    wide ? lora_few_kernel<16, kFp8, false><<<grid, dim3(1024), 0, st>>>(p)
-         : lora_few_kernel<8, kFp8, false><<<grid, dim3(512), 0, st>>>(p);
+    lora_few_kernel<kFp8, false><<<grid, dim3(64 * kFewWaves), 0, st>>>(p);
   return gdn_launch_status();
 }
 
