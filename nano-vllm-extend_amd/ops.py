@@ -1613,6 +1613,18 @@ def _lora_check(x, N, K, widths, lora_a, lora_b, lora_scale, ids):
     return M, P, R
 
 
+def _check_gates(gates, N):
+    """gates' parameters beside a product with N columns."""
+    a_log, dt_bias, col = gates["A_log"], gates["dt_bias"], int(gates["gate_col"])
+    if not (a_log.dtype.is_floating_point and dt_bias.dtype.is_floating_point):
+        raise TypeError(f"A_log and dt_bias must be floating point, got {a_log.dtype} and {dt_bias.dtype}")
+    Hv = a_log.numel()
+    if Hv < 1 or dt_bias.numel() != Hv or not 0 <= col <= N - 2 * Hv:
+        raise ValueError(f"A_log and dt_bias must have as many values, their columns within the product's {N}, got {Hv} and "
+                         f"{dt_bias.numel()} from column {col}")
+    return a_log, dt_bias
+
+
 def _lora_shrink(idx, rows, stride, x_scale, lora_a, lora_scale, ids, M, K, P, R, x8=None, x8_scale=None):
     """(v [M, P, 2, R] of the rows with an adapter, the adapters of their groups of 16 and, of few
     rows, their order); x8 and its scales [M, K / 128] take quantize_fp8 of the rows."""
@@ -1697,7 +1709,7 @@ def linear_lora(x: torch.Tensor, weight: torch.Tensor, lora_a: torch.Tensor, lor
     if K == 0 or K % 64 or x.shape[-1] != K:
         raise ValueError(f"x [..., {x.shape[-1]}] and weight [{N}, {K}]: equal last dims, a positive multiple of 64")
     M, P, R = _lora_check(x, N, K, parts, lora_a, lora_b, lora_scale, ids)
-    idx = _device_of(x, weight, lora_a, lora_b, lora_scale, ids)
+    idx = _device_of(x, weight, lora_a, lora_b, lora_scale, ids, *(() if gates is None else _check_gates(gates, N)))
     rows, _, stride = _rows_of(x, 8)
     weight, ids = _weight_rows(weight, 8), ids.contiguous()
     outs = [torch.empty(M, w, dtype=torch.bfloat16, device=x.device) for w in parts]
@@ -1742,7 +1754,8 @@ def linear_fp8_lora(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.T
     if not narrow:
         raise ValueError(f"widths {parts}: a boundary at {N}")
     n = narrow[0]
-    idx = _device_of(x, weight, weight_scale, x_scale, wide, lora_a, lora_b, lora_scale, ids)
+    idx = _device_of(x, weight, weight_scale, x_scale, wide, lora_a, lora_b, lora_scale, ids,
+                     *(() if gates is None else _check_gates(gates, total - N)))
     rows, _, stride = _rows_of(x, 8 if x_scale is None else 16)
     weight, ids = _weight_rows(weight, 16), ids.contiguous()
     G = K // FP8_GROUP

@@ -102,6 +102,35 @@ def test_linear_fp8_lora_refuses(ops):
         ops.linear_fp8_lora(**{**more, "x": x.to(FP8), "x_scale": torch.zeros(M, 1)})
 
 
+def _bad_gates(N, Hv=8):
+    z = torch.zeros
+    good = dict(A_log=z(Hv), dt_bias=z(Hv), gate_col=N - 2 * Hv)
+    return good, [dict(good, **bad) for bad in (
+        dict(dt_bias=z(Hv - 1)), dict(dt_bias=z(Hv + 1)), dict(A_log=z(Hv - 1)), dict(A_log=z(0), dt_bias=z(0)), dict(gate_col=-1),
+        dict(gate_col=N - 2 * Hv + 1), dict(A_log=z(Hv, dtype=I32)), dict(dt_bias=z(Hv, dtype=torch.int64)))]
+
+
+def test_gates_refuse(ops, monkeypatch):
+    """Gates' parameters of another length, or whose columns are not the product's; all of them
+    go through the device check."""
+    M, N, K = 5, 96, 128
+    x, w, ids = torch.zeros(M, K, dtype=BF16), torch.zeros(N, K, dtype=BF16), torch.zeros(M, dtype=I32)
+    gates, bad = _bad_gates(N)
+    _refused(ops.linear_lora, dict(x=x, weight=w, ids=ids, widths=[64, 32], gates=gates, **_lora()), gates=bad)
+    wide = dict(x=x, weight=torch.zeros(N, K, dtype=torch.uint8).view(FP8), weight_scale=torch.zeros(1, 1), ids=ids, widths=[96, 32],
+                wide=torch.zeros(32, K, dtype=BF16), **_lora(N=128))
+    gates, bad = _bad_gates(32)
+    _refused(ops.linear_fp8_lora, dict(wide, gates=gates), gates=bad)
+    seen = []
+    monkeypatch.setattr(ops, "_device_of", lambda *ts: seen.extend(map(id, ts)) or 0)
+    for call in (lambda: ops.linear_fp8_lora(gates=gates, **wide),
+                 lambda: ops.linear_lora(x, w, ids=ids, widths=[64, 32], gates=gates, **_lora())):
+        seen.clear()
+        with pytest.raises(Launched):
+            call()
+        assert {id(gates["A_log"]), id(gates["dt_bias"])} <= set(seen)
+
+
 def test_pool_refuses(pkg):
     with pytest.raises(ValueError):
         pkg.LoraPool(2, 0, 64, [32], device="cpu")
