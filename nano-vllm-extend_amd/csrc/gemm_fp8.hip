@@ -278,7 +278,7 @@ __global__ __launch_bounds__(kPPThreads, 2) void gemm_fp8_pp_kernel(const uint8_
     auto set_lora_offsets = [&](int e, int m, int n) {
       if constexpr (kLora) {
         const Lora lo = kernel_arg<Lora>(kLoraAt);
-        lora_offsets(lo, lt, lora_pair(tiles_l, lo, lt, e, N, n), M, N, m, n, wave, new_lane(), va, vb, na, nb, lora_lo, lora_all);
+        lora_offsets(tiles_l, lo, lt, lora_pair(tiles_l, lo, lt, e, N, n), M, N, m, n, wave, new_lane(), va, vb, na, nb, lora_lo, lora_all);
       }
     };
     int at = 0;

@@ -388,8 +388,11 @@ __device__ __forceinline__ void lora_init(const Lora& lo, int M, int N, int row0
 // zeros.  Where that is not all of the tile, a result that is not finite may be the zeros' fault:
 // the tile is then done again as quarters of 128 x 128, whose sums are kept apart per row
 // (lora_add, the same products in the same order: a row has the same bits).  So are the tiles with
-// more than kLoraMix adapters or kLoraPairs pairs.
-constexpr int kLoraMix = 6, kLoraPairs = 12, kLoraTiles = 448, kLoraMixed = 48;
+// more than kLoraMix adapters or kLoraPairs pairs, 2 to 3 us each (us, 768 rows, 12352 columns, rank 16, 7 / 8 / 12
+// adapters a tile: 56 / 59 / 71 in pairs, 64 / 64 / 65 in quarters; of bf16 rows 65 / 67 / 78 and 86 / 85 / 87), and those of at
+// most 128 columns, which are two quarters and not four, with more than kLoraNarrow pairs (the same of 2 / 4 / 6 adapters, whose
+// last 64 columns are two slices: 42 / 47 / 53, all whole 43 / 54 / 65).
+constexpr int kLoraMix = 12, kLoraPairs = 12, kLoraNarrow = 2, kLoraTiles = 448, kLoraMixed = 48;
 
 // The tiles of a workgroup, made once: those that run whole with what they need, and those that
 // run as quarters behind them.  (Found out tile by tile, a load waits for the stores of the tile
@@ -400,6 +403,7 @@ struct LoraTiles {
   // code: the one adapter of all rows, kNone, or kMixed - i for entry i of mix
   int tile[kLoraTiles], code[kLoraTiles], in_quarters[kLoraTiles];
   int mix[kLoraMixed][kLoraMix + 1];  // how many, and which
+  uint8_t which[kLoraMixed][256];     // each row's of them, kLoraMix: none
   uint8_t pairs[kLoraTiles];  // of steps, + kPart: of which not all rows or columns have the same
   uint8_t again[kLoraTiles];
   static constexpr int kNone = -1, kMixed = -2, kPart = 128;
@@ -440,9 +444,9 @@ __device__ __forceinline__ void lora_tiles(LoraTiles& list, const Lora& lo, int 
       // the tiles whose rows differ, one after the other by the whole wave
       for (uint64_t todo = __ballot(code == LoraTiles::kMixed); todo; todo &= todo - 1) {
         const int at = __builtin_ctzll(todo), m = __builtin_amdgcn_readlane(m0, at);
-        int id[4], n = 0;
+        int id[4], which[4], n = 0;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) id[i] = lora_id(lo, m + 64 * i + lane, M);
+        for (int i = 0; i < 4; ++i) id[i] = lora_id(lo, m + 64 * i + lane, M), which[i] = kLoraMix;
         for (;;) {
           int s = -1;
 #pragma unroll
@@ -452,13 +456,19 @@ __device__ __forceinline__ void lora_tiles(LoraTiles& list, const Lora& lo, int 
           }
           if (s < 0) break;
           if (n < kLoraMix && nm < kLoraMixed && lane == 0) list.mix[nm][n + 1] = s;
-          ++n;
-          if (n > kLoraMix) break;
 #pragma unroll
-          for (int i = 0; i < 4; ++i) id[i] = id[i] == s ? -1 : id[i];
+          for (int i = 0; i < 4; ++i) {
+            which[i] = id[i] == s ? n : which[i];
+            id[i] = id[i] == s ? -1 : id[i];
+          }
+          if (++n > kLoraMix) break;
         }
         const bool fits = n <= kLoraMix && nm < kLoraMixed;
         if (fits && lane == 0) list.mix[nm][0] = n;
+        if (fits) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) list.which[nm][64 * i + lane] = static_cast<uint8_t>(which[i]);
+        }
         if (lane == at) {
           quarters = !fits;
           code = LoraTiles::kMixed - nm;
@@ -470,7 +480,7 @@ __device__ __forceinline__ void lora_tiles(LoraTiles& list, const Lora& lo, int 
         lora_slices(lo, n0, min(n0 + 256, N), p0, p1);
         const int n = code >= 0 ? 1 : quarters ? 0 : list.mix[LoraTiles::kMixed - code][0];
         pairs = n * (p1 - p0) * parts;
-        quarters = quarters || pairs > kLoraPairs;
+        quarters = quarters || pairs > (N - n0 <= 128 ? kLoraNarrow : kLoraPairs);
         pairs += code < LoraTiles::kNone || p1 - p0 > 1 ? LoraTiles::kPart : 0;
       }
       const uint64_t w = __ballot(valid && !quarters), q = __ballot(valid && quarters);
@@ -501,9 +511,10 @@ __device__ __forceinline__ LoraSteps lora_steps(const LoraTiles& list, int at) {
   const int pairs = __builtin_amdgcn_readfirstlane(list.pairs[at]);
   return LoraSteps{__builtin_amdgcn_readfirstlane(list.code[at]), pairs % LoraTiles::kPart, pairs >= LoraTiles::kPart};
 }
-// Pair e of them: the adapter, the slice and its columns, the first of the rank's values.
+// Pair e of them: the adapter and its number among the tile's, the slice and its columns, the first of the
+// rank's values.
 struct LoraPair {
-  int s, p, beg, end, r0;
+  int s, of, p, beg, end, r0;
 };
 __device__ __forceinline__ LoraPair lora_pair(const LoraTiles& list, const Lora& lo, const LoraSteps& t, int e, int N,
                                               int n0) {
@@ -512,6 +523,7 @@ __device__ __forceinline__ LoraPair lora_pair(const LoraTiles& list, const Lora&
   const int parts = (lo.rank + 63) / 64, per = parts * (p1 - p0), i = e / per, r = e - i * per;
   LoraPair q;
   q.s = t.code >= 0 ? t.code : __builtin_amdgcn_readfirstlane(list.mix[LoraTiles::kMixed - t.code][1 + i]);
+  q.of = i;
   q.p = p0 + r / parts;
   q.r0 = 64 * (r % parts);
   q.beg = q.p == 0 ? 0 : lora_end(lo, q.p - 1);
@@ -521,7 +533,7 @@ __device__ __forceinline__ LoraPair lora_pair(const LoraTiles& list, const Lora&
 // Offsets of the wave's loads for a pair (rows m0 .., columns n0 ..; va and vb as the products'),
 // the pointers in A's and B's place, the bytes from the high parts to the low ones (0: both are in the first
 // step), and whether a step's second half has values.
-__device__ __forceinline__ void lora_offsets(const Lora& lo, const LoraSteps& t, const LoraPair& q, int M, int N, int m0,
+__device__ __forceinline__ void lora_offsets(const LoraTiles& list, const Lora& lo, const LoraSteps& t, const LoraPair& q, int M, int N, int m0,
                                              int n0, int wave, int lane, int (&va)[2][2], int (&vb)[2][2], LoraBase& na,
                                              LoraBase& nb, int& low, bool& all) {
   const int half = lo.rank / 8, r = 8 * wave + (lane >> 3);
@@ -538,7 +550,8 @@ __device__ __forceinline__ void lora_offsets(const Lora& lo, const LoraSteps& t,
       const int row = m0 + 128 * h + 64 * i + r, col = n0 + 128 * h + 64 * i + r;
       va[h][i] = (min(row, M - 1) * static_cast<int>(lo.ldv) * 2 + 16 * ga) | oa;
       vb[h][i] = (min(col, N - 1) * lo.rank * 2 + 16 * gb) | ob | (col >= q.beg && col < q.end ? 0 : kNoOffset);
-      if (t.code < LoraTiles::kNone) va[h][i] |= lora_id(lo, row, M) == q.s ? 0 : kNoOffset;
+      // (a load from memory here would wait for all that are in flight, 0.5 us a pair)
+      if (t.code < LoraTiles::kNone) va[h][i] |= list.which[LoraTiles::kMixed - t.code][row - m0] == q.of ? 0 : kNoOffset;
     }
   na = LoraBase(lo.v + 2 * q.p * lo.rank + q.r0);
   nb = LoraBase(lo.b + q.s * lo.b_slot + q.r0);

@@ -494,3 +494,39 @@ def test_two_streams_at_once(pkg, dev):
                     g.replay()
             torch.cuda.synchronize()
             assert all(torch.equal(a, b) for a, b in zip(out, want))
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("R", [8, 16, 40, 72])
+@pytest.mark.parametrize("n", [2, 3, 6, 7, 12, 13, 40])
+def test_large_tiles_of_several_adapters(pkg, dev, n, R, fp8):
+    """256 rows with n adapters each, in runs and row by row: up to, at and past what a tile takes as more steps, in whole tiles
+    and in a last one of two slices; a row's bits are those that it has when the others have no adapter, whatever theirs hold."""
+    gen = torch.Generator().manual_seed(n + R)
+    M, K, S, widths = 1300, 256, 48, [8192, 4096, 32, 32]
+    N = sum(widths)
+    x = torch.randn(M, K, generator=gen).to(BF16).to(dev)
+    w = (torch.randn(N, K, generator=gen) * K ** -0.5).to(BF16).to(dev)
+    a, b, scale = (t.to(dev) for t in _adapters(gen, S, widths, K, R))
+    row = torch.arange(M)
+    ids = torch.where(row < 768, row // 256 * n + row % 256 * n // 256, row * 7 % n) % (S - 1)
+    ids = torch.where(row % 50 == 9, torch.tensor(-1), ids).to(torch.int32).to(dev)
+    delta, slack = _delta(x, a, b, scale, ids, widths, K)
+    if fp8:
+        w8, ws = pkg.quantize_weight_fp8(w)
+        x8, xs = pkg.quantize_fp8(x)
+        call = lambda i: torch.cat(pkg.linear_fp8_lora(x, w8, ws, a, b, scale, i, widths=widths), 1)  # noqa: E731
+        want, base = ref.linear(x8, xs, w8, ws)
+        base = base + 4 * R * U * (want.abs() + delta.abs())
+    else:
+        call = lambda i: torch.cat(pkg.linear_lora(x, w, a, b, scale, i, widths=widths), 1)  # noqa: E731
+        want, base = x.double() @ w.double().t(), 2 * (K + 2 * R) * U * (x.double().abs() @ w.double().abs().t())
+    y = call(ids)
+    _check(y, want + delta, slack + base)
+    for s in ids[[0, 300, 1299]].tolist():
+        rows = ids == s
+        assert torch.equal(call(torch.where(rows, ids, -1))[rows], y[rows])
+    b[S - 1, ::3] = float("inf")
+    last = torch.where(ids == int(ids[100]), S - 1, ids).int()
+    rows = last != S - 1
+    assert torch.equal(call(last)[rows], y[rows])
