@@ -13,6 +13,7 @@
 // done again with the sums kept apart per row: a row never sees another one's adapter.
 #pragma once
 
+#include <algorithm>
 #include <type_traits>
 
 #include "gemm_tile.h"
@@ -39,6 +40,7 @@ struct Lora {
   const int* order;     // lora_sorted: [M] the rows in the order of their adapters, [M] the adapters
   int slots, rank, slices;
   int end[kMaxParts];   // slice p: columns end[p - 1] .. end[p] - 1; multiples of 16
+  int two;              // 256 x 256 tiles: two adapters to a pair of steps
 };
 struct NoLora {};
 template <bool kLora>
@@ -384,15 +386,16 @@ __device__ __forceinline__ void lora_init(const Lora& lo, int M, int N, int row0
 // A tile takes its rows' adapters as more steps of 64 values behind K, in pairs: the high parts of
 // 64 of the rank's values, then the low ones, for each adapter among its rows, each slice among
 // its columns and each 64 of the rank; of ranks up to 32 both parts are in the first step, B's values
-// twice, and the second one is empty.  Rows of other adapters and columns of other slices come as
+// twice, and the second one is empty; of ranks up to 16 the first step's halves are two adapters' (Lora::two: their slots must
+// be within one 32-bit offset of each other).  Rows of other adapters and columns of other slices come as
 // zeros.  Where that is not all of the tile, a result that is not finite may be the zeros' fault:
 // the tile is then done again as quarters of 128 x 128, whose sums are kept apart per row
 // (lora_add, the same products in the same order: a row has the same bits).  So are the tiles with
-// more than kLoraMix adapters or kLoraPairs pairs, 2 to 3 us each (us, 768 rows, 12352 columns, rank 16, 7 / 8 / 12
-// adapters a tile: 56 / 59 / 71 in pairs, 64 / 64 / 65 in quarters; of bf16 rows 65 / 67 / 78 and 86 / 85 / 87), and those of at
-// most 128 columns, which are two quarters and not four, with more than kLoraNarrow pairs (the same of 2 / 4 / 6 adapters, whose
-// last 64 columns are two slices: 42 / 47 / 53, all whole 43 / 54 / 65).
-constexpr int kLoraMix = 12, kLoraPairs = 12, kLoraNarrow = 2, kLoraTiles = 448, kLoraMixed = 48;
+// more than kLoraMix adapters or kLoraPairs pairs, 2 to 3 us each (us, 768 rows, 12352 columns, 6 / 12 / 20 adapters
+// a tile, in pairs: rank 16 47 / 58 / 73, one to a pair 54 / 71; in quarters 65 / 65 / 70; of bf16 rows 57 / 68 / 82,
+// 62 / 78, 85 / 87 / 93), and those of at most 128 columns, which are two quarters and not four, with more than kLoraNarrow
+// pairs (one to a pair, 2 / 4 / 6 adapters, the last 64 columns two slices: 42 / 47 / 53, all whole 43 / 54 / 65).
+constexpr int kLoraMix = 20, kLoraPairs = 12, kLoraNarrow = 2, kLoraTiles = 448, kLoraMixed = 48;
 
 // The tiles of a workgroup, made once: those that run whole with what they need, and those that
 // run as quarters behind them.  (Found out tile by tile, a load waits for the stores of the tile
@@ -479,7 +482,7 @@ __device__ __forceinline__ void lora_tiles(LoraTiles& list, const Lora& lo, int 
         int p0, p1;
         lora_slices(lo, n0, min(n0 + 256, N), p0, p1);
         const int n = code >= 0 ? 1 : quarters ? 0 : list.mix[LoraTiles::kMixed - code][0];
-        pairs = n * (p1 - p0) * parts;
+        pairs = (lo.two ? (n + 1) / 2 : n) * (p1 - p0) * parts;
         quarters = quarters || pairs > (N - n0 <= 128 ? kLoraNarrow : kLoraPairs);
         pairs += code < LoraTiles::kNone || p1 - p0 > 1 ? LoraTiles::kPart : 0;
       }
@@ -511,10 +514,11 @@ __device__ __forceinline__ LoraSteps lora_steps(const LoraTiles& list, int at) {
   const int pairs = __builtin_amdgcn_readfirstlane(list.pairs[at]);
   return LoraSteps{__builtin_amdgcn_readfirstlane(list.code[at]), pairs % LoraTiles::kPart, pairs >= LoraTiles::kPart};
 }
-// Pair e of them: the adapter and its number among the tile's, the slice and its columns, the first of the
-// rank's values.
+// Pair e of them: the adapter and its number among the tile's, the next one that goes with it (-1: none), the slice and its
+// columns, the first of the rank's values.
 struct LoraPair {
-  int s, of, p, beg, end, r0;
+  int s, s2, of, p, beg, end, r0;
+  bool both;  // a pair of the tile has a second one (the same for all of them: the next pair's is asked for before the products)
 };
 __device__ __forceinline__ LoraPair lora_pair(const LoraTiles& list, const Lora& lo, const LoraSteps& t, int e, int N,
                                               int n0) {
@@ -522,8 +526,17 @@ __device__ __forceinline__ LoraPair lora_pair(const LoraTiles& list, const Lora&
   lora_slices(lo, n0, min(n0 + 256, N), p0, p1);
   const int parts = (lo.rank + 63) / 64, per = parts * (p1 - p0), i = e / per, r = e - i * per;
   LoraPair q;
-  q.s = t.code >= 0 ? t.code : __builtin_amdgcn_readfirstlane(list.mix[LoraTiles::kMixed - t.code][1 + i]);
-  q.of = i;
+  q.of = lo.two ? 2 * i : i;
+  q.s = t.code;
+  q.s2 = -1;
+  q.both = false;
+  if (t.code < LoraTiles::kNone) {
+    const int* mix = list.mix[LoraTiles::kMixed - t.code];
+    q.s = __builtin_amdgcn_readfirstlane(mix[1 + q.of]);
+    const int n = __builtin_amdgcn_readfirstlane(mix[0]);
+    q.both = lo.two && n > 1;
+    if (lo.two && q.of + 1 < n) q.s2 = __builtin_amdgcn_readfirstlane(mix[2 + q.of]);
+  }
   q.p = p0 + r / parts;
   q.r0 = 64 * (r % parts);
   q.beg = q.p == 0 ? 0 : lora_end(lo, q.p - 1);
@@ -538,9 +551,18 @@ __device__ __forceinline__ void lora_offsets(const LoraTiles& list, const Lora& 
                                              LoraBase& nb, int& low, bool& all) {
   const int half = lo.rank / 8, r = 8 * wave + (lane >> 3);
   const bool one = half <= 4;
-  const int ga = (lane & 7) ^ (((wave & 1) << 2) | (lane >> 4));
+  int ga = (lane & 7) ^ (((wave & 1) << 2) | (lane >> 4));
   int gb = (lane & 7) ^ (((wave & 3) << 1) | ((lane >> 4) & 1));
   const int to = one ? 2 * half : half - q.r0 / 8;
+  // (a second adapter: its values in the step's second half)
+  int base = q.s, of = q.of, more = 0;
+  if (q.s2 >= 0) {
+    base = min(q.s, q.s2);
+    of += ga >> 2;
+    more = ((gb >> 2 ? q.s2 : q.s) - base) * static_cast<int>(lo.b_slot) * 2;
+    ga &= 3;
+    gb &= 3;
+  }
   const int oa = ga < to ? 0 : kNoOffset, ob = gb < to ? 0 : kNoOffset;
   gb -= one && gb >= half ? half : 0;
 #pragma unroll
@@ -549,14 +571,14 @@ __device__ __forceinline__ void lora_offsets(const LoraTiles& list, const Lora& 
     for (int i = 0; i < 2; ++i) {
       const int row = m0 + 128 * h + 64 * i + r, col = n0 + 128 * h + 64 * i + r;
       va[h][i] = (min(row, M - 1) * static_cast<int>(lo.ldv) * 2 + 16 * ga) | oa;
-      vb[h][i] = (min(col, N - 1) * lo.rank * 2 + 16 * gb) | ob | (col >= q.beg && col < q.end ? 0 : kNoOffset);
+      vb[h][i] = (min(col, N - 1) * lo.rank * 2 + 16 * gb + more) | ob | (col >= q.beg && col < q.end ? 0 : kNoOffset);
       // (a load from memory here would wait for all that are in flight, 0.5 us a pair)
-      if (t.code < LoraTiles::kNone) va[h][i] |= list.which[LoraTiles::kMixed - t.code][row - m0] == q.of ? 0 : kNoOffset;
+      if (t.code < LoraTiles::kNone) va[h][i] |= list.which[LoraTiles::kMixed - t.code][row - m0] == of ? 0 : kNoOffset;
     }
   na = LoraBase(lo.v + 2 * q.p * lo.rank + q.r0);
-  nb = LoraBase(lo.b + q.s * lo.b_slot + q.r0);
+  nb = LoraBase(lo.b + base * lo.b_slot + q.r0);
   low = one ? 0 : 2 * lo.rank;
-  all = half > 2;
+  all = half > 2 || q.both;
 }
 // The tiles to be done again, behind the others' quarters; returns how many quarters.
 __device__ __forceinline__ int lora_quarters(LoraTiles& list) {
@@ -586,7 +608,8 @@ bool lora_of(Lora& lo, const uint16_t* v, int64_t ldv, const int* groups, const 
       b_slot % 8 || (slots > 1 && b_slot < static_cast<int64_t>(N) * rank) ||
       static_cast<int64_t>(N + 256) * rank * 2 >= kLimit)
     return false;
-  lo = Lora{v, ldv, b, b_slot, ids, groups, lora_sorted(M, slots) ? groups + (M + 15) / 16 : nullptr, slots, rank, slices, {N, N, N, N}};
+  lo = Lora{v, ldv, b, b_slot, ids, groups, lora_sorted(M, slots) ? groups + (M + 15) / 16 : nullptr, slots, rank, slices, {N, N, N, N},
+            rank <= 16 && slots <= (kLimit / 2 - 1) / std::max<int64_t>(b_slot, 1)};
   for (int p = 0, beg = 0; p < slices; beg = slice_end[p++]) {
     const bool last = p + 1 == slices;
     if (slice_end[p] <= beg || (last ? slice_end[p] != N : slice_end[p] % 16 != 0 || slice_end[p] >= N)) return false;

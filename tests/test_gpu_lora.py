@@ -498,7 +498,7 @@ def test_two_streams_at_once(pkg, dev):
 
 @pytest.mark.parametrize("fp8", [False, True])
 @pytest.mark.parametrize("R", [8, 16, 40, 72])
-@pytest.mark.parametrize("n", [2, 3, 6, 7, 12, 13, 40])
+@pytest.mark.parametrize("n", [2, 3, 6, 7, 12, 13, 20, 21, 40])
 def test_large_tiles_of_several_adapters(pkg, dev, n, R, fp8):
     """256 rows with n adapters each, in runs and row by row: up to, at and past what a tile takes as more steps, in whole tiles
     and in a last one of two slices; a row's bits are those that it has when the others have no adapter, whatever theirs hold."""
