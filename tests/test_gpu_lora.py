@@ -463,6 +463,23 @@ def test_slots_past_32_bits(pkg, dev):
         assert torch.equal(pkg.linear_fp8_lora(x, w8, ws, *views, scale, moved), pkg.linear_fp8_lora(x, w8, ws, *near, ids)), M
 
 
+@pytest.mark.parametrize("S", [15, 16, 34])
+def test_large_tiles_of_far_slots(pkg, dev, S):
+    """Tiles of several adapters whose slots in B lie up to, at and past 2^31 bytes: the same bits as from a pool side by side."""
+    gen = torch.Generator().manual_seed(S)
+    M, N, K, R = 2000, 12352, 1024, 16
+    a, b, scale = (t.to(dev) for t in _adapters(gen, S, [N], K, R))
+    far = torch.empty(S, 1 << 26, dtype=BF16, device=dev).as_strided(b.shape, (1 << 26, R, 1))
+    for s in range(S):
+        far[s].copy_(b[s])
+    x = torch.randn(M, K, generator=gen).to(BF16).to(dev)
+    w = torch.randn(N, K, generator=gen).to(BF16).to(dev)
+    ids = torch.randint(-1, S, (40,), generator=gen).repeat_interleave(50).to(torch.int32).to(dev)
+    assert torch.equal(pkg.linear_lora(x, w, a, far, scale, ids), pkg.linear_lora(x, w, a, b, scale, ids))
+    w8, ws = pkg.quantize_weight_fp8(w)
+    assert torch.equal(pkg.linear_fp8_lora(x, w8, ws, a, far, scale, ids), pkg.linear_fp8_lora(x, w8, ws, a, b, scale, ids))
+
+
 def test_two_streams_at_once(pkg, dev):
     """Calls that overlap on two streams, and two graphs replayed in turn and at once: each has rows of its own."""
     gen = torch.Generator().manual_seed(59)
