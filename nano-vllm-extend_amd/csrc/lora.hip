@@ -446,8 +446,10 @@ __global__ __launch_bounds__(64 * NW) void lora_shrink_kernel(Shrink p) {
 // Whether the kernel of few rows takes them: its 16 x 16 tiles read A and x again for each other, the prompts' 64-row
 // tiles take 9 to 12 us for any number up to the CUs (us, few / prompts, 2048 columns of bf16 x, one adapter: 2000 x 64 8.8 /
 // 11.6, 2000 x 128 14.8 / 12.2, 800 x 256 10.4 / 12.1, 1100 x 256 13.5 / 12.3, 800 x 512 15.5 / 12.5; of rows at random
-// 1100 x 256 56 / 41).
-bool few_rows(int M, int cols) { return M <= 2048 && (M + 15) / 16 * ((cols + 15) / 16) <= 7 * gdn::kNumCu / 2; }
+// 1100 x 256 56 / 41).  Rows whose order the product goes by are its whatever their columns: it writes the order.
+bool few_rows(int M, int cols, int slots) {
+  return lora_sorted(M, slots) || (M <= 2048 && (M + 15) / 16 * ((cols + 15) / 16) <= 7 * gdn::kNumCu / 2);
+}
 
 template <bool kFp8>
 int launch(Shrink p, hipStream_t st) {
@@ -457,7 +459,7 @@ int launch(Shrink p, hipStream_t st) {
   // half of it, so that a second tile runs beside the first.  us, four waves / two, 2048 columns of bf16 x, all rows one
   // adapter's: 17001 x 64 (266 tiles) 26.3 / 21.5, 16384 x 128 (512) 25.9 / 20.9, 16384 x 64 (256) 18.1 / 18.0, 4096 x 128
   // (128) 12.5 / 15.1; e4m3, 16384 x 64 (512) 21.2 / 17.0, 16384 x 16 (256) 11.9 / 13.7, 4096 x 128 (256) 10.9 / 13.3.
-  if (!few_rows(p.M, p.cols)) {
+  if (!few_rows(p.M, p.cols, p.slots)) {
     const int bn = !kFp8 && p.cols > 32 ? 64 : 32, n = tiles(p.M, 64) * tiles(p.cols, bn);
     const bool two = n > gdn::kNumCu;
     // Workgroups share a tile's adapters where that leaves no more of them than find room at once (one that finds
@@ -519,7 +521,7 @@ extern "C" int gdn_lora_shrink(const void* x, int x_is_bf16, int64_t ldx, const 
   if (x8 && (K % gdn::kFp8Group || !x8_scale || reinterpret_cast<uintptr_t>(x8) % 8 || sx8 % 8 || sx8 < K ||
              reinterpret_cast<uintptr_t>(x8_scale) % 4))
     return GDN_ERR_INVALID_ARG;
-  if (x8 && !few_rows(M, cols)) {
+  if (x8 && !few_rows(M, cols, slots)) {
     const int status = gdn_quantize_fp8(x, 0, ldx, x8, sx8, x8_scale, s8_row, s8_grp, M, K, 1, stream);
     if (status != GDN_OK) return status;
   }

@@ -22,7 +22,8 @@ namespace {
 
 constexpr int kMaxRank = 256;
 // Up to so many rows, and more than one tile's, are sorted by their adapters (lora.hip), and the kernels
-// of few rows take them in that order.  200 rows of 32 adapters at random, 12352 columns of e4m3 x 2048, rank 32: 32 us,
+// of few rows take them in that order: where lora_sorted is true the shrink writes it and the product reads it,
+// whatever the columns of either.  200 rows of 32 adapters at random, 12352 columns of e4m3 x 2048, rank 32: 32 us,
 // as they come 42.  (One tile's have nothing to gain: 1 row 16.0 us, sorted 17.3.  The counting grows
 // with the square of the rows: 1.3 us for 256, 5 for 512.)
 constexpr int kLoraSort = GDN_LORA_SORT;
