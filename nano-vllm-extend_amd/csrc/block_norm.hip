@@ -38,9 +38,10 @@ struct NormArgs {
 };
 
 // 1 / (1 + e^-g): the hardware reciprocal and one Newton step; 0 below -88, where it is less
-// than 2^-126.
+// than 2^-126.  The exponent is capped on both sides: exp_acc makes a NaN of one whose product with log2(e) is
+// infinite, and past 88 e^-g adds nothing to 1.
 __device__ __forceinline__ float sigmoid_ulp(float g) {
-  const float d = 1.0f + gdn::exp_acc(fminf(0.0f - g, 88.0f));
+  const float d = 1.0f + gdn::exp_acc(fmaxf(fminf(0.0f - g, 88.0f), -88.0f));
   const float rc = __builtin_amdgcn_rcpf(d);
   return g < -88.0f ? 0.0f : g != g ? g : fmaf(rc, fmaf(-d, rc, 1.0f), rc);
 }
