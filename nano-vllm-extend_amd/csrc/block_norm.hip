@@ -11,6 +11,7 @@
 // All of it in fp32 from the inputs' values; r is rounded once, to the stream's type, and y
 // is formed from the r that was not rounded (as the reference forms it), so that y has one
 // rounding.
+#include <algorithm>
 #include <type_traits>
 
 #include "gdn_common.h"
@@ -228,14 +229,36 @@ __global__ __launch_bounds__(T > 256 ? T : 256) void block_norm_kernel(NormArgs 
   }
 }
 
+// Rows `first` .. first + rows - 1.
+NormArgs rows_of(const NormArgs& a, int64_t first, int64_t rows) {
+  auto at = [](auto* p, int64_t bytes) { return p ? (decltype(p))((uintptr_t)p + bytes) : p; };
+  const int64_t dense = first * a.H;
+  NormArgs part = a;
+  part.x = a.x + first * a.sx;
+  part.residual = at(a.residual, first * a.sr * (a.stream_f32 ? 4 : 2));
+  part.gate = at(a.gate, first * a.g_row * (a.gate_f32 ? 4 : 2));
+  part.stream = at(a.stream, dense * (a.stream_f32 ? 4 : 2));
+  part.y = at(a.y, dense * 2);
+  part.y8 = at(a.y8, dense);
+  part.y8_scale = at(a.y8_scale, first * a.ss_row * 4);
+  part.M = rows;
+  return part;
+}
+
 template <bool kAny, int T, bool kFp8, int... N>
 int launch(const NormArgs& a, hipStream_t st) {
   constexpr int kRows = T > 256 ? 1 : 256 / T;
-  const dim3 grid(static_cast<unsigned>((a.M + kRows - 1) / kRows)), block(T > 256 ? T : 256);
+  constexpr int kThreads = T > 256 ? T : 256;
+  // (a launch has less than 2^32 threads: 2^26 rows of up to 1024 columns are past that, 2^24 of up to 2048)
+  constexpr int64_t kMost = kRows * (((int64_t{1} << 32) - 1) / kThreads);
   bool done = false;
   auto one = [&](auto n) {
     if (done || a.H > V * T * n.value) return;
-    block_norm_kernel<kAny, n.value, T, kFp8><<<grid, block, 0, st>>>(a);
+    for (int64_t first = 0; first < a.M; first += kMost) {
+      const NormArgs part = rows_of(a, first, std::min(kMost, a.M - first));
+      const dim3 grid(static_cast<unsigned>((part.M + kRows - 1) / kRows));
+      block_norm_kernel<kAny, n.value, T, kFp8><<<grid, dim3(kThreads), 0, st>>>(part);
+    }
     done = true;
   };
   (one(std::integral_constant<int, N>{}), ...);

@@ -1,4 +1,4 @@
-"""The norms around a block where their arguments end: gates past what an exponential holds."""
+"""The norms around a block where their arguments end: gates past what an exponential holds, rows past one launch."""
 import pytest
 import torch
 
@@ -49,3 +49,23 @@ def test_gates_of_any_size(pkg, dev, form, dtype):
                             scale=0.5)
     torch.cuda.synchronize()
     assert torch.equal(r.isnan(), nan[:, :odd])
+
+
+def test_more_rows_than_a_launch_has(pkg, dev):
+    """Narrow rows past what one launch's threads number: the bits of the calls with a part of the rows."""
+    M, H, part = (1 << 26) + 5, 8, 1 << 22
+    gen = torch.Generator(device=dev).manual_seed(3)
+    x = torch.randn(M, H, generator=gen, device=dev, dtype=BF16)
+    res = torch.randn(M, H, generator=gen, device=dev)
+    gate = torch.randn(M, 1, generator=gen, device=dev, dtype=BF16)
+    w = torch.randn(H, generator=gen, device=dev, dtype=BF16)
+    y, r = pkg.add_rms_norm(x, res, w, EPS, gate=gate, gate_sigmoid=True)
+    torch.cuda.synchronize()
+    for at in range(0, M, part):
+        to = min(M, at + part)
+        if to - at < 2048:
+            at = to - 2048
+        ey, er = pkg.add_rms_norm(x[at:to], res[at:to], w, EPS, gate=gate[at:to], gate_sigmoid=True)
+        assert torch.equal(y[at:to], ey) and torch.equal(r[at:to], er), at
+    last = slice(M - 2048, M)
+    _check(y[last], r[last], x[last], res[last], w, dict(gate=gate[last], gate_sigmoid=True))

@@ -24,6 +24,6 @@ def _run(name, tmp_path):
     return ran.stdout
 
 
-@pytest.mark.parametrize("name", ["lora_order"])
+@pytest.mark.parametrize("name", ["lora_order", "norm_rows"])
 def test_launches(name, tmp_path):
     print(_run(name, tmp_path))
