@@ -1538,10 +1538,13 @@ class LoraPool:
         self.b = torch.zeros(slots, sum(self.widths), self.rank, dtype=torch.bfloat16, device=device)
         self.scale = torch.zeros(slots, dtype=torch.float32, device=device)
 
-    def check(self, slot: int, parts) -> None:
-        """Raises where load would."""
+    def _slot(self, slot: int) -> None:
         if not 0 <= slot < self.a.shape[0]:
             raise ValueError(f"slot {slot} of {self.a.shape[0]}")
+
+    def check(self, slot: int, parts) -> None:
+        """Raises where load would."""
+        self._slot(slot)
         if len(parts) != len(self.widths):
             raise ValueError(f"{len(parts)} parts for {len(self.widths)} projections")
         for part, width in zip(parts, self.widths):
@@ -1568,6 +1571,7 @@ class LoraPool:
 
     def clear(self, slot: int) -> None:
         """An empty adapter (its rows get the projection alone)."""
+        self._slot(slot)
         self.a[slot].zero_()
         self.b[slot].zero_()
         self.scale[slot] = 0.0

@@ -1,0 +1,18 @@
+"""Slots of adapters and the block's norms: what is refused before anything changes (CPU tensors)."""
+import pytest
+import torch
+
+
+def test_clear_refuses_slots_that_are_not_there(pkg):
+    """-1 is the slot of rows without an adapter: clearing it leaves the last one as it was."""
+    pool = pkg.LoraPool(3, 8, 64, [32, 16], device="cpu")
+    for slot in range(3):
+        pool.load(slot, [(torch.ones(8, 64), torch.ones(32, 8)), (torch.ones(8, 64), torch.ones(16, 8))], 1.0 + slot)
+    before = [t.clone() for t in (pool.a, pool.b, pool.scale)]
+    for slot in (-1, -3, 3, 100):
+        with pytest.raises(ValueError, match="slot"):
+            pool.clear(slot)
+        assert all(torch.equal(p, q) for p, q in zip(before, (pool.a, pool.b, pool.scale))), slot
+    pool.clear(1)
+    assert not pool.a[1].any() and not pool.b[1].any() and pool.scale.tolist() == [1.0, 0.0, 3.0]
+    assert torch.equal(pool.a[2], before[0][2]) and torch.equal(pool.b[0], before[1][0])
