@@ -789,6 +789,11 @@ class GatedDeltaNetBlock:
         for t, name in ((input_norm, "input_norm"), (post_norm, "post_norm")):
             if t.shape != (layer.hidden,):
                 raise ValueError(f"{name} must be [{layer.hidden}], got {list(t.shape)}")
+            # (what post_norm's call would refuse, it would after the mixer has moved its pools on)
+            if t.dtype not in (torch.bfloat16, torch.float32):
+                raise TypeError(f"{name} must be bfloat16 or float32, got {t.dtype}")
+            if t.device != layer.w_in.device:
+                raise ValueError(f"{name} is on {t.device}, the layer on {layer.w_in.device}")
         self.layer, self.input_norm, self.post_norm, self.eps, self.offset = layer, input_norm, post_norm, eps, offset
 
     def _input(self, hidden, residual, adapters):

@@ -1,4 +1,6 @@
 """Slots of adapters and the block's norms: what is refused before anything changes (CPU tensors)."""
+from types import SimpleNamespace
+
 import pytest
 import torch
 
@@ -16,3 +18,17 @@ def test_clear_refuses_slots_that_are_not_there(pkg):
     pool.clear(1)
     assert not pool.a[1].any() and not pool.b[1].any() and pool.scale.tolist() == [1.0, 0.0, 3.0]
     assert torch.equal(pool.a[2], before[0][2]) and torch.equal(pool.b[0], before[1][0])
+
+
+def test_block_refuses_norms_before_a_step(pkg):
+    """What the second norm's call would refuse only after the mixer has moved its pools on."""
+    layer = SimpleNamespace(hidden=64, w_in=torch.zeros(8, 64))
+    good = torch.zeros(64, dtype=torch.bfloat16)
+    for norm in (good, good.float()):
+        block = pkg.GatedDeltaNetBlock(layer, good, norm)
+        assert block.post_norm is norm
+    for bad, error in ((good.half(), TypeError), (good.double(), TypeError), (good.to(torch.int16), TypeError),
+                       (good.to("meta"), ValueError), (good[:32], ValueError), (good[None], ValueError)):
+        for norms in ((good, bad), (bad, good)):
+            with pytest.raises(error):
+                pkg.GatedDeltaNetBlock(layer, *norms)
