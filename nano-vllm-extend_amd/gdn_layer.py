@@ -630,13 +630,24 @@ class GatedDeltaNetLayer:
         return self.w_in.shape[0] + (self.w_ba.shape[0] if self.fp8 else 0)
 
     def add_adapters(self, slots: int, rank: int) -> None:
-        """Room for `slots` low-rank adapters of at most `rank`, all of them empty, in the
-        place of those that were there.  (The value heads are a multiple of 16: where a
-        product's columns change from one projection to the next.)"""
+        """Room for `slots` low-rank adapters of at most `rank`, all of them empty.  (The value
+        heads are a multiple of 16: where a product's columns change from one projection to
+        the next.)  Once made, the room stays: graphs that were captured with it read it.  A
+        call with the same sizes empties its slots; one with others is refused, until lora_in
+        and lora_out, set to None, have let it go."""
         c, dev = self.core, self.w_in.device
         if c.Hv % 16 or self.hidden % 64 or c.value_dim % 64:
             raise ValueError(f"adapters need value heads in multiples of 16 and rows in multiples of 64, got {c.Hv} heads, "
                              f"{self.hidden} and {c.value_dim} columns")
+        if self.lora_in is not None:
+            had = self.lora_in.a.shape[0], self.lora_in.rank
+            if had != (slots, -(-rank // 8) * 8):
+                raise ValueError(f"the layer has room for {had[0]} adapters of rank {had[1]}, which captured graphs may read: set "
+                                 f"lora_in and lora_out to None before making it anew for {slots} of rank {rank}")
+            for pool in (self.lora_in, self.lora_out):
+                for t in (pool.a, pool.b, pool.scale):
+                    t.zero_()
+            return
         pools = (ops.LoraPool(slots, rank, self.hidden, [c.conv_dim, c.value_dim, c.Hv, c.Hv], dev),
                  ops.LoraPool(slots, rank, c.value_dim, [self.hidden], dev))
         self.lora_in, self.lora_out = pools

@@ -32,3 +32,28 @@ def test_block_refuses_norms_before_a_step(pkg):
         for norms in ((good, bad), (bad, good)):
             with pytest.raises(error):
                 pkg.GatedDeltaNetBlock(layer, *norms)
+
+
+def test_room_for_adapters_stays(pkg):
+    """Captured graphs read the pools: a second add_adapters empties them in place or is refused."""
+    hidden, Hk, Hv, D = 64, 8, 16, 64
+    z = lambda *s: torch.zeros(*s, dtype=torch.bfloat16)  # noqa: E731
+    C = (2 * Hk + Hv) * D
+    layer = pkg.GatedDeltaNetLayer(z(C, hidden), z(Hv * D, hidden), z(Hv, hidden), z(Hv, hidden), z(hidden, Hv * D), Hk, Hv, D,
+                                   z(C, 4), z(Hv), z(Hv), z(D))
+    layer.add_adapters(3, 12)
+    held = [t for pool in (layer.lora_in, layer.lora_out) for t in (pool.a, pool.b, pool.scale)]
+    layer.load_adapter(2, 0.5, z=(torch.ones(12, hidden), torch.ones(Hv * D, 12)), out=(torch.ones(8, Hv * D), torch.ones(hidden, 8)))
+    assert all(bool(t[2].any()) for t in held)
+    kept = [t.clone() for t in held]
+    for slots, rank in ((4, 12), (2, 12), (3, 8), (3, 17), (0, 12), (3, 0)):
+        with pytest.raises(ValueError, match="room for 3 adapters of rank 16"):
+            layer.add_adapters(slots, rank)
+    now = lambda: [t for pool in (layer.lora_in, layer.lora_out) for t in (pool.a, pool.b, pool.scale)]  # noqa: E731
+    assert all(p is q and torch.equal(p, k) for p, q, k in zip(held, now(), kept))
+    layer.add_adapters(3, 16)
+    assert all(p is q and not p.any() for p, q in zip(held, now()))
+    layer.lora_in = layer.lora_out = None
+    layer.add_adapters(4, 40)
+    assert layer.lora_in.a.shape == (4, 160, hidden) and layer.lora_out.b.shape == (4, hidden, 40)
+    layer.load_adapter(3, 1.0)
