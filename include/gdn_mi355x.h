@@ -603,7 +603,8 @@ int gdn_commit_tree(float* s_pool, int64_t s_slot, uint16_t* conv_pool, int64_t 
  *   gate      fp32 (gate_is_fp32) or bf16, NULL: none; of row m and column n at gate[m g_row +
  *             n g_col], g_col 0 (one per row) or 1 (g_row 0: one per column)
  *   stream_out [M, H] contiguous, the type of residual: r (NULL: not written). It may be
- *             residual itself, where that is contiguous
+ *             residual itself (or x, or a gate of its shape), where that is contiguous and of its
+ *             type, and overlaps what is read in no other way
  *   y         [M, H] bf16 contiguous, y8 [M, H] e4m3 contiguous with the scale of row m and
  *             columns 128 g .. at y8_scale[m ss_row + g ss_grp] as gdn_quantize_fp8 of the
  *             fp32 values (H a multiple of 128 then); one of the two may be NULL

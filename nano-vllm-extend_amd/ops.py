@@ -1809,8 +1809,8 @@ def add_rms_norm(x: torch.Tensor, residual: torch.Tensor | None, weight: torch.T
     (per row), [H] (per column) or like x.  H up to 16384.
 
     Returns (y bf16, r in the residual's type, bf16 without one).  y is formed before r is
-    rounded.  r goes into residual_out where that is given (contiguous, r's type; residual
-    itself is allowed); where r is x (no residual, nothing else either), it is x that is
+    rounded.  r goes into residual_out where that is given (contiguous, r's type; it may be
+    an input of its shape and type, the residual as a rule, and overlaps none otherwise); where r is x (no residual, nothing else either), it is x that is
     returned.
     Reference: _gemma_rms_forward, _gemma_add_rms_forward,
     nanovllm/models/qwen3_5.py:99-118 (x and residual alone)."""
@@ -1909,12 +1909,28 @@ def _add_rms_norm(x, residual, weight, eps, post_weight, gate, gate_sigmoid, sca
             raise ValueError("residual_out must be 16-byte aligned")
         y8 = torch.empty(x.shape, dtype=FP8, device=x.device)
         y_scale = _fp8_scales(M, H // FP8_GROUP, x.device)
+    if residual_out is not None and M:
+        _check_in_place(r, M, H, (x2, sx, H, "x"), (r2, sr, H, "residual"), (gate, g_row, H if g_col else 1, "gate"),
+                        (weight, 0, H, "weight"), (post_weight, 0, H, "post_weight"))
     ptr = lambda t: 0 if t is None else t.data_ptr()  # noqa: E731
     f32 = lambda t: int(t is not None and t.dtype == torch.float32)  # noqa: E731
     _call_on(idx, "gdn_add_rms_norm", x2.data_ptr(), sx, ptr(r2), sr, int(kind == torch.float32), weight.data_ptr(),
              ptr(post_weight), f32(weight), float(offset), ptr(gate), f32(gate), g_row, g_col, int(bool(gate_sigmoid)),
              float(scale), float(eps), r.data_ptr() if written else 0, ptr(y), ptr(y8), ptr(y_scale), 1, max(M, 1), M, H)
     return y, y8, y_scale, r
+
+
+def _check_in_place(r, M, H, *read):
+    """read: (tensor, stride of its M rows, their columns, name) of what a norm's call reads.  A row is read and then
+    written by the same threads: r may lie where rows like its own do, value for value, and apart from all else."""
+    size, at = r.element_size(), r.data_ptr()
+    for t, stride, cols, name in read:
+        if t is None:
+            continue
+        begin, n = t.data_ptr(), t.element_size()
+        if begin < at + M * H * size and at < begin + ((M - 1) * stride + cols) * n:
+            if begin != at or n != size or cols != H or (M > 1 and stride != H):
+                raise ValueError(f"residual_out overlaps {name} otherwise than value for value")
 
 
 def _pieces(t, stride, H, align):
