@@ -1586,6 +1586,8 @@ def adapter_rows(adapters: torch.Tensor, cu_seqlens: torch.Tensor, rows: int) ->
                          f"and {list(cu_seqlens.shape)} on {cu_seqlens.device}")
     at = torch.searchsorted(cu_seqlens[1:].contiguous(), torch.arange(rows, dtype=cu_seqlens.dtype, device=adapters.device),
                             right=True)
+    if adapters.dtype == torch.int64:   # (a number that 32 bits do not hold is no slot either)
+        adapters = adapters.clamp(-1, 2**31 - 1)
     return torch.cat([adapters.to(torch.int32), adapters.new_full((1,), -1, dtype=torch.int32)])[at]
 
 

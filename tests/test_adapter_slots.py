@@ -57,3 +57,14 @@ def test_room_for_adapters_stays(pkg):
     layer.add_adapters(4, 40)
     assert layer.lora_in.a.shape == (4, 160, hidden) and layer.lora_out.b.shape == (4, hidden, 40)
     layer.load_adapter(3, 1.0)
+
+
+def test_adapter_rows_of_64_bits(pkg):
+    """Numbers that 32 bits do not hold name no slot, whatever their low bits are."""
+    far = torch.tensor([3, (1 << 32) + 3, -(1 << 32), 1 << 40, (1 << 31) - 1, -1, -(1 << 63), 0])
+    rows = pkg.adapter_rows(far, torch.arange(9), 8)
+    assert rows.dtype == torch.int32
+    for slots in (4, 1 << 20):
+        named = [int(r) if 0 <= r < slots else None for r in rows]
+        assert named == [3, None, None, None, None, None, None, 0]
+    assert pkg.adapter_rows(far[5:6], torch.arange(2), 1).tolist() == [-1]
