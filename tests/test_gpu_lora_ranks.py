@@ -66,3 +66,15 @@ def test_layer_with_the_largest_adapters(pkg, dev, weights):
         slack = slack + 4 * 256 * U * (want.abs() + delta.abs())
     torch.cuda.synchronize()
     _check(y, want + delta, slack + loose)
+
+
+@pytest.mark.parametrize("M,widths,R", [
+    # the last shapes of the few rows' shrink (tiles of 16 x 16 up to 896) and the first ones past them
+    (257, [96, 32, 48, 80], 208), (257, [96, 32, 48, 80], 216), (1024, [96, 32, 48, 80], 56), (1024, [64, 48, 16], 80),
+    (1025, [96, 32, 48, 80], 56), (2048, [80, 16], 56), (2048, [80, 16], 64), (2049, [80, 16], 56),
+    # ranks past 128: small products, 256 x 256 tiles with a rest, a last tile of two slices
+    (257, [512], 256), (300, [8192, 4096, 32, 32], 136), (900, [4096, 4096], 200), (1300, [8192, 4096, 32, 32], 256),
+    (2500, [2048, 4096, 16, 32], 248), (4100, [2064], 192)])
+@pytest.mark.parametrize("how", ["mixed", "sequences"])
+def test_more_rows_and_large_ranks(pkg, dev, M, widths, R, how):
+    _products(pkg, dev, M, widths, 256, R, 6, how, ("bf16", "quantized", "e4m3"))
