@@ -634,11 +634,14 @@ int gdn_add_rms_norm(const uint16_t* x, int64_t sx, const void* residual, int64_
  *         of two.  Rows without an adapter are not written, and count for nothing in what follows
  *   groups int32 [ceil(M / 16)], written by the first call for the second: the adapter of 16
  *         rows (-1: none of them has one, -2: they differ); with M <= GDN_LORA_SORT 2 M more:
- *         the rows in the order of their adapters, and these
+ *         from 17 rows on, the rows in the order of their adapters, and these (both calls with the same
+ *         slots)
  *   lb    [slots][N, rank] bf16, slot stride lb_slot (a multiple of 8), 16-byte aligned
  * x as the GEMM's A: bf16 with K in steps of 64, or e4m3 with its scales (K in steps of
  * 128).  x8 (NULL: not wanted; x bf16, K in steps of 128) takes gdn_quantize_fp8 of x, one scale for
- * each row's group, for the product that reads e4m3 rows.  An adapter's rows do not change the bits of others, whatever it holds.
+ * each row's group, for the product that reads e4m3 rows.  An adapter's rows do not change the bits of others, whatever it holds
+ * (its own are not finite where it is not: an infinity in lb times the two values of v may be NaN).
+ * v is below 2 GiB (M ldv 2), as are x's rows, a slot of a and one of lb.
  */
 #define GDN_LORA_SORT 256
 int gdn_lora_shrink(const void* x, int x_is_bf16, int64_t ldx, const float* xs, int64_t xs_row, int64_t xs_grp,

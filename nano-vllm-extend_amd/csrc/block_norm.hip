@@ -124,8 +124,8 @@ __device__ __forceinline__ float row_sum(float v, float* part) {
 }
 
 // One pass: the row stays in registers between its sums.  What bounds it: HBM, 16384 x 2048 41 us (6.5
-// TB/s; 4 bytes read and 4 written a value), with a norm behind the block and a gate 44, in bf16 and e4m3 55; a few rows one
-// launch's latency (1 x 2048 2.8, 201 rows with both norms 3.8).
+// TB/s; 4 bytes read and 4 written a value), with a norm behind the block and a gate 45, in bf16 and e4m3 56; a few rows one
+// launch's latency (1 x 2048 2.8 to 4.4, 201 rows with both norms 3.8 to 4.3).
 //
 // T threads per row, N pieces of 8 values per thread: piece i of thread t is columns V (T i +
 // t) .., so that 16 neighbouring lanes hold a group of 128.
@@ -271,7 +271,9 @@ int launch_rows(const NormArgs& a, hipStream_t st) {
   // bounded by the rows that run at once and not by a thread's chain (us, replayed; 256 threads for all: 16 x 4096
   // 4.2, in 512 3.9; 16 x 16384 8.6, in 1024 4.7; 8192 x 16384 317 and 188, 8192 x 8192 107 and 97).  Many short
   // rows go to a wave each, without a barrier: 16384 x 1024 22.1 (256 threads 24.5), 4096 x 1024 7.4 (7.8); 16384 x 2048 45.3
-  // (41.1), 1024 x 1024 4.7 (4.3).
+  // (41.1), 1024 x 1024 4.7 (4.3).  What is just past a step pays for threads without a piece, and rows of odd widths
+  // for pieces that straddle lines: 1031 x 4096 7.9, x 4296 9.7, x 4299 14.2, x 6144 11.6, x 8192 14.2; 4096 x 4096 22.4, x 4608 25.8,
+  // x 6144 31.4, x 8192 41.0.
   if (a.M >= 2048 && a.H <= 1024) return launch<kAny, 64, kFp8, 1, 2>(a, st);
   if (a.H <= 2048) return launch<kAny, 256, kFp8, 1>(a, st);
   if (a.H <= 4096) return launch<kAny, 512, kFp8, 1>(a, st);

@@ -1179,7 +1179,8 @@ namespace {
 // entry points).
 //
 // With adapters (kLora) the kernels with their products are fewer: the general one has none, and
-// what it would take goes to the kernel with 64-row tiles.
+// what it would take goes to the kernel with 64-row tiles (16384 x 4096 x 2112, rank 16, 373 us, without adapters 229; K = 2048, in the
+// large tiles, 219 and 196).
 template <bool kLora>
 int gemm_launch(const uint16_t* A, int64_t lda, const uint16_t* B, int64_t ldb, const GemmOut& out, int M, int N,
                 int K, const GemmGates& gt, const LoraArg<kLora>& lo, void* stream) {

@@ -54,15 +54,16 @@ __device__ __forceinline__ void dma16(__amdgpu_buffer_rsrc_t rsrc, uint8_t* lds,
   __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_ptr_t)lds, 16, voff, soff, 0, 0);
 }
 
+// order(r): the row of the output that a tile's row r is.
+struct SameRow {
+  __device__ __forceinline__ int operator()(int r) const { return r; }
+};
+
 // ---- 16 rows x 32 columns of accumulators to the output (the 8-wave kernel) ----
 // Lane (lr, lg) holds C[row0 + lr][cb + 8 lg .. + 7] in c0 (the first four) and
 // c1: one 16-byte piece, four lanes filling 64 contiguous bytes of a row.  kAnyRow: the piece
 // goes out whole in rows without 16-byte alignment too (the 8-bit GEMM's kernels: 8192 x
 // 4001 x 256 36 us, value by value 77; 4002 columns 26).
-// order(r): the row of the output that the tile's row r is.
-struct SameRow {
-  __device__ __forceinline__ int operator()(int r) const { return r; }
-};
 template <bool kAnyRow = false, class Order = SameRow>
 __device__ __forceinline__ void gemm_store16(const gdn::f32x4_t& c0, const gdn::f32x4_t& c1, const GemmOut& out,
                                              int M, int N, int row0, int cb, int lane, const GemmGates& gt,

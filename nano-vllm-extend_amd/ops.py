@@ -1699,8 +1699,9 @@ def linear_lora(x: torch.Tensor, weight: torch.Tensor, lora_a: torch.Tensor, lor
     [slots] fp32: a LoraPool's.  gates: as linear_cols; they are of the adapted columns.
 
     fp32 accumulation of both, one rounding; x A_s^T is held to 2^-16 in between.  A row's
-    result does not depend on the adapters of the others, whatever these hold.  Two
-    launches; x, weight and one slot of the adapters below 2 GiB each.  Returns [..., N], or the list of
+    result does not depend on the adapters of the others, whatever these hold (an infinity in
+    its own makes it infinite or NaN).  Two launches; x, weight, one slot of the adapters and the
+    shrunk rows (4 parts R bytes each) below 2 GiB.  Returns [..., N], or the list of
     parts, with gates (that, g, beta)."""
     if gates is None:
         y = _lib.quick().linear_lora(x, weight, lora_a, lora_b, lora_scale, ids, widths)
