@@ -1914,7 +1914,7 @@ def _add_rms_norm(x, residual, weight, eps, post_weight, gate, gate_sigmoid, sca
         y_scale = _fp8_scales(M, H // FP8_GROUP, x.device)
     if residual_out is not None and M:
         _check_in_place(r, M, H, (x2, sx, H, "x"), (r2, sr, H, "residual"), (gate, g_row, H if g_col else 1, "gate"),
-                        (weight, 0, H, "weight"), (post_weight, 0, H, "post_weight"))
+                        (weight, None, H, "weight"), (post_weight, None, H, "post_weight"))
     ptr = lambda t: 0 if t is None else t.data_ptr()  # noqa: E731
     f32 = lambda t: int(t is not None and t.dtype == torch.float32)  # noqa: E731
     _call_on(idx, "gdn_add_rms_norm", x2.data_ptr(), sx, ptr(r2), sr, int(kind == torch.float32), weight.data_ptr(),
@@ -1924,15 +1924,16 @@ def _add_rms_norm(x, residual, weight, eps, post_weight, gate, gate_sigmoid, sca
 
 
 def _check_in_place(r, M, H, *read):
-    """read: (tensor, stride of its M rows, their columns, name) of what a norm's call reads.  A row is read and then
-    written by the same threads: r may lie where rows like its own do, value for value, and apart from all else."""
+    """read: (tensor, stride of its M rows, their columns, name) of what a norm's call reads; stride None: one row for all,
+    read behind the store.  A row is read and then written by the same threads: r may lie where rows like its own do, value
+    for value, and apart from all else."""
     size, at = r.element_size(), r.data_ptr()
     for t, stride, cols, name in read:
         if t is None:
             continue
         begin, n = t.data_ptr(), t.element_size()
-        if begin < at + M * H * size and at < begin + ((M - 1) * stride + cols) * n:
-            if begin != at or n != size or cols != H or (M > 1 and stride != H):
+        if begin < at + M * H * size and at < begin + ((M - 1) * (stride or 0) + cols) * n:
+            if begin != at or n != size or cols != H or stride is None or (M > 1 and stride != H):
                 raise ValueError(f"residual_out overlaps {name} otherwise than value for value")
 
 

@@ -49,3 +49,17 @@ def test_residual_out_overlaps(ops, fp8):  # noqa: F811
         fn(residual=buf[:2 * H].view(1, 2 * H)[:, :H], residual_out=rows(0)[:1], **fn_one)
     with pytest.raises(Launched):
         fn(x=x[:0], residual=rows(0)[:0], weight=w, eps=1e-6, residual_out=rows(1)[:0])
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+def test_one_row_over_its_weights(ops, fp8):  # noqa: F811
+    """The weights are read behind the store of the stream: a single row's are not its output's place either."""
+    H = 256
+    fn = ops.add_rms_norm_fp8 if fp8 else ops.add_rms_norm
+    buf, x = torch.zeros(1, H, dtype=BF16), torch.zeros(1, H, dtype=BF16)
+    good = dict(x=x, residual=x, weight=x[0].clone(), eps=1e-6, post_weight=x[0].clone(), residual_out=buf)
+    for name in ("weight", "post_weight"):
+        with pytest.raises(ValueError, match=f"overlaps {name}"):
+            fn(**{**good, name: buf[0]})
+    with pytest.raises(Launched):
+        fn(**{**good, "gate": buf[0]})
