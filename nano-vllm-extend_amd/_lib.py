@@ -132,7 +132,7 @@ def load() -> ctypes.CDLL:
             f"{LIB_PATH} not found: build it with `python nano-vllm-extend_amd/build.py` "
             "(or __graft_entry__.build()); there is no fallback path")
     try:
-        lib = ctypes.CDLL(str(LIB_PATH), mode=ctypes.RTLD_GLOBAL)
+        lib = ctypes.CDLL(str(LIB_PATH), mode=ctypes.RTLD_LOCAL)
     except OSError as e:  # pragma: no cover - environment dependent
         raise GDNLibraryError(f"cannot load {LIB_PATH}: {e}") from e
     # the version first: a library of another version may lack entry points
@@ -141,6 +141,9 @@ def load() -> ctypes.CDLL:
     v = lib.gdn_abi_version()
     if v != ABI_VERSION:
         raise GDNLibraryError(f"ABI mismatch: library {v}, bindings {ABI_VERSION}")
+    # the quick calls' module finds the entry points among the process' symbols: this library's, and
+    # not those of one that was refused
+    lib = ctypes.CDLL(str(LIB_PATH), mode=ctypes.RTLD_GLOBAL)
     for name, argtypes in SIGNATURES.items():
         fn = getattr(lib, name)
         fn.argtypes = argtypes

@@ -4,6 +4,7 @@ rejects bad calls before any device work.  CPU only (no kernel launches)."""
 import ctypes
 import re
 import subprocess
+import sys
 from pathlib import Path
 
 import pytest
@@ -239,3 +240,38 @@ def test_stream_handle_of_a_device_without_an_index(pkg, monkeypatch):
 
     monkeypatch.setattr(torch.cuda, "current_stream", current_stream)
     assert pkg._lib.stream_handle(torch.device("cuda")) == 7 and seen == [torch.device("cuda")]
+
+
+def test_a_refused_library_leaves_no_symbols(tmp_path):
+    """A library that is refused by its version has entry points of the same names: a process that goes on with the
+    right one has that one's, inside of the library and from the quick calls' module."""
+    src, so = tmp_path / "old.c", tmp_path / "old.so"
+    program = f"""
+import sys
+sys.path.insert(0, {str(ROOT)!r})
+import ctypes, subprocess
+from pathlib import Path
+import __graft_entry__ as ge
+pkg = ge.load_package()
+_lib = pkg._lib
+names = sorted(set(_lib.SIGNATURES) - {{"gdn_abi_version"}})
+Path({str(src)!r}).write_text("int gdn_abi_version(void) {{ return 4; }}\\n" + "".join(f"int {{n}}(void) {{{{ return -7; }}}}\\n" for n in names))
+subprocess.run(["gcc", "-shared", "-fPIC", "-o", {str(so)!r}, {str(src)!r}], check=True)
+right, _lib.LIB_PATH = _lib.LIB_PATH, Path({str(so)!r})
+try:
+    _lib.load()
+    raise SystemExit("not refused")
+except _lib.GDNLibraryError as e:
+    assert "library 4" in str(e), e
+_lib.LIB_PATH = right
+lib = _lib.load()
+pack, head = _lib.WORDS["gdn_quantize_fp8"]
+none = [0] * (head >> 32)
+assert lib.gdn_call_words(pack(head, *none)) == lib.gdn_quantize_fp8(*none) != -7, lib.gdn_call_words(pack(head, *none))
+_lib.quick()
+here = lambda name: ctypes.cast(getattr(ctypes.CDLL(None), name), ctypes.c_void_p).value
+for name in names:
+    assert here(name) == ctypes.cast(getattr(lib, name), ctypes.c_void_p).value, name
+"""
+    ran = subprocess.run([sys.executable, "-c", program], capture_output=True, text=True, timeout=300)
+    assert ran.returncode == 0, ran.stderr[-2000:]
